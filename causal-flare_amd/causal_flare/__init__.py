@@ -6,7 +6,7 @@ Every compute call runs hand-written HIP kernels for gfx950 from
 raising ``NotImplementedError``: the semi-autoregressive prefill/decode stubs
 (stubs in the reference too).
 """
-from . import autoregressive, semi_autoregressive
+from . import autoregressive, mixers, semi_autoregressive
 from .autoregressive.training import flare_autoregressive_triton
 from .autoregressive.recurrent import flare_recurrent_triton
 from .autoregressive.inference import (
@@ -18,12 +18,24 @@ from .semi_autoregressive.inference import (
     flare_semi_autoregressive_decode_trition,
     flare_semi_autoregressive_prefill_trition,
 )
+from .mixers import (
+    short_convolution,
+    short_convolution_decode,
+    short_convolution_prefill,
+    softmax_attention,
+    softmax_attention_decode,
+    softmax_attention_prefill,
+    state_space_scan,
+    state_space_scan_decode,
+    state_space_scan_prefill,
+)
 
 __version__ = "0.0.1+mi355x"
 
 
 __all__ = [
     "autoregressive",
+    "mixers",
     "semi_autoregressive",
     "flare_autoregressive_triton",
     "flare_autoregressive_decode_triton",
@@ -32,5 +44,14 @@ __all__ = [
     "flare_semi_autoregressive_decode_trition",
     "flare_semi_autoregressive_prefill_trition",
     "flare_semi_autoregressive_trition",
+    "short_convolution",
+    "short_convolution_decode",
+    "short_convolution_prefill",
+    "softmax_attention",
+    "softmax_attention_decode",
+    "softmax_attention_prefill",
+    "state_space_scan",
+    "state_space_scan_decode",
+    "state_space_scan_prefill",
     "__version__",
 ]

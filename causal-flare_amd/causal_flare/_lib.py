@@ -45,6 +45,23 @@ HEADER_FUNCTIONS = (
     "flare_ar_forward_noalloc",
     "flare_device_faults",
     "flare_set_meet_spin_limit",
+    "flare_conv_forward",
+    "flare_conv_backward_workspace_size",
+    "flare_conv_backward",
+    "flare_conv_step",
+    "flare_scan_chunk",
+    "flare_scan_forward_workspace_size",
+    "flare_scan_forward",
+    "flare_scan_backward_workspace_size",
+    "flare_scan_backward",
+    "flare_scan_step",
+    "flare_attn_forward_workspace_size",
+    "flare_attn_forward",
+    "flare_attn_backward_workspace_size",
+    "flare_attn_backward",
+    "flare_attn_append",
+    "flare_attn_step_workspace_size",
+    "flare_attn_step",
 )
 
 F32, BF16, F16 = 0, 1, 2
@@ -122,6 +139,45 @@ def _declare(lib):
     lib.flare_semi_ar_forward.restype = _i
     lib.flare_semi_ar_forward.argtypes = ([_vp] * 5 + [_i] + [_i64] * 6 + [_f, _i64] + [_vp, _i, _vp, _vp]
                                           + [_vp, _sz, _vp])
+    lib.flare_conv_forward.restype = _i
+    lib.flare_conv_forward.argtypes = [_vp, _i64, _i64, _vp, _vp, _i, _i] + [_i64] * 4 + [_vp] * 6
+    lib.flare_conv_backward_workspace_size.restype = _sz
+    lib.flare_conv_backward_workspace_size.argtypes = [_i64] * 4
+    lib.flare_conv_backward.restype = _i
+    lib.flare_conv_backward.argtypes = ([_vp, _i64, _i64, _vp, _vp, _i, _i] + [_i64] * 4 + [_vp] * 5
+                                        + [_vp, _sz, _vp])
+    lib.flare_conv_step.restype = _i
+    lib.flare_conv_step.argtypes = [_vp, _i64, _vp, _vp, _i, _i] + [_i64] * 3 + [_vp] * 4
+    lib.flare_scan_chunk.restype = _i64
+    lib.flare_scan_chunk.argtypes = [_i64] * 5 + [_i]
+    lib.flare_scan_forward_workspace_size.restype = _sz
+    lib.flare_scan_forward_workspace_size.argtypes = [_i64] * 6
+    lib.flare_scan_forward.restype = _i
+    lib.flare_scan_forward.argtypes = ([_vp] * 8 + [_i, _i] + [_i64] * 5 + [_vp] * 6 + [_i64, _vp]
+                                       + [_vp, _sz, _vp])
+    lib.flare_scan_backward_workspace_size.restype = _sz
+    lib.flare_scan_backward_workspace_size.argtypes = [_i64] * 6
+    lib.flare_scan_backward.restype = _i
+    lib.flare_scan_backward.argtypes = ([_vp] * 8 + [_i, _i] + [_i64] * 5 + [_vp] * 3 + [_i64, _vp] + [_vp] * 8
+                                        + [_vp, _sz, _vp])
+    lib.flare_scan_step.restype = _i
+    lib.flare_scan_step.argtypes = [_vp] * 8 + [_i, _i] + [_i64] * 4 + [_vp] * 5
+    lib.flare_attn_forward_workspace_size.restype = _sz
+    lib.flare_attn_forward_workspace_size.argtypes = [_i64] * 2
+    lib.flare_attn_forward.restype = _i
+    lib.flare_attn_forward.argtypes = ([_vp] * 4 + [_i] + [_i64] * 6 + [_f, _f, _vp, _i] + [_vp] * 6
+                                       + [_vp, _sz, _vp])
+    lib.flare_attn_backward_workspace_size.restype = _sz
+    lib.flare_attn_backward_workspace_size.argtypes = [_i64] * 3
+    lib.flare_attn_backward.restype = _i
+    lib.flare_attn_backward.argtypes = ([_vp] * 4 + [_i] + [_i64] * 5 + [_f, _f, _vp, _i] + [_vp] * 8
+                                        + [_vp, _sz, _vp])
+    lib.flare_attn_append.restype = _i
+    lib.flare_attn_append.argtypes = [_vp] * 3 + [_i] + [_i64] * 5 + [_vp] * 5
+    lib.flare_attn_step_workspace_size.restype = _sz
+    lib.flare_attn_step_workspace_size.argtypes = [_i64] * 5
+    lib.flare_attn_step.restype = _i
+    lib.flare_attn_step.argtypes = ([_vp] * 4 + [_i] + [_i64] * 5 + [_f, _f] + [_vp] * 5 + [_vp, _sz, _vp])
 
 
 def _check_single_hip_runtime():

@@ -1,0 +1,259 @@
+"""Selective state space scan.
+
+    delta_t = dt_t + dt_bias, or softplus of it
+    h_t     = exp(delta_t A) h_{t-1} + delta_t x_t B_t          [C, S]
+    y_t     = (sum_s C_t h_t + D x_t) silu(z_t)                 [C]
+
+Layouts: x, dt, z [B, N, C]; A [C, S] (1 to 64 states a channel); B, C [B, N, S], or [B, N, G, S]
+where channel c reads group c // (C / G); D, dt_bias [C].  x, dt, z, B and C may be slices of
+wider tensors: the last dimension has to be adjacent in memory, and anything else is copied.
+They may be float32, bfloat16 or float16 (one type: their promotion); A, D and dt_bias are used
+in float32, and so are states, decays and sums.
+
+A cache is ``{"h": [B, C, S]}`` in float32.
+"""
+from __future__ import annotations
+
+import torch
+import torch.autograd as autograd
+from torch.autograd.function import once_differentiable
+
+from .. import _lib
+from .._common import _compute_dtype
+from ._inputs import (
+    _check_device,
+    _check_float,
+    _check_integers,
+    _check_shape,
+    _f32,
+    _int32,
+    _on,
+    _row_mask,
+    _rows,
+    _strides,
+    _training,
+)
+
+_MAX_STATES = 64
+
+
+def _check(name, x, dt, A, B, C, D, z, dt_bias):
+    """(batch, tokens, channels, states, groups) of checked inputs."""
+    if x.dim() != 3:
+        raise ValueError(f"{name} expects x [B, N, C]. Got {tuple(x.shape)}")
+    nb, n, c = x.shape
+    _check_shape(name, "dt", dt, x.shape)
+    _check_shape(name, "z", z, x.shape)
+    if A.dim() != 2 or A.shape[0] != c:
+        raise ValueError(f"{name} expects A [C, S] with C={c}. Got {tuple(A.shape)}")
+    s = A.shape[1]
+    if not 1 <= s <= _MAX_STATES:
+        raise ValueError(f"{name} supports 1 to {_MAX_STATES} states a channel. Got S={s}")
+    if B.dim() not in (3, 4) or tuple(B.shape[:2]) != (nb, n) or B.shape[-1] != s:
+        raise ValueError(f"{name} expects B [B, N, S] or [B, N, G, S] with B={nb}, N={n}, S={s}. Got {tuple(B.shape)}")
+    g = B.shape[2] if B.dim() == 4 else 1
+    _check_shape(name, "C", C, B.shape)
+    if g < 1 or c % g:
+        raise ValueError(f"{name} expects channels that divide into the groups of B and C. Got C={c}, G={g}")
+    _check_shape(name, "D", D, (c,))
+    _check_shape(name, "dt_bias", dt_bias, (c,))
+    _check_float(name, x=x, dt=dt, A=A, B=B, C=C, D=D, z=z, dt_bias=dt_bias)
+    return nb, n, c, s, g
+
+
+class _Inputs:
+    """The tensors as the kernels take them, and the strides that go with them."""
+
+    def __init__(self, x, dt, A, B, C, D, z, dt_bias):
+        self.dtype = _compute_dtype(x, dt, B, C, z)
+        self.x, self.dt, self.z = (_rows(t, self.dtype) for t in (x, dt, z))
+        self.B, self.C = (_rows(t if t.dim() == 4 else t[:, :, None], self.dtype) for t in (B, C))
+        self.A, self.D, self.dt_bias = _f32(A), _f32(D), _f32(dt_bias)
+        zs = (0, 0) if z is None else (self.z.stride(0), self.z.stride(1))
+        self.strides = _strides(self.x.stride(0), self.x.stride(1), self.dt.stride(0), self.dt.stride(1), *zs,
+                                *self.B.stride()[:3], *self.C.stride()[:3])
+
+    def pointers(self):
+        P = _lib.ptr
+        return P(self.x), P(self.dt), P(self.A), P(self.B), P(self.C), P(self.D), P(self.z), P(self.dt_bias)
+
+
+def _padded(S):
+    return 8 if S <= 8 else 16 if S <= 16 else 32 if S <= 32 else 64
+
+
+def _run(x, dt, A, B, C, D, z, dt_bias, dt_softplus, sizes, training, document_ids=None, lengths=None, h0=None,
+         h_fin=None):
+    """(y, the states before the chunks or None, the chunk length)."""
+    nb, n, c, s, g = sizes
+    t = _Inputs(x, dt, A, B, C, D, z, dt_bias)
+    lib = _lib.lib()
+    chunk = int(lib.flare_scan_chunk(nb, n, c, s, g, int(training)))
+    chunks = -(-n // chunk)
+    states = torch.empty((nb, chunks, _padded(s), c), device=x.device, dtype=torch.float32) if chunks > 1 else None
+    nbytes = lib.flare_scan_forward_workspace_size(nb, n, c, s, g, chunk)
+    ws = torch.empty(nbytes, device=x.device, dtype=torch.uint8)
+    y = torch.empty((nb, n, c), device=x.device, dtype=t.dtype)
+    ids, lens = _int32(document_ids), _int32(lengths)
+    P = _lib.ptr
+    with _on(x.device):
+        rc = lib.flare_scan_forward(*t.pointers(), int(bool(dt_softplus)), _lib.dtype_code(t.dtype), nb, n, c, s, g,
+                                    t.strides, P(ids), P(lens), P(h0), P(y), P(h_fin), chunk, P(states), P(ws),
+                                    nbytes, _lib.stream_of(x.device))
+    _lib.check(rc, "flare_scan_forward")
+    return y, states, chunk
+
+
+class StateSpaceScan(autograd.Function):
+    """The scan over whole sequences, with gradients for every floating-point input."""
+
+    @staticmethod
+    def forward(ctx, x, dt, A, B, C, D, z, dt_bias, dt_softplus, document_ids, sizes, training):
+        ctx.sizes, ctx.softplus, ctx.chunk = sizes, dt_softplus, 0
+        if x.numel() == 0:
+            ctx.save_for_backward(x, dt, A, B, C, D, z, dt_bias, document_ids, None)
+            return torch.empty_like(x)
+        y, states, ctx.chunk = _run(x, dt, A, B, C, D, z, dt_bias, dt_softplus, sizes, training, document_ids)
+        ctx.save_for_backward(x, dt, A, B, C, D, z, dt_bias, document_ids, states if training else None)
+        return y.to(x.dtype)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        x, dt, A, B, C, D, z, dt_bias, document_ids, states = ctx.saved_tensors
+        leaves = (x, dt, A, B, C, D, z, dt_bias)
+        if x.numel() == 0:
+            return tuple(None if t is None else torch.zeros_like(t) for t in leaves) + (None,) * 4
+        nb, n, c, s, g = ctx.sizes
+        t = _Inputs(*leaves)
+        device, f32 = x.device, torch.float32
+        gy = dy.to(t.dtype).contiguous()
+
+        def empty(*shape, dtype=t.dtype):
+            return torch.empty(shape, device=device, dtype=dtype)
+
+        dx, ddt, dB, dC = empty(nb, n, c), empty(nb, n, c), empty(nb, n, g, s), empty(nb, n, g, s)
+        dA = empty(c, s, dtype=f32)
+        dz = None if z is None else empty(nb, n, c)
+        dD = None if D is None else empty(c, dtype=f32)
+        dbias = None if dt_bias is None else empty(c, dtype=f32)
+        ids = _int32(document_ids)
+        lib = _lib.lib()
+        nbytes = lib.flare_scan_backward_workspace_size(nb, n, c, s, g, ctx.chunk)
+        ws = torch.empty(nbytes, device=device, dtype=torch.uint8)
+        P = _lib.ptr
+        with _on(device):
+            rc = lib.flare_scan_backward(*t.pointers(), int(bool(ctx.softplus)), _lib.dtype_code(t.dtype), nb, n, c, s,
+                                         g, t.strides, P(ids), P(gy), ctx.chunk, P(states), P(dx), P(ddt), P(dA),
+                                         P(dB), P(dC), P(dD), P(dz), P(dbias), P(ws), nbytes, _lib.stream_of(device))
+        _lib.check(rc, "flare_scan_backward")
+        grads = (dx, ddt, dA, dB.view(B.shape), dC.view(C.shape), dD, dz, dbias)
+        return tuple(None if d is None else d.to(ref.dtype) for d, ref in zip(grads, leaves)) + (None,) * 4
+
+
+def _state(name, state, nb, c, s, device):
+    if not isinstance(state, dict) or "h" not in state:
+        raise ValueError(f"{name} expects a state {{'h': [B, C, S]}}. Got {state!r:.80}")
+    _check_shape(name, "state['h']", state["h"], (nb, c, s))
+    return state["h"].to(device=device, dtype=torch.float32).contiguous()
+
+
+def state_space_scan(
+    x: torch.Tensor,
+    dt: torch.Tensor,
+    A: torch.Tensor,
+    B: torch.Tensor,
+    C: torch.Tensor,
+    D: torch.Tensor | None = None,
+    z: torch.Tensor | None = None,
+    dt_bias: torch.Tensor | None = None,
+    dt_softplus: bool = False,
+    document_ids: torch.Tensor | None = None,
+):
+    """Selective scan of whole sequences from h = 0, differentiable in every floating-point input.
+
+    document_ids: integers [B, N].  The state starts from 0 where an id differs from the one
+    before; a token of a negative id is padding, with y = 0 and no gradient.
+    """
+    name = "state_space_scan"
+    sizes = _check(name, x, dt, A, B, C, D, z, dt_bias)
+    _check_integers(name, "document_ids", document_ids, x.shape[:2])
+    _check_device(name, x=x, dt=dt, A=A, B=B, C=C, D=D, z=z, dt_bias=dt_bias, document_ids=document_ids)
+    return StateSpaceScan.apply(x, dt, A, B, C, D, z, dt_bias, dt_softplus, document_ids, sizes,
+                                _training(x, dt, A, B, C, D, z, dt_bias))
+
+
+def state_space_scan_prefill(
+    x: torch.Tensor,
+    dt: torch.Tensor,
+    A: torch.Tensor,
+    B: torch.Tensor,
+    C: torch.Tensor,
+    D: torch.Tensor | None = None,
+    z: torch.Tensor | None = None,
+    dt_bias: torch.Tensor | None = None,
+    dt_softplus: bool = False,
+    state: dict[str, torch.Tensor] | None = None,
+    lengths: torch.Tensor | None = None,
+):
+    """Prompts that continue `state` (None: h = 0): (y, new state).
+
+    lengths: integers [B], each sequence's real tokens (all N by default; taken as 0 or N where
+    they lie outside that).  Rows behind them give y = 0 and leave the state alone.  The input
+    state is left as it is.
+    """
+    name = "state_space_scan_prefill"
+    sizes = nb, n, c, s, g = _check(name, x, dt, A, B, C, D, z, dt_bias)
+    _check_integers(name, "lengths", lengths, (nb,))
+    device = _check_device(name, x=x, dt=dt, A=A, B=B, C=C, D=D, z=z, dt_bias=dt_bias, lengths=lengths)
+    h0 = None if state is None else _state(name, state, nb, c, s, device)
+    if x.numel() == 0:
+        h = torch.zeros((nb, c, s), device=device) if h0 is None else h0.clone()
+        return torch.empty_like(x, requires_grad=False), {"h": h}
+    h = torch.empty((nb, c, s), device=device, dtype=torch.float32)
+    y, _, _ = _run(x, dt, A, B, C, D, z, dt_bias, dt_softplus, sizes, False, lengths=lengths, h0=h0, h_fin=h)
+    return y.to(x.dtype), {"h": h}
+
+
+def state_space_scan_decode(
+    x: torch.Tensor,
+    dt: torch.Tensor,
+    A: torch.Tensor,
+    B: torch.Tensor,
+    C: torch.Tensor,
+    D: torch.Tensor | None = None,
+    z: torch.Tensor | None = None,
+    dt_bias: torch.Tensor | None = None,
+    dt_softplus: bool = False,
+    state: dict[str, torch.Tensor] | None = None,
+    attention_mask: torch.Tensor | None = None,
+):
+    """One token a sequence: (y [B, 1, C], state).
+
+    x, dt, z [B, 1, C] and B, C [B, 1, S] or [B, 1, G, S], or all of them without the dimension
+    of the token (B and C then [B, S] or [B, G, S]).  A contiguous float32 state is updated in
+    place and returned.  attention_mask [B] or [B, 1]: a row of 0 keeps its state and gets y = 0.
+    """
+    name = "state_space_scan_decode"
+    if x.dim() == 2:
+        x, dt, B, C = x[:, None], dt[:, None], B[:, None], C[:, None]
+        z = None if z is None else z[:, None]
+    nb, n, c, s, g = _check(name, x, dt, A, B, C, D, z, dt_bias)
+    if n != 1:
+        raise ValueError(f"{name} expects one token a sequence. Got x {tuple(x.shape)}")
+    device = _check_device(name, x=x, dt=dt, A=A, B=B, C=C, D=D, z=z, dt_bias=dt_bias)
+    mask = _row_mask(name, attention_mask, nb, device)
+    if state is None:
+        h = torch.zeros((nb, c, s), device=device, dtype=torch.float32)
+    else:
+        h = _state(name, state, nb, c, s, device)
+    t = _Inputs(x, dt, A, B, C, D, z, dt_bias)
+    y = torch.empty((nb, 1, c), device=device, dtype=t.dtype)
+    if y.numel() == 0:
+        return y.to(x.dtype), {"h": h}
+    P = _lib.ptr
+    with _on(device):
+        rc = _lib.lib().flare_scan_step(*t.pointers(), int(bool(dt_softplus)), _lib.dtype_code(t.dtype), nb, c, s, g,
+                                        t.strides, P(mask), P(h), P(y), _lib.stream_of(device))
+    _lib.check(rc, "flare_scan_step")
+    return y.to(x.dtype), {"h": h}

@@ -1,0 +1,279 @@
+// flare_attn.h -- exact softmax attention: what its kernels share.
+//
+//   x_ij = scale q_i . k_j, or cap tanh(scale q_i . k_j / cap);  s_ij = x_ij - slope |i - j|
+//   p_ij = exp(s_ij) / sum_j exp(s_ij) over the keys j that i sees;   y_i = sum_j p_ij v_j
+//
+// Query i sees key j if j <= i or j < prefix (or all, without `causal`), if the two have the
+// same document id and it is not negative, and if neither lies behind its sequence's end.  A
+// query that sees nothing has y = 0.  Positions count from the front of the cache where there
+// is one.  Scores are kept in log2 units.
+//
+// Products.  With lane = (g, c), g = lane / 16, c = lane % 16, the 16x16 MFMA takes row c of A
+// and column c of B with contraction indices 8g .. 8g+7 (of 32), and leaves rows 4g .. 4g+3 of
+// column c.  So S^T = K Q^T leaves a lane 4 keys of each 16 of one query, and two such tiles are
+// the B operand of a product over keys, if its A operand takes the keys in the same order: 4g+i
+// of the first 16 and 4g+i of the second.  Transposed LDS reads give just that from rows of V.
+// Scores, weights and outputs thus never change lanes.  fp32 operands go through eight 16x16x4
+// products, which take the same registers.
+#pragma once
+
+#include "flare_mix.h"
+
+namespace flare {
+namespace attn {
+
+using mfma::bf16;
+using mfma::bf16x8;
+using mfma::f16;
+using mfma::f16x8;
+using mfma::f32x4;
+using mix::ceil_div;
+using mix::kLn2;
+using mix::kLog2e;
+using mix::known_dtype;
+
+typedef float f32x8 __attribute__((ext_vector_type(8)));
+typedef unsigned u32;
+typedef u32 u32x2 __attribute__((ext_vector_type(2)));
+typedef u32 u32x4 __attribute__((ext_vector_type(4)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+
+constexpr int kIdTile = 64;          // tokens of one entry of the id statistics
+
+struct Rows {                        // a [B, n, heads, D] tensor: element strides
+    const void* p;
+    int64_t sb, sn, sh;
+};
+
+struct AttnArgs {
+    Rows q, k, v;
+    void* y;                         // [B, N, H, D]
+    float* lse;                      // [B, H, N], log2 units; +inf for a row that sees nothing
+    const float* slopes;             // [H]
+    const int32_t *ids, *prefix;     // [B, N], [B]
+    const int32_t* id_stats;         // [B, tiles, 3]: smallest and largest id of 64 tokens, whether they have just one
+    const int32_t *lengths, *fresh;  // [B]: tokens in the cache before these, and how many of these are real
+    int64_t B, N, M, H, G, D;        // M: rows of k and v
+    float scale, cap;
+    int causal;
+    // backward
+    const void* dy;                  // [B, N, H, D]
+    const float* delta;              // [B, H, N]: dy . y
+    void *dq, *dk, *dv;
+    // single tokens
+    const void *k_new, *v_new;       // [B, G, D]
+    int64_t kn_sb, kn_sg, vn_sb, vn_sg;
+    float* parts;
+    int64_t splits;
+};
+
+__device__ __forceinline__ int64_t clamp_to(int64_t n, int64_t most) { return n < 0 ? 0 : (n > most ? most : n); }
+
+template <typename E> struct Elem;
+template <> struct Elem<__hip_bfloat16> {
+    typedef bf16 S;
+    typedef bf16x8 Frag;
+};
+template <> struct Elem<__half> {
+    typedef f16 S;
+    typedef f16x8 Frag;
+};
+template <> struct Elem<float> {
+    typedef float S;
+    typedef f32x8 Frag;
+};
+
+__device__ __forceinline__ f32x4 mma(bf16x8 a, bf16x8 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4 mma(f16x8 a, f16x8 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4 mma(f32x8 a, f32x8 b, f32x4 c) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[i], b[i], c, 0, 0, 0);
+    return c;
+}
+
+// Eight elements as an operand; p is 16-byte aligned.
+template <typename E>
+__device__ __forceinline__ typename Elem<E>::Frag frag_rows(const typename Elem<E>::S* p) {
+    typedef typename Elem<E>::Frag F;
+    if constexpr (sizeof(E) == 4) {
+        const f32x4* q = reinterpret_cast<const f32x4*>(p);
+        return __builtin_shufflevector(q[0], q[1], 0, 1, 2, 3, 4, 5, 6, 7);
+    } else {
+        return *reinterpret_cast<const F*>(p);
+    }
+}
+// The two tiles of weights of one query (or key) as an operand over 32 keys (queries).
+__device__ __forceinline__ bf16x8 frag_tiles(f32x4 a, f32x4 b, bf16) {
+    typedef bf16 v4 __attribute__((ext_vector_type(4)));
+    return __builtin_shufflevector(__builtin_convertvector(a, v4), __builtin_convertvector(b, v4), 0, 1, 2, 3, 4, 5, 6, 7);
+}
+__device__ __forceinline__ f16x8 frag_tiles(f32x4 a, f32x4 b, f16) {
+    typedef f16 v4 __attribute__((ext_vector_type(4)));
+    return __builtin_shufflevector(__builtin_convertvector(a, v4), __builtin_convertvector(b, v4), 0, 1, 2, 3, 4, 5, 6, 7);
+}
+__device__ __forceinline__ f32x8 frag_tiles(f32x4 a, f32x4 b, float) {
+    return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+}
+// Rows 4g+i and 16+4g+i of column c of a tile in LDS (rows `pitch` apart): the operand that
+// goes with frag_tiles.
+template <typename E>
+__device__ __forceinline__ typename Elem<E>::Frag frag_columns(const typename Elem<E>::S* tile, int pitch, int g, int c) {
+    if constexpr (sizeof(E) == 2) {
+        const short* p = (const short*)tile + (4 * g + (c >> 2)) * pitch + 4 * (c & 3);
+        const u32x2 a = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)p));
+        const u32x2 b = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(p + 16 * pitch)));
+        return __builtin_bit_cast(typename Elem<E>::Frag, __builtin_shufflevector(a, b, 0, 1, 2, 3));
+    } else {
+        f32x8 r;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            r[i] = tile[(4 * g + i) * pitch + c];
+            r[4 + i] = tile[(16 + 4 * g + i) * pitch + c];
+        }
+        return r;
+    }
+}
+
+// Over the four lanes of one column (g = 0 .. 3).
+__device__ __forceinline__ float column_max(float x) {
+    const mix::Halves a = mix::swap32(x, x);
+    x = fmaxf(a.first, a.second);
+    const mix::Halves b = mix::swap16(x, x);
+    return fmaxf(b.first, b.second);
+}
+__device__ __forceinline__ float column_sum(float x) {
+    const mix::Halves a = mix::swap32(x, x);
+    x = a.first + a.second;
+    const mix::Halves b = mix::swap16(x, x);
+    return b.first + b.second;
+}
+
+// tanh(x) = 1 - 2 / (e^2x + 1): absolute error some 1e-7, which is what a score needs.
+// `x2`: 2 x log2(e).
+__device__ __forceinline__ float tanh_log2(float x2) {
+    return 1.0f - 2.0f * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(x2));
+}
+
+// ROWS rows of DP elements from memory to LDS through registers, 16 bytes a thread at a time:
+// rows that are none and columns behind D become 0.
+template <typename E, int ROWS, int DP, int PITCH, int NT>
+struct Stage {
+    typedef typename Elem<E>::S S;
+    static constexpr int PER = 16 / sizeof(E), CPR = DP / PER, N = (ROWS * CPR + NT - 1) / NT;
+    static constexpr bool WHOLE = ROWS * CPR % NT == 0;
+    u32x4 r[N];
+    // `base`: row 0 of this head; rows first .. first+ROWS-1, those at or behind `end` are none
+    __device__ __forceinline__ void load(const S* base, int64_t stride, int64_t first, int64_t end, int D, int tid) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int e = i * NT + tid, row = e / CPR, col = e % CPR * PER;
+            r[i] = u32x4{0, 0, 0, 0};
+            if ((WHOLE || e < ROWS * CPR) && first + row < end && col < D)
+                r[i] = *reinterpret_cast<const u32x4*>(base + (first + row) * stride + col);
+        }
+    }
+    __device__ __forceinline__ void store(S* lds, int tid) const {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int e = i * NT + tid;
+            if (WHOLE || e < ROWS * CPR) *reinterpret_cast<u32x4*>(lds + e / CPR * PITCH + e % CPR * PER) = r[i];
+        }
+    }
+    // whether one of these elements is infinite or NaN
+    __device__ __forceinline__ bool odd() const {
+        bool any = false;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                if constexpr (sizeof(E) == 4) any |= (r[i][j] & 0x7f800000u) == 0x7f800000u;
+                else {
+                    constexpr u32 m = __is_same(E, __half) ? 0x7c00u : 0x7f80u;
+                    any |= (r[i][j] & m) == m || (r[i][j] >> 16 & m) == m;
+                }
+            }
+        }
+        return any;
+    }
+    // ... and those set to 0
+    __device__ __forceinline__ void clean() {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                if constexpr (sizeof(E) == 4) {
+                    if ((r[i][j] & 0x7f800000u) == 0x7f800000u) r[i][j] = 0;
+                } else {
+                    constexpr u32 m = __is_same(E, __half) ? 0x7c00u : 0x7f80u;
+                    if ((r[i][j] & m) == m) r[i][j] &= 0xffff0000u;
+                    if ((r[i][j] >> 16 & m) == m) r[i][j] &= 0xffffu;
+                }
+            }
+        }
+    }
+};
+
+// Pitches (elements) that spread the rows over the banks: a 16-byte read of 16 rows, and a
+// transposed read of four rows of 32 bytes in each 16 lanes.
+template <typename E, int DP> constexpr int row_pitch() { return DP + (sizeof(E) == 2 ? 8 : 4); }
+template <typename E, int DP> constexpr int column_pitch() { return DP + (sizeof(E) == 2 ? 16 : 4); }
+
+// What the tokens of a block of queries (or keys) may meet, by document ids.
+struct IdRange {
+    int lo, hi;                      // of the ids that are not negative; lo > hi if there is none
+    bool pure;                       // one id alone, none negative
+    __device__ __forceinline__ bool meets(const IdRange& o) const { return lo <= o.hi && o.lo <= hi; }
+    __device__ __forceinline__ bool same(const IdRange& o) const { return pure && o.pure && lo == o.lo; }
+};
+__device__ __forceinline__ int64_t id_tiles(int64_t N) { return (N + kIdTile - 1) / kIdTile; }
+__device__ __forceinline__ IdRange id_range(const AttnArgs& p, int64_t b, int64_t tile) {
+    const int32_t* s = p.id_stats + (b * id_tiles(p.N) + tile) * 3;
+    return IdRange{s[0], s[1], s[2] != 0};
+}
+// Tokens first .. first+n-1 (first a multiple of 64, or all within one tile).
+__device__ __forceinline__ IdRange id_block(const AttnArgs& p, int64_t b, int64_t first, int64_t n) {
+    IdRange r = id_range(p, b, first / kIdTile);
+    for (int64_t t = first / kIdTile + 1; t * kIdTile < min(first + n, p.N); ++t) {
+        const IdRange o = id_range(p, b, t);
+        r.pure = r.same(o);
+        r.lo = min(r.lo, o.lo);
+        r.hi = max(r.hi, o.hi);
+    }
+    return r;
+}
+
+// The tiles of STEP tokens in [begin, end) whose ids meet `mine`, in order; all of them without
+// ids.  64 tiles are looked at in one go, so every lane of the wave has to take part.
+template <int STEP>
+struct TileWalk {
+    const AttnArgs& p;
+    int64_t b, end;
+    IdRange mine;
+    int64_t window;                  // the 64 tiles of ids that `mask` tells of begin here
+    uint64_t mask;
+    __device__ __forceinline__ TileWalk(const AttnArgs& p, int64_t b, int64_t end, IdRange mine)
+        : p(p), b(b), end(end), mine(mine), window(-64), mask(0) {}
+    __device__ __forceinline__ int64_t next(int64_t k) {       // k: a multiple of STEP
+        if (!p.ids) return k;
+        while (k < end) {
+            const int64_t t = k / kIdTile;
+            if (t >= window + 64) {
+                window = t;
+                const int64_t at = t + (threadIdx.x & 63);
+                mask = __ballot(at < id_tiles(p.N) && id_range(p, b, at).meets(mine));
+            }
+            const uint64_t left = mask >> (t - window);
+            if (left & 1) return k;
+            k = (left ? t + __builtin_ctzll(left) : window + 64) * kIdTile;
+        }
+        return k;
+    }
+};
+
+}  // namespace attn
+}  // namespace flare

@@ -1,0 +1,196 @@
+// flare_attn.hip -- softmax attention: C entry points, id statistics, and writing prompts to caches.
+#include "flare_attn.h"
+#include "flare_internal.h"
+
+namespace flare {
+namespace attn {
+
+template <typename E> int forward_e(const AttnArgs& p, hipStream_t stream);
+template <typename E> int backward_e(const AttnArgs& p, float* delta, hipStream_t stream);
+int attn_step(const AttnArgs& p, int dtype, hipStream_t stream);
+
+// A wave for each 64 tokens.
+__global__ __launch_bounds__(64) void attn_ids_kernel(const int32_t* ids, int64_t N, int32_t* stats) {
+    const int64_t tile = blockIdx.x, b = blockIdx.y, t = tile * kIdTile + threadIdx.x;
+    const bool there = t < N;
+    const int id = there ? ids[b * N + t] : 0;
+    int lo = there && id >= 0 ? id : INT32_MAX, hi = there && id >= 0 ? id : -1;
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) {
+        lo = min(lo, __shfl_xor(lo, o, 64));
+        hi = max(hi, __shfl_xor(hi, o, 64));
+    }
+    const bool negative = __any(there && id < 0);
+    if (threadIdx.x == 0) {
+        int32_t* s = stats + (b * gridDim.x + tile) * 3;
+        s[0] = lo, s[1] = hi, s[2] = lo == hi && !negative;
+    }
+}
+
+// New keys and values to their place behind what each sequence's cache holds.  Nothing of a
+// sequence that does not fit.
+__global__ __launch_bounds__(256) void attn_append_kernel(Rows k, Rows v, const int32_t* lengths, const int32_t* fresh,
+                                                          int64_t B, int64_t N, int64_t M, int64_t row_bytes,
+                                                          int64_t G, int64_t size, char* kc, char* vc) {
+    const int64_t per = row_bytes / 16, id = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (id >= B * N * G * per) return;
+    const int64_t at = id % per * 16, g = id / per % G, t = id / per / G % N, b = id / per / G / N;
+    const int64_t off = lengths[b], n = fresh ? clamp_to(fresh[b], N) : N;
+    if (off < 0 || off + n > M || t >= n) return;
+    const int64_t to = ((b * M + off + t) * G + g) * row_bytes + at;
+    *reinterpret_cast<u32x4*>(kc + to) =
+        *reinterpret_cast<const u32x4*>((const char*)k.p + (b * k.sb + t * k.sn + g * k.sh) * size + at);
+    *reinterpret_cast<u32x4*>(vc + to) =
+        *reinterpret_cast<const u32x4*>((const char*)v.p + (b * v.sb + t * v.sn + g * v.sh) * size + at);
+}
+
+static size_t stats_bytes(int64_t B, int64_t N) { return (size_t)(B * ceil_div(N, kIdTile) * 3) * sizeof(int32_t); }
+
+static int launch_ids(AttnArgs& p, int32_t* stats, hipStream_t stream) {
+    if (!p.ids) return FLARE_OK;
+    attn_ids_kernel<<<dim3((unsigned)ceil_div(p.N, kIdTile), (unsigned)p.B), 64, 0, stream>>>(p.ids, p.N, stats);
+    p.id_stats = stats;
+    return check_launch("attn_ids");
+}
+
+static bool aligned(const Rows& r, int dtype) {
+    const int64_t per = dtype == FLARE_F32 ? 4 : 8;
+    return ((uintptr_t)r.p & 15) == 0 && r.sb % per == 0 && r.sn % per == 0 && r.sh % per == 0;
+}
+
+// Workgroups of the step kernel for each sequence's keys: enough for four on each CU (1024 on
+// the card), and no more than the cache has shares of 128 keys.
+static int64_t step_splits(int64_t B, int64_t M, int64_t H, int64_t G) {
+    const int64_t rows = B * G * ceil_div(H / G, 16), s = ceil_div(1024, rows), most = ceil_div(M, 128);
+    return s < 1 ? 1 : (s > most ? most : s);
+}
+
+}  // namespace attn
+}  // namespace flare
+
+using namespace flare;
+using namespace flare::attn;
+
+#define ATTN_REQUIRE_SIZES(name)                                                                                  \
+    FLARE_REQUIRE(known_dtype(dtype), name ": unknown dtype %d", dtype);                                          \
+    FLARE_REQUIRE(B >= 1 && N >= 1 && M >= 1 && H >= 1 && G >= 1, name ": sizes must be positive");               \
+    FLARE_REQUIRE(H % G == 0, name ": the query heads must divide into the key heads");                           \
+    FLARE_REQUIRE(D >= 16 && D <= 128 && D % 16 == 0, name ": head dimension %lld is not a multiple of 16 up to " \
+                  "128", (long long)D);                                                                           \
+    FLARE_REQUIRE(N <= (1 << 30) && M <= (1 << 30) && B <= 65535 && H <= 65535 && B * H <= (1 << 24) &&           \
+                  (N + 63) / 64 * B * H <= INT32_MAX, name ": too large");                                        \
+    FLARE_REQUIRE(softcap >= 0.0f && softcap < __builtin_huge_valf(), name ": the cap must be finite and not negative")
+
+static AttnArgs attn_args(const void* q, const void* k, const void* v, const int64_t* st, int64_t B, int64_t N,
+                          int64_t M, int64_t H, int64_t G, int64_t D, float scale, float softcap,
+                          const float* slopes) {
+    AttnArgs p = {};
+    p.q = {q, st[0], st[1], st[2]}, p.k = {k, st[3], st[4], st[5]}, p.v = {v, st[6], st[7], st[8]};
+    p.B = B, p.N = N, p.M = M, p.H = H, p.G = G, p.D = D, p.scale = scale, p.cap = softcap, p.slopes = slopes;
+    return p;
+}
+
+extern "C" size_t flare_attn_forward_workspace_size(int64_t B, int64_t N) { return stats_bytes(B, N); }
+
+extern "C" int flare_attn_forward(const void* q, const void* k, const void* v, const int64_t* strides, int dtype,
+                                  int64_t B, int64_t N, int64_t M, int64_t H, int64_t G, int64_t D, float scale,
+                                  float softcap, const float* slopes, int causal, const int32_t* document_ids,
+                                  const int32_t* prefix_lengths, const int32_t* lengths, const int32_t* new_lengths,
+                                  void* y, float* lse, void* workspace, size_t workspace_bytes, void* stream) {
+    FLARE_REQUIRE(q && k && v && strides && y, "flare_attn_forward: null pointer");
+    ATTN_REQUIRE_SIZES("flare_attn_forward");
+    FLARE_REQUIRE(lengths || M == N, "flare_attn_forward: as many keys as queries without a cache");
+    FLARE_REQUIRE(!(document_ids && lengths), "flare_attn_forward: document_ids exclude a cache");
+    FLARE_REQUIRE(lengths || !new_lengths, "flare_attn_forward: new_lengths without lengths");
+    AttnArgs p = attn_args(q, k, v, strides, B, N, M, H, G, D, scale, softcap, slopes);
+    FLARE_REQUIRE(aligned(p.q, dtype) && aligned(p.k, dtype) && aligned(p.v, dtype) && ((uintptr_t)y & 15) == 0,
+                  "flare_attn_forward: rows must be 16-byte aligned");
+    p.causal = causal, p.ids = document_ids, p.prefix = prefix_lengths, p.lengths = lengths, p.fresh = new_lengths;
+    p.y = y, p.lse = lse;
+    if (document_ids && (!workspace || workspace_bytes < stats_bytes(B, N))) {
+        set_error("flare_attn_forward: workspace of %zu bytes is too small", workspace_bytes);
+        return FLARE_ERR_WORKSPACE;
+    }
+    const int rc = launch_ids(p, (int32_t*)workspace, (hipStream_t)stream);
+    if (rc != FLARE_OK) return rc;
+    return FLARE_BY_DTYPE(dtype, forward_e, (p, (hipStream_t)stream));
+}
+
+extern "C" size_t flare_attn_backward_workspace_size(int64_t B, int64_t N, int64_t H) {
+    return (size_t)(B * H * N) * sizeof(float) + stats_bytes(B, N);
+}
+
+extern "C" int flare_attn_backward(const void* q, const void* k, const void* v, const int64_t* strides, int dtype,
+                                   int64_t B, int64_t N, int64_t H, int64_t G, int64_t D, float scale, float softcap,
+                                   const float* slopes, int causal, const int32_t* document_ids,
+                                   const int32_t* prefix_lengths, const void* y, const float* lse, const void* dy,
+                                   void* dq, void* dk, void* dv, void* workspace, size_t workspace_bytes,
+                                   void* stream) {
+    const int64_t M = N;
+    FLARE_REQUIRE(q && k && v && strides && y && lse && dy && dq && dk && dv && workspace,
+                  "flare_attn_backward: null pointer");
+    ATTN_REQUIRE_SIZES("flare_attn_backward");
+    AttnArgs p = attn_args(q, k, v, strides, B, N, M, H, G, D, scale, softcap, slopes);
+    const uintptr_t out = (uintptr_t)y | (uintptr_t)dy | (uintptr_t)dq | (uintptr_t)dk | (uintptr_t)dv;
+    FLARE_REQUIRE(aligned(p.q, dtype) && aligned(p.k, dtype) && aligned(p.v, dtype) && (out & 15) == 0,
+                  "flare_attn_backward: rows must be 16-byte aligned");
+    if (workspace_bytes < flare_attn_backward_workspace_size(B, N, H)) {
+        set_error("flare_attn_backward: workspace of %zu bytes is too small", workspace_bytes);
+        return FLARE_ERR_WORKSPACE;
+    }
+    float* delta = (float*)workspace;
+    p.causal = causal, p.ids = document_ids, p.prefix = prefix_lengths;
+    p.y = const_cast<void*>(y), p.lse = const_cast<float*>(lse), p.dy = dy, p.delta = delta;
+    p.dq = dq, p.dk = dk, p.dv = dv;
+    const int rc = launch_ids(p, (int32_t*)(delta + B * H * N), (hipStream_t)stream);
+    if (rc != FLARE_OK) return rc;
+    return FLARE_BY_DTYPE(dtype, backward_e, (p, delta, (hipStream_t)stream));
+}
+
+extern "C" int flare_attn_append(const void* k, const void* v, const int64_t* strides, int dtype, int64_t B, int64_t N,
+                                 int64_t M, int64_t G, int64_t D, const int32_t* lengths, const int32_t* new_lengths,
+                                 void* k_cache, void* v_cache, void* stream) {
+    const int64_t H = G;
+    const float softcap = 0.0f;
+    FLARE_REQUIRE(k && v && strides && lengths && k_cache && v_cache, "flare_attn_append: null pointer");
+    ATTN_REQUIRE_SIZES("flare_attn_append");
+    const Rows kr = {k, strides[0], strides[1], strides[2]}, vr = {v, strides[3], strides[4], strides[5]};
+    FLARE_REQUIRE(aligned(kr, dtype) && aligned(vr, dtype) && (((uintptr_t)k_cache | (uintptr_t)v_cache) & 15) == 0,
+                  "flare_attn_append: rows must be 16-byte aligned");
+    const int64_t size = dtype == FLARE_F32 ? 4 : 2, work = B * N * G * (D * size / 16);
+    FLARE_REQUIRE(work <= (int64_t)INT32_MAX * 256, "flare_attn_append: too large");
+    attn_append_kernel<<<dim3((unsigned)ceil_div(work, 256)), 256, 0, (hipStream_t)stream>>>(
+        kr, vr, lengths, new_lengths, B, N, M, D * size, G, size, (char*)k_cache, (char*)v_cache);
+    return check_launch("attn_append");
+}
+
+extern "C" size_t flare_attn_step_workspace_size(int64_t B, int64_t M, int64_t H, int64_t G, int64_t D) {
+    if (B < 1 || M < 1 || G < 1 || H % G) return 0;
+    const int64_t s = step_splits(B, M, H, G);
+    return s == 1 ? 0 : (size_t)(B * H * s * (D + 2)) * sizeof(float);
+}
+
+extern "C" int flare_attn_step(const void* q, const void* k, const void* v, const int64_t* strides, int dtype,
+                               int64_t B, int64_t M, int64_t H, int64_t G, int64_t D, float scale, float softcap,
+                               const float* slopes, const int32_t* lengths, void* k_cache, void* v_cache, void* y,
+                               void* workspace, size_t workspace_bytes, void* stream) {
+    const int64_t N = 1;
+    FLARE_REQUIRE(q && k && v && strides && lengths && k_cache && v_cache && y, "flare_attn_step: null pointer");
+    ATTN_REQUIRE_SIZES("flare_attn_step");
+    const int64_t none[9] = {};
+    AttnArgs p = attn_args(q, k_cache, v_cache, none, B, N, M, H, G, D, scale, softcap, slopes);
+    p.q.sb = strides[0], p.q.sh = strides[1];
+    p.k_new = k, p.kn_sb = strides[2], p.kn_sg = strides[3];
+    p.v_new = v, p.vn_sb = strides[4], p.vn_sg = strides[5];
+    const Rows kr = {k, strides[2], 0, strides[3]}, vr = {v, strides[4], 0, strides[5]};
+    FLARE_REQUIRE(aligned(p.q, dtype) && aligned(kr, dtype) && aligned(vr, dtype) && aligned(p.k, dtype) &&
+                  aligned(p.v, dtype), "flare_attn_step: rows must be 16-byte aligned");
+    FLARE_REQUIRE(B * G * ceil_div(H / G, 16) <= 65535, "flare_attn_step: too large");
+    p.splits = step_splits(B, M, H, G);
+    if (workspace_bytes < flare_attn_step_workspace_size(B, M, H, G, D) || (p.splits > 1 && !workspace)) {
+        set_error("flare_attn_step: workspace of %zu bytes is too small", workspace_bytes);
+        return FLARE_ERR_WORKSPACE;
+    }
+    p.lengths = lengths, p.y = y, p.parts = (float*)workspace;
+    return attn_step(p, dtype, (hipStream_t)stream);
+}

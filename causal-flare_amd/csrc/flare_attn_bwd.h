@@ -1,0 +1,488 @@
+// flare_attn_bwd.h -- gradients of softmax attention.
+//
+//   delta_i = dy_i . y_i;  dP_ij = dy_i . v_j;  dS_ij = P_ij (dP_ij - delta_i) (1 - tanh^2) scale
+//   dq_i = sum_j dS_ij k_j;  dk_j = sum_i dS_ij q_i;  dv_j = sum_i P_ij dy_i
+//
+// The weights come again from the scores and the forward's log-sum-exp.  Two kernels, so that
+// every sum has one owner and one order: attn_dq owns queries and walks over keys, attn_dkv owns
+// keys and walks over the queries of every head that shares them.  That costs seven products for
+// the five of a joint kernel, whose dq would be added up by atomics.
+#pragma once
+
+#include "flare_attn.h"
+
+namespace flare {
+namespace attn {
+
+// delta: a wave for each row of a head.
+template <typename E>
+__global__ __launch_bounds__(256) void attn_delta_kernel(AttnArgs p, float* delta) {
+    typedef typename Elem<E>::S S;
+    const int lane = threadIdx.x & 63;
+    const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);         // (b, i, h)
+    if (row >= p.B * p.N * p.H) return;
+    const S *y = (const S*)p.y + row * p.D, *dy = (const S*)p.dy + row * p.D;
+    float s = 0.0f;
+    for (int d = 2 * lane; d < p.D; d += 128) s += (float)y[d] * (float)dy[d] + (float)y[d + 1] * (float)dy[d + 1];
+    s = wave_sum(s);
+    const int64_t h = row % p.H, i = row / p.H % p.N, b = row / p.H / p.N;
+    if (lane == 0) delta[(b * p.H + h) * p.N + i] = s;
+}
+
+// An operand's infinite values and NaNs set to 0.
+template <typename F>
+__device__ __forceinline__ F finite(F f) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        if (!(fabsf((float)f[i]) < -kNegInf)) f[i] = 0.0f;
+    return f;
+}
+
+// The weights of the dv product are normalised ones, which in a long row lie below fp16's
+// smallest normal number (2^-14): there they come 2^10 times as large.
+template <typename E> constexpr float weight_shift() { return __is_same(E, __half) ? 10.0f : 0.0f; }
+
+template <typename E, int DP>
+struct BackwardLds {
+    static constexpr int T = 32, P = column_pitch<E, DP>();            // rows of a tile; read both ways
+    static constexpr size_t tile = sizeof(E) * T * P;
+    static constexpr size_t bytes = 4 * tile + 2 * (3 * T + 4) * sizeof(float);
+};
+
+template <typename E, int DP, int QT, bool CAP>
+__global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnArgs p) {
+    typedef typename Elem<E>::S S;
+    typedef typename Elem<E>::Frag Frag;
+    using Lds = BackwardLds<E, DP>;
+    constexpr int KT = Lds::T, QB = 64 * QT, DK = DP / 32, DT = DP / 16, P = Lds::P;
+    extern __shared__ __align__(16) char smem[];
+    S* kl = (S*)smem;                                   // [2][KT][P]
+    S* vl = (S*)(smem + 2 * Lds::tile);
+    int* idl = (int*)(smem + 4 * Lds::tile);            // [2][KT]
+    int* oddl = idl + 2 * KT;                           // [2][4]
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int g = lane >> 4, c = lane & 15;
+    const int64_t R = p.H / p.G, nq = (p.N + QB - 1) / QB;
+    int64_t id = blockIdx.x;
+    const int64_t kvh = id % p.G;
+    id /= p.G;
+    const int64_t b = id % p.B;
+    id /= p.B;
+    const int64_t h = kvh * R + id % R, q0 = (nq - 1 - id / R) * QB;
+
+    const int64_t prefix = p.prefix ? clamp_to(p.prefix[b], p.N) : 0;
+    const int64_t kv_end = p.causal ? max(min(q0 + QB, p.N), prefix) : p.N;
+    IdRange mine{0, 0, true};
+    if (p.ids) mine = id_block(p, b, q0, QB);
+    const int64_t w0 = q0 + wave * 16 * QT;
+    Frag qf[QT][DK], gf[QT][DK];
+    int64_t pos[QT];
+    int qid[QT];
+    float lse[QT], delta[QT];
+#pragma unroll
+    for (int t = 0; t < QT; ++t) {
+        const int64_t i = w0 + 16 * t + c;
+        const bool live = i < p.N;
+        pos[t] = live ? i : -1;
+        qid[t] = p.ids && live ? p.ids[b * p.N + i] : -1;
+        lse[t] = live ? p.lse[(b * p.H + h) * p.N + i] : -kNegInf;
+        delta[t] = live ? p.delta[(b * p.H + h) * p.N + i] : 0.0f;
+        const S* q = (const S*)p.q.p + b * p.q.sb + (live ? i : 0) * p.q.sn + h * p.q.sh;
+        const S* dy = (const S*)p.dy + ((b * p.N + (live ? i : 0)) * p.H + h) * p.D;
+#pragma unroll
+        for (int kk = 0; kk < DK; ++kk) {
+            const int d = 32 * kk + 8 * g;
+            qf[t][kk] = gf[t][kk] = Frag{};
+            if (live && d < p.D) {
+                qf[t][kk] = frag_rows<E>(q + d);
+                gf[t][kk] = frag_rows<E>(dy + d);
+            }
+        }
+    }
+    const S* kbase = (const S*)p.k.p + b * p.k.sb + kvh * p.k.sh;
+    const S* vbase = (const S*)p.v.p + b * p.v.sb + kvh * p.v.sh;
+    const float scale2 = p.scale * kLog2e, slope2 = p.slopes ? p.slopes[h] * kLog2e : 0.0f;
+    const float cap2 = p.cap * kLog2e, into_cap = CAP ? 2.0f * kLog2e * p.scale / p.cap : 0.0f;
+
+    f32x4 acc[QT][DT];
+#pragma unroll
+    for (int t = 0; t < QT; ++t)
+#pragma unroll
+        for (int d = 0; d < DT; ++d) acc[t][d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+
+    auto covers = [&](int64_t k0, int64_t first, int64_t last) {
+        if (k0 + KT > p.N || last >= p.N) return false;
+        if (p.causal && k0 + KT - 1 > first && k0 + KT > prefix) return false;
+        return !p.ids || mine.same(id_range(p, b, k0 / kIdTile));
+    };
+    Stage<E, KT, DP, P, 256> ks, vs;
+    int next_id = -1;
+    auto fetch = [&](int64_t k0) {
+        ks.load(kbase, p.k.sn, k0, p.N, p.D, tid);
+        vs.load(vbase, p.v.sn, k0, p.N, p.D, tid);
+        if (p.ids && tid < KT) next_id = k0 + tid < p.N ? p.ids[b * p.N + k0 + tid] : -1;
+    };
+    auto place = [&](int64_t k0, int buf) {
+        ks.store(kl + buf * KT * P, tid);
+        vs.store(vl + buf * KT * P, tid);
+        if (p.ids && tid < KT) idl[buf * KT + tid] = next_id;
+        const bool odd = !covers(k0, q0, q0 + QB - 1) && __any(ks.odd());
+        if (lane == 0) oddl[buf * 4 + wave] = odd;
+    };
+    TileWalk<KT> walk(p, b, kv_end, mine);
+    int64_t k0 = walk.next(0);
+    int buf = 0;
+    if (k0 < kv_end) {
+        fetch(k0);
+        place(k0, 0);
+    }
+    __syncthreads();
+    while (k0 < kv_end) {
+        const int64_t k1 = walk.next(k0 + KT);
+        if (k1 < kv_end) fetch(k1);
+        const bool hidden = w0 >= p.N || (p.causal && k0 > w0 + 16 * QT - 1 && k0 >= prefix);
+        if (!hidden) {
+            const S* kt = kl + buf * KT * P;
+            const S* vt = vl + buf * KT * P;
+            f32x4 s[QT][2], dp[QT][2];
+#pragma unroll
+            for (int t = 0; t < QT; ++t)
+#pragma unroll
+                for (int n = 0; n < 2; ++n) s[t][n] = dp[t][n] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int n = 0; n < 2; ++n) {
+#pragma unroll
+                for (int kk = 0; kk < DK; ++kk) {
+                    const Frag a = frag_rows<E>(kt + (16 * n + c) * P + 32 * kk + 8 * g);
+                    const Frag v = frag_rows<E>(vt + (16 * n + c) * P + 32 * kk + 8 * g);
+#pragma unroll
+                    for (int t = 0; t < QT; ++t) {
+                        s[t][n] = mma(a, qf[t][kk], s[t][n]);
+                        dp[t][n] = mma(v, gf[t][kk], dp[t][n]);
+                    }
+                }
+            }
+            const bool whole = covers(k0, w0, w0 + 16 * QT - 1);
+#pragma unroll
+            for (int t = 0; t < QT; ++t) {
+                const float base = (float)(int)(pos[t] - k0 - 4 * g);
+#pragma unroll
+                for (int n = 0; n < 2; ++n) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        float x = s[t][n][i], slant = 1.0f;
+                        if (CAP) {
+                            const float th = tanh_log2(x * into_cap);
+                            x = cap2 * th;
+                            slant = 1.0f - th * th;
+                        } else {
+                            x *= scale2;
+                        }
+                        if (p.slopes) x -= slope2 * fabsf(base - (float)(16 * n + i));
+                        const float w = __builtin_amdgcn_exp2f(x - lse[t]);
+                        float ds = w * (dp[t][n][i] - delta[t]);
+                        if (CAP) ds *= slant;
+                        s[t][n][i] = ds;
+                    }
+                }
+                if (!whole) {
+#pragma unroll
+                    for (int n = 0; n < 2; ++n) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const int64_t j = k0 + 16 * n + 4 * g + i;
+                            bool see = j < p.N && pos[t] >= 0;
+                            if (p.causal) see = see && (j <= pos[t] || j < prefix);
+                            if (p.ids) see = see && qid[t] >= 0 && idl[buf * KT + 16 * n + 4 * g + i] == qid[t];
+                            if (!see) s[t][n][i] = 0.0f;
+                        }
+                    }
+                }
+            }
+            const bool odd = (oddl[buf * 4] | oddl[buf * 4 + 1] | oddl[buf * 4 + 2] | oddl[buf * 4 + 3]) != 0;
+            Frag w[QT];
+#pragma unroll
+            for (int t = 0; t < QT; ++t) w[t] = frag_tiles(s[t][0], s[t][1], S{});
+#pragma unroll
+            for (int d = 0; d < DT; ++d) {
+                Frag a = frag_columns<E>(kt + 16 * d, P, g, c);
+                if (odd) a = finite(a);                 // 0 times an infinite value is NaN
+#pragma unroll
+                for (int t = 0; t < QT; ++t) acc[t][d] = mma(a, w[t], acc[t][d]);
+            }
+        }
+        if (k1 < kv_end) place(k1, buf ^ 1);
+        __syncthreads();
+        buf ^= 1;
+        k0 = k1;
+    }
+#pragma unroll
+    for (int t = 0; t < QT; ++t) {
+        const int64_t i = w0 + 16 * t + c;
+        if (i >= p.N) continue;
+        S* row = (S*)p.dq + ((b * p.N + i) * p.H + h) * p.D;
+#pragma unroll
+        for (int d = 0; d < DT; ++d) {
+            if (16 * d < p.D) {
+                typedef S S4 __attribute__((ext_vector_type(4)));
+                *reinterpret_cast<S4*>(row + 16 * d + 4 * g) = __builtin_convertvector(acc[t][d] * p.scale, S4);
+            }
+        }
+    }
+}
+
+template <typename E, int DP, int KQ, bool CAP>
+__global__ __launch_bounds__(256, DP > 96 && sizeof(E) == 2 ? 1 : 2) void attn_dkv_kernel(AttnArgs p) {
+    typedef typename Elem<E>::S S;
+    typedef typename Elem<E>::Frag Frag;
+    using Lds = BackwardLds<E, DP>;
+    constexpr float kShift = weight_shift<E>(), kUnshift = kShift == 0.0f ? 1.0f : 0x1p-10f;
+    constexpr int QR = Lds::T, KB = 64 * KQ, DK = DP / 32, DT = DP / 16, P = Lds::P;
+    extern __shared__ __align__(16) char smem[];
+    S* ql = (S*)smem;                                   // [2][QR][P]
+    S* gl = (S*)(smem + 2 * Lds::tile);
+    float* lsel = (float*)(smem + 4 * Lds::tile);       // [2][QR]
+    float* dell = lsel + 2 * QR;
+    int* idl = (int*)(dell + 2 * QR);
+    int* oddl = idl + 2 * QR;                           // [2][4]
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int g = lane >> 4, c = lane & 15;
+    const int64_t R = p.H / p.G;
+    int64_t id = blockIdx.x;
+    const int64_t kvh = id % p.G;
+    id /= p.G;
+    const int64_t b = id % p.B, kb = id / p.B * KB;     // the keys most queries see come first
+
+    const int64_t prefix = p.prefix ? clamp_to(p.prefix[b], p.N) : 0;
+    const int64_t q_begin = p.causal && kb >= prefix ? kb : 0;
+    IdRange mine{0, 0, true};
+    if (p.ids) mine = id_block(p, b, kb, KB);
+    const int64_t w0 = kb + wave * 16 * KQ;             // this wave's first key
+    Frag kf[KQ][DK], vf[KQ][DK];
+    int kid[KQ];
+#pragma unroll
+    for (int t = 0; t < KQ; ++t) {
+        const int64_t j = w0 + 16 * t + c;
+        const bool live = j < p.N;
+        kid[t] = p.ids && live ? p.ids[b * p.N + j] : -1;
+        const S* k = (const S*)p.k.p + b * p.k.sb + (live ? j : 0) * p.k.sn + kvh * p.k.sh;
+        const S* v = (const S*)p.v.p + b * p.v.sb + (live ? j : 0) * p.v.sn + kvh * p.v.sh;
+#pragma unroll
+        for (int kk = 0; kk < DK; ++kk) {
+            const int d = 32 * kk + 8 * g;
+            kf[t][kk] = vf[t][kk] = Frag{};
+            if (live && d < p.D) {
+                kf[t][kk] = frag_rows<E>(k + d);
+                vf[t][kk] = frag_rows<E>(v + d);
+            }
+        }
+    }
+    const float scale2 = p.scale * kLog2e;
+    const float cap2 = p.cap * kLog2e, into_cap = CAP ? 2.0f * kLog2e * p.scale / p.cap : 0.0f;
+    f32x4 dk[KQ][DT], dv[KQ][DT];
+#pragma unroll
+    for (int t = 0; t < KQ; ++t)
+#pragma unroll
+        for (int d = 0; d < DT; ++d) dk[t][d] = dv[t][d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+
+    auto covers = [&](int64_t q0, int64_t first, int64_t last) {
+        if (q0 + QR > p.N || last >= p.N) return false;
+        if (p.causal && last > q0 && last >= prefix) return false;
+        return !p.ids || mine.same(id_range(p, b, q0 / kIdTile));
+    };
+    Stage<E, QR, DP, P, 256> qs, gs;
+    float next_lse = 0.0f, next_delta = 0.0f;
+    int next_id = -1;
+    auto fetch = [&](int64_t h, int64_t q0) {
+        qs.load((const S*)p.q.p + b * p.q.sb + h * p.q.sh, p.q.sn, q0, p.N, p.D, tid);
+        gs.load((const S*)p.dy + (b * p.N * p.H + h) * p.D, p.H * p.D, q0, p.N, p.D, tid);
+        if (tid < QR) {
+            const bool live = q0 + tid < p.N;
+            const int64_t at = (b * p.H + h) * p.N + q0 + tid;
+            next_lse = live ? p.lse[at] - kShift : -kNegInf;
+            next_delta = live ? p.delta[at] * kUnshift : 0.0f;
+            if (p.ids) next_id = live ? p.ids[b * p.N + q0 + tid] : -1;
+        }
+    };
+    // Tiles seen in part keep infinite values and NaNs out of LDS (0 times them is NaN); the rows
+    // they are in have a log-sum-exp or a delta that is none, and their weights are NaN then.
+    auto place = [&](int64_t q0, int buf) {
+        bool odd = false;
+        if (!covers(q0, kb, kb + KB - 1)) {
+            if (qs.odd()) {
+                odd = true;
+                qs.clean();
+            }
+            if (gs.odd()) {
+                odd = true;
+                gs.clean();
+            }
+        }
+        odd = __any(odd);
+        if (lane == 0) oddl[buf * 4 + wave] = odd;
+        qs.store(ql + buf * QR * P, tid);
+        gs.store(gl + buf * QR * P, tid);
+        if (tid < QR) {
+            lsel[buf * QR + tid] = next_lse;
+            dell[buf * QR + tid] = next_delta;
+            idl[buf * QR + tid] = next_id;
+        }
+    };
+    int buf = 0;
+    for (int64_t rep = 0; rep < R; ++rep) {
+        const int64_t h = kvh * R + rep;
+        const float slope2 = p.slopes ? p.slopes[h] * kLog2e : 0.0f;
+        TileWalk<QR> walk(p, b, p.N, mine);
+        int64_t q0 = walk.next(q_begin);
+        if (q0 < p.N) {
+            fetch(h, q0);
+            place(q0, buf);
+        }
+        __syncthreads();
+        while (q0 < p.N) {
+            const int64_t q1 = walk.next(q0 + QR);
+            if (q1 < p.N) fetch(h, q1);
+            const bool hidden = w0 >= p.N || (p.causal && w0 > q0 + QR - 1 && w0 >= prefix);
+            if (!hidden) {
+                const S* qt = ql + buf * QR * P;
+                const S* gt = gl + buf * QR * P;
+                f32x4 s[KQ][2], dp[KQ][2];
+#pragma unroll
+                for (int t = 0; t < KQ; ++t)
+#pragma unroll
+                    for (int n = 0; n < 2; ++n) s[t][n] = dp[t][n] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int n = 0; n < 2; ++n) {
+#pragma unroll
+                    for (int kk = 0; kk < DK; ++kk) {
+                        const Frag a = frag_rows<E>(qt + (16 * n + c) * P + 32 * kk + 8 * g);
+                        const Frag o = frag_rows<E>(gt + (16 * n + c) * P + 32 * kk + 8 * g);
+#pragma unroll
+                        for (int t = 0; t < KQ; ++t) {
+                            s[t][n] = mma(a, kf[t][kk], s[t][n]);
+                            dp[t][n] = mma(o, vf[t][kk], dp[t][n]);
+                        }
+                    }
+                }
+                const bool whole = covers(q0, w0, w0 + 16 * KQ - 1);
+                const bool odd = (oddl[buf * 4] | oddl[buf * 4 + 1] | oddl[buf * 4 + 2] | oddl[buf * 4 + 3]) != 0;
+#pragma unroll
+                for (int n = 0; n < 2; ++n) {
+                    const f32x4 lse = *reinterpret_cast<const f32x4*>(lsel + buf * QR + 16 * n + 4 * g);
+                    const f32x4 delta = *reinterpret_cast<const f32x4*>(dell + buf * QR + 16 * n + 4 * g);
+#pragma unroll
+                    for (int t = 0; t < KQ; ++t) {
+                        const float base = (float)(int)(q0 + 4 * g - (w0 + 16 * t + c));
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            float x = s[t][n][i], slant = 1.0f;
+                            if (CAP) {
+                                const float th = tanh_log2(x * into_cap);
+                                x = cap2 * th;
+                                slant = 1.0f - th * th;
+                            } else {
+                                x *= scale2;
+                            }
+                            if (p.slopes) x -= slope2 * fabsf(base + (float)(16 * n + i));
+                            const float w = __builtin_amdgcn_exp2f(x - lse[i]);
+                            float ds = w * (dp[t][n][i] * kUnshift - delta[i]);
+                            if (CAP) ds *= slant;
+                            s[t][n][i] = w;
+                            dp[t][n][i] = ds;
+                        }
+                        if (!whole) {
+                            const int64_t j = w0 + 16 * t + c;
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                const int64_t at = q0 + 16 * n + 4 * g + i;
+                                bool see = j < p.N && at < p.N;
+                                if (p.causal) see = see && (j <= at || j < prefix);
+                                if (p.ids) see = see && kid[t] >= 0 && idl[buf * QR + 16 * n + 4 * g + i] == kid[t];
+                                if (odd && !(fabsf(lse[i]) < -kNegInf && fabsf(delta[i]) < -kNegInf))
+                                    s[t][n][i] = dp[t][n][i] = __builtin_nanf("");
+                                if (!see) s[t][n][i] = dp[t][n][i] = 0.0f;
+                            }
+                        }
+                    }
+                }
+                Frag w[KQ], ds[KQ];
+#pragma unroll
+                for (int t = 0; t < KQ; ++t) {
+                    w[t] = frag_tiles(s[t][0], s[t][1], S{});
+                    ds[t] = frag_tiles(dp[t][0], dp[t][1], S{});
+                }
+#pragma unroll
+                for (int d = 0; d < DT; ++d) {
+                    const Frag a = frag_columns<E>(qt + 16 * d, P, g, c);
+                    const Frag o = frag_columns<E>(gt + 16 * d, P, g, c);
+#pragma unroll
+                    for (int t = 0; t < KQ; ++t) {
+                        dk[t][d] = mma(a, ds[t], dk[t][d]);
+                        dv[t][d] = mma(o, w[t], dv[t][d]);
+                    }
+                }
+            }
+            if (q1 < p.N) place(q1, buf ^ 1);
+            __syncthreads();
+            buf ^= 1;
+            q0 = q1;
+        }
+    }
+#pragma unroll
+    for (int t = 0; t < KQ; ++t) {
+        const int64_t j = w0 + 16 * t + c;
+        if (j >= p.N) continue;
+        const int64_t row = ((b * p.N + j) * p.G + kvh) * p.D;
+#pragma unroll
+        for (int d = 0; d < DT; ++d) {
+            if (16 * d < p.D) {
+                typedef S S4 __attribute__((ext_vector_type(4)));
+                *reinterpret_cast<S4*>((S*)p.dk + row + 16 * d + 4 * g) = __builtin_convertvector(dk[t][d] * p.scale, S4);
+                *reinterpret_cast<S4*>((S*)p.dv + row + 16 * d + 4 * g) = __builtin_convertvector(dv[t][d] * kUnshift, S4);
+            }
+        }
+    }
+}
+
+template <typename K>
+static int allow_lds(K kernel, size_t bytes, const char* what) {
+    if (bytes <= 65536) return FLARE_OK;
+    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
+                                             hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+    if (e == hipSuccess) return FLARE_OK;
+    set_error("%s: %s", what, hipGetErrorString(e));
+    return FLARE_ERR_LAUNCH;
+}
+
+template <typename E, int DP, bool CAP>
+static int backward_cap(const AttnArgs& p, hipStream_t stream) {
+    constexpr int QT = sizeof(E) == 2 ? 2 : 1;
+    constexpr size_t bytes = BackwardLds<E, DP>::bytes;
+    auto dq = attn_dq_kernel<E, DP, QT, CAP>;
+    auto dkv = attn_dkv_kernel<E, DP, QT, CAP>;
+    int rc = allow_lds(dq, bytes, "attn_dq");
+    if (rc == FLARE_OK) rc = allow_lds(dkv, bytes, "attn_dkv");
+    if (rc != FLARE_OK) return rc;
+    const int64_t blocks = ceil_div(p.N, 64 * QT) * p.B;
+    dq<<<dim3((unsigned)(blocks * p.H)), 256, bytes, stream>>>(p);
+    if ((rc = check_launch("attn_dq")) != FLARE_OK) return rc;
+    dkv<<<dim3((unsigned)(blocks * p.G)), 256, bytes, stream>>>(p);
+    return check_launch("attn_dkv");
+}
+template <typename E, int DP>
+static int backward_dp(const AttnArgs& p, hipStream_t stream) {
+    return p.cap > 0.0f ? backward_cap<E, DP, true>(p, stream) : backward_cap<E, DP, false>(p, stream);
+}
+template <typename E>
+int backward_e(const AttnArgs& p, float* delta, hipStream_t stream) {
+    attn_delta_kernel<E><<<dim3((unsigned)ceil_div(p.B * p.N * p.H, 4)), 256, 0, stream>>>(p, delta);
+    const int rc = check_launch("attn_delta");
+    if (rc != FLARE_OK) return rc;
+    return p.D <= 32   ? backward_dp<E, 32>(p, stream)
+           : p.D <= 64 ? backward_dp<E, 64>(p, stream)
+           : p.D <= 96 ? backward_dp<E, 96>(p, stream)
+                       : backward_dp<E, 128>(p, stream);
+}
+
+}  // namespace attn
+}  // namespace flare

@@ -1,0 +1,307 @@
+// flare_attn_fwd.h -- softmax attention, forward (training and prompts that continue a cache).
+//
+// A workgroup of four waves owns 64 QT queries of one head, 16 QT a wave, with Q as the B
+// operand in registers; K and V come through LDS in tiles of KT keys, two of each, the next
+// one's loads in flight while one is computed.  The running maximum moves only when a score
+// passes it by 2^8, so that most tiles rescale nothing.  Weights are rounded to the inputs' type
+// for the product with V (their sum is taken before that, in fp32).
+#pragma once
+
+#include "flare_attn.h"
+
+namespace flare {
+namespace attn {
+
+constexpr float kSlack = 8.0f;       // log2 of the largest weight before the reference moves
+
+template <typename E, int DP, int KT>
+struct ForwardLds {
+    static constexpr int KP = row_pitch<E, DP>(), VP = column_pitch<E, DP>();
+    static constexpr size_t k_bytes = sizeof(E) * KT * KP, v_bytes = sizeof(E) * KT * VP;
+    static constexpr size_t bytes = 2 * (k_bytes + v_bytes + KT * sizeof(int)) + sizeof(int);
+};
+
+template <typename E, int DP, int QT, int KT, bool CAP>
+__global__ __launch_bounds__(256, 2) void attn_forward_kernel(AttnArgs p) {
+    typedef typename Elem<E>::S S;
+    typedef typename Elem<E>::Frag Frag;
+    using Lds = ForwardLds<E, DP, KT>;
+    constexpr int QB = 64 * QT, DK = DP / 32, DT = DP / 16, NK = KT / 16, KP = Lds::KP, VP = Lds::VP;
+    extern __shared__ __align__(16) char smem[];
+    S* kl = (S*)smem;
+    S* vl = (S*)(smem + 2 * Lds::k_bytes);
+    int* idl = (int*)(smem + 2 * (Lds::k_bytes + Lds::v_bytes));
+    int* oddl = idl + 2 * KT;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int g = lane >> 4, c = lane & 15;
+
+    // heads that share keys, and then the tiles of one head, are 8 workgroups or a multiple of
+    // that apart where there are 8 key heads: one XCD and its L2.  The longest rows come first.
+    const int64_t R = p.H / p.G, nq = (p.N + QB - 1) / QB;
+    int64_t id = blockIdx.x;
+    const int64_t kvh = id % p.G;
+    id /= p.G;
+    const int64_t b = id % p.B;
+    id /= p.B;
+    const int64_t h = kvh * R + id % R, q0 = (nq - 1 - id / R) * QB;
+
+    int64_t off = 0, qlen = p.N, kvlen = p.M;
+    bool refused = false;
+    if (p.lengths) {
+        off = p.lengths[b];
+        qlen = p.fresh ? clamp_to(p.fresh[b], p.N) : p.N;
+        if (off < 0) off = qlen = 0;
+        kvlen = off + qlen;
+        if (kvlen > p.M) {
+            refused = true;
+            qlen = kvlen = 0;
+        }
+    }
+    const int64_t prefix = p.prefix ? clamp_to(p.prefix[b], p.M) : 0;
+    int64_t kv_end = 0;
+    if (q0 < qlen) {
+        kv_end = kvlen;
+        if (p.causal) kv_end = min(kvlen, max(off + min(q0 + QB, qlen), prefix));
+    }
+    IdRange mine{0, 0, true};
+    if (p.ids) mine = id_block(p, b, q0, QB);
+
+    const int64_t w0 = q0 + wave * 16 * QT;            // this wave's first query
+    Frag qf[QT][DK];
+    int64_t pos[QT];                                   // of this lane's queries
+    int qid[QT];
+#pragma unroll
+    for (int t = 0; t < QT; ++t) {
+        const int64_t i = w0 + 16 * t + c;
+        const bool live = i < qlen;
+        pos[t] = live ? i + off : -1;                  // sees nothing but what a prefix shows
+        qid[t] = p.ids && live ? p.ids[b * p.N + i] : -1;
+        const S* row = (const S*)p.q.p + b * p.q.sb + (live ? i : 0) * p.q.sn + h * p.q.sh;
+#pragma unroll
+        for (int kk = 0; kk < DK; ++kk) {
+            const int d = 32 * kk + 8 * g;
+            if (live && d < p.D) qf[t][kk] = frag_rows<E>(row + d);
+            else qf[t][kk] = Frag{};
+        }
+    }
+    const S* kbase = (const S*)p.k.p + b * p.k.sb + kvh * p.k.sh;
+    const S* vbase = (const S*)p.v.p + b * p.v.sb + kvh * p.v.sh;
+    const float scale2 = p.scale * kLog2e, slope2 = p.slopes ? p.slopes[h] * kLog2e : 0.0f;
+    const float cap2 = p.cap * kLog2e, into_cap = CAP ? 2.0f * kLog2e * p.scale / p.cap : 0.0f;
+
+    f32x4 acc[QT][DT];
+    float top[QT], sum[QT];
+#pragma unroll
+    for (int t = 0; t < QT; ++t) {
+        top[t] = kNegInf;
+        sum[t] = 0.0f;
+#pragma unroll
+        for (int d = 0; d < DT; ++d) acc[t][d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+
+    auto covers = [&](int64_t k0, int64_t first, int64_t last) {       // every query sees every key
+        if (k0 + KT > kvlen || last >= qlen) return false;
+        if (p.causal && k0 + KT - 1 > first + off && k0 + KT > prefix) return false;
+        return !p.ids || mine.same(id_range(p, b, k0 / kIdTile));
+    };
+    Stage<E, KT, DP, KP, 256> ks;
+    Stage<E, KT, DP, VP, 256> vs;
+    int next_id = -1;
+    auto fetch = [&](int64_t k0) {
+        ks.load(kbase, p.k.sn, k0, kvlen, p.D, tid);
+        vs.load(vbase, p.v.sn, k0, kvlen, p.D, tid);
+        if (p.ids && tid < KT) next_id = k0 + tid < p.N ? p.ids[b * p.N + k0 + tid] : -1;
+    };
+    auto place = [&](int64_t k0, int buf) {
+        // A weight of 0 times an infinite value is NaN: tiles that some query does not see whole
+        // leave such values to the end.
+        if (!covers(k0, q0, q0 + QB - 1) && vs.odd()) {
+            vs.clean();
+            *oddl = 1;
+        }
+        ks.store(kl + buf * KT * KP, tid);
+        vs.store(vl + buf * KT * VP, tid);
+        if (p.ids && tid < KT) idl[buf * KT + tid] = next_id;
+    };
+
+    TileWalk<KT> walk(p, b, kv_end, mine);
+    int64_t k0 = walk.next(0);
+    int buf = 0;
+    if (tid == 0) *oddl = 0;
+    __syncthreads();
+    if (k0 < kv_end) {
+        fetch(k0);
+        place(k0, 0);
+    }
+    __syncthreads();
+    while (k0 < kv_end) {
+        const int64_t k1 = walk.next(k0 + KT);
+        if (k1 < kv_end) fetch(k1);
+        const bool hidden = w0 >= qlen || (p.causal && k0 > w0 + 16 * QT - 1 + off && k0 >= prefix);
+        if (!hidden) {
+            const S* kt = kl + buf * KT * KP;
+            const S* vt = vl + buf * KT * VP;
+            f32x4 s[QT][NK];
+#pragma unroll
+            for (int t = 0; t < QT; ++t)
+#pragma unroll
+                for (int n = 0; n < NK; ++n) s[t][n] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int n = 0; n < NK; ++n) {
+#pragma unroll
+                for (int kk = 0; kk < DK; ++kk) {
+                    const Frag a = frag_rows<E>(kt + (16 * n + c) * KP + 32 * kk + 8 * g);
+#pragma unroll
+                    for (int t = 0; t < QT; ++t) s[t][n] = mma(a, qf[t][kk], s[t][n]);
+                }
+            }
+            const bool whole = covers(k0, w0, w0 + 16 * QT - 1);
+#pragma unroll
+            for (int t = 0; t < QT; ++t) {
+                const float base = (float)(int)(pos[t] - k0 - 4 * g);
+#pragma unroll
+                for (int n = 0; n < NK; ++n) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        float x = s[t][n][i];
+                        x = CAP ? cap2 * tanh_log2(x * into_cap) : x * scale2;
+                        if (p.slopes) x -= slope2 * fabsf(base - (float)(16 * n + i));
+                        s[t][n][i] = x;
+                    }
+                }
+                if (!whole) {
+#pragma unroll
+                    for (int n = 0; n < NK; ++n) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const int64_t j = k0 + 16 * n + 4 * g + i;
+                            bool see = j < kvlen && pos[t] >= 0;
+                            if (p.causal) see = see && (j <= pos[t] || j < prefix);
+                            if (p.ids) see = see && qid[t] >= 0 && idl[buf * KT + 16 * n + 4 * g + i] == qid[t];
+                            if (!see) s[t][n][i] = kNegInf;
+                        }
+                    }
+                }
+                float m = s[t][0][0];
+#pragma unroll
+                for (int n = 0; n < NK; ++n)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) m = fmaxf(m, s[t][n][i]);
+                m = column_max(m);
+                if (__any(m > top[t] + kSlack)) {
+                    const float to = fmaxf(m, top[t]);
+                    const float f = top[t] == to ? 1.0f : __builtin_amdgcn_exp2f(top[t] - to);
+                    top[t] = to;
+                    sum[t] *= f;
+#pragma unroll
+                    for (int d = 0; d < DT; ++d) acc[t][d] *= f;
+                }
+                const float ref = top[t] == kNegInf ? 0.0f : top[t];
+#pragma unroll
+                for (int n = 0; n < NK; ++n) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        s[t][n][i] = __builtin_amdgcn_exp2f(s[t][n][i] - ref);
+                        sum[t] += s[t][n][i];
+                    }
+                }
+            }
+            Frag w[QT][NK / 2];
+#pragma unroll
+            for (int t = 0; t < QT; ++t)
+#pragma unroll
+                for (int n = 0; n < NK / 2; ++n) w[t][n] = frag_tiles(s[t][2 * n], s[t][2 * n + 1], S{});
+#pragma unroll
+            for (int n = 0; n < NK / 2; ++n) {
+#pragma unroll
+                for (int d = 0; d < DT; ++d) {
+                    const Frag a = frag_columns<E>(vt + 32 * n * VP + 16 * d, VP, g, c);
+#pragma unroll
+                    for (int t = 0; t < QT; ++t) acc[t][d] = mma(a, w[t][n], acc[t][d]);
+                }
+            }
+        }
+        if (k1 < kv_end) place(k1, buf ^ 1);
+        __syncthreads();
+        buf ^= 1;
+        k0 = k1;
+    }
+
+    if (*oddl) {
+        // the infinite values and NaNs that a query does see, from memory
+        TileWalk<KT> again(p, b, kv_end, mine);
+        for (k0 = again.next(0); k0 < kv_end; k0 = again.next(k0 + KT)) {
+            if (covers(k0, q0, q0 + QB - 1)) continue;
+            for (int64_t j = k0; j < min(k0 + KT, kvlen); ++j) {
+#pragma unroll
+                for (int t = 0; t < QT; ++t) {
+                    bool see = pos[t] >= 0;
+                    if (p.causal) see = see && (j <= pos[t] || j < prefix);
+                    if (p.ids) see = see && qid[t] >= 0 && p.ids[b * p.N + j] == qid[t];
+                    if (!see) continue;
+#pragma unroll
+                    for (int d = 0; d < DT; ++d) {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            if (16 * d >= p.D) continue;
+                            const float v = (float)vbase[j * p.v.sn + 16 * d + 4 * g + e];
+                            if (!(fabsf(v) < -kNegInf)) acc[t][d][e] += v;
+                        }
+                    }
+                }
+            }
+        }
+    }
+
+#pragma unroll
+    for (int t = 0; t < QT; ++t) {
+        const int64_t i = w0 + 16 * t + c;
+        const float total = column_sum(sum[t]);
+        const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+        if (i >= p.N) continue;
+        if (p.lse && g == 0)
+            p.lse[(b * p.H + h) * p.N + i] = total == 0.0f ? -kNegInf : top[t] + __builtin_amdgcn_logf(total);
+        S* row = (S*)p.y + ((b * p.N + i) * p.H + h) * p.D;
+#pragma unroll
+        for (int d = 0; d < DT; ++d) {
+            if (16 * d < p.D) {
+                f32x4 o = acc[t][d] * inv;
+                if (refused) o = f32x4{__builtin_nanf(""), __builtin_nanf(""), __builtin_nanf(""), __builtin_nanf("")};
+                typedef S S4 __attribute__((ext_vector_type(4)));
+                *reinterpret_cast<S4*>(row + 16 * d + 4 * g) = __builtin_convertvector(o, S4);
+            }
+        }
+    }
+}
+
+template <typename E, int DP, bool CAP>
+static int forward_cap(const AttnArgs& p, hipStream_t stream) {
+    constexpr int QT = sizeof(E) == 2 ? 2 : 1, KT = sizeof(E) == 2 ? 64 : 32;
+    constexpr size_t bytes = ForwardLds<E, DP, KT>::bytes;
+    auto kernel = attn_forward_kernel<E, DP, QT, KT, CAP>;
+    if (bytes > 65536) {
+        const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
+                                                 hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+        if (e != hipSuccess) {
+            set_error("attn_forward: %s", hipGetErrorString(e));
+            return FLARE_ERR_LAUNCH;
+        }
+    }
+    const int64_t blocks = ceil_div(p.N, 64 * QT) * p.H * p.B;
+    kernel<<<dim3((unsigned)blocks), 256, bytes, stream>>>(p);
+    return check_launch("attn_forward");
+}
+template <typename E, int DP>
+static int forward_dp(const AttnArgs& p, hipStream_t stream) {
+    return p.cap > 0.0f ? forward_cap<E, DP, true>(p, stream) : forward_cap<E, DP, false>(p, stream);
+}
+template <typename E>
+int forward_e(const AttnArgs& p, hipStream_t stream) {
+    return p.D <= 32   ? forward_dp<E, 32>(p, stream)
+           : p.D <= 64 ? forward_dp<E, 64>(p, stream)
+           : p.D <= 96 ? forward_dp<E, 96>(p, stream)
+                       : forward_dp<E, 128>(p, stream);
+}
+
+}  // namespace attn
+}  // namespace flare

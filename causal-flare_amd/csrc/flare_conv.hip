@@ -1,0 +1,415 @@
+// flare_conv.hip -- the short causal convolution: forward, backward and single-token step.
+//
+//   pre_t = bias + sum_{k < W} w[W-1-k] x_{t-k}      (k back within the same document; before
+//                                                      the first token: the cached window, or 0)
+//   y_t   = pre_t, or pre_t sigmoid(pre_t)
+//   d_t   = dy_t, or dy_t s (1 + pre (1 - s)), s = sigmoid(pre)
+//   dx_t  = sum_k w[W-1-k] d_{t+k};   dw[W-1-k] = sum_t d_t x_{t-k};   db = sum_t d_t
+//
+// Channels are independent, so a thread owns a few adjacent channels (16 bytes of them) and
+// walks over a run of tokens with the last W inputs in registers.  Bytes bound it: each input
+// is read once from memory (the W - 1 rows before a run again, from the L2) and each output
+// written once.
+#include "flare_internal.h"
+#include "flare_mix.h"
+
+namespace flare {
+namespace mix {
+
+struct ConvArgs {
+    const void* x;
+    int64_t x_sb, x_sn;
+    const float *weight, *bias;
+    const int32_t *ids, *lengths;
+    const void* window;
+    void *y, *window_out;
+    const void* dy;
+    void* dx;
+    float* partial;
+    int64_t B, N, C, tiles;
+    int silu;
+};
+
+__device__ __forceinline__ int64_t row_length(const int32_t* lengths, int64_t b, int64_t N) {
+    if (!lengths) return N;
+    const int64_t n = lengths[b];
+    return n < 0 ? 0 : (n > N ? N : n);
+}
+
+// How many tokens before t belong to its document, up to `most`.
+__device__ __forceinline__ int tokens_back(const int32_t* ids, int64_t t, int most) {
+    int n = 0;
+    while (n < most && t - n > 0 && ids[t - n] == ids[t - n - 1]) ++n;
+    return n;
+}
+
+// T tokens a thread; threads of neighbouring channels are neighbours.
+template <typename E, int W, int VEC, int T>
+__global__ __launch_bounds__(256) void conv_forward_kernel(ConvArgs p) {
+    const int64_t groups = p.C / VEC;
+    const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (id >= groups * p.tiles * p.B) return;
+    const int64_t c = (id % groups) * VEC, tile = id / groups % p.tiles, b = id / groups / p.tiles;
+    const int64_t t0 = tile * T, len = row_length(p.lengths, b, p.N);
+    const E* x = (const E*)p.x + b * p.x_sb + c;
+    const E* win = p.window ? (const E*)p.window + b * (W - 1) * p.C + c : nullptr;
+    const int32_t* ids = p.ids ? p.ids + b * p.N : nullptr;
+    E* y = (E*)p.y + b * p.N * p.C + c;
+
+    float w[W][VEC], bias[VEC];
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) {
+        bias[i] = p.bias ? p.bias[c + i] : 0.0f;
+#pragma unroll
+        for (int k = 0; k < W; ++k) w[k][i] = p.weight[(c + i) * W + W - 1 - k];
+    }
+    // rows t0-W+1 .. t0+T-1 of the input; those before the first token come from the window
+    float in[T + W - 1][VEC];
+#pragma unroll
+    for (int r = 0; r < T + W - 1; ++r) {
+        const int64_t t = t0 + r - (W - 1);
+        if (t >= 0 && t < len) load_row<E, VEC>(x + t * p.x_sn, in[r]);
+        else if (t < 0 && win) load_row<E, VEC>(win + (t + W - 1) * p.C, in[r]);
+        else {
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) in[r][i] = 0.0f;
+        }
+    }
+    int back = ids ? tokens_back(ids, t0 < p.N ? t0 : 0, W - 1) : W - 1;
+#pragma unroll
+    for (int r = 0; r < T; ++r) {
+        const int64_t t = t0 + r;
+        if (t >= p.N) break;
+        bool live = t < len;
+        if (ids) {
+            if (r) back = ids[t] == ids[t - 1] ? min(back + 1, W - 1) : 0;
+            live = ids[t] >= 0;
+        }
+        float out[VEC];
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+            float s = bias[i];
+#pragma unroll
+            for (int k = 0; k < W; ++k) s += k <= back ? w[k][i] * in[r + W - 1 - k][i] : 0.0f;
+            if (p.silu) s *= sigmoid(s);
+            out[i] = live ? s : 0.0f;
+        }
+        store_row<E, VEC>(y + t * p.C, out);
+    }
+    // the window after the last token: inputs len-W+1 .. len-1
+    if (p.window_out && tile == 0) {
+        E* wo = (E*)p.window_out + b * (W - 1) * p.C + c;
+#pragma unroll
+        for (int r = 0; r < W - 1; ++r) {
+            const int64_t t = len - (W - 1) + r;
+            float v[VEC];
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) v[i] = 0.0f;
+            if (t >= 0) load_row<E, VEC>(x + t * p.x_sn, v);
+            else if (win) load_row<E, VEC>(win + (t + W - 1) * p.C, v);
+            store_row<E, VEC>(wo + r * p.C, v);
+        }
+    }
+}
+
+// A thread walks over tokens t0 .. t0+T+W-2: the last W - 1 of them only for the dx of the ones
+// before.  It leaves its sums for dw and db in partial [B * tiles][W + 1][C].
+template <typename E, int W, int VEC, int T>
+__global__ __launch_bounds__(256) void conv_backward_kernel(ConvArgs p) {
+    const int64_t groups = p.C / VEC;
+    const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (id >= groups * p.tiles * p.B) return;
+    const int64_t c = (id % groups) * VEC, tile = id / groups % p.tiles, b = id / groups / p.tiles;
+    const int64_t t0 = tile * T;
+    const E* x = (const E*)p.x + b * p.x_sb + c;
+    const E* dy = (const E*)p.dy + b * p.N * p.C + c;
+    E* dx = (E*)p.dx + b * p.N * p.C + c;
+    const int32_t* ids = p.ids ? p.ids + b * p.N : nullptr;
+
+    float w[W][VEC], bias[VEC], dw[W][VEC], db[VEC];
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) {
+        bias[i] = p.bias ? p.bias[c + i] : 0.0f;
+        db[i] = 0.0f;
+#pragma unroll
+        for (int k = 0; k < W; ++k) {
+            w[k][i] = p.weight[(c + i) * W + W - 1 - k];
+            dw[k][i] = 0.0f;
+        }
+    }
+    // in[k]: the input k tokens back; acc[k]: the dx so far of the token k back
+    float in[W][VEC], acc[W][VEC];
+#pragma unroll
+    for (int k = 0; k < W; ++k) {
+        const int64_t t = t0 - 1 - k;
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) in[k][i] = acc[k][i] = 0.0f;
+        if (k < W - 1 && t >= 0 && (!ids || ids[t] >= 0)) load_row<E, VEC>(x + t * p.x_sn, in[k]);
+    }
+    int back = ids ? tokens_back(ids, t0, W - 1) : W - 1;
+    const int64_t end = min(t0 + T, p.N), stop = min(end + W - 1, p.N);
+    // A block of U tokens at once keeps 2 U loads in flight.
+    constexpr int U = 4;
+    for (int64_t t4 = t0; t4 < end + W - 1; t4 += U) {
+        float xs[U][VEC], ds[U][VEC];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) xs[u][i] = ds[u][i] = 0.0f;
+            if (t4 + u < stop && (!ids || ids[t4 + u] >= 0)) {
+                load_row<E, VEC>(x + (t4 + u) * p.x_sn, xs[u]);
+                load_row<E, VEC>(dy + (t4 + u) * p.C, ds[u]);
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int64_t t = t4 + u;
+            if (ids && t > t0 && t < stop) back = ids[t] == ids[t - 1] ? min(back + 1, W - 1) : 0;
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) {
+#pragma unroll
+                for (int k = W - 1; k > 0; --k) {
+                    in[k][i] = in[k - 1][i];
+                    acc[k][i] = acc[k - 1][i];
+                }
+                in[0][i] = xs[u][i];
+                acc[0][i] = 0.0f;
+                float d = ds[u][i];
+                if (p.silu) {
+                    float s = bias[i];
+#pragma unroll
+                    for (int k = 0; k < W; ++k) s += k <= back ? w[k][i] * in[k][i] : 0.0f;
+                    const float g = sigmoid(s);
+                    d *= g * (1.0f + s * (1.0f - g));
+                }
+#pragma unroll
+                for (int k = 0; k < W; ++k) {
+                    acc[k][i] += k <= back ? w[k][i] * d : 0.0f;
+                    if (t < end) dw[k][i] += k <= back ? d * in[k][i] : 0.0f;
+                }
+                if (t < end) db[i] += d;
+            }
+            // token t - (W-1) has all its terms
+            const int64_t done = t - (W - 1);
+            if (done >= t0 && done < end) store_row<E, VEC>(dx + done * p.C, acc[W - 1]);
+        }
+    }
+    float* out = p.partial + (b * p.tiles + tile) * (W + 1) * p.C + c;
+#pragma unroll
+    for (int k = 0; k < W; ++k) store_row<float, VEC>(out + (W - 1 - k) * p.C, dw[k]);
+    store_row<float, VEC>(out + W * p.C, db);
+}
+
+// One token: the window moves on by it in place.  mask 0: nothing changes and y = 0.
+template <typename E, int W, int VEC>
+__global__ __launch_bounds__(256) void conv_step_kernel(ConvArgs p, const int32_t* mask) {
+    const int64_t groups = p.C / VEC;
+    const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (id >= groups * p.B) return;
+    const int64_t c = (id % groups) * VEC, b = id / groups;
+    float out[VEC];
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) out[i] = 0.0f;
+    if (!mask || mask[b]) {
+        E* win = (E*)p.window_out + b * (W - 1) * p.C + c;
+        float in[W][VEC];
+        load_row<E, VEC>((const E*)p.x + b * p.x_sb + c, in[0]);
+#pragma unroll
+        for (int k = 1; k < W; ++k) load_row<E, VEC>(win + (W - 1 - k) * p.C, in[k]);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+            float s = p.bias ? p.bias[c + i] : 0.0f;
+#pragma unroll
+            for (int k = 0; k < W; ++k) s += p.weight[(c + i) * W + W - 1 - k] * in[k][i];
+            if (p.silu) s *= sigmoid(s);
+            out[i] = s;
+        }
+#pragma unroll
+        for (int r = 0; r < W - 1; ++r) store_row<E, VEC>(win + r * p.C, in[W - 2 - r]);
+    }
+    store_row<E, VEC>((E*)p.y + b * p.C + c, out);
+}
+
+// dw [C, W] and db [C] from the sums of the column sums' layout [W + 1][C].
+__global__ __launch_bounds__(256) void conv_weight_grad_kernel(const float* sums, int64_t C, int W, float* dw,
+                                                               float* db) {
+    const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (id >= C * (W + 1)) return;
+    const int64_t k = id / C, c = id % C;
+    if (k < W) dw[c * W + k] = sums[id];
+    else if (db) db[c] = sums[id];
+}
+
+// 64 columns a workgroup, 16 threads to a column, each over its share of the rows in order.
+__global__ __launch_bounds__(1024) void column_sums_kernel(const float* partial, int64_t R, int64_t cols, float* out) {
+    __shared__ float red[16][65];
+    const int lane = threadIdx.x & 63, part = threadIdx.x >> 6;
+    const int64_t col = (int64_t)blockIdx.x * 64 + lane;
+    float s = 0.0f;
+    if (col < cols) {
+        const int64_t per = (R + 15) / 16, r0 = part * per, r1 = min(r0 + per, R);
+        int64_t r = r0;
+        for (; r + 8 <= r1; r += 8) {
+            float v[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = partial[(r + i) * cols + col];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) s += v[i];
+        }
+        for (; r < r1; ++r) s += partial[r * cols + col];
+    }
+    red[part][lane] = s;
+    __syncthreads();
+    if (part == 0 && col < cols) {
+        float t = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) t += red[i][lane];
+        out[col] = t;
+    }
+}
+
+int launch_column_sums(const float* partial, int64_t R, int64_t cols, float* out, hipStream_t stream) {
+    column_sums_kernel<<<dim3((unsigned)ceil_div(cols, 64)), 1024, 0, stream>>>(partial, R, cols, out);
+    return check_launch("column_sums");
+}
+
+constexpr int kConvBackTokens = 32;
+
+template <typename E>
+static bool conv_vector(const ConvArgs& p, int64_t W) {
+    constexpr int V = 16 / sizeof(E);
+    auto bad = [](const void* q) { return ((uintptr_t)q & 15) != 0; };
+    return p.C % V == 0 && p.x_sb % V == 0 && p.x_sn % V == 0 && !bad(p.x) && !bad(p.y) && !bad(p.window) &&
+           !bad(p.window_out) && !bad(p.dy) && !bad(p.dx) && !bad(p.partial);
+}
+
+template <typename E, int W, int VEC>
+static void conv_forward_go(ConvArgs p, hipStream_t stream) {
+    // Long runs read the rows before a run less often, short ones spread a small call over the
+    // GPU.
+    const int64_t lanes = p.B * (p.C / VEC);
+    auto grid = [&](int T) {
+        p.tiles = ceil_div(p.N, T);
+        return dim3((unsigned)ceil_div(lanes * p.tiles, 256));
+    };
+    if (lanes * p.N >= (int64_t)8 * 65536) {
+        const dim3 g = grid(8);
+        conv_forward_kernel<E, W, VEC, 8><<<g, 256, 0, stream>>>(p);
+    } else {
+        const dim3 g = grid(2);
+        conv_forward_kernel<E, W, VEC, 2><<<g, 256, 0, stream>>>(p);
+    }
+}
+
+template <typename E, int VEC>
+static int conv_forward_w(const ConvArgs& p, int64_t W, hipStream_t stream) {
+    if (W == 2) conv_forward_go<E, 2, VEC>(p, stream);
+    else if (W == 3) conv_forward_go<E, 3, VEC>(p, stream);
+    else conv_forward_go<E, 4, VEC>(p, stream);
+    return check_launch("conv_forward");
+}
+template <typename E>
+static int conv_forward_e(const ConvArgs& p, int64_t W, hipStream_t stream) {
+    return conv_vector<E>(p, W) ? conv_forward_w<E, 16 / sizeof(E)>(p, W, stream) : conv_forward_w<E, 1>(p, W, stream);
+}
+
+template <typename E, int VEC>
+static int conv_backward_w(ConvArgs p, int64_t W, hipStream_t stream) {
+    p.tiles = ceil_div(p.N, kConvBackTokens);
+    const dim3 g((unsigned)ceil_div(p.B * (p.C / VEC) * p.tiles, 256));
+    if (W == 2) conv_backward_kernel<E, 2, VEC, kConvBackTokens><<<g, 256, 0, stream>>>(p);
+    else if (W == 3) conv_backward_kernel<E, 3, VEC, kConvBackTokens><<<g, 256, 0, stream>>>(p);
+    else conv_backward_kernel<E, 4, VEC, kConvBackTokens><<<g, 256, 0, stream>>>(p);
+    return check_launch("conv_backward");
+}
+template <typename E>
+static int conv_backward_e(const ConvArgs& p, int64_t W, hipStream_t stream) {
+    return conv_vector<E>(p, W) ? conv_backward_w<E, 16 / sizeof(E)>(p, W, stream) : conv_backward_w<E, 1>(p, W, stream);
+}
+
+template <typename E, int VEC>
+static int conv_step_w(const ConvArgs& p, int64_t W, const int32_t* mask, hipStream_t stream) {
+    const dim3 g((unsigned)ceil_div(p.B * (p.C / VEC), 256));
+    if (W == 2) conv_step_kernel<E, 2, VEC><<<g, 256, 0, stream>>>(p, mask);
+    else if (W == 3) conv_step_kernel<E, 3, VEC><<<g, 256, 0, stream>>>(p, mask);
+    else conv_step_kernel<E, 4, VEC><<<g, 256, 0, stream>>>(p, mask);
+    return check_launch("conv_step");
+}
+template <typename E>
+static int conv_step_e(const ConvArgs& p, int64_t W, const int32_t* mask, hipStream_t stream) {
+    return conv_vector<E>(p, W) ? conv_step_w<E, 16 / sizeof(E)>(p, W, mask, stream)
+                                : conv_step_w<E, 1>(p, W, mask, stream);
+}
+
+static size_t conv_backward_bytes(int64_t B, int64_t N, int64_t C, int64_t W) {
+    return (size_t)(B * ceil_div(N, kConvBackTokens) + 1) * (W + 1) * C * sizeof(float);
+}
+
+}  // namespace mix
+}  // namespace flare
+
+using namespace flare;
+using namespace flare::mix;
+
+#define CONV_REQUIRE_SIZES(name)                                                                             \
+    FLARE_REQUIRE(known_dtype(dtype), name ": unknown dtype %d", dtype);                                     \
+    FLARE_REQUIRE(B >= 1 && N >= 1 && C >= 1, name ": B, N and C must be positive");                         \
+    FLARE_REQUIRE(W >= 2 && W <= 4, name ": W must be 2, 3 or 4, got %lld", (long long)W);                   \
+    FLARE_REQUIRE(B <= INT32_MAX && N <= INT32_MAX && C <= (1 << 20) && B * N <= ((int64_t)1 << 38) / C,      \
+                  name ": too large")
+
+extern "C" int flare_conv_forward(const void* x, int64_t x_stride_b, int64_t x_stride_n, const float* weight,
+                                  const float* bias, int silu, int dtype, int64_t B, int64_t N, int64_t C, int64_t W,
+                                  const int32_t* document_ids, const int32_t* lengths, const void* window, void* y,
+                                  void* window_out, void* stream) {
+    CONV_REQUIRE_SIZES("flare_conv_forward");
+    FLARE_REQUIRE(x && weight && y, "flare_conv_forward: null pointer");
+    FLARE_REQUIRE(!(document_ids && (lengths || window || window_out)),
+                  "flare_conv_forward: document_ids exclude lengths and windows");
+    FLARE_REQUIRE(!window_out || window_out != window, "flare_conv_forward: the windows overlap");
+    ConvArgs p = {};
+    p.x = x, p.x_sb = x_stride_b, p.x_sn = x_stride_n, p.weight = weight, p.bias = bias, p.ids = document_ids;
+    p.lengths = lengths, p.window = window, p.y = y, p.window_out = window_out, p.B = B, p.N = N, p.C = C;
+    p.silu = silu;
+    return FLARE_BY_DTYPE(dtype, conv_forward_e, (p, W, (hipStream_t)stream));
+}
+
+extern "C" size_t flare_conv_backward_workspace_size(int64_t B, int64_t N, int64_t C, int64_t W) {
+    return conv_backward_bytes(B, N, C, W);
+}
+
+extern "C" int flare_conv_backward(const void* x, int64_t x_stride_b, int64_t x_stride_n, const float* weight,
+                                   const float* bias, int silu, int dtype, int64_t B, int64_t N, int64_t C, int64_t W,
+                                   const int32_t* document_ids, const void* dy, void* dx, float* dweight,
+                                   float* dbias, void* workspace, size_t workspace_bytes, void* stream) {
+    CONV_REQUIRE_SIZES("flare_conv_backward");
+    FLARE_REQUIRE(x && weight && dy && dx && dweight && workspace, "flare_conv_backward: null pointer");
+    if (workspace_bytes < conv_backward_bytes(B, N, C, W)) {
+        set_error("flare_conv_backward: workspace of %zu bytes is too small", workspace_bytes);
+        return FLARE_ERR_WORKSPACE;
+    }
+    ConvArgs p = {};
+    p.x = x, p.x_sb = x_stride_b, p.x_sn = x_stride_n, p.weight = weight, p.bias = bias, p.ids = document_ids;
+    p.dy = dy, p.dx = dx, p.partial = (float*)workspace, p.B = B, p.N = N, p.C = C, p.silu = silu;
+    int rc = FLARE_BY_DTYPE(dtype, conv_backward_e, (p, W, (hipStream_t)stream));
+    if (rc != FLARE_OK) return rc;
+    const int64_t rows = B * ceil_div(N, kConvBackTokens), cols = (W + 1) * C;
+    float* sums = p.partial + rows * cols;
+    rc = launch_column_sums(p.partial, rows, cols, sums, (hipStream_t)stream);
+    if (rc != FLARE_OK) return rc;
+    conv_weight_grad_kernel<<<dim3((unsigned)ceil_div(cols, 256)), 256, 0, (hipStream_t)stream>>>(sums, C, (int)W,
+                                                                                                 dweight, dbias);
+    return check_launch("conv_weight_grad");
+}
+
+extern "C" int flare_conv_step(const void* x, int64_t x_stride_b, const float* weight, const float* bias, int silu,
+                               int dtype, int64_t B, int64_t C, int64_t W, const int32_t* mask, void* window, void* y,
+                               void* stream) {
+    const int64_t N = 1;
+    CONV_REQUIRE_SIZES("flare_conv_step");
+    FLARE_REQUIRE(x && weight && window && y, "flare_conv_step: null pointer");
+    ConvArgs p = {};
+    p.x = x, p.x_sb = x_stride_b, p.weight = weight, p.bias = bias, p.window_out = window, p.y = y;
+    p.B = B, p.N = 1, p.C = C, p.silu = silu;
+    return FLARE_BY_DTYPE(dtype, conv_step_e, (p, W, mask, (hipStream_t)stream));
+}

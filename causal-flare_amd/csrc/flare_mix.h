@@ -1,0 +1,73 @@
+// flare_mix.h -- helpers of the short convolution, the state space scan and softmax attention.
+#pragma once
+
+#include "flare_common.h"
+#include "flare_mfma.h"
+
+namespace flare {
+namespace mix {
+
+using mfma::kLn2;
+using mfma::kLog2e;
+
+// Function `fn`<element type>(...) for the element type code `dtype`.
+#define FLARE_BY_DTYPE(dtype, fn, ...)                               \
+    ((dtype) == FLARE_F32    ? fn<float> __VA_ARGS__                 \
+     : (dtype) == FLARE_BF16 ? fn<__hip_bfloat16> __VA_ARGS__        \
+                             : fn<__half> __VA_ARGS__)
+
+inline bool known_dtype(int dtype) { return dtype == FLARE_F32 || dtype == FLARE_BF16 || dtype == FLARE_F16; }
+inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+__device__ __forceinline__ float sigmoid(float x) { return __builtin_amdgcn_rcpf(1.0f + __expf(-x)); }
+
+// log(1 + e^x): the larger part exactly, the rest through log1p, so that the small steps of
+// x far below 0 keep their relative accuracy.
+__device__ __forceinline__ float softplus(float x) { return fmaxf(x, 0.0f) + log1pf(__expf(-fabsf(x))); }
+
+// a of the lower and b of the upper 32 lanes, then the other halves (permlane32_swap); the same
+// for each 16 of 32 lanes (permlane16_swap).  What add(first, second) leaves is thus the sum
+// of a over lanes l and l ^ 32 (or 16) in one half of the lanes and that of b in the other.
+struct Halves {
+    float first, second;
+};
+__device__ __forceinline__ Halves swap32(float a, float b) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(unsigned, a), __builtin_bit_cast(unsigned, b),
+                                                    false, false);
+    const unsigned lo = r[0], hi = r[1];      // a bit cast of r[1] itself reads r[0]
+    return Halves{__builtin_bit_cast(float, lo), __builtin_bit_cast(float, hi)};
+}
+__device__ __forceinline__ Halves swap16(float a, float b) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(unsigned, a), __builtin_bit_cast(unsigned, b),
+                                                    false, false);
+    const unsigned lo = r[0], hi = r[1];
+    return Halves{__builtin_bit_cast(float, lo), __builtin_bit_cast(float, hi)};
+}
+
+// VEC consecutive elements of one row as floats, one load where VEC is more than 1.
+template <typename T, int VEC>
+struct Pack {
+    T v[VEC];
+};
+template <typename T, int VEC>
+__device__ __forceinline__ void load_row(const T* p, float (&out)[VEC]) {
+    typedef Pack<T, VEC> P;
+    struct alignas(VEC * sizeof(T)) A { P p; };
+    const A a = *reinterpret_cast<const A*>(p);
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) out[i] = to_f32(a.p.v[i]);
+}
+template <typename T, int VEC>
+__device__ __forceinline__ void store_row(T* p, const float (&in)[VEC]) {
+    typedef Pack<T, VEC> P;
+    struct alignas(VEC * sizeof(T)) A { P p; } a;
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) a.p.v[i] = from_f32<T>(in[i]);
+    *reinterpret_cast<A*>(p) = a;
+}
+
+// Sums the R rows of partial [R, cols] in a fixed order into out [cols] (flare_conv.hip).
+int launch_column_sums(const float* partial, int64_t R, int64_t cols, float* out, hipStream_t stream);
+
+}  // namespace mix
+}  // namespace flare

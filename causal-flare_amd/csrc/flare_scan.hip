@@ -1,0 +1,353 @@
+// flare_scan.hip -- the selective state space scan: forward and single-token step.
+//
+// scan_chunk: a lane is a channel and holds its S states and rates in registers, so B_t and
+// C_t are the same for the whole wave: they are scalar loads, and scalar operands of the
+// vector instructions.  An element of the state costs an exponential (16 cycles of a SIMD a
+// wave), two products and two fused products (4 each): the exponentials bound it, and both
+// passes over a chunk pay them.
+#include "flare_scan.h"
+
+namespace flare {
+namespace scan {
+
+// B and C of every token in fp32 with zeros behind S: rows that scalar loads can take whole.
+// Padding's rows are 0, whatever they hold.
+template <typename E>
+__global__ __launch_bounds__(256) void scan_pack_kernel(ScanArgs p, int SP) {
+    const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (id >= p.B * p.N * p.G * 2 * SP) return;
+    const int s = (int)(id % SP), which = (int)(id / SP % 2);
+    const int64_t g = id / (2 * SP) % p.G, t = id / (2 * SP) / p.G % p.N, b = id / (2 * SP) / p.G / p.N;
+    float v = 0.0f;
+    if (s < p.S && !(p.ids && p.ids[b * p.N + t] < 0)) {
+        v = which ? to_f32(((const E*)p.Cm)[b * p.C_sb + t * p.C_sn + g * p.C_sg + s])
+                  : to_f32(((const E*)p.Bm)[b * p.B_sb + t * p.B_sn + g * p.B_sg + s]);
+    }
+    p.bc[id] = v;
+}
+
+template <typename E>
+static int pack_go(const ScanArgs& p, int64_t SP, hipStream_t stream) {
+    scan_pack_kernel<E><<<dim3((unsigned)ceil_div(p.B * p.N * p.G * 2 * SP, 256)), 256, 0, stream>>>(p, (int)SP);
+    return check_launch("scan_pack");
+}
+int launch_pack(const ScanArgs& p, int dtype, int64_t SP, hipStream_t stream) {
+    return FLARE_BY_DTYPE(dtype, pack_go, (p, SP, stream));
+}
+
+// One channel block of 64 (within a group) and one chunk a wave.  OUT false: leaves the chunk's
+// end state in the next chunk's slot of `states` and its sum of delta in `dsum`.
+template <typename E, int SP, bool OUT>
+__global__ __launch_bounds__(256) void scan_chunk_kernel(ScanArgs p) {
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int64_t per = (p.Cg + 63) / 64, cb = (int64_t)blockIdx.y * 4 + wave, b = blockIdx.z, chunk = blockIdx.x;
+    if (cb >= p.G * per) return;
+    const int64_t g = cb / per, cl = cb % per * 64 + lane;
+    const bool active = cl < p.Cg;
+    const int64_t c = g * p.Cg + (active ? cl : p.Cg - 1);
+    const int64_t len = row_length(p, b);
+    const int64_t t0 = chunk * p.L, t1 = min(t0 + p.L, len), tn = min(t0 + p.L, p.N);
+    const E* x = (const E*)p.x + b * p.x_sb + c;
+    const E* dt = (const E*)p.dt + b * p.dt_sb + c;
+    const E* z = p.z ? (const E*)p.z + b * p.z_sb + c : nullptr;
+    E* y = (E*)p.y + (b * p.N) * p.C + c;
+    const int32_t* ids = p.ids ? p.ids + b * p.N : nullptr;
+    scalar_f* bc = scalar_ptr(p.bc + ((b * p.N) * p.G + g) * 2 * SP);
+    const int64_t bc_step = p.G * 2 * SP;
+
+    float h[SP], A2[SP];
+#pragma unroll
+    for (int s = 0; s < SP; ++s) {
+        A2[s] = s < p.S ? p.A[c * p.S + s] * kLog2e : 0.0f;
+        h[s] = 0.0f;
+    }
+    if (OUT) {
+        if (p.NC > 1) {
+#pragma unroll
+            for (int s = 0; s < SP; ++s) h[s] = p.states[((b * p.NC + chunk) * SP + s) * p.C + c];
+        } else if (p.h0) {
+#pragma unroll
+            for (int s = 0; s < SP; ++s) h[s] = s < p.S ? p.h0[(b * p.C + c) * p.S + s] : 0.0f;
+        }
+    }
+    const float bias = p.dt_bias ? p.dt_bias[c] : 0.0f;
+    const float skip = OUT && p.D ? p.D[c] : 0.0f;
+    float sum = 0.0f;
+    bool cut = false;                              // a document begins within the chunk
+
+    constexpr int U = 4;
+    E xr[U], dr[U], zr[U];
+    auto fetch = [&](int64_t t) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int64_t at = min(t + u, t1 - 1);
+            xr[u] = x[at * p.x_sn];
+            dr[u] = dt[at * p.dt_sn];
+            if (OUT && z) zr[u] = z[at * p.z_sn];
+        }
+    };
+    if (t0 < t1) fetch(t0);
+    for (int64_t t4 = t0; t4 < t1; t4 += U) {
+        float xs[U], ds[U], zs[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            xs[u] = to_f32(xr[u]);
+            ds[u] = to_f32(dr[u]) + bias;
+            if (p.softplus) ds[u] = mix::softplus(ds[u]);
+            zs[u] = OUT && z ? to_f32(zr[u]) : 0.0f;
+        }
+        if (t4 + U < t1) fetch(t4 + U);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int64_t t = t4 + u;
+            if (t >= t1) break;
+            if (ids) {
+                if (begins(ids, t)) {
+                    cut = true;
+#pragma unroll
+                    for (int s = 0; s < SP; ++s) h[s] = 0.0f;
+                }
+                if (ids[t] < 0) {
+                    if (OUT && active) y[t * p.C] = from_f32<E>(0.0f);
+                    continue;
+                }
+            }
+            const float delta = ds[u], du = delta * xs[u];
+            sum += delta;
+            scalar_f* row = bc + t * bc_step;
+            float out[4] = {skip * xs[u], 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int s = 0; s < SP; ++s) {
+                h[s] = __builtin_amdgcn_exp2f(delta * A2[s]) * h[s] + du * row[s];
+                if (OUT) out[s & 3] += row[SP + s] * h[s];
+            }
+            if (OUT) {
+                float o = (out[0] + out[1]) + (out[2] + out[3]);
+                if (z) o *= zs[u] * mix::sigmoid(zs[u]);
+                if (active) y[t * p.C] = from_f32<E>(o);
+            }
+        }
+    }
+    if (!active) return;
+    if (OUT) {
+        for (int64_t t = max(t0, len); t < tn; ++t) y[t * p.C] = from_f32<E>(0.0f);
+        const int64_t last = len > 0 ? (len - 1) / p.L : 0;
+        if (p.h_fin && chunk == last) {
+#pragma unroll
+            for (int s = 0; s < SP; ++s)
+                if (s < p.S) p.h_fin[(b * p.C + c) * p.S + s] = h[s];
+        }
+    } else {
+#pragma unroll
+        for (int s = 0; s < SP; ++s) p.states[((b * p.NC + chunk + 1) * SP + s) * p.C + c] = h[s];
+        p.dsum[(b * p.NC + chunk) * p.C + c] = sum;
+        if (ids && c == 0) p.cuts[b * p.NC + chunk] = cut;
+    }
+}
+
+// The state before each chunk from the chunks' end states, in place: slot k + 1 holds chunk k's
+// own end state, and then the state before chunk k + 1.
+__global__ __launch_bounds__(256) void scan_states_kernel(ScanArgs p, int SP) {
+    const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (id >= p.B * SP * p.C) return;
+    const int64_t c = id % p.C, s = id / p.C % SP, b = id / p.C / SP;
+    const float A2 = s < p.S ? p.A[c * p.S + s] * kLog2e : 0.0f;
+    float h = p.h0 && s < p.S ? p.h0[(b * p.C + c) * p.S + s] : 0.0f;
+    float* slot = p.states + ((b * p.NC) * SP + s) * p.C + c;
+    const int64_t step = SP * p.C;
+    const float* dsum = p.dsum + (b * p.NC) * p.C + c;
+    slot[0] = h;
+    constexpr int U = 8;
+    for (int64_t k0 = 0; k0 + 1 < p.NC; k0 += U) {
+        float own[U], dec[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int64_t k = min(k0 + u, p.NC - 2);
+            own[u] = slot[(k + 1) * step];
+            dec[u] = __builtin_amdgcn_exp2f(A2 * dsum[k * p.C]);
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int64_t k = k0 + u;
+            if (k + 1 >= p.NC) break;
+            // a document's beginning cuts off what came before it
+            h = p.ids && p.cuts[b * p.NC + k] ? own[u] : dec[u] * h + own[u];
+            slot[(k + 1) * step] = h;
+        }
+    }
+}
+
+int launch_states(const ScanArgs& p, int64_t SP, hipStream_t stream) {
+    scan_states_kernel<<<dim3((unsigned)ceil_div(p.B * SP * p.C, 256)), 256, 0, stream>>>(p, (int)SP);
+    return check_launch("scan_states");
+}
+
+template <typename E, int SP>
+static int forward_go(const ScanArgs& p, hipStream_t stream) {
+    const int64_t blocks = ceil_div(p.G * ceil_div(p.Cg, 64), 4);
+    if (p.NC > 1) {
+        scan_chunk_kernel<E, SP, false>
+            <<<dim3((unsigned)(p.NC - 1), (unsigned)blocks, (unsigned)p.B), 256, 0, stream>>>(p);
+        int rc = check_launch("scan_chunk");
+        if (rc == FLARE_OK) rc = launch_states(p, SP, stream);
+        if (rc != FLARE_OK) return rc;
+    }
+    scan_chunk_kernel<E, SP, true><<<dim3((unsigned)p.NC, (unsigned)blocks, (unsigned)p.B), 256, 0, stream>>>(p);
+    return check_launch("scan_output");
+}
+template <typename E>
+static int forward_e(const ScanArgs& p, int64_t SP, hipStream_t stream) {
+    return SP == 8    ? forward_go<E, 8>(p, stream)
+           : SP == 16 ? forward_go<E, 16>(p, stream)
+           : SP == 32 ? forward_go<E, 32>(p, stream)
+                      : forward_go<E, 64>(p, stream);
+}
+
+// One token.  Four lanes share a channel, SP / 4 states each, so a wave reads and writes the
+// states of 16 channels as one run of memory; the states' bytes bound it.
+template <typename E, int SP, bool WHOLE>
+__global__ __launch_bounds__(256) void scan_step_kernel(ScanArgs p, const int32_t* mask, float* state) {
+    constexpr int SL = SP / 4;
+    const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const int q = (int)(id & 3);
+    if ((id >> 2) >= p.B * p.C) return;                 // whole quads
+    const int64_t b = (id >> 2) / p.C, c = (id >> 2) % p.C, g = c / p.Cg;
+    float o = 0.0f;
+    if (!mask || mask[b]) {
+        const int s0 = q * SL;
+        float* hp = state + (b * p.C + c) * p.S + s0;
+        const float* A = p.A + c * p.S + s0;
+        const E* Bm = (const E*)p.Bm + b * p.B_sb + g * p.B_sg + s0;
+        const E* Cm = (const E*)p.Cm + b * p.C_sb + g * p.C_sg + s0;
+        const float xv = to_f32(((const E*)p.x)[b * p.x_sb + c]);
+        float delta = to_f32(((const E*)p.dt)[b * p.dt_sb + c]) + (p.dt_bias ? p.dt_bias[c] : 0.0f);
+        float h[SL], av[SL];
+        if (WHOLE) {
+            typedef float fv __attribute__((ext_vector_type(SL < 4 ? SL : 4)));
+            constexpr int V = SL < 4 ? SL : 4;
+#pragma unroll
+            for (int i = 0; i < SL; i += V) {
+                const fv hv = *reinterpret_cast<const fv*>(hp + i), a4 = *reinterpret_cast<const fv*>(A + i);
+#pragma unroll
+                for (int j = 0; j < V; ++j) {
+                    h[i + j] = hv[j];
+                    av[i + j] = a4[j];
+                }
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < SL; ++i) {
+                h[i] = s0 + i < p.S ? hp[i] : 0.0f;
+                av[i] = s0 + i < p.S ? A[i] : 0.0f;
+            }
+        }
+        if (p.softplus) delta = mix::softplus(delta);
+        const float du = delta * xv;
+#pragma unroll
+        for (int i = 0; i < SL; ++i) {
+            if (WHOLE || s0 + i < p.S) {
+                h[i] = __builtin_amdgcn_exp2f(delta * av[i] * kLog2e) * h[i] + du * to_f32(Bm[i]);
+                o += to_f32(Cm[i]) * h[i];
+            }
+        }
+        if (WHOLE) {
+            typedef float fv __attribute__((ext_vector_type(SL < 4 ? SL : 4)));
+            constexpr int V = SL < 4 ? SL : 4;
+#pragma unroll
+            for (int i = 0; i < SL; i += V) {
+                fv hv;
+#pragma unroll
+                for (int j = 0; j < V; ++j) hv[j] = h[i + j];
+                *reinterpret_cast<fv*>(hp + i) = hv;
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < SL; ++i)
+                if (s0 + i < p.S) hp[i] = h[i];
+        }
+        o += mfma::dpp<mfma::kQuadXor1>(o);
+        o += mfma::dpp<mfma::kQuadXor2>(o);
+        if (p.D) o += p.D[c] * xv;
+        if (p.z) {
+            const float zv = to_f32(((const E*)p.z)[b * p.z_sb + c]);
+            o *= zv * mix::sigmoid(zv);
+        }
+    }
+    if (q == 0) ((E*)p.y)[b * p.C + c] = from_f32<E>(o);
+}
+
+template <typename E, int SP>
+static int step_go(const ScanArgs& p, const int32_t* mask, float* state, hipStream_t stream) {
+    const dim3 g((unsigned)ceil_div(p.B * p.C * 4, 256));
+    const bool whole = p.S == SP && ((uintptr_t)state & 15) == 0 && ((uintptr_t)p.A & 15) == 0;
+    if (whole) scan_step_kernel<E, SP, true><<<g, 256, 0, stream>>>(p, mask, state);
+    else scan_step_kernel<E, SP, false><<<g, 256, 0, stream>>>(p, mask, state);
+    return check_launch("scan_step");
+}
+template <typename E>
+static int step_e(const ScanArgs& p, const int32_t* mask, float* state, hipStream_t stream) {
+    const int64_t SP = padded_states(p.S);
+    return SP == 8    ? step_go<E, 8>(p, mask, state, stream)
+           : SP == 16 ? step_go<E, 16>(p, mask, state, stream)
+           : SP == 32 ? step_go<E, 32>(p, mask, state, stream)
+                      : step_go<E, 64>(p, mask, state, stream);
+}
+
+}  // namespace scan
+}  // namespace flare
+
+using namespace flare;
+using namespace flare::scan;
+
+extern "C" int64_t flare_scan_chunk(int64_t B, int64_t N, int64_t C, int64_t S, int64_t G, int for_backward) {
+    if (B < 1 || N < 1 || C < 1 || S < 1 || S > 64 || G < 1 || C % G) return 0;
+    return chunk_length(B, N, C, G, for_backward ? backward_chunk_most(padded_states(S)) : 0);
+}
+
+extern "C" size_t flare_scan_forward_workspace_size(int64_t B, int64_t N, int64_t C, int64_t S, int64_t G,
+                                                    int64_t chunk) {
+    if (chunk < 1) return 0;
+    const int64_t SP = padded_states(S), NC = ceil_div(N, chunk);
+    return (size_t)(B * N * G * 2 * SP + B * NC * (C + 1)) * sizeof(float);
+}
+
+extern "C" int flare_scan_forward(const void* x, const void* dt, const float* A, const void* Bm, const void* Cm,
+                                  const float* D, const void* z, const float* dt_bias, int softplus, int dtype,
+                                  int64_t B, int64_t N, int64_t C, int64_t S, int64_t G, const int64_t* strides,
+                                  const int32_t* document_ids, const int32_t* lengths, const float* h0, void* y,
+                                  float* h_fin, int64_t chunk, float* states, void* workspace,
+                                  size_t workspace_bytes, void* stream) {
+    FLARE_REQUIRE(x && dt && A && Bm && Cm && y && strides && workspace, "flare_scan_forward: null pointer");
+    FLARE_REQUIRE(!(document_ids && (lengths || h0 || h_fin)),
+                  "flare_scan_forward: document_ids exclude lengths and states");
+    FLARE_REQUIRE(!h_fin || h_fin != h0, "flare_scan_forward: the states overlap");
+    SCAN_REQUIRE_SIZES("flare_scan_forward");
+    FLARE_REQUIRE(chunk >= 1, "flare_scan_forward: chunk must be positive");
+    ScanArgs p = scan_args(x, dt, A, Bm, Cm, D, z, dt_bias, softplus, B, N, C, S, G, strides);
+    const int64_t SP = padded_states(S);
+    p.L = chunk, p.NC = ceil_div(N, chunk);
+    FLARE_REQUIRE(p.NC == 1 || states, "flare_scan_forward: more than one chunk needs `states`");
+    if (workspace_bytes < flare_scan_forward_workspace_size(B, N, C, S, G, chunk)) {
+        set_error("flare_scan_forward: workspace of %zu bytes is too small", workspace_bytes);
+        return FLARE_ERR_WORKSPACE;
+    }
+    p.ids = document_ids, p.lengths = lengths, p.h0 = h0, p.y = y, p.h_fin = h_fin, p.states = states;
+    p.bc = (float*)workspace;
+    p.dsum = p.bc + B * N * G * 2 * SP;
+    p.cuts = (int32_t*)(p.dsum + B * p.NC * C);
+    const int rc = launch_pack(p, dtype, SP, (hipStream_t)stream);
+    if (rc != FLARE_OK) return rc;
+    return FLARE_BY_DTYPE(dtype, forward_e, (p, SP, (hipStream_t)stream));
+}
+
+extern "C" int flare_scan_step(const void* x, const void* dt, const float* A, const void* Bm, const void* Cm,
+                               const float* D, const void* z, const float* dt_bias, int softplus, int dtype,
+                               int64_t B, int64_t C, int64_t S, int64_t G, const int64_t* strides,
+                               const int32_t* mask, float* state, void* y, void* stream) {
+    const int64_t N = 1;
+    FLARE_REQUIRE(x && dt && A && Bm && Cm && y && strides && state, "flare_scan_step: null pointer");
+    SCAN_REQUIRE_SIZES("flare_scan_step");
+    ScanArgs p = scan_args(x, dt, A, Bm, Cm, D, z, dt_bias, softplus, B, N, C, S, G, strides);
+    p.y = y;
+    return FLARE_BY_DTYPE(dtype, step_e, (p, mask, state, (hipStream_t)stream));
+}

@@ -1,0 +1,544 @@
+// flare_scan_bwd.hip -- gradients of the selective state space scan.
+//
+//   r_t = C_t dyg_t + a_{t+1} r_{t+1}        the gradient of h_t; dyg = dy z sigmoid(z)
+//   ddelta_t = sum_s r a h_{t-1} A + x_t sum_s r B_t     dx_t = delta_t sum_s r B_t + D dyg_t
+//   dA += r a h_{t-1} delta_t       dB_t = sum_c r delta x      dC_t = sum_c dyg h_t
+//
+// scan_reverse leaves each chunk's r from behind as if nothing entered it; scan_carries joins
+// them; scan_gradient then walks each chunk twice: forward from its saved start state, keeping
+// a state every T tokens in LDS, and backward over these pieces of T tokens, each recomputed
+// with a_t and a_t h_{t-1} in registers.
+//
+// There four lanes share a channel (SL = S / 4 states each) and a wave has 16 channels: a piece
+// of T = 16 tokens then fits 128 registers at S = 16, where a lane with all the states of a
+// channel could hold only 4 tokens.  What one lane would do alone for a token (the exponentials
+// of the gates, the loads and stores) lane q of a channel does for the tokens 4i + q, and the
+// others read it through DPP.  dB and dC are summed over the wave's channels by halving: each
+// step adds two values and leaves one, half the lanes' worth of work at a time; the waves' sums
+// meet in LDS and the workgroups' in scan_dbc, always in the same order.
+#include <type_traits>
+#include <utility>
+
+#include "flare_scan.h"
+
+namespace flare {
+namespace scan {
+
+// Channel a lane, as scan_chunk: the gradient that leaves the chunk at its front.
+template <typename E, int SP>
+__global__ __launch_bounds__(256) void scan_reverse_kernel(ScanArgs p) {
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int64_t per = (p.Cg + 63) / 64, cb = (int64_t)blockIdx.y * 4 + wave, b = blockIdx.z;
+    const int64_t chunk = (int64_t)blockIdx.x + 1;             // nothing is before chunk 0
+    if (cb >= p.G * per) return;
+    const int64_t g = cb / per, cl = cb % per * 64 + lane;
+    const bool active = cl < p.Cg;
+    const int64_t c = g * p.Cg + (active ? cl : p.Cg - 1);
+    const int64_t t0 = chunk * p.L, t1 = min(t0 + p.L, p.N);
+    const E* dt = (const E*)p.dt + b * p.dt_sb + c;
+    const E* z = p.z ? (const E*)p.z + b * p.z_sb + c : nullptr;
+    const E* dy = (const E*)p.dy + (b * p.N) * p.C + c;
+    const int32_t* ids = p.ids ? p.ids + b * p.N : nullptr;
+    scalar_f* bc = scalar_ptr(p.bc + ((b * p.N) * p.G + g) * 2 * SP);
+    const int64_t bc_step = p.G * 2 * SP;
+    float r[SP], A2[SP];
+#pragma unroll
+    for (int s = 0; s < SP; ++s) {
+        A2[s] = s < p.S ? p.A[c * p.S + s] * kLog2e : 0.0f;
+        r[s] = 0.0f;
+    }
+    const float bias = p.dt_bias ? p.dt_bias[c] : 0.0f;
+    float sum = 0.0f;
+    bool cut = false;
+    constexpr int U = 4;
+    E gr[U], dr[U], zr[U];
+    auto fetch = [&](int64_t t) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int64_t at = max(t - u, t0);
+            gr[u] = dy[at * p.C];
+            dr[u] = dt[at * p.dt_sn];
+            if (z) zr[u] = z[at * p.z_sn];
+        }
+    };
+    fetch(t1 - 1);
+    for (int64_t t4 = t1 - 1; t4 >= t0; t4 -= U) {
+        float gs[U], ds[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            gs[u] = to_f32(gr[u]);
+            ds[u] = to_f32(dr[u]) + bias;
+            if (p.softplus) ds[u] = mix::softplus(ds[u]);
+            if (z) {
+                const float zv = to_f32(zr[u]);
+                gs[u] *= zv * mix::sigmoid(zv);
+            }
+        }
+        if (t4 - U >= t0) fetch(t4 - U);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int64_t t = t4 - u;
+            if (t < t0) break;
+            if (!ids || ids[t] >= 0) {
+                scalar_f* row = bc + t * bc_step + SP;
+                sum += ds[u];
+#pragma unroll
+                for (int s = 0; s < SP; ++s)
+                    r[s] = __builtin_amdgcn_exp2f(ds[u] * A2[s]) * (r[s] + gs[u] * row[s]);
+            }
+            if (ids && begins(ids, t)) {
+                cut = true;
+#pragma unroll
+                for (int s = 0; s < SP; ++s) r[s] = 0.0f;
+            }
+        }
+    }
+    if (!active) return;
+#pragma unroll
+    for (int s = 0; s < SP; ++s) p.carry[((b * p.NC + chunk - 1) * SP + s) * p.C + c] = r[s];
+    p.dsum[(b * p.NC + chunk) * p.C + c] = sum;
+    if (ids && c == 0) p.cuts[b * p.NC + chunk] = cut;
+}
+
+// Slot k - 1 of `carry` holds what leaves chunk k at its front, and then all that enters k - 1.
+__global__ __launch_bounds__(256) void scan_carries_kernel(ScanArgs p, int SP) {
+    const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (id >= p.B * SP * p.C) return;
+    const int64_t c = id % p.C, s = id / p.C % SP, b = id / p.C / SP;
+    const float A2 = s < p.S ? p.A[c * p.S + s] * kLog2e : 0.0f;
+    float* slot = p.carry + ((b * p.NC) * SP + s) * p.C + c;
+    const int64_t step = SP * p.C;
+    const float* dsum = p.dsum + (b * p.NC) * p.C + c;
+    float r = 0.0f;
+    slot[(p.NC - 1) * step] = 0.0f;
+    constexpr int U = 8;
+    for (int64_t k0 = p.NC - 1; k0 > 0; k0 -= U) {
+        float own[U], dec[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int64_t k = max(k0 - u, (int64_t)1);
+            own[u] = slot[(k - 1) * step];
+            dec[u] = __builtin_amdgcn_exp2f(A2 * dsum[k * p.C]);
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int64_t k = k0 - u;
+            if (k < 1) break;
+            r = p.ids && p.cuts[b * p.NC + k] ? own[u] : dec[u] * r + own[u];
+            slot[(k - 1) * step] = r;
+        }
+    }
+}
+
+__device__ __forceinline__ float lane_xor4(float x) {     // within 8 lanes: mirror, then each quad again
+    return mfma::dpp<0x1B>(mfma::dpp<mfma::kRowHalfMirror>(x));
+}
+__device__ __forceinline__ float lane_xor8(float x) { return mfma::dpp<0x128>(x); }   // row_ror:8
+
+// v[0 .. NV-1] of each lane summed over the 16 channels of the wave (lane bits 2 .. 5).  Leaves
+// max(1, NV / 16) values in v; `first` is the index of v[0], `own` whether this lane stores it.
+template <int NV>
+__device__ __forceinline__ void sum_channels(float (&v)[NV], int lane, int& first, bool& own) {
+    first = 0;
+    own = true;
+    auto sum = [](mix::Halves r) { return r.first + r.second; };
+    // NV >= 4: the steps over lane bits 5 and 4 always halve
+#pragma unroll
+    for (int i = 0; i < NV / 2; ++i) v[i] = sum(mix::swap32(v[i], v[i + NV / 2]));
+    first += lane & 32 ? NV / 2 : 0;
+#pragma unroll
+    for (int i = 0; i < NV / 4; ++i) v[i] = sum(mix::swap16(v[i], v[i + NV / 4]));
+    first += lane & 16 ? NV / 4 : 0;
+    if constexpr (NV >= 8) {
+#pragma unroll
+        for (int i = 0; i < NV / 8; ++i) {
+            const float a = v[i], b = v[i + NV / 8];
+            v[i] = (lane & 8 ? b : a) + lane_xor8(lane & 8 ? a : b);
+        }
+        first += lane & 8 ? NV / 8 : 0;
+    } else {
+        v[0] += lane_xor8(v[0]);
+        own = own && !(lane & 8);
+    }
+    if constexpr (NV >= 16) {
+#pragma unroll
+        for (int i = 0; i < NV / 16; ++i) {
+            const float a = v[i], b = v[i + NV / 16];
+            v[i] = (lane & 4 ? b : a) + lane_xor4(lane & 4 ? a : b);
+        }
+        first += lane & 4 ? NV / 16 : 0;
+    } else {
+        v[0] += lane_xor4(v[0]);
+        own = own && !(lane & 4);
+    }
+}
+
+// a[0 .. 3] of each lane summed over the quad; lane q gets the sum of a[q].
+__device__ __forceinline__ float quad_gather(const float (&a)[4], int q) {
+    const float lo = (q & 1 ? a[1] : a[0]) + mfma::dpp<mfma::kQuadXor1>(q & 1 ? a[0] : a[1]);
+    const float hi = (q & 1 ? a[3] : a[2]) + mfma::dpp<mfma::kQuadXor1>(q & 1 ? a[2] : a[3]);
+    return (q & 2 ? hi : lo) + mfma::dpp<mfma::kQuadXor2>(q & 2 ? lo : hi);
+}
+__device__ __forceinline__ float quad_sum(float x) {
+    x += mfma::dpp<mfma::kQuadXor1>(x);
+    return x + mfma::dpp<mfma::kQuadXor2>(x);
+}
+// Lane J of the quad, to all four.
+template <int J>
+__device__ __forceinline__ float quad_bcast(float x) {
+    return mfma::dpp<J * 0x55>(x);
+}
+
+// fn(0), fn(1), ... with compile-time indices: register arrays and DPP controls need them.
+template <typename F, int... J>
+__device__ __forceinline__ void each_token(F&& fn, std::integer_sequence<int, J...>) {
+    (fn(std::integral_constant<int, J>{}), ...);
+}
+
+constexpr int kWaves = 8;              // 128 channels a workgroup
+
+template <int SP>
+struct GradLayout {
+    static constexpr int SL = SP / 4;
+    static constexpr int T = SL <= 4 ? 16 : SL == 8 ? 8 : 4;
+    static constexpr int most = SP <= 16 ? 128 : SP == 32 ? 32 : 16;     // backward_chunk_most
+    static constexpr int pieces = most / T;
+    static constexpr int bc_floats = most * 2 * SP;
+    static constexpr int keep_floats = kWaves * pieces * 64 * SL;
+    static constexpr int red_floats = kWaves * T * 2 * SP;
+    static constexpr size_t bytes = sizeof(float) * (bc_floats + keep_floats + red_floats);
+    static_assert(bytes <= 160 * 1024, "LDS of a CU");
+};
+
+template <typename E, int SP>
+__global__ __launch_bounds__(64 * kWaves) void scan_gradient_kernel(ScanArgs p) {
+    using Lay = GradLayout<SP>;
+    constexpr int SL = Lay::SL, T = Lay::T, TQ = T / 4;
+    extern __shared__ float lds[];
+    float* bcs = lds;                                      // [L][2][SP]
+    float* keeps = bcs + Lay::bc_floats;                   // [waves][pieces][SL][64]
+    float* red = keeps + Lay::keep_floats;                 // [waves][T][2 SP]
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, q = lane & 3;
+    const int64_t per = (p.Cg + 16 * kWaves - 1) / (16 * kWaves);
+    const int64_t cb = blockIdx.y, b = blockIdx.z, chunk = blockIdx.x;
+    const int64_t g = cb / per, cl = cb % per * 16 * kWaves + wave * 16 + (lane >> 2);
+    const bool active = cl < p.Cg;
+    const int64_t c = g * p.Cg + (active ? cl : p.Cg - 1);
+    const int64_t t0 = chunk * p.L;
+    const int n = (int)(min(t0 + p.L, p.N) - t0);          // tokens of this chunk
+    const int32_t* ids = p.ids ? p.ids + b * p.N + t0 : nullptr;
+    const E* x = (const E*)p.x + b * p.x_sb + t0 * p.x_sn + c;
+    const E* dt = (const E*)p.dt + b * p.dt_sb + t0 * p.dt_sn + c;
+    const E* z = p.z ? (const E*)p.z + b * p.z_sb + t0 * p.z_sn + c : nullptr;
+    const int64_t row0 = (b * p.N + t0) * p.C + c;
+    const E* dy = (const E*)p.dy + row0;
+
+    for (int i = tid; i < n * 2 * SP; i += 64 * kWaves)
+        bcs[i] = p.bc[((b * p.N + t0 + i / (2 * SP)) * p.G + g) * 2 * SP + i % (2 * SP)];
+    __syncthreads();
+
+    float A2[SL], h[SL], r[SL], dA[SL];
+    float* keep = keeps + (size_t)wave * Lay::pieces * 64 * SL + lane;
+#pragma unroll
+    for (int i = 0; i < SL; ++i) {
+        const int s = q * SL + i;
+        A2[i] = s < p.S ? p.A[c * p.S + s] * kLog2e : 0.0f;
+        h[i] = p.NC > 1 ? p.states[((b * p.NC + chunk) * SP + s) * p.C + c] : 0.0f;
+        r[i] = p.NC > 1 ? p.carry[((b * p.NC + chunk) * SP + s) * p.C + c] : 0.0f;
+        dA[i] = 0.0f;
+    }
+    const float bias = p.dt_bias ? p.dt_bias[c] : 0.0f, skip = p.D ? p.D[c] : 0.0f;
+    float dD = 0.0f, dbias = 0.0f;
+
+    // the tokens 4 i + q of the piece at k0; a token that is none has delta = x = 0
+    auto step_of = [&](int k, float& raw, float& delta, float& xv) {
+        raw = delta = xv = 0.0f;
+        const bool live = active && k < n && (!ids || ids[k] >= 0);
+        if (live) {
+            raw = to_f32(dt[k * p.dt_sn]) + bias;
+            delta = p.softplus ? mix::softplus(raw) : raw;
+            xv = to_f32(x[k * p.x_sn]);
+        }
+        return live;
+    };
+    auto piece_begins = [&](int k0) {      // bit j: a document begins at token k0 + j
+        unsigned m = 0;
+        if (ids) {
+#pragma unroll
+            for (int j = 0; j < T; ++j) {
+                const int k = k0 + j;
+                if (k < n && t0 + k > 0 && ids[k] != ids[k - 1]) m |= 1u << j;
+            }
+        }
+        return m;
+    };
+
+    // forward over the chunk, keeping the state before each piece
+    const int pieces = (n + T - 1) / T;
+    for (int piece = 0; piece < pieces; ++piece) {
+#pragma unroll
+        for (int i = 0; i < SL; ++i) keep[(piece * SL + i) * 64] = h[i];
+        if (piece + 1 == pieces) break;
+        const int k0 = piece * T;
+        const unsigned starts = piece_begins(k0);
+        float delta[TQ], du[TQ];
+#pragma unroll
+        for (int i = 0; i < TQ; ++i) {
+            float raw, xv;
+            step_of(k0 + 4 * i + q, raw, delta[i], xv);
+            du[i] = delta[i] * xv;
+        }
+        auto token = [&](auto jc) {
+            constexpr int j = decltype(jc)::value;
+            const float* row = bcs + (k0 + j) * 2 * SP + q * SL;
+            const float dj = quad_bcast<(j & 3)>(delta[j / 4]), uj = quad_bcast<(j & 3)>(du[j / 4]);
+            if (starts >> j & 1) {
+#pragma unroll
+                for (int i = 0; i < SL; ++i) h[i] = 0.0f;
+            }
+#pragma unroll
+            for (int i = 0; i < SL; ++i) h[i] = __builtin_amdgcn_exp2f(dj * A2[i]) * h[i] + uj * row[i];
+        };
+        each_token(token, std::make_integer_sequence<int, T>{});
+    }
+
+    // backward over the pieces
+    for (int piece = pieces - 1; piece >= 0; --piece) {
+        const int k0 = piece * T;
+        const unsigned starts = piece_begins(k0);
+        float raw[TQ], delta[TQ], xv[TQ], du[TQ], gy[TQ], dyv[TQ], zv[TQ];
+        bool live[TQ];
+#pragma unroll
+        for (int i = 0; i < TQ; ++i) {
+            const int k = k0 + 4 * i + q;
+            live[i] = step_of(k, raw[i], delta[i], xv[i]);
+            du[i] = delta[i] * xv[i];
+            dyv[i] = zv[i] = 0.0f;
+            if (live[i]) {
+                dyv[i] = to_f32(dy[k * p.C]);
+                if (z) zv[i] = to_f32(z[k * p.z_sn]);
+            }
+            gy[i] = z ? dyv[i] * zv[i] * mix::sigmoid(zv[i]) : dyv[i];
+        }
+        float a[T][SL], ah[T][SL];
+#pragma unroll
+        for (int i = 0; i < SL; ++i) h[i] = keep[(piece * SL + i) * 64];
+        auto token = [&](auto jc) {
+            constexpr int j = decltype(jc)::value;
+            const float* row = bcs + min(k0 + j, n - 1) * 2 * SP + q * SL;
+            const float dj = quad_bcast<(j & 3)>(delta[j / 4]), uj = quad_bcast<(j & 3)>(du[j / 4]);
+            const bool cut = starts >> j & 1;
+#pragma unroll
+            for (int i = 0; i < SL; ++i) {
+                a[j][i] = __builtin_amdgcn_exp2f(dj * A2[i]);
+                ah[j][i] = a[j][i] * h[i];
+            }
+            if (cut) {
+#pragma unroll
+                for (int i = 0; i < SL; ++i) a[j][i] = ah[j][i] = 0.0f;
+            }
+#pragma unroll
+            for (int i = 0; i < SL; ++i) h[i] = ah[j][i] + uj * row[i];
+        };
+        each_token(token, std::make_integer_sequence<int, T>{});
+        float pA[T], sB[T], lin[T];
+        auto back = [&](auto jc) {
+            constexpr int j = T - 1 - decltype(jc)::value;
+            const float* row = bcs + min(k0 + j, n - 1) * 2 * SP + q * SL;
+            const float dj = quad_bcast<(j & 3)>(delta[j / 4]), uj = quad_bcast<(j & 3)>(du[j / 4]);
+            const float gj = quad_bcast<(j & 3)>(gy[j / 4]);
+            float v[2 * SL];
+            pA[j] = sB[j] = lin[j] = 0.0f;
+#pragma unroll
+            for (int i = 0; i < SL; ++i) {
+                const float Bv = row[i], Cv = row[SP + i];
+                const float hv = ah[j][i] + uj * Bv;
+                r[i] += Cv * gj;
+                const float w = r[i] * ah[j][i];
+                pA[j] += w * A2[i];
+                dA[i] += w * dj;
+                sB[j] += r[i] * Bv;
+                lin[j] += Cv * hv;
+                v[i] = r[i] * uj;
+                v[SL + i] = gj * hv;
+                r[i] *= a[j][i];
+            }
+            int first;
+            bool own;
+            sum_channels(v, lane, first, own);
+            if (own) {
+                constexpr int NK = SL >= 8 ? SL / 8 : 1;
+                float* out = red + (wave * T + j) * 2 * SP + q * SL;
+#pragma unroll
+                for (int m = 0; m < NK; ++m) {
+                    const int idx = first + m;           // state idx of B, or idx - SL of C
+                    out[idx < SL ? idx : SP + idx - SL] = v[m];
+                }
+            }
+        };
+        each_token(back, std::make_integer_sequence<int, T>{});
+#pragma unroll
+        for (int i = 0; i < TQ; ++i) {
+            const float pa[4] = {pA[4 * i], pA[4 * i + 1], pA[4 * i + 2], pA[4 * i + 3]};
+            const float sb[4] = {sB[4 * i], sB[4 * i + 1], sB[4 * i + 2], sB[4 * i + 3]};
+            const float ln[4] = {lin[4 * i], lin[4 * i + 1], lin[4 * i + 2], lin[4 * i + 3]};
+            const float pq = quad_gather(pa, q) * kLn2, sq = quad_gather(sb, q), lq = quad_gather(ln, q);
+            const int k = k0 + 4 * i + q;
+            float ddt = pq + xv[i] * sq;
+            if (p.softplus) ddt *= mix::sigmoid(raw[i]);
+            if (!live[i]) ddt = 0.0f;
+            dbias += ddt;
+            dD += gy[i] * xv[i];
+            if (active && k < n) {
+                ((E*)p.dx)[row0 + k * p.C] = from_f32<E>(live[i] ? delta[i] * sq + gy[i] * skip : 0.0f);
+                ((E*)p.ddt)[row0 + k * p.C] = from_f32<E>(ddt);
+                if (z) {
+                    const float sg = mix::sigmoid(zv[i]);
+                    const float dz = dyv[i] * (lq + skip * xv[i]) * sg * (1.0f + zv[i] * (1.0f - sg));
+                    ((E*)p.dz)[row0 + k * p.C] = from_f32<E>(live[i] ? dz : 0.0f);
+                }
+            }
+        }
+        // the piece's dB and dC: the waves' sums, in order
+        __syncthreads();
+        const int live_tokens = min(T, n - k0);
+        float* out = p.dbc + ((cb * p.B + b) * p.N + t0 + k0) * 2 * SP;
+        for (int i = tid; i < live_tokens * 2 * SP; i += 64 * kWaves) {
+            float s = 0.0f;
+#pragma unroll
+            for (int w = 0; w < kWaves; ++w) s += red[w * T * 2 * SP + i];
+            out[i] = s;
+        }
+        __syncthreads();
+    }
+    if (!active) return;
+    float* par = p.dpar + ((b * p.NC + chunk) * p.C + c) * (SP + 2);
+#pragma unroll
+    for (int i = 0; i < SL; ++i) par[q * SL + i] = dA[i];
+    dD = quad_sum(dD);
+    dbias = quad_sum(dbias);
+    if (q < 2) par[SP + q] = q ? dbias : dD;
+}
+
+// dB and dC of each token: the sum over the channel blocks of its group, in order.
+template <typename E>
+__global__ __launch_bounds__(256) void scan_dbc_kernel(ScanArgs p, int SP, int64_t per) {
+    const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (id >= p.B * p.N * p.G * 2 * SP) return;
+    const int64_t s = id % (2 * SP), bn = id / (2 * SP) % (p.B * p.N), g = id / (2 * SP) / (p.B * p.N);
+    float v = 0.0f;
+    for (int64_t k = 0; k < per; ++k) v += p.dbc[((g * per + k) * p.B * p.N + bn) * 2 * SP + s];
+    const int64_t col = s % SP;
+    if (col >= p.S) return;
+    E* out = (E*)(s < SP ? p.dB : p.dC);
+    out[(bn * p.G + g) * p.S + col] = from_f32<E>(v);
+}
+
+// dA [C, S], dD [C] and ddt_bias [C] from the column sums [C, SP + 2].
+__global__ __launch_bounds__(256) void scan_param_kernel(const float* sums, int64_t C, int S, int SP, float* dA,
+                                                         float* dD, float* dbias) {
+    const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (id >= C * (SP + 2)) return;
+    const int64_t c = id / (SP + 2), s = id % (SP + 2);
+    if (s < S) dA[c * S + s] = sums[id];
+    else if (s == SP && dD) dD[c] = sums[id];
+    else if (s == SP + 1 && dbias) dbias[c] = sums[id];
+}
+
+template <typename E, int SP>
+static int backward_go(const ScanArgs& p, hipStream_t stream) {
+    int rc;
+    if (p.NC > 1) {
+        const int64_t blocks = ceil_div(p.G * ceil_div(p.Cg, 64), 4);
+        scan_reverse_kernel<E, SP>
+            <<<dim3((unsigned)(p.NC - 1), (unsigned)blocks, (unsigned)p.B), 256, 0, stream>>>(p);
+        if ((rc = check_launch("scan_reverse")) != FLARE_OK) return rc;
+        scan_carries_kernel<<<dim3((unsigned)ceil_div(p.B * SP * p.C, 256)), 256, 0, stream>>>(p, SP);
+        if ((rc = check_launch("scan_carries")) != FLARE_OK) return rc;
+    }
+    using Lay = GradLayout<SP>;
+    const int64_t per = ceil_div(p.Cg, 16 * kWaves);
+    if (Lay::bytes > 65536) {
+        const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(&scan_gradient_kernel<E, SP>),
+                                                 hipFuncAttributeMaxDynamicSharedMemorySize, (int)Lay::bytes);
+        if (e != hipSuccess) {
+            set_error("scan_gradient: %s", hipGetErrorString(e));
+            return FLARE_ERR_LAUNCH;
+        }
+    }
+    scan_gradient_kernel<E, SP><<<dim3((unsigned)p.NC, (unsigned)(p.G * per), (unsigned)p.B), 64 * kWaves, Lay::bytes,
+                                  stream>>>(p);
+    if ((rc = check_launch("scan_gradient")) != FLARE_OK) return rc;
+    scan_dbc_kernel<E><<<dim3((unsigned)ceil_div(p.B * p.N * p.G * 2 * SP, 256)), 256, 0, stream>>>(p, SP, per);
+    return check_launch("scan_dbc");
+}
+template <typename E>
+static int backward_e(const ScanArgs& p, int64_t SP, hipStream_t stream) {
+    return SP == 8    ? backward_go<E, 8>(p, stream)
+           : SP == 16 ? backward_go<E, 16>(p, stream)
+           : SP == 32 ? backward_go<E, 32>(p, stream)
+                      : backward_go<E, 64>(p, stream);
+}
+
+struct BackwardLayout {
+    size_t bc, carry, dsum, cuts, dbc, dpar, sums, total;      // in floats
+    BackwardLayout(int64_t B, int64_t N, int64_t C, int64_t S, int64_t G, int64_t NC) {
+        const int64_t SP = padded_states(S), blocks = G * ceil_div(C / G, 16 * kWaves);
+        bc = 0;
+        carry = bc + B * N * G * 2 * SP;
+        dsum = carry + B * NC * SP * C;
+        cuts = dsum + B * NC * C;
+        dbc = cuts + B * NC;
+        dpar = dbc + blocks * B * N * 2 * SP;
+        sums = dpar + B * NC * C * (SP + 2);
+        total = sums + C * (SP + 2);
+    }
+};
+
+}  // namespace scan
+}  // namespace flare
+
+using namespace flare;
+using namespace flare::scan;
+
+extern "C" size_t flare_scan_backward_workspace_size(int64_t B, int64_t N, int64_t C, int64_t S, int64_t G,
+                                                     int64_t chunk) {
+    if (chunk < 1 || G < 1) return 0;
+    return BackwardLayout(B, N, C, S, G, ceil_div(N, chunk)).total * sizeof(float);
+}
+
+extern "C" int flare_scan_backward(const void* x, const void* dt, const float* A, const void* Bm, const void* Cm,
+                                   const float* D, const void* z, const float* dt_bias, int softplus, int dtype,
+                                   int64_t B, int64_t N, int64_t C, int64_t S, int64_t G, const int64_t* strides,
+                                   const int32_t* document_ids, const void* dy, int64_t chunk, const float* states,
+                                   void* dx, void* ddt, float* dA, void* dB, void* dC, float* dD, void* dz,
+                                   float* ddt_bias, void* workspace, size_t workspace_bytes, void* stream) {
+    FLARE_REQUIRE(x && dt && A && Bm && Cm && dy && strides && workspace && dx && ddt && dA && dB && dC,
+                  "flare_scan_backward: null pointer");
+    FLARE_REQUIRE(!z || dz, "flare_scan_backward: z without dz");
+    SCAN_REQUIRE_SIZES("flare_scan_backward");
+    const int64_t SP = padded_states(S);
+    FLARE_REQUIRE(chunk >= 1 && chunk <= backward_chunk_most(SP), "flare_scan_backward: chunks of 1 to %lld tokens",
+                  (long long)backward_chunk_most(SP));
+    ScanArgs p = scan_args(x, dt, A, Bm, Cm, D, z, dt_bias, softplus, B, N, C, S, G, strides);
+    p.L = chunk, p.NC = ceil_div(N, chunk);
+    FLARE_REQUIRE(p.NC == 1 || states, "flare_scan_backward: more than one chunk needs the forward's states");
+    const BackwardLayout lay(B, N, C, S, G, p.NC);
+    if (workspace_bytes < lay.total * sizeof(float)) {
+        set_error("flare_scan_backward: workspace of %zu bytes is too small", workspace_bytes);
+        return FLARE_ERR_WORKSPACE;
+    }
+    float* ws = (float*)workspace;
+    p.ids = document_ids, p.dy = dy, p.states = const_cast<float*>(states);
+    p.dx = dx, p.ddt = ddt, p.dB = dB, p.dC = dC, p.dz = dz;
+    p.bc = ws + lay.bc, p.carry = ws + lay.carry, p.dsum = ws + lay.dsum, p.cuts = (int32_t*)(ws + lay.cuts);
+    p.dbc = ws + lay.dbc, p.dpar = ws + lay.dpar;
+    hipStream_t st = (hipStream_t)stream;
+    int rc = launch_pack(p, dtype, SP, st);
+    if (rc == FLARE_OK) rc = FLARE_BY_DTYPE(dtype, backward_e, (p, SP, st));
+    if (rc == FLARE_OK) rc = mix::launch_column_sums(p.dpar, B * p.NC, C * (SP + 2), ws + lay.sums, st);
+    if (rc != FLARE_OK) return rc;
+    scan_param_kernel<<<dim3((unsigned)ceil_div(C * (SP + 2), 256)), 256, 0, st>>>(ws + lay.sums, C, (int)S, (int)SP, dA,
+                                                                                dD, ddt_bias);
+    return check_launch("scan_param");
+}

@@ -312,6 +312,121 @@ int flare_ar_forward_noalloc(const void* Q, const void* K, const void* V, const 
 int flare_device_faults(void* stream, uint32_t* count, int reset);
 int flare_set_meet_spin_limit(int limit);
 
+/*
+ * Token mixers a hybrid stack sets beside its FLARE layers (no counterpart in the reference):
+ * a short causal convolution, a selective state space scan and exact softmax attention.
+ *
+ * Tensors whose strides are arguments may be slices of wider ones: strides count elements, and
+ * the last dimension is adjacent.  All other tensors are contiguous.  `dtype` is the element type
+ * of every tensor given as (const) void*; float tensors are fp32 whatever it is.  Integers are
+ * int32.  Workspaces need no contents and hold nothing between calls.
+ *
+ * document_ids [B, N]: a token mixes with those of its own document only; ids below 0 are
+ * padding, with zero outputs and gradients.  lengths [B]: the tokens of each sequence that are
+ * real (outputs behind them are 0), or for attention those that its cache holds already.
+ */
+
+/*
+ * pre_t = bias + sum_{k < W} weight[c][W-1-k] x_{t-k};  y = pre, or pre sigmoid(pre) with `silu`.
+ * x [B, N, C], weight [C, W], bias [C] or NULL, W of 2 to 4, y [B, N, C].  window [B, W-1, C] (or
+ * NULL: zeros) holds the inputs before the first token, oldest first, and window_out (or NULL)
+ * receives those after the last one.  document_ids exclude lengths and windows.
+ */
+int flare_conv_forward(const void* x, int64_t x_stride_b, int64_t x_stride_n, const float* weight,
+                       const float* bias, int silu, int dtype, int64_t B, int64_t N, int64_t C, int64_t W,
+                       const int32_t* document_ids, const int32_t* lengths, const void* window, void* y,
+                       void* window_out, void* stream);
+
+/* Its gradients: dx [B, N, C], dweight [C, W], dbias [C] (or NULL), from dy [B, N, C]. */
+size_t flare_conv_backward_workspace_size(int64_t B, int64_t N, int64_t C, int64_t W);
+int flare_conv_backward(const void* x, int64_t x_stride_b, int64_t x_stride_n, const float* weight,
+                        const float* bias, int silu, int dtype, int64_t B, int64_t N, int64_t C, int64_t W,
+                        const int32_t* document_ids, const void* dy, void* dx, float* dweight, float* dbias,
+                        void* workspace, size_t workspace_bytes, void* stream);
+
+/* One token: x [B, C], y [B, C]; window [B, W-1, C] moves on in place.  mask [B] or NULL: a row of
+ * 0 keeps its window and gets y = 0. */
+int flare_conv_step(const void* x, int64_t x_stride_b, const float* weight, const float* bias, int silu,
+                    int dtype, int64_t B, int64_t C, int64_t W, const int32_t* mask, void* window, void* y,
+                    void* stream);
+
+/*
+ * delta = dt + dt_bias, or softplus of it;  h_t = exp(delta A) h_{t-1} + delta x B_t;
+ * y_t = (sum_s C_t h_t + D x_t) z sigmoid(z).  x, dt, z (or NULL) [B, N, C]; A [C, S]; Bm, Cm
+ * [B, N, G, S] (channel c reads group c / (C / G)); D, dt_bias [C] or NULL; 1 <= S <= 64.
+ * strides: batch and token of x, dt, z; batch, token and group of Bm, Cm (12 numbers, host).
+ * h0 (or NULL: zeros), h_fin (or NULL) [B, C, S].  The tokens run in chunks of `chunk`
+ * (flare_scan_chunk chooses; for_backward: short enough for flare_scan_backward); with more than
+ * one, `states` [B, ceil(N / chunk), SP, C] receives the state before each, SP being S rounded up
+ * to 8, 16, 32 or 64.  document_ids exclude lengths, h0 and h_fin.
+ */
+int64_t flare_scan_chunk(int64_t B, int64_t N, int64_t C, int64_t S, int64_t G, int for_backward);
+size_t flare_scan_forward_workspace_size(int64_t B, int64_t N, int64_t C, int64_t S, int64_t G, int64_t chunk);
+int flare_scan_forward(const void* x, const void* dt, const float* A, const void* Bm, const void* Cm,
+                       const float* D, const void* z, const float* dt_bias, int softplus, int dtype, int64_t B,
+                       int64_t N, int64_t C, int64_t S, int64_t G, const int64_t* strides,
+                       const int32_t* document_ids, const int32_t* lengths, const float* h0, void* y, float* h_fin,
+                       int64_t chunk, float* states, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Its gradients from h0 = 0, from dy [B, N, C] and the forward's states: dx, ddt, dz [B, N, C], dB,
+ * dC [B, N, G, S] in `dtype`; dA [C, S], dD, ddt_bias [C] (or NULL). */
+size_t flare_scan_backward_workspace_size(int64_t B, int64_t N, int64_t C, int64_t S, int64_t G, int64_t chunk);
+int flare_scan_backward(const void* x, const void* dt, const float* A, const void* Bm, const void* Cm,
+                        const float* D, const void* z, const float* dt_bias, int softplus, int dtype, int64_t B,
+                        int64_t N, int64_t C, int64_t S, int64_t G, const int64_t* strides,
+                        const int32_t* document_ids, const void* dy, int64_t chunk, const float* states, void* dx,
+                        void* ddt, float* dA, void* dB, void* dC, float* dD, void* dz, float* ddt_bias,
+                        void* workspace, size_t workspace_bytes, void* stream);
+
+/* One token (the token strides are not used): y [B, C]; state [B, C, S] moves on in place.  mask [B]
+ * or NULL: a row of 0 keeps its state and gets y = 0. */
+int flare_scan_step(const void* x, const void* dt, const float* A, const void* Bm, const void* Cm, const float* D,
+                    const void* z, const float* dt_bias, int softplus, int dtype, int64_t B, int64_t C, int64_t S,
+                    int64_t G, const int64_t* strides, const int32_t* mask, float* state, void* y, void* stream);
+
+/*
+ * y_i = sum_j softmax_j(s_ij) v_j, s_ij = x_ij - slopes[h] |i - j|, x_ij = scale q_i . k_j or (softcap
+ * > 0) softcap tanh(scale q_i . k_j / softcap).  q [B, N, H, D], k and v [B, M, G, D], head h reads
+ * key head h / (H / G); D a multiple of 16 up to 128; every row on a 16-byte boundary.  strides:
+ * batch, token and head of q, k, v (9 numbers, host).  causal: query i sees keys j <= i, and
+ * those below prefix_lengths[b] (or NULL).  Without `lengths` M == N.  With them k and v are
+ * caches of M rows, the queries are at positions lengths[b] + i, and new_lengths[b] of them (all
+ * if NULL) are real, whose keys are in the caches already (flare_attn_append); lengths[b] < 0: y =
+ * 0; lengths[b] + new_lengths[b] > M: y is NaN.  document_ids exclude lengths and need the
+ * workspace.  A query that sees nothing has y = 0.  lse [B, H, N] or NULL receives log2 of the sum
+ * of exp(s_ij).
+ */
+size_t flare_attn_forward_workspace_size(int64_t B, int64_t N);
+int flare_attn_forward(const void* q, const void* k, const void* v, const int64_t* strides, int dtype, int64_t B,
+                       int64_t N, int64_t M, int64_t H, int64_t G, int64_t D, float scale, float softcap,
+                       const float* slopes, int causal, const int32_t* document_ids,
+                       const int32_t* prefix_lengths, const int32_t* lengths, const int32_t* new_lengths, void* y,
+                       float* lse, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Its gradients without a cache, from y, lse and dy [B, N, H, D]: dq [B, N, H, D], dk, dv [B, N, G, D]. */
+size_t flare_attn_backward_workspace_size(int64_t B, int64_t N, int64_t H);
+int flare_attn_backward(const void* q, const void* k, const void* v, const int64_t* strides, int dtype, int64_t B,
+                        int64_t N, int64_t H, int64_t G, int64_t D, float scale, float softcap, const float* slopes,
+                        int causal, const int32_t* document_ids, const int32_t* prefix_lengths, const void* y,
+                        const float* lse, const void* dy, void* dq, void* dk, void* dv, void* workspace,
+                        size_t workspace_bytes, void* stream);
+
+/* Rows k, v [B, N, G, D] (strides: batch, token and head of k, v; 6 numbers, host) to positions
+ * lengths[b] + t of the caches [B, M, G, D], new_lengths[b] of them (all if NULL).  Nothing of a
+ * sequence of negative length or whose rows do not fit. */
+int flare_attn_append(const void* k, const void* v, const int64_t* strides, int dtype, int64_t B, int64_t N,
+                      int64_t M, int64_t G, int64_t D, const int32_t* lengths, const int32_t* new_lengths,
+                      void* k_cache, void* v_cache, void* stream);
+
+/* One token: q [B, H, D], k and v [B, G, D] (strides: batch and head of q, k, v; 6 numbers, host) at
+ * position lengths[b] of the caches [B, M, G, D], which receive k and v there; y [B, H, D].
+ * lengths[b] < 0: y = 0, nothing written; lengths[b] >= M: y is NaN, nothing written. */
+size_t flare_attn_step_workspace_size(int64_t B, int64_t M, int64_t H, int64_t G, int64_t D);
+int flare_attn_step(const void* q, const void* k, const void* v, const int64_t* strides, int dtype, int64_t B,
+                    int64_t M, int64_t H, int64_t G, int64_t D, float scale, float softcap, const float* slopes,
+                    const int32_t* lengths, void* k_cache, void* v_cache, void* y, void* workspace,
+                    size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
