@@ -21,9 +21,21 @@ inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 __device__ __forceinline__ float sigmoid(float x) { return __builtin_amdgcn_rcpf(1.0f + __expf(-x)); }
 
-// log(1 + e^x): the larger part exactly, the rest through log1p, so that the small steps of
-// x far below 0 keep their relative accuracy.
-__device__ __forceinline__ float softplus(float x) { return fmaxf(x, 0.0f) + log1pf(__expf(-fabsf(x))); }
+// log(1 + e^x): the larger part exactly, and log(1 + e) of e = e^-|x| <= 1 as 2 artanh(s), s = e /
+// (2 + e) <= 1/3, whose series keeps the relative accuracy of the small steps of x far below 0
+// (the first term left out, s^17 / 17, is below 2^-29 of the sum).  A third of the instructions
+// of log1pf, which were a fifth of the scan's backward.
+__device__ __forceinline__ float softplus(float x) {
+    const float e = __expf(-fabsf(x)), s = e * __builtin_amdgcn_rcpf(2.0f + e), q = s * s;
+    float p = 1.0f / 15.0f;
+    p = p * q + 1.0f / 13.0f;
+    p = p * q + 1.0f / 11.0f;
+    p = p * q + 1.0f / 9.0f;
+    p = p * q + 1.0f / 7.0f;
+    p = p * q + 1.0f / 5.0f;
+    p = p * q + 1.0f / 3.0f;
+    return fmaxf(x, 0.0f) + 2.0f * (s + s * (q * p));
+}
 
 // a of the lower and b of the upper 32 lanes, then the other halves (permlane32_swap); the same
 // for each 16 of 32 lanes (permlane16_swap).  What add(first, second) leaves is thus the sum

@@ -200,7 +200,7 @@ constexpr int kWaves = 8;              // 128 channels a workgroup
 template <int SP>
 struct GradLayout {
     static constexpr int SL = SP / 4;
-    static constexpr int T = SL <= 4 ? 16 : SL == 8 ? 8 : 4;
+    static constexpr int T = SL <= 4 ? 8 : 4;
     static constexpr int most = SP <= 16 ? 128 : SP == 32 ? 32 : 16;     // backward_chunk_most
     static constexpr int pieces = most / T;
     static constexpr int bc_floats = most * 2 * SP;
@@ -341,24 +341,25 @@ __global__ __launch_bounds__(64 * kWaves) void scan_gradient_kernel(ScanArgs p) 
             for (int i = 0; i < SL; ++i) h[i] = ah[j][i] + uj * row[i];
         };
         each_token(token, std::make_integer_sequence<int, T>{});
-        float pA[T], sB[T], lin[T];
+        // the tokens in reverse, and after each four of them what their lanes do with the sums
+        float pA[4], sB[4], lin[4];
         auto back = [&](auto jc) {
-            constexpr int j = T - 1 - decltype(jc)::value;
+            constexpr int j = T - 1 - decltype(jc)::value, jq = j & 3;
             const float* row = bcs + min(k0 + j, n - 1) * 2 * SP + q * SL;
-            const float dj = quad_bcast<(j & 3)>(delta[j / 4]), uj = quad_bcast<(j & 3)>(du[j / 4]);
-            const float gj = quad_bcast<(j & 3)>(gy[j / 4]);
+            const float dj = quad_bcast<jq>(delta[j / 4]), uj = quad_bcast<jq>(du[j / 4]);
+            const float gj = quad_bcast<jq>(gy[j / 4]);
             float v[2 * SL];
-            pA[j] = sB[j] = lin[j] = 0.0f;
+            pA[jq] = sB[jq] = lin[jq] = 0.0f;
 #pragma unroll
             for (int i = 0; i < SL; ++i) {
                 const float Bv = row[i], Cv = row[SP + i];
                 const float hv = ah[j][i] + uj * Bv;
                 r[i] += Cv * gj;
                 const float w = r[i] * ah[j][i];
-                pA[j] += w * A2[i];
+                pA[jq] += w * A2[i];
                 dA[i] += w * dj;
-                sB[j] += r[i] * Bv;
-                lin[j] += Cv * hv;
+                sB[jq] += r[i] * Bv;
+                lin[jq] += Cv * hv;
                 v[i] = r[i] * uj;
                 v[SL + i] = gj * hv;
                 r[i] *= a[j][i];
@@ -375,30 +376,27 @@ __global__ __launch_bounds__(64 * kWaves) void scan_gradient_kernel(ScanArgs p) 
                     out[idx < SL ? idx : SP + idx - SL] = v[m];
                 }
             }
-        };
-        each_token(back, std::make_integer_sequence<int, T>{});
-#pragma unroll
-        for (int i = 0; i < TQ; ++i) {
-            const float pa[4] = {pA[4 * i], pA[4 * i + 1], pA[4 * i + 2], pA[4 * i + 3]};
-            const float sb[4] = {sB[4 * i], sB[4 * i + 1], sB[4 * i + 2], sB[4 * i + 3]};
-            const float ln[4] = {lin[4 * i], lin[4 * i + 1], lin[4 * i + 2], lin[4 * i + 3]};
-            const float pq = quad_gather(pa, q) * kLn2, sq = quad_gather(sb, q), lq = quad_gather(ln, q);
-            const int k = k0 + 4 * i + q;
-            float ddt = pq + xv[i] * sq;
-            if (p.softplus) ddt *= mix::sigmoid(raw[i]);
-            if (!live[i]) ddt = 0.0f;
-            dbias += ddt;
-            dD += gy[i] * xv[i];
-            if (active && k < n) {
-                ((E*)p.dx)[row0 + k * p.C] = from_f32<E>(live[i] ? delta[i] * sq + gy[i] * skip : 0.0f);
-                ((E*)p.ddt)[row0 + k * p.C] = from_f32<E>(ddt);
-                if (z) {
-                    const float sg = mix::sigmoid(zv[i]);
-                    const float dz = dyv[i] * (lq + skip * xv[i]) * sg * (1.0f + zv[i] * (1.0f - sg));
-                    ((E*)p.dz)[row0 + k * p.C] = from_f32<E>(live[i] ? dz : 0.0f);
+            if constexpr (jq == 0) {
+                constexpr int i = j / 4;
+                const float pq = quad_gather(pA, q) * kLn2, sq = quad_gather(sB, q), lq = quad_gather(lin, q);
+                const int k = k0 + 4 * i + q;
+                float ddt = pq + xv[i] * sq;
+                if (p.softplus) ddt *= mix::sigmoid(raw[i]);
+                if (!live[i]) ddt = 0.0f;
+                dbias += ddt;
+                dD += gy[i] * xv[i];
+                if (active && k < n) {
+                    ((E*)p.dx)[row0 + k * p.C] = from_f32<E>(live[i] ? delta[i] * sq + gy[i] * skip : 0.0f);
+                    ((E*)p.ddt)[row0 + k * p.C] = from_f32<E>(ddt);
+                    if (z) {
+                        const float sg = mix::sigmoid(zv[i]);
+                        const float dz = dyv[i] * (lq + skip * xv[i]) * sg * (1.0f + zv[i] * (1.0f - sg));
+                        ((E*)p.dz)[row0 + k * p.C] = from_f32<E>(live[i] ? dz : 0.0f);
+                    }
                 }
             }
-        }
+        };
+        each_token(back, std::make_integer_sequence<int, T>{});
         // the piece's dB and dC: the waves' sums, in order
         __syncthreads();
         const int live_tokens = min(T, n - k0);
