@@ -50,6 +50,7 @@ HEADER_FUNCTIONS = (
     "flare_conv_backward",
     "flare_conv_step",
     "flare_scan_chunk",
+    "flare_scan_kept_tokens",
     "flare_scan_forward_workspace_size",
     "flare_scan_forward",
     "flare_scan_backward_workspace_size",
@@ -150,6 +151,8 @@ def _declare(lib):
     lib.flare_conv_step.argtypes = [_vp, _i64, _vp, _vp, _i, _i] + [_i64] * 3 + [_vp] * 4
     lib.flare_scan_chunk.restype = _i64
     lib.flare_scan_chunk.argtypes = [_i64] * 5 + [_i]
+    lib.flare_scan_kept_tokens.restype = _i64
+    lib.flare_scan_kept_tokens.argtypes = [_i64]
     lib.flare_scan_forward_workspace_size.restype = _sz
     lib.flare_scan_forward_workspace_size.argtypes = [_i64] * 6
     lib.flare_scan_forward.restype = _i

@@ -84,13 +84,15 @@ def _padded(S):
 
 def _run(x, dt, A, B, C, D, z, dt_bias, dt_softplus, sizes, training, document_ids=None, lengths=None, h0=None,
          h_fin=None):
-    """(y, the states before the chunks or None, the chunk length)."""
+    """(y, the states kept for the backward or None, the chunk length)."""
     nb, n, c, s, g = sizes
     t = _Inputs(x, dt, A, B, C, D, z, dt_bias)
     lib = _lib.lib()
     chunk = int(lib.flare_scan_chunk(nb, n, c, s, g, int(training)))
-    chunks = -(-n // chunk)
-    states = torch.empty((nb, chunks, _padded(s), c), device=x.device, dtype=torch.float32) if chunks > 1 else None
+    kept = None
+    if training:
+        kept = torch.empty((nb, -(-n // int(lib.flare_scan_kept_tokens(s))), _padded(s), c), device=x.device,
+                           dtype=torch.float32)
     nbytes = lib.flare_scan_forward_workspace_size(nb, n, c, s, g, chunk)
     ws = torch.empty(nbytes, device=x.device, dtype=torch.uint8)
     y = torch.empty((nb, n, c), device=x.device, dtype=t.dtype)
@@ -98,10 +100,10 @@ def _run(x, dt, A, B, C, D, z, dt_bias, dt_softplus, sizes, training, document_i
     P = _lib.ptr
     with _on(x.device):
         rc = lib.flare_scan_forward(*t.pointers(), int(bool(dt_softplus)), _lib.dtype_code(t.dtype), nb, n, c, s, g,
-                                    t.strides, P(ids), P(lens), P(h0), P(y), P(h_fin), chunk, P(states), P(ws),
+                                    t.strides, P(ids), P(lens), P(h0), P(y), P(h_fin), chunk, P(kept), P(ws),
                                     nbytes, _lib.stream_of(x.device))
     _lib.check(rc, "flare_scan_forward")
-    return y, states, chunk
+    return y, kept, chunk
 
 
 class StateSpaceScan(autograd.Function):
@@ -113,14 +115,14 @@ class StateSpaceScan(autograd.Function):
         if x.numel() == 0:
             ctx.save_for_backward(x, dt, A, B, C, D, z, dt_bias, document_ids, None)
             return torch.empty_like(x)
-        y, states, ctx.chunk = _run(x, dt, A, B, C, D, z, dt_bias, dt_softplus, sizes, training, document_ids)
-        ctx.save_for_backward(x, dt, A, B, C, D, z, dt_bias, document_ids, states if training else None)
+        y, kept, ctx.chunk = _run(x, dt, A, B, C, D, z, dt_bias, dt_softplus, sizes, training, document_ids)
+        ctx.save_for_backward(x, dt, A, B, C, D, z, dt_bias, document_ids, kept)
         return y.to(x.dtype)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        x, dt, A, B, C, D, z, dt_bias, document_ids, states = ctx.saved_tensors
+        x, dt, A, B, C, D, z, dt_bias, document_ids, kept = ctx.saved_tensors
         leaves = (x, dt, A, B, C, D, z, dt_bias)
         if x.numel() == 0:
             return tuple(None if t is None else torch.zeros_like(t) for t in leaves) + (None,) * 4
@@ -144,7 +146,7 @@ class StateSpaceScan(autograd.Function):
         P = _lib.ptr
         with _on(device):
             rc = lib.flare_scan_backward(*t.pointers(), int(bool(ctx.softplus)), _lib.dtype_code(t.dtype), nb, n, c, s,
-                                         g, t.strides, P(ids), P(gy), ctx.chunk, P(states), P(dx), P(ddt), P(dA),
+                                         g, t.strides, P(ids), P(gy), ctx.chunk, P(kept), P(dx), P(ddt), P(dA),
                                          P(dB), P(dC), P(dD), P(dz), P(dbias), P(ws), nbytes, _lib.stream_of(device))
         _lib.check(rc, "flare_scan_backward")
         grads = (dx, ddt, dA, dB.view(B.shape), dC.view(C.shape), dD, dz, dbias)

@@ -36,9 +36,12 @@ struct ScanArgs {
     void* y;
     // workspace
     float* bc;                          // [B, N, G, 2, SP]: B_t and C_t in fp32, zeros behind S
+    float* A2;                          // [SP, C]: A log2(e), zeros behind S
     float* states;                      // [B, NC, SP, C]: the state before each chunk
     float* dsum;                        // [B, NC, C]
     int32_t* cuts;                      // [B, NC]: whether a document begins within the chunk
+    float* kept;                        // [B, ceil(N / keep), SP, C]: the state before every keep-th token
+    int64_t keep;
     // backward
     const void* dy;
     void *dx, *ddt, *dz;
@@ -64,18 +67,18 @@ __device__ __forceinline__ scalar_f* scalar_ptr(const float* p) { return (scalar
 
 inline int64_t padded_states(int64_t S) { return S <= 8 ? 8 : S <= 16 ? 16 : S <= 32 ? 32 : 64; }
 
-// Chunk length: some four waves a SIMD (4096 on the card), in multiples of 16 tokens, and no
-// chunk so short that its states cost more than its tokens.  `most`: the longest chunk whose
-// start states the backward can walk from (0: any).
+// Chunk length: some four waves a SIMD (4096 on the card), in multiples of 32 tokens, and at most
+// `most` (0: any).
 inline int64_t chunk_length(int64_t B, int64_t N, int64_t C, int64_t G, int64_t most) {
     const int64_t waves = B * G * ceil_div(C / G, 64);
-    int64_t nc = ceil_div(4096, waves);
-    int64_t L = ceil_div(ceil_div(N, nc), 16) * 16;
-    L = L < 32 ? 32 : L;
+    const int64_t nc = ceil_div(4096, waves);
+    const int64_t L = ceil_div(ceil_div(N, nc), 32) * 32;
     return most && L > most ? most : L;
 }
-// The backward keeps a state every T tokens of a chunk in LDS (see flare_scan_bwd.hip).
-inline int64_t backward_chunk_most(int64_t SP) { return SP <= 16 ? 128 : SP == 32 ? 32 : 16; }
+// The backward holds B and C of a chunk in LDS, and recomputes its states from those the forward
+// kept: so far apart that what it keeps of a stretch itself stays small.
+constexpr int64_t kBackwardChunkMost = 128;
+constexpr int64_t kept_tokens(int64_t SP) { return SP <= 16 ? 32 : SP == 32 ? 16 : 8; }
 
 // strides: batch and token strides of x, dt, z; batch, token and group strides of B, C (elements).
 inline ScanArgs scan_args(const void* x, const void* dt, const float* A, const void* Bm, const void* Cm,
@@ -94,8 +97,11 @@ inline ScanArgs scan_args(const void* x, const void* dt, const float* A, const v
     FLARE_REQUIRE(B >= 1 && N >= 1 && C >= 1, name ": B, N and C must be positive");                          \
     FLARE_REQUIRE(S >= 1 && S <= 64, name ": 1 to 64 states a channel, got %lld", (long long)S);              \
     FLARE_REQUIRE(G >= 1 && C % G == 0, name ": the channels must divide into the groups of B and C");        \
-    FLARE_REQUIRE(B <= 65535 && C <= (1 << 20) && N <= INT32_MAX && B * N <= ((int64_t)1 << 36) / (128 * G),  \
+    FLARE_REQUIRE(B <= 65535 && C <= (1 << 20) && N <= (1 << 30) && B * N <= ((int64_t)1 << 36) / (128 * G),  \
                   name ": too large")
+
+// Waves a SIMD of the kernels whose lanes hold all SP states of a channel.
+constexpr int lane_waves(int SP) { return SP <= 16 ? 4 : SP == 32 ? 2 : 1; }
 
 int launch_pack(const ScanArgs& p, int dtype, int64_t SP, hipStream_t stream);
 int launch_states(const ScanArgs& p, int64_t SP, hipStream_t stream);

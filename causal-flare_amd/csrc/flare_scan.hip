@@ -26,10 +26,23 @@ __global__ __launch_bounds__(256) void scan_pack_kernel(ScanArgs p, int SP) {
     p.bc[id] = v;
 }
 
+// A in log2 units and the state before the first chunk, [SP, C] each, so that lanes of
+// neighbouring channels read neighbouring words.
+__global__ __launch_bounds__(256) void scan_lay_kernel(ScanArgs p, int SP) {
+    const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x, n = (int64_t)SP * p.C;
+    if (id >= n * (1 + p.B)) return;
+    const int64_t c = id % p.C, s = id / p.C % SP, b = id / n - 1;
+    if (b < 0) p.A2[id] = s < p.S ? p.A[c * p.S + s] * kLog2e : 0.0f;
+    else if (p.states) p.states[(b * p.NC * SP + s) * p.C + c] = p.h0 && s < p.S ? p.h0[(b * p.C + c) * p.S + s] : 0.0f;
+}
+
 template <typename E>
 static int pack_go(const ScanArgs& p, int64_t SP, hipStream_t stream) {
     scan_pack_kernel<E><<<dim3((unsigned)ceil_div(p.B * p.N * p.G * 2 * SP, 256)), 256, 0, stream>>>(p, (int)SP);
-    return check_launch("scan_pack");
+    const int rc = check_launch("scan_pack");
+    if (rc != FLARE_OK) return rc;
+    scan_lay_kernel<<<dim3((unsigned)ceil_div(SP * p.C * (1 + p.B), 256)), 256, 0, stream>>>(p, (int)SP);
+    return check_launch("scan_lay");
 }
 int launch_pack(const ScanArgs& p, int dtype, int64_t SP, hipStream_t stream) {
     return FLARE_BY_DTYPE(dtype, pack_go, (p, SP, stream));
@@ -38,108 +51,158 @@ int launch_pack(const ScanArgs& p, int dtype, int64_t SP, hipStream_t stream) {
 // One channel block of 64 (within a group) and one chunk a wave.  OUT false: leaves the chunk's
 // end state in the next chunk's slot of `states` and its sum of delta in `dsum`.
 template <typename E, int SP, bool OUT>
-__global__ __launch_bounds__(256) void scan_chunk_kernel(ScanArgs p) {
+__global__ __launch_bounds__(256, lane_waves(SP)) void scan_chunk_kernel(ScanArgs p) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int64_t per = (p.Cg + 63) / 64, cb = (int64_t)blockIdx.y * 4 + wave, b = blockIdx.z, chunk = blockIdx.x;
     if (cb >= p.G * per) return;
-    const int64_t g = cb / per, cl = cb % per * 64 + lane;
-    const bool active = cl < p.Cg;
-    const int64_t c = g * p.Cg + (active ? cl : p.Cg - 1);
-    const int64_t len = row_length(p, b);
-    const int64_t t0 = chunk * p.L, t1 = min(t0 + p.L, len), tn = min(t0 + p.L, p.N);
-    const E* x = (const E*)p.x + b * p.x_sb + c;
-    const E* dt = (const E*)p.dt + b * p.dt_sb + c;
-    const E* z = p.z ? (const E*)p.z + b * p.z_sb + c : nullptr;
-    E* y = (E*)p.y + (b * p.N) * p.C + c;
+    // Lanes behind the last channel do as that one does, and write what it writes.
+    const int64_t g = cb / per, cl = cb % per * 64 + lane, c = g * p.Cg + min(cl, p.Cg - 1);
+    const unsigned cu = (unsigned)c;               // the lane's part of every address
+    const int len = (int)row_length(p, b), L = (int)p.L;
+    const int t0 = (int)chunk * L, t1 = min(t0 + L, len), tn = min(t0 + L, (int)p.N);
+    const E* x = (const E*)p.x + b * p.x_sb;
+    const E* dt = (const E*)p.dt + b * p.dt_sb;
+    const E* z = p.z ? (const E*)p.z + b * p.z_sb : nullptr;
+    E* y = (E*)p.y + (b * p.N) * p.C;
     const int32_t* ids = p.ids ? p.ids + b * p.N : nullptr;
     scalar_f* bc = scalar_ptr(p.bc + ((b * p.N) * p.G + g) * 2 * SP);
-    const int64_t bc_step = p.G * 2 * SP;
+    const int bc_step = (int)p.G * 2 * SP;
 
     float h[SP], A2[SP];
 #pragma unroll
     for (int s = 0; s < SP; ++s) {
-        A2[s] = s < p.S ? p.A[c * p.S + s] * kLog2e : 0.0f;
-        h[s] = 0.0f;
-    }
-    if (OUT) {
-        if (p.NC > 1) {
-#pragma unroll
-            for (int s = 0; s < SP; ++s) h[s] = p.states[((b * p.NC + chunk) * SP + s) * p.C + c];
-        } else if (p.h0) {
-#pragma unroll
-            for (int s = 0; s < SP; ++s) h[s] = s < p.S ? p.h0[(b * p.C + c) * p.S + s] : 0.0f;
-        }
+        A2[s] = (p.A2 + s * p.C)[cu];
+        h[s] = OUT ? (p.states + ((b * p.NC + chunk) * SP + s) * p.C)[cu] : 0.0f;
     }
     const float bias = p.dt_bias ? p.dt_bias[c] : 0.0f;
     const float skip = OUT && p.D ? p.D[c] : 0.0f;
     float sum = 0.0f;
     bool cut = false;                              // a document begins within the chunk
 
-    constexpr int U = 4;
+    constexpr int U = 4, NB = SP < 16 ? SP : 16;
     E xr[U], dr[U], zr[U];
-    auto fetch = [&](int64_t t) {
+    auto fetch = [&](int t) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int64_t at = min(t + u, t1 - 1);
-            xr[u] = x[at * p.x_sn];
-            dr[u] = dt[at * p.dt_sn];
-            if (OUT && z) zr[u] = z[at * p.z_sn];
+            xr[u] = (x + at * p.x_sn)[cu];
+            dr[u] = (dt + at * p.dt_sn)[cu];
+            if (OUT && z) zr[u] = (z + at * p.z_sn)[cu];
         }
     };
-    if (t0 < t1) fetch(t0);
-    for (int64_t t4 = t0; t4 < t1; t4 += U) {
-        float xs[U], ds[U], zs[U];
+    auto step_of = [&](E raw) {
+        const float v = to_f32(raw) + bias;
+        return p.softplus ? mix::softplus(v) : v;
+    };
+    auto rows = [&](int t, int k, float (&B)[NB], float (&C)[NB]) {
+        scalar_f* row = bc + (int64_t)t * bc_step + k * NB;
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            xs[u] = to_f32(xr[u]);
-            ds[u] = to_f32(dr[u]) + bias;
-            if (p.softplus) ds[u] = mix::softplus(ds[u]);
-            zs[u] = OUT && z ? to_f32(zr[u]) : 0.0f;
+        for (int i = 0; i < NB; ++i) {
+            B[i] = row[i];
+            C[i] = OUT ? row[SP + i] : 0.0f;
         }
-        if (t4 + U < t1) fetch(t4 + U);
+    };
+    auto part = [&](float delta, float xv, int k, const float (&B)[NB], const float (&C)[NB], float (&out)[4]) {
+        const float du = delta * xv;
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int64_t t = t4 + u;
-            if (t >= t1) break;
-            if (ids) {
-                if (begins(ids, t)) {
+        for (int i = 0; i < NB; ++i) {
+            const int s = k * NB + i;
+            h[s] = __builtin_amdgcn_exp2f(delta * A2[s]) * h[s] + du * B[i];
+            if (OUT) out[i & 3] += C[i] * h[s];
+        }
+    };
+    auto keep = [&](int t) {
+        if (!OUT || !p.kept || (t & ((int)p.keep - 1))) return;
+        int64_t step = p.C;
+        asm volatile("" : "+s"(step));             // keeps the 16 addresses out of the loop's registers
+        float* to = p.kept + (b * ((p.N + p.keep - 1) / p.keep) + t / (int)p.keep) * SP * step;
+#pragma unroll
+        for (int s = 0; s < SP; ++s) (to + s * step)[cu] = h[s];
+    };
+    if (t0 < t1) fetch(t0);
+    for (int t4 = t0; t4 < t1; t4 += U) {
+        keep(t4);
+        // Four tokens of one document run without a branch between them.  The scalar loads of the
+        // next NB states are issued once those of the present ones are there.
+        bool plain = t4 + U <= t1;
+        if (ids && plain) {
+            const int id = ids[t4];
+            plain = id >= 0 && ids[t4 + 1] == id && ids[t4 + 2] == id && ids[t4 + 3] == id && !begins(ids, t4);
+        }
+        if (plain) {
+            float xs[U], ds[U], gate[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                xs[u] = to_f32(xr[u]);
+                ds[u] = step_of(dr[u]);
+                gate[u] = 1.0f;
+                if (OUT && z) {
+                    const float zv = to_f32(zr[u]);
+                    gate[u] = zv * mix::sigmoid(zv);
+                }
+            }
+            if (t4 + U < t1) fetch(t4 + U);
+            float Bv[2][NB], Cv[2][NB];
+            rows(t4, 0, Bv[0], Cv[0]);
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                float out[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int k = 0; k < SP / NB; ++k) {
+                    const int step = u * (SP / NB) + k, next = step + 1;
+                    asm volatile("" ::"s"(Bv[step & 1][0]));
+                    if (next < U * (SP / NB)) rows(t4 + next / (SP / NB), next % (SP / NB), Bv[next & 1], Cv[next & 1]);
+                    __builtin_amdgcn_sched_barrier(0);
+                    part(ds[u], xs[u], k, Bv[step & 1], Cv[step & 1], out);
+                }
+                sum += ds[u];
+                if (OUT) {
+                    const float o = (out[0] + out[1]) + (out[2] + out[3]) + skip * xs[u];
+                    (y + (int64_t)(t4 + u) * p.C)[cu] = from_f32<E>(o * gate[u]);
+                }
+            }
+        } else {
+#pragma unroll 1
+            for (int t = t4; t < min(t4 + U, t1); ++t) {
+                if (ids && begins(ids, t)) {
                     cut = true;
 #pragma unroll
                     for (int s = 0; s < SP; ++s) h[s] = 0.0f;
                 }
-                if (ids[t] < 0) {
-                    if (OUT && active) y[t * p.C] = from_f32<E>(0.0f);
-                    continue;
-                }
-            }
-            const float delta = ds[u], du = delta * xs[u];
-            sum += delta;
-            scalar_f* row = bc + t * bc_step;
-            float out[4] = {skip * xs[u], 0.0f, 0.0f, 0.0f};
+                float o = 0.0f;
+                if (!ids || ids[t] >= 0) {
+                    const float xv = to_f32((x + t * p.x_sn)[cu]), delta = step_of((dt + t * p.dt_sn)[cu]);
+                    float out[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-            for (int s = 0; s < SP; ++s) {
-                h[s] = __builtin_amdgcn_exp2f(delta * A2[s]) * h[s] + du * row[s];
-                if (OUT) out[s & 3] += row[SP + s] * h[s];
+                    for (int k = 0; k < SP / NB; ++k) {
+                        float Bv[NB], Cv[NB];
+                        rows(t, k, Bv, Cv);
+                        part(delta, xv, k, Bv, Cv, out);
+                    }
+                    sum += delta;
+                    o = (out[0] + out[1]) + (out[2] + out[3]) + skip * xv;
+                    if (OUT && z) {
+                        const float zv = to_f32((z + t * p.z_sn)[cu]);
+                        o *= zv * mix::sigmoid(zv);
+                    }
+                }
+                if (OUT) (y + (int64_t)t * p.C)[cu] = from_f32<E>(o);
             }
-            if (OUT) {
-                float o = (out[0] + out[1]) + (out[2] + out[3]);
-                if (z) o *= zs[u] * mix::sigmoid(zs[u]);
-                if (active) y[t * p.C] = from_f32<E>(o);
-            }
+            if (t4 + U < t1) fetch(t4 + U);
         }
     }
-    if (!active) return;
     if (OUT) {
-        for (int64_t t = max(t0, len); t < tn; ++t) y[t * p.C] = from_f32<E>(0.0f);
-        const int64_t last = len > 0 ? (len - 1) / p.L : 0;
+        for (int t = max(t0, len); t < tn; ++t) (y + (int64_t)t * p.C)[cu] = from_f32<E>(0.0f);
+        const int last = len > 0 ? (len - 1) / L : 0;
         if (p.h_fin && chunk == last) {
+            float* to = p.h_fin + (b * p.C + c) * p.S;
 #pragma unroll
             for (int s = 0; s < SP; ++s)
-                if (s < p.S) p.h_fin[(b * p.C + c) * p.S + s] = h[s];
+                if (s < p.S) to[s] = h[s];
         }
     } else {
 #pragma unroll
-        for (int s = 0; s < SP; ++s) p.states[((b * p.NC + chunk + 1) * SP + s) * p.C + c] = h[s];
+        for (int s = 0; s < SP; ++s) (p.states + ((b * p.NC + chunk + 1) * SP + s) * p.C)[cu] = h[s];
         p.dsum[(b * p.NC + chunk) * p.C + c] = sum;
         if (ids && c == 0) p.cuts[b * p.NC + chunk] = cut;
     }
@@ -151,12 +214,11 @@ __global__ __launch_bounds__(256) void scan_states_kernel(ScanArgs p, int SP) {
     const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
     if (id >= p.B * SP * p.C) return;
     const int64_t c = id % p.C, s = id / p.C % SP, b = id / p.C / SP;
-    const float A2 = s < p.S ? p.A[c * p.S + s] * kLog2e : 0.0f;
-    float h = p.h0 && s < p.S ? p.h0[(b * p.C + c) * p.S + s] : 0.0f;
+    const float A2 = p.A2[s * p.C + c];
     float* slot = p.states + ((b * p.NC) * SP + s) * p.C + c;
+    float h = slot[0];
     const int64_t step = SP * p.C;
     const float* dsum = p.dsum + (b * p.NC) * p.C + c;
-    slot[0] = h;
     constexpr int U = 8;
     for (int64_t k0 = 0; k0 + 1 < p.NC; k0 += U) {
         float own[U], dec[U];
@@ -301,39 +363,43 @@ using namespace flare::scan;
 
 extern "C" int64_t flare_scan_chunk(int64_t B, int64_t N, int64_t C, int64_t S, int64_t G, int for_backward) {
     if (B < 1 || N < 1 || C < 1 || S < 1 || S > 64 || G < 1 || C % G) return 0;
-    return chunk_length(B, N, C, G, for_backward ? backward_chunk_most(padded_states(S)) : 0);
+    return chunk_length(B, N, C, G, for_backward ? kBackwardChunkMost : 0);
 }
+extern "C" int64_t flare_scan_kept_tokens(int64_t S) { return S < 1 || S > 64 ? 0 : kept_tokens(padded_states(S)); }
 
 extern "C" size_t flare_scan_forward_workspace_size(int64_t B, int64_t N, int64_t C, int64_t S, int64_t G,
                                                     int64_t chunk) {
     if (chunk < 1) return 0;
     const int64_t SP = padded_states(S), NC = ceil_div(N, chunk);
-    return (size_t)(B * N * G * 2 * SP + B * NC * (C + 1)) * sizeof(float);
+    return (size_t)(B * N * G * 2 * SP + SP * C + B * NC * (C * (SP + 1) + 1)) * sizeof(float);
 }
 
 extern "C" int flare_scan_forward(const void* x, const void* dt, const float* A, const void* Bm, const void* Cm,
                                   const float* D, const void* z, const float* dt_bias, int softplus, int dtype,
                                   int64_t B, int64_t N, int64_t C, int64_t S, int64_t G, const int64_t* strides,
                                   const int32_t* document_ids, const int32_t* lengths, const float* h0, void* y,
-                                  float* h_fin, int64_t chunk, float* states, void* workspace,
+                                  float* h_fin, int64_t chunk, float* kept, void* workspace,
                                   size_t workspace_bytes, void* stream) {
     FLARE_REQUIRE(x && dt && A && Bm && Cm && y && strides && workspace, "flare_scan_forward: null pointer");
     FLARE_REQUIRE(!(document_ids && (lengths || h0 || h_fin)),
                   "flare_scan_forward: document_ids exclude lengths and states");
     FLARE_REQUIRE(!h_fin || h_fin != h0, "flare_scan_forward: the states overlap");
     SCAN_REQUIRE_SIZES("flare_scan_forward");
-    FLARE_REQUIRE(chunk >= 1, "flare_scan_forward: chunk must be positive");
+    FLARE_REQUIRE(chunk >= 1 && (!kept || chunk % kept_tokens(padded_states(S)) == 0),
+                  "flare_scan_forward: chunks must be positive, and multiples of the kept states' distance");
     ScanArgs p = scan_args(x, dt, A, Bm, Cm, D, z, dt_bias, softplus, B, N, C, S, G, strides);
     const int64_t SP = padded_states(S);
     p.L = chunk, p.NC = ceil_div(N, chunk);
-    FLARE_REQUIRE(p.NC == 1 || states, "flare_scan_forward: more than one chunk needs `states`");
     if (workspace_bytes < flare_scan_forward_workspace_size(B, N, C, S, G, chunk)) {
         set_error("flare_scan_forward: workspace of %zu bytes is too small", workspace_bytes);
         return FLARE_ERR_WORKSPACE;
     }
-    p.ids = document_ids, p.lengths = lengths, p.h0 = h0, p.y = y, p.h_fin = h_fin, p.states = states;
+    p.ids = document_ids, p.lengths = lengths, p.h0 = h0, p.y = y, p.h_fin = h_fin;
+    p.kept = kept, p.keep = kept_tokens(SP);
     p.bc = (float*)workspace;
-    p.dsum = p.bc + B * N * G * 2 * SP;
+    p.A2 = p.bc + B * N * G * 2 * SP;
+    p.states = p.A2 + SP * C;
+    p.dsum = p.states + B * p.NC * SP * C;
     p.cuts = (int32_t*)(p.dsum + B * p.NC * C);
     const int rc = launch_pack(p, dtype, SP, (hipStream_t)stream);
     if (rc != FLARE_OK) return rc;

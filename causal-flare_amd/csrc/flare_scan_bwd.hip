@@ -5,9 +5,9 @@
 //   dA += r a h_{t-1} delta_t       dB_t = sum_c r delta x      dC_t = sum_c dyg h_t
 //
 // scan_reverse leaves each chunk's r from behind as if nothing entered it; scan_carries joins
-// them; scan_gradient then walks each chunk twice: forward from its saved start state, keeping
-// a state every T tokens in LDS, and backward over these pieces of T tokens, each recomputed
-// with a_t and a_t h_{t-1} in registers.
+// them; scan_gradient then takes each chunk in stretches between the states that the forward
+// kept, the last one first: forward over a stretch, leaving a state every T tokens in LDS, and
+// backward over these pieces of T tokens, each recomputed with a_t and a_t h_{t-1} in registers.
 //
 // There four lanes share a channel (SL = S / 4 states each) and a wave has 16 channels: a piece
 // of T = 16 tokens then fits 128 registers at S = 16, where a lane with all the states of a
@@ -26,76 +26,118 @@ namespace scan {
 
 // Channel a lane, as scan_chunk: the gradient that leaves the chunk at its front.
 template <typename E, int SP>
-__global__ __launch_bounds__(256) void scan_reverse_kernel(ScanArgs p) {
+__global__ __launch_bounds__(256, lane_waves(SP)) void scan_reverse_kernel(ScanArgs p) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int64_t per = (p.Cg + 63) / 64, cb = (int64_t)blockIdx.y * 4 + wave, b = blockIdx.z;
     const int64_t chunk = (int64_t)blockIdx.x + 1;             // nothing is before chunk 0
     if (cb >= p.G * per) return;
-    const int64_t g = cb / per, cl = cb % per * 64 + lane;
-    const bool active = cl < p.Cg;
-    const int64_t c = g * p.Cg + (active ? cl : p.Cg - 1);
-    const int64_t t0 = chunk * p.L, t1 = min(t0 + p.L, p.N);
-    const E* dt = (const E*)p.dt + b * p.dt_sb + c;
-    const E* z = p.z ? (const E*)p.z + b * p.z_sb + c : nullptr;
-    const E* dy = (const E*)p.dy + (b * p.N) * p.C + c;
+    const int64_t g = cb / per, cl = cb % per * 64 + lane, c = g * p.Cg + min(cl, p.Cg - 1);
+    const unsigned cu = (unsigned)c;
+    const int t0 = (int)(chunk * p.L), t1 = (int)min((chunk + 1) * p.L, p.N);
+    const E* dt = (const E*)p.dt + b * p.dt_sb;
+    const E* z = p.z ? (const E*)p.z + b * p.z_sb : nullptr;
+    const E* dy = (const E*)p.dy + (b * p.N) * p.C;
     const int32_t* ids = p.ids ? p.ids + b * p.N : nullptr;
-    scalar_f* bc = scalar_ptr(p.bc + ((b * p.N) * p.G + g) * 2 * SP);
-    const int64_t bc_step = p.G * 2 * SP;
+    scalar_f* bc = scalar_ptr(p.bc + ((b * p.N) * p.G + g) * 2 * SP) + SP;
+    const int bc_step = (int)p.G * 2 * SP;
     float r[SP], A2[SP];
 #pragma unroll
     for (int s = 0; s < SP; ++s) {
-        A2[s] = s < p.S ? p.A[c * p.S + s] * kLog2e : 0.0f;
+        A2[s] = (p.A2 + s * p.C)[cu];
         r[s] = 0.0f;
     }
     const float bias = p.dt_bias ? p.dt_bias[c] : 0.0f;
     float sum = 0.0f;
     bool cut = false;
-    constexpr int U = 4;
+    constexpr int U = 4, NB = SP < 16 ? SP : 16;
     E gr[U], dr[U], zr[U];
-    auto fetch = [&](int64_t t) {
+    auto fetch = [&](int t) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int64_t at = max(t - u, t0);
-            gr[u] = dy[at * p.C];
-            dr[u] = dt[at * p.dt_sn];
-            if (z) zr[u] = z[at * p.z_sn];
+            gr[u] = (dy + at * p.C)[cu];
+            dr[u] = (dt + at * p.dt_sn)[cu];
+            if (z) zr[u] = (z + at * p.z_sn)[cu];
+        }
+    };
+    auto step_of = [&](E raw) {
+        const float v = to_f32(raw) + bias;
+        return p.softplus ? mix::softplus(v) : v;
+    };
+    auto rows = [&](int t, int k, float (&C)[NB]) {
+        scalar_f* row = bc + (int64_t)t * bc_step + k * NB;
+#pragma unroll
+        for (int i = 0; i < NB; ++i) C[i] = row[i];
+    };
+    auto part = [&](float delta, float gy, int k, const float (&C)[NB]) {
+#pragma unroll
+        for (int i = 0; i < NB; ++i) {
+            const int s = k * NB + i;
+            r[s] = __builtin_amdgcn_exp2f(delta * A2[s]) * (r[s] + gy * C[i]);
         }
     };
     fetch(t1 - 1);
-    for (int64_t t4 = t1 - 1; t4 >= t0; t4 -= U) {
-        float gs[U], ds[U];
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            gs[u] = to_f32(gr[u]);
-            ds[u] = to_f32(dr[u]) + bias;
-            if (p.softplus) ds[u] = mix::softplus(ds[u]);
-            if (z) {
-                const float zv = to_f32(zr[u]);
-                gs[u] *= zv * mix::sigmoid(zv);
-            }
+    for (int t4 = t1 - 1; t4 >= t0; t4 -= U) {
+        bool plain = t4 - U + 1 >= t0;             // as in scan_chunk
+        if (ids && plain) {
+            const int id = ids[t4];
+            plain = id >= 0 && ids[t4 - 1] == id && ids[t4 - 2] == id && ids[t4 - 3] == id && !begins(ids, t4 - 3);
         }
-        if (t4 - U >= t0) fetch(t4 - U);
+        if (plain) {
+            float gs[U], ds[U];
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int64_t t = t4 - u;
-            if (t < t0) break;
-            if (!ids || ids[t] >= 0) {
-                scalar_f* row = bc + t * bc_step + SP;
+            for (int u = 0; u < U; ++u) {
+                gs[u] = to_f32(gr[u]);
+                ds[u] = step_of(dr[u]);
+                if (z) {
+                    const float zv = to_f32(zr[u]);
+                    gs[u] *= zv * mix::sigmoid(zv);
+                }
+            }
+            if (t4 - U >= t0) fetch(t4 - U);
+            float Cv[2][NB];
+            rows(t4, 0, Cv[0]);
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+#pragma unroll
+                for (int k = 0; k < SP / NB; ++k) {
+                    const int step = u * (SP / NB) + k, next = step + 1;
+                    asm volatile("" ::"s"(Cv[step & 1][0]));
+                    if (next < U * (SP / NB)) rows(t4 - next / (SP / NB), next % (SP / NB), Cv[next & 1]);
+                    __builtin_amdgcn_sched_barrier(0);
+                    part(ds[u], gs[u], k, Cv[step & 1]);
+                }
                 sum += ds[u];
-#pragma unroll
-                for (int s = 0; s < SP; ++s)
-                    r[s] = __builtin_amdgcn_exp2f(ds[u] * A2[s]) * (r[s] + gs[u] * row[s]);
             }
-            if (ids && begins(ids, t)) {
-                cut = true;
+        } else {
+#pragma unroll 1
+            for (int t = t4; t >= max(t4 - U + 1, t0); --t) {
+                if (!ids || ids[t] >= 0) {
+                    const float delta = step_of((dt + t * p.dt_sn)[cu]);
+                    float gy = to_f32((dy + (int64_t)t * p.C)[cu]);
+                    if (z) {
+                        const float zv = to_f32((z + t * p.z_sn)[cu]);
+                        gy *= zv * mix::sigmoid(zv);
+                    }
 #pragma unroll
-                for (int s = 0; s < SP; ++s) r[s] = 0.0f;
+                    for (int k = 0; k < SP / NB; ++k) {
+                        float Cv[NB];
+                        rows(t, k, Cv);
+                        part(delta, gy, k, Cv);
+                    }
+                    sum += delta;
+                }
+                if (ids && begins(ids, t)) {
+                    cut = true;
+#pragma unroll
+                    for (int s = 0; s < SP; ++s) r[s] = 0.0f;
+                }
             }
+            if (t4 - U >= t0) fetch(t4 - U);
         }
     }
-    if (!active) return;
 #pragma unroll
-    for (int s = 0; s < SP; ++s) p.carry[((b * p.NC + chunk - 1) * SP + s) * p.C + c] = r[s];
+    for (int s = 0; s < SP; ++s) (p.carry + ((b * p.NC + chunk - 1) * SP + s) * p.C)[cu] = r[s];
     p.dsum[(b * p.NC + chunk) * p.C + c] = sum;
     if (ids && c == 0) p.cuts[b * p.NC + chunk] = cut;
 }
@@ -105,7 +147,7 @@ __global__ __launch_bounds__(256) void scan_carries_kernel(ScanArgs p, int SP) {
     const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
     if (id >= p.B * SP * p.C) return;
     const int64_t c = id % p.C, s = id / p.C % SP, b = id / p.C / SP;
-    const float A2 = s < p.S ? p.A[c * p.S + s] * kLog2e : 0.0f;
+    const float A2 = p.A2[s * p.C + c];
     float* slot = p.carry + ((b * p.NC) * SP + s) * p.C + c;
     const int64_t step = SP * p.C;
     const float* dsum = p.dsum + (b * p.NC) * p.C + c;
@@ -201,20 +243,32 @@ template <int SP>
 struct GradLayout {
     static constexpr int SL = SP / 4;
     static constexpr int T = SL <= 4 ? 8 : 4;
-    static constexpr int most = SP <= 16 ? 128 : SP == 32 ? 32 : 16;     // backward_chunk_most
-    static constexpr int pieces = most / T;
-    static constexpr int bc_floats = most * 2 * SP;
+    static constexpr int keep = (int)kept_tokens(SP), pieces = keep / T;
+    static constexpr int bc_floats = (int)kBackwardChunkMost * 2 * SP;
     static constexpr int keep_floats = kWaves * pieces * 64 * SL;
     static constexpr int red_floats = kWaves * T * 2 * SP;
     static constexpr size_t bytes = sizeof(float) * (bc_floats + keep_floats + red_floats);
     static_assert(bytes <= 160 * 1024, "LDS of a CU");
 };
 
+// SL adjacent floats of LDS, aligned to all of them (or 16 bytes).
+template <int SL>
+__device__ __forceinline__ void lds_row(const float* p, float (&out)[SL]) {
+    constexpr int V = SL < 4 ? SL : 4;
+    typedef float fv __attribute__((ext_vector_type(V)));
+#pragma unroll
+    for (int i = 0; i < SL; i += V) {
+        const fv v = *reinterpret_cast<const fv*>(p + i);
+#pragma unroll
+        for (int j = 0; j < V; ++j) out[i + j] = v[j];
+    }
+}
+
 template <typename E, int SP>
 __global__ __launch_bounds__(64 * kWaves) void scan_gradient_kernel(ScanArgs p) {
     using Lay = GradLayout<SP>;
-    constexpr int SL = Lay::SL, T = Lay::T, TQ = T / 4;
-    extern __shared__ float lds[];
+    constexpr int SL = Lay::SL, T = Lay::T, TQ = T / 4, KEEP = Lay::keep;
+    extern __shared__ __align__(16) float lds[];
     float* bcs = lds;                                      // [L][2][SP]
     float* keeps = bcs + Lay::bc_floats;                   // [waves][pieces][SL][64]
     float* red = keeps + Lay::keep_floats;                 // [waves][T][2 SP]
@@ -233,8 +287,9 @@ __global__ __launch_bounds__(64 * kWaves) void scan_gradient_kernel(ScanArgs p) 
     const int64_t row0 = (b * p.N + t0) * p.C + c;
     const E* dy = (const E*)p.dy + row0;
 
-    for (int i = tid; i < n * 2 * SP; i += 64 * kWaves)
-        bcs[i] = p.bc[((b * p.N + t0 + i / (2 * SP)) * p.G + g) * 2 * SP + i % (2 * SP)];
+    const int rows = (n + T - 1) / T * T;                  // tokens behind the last one have B = C = 0
+    for (int i = tid; i < rows * 2 * SP; i += 64 * kWaves)
+        bcs[i] = i < n * 2 * SP ? p.bc[((b * p.N + t0 + i / (2 * SP)) * p.G + g) * 2 * SP + i % (2 * SP)] : 0.0f;
     __syncthreads();
 
     float A2[SL], h[SL], r[SL], dA[SL];
@@ -242,172 +297,190 @@ __global__ __launch_bounds__(64 * kWaves) void scan_gradient_kernel(ScanArgs p) 
 #pragma unroll
     for (int i = 0; i < SL; ++i) {
         const int s = q * SL + i;
-        A2[i] = s < p.S ? p.A[c * p.S + s] * kLog2e : 0.0f;
-        h[i] = p.NC > 1 ? p.states[((b * p.NC + chunk) * SP + s) * p.C + c] : 0.0f;
+        A2[i] = p.A2[s * p.C + c];
         r[i] = p.NC > 1 ? p.carry[((b * p.NC + chunk) * SP + s) * p.C + c] : 0.0f;
         dA[i] = 0.0f;
     }
+    const float* kept = p.kept + ((b * ((p.N + KEEP - 1) / KEEP) + t0 / KEEP) * SP + q * SL) * p.C + c;
     const float bias = p.dt_bias ? p.dt_bias[c] : 0.0f, skip = p.D ? p.D[c] : 0.0f;
     float dD = 0.0f, dbias = 0.0f;
 
-    // the tokens 4 i + q of the piece at k0; a token that is none has delta = x = 0
-    auto step_of = [&](int k, float& raw, float& delta, float& xv) {
-        raw = delta = xv = 0.0f;
-        const bool live = active && k < n && (!ids || ids[k] >= 0);
-        if (live) {
-            raw = to_f32(dt[k * p.dt_sn]) + bias;
-            delta = p.softplus ? mix::softplus(raw) : raw;
-            xv = to_f32(x[k * p.x_sn]);
+    // The tokens 4 i + q of the piece at k0, as loaded: rows that are none load the last one's.
+    struct Raw {
+        E dt[TQ], x[TQ], dy[TQ], z[TQ];
+        int id[TQ];
+    };
+    auto fetch = [&](Raw& r, int k0, bool all) {
+#pragma unroll
+        for (int i = 0; i < TQ; ++i) {
+            const int k = min(max(k0, 0) + 4 * i + q, n - 1);
+            r.dt[i] = dt[k * p.dt_sn];
+            r.x[i] = x[k * p.x_sn];
+            if (all) r.dy[i] = dy[k * p.C];
+            if (all && z) r.z[i] = z[k * p.z_sn];
+            r.id[i] = ids ? ids[k] : 0;
         }
+    };
+    // a token that is none has delta = x = 0
+    auto step_of = [&](const Raw& r, int i, int k, float& raw, float& delta, float& xv) {
+        const bool live = active && k < n && r.id[i] >= 0;
+        raw = live ? to_f32(r.dt[i]) + bias : 0.0f;
+        delta = live ? (p.softplus ? mix::softplus(raw) : raw) : 0.0f;
+        xv = live ? to_f32(r.x[i]) : 0.0f;
         return live;
     };
     auto piece_begins = [&](int k0) {      // bit j: a document begins at token k0 + j
-        unsigned m = 0;
-        if (ids) {
+        if (!ids) return 0u;
+        const int k = k0 + (lane & (T - 1));
+        return (unsigned)__ballot(lane < T && k < n && t0 + k > 0 && ids[k] != ids[k - 1]);
+    };
+    // h over the piece at k0; `take`(j, i, a, a h) sees each decay and what it leaves.  CUT: a
+    // document begins in it.
+    auto forward = [&](auto cutc, int k0, unsigned starts, const float (&delta)[TQ], const float (&du)[TQ], auto&& take) {
+        constexpr bool CUT = decltype(cutc)::value;
+        auto token = [&](auto jc) {
+            constexpr int j = decltype(jc)::value;
+            float B[SL];
+            lds_row<SL>(bcs + (k0 + j) * 2 * SP + q * SL, B);
+            const float dj = quad_bcast<(j & 3)>(delta[j / 4]), uj = quad_bcast<(j & 3)>(du[j / 4]);
+            const bool cut = CUT && (starts >> j & 1);
 #pragma unroll
-            for (int j = 0; j < T; ++j) {
-                const int k = k0 + j;
-                if (k < n && t0 + k > 0 && ids[k] != ids[k - 1]) m |= 1u << j;
+            for (int i = 0; i < SL; ++i) {
+                float a = __builtin_amdgcn_exp2f(dj * A2[i]), ah = a * h[i];
+                if (cut) a = ah = 0.0f;
+                take(jc, i, a, ah);
+                h[i] = ah + uj * B[i];
             }
-        }
-        return m;
+        };
+        each_token(token, std::make_integer_sequence<int, T>{});
     };
 
-    // forward over the chunk, keeping the state before each piece
-    const int pieces = (n + T - 1) / T;
-    for (int piece = 0; piece < pieces; ++piece) {
+    for (int first = (n - 1) / KEEP * KEEP; first >= 0; first -= KEEP) {
+        const int here = min(KEEP, n - first), pieces = (here + T - 1) / T;
 #pragma unroll
-        for (int i = 0; i < SL; ++i) keep[(piece * SL + i) * 64] = h[i];
-        if (piece + 1 == pieces) break;
-        const int k0 = piece * T;
-        const unsigned starts = piece_begins(k0);
-        float delta[TQ], du[TQ];
+        for (int i = 0; i < SL; ++i) h[i] = kept[(int64_t)(first / KEEP) * SP * p.C + i * p.C];
+        // forward, keeping the state before each piece
+        Raw raws[Lay::pieces - 1];
 #pragma unroll
-        for (int i = 0; i < TQ; ++i) {
-            float raw, xv;
-            step_of(k0 + 4 * i + q, raw, delta[i], xv);
-            du[i] = delta[i] * xv;
-        }
-        auto token = [&](auto jc) {
-            constexpr int j = decltype(jc)::value;
-            const float* row = bcs + (k0 + j) * 2 * SP + q * SL;
-            const float dj = quad_bcast<(j & 3)>(delta[j / 4]), uj = quad_bcast<(j & 3)>(du[j / 4]);
-            if (starts >> j & 1) {
+        for (int piece = 0; piece + 1 < Lay::pieces; ++piece)
+            if (piece + 1 < pieces) fetch(raws[piece], first + piece * T, false);
+        Raw next;
+        fetch(next, first + (pieces - 1) * T, true);
 #pragma unroll
-                for (int i = 0; i < SL; ++i) h[i] = 0.0f;
+        for (int i = 0; i < SL; ++i) keep[i * 64] = h[i];
+#pragma unroll
+        for (int piece = 0; piece + 1 < Lay::pieces; ++piece) {
+            if (piece + 1 >= pieces) break;
+            const int k0 = first + piece * T;
+            float delta[TQ], du[TQ];
+#pragma unroll
+            for (int i = 0; i < TQ; ++i) {
+                float raw, xv;
+                step_of(raws[piece], i, k0 + 4 * i + q, raw, delta[i], xv);
+                du[i] = delta[i] * xv;
             }
+            const unsigned starts = piece_begins(k0);
+            auto nothing = [](auto, int, float, float) {};
+            if (starts) forward(std::true_type{}, k0, starts, delta, du, nothing);
+            else forward(std::false_type{}, k0, 0u, delta, du, nothing);
 #pragma unroll
-            for (int i = 0; i < SL; ++i) h[i] = __builtin_amdgcn_exp2f(dj * A2[i]) * h[i] + uj * row[i];
-        };
-        each_token(token, std::make_integer_sequence<int, T>{});
-    }
+            for (int i = 0; i < SL; ++i) keep[((piece + 1) * SL + i) * 64] = h[i];
+        }
 
-    // backward over the pieces
-    for (int piece = pieces - 1; piece >= 0; --piece) {
-        const int k0 = piece * T;
-        const unsigned starts = piece_begins(k0);
-        float raw[TQ], delta[TQ], xv[TQ], du[TQ], gy[TQ], dyv[TQ], zv[TQ];
-        bool live[TQ];
+        // backward over the pieces
+        for (int piece = pieces - 1; piece >= 0; --piece) {
+            const int k0 = first + piece * T;
+            const Raw now = next;
+            fetch(next, k0 - T, true);
+            float raw[TQ], delta[TQ], xv[TQ], du[TQ], gy[TQ], dyv[TQ], zv[TQ];
+            bool live[TQ];
 #pragma unroll
-        for (int i = 0; i < TQ; ++i) {
-            const int k = k0 + 4 * i + q;
-            live[i] = step_of(k, raw[i], delta[i], xv[i]);
-            du[i] = delta[i] * xv[i];
-            dyv[i] = zv[i] = 0.0f;
-            if (live[i]) {
-                dyv[i] = to_f32(dy[k * p.C]);
-                if (z) zv[i] = to_f32(z[k * p.z_sn]);
+            for (int i = 0; i < TQ; ++i) {
+                live[i] = step_of(now, i, k0 + 4 * i + q, raw[i], delta[i], xv[i]);
+                du[i] = delta[i] * xv[i];
+                dyv[i] = live[i] ? to_f32(now.dy[i]) : 0.0f;
+                zv[i] = live[i] && z ? to_f32(now.z[i]) : 0.0f;
+                gy[i] = z ? dyv[i] * zv[i] * mix::sigmoid(zv[i]) : dyv[i];
             }
-            gy[i] = z ? dyv[i] * zv[i] * mix::sigmoid(zv[i]) : dyv[i];
-        }
-        float a[T][SL], ah[T][SL];
+            float a[T][SL], ah[T][SL];
 #pragma unroll
-        for (int i = 0; i < SL; ++i) h[i] = keep[(piece * SL + i) * 64];
-        auto token = [&](auto jc) {
-            constexpr int j = decltype(jc)::value;
-            const float* row = bcs + min(k0 + j, n - 1) * 2 * SP + q * SL;
-            const float dj = quad_bcast<(j & 3)>(delta[j / 4]), uj = quad_bcast<(j & 3)>(du[j / 4]);
-            const bool cut = starts >> j & 1;
+            for (int i = 0; i < SL; ++i) h[i] = keep[(piece * SL + i) * 64];
+            const unsigned starts = piece_begins(k0);
+            auto hold = [&](auto jc, int i, float av, float ahv) {
+                a[decltype(jc)::value][i] = av;
+                ah[decltype(jc)::value][i] = ahv;
+            };
+            if (starts) forward(std::true_type{}, k0, starts, delta, du, hold);
+            else forward(std::false_type{}, k0, 0u, delta, du, hold);
+            // the tokens in reverse, and after each four of them what their lanes do with the sums
+            float pA[4], sB[4], lin[4];
+            auto back = [&](auto jc) {
+                constexpr int j = T - 1 - decltype(jc)::value, jq = j & 3;
+                const float* row = bcs + (k0 + j) * 2 * SP + q * SL;
+                const float dj = quad_bcast<jq>(delta[j / 4]), uj = quad_bcast<jq>(du[j / 4]);
+                const float gj = quad_bcast<jq>(gy[j / 4]);
+                float v[2 * SL], B[SL], Cv[SL];
+                lds_row<SL>(row, B);
+                lds_row<SL>(row + SP, Cv);
+                pA[jq] = sB[jq] = lin[jq] = 0.0f;
 #pragma unroll
-            for (int i = 0; i < SL; ++i) {
-                a[j][i] = __builtin_amdgcn_exp2f(dj * A2[i]);
-                ah[j][i] = a[j][i] * h[i];
-            }
-            if (cut) {
-#pragma unroll
-                for (int i = 0; i < SL; ++i) a[j][i] = ah[j][i] = 0.0f;
-            }
-#pragma unroll
-            for (int i = 0; i < SL; ++i) h[i] = ah[j][i] + uj * row[i];
-        };
-        each_token(token, std::make_integer_sequence<int, T>{});
-        // the tokens in reverse, and after each four of them what their lanes do with the sums
-        float pA[4], sB[4], lin[4];
-        auto back = [&](auto jc) {
-            constexpr int j = T - 1 - decltype(jc)::value, jq = j & 3;
-            const float* row = bcs + min(k0 + j, n - 1) * 2 * SP + q * SL;
-            const float dj = quad_bcast<jq>(delta[j / 4]), uj = quad_bcast<jq>(du[j / 4]);
-            const float gj = quad_bcast<jq>(gy[j / 4]);
-            float v[2 * SL];
-            pA[jq] = sB[jq] = lin[jq] = 0.0f;
-#pragma unroll
-            for (int i = 0; i < SL; ++i) {
-                const float Bv = row[i], Cv = row[SP + i];
-                const float hv = ah[j][i] + uj * Bv;
-                r[i] += Cv * gj;
-                const float w = r[i] * ah[j][i];
-                pA[jq] += w * A2[i];
-                dA[i] += w * dj;
-                sB[jq] += r[i] * Bv;
-                lin[jq] += Cv * hv;
-                v[i] = r[i] * uj;
-                v[SL + i] = gj * hv;
-                r[i] *= a[j][i];
-            }
-            int first;
-            bool own;
-            sum_channels(v, lane, first, own);
-            if (own) {
-                constexpr int NK = SL >= 8 ? SL / 8 : 1;
-                float* out = red + (wave * T + j) * 2 * SP + q * SL;
-#pragma unroll
-                for (int m = 0; m < NK; ++m) {
-                    const int idx = first + m;           // state idx of B, or idx - SL of C
-                    out[idx < SL ? idx : SP + idx - SL] = v[m];
+                for (int i = 0; i < SL; ++i) {
+                    const float hv = ah[j][i] + uj * B[i];
+                    r[i] += Cv[i] * gj;
+                    const float w = r[i] * ah[j][i];
+                    pA[jq] += w * A2[i];
+                    dA[i] += w * dj;
+                    sB[jq] += r[i] * B[i];
+                    lin[jq] += Cv[i] * hv;
+                    v[i] = r[i] * uj;
+                    v[SL + i] = gj * hv;
+                    r[i] *= a[j][i];
                 }
-            }
-            if constexpr (jq == 0) {
-                constexpr int i = j / 4;
-                const float pq = quad_gather(pA, q) * kLn2, sq = quad_gather(sB, q), lq = quad_gather(lin, q);
-                const int k = k0 + 4 * i + q;
-                float ddt = pq + xv[i] * sq;
-                if (p.softplus) ddt *= mix::sigmoid(raw[i]);
-                if (!live[i]) ddt = 0.0f;
-                dbias += ddt;
-                dD += gy[i] * xv[i];
-                if (active && k < n) {
-                    ((E*)p.dx)[row0 + k * p.C] = from_f32<E>(live[i] ? delta[i] * sq + gy[i] * skip : 0.0f);
-                    ((E*)p.ddt)[row0 + k * p.C] = from_f32<E>(ddt);
-                    if (z) {
-                        const float sg = mix::sigmoid(zv[i]);
-                        const float dz = dyv[i] * (lq + skip * xv[i]) * sg * (1.0f + zv[i] * (1.0f - sg));
-                        ((E*)p.dz)[row0 + k * p.C] = from_f32<E>(live[i] ? dz : 0.0f);
+                int at;
+                bool own;
+                sum_channels(v, lane, at, own);
+                if (own) {
+                    constexpr int NK = SL >= 8 ? SL / 8 : 1;
+                    float* out = red + (wave * T + j) * 2 * SP + q * SL;
+#pragma unroll
+                    for (int m = 0; m < NK; ++m) {
+                        const int idx = at + m;              // state idx of B, or idx - SL of C
+                        out[idx < SL ? idx : SP + idx - SL] = v[m];
                     }
                 }
-            }
-        };
-        each_token(back, std::make_integer_sequence<int, T>{});
-        // the piece's dB and dC: the waves' sums, in order
-        __syncthreads();
-        const int live_tokens = min(T, n - k0);
-        float* out = p.dbc + ((cb * p.B + b) * p.N + t0 + k0) * 2 * SP;
-        for (int i = tid; i < live_tokens * 2 * SP; i += 64 * kWaves) {
-            float s = 0.0f;
+                if constexpr (jq == 0) {
+                    constexpr int i = j / 4;
+                    const float pq = quad_gather(pA, q) * kLn2, sq = quad_gather(sB, q), lq = quad_gather(lin, q);
+                    const int k = k0 + 4 * i + q;
+                    float ddt = pq + xv[i] * sq;
+                    if (p.softplus) ddt *= mix::sigmoid(raw[i]);
+                    if (!live[i]) ddt = 0.0f;
+                    dbias += ddt;
+                    dD += gy[i] * xv[i];
+                    if (active && k < n) {
+                        ((E*)p.dx)[row0 + k * p.C] = from_f32<E>(live[i] ? delta[i] * sq + gy[i] * skip : 0.0f);
+                        ((E*)p.ddt)[row0 + k * p.C] = from_f32<E>(ddt);
+                        if (z) {
+                            const float sg = mix::sigmoid(zv[i]);
+                            const float dz = dyv[i] * (lq + skip * xv[i]) * sg * (1.0f + zv[i] * (1.0f - sg));
+                            ((E*)p.dz)[row0 + k * p.C] = from_f32<E>(live[i] ? dz : 0.0f);
+                        }
+                    }
+                }
+            };
+            each_token(back, std::make_integer_sequence<int, T>{});
+            // the piece's dB and dC: the waves' sums, in order
+            __syncthreads();
+            const int live_tokens = min(T, n - k0);
+            float* out = p.dbc + ((cb * p.B + b) * p.N + t0 + k0) * 2 * SP;
+            for (int i = tid; i < live_tokens * 2 * SP; i += 64 * kWaves) {
+                float s = 0.0f;
 #pragma unroll
-            for (int w = 0; w < kWaves; ++w) s += red[w * T * 2 * SP + i];
-            out[i] = s;
+                for (int w = 0; w < kWaves; ++w) s += red[w * T * 2 * SP + i];
+                out[i] = s;
+            }
+            __syncthreads();
         }
-        __syncthreads();
     }
     if (!active) return;
     float* par = p.dpar + ((b * p.NC + chunk) * p.C + c) * (SP + 2);
@@ -479,11 +552,12 @@ static int backward_e(const ScanArgs& p, int64_t SP, hipStream_t stream) {
 }
 
 struct BackwardLayout {
-    size_t bc, carry, dsum, cuts, dbc, dpar, sums, total;      // in floats
+    size_t bc, A2, carry, dsum, cuts, dbc, dpar, sums, total;      // in floats
     BackwardLayout(int64_t B, int64_t N, int64_t C, int64_t S, int64_t G, int64_t NC) {
         const int64_t SP = padded_states(S), blocks = G * ceil_div(C / G, 16 * kWaves);
         bc = 0;
-        carry = bc + B * N * G * 2 * SP;
+        A2 = bc + B * N * G * 2 * SP;
+        carry = A2 + SP * C;
         dsum = carry + B * NC * SP * C;
         cuts = dsum + B * NC * C;
         dbc = cuts + B * NC;
@@ -508,28 +582,28 @@ extern "C" size_t flare_scan_backward_workspace_size(int64_t B, int64_t N, int64
 extern "C" int flare_scan_backward(const void* x, const void* dt, const float* A, const void* Bm, const void* Cm,
                                    const float* D, const void* z, const float* dt_bias, int softplus, int dtype,
                                    int64_t B, int64_t N, int64_t C, int64_t S, int64_t G, const int64_t* strides,
-                                   const int32_t* document_ids, const void* dy, int64_t chunk, const float* states,
+                                   const int32_t* document_ids, const void* dy, int64_t chunk, const float* kept,
                                    void* dx, void* ddt, float* dA, void* dB, void* dC, float* dD, void* dz,
                                    float* ddt_bias, void* workspace, size_t workspace_bytes, void* stream) {
-    FLARE_REQUIRE(x && dt && A && Bm && Cm && dy && strides && workspace && dx && ddt && dA && dB && dC,
+    FLARE_REQUIRE(x && dt && A && Bm && Cm && dy && kept && strides && workspace && dx && ddt && dA && dB && dC,
                   "flare_scan_backward: null pointer");
     FLARE_REQUIRE(!z || dz, "flare_scan_backward: z without dz");
     SCAN_REQUIRE_SIZES("flare_scan_backward");
     const int64_t SP = padded_states(S);
-    FLARE_REQUIRE(chunk >= 1 && chunk <= backward_chunk_most(SP), "flare_scan_backward: chunks of 1 to %lld tokens",
-                  (long long)backward_chunk_most(SP));
+    FLARE_REQUIRE(chunk >= 1 && chunk <= kBackwardChunkMost && chunk % kept_tokens(SP) == 0,
+                  "flare_scan_backward: chunks of up to %lld tokens, multiples of the kept states' distance",
+                  (long long)kBackwardChunkMost);
     ScanArgs p = scan_args(x, dt, A, Bm, Cm, D, z, dt_bias, softplus, B, N, C, S, G, strides);
     p.L = chunk, p.NC = ceil_div(N, chunk);
-    FLARE_REQUIRE(p.NC == 1 || states, "flare_scan_backward: more than one chunk needs the forward's states");
     const BackwardLayout lay(B, N, C, S, G, p.NC);
     if (workspace_bytes < lay.total * sizeof(float)) {
         set_error("flare_scan_backward: workspace of %zu bytes is too small", workspace_bytes);
         return FLARE_ERR_WORKSPACE;
     }
     float* ws = (float*)workspace;
-    p.ids = document_ids, p.dy = dy, p.states = const_cast<float*>(states);
+    p.ids = document_ids, p.dy = dy, p.kept = const_cast<float*>(kept), p.keep = kept_tokens(SP);
     p.dx = dx, p.ddt = ddt, p.dB = dB, p.dC = dC, p.dz = dz;
-    p.bc = ws + lay.bc, p.carry = ws + lay.carry, p.dsum = ws + lay.dsum, p.cuts = (int32_t*)(ws + lay.cuts);
+    p.bc = ws + lay.bc, p.A2 = ws + lay.A2, p.carry = ws + lay.carry, p.dsum = ws + lay.dsum, p.cuts = (int32_t*)(ws + lay.cuts);
     p.dbc = ws + lay.dbc, p.dpar = ws + lay.dpar;
     hipStream_t st = (hipStream_t)stream;
     int rc = launch_pack(p, dtype, SP, st);

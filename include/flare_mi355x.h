@@ -356,25 +356,27 @@ int flare_conv_step(const void* x, int64_t x_stride_b, const float* weight, cons
  * [B, N, G, S] (channel c reads group c / (C / G)); D, dt_bias [C] or NULL; 1 <= S <= 64.
  * strides: batch and token of x, dt, z; batch, token and group of Bm, Cm (12 numbers, host).
  * h0 (or NULL: zeros), h_fin (or NULL) [B, C, S].  The tokens run in chunks of `chunk`
- * (flare_scan_chunk chooses; for_backward: short enough for flare_scan_backward); with more than
- * one, `states` [B, ceil(N / chunk), SP, C] receives the state before each, SP being S rounded up
- * to 8, 16, 32 or 64.  document_ids exclude lengths, h0 and h_fin.
+ * (flare_scan_chunk chooses; for_backward: as flare_scan_backward takes them).  kept (or NULL) [B,
+ * ceil(N / T), SP, C] receives the state before every T-th token for the backward, T being
+ * flare_scan_kept_tokens(S) and SP S rounded up to 8, 16, 32 or 64.  document_ids exclude lengths,
+ * h0 and h_fin.
  */
 int64_t flare_scan_chunk(int64_t B, int64_t N, int64_t C, int64_t S, int64_t G, int for_backward);
+int64_t flare_scan_kept_tokens(int64_t S);
 size_t flare_scan_forward_workspace_size(int64_t B, int64_t N, int64_t C, int64_t S, int64_t G, int64_t chunk);
 int flare_scan_forward(const void* x, const void* dt, const float* A, const void* Bm, const void* Cm,
                        const float* D, const void* z, const float* dt_bias, int softplus, int dtype, int64_t B,
                        int64_t N, int64_t C, int64_t S, int64_t G, const int64_t* strides,
                        const int32_t* document_ids, const int32_t* lengths, const float* h0, void* y, float* h_fin,
-                       int64_t chunk, float* states, void* workspace, size_t workspace_bytes, void* stream);
+                       int64_t chunk, float* kept, void* workspace, size_t workspace_bytes, void* stream);
 
-/* Its gradients from h0 = 0, from dy [B, N, C] and the forward's states: dx, ddt, dz [B, N, C], dB,
+/* Its gradients from h0 = 0, from dy [B, N, C] and what the forward kept: dx, ddt, dz [B, N, C], dB,
  * dC [B, N, G, S] in `dtype`; dA [C, S], dD, ddt_bias [C] (or NULL). */
 size_t flare_scan_backward_workspace_size(int64_t B, int64_t N, int64_t C, int64_t S, int64_t G, int64_t chunk);
 int flare_scan_backward(const void* x, const void* dt, const float* A, const void* Bm, const void* Cm,
                         const float* D, const void* z, const float* dt_bias, int softplus, int dtype, int64_t B,
                         int64_t N, int64_t C, int64_t S, int64_t G, const int64_t* strides,
-                        const int32_t* document_ids, const void* dy, int64_t chunk, const float* states, void* dx,
+                        const int32_t* document_ids, const void* dy, int64_t chunk, const float* kept, void* dx,
                         void* ddt, float* dA, void* dB, void* dC, float* dD, void* dz, float* ddt_bias,
                         void* workspace, size_t workspace_bytes, void* stream);
 

@@ -107,17 +107,19 @@ def test_c_entry_points_check_before_they_launch():
                     b"1 to 64")
     assert _refused(lib.flare_scan_forward(*scan, 1, 4, 8, 16, 3, twelve, None, None, None, P, None, 4, None, P, 0, None),
                     b"groups")
-    assert _refused(lib.flare_scan_forward(*scan, 1, 4, 8, 16, 1, twelve, None, None, None, P, None, 2, None, P, 0, None),
-                    b"needs `states`")
+    assert _refused(lib.flare_scan_forward(*scan, 1, 4, 8, 16, 1, twelve, None, None, None, P, None, 48, P, P, 0, None),
+                    b"multiples")
     assert lib.flare_scan_forward(*scan, 1, 4, 8, 16, 1, twelve, None, None, None, P, None, 4, None, P, 8, None) == -3
     assert _refused(lib.flare_scan_forward(*scan, 1, 4, 8, 16, 1, twelve, P, None, P, P, None, 4, None, P, 0, None), b"exclude")
-    assert _refused(lib.flare_scan_backward(*scan, 1, 400, 8, 16, 1, twelve, None, P, 400, P, *[P] * 5, None, None, None, P,
-                                            0, None), b"chunks of 1 to 128")
-    assert lib.flare_scan_backward(*scan, 1, 4, 8, 16, 1, twelve, None, P, 4, P, *[P] * 5, None, None, None, P, 0, None) == -3
+    for chunk in (160, 48, 0):
+        assert _refused(lib.flare_scan_backward(*scan, 1, 400, 8, 16, 1, twelve, None, P, chunk, P, *[P] * 5, None, None,
+                                                None, P, 0, None), b"chunks of up to 128")
+    assert lib.flare_scan_backward(*scan, 1, 4, 8, 16, 1, twelve, None, P, 32, P, *[P] * 5, None, None, None, P, 0, None) == -3
     assert _refused(lib.flare_scan_step(*scan, 1, 8, 16, 1, twelve, None, None, P, None), b"null pointer")
     assert lib.flare_scan_chunk(1, 4, 8, 65, 1, 0) == 0
-    for states, most in ((4, 128), (16, 128), (32, 32), (64, 16)):
-        assert 1 <= lib.flare_scan_chunk(1, 10 ** 6, 64, states, 1, 1) <= most
+    for states in (4, 16, 32, 64):
+        chunk = lib.flare_scan_chunk(1, 10 ** 7, 64, states, 1, 1)
+        assert 1 <= chunk <= 128 and chunk % lib.flare_scan_kept_tokens(states) == 0
     attn = [P, P, P, nine, 1]
     assert _refused(lib.flare_attn_forward(*attn, 1, 4, 4, 4, 3, 64, 1.0, 0.0, None, 1, None, None, None, None, P, None, None,
                                            0, None), b"divide")
