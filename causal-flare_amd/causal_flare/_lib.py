@@ -171,7 +171,7 @@ def _declare(lib):
     lib.flare_attn_forward.argtypes = ([_vp] * 4 + [_i] + [_i64] * 6 + [_f, _f, _vp, _i] + [_vp] * 6
                                        + [_vp, _sz, _vp])
     lib.flare_attn_backward_workspace_size.restype = _sz
-    lib.flare_attn_backward_workspace_size.argtypes = [_i64] * 3
+    lib.flare_attn_backward_workspace_size.argtypes = [_i64] * 5 + [_i]
     lib.flare_attn_backward.restype = _i
     lib.flare_attn_backward.argtypes = ([_vp] * 4 + [_i] + [_i64] * 5 + [_f, _f, _vp, _i] + [_vp] * 8
                                         + [_vp, _sz, _vp])

@@ -135,7 +135,7 @@ class SoftmaxAttention(autograd.Function):
         g = _aligned_rows(dy, dtype).contiguous()
         dq, dk, dv = (torch.empty(t.shape, device=t.device, dtype=dtype) for t in (Q, K, V))
         lib = _lib.lib()
-        nbytes = lib.flare_attn_backward_workspace_size(B, N, H)
+        nbytes = lib.flare_attn_backward_workspace_size(B, N, H, G, D, _lib.dtype_code(dtype))
         ws = torch.empty(nbytes, device=Q.device, dtype=torch.uint8)
         P = _lib.ptr
         with _on(Q.device):

@@ -61,12 +61,16 @@ struct AttnArgs {
     const void* dy;                  // [B, N, H, D]
     const float* delta;              // [B, H, N]: dy . y
     void *dq, *dk, *dv;
+    int64_t row_splits;              // of `splits`: parts of the rows, times parts of the heads
     // single tokens
     const void *k_new, *v_new;       // [B, G, D]
     int64_t kn_sb, kn_sg, vn_sb, vn_sg;
-    float* parts;
+    float* parts;                    // what `splits` workgroups leave of each sum
     int64_t splits;
 };
+
+// Tiles of 16 keys a wave of the key gradients' kernel owns.
+constexpr int kv_tiles(int size, int DP) { return size == 2 && DP <= 64 ? 2 : 1; }
 
 __device__ __forceinline__ int64_t clamp_to(int64_t n, int64_t most) { return n < 0 ? 0 : (n > most ? most : n); }
 

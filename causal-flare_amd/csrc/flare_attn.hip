@@ -53,6 +53,22 @@ static int launch_ids(AttnArgs& p, int32_t* stats, hipStream_t stream) {
     return check_launch("attn_ids");
 }
 
+// Parts that the queries of each block of keys are split into: so many that there are 2048
+// workgroups (eight a CU: blocks of keys cost very different amounts of work under a causal or
+// document mask), the heads first and then the rows, in parts of 256 or more.
+static void split_backward(AttnArgs& p, int dtype) {
+    const int64_t DP = ceil_div(p.D, 32) * 32, blocks = ceil_div(p.N, 64 * kv_tiles(dtype == FLARE_F32 ? 4 : 2, (int)DP));
+    const int64_t R = p.H / p.G;
+    int64_t want = ceil_div(2048, blocks * p.B * p.G);
+    want = want > 8 ? 8 : want;
+    const int64_t heads = want < R ? want : R, rows = ceil_div(want, heads), most = ceil_div(p.N, 256);
+    p.row_splits = rows < most ? rows : most;
+    p.splits = heads * p.row_splits;
+}
+static size_t parts_bytes(const AttnArgs& p) {
+    return p.splits == 1 ? 0 : (size_t)(p.splits * 2 * p.B * p.N * p.G * p.D) * sizeof(float);
+}
+
 static bool aligned(const Rows& r, int dtype) {
     const int64_t per = dtype == FLARE_F32 ? 4 : 8;
     return ((uintptr_t)r.p & 15) == 0 && r.sb % per == 0 && r.sn % per == 0 && r.sh % per == 0;
@@ -116,8 +132,15 @@ extern "C" int flare_attn_forward(const void* q, const void* k, const void* v, c
     return FLARE_BY_DTYPE(dtype, forward_e, (p, (hipStream_t)stream));
 }
 
-extern "C" size_t flare_attn_backward_workspace_size(int64_t B, int64_t N, int64_t H) {
-    return (size_t)(B * H * N) * sizeof(float) + stats_bytes(B, N);
+static size_t backward_head_bytes(int64_t B, int64_t N, int64_t H) {
+    return ((size_t)(B * H * N) * sizeof(float) + stats_bytes(B, N) + 255) / 256 * 256;
+}
+extern "C" size_t flare_attn_backward_workspace_size(int64_t B, int64_t N, int64_t H, int64_t G, int64_t D, int dtype) {
+    if (B < 1 || N < 1 || H < 1 || G < 1 || H % G) return 0;
+    AttnArgs p = {};
+    p.B = B, p.N = N, p.H = H, p.G = G, p.D = D;
+    split_backward(p, dtype);
+    return backward_head_bytes(B, N, H) + parts_bytes(p);
 }
 
 extern "C" int flare_attn_backward(const void* q, const void* k, const void* v, const int64_t* strides, int dtype,
@@ -132,9 +155,9 @@ extern "C" int flare_attn_backward(const void* q, const void* k, const void* v, 
     ATTN_REQUIRE_SIZES("flare_attn_backward");
     AttnArgs p = attn_args(q, k, v, strides, B, N, M, H, G, D, scale, softcap, slopes);
     const uintptr_t out = (uintptr_t)y | (uintptr_t)dy | (uintptr_t)dq | (uintptr_t)dk | (uintptr_t)dv;
-    FLARE_REQUIRE(aligned(p.q, dtype) && aligned(p.k, dtype) && aligned(p.v, dtype) && (out & 15) == 0,
-                  "flare_attn_backward: rows must be 16-byte aligned");
-    if (workspace_bytes < flare_attn_backward_workspace_size(B, N, H)) {
+    FLARE_REQUIRE(aligned(p.q, dtype) && aligned(p.k, dtype) && aligned(p.v, dtype) && (out & 15) == 0 &&
+                  ((uintptr_t)workspace & 15) == 0, "flare_attn_backward: rows must be 16-byte aligned");
+    if (workspace_bytes < flare_attn_backward_workspace_size(B, N, H, G, D, dtype)) {
         set_error("flare_attn_backward: workspace of %zu bytes is too small", workspace_bytes);
         return FLARE_ERR_WORKSPACE;
     }
@@ -142,6 +165,8 @@ extern "C" int flare_attn_backward(const void* q, const void* k, const void* v, 
     p.causal = causal, p.ids = document_ids, p.prefix = prefix_lengths;
     p.y = const_cast<void*>(y), p.lse = const_cast<float*>(lse), p.dy = dy, p.delta = delta;
     p.dq = dq, p.dk = dk, p.dv = dv;
+    split_backward(p, dtype);
+    p.parts = (float*)((char*)workspace + backward_head_bytes(B, N, H));
     const int rc = launch_ids(p, (int32_t*)(delta + B * H * N), (hipStream_t)stream);
     if (rc != FLARE_OK) return rc;
     return FLARE_BY_DTYPE(dtype, backward_e, (p, delta, (hipStream_t)stream));

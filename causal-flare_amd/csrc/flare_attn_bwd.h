@@ -232,7 +232,7 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnArgs p) {
 }
 
 template <typename E, int DP, int KQ, bool CAP>
-__global__ __launch_bounds__(256, DP > 96 && sizeof(E) == 2 ? 1 : 2) void attn_dkv_kernel(AttnArgs p) {
+__global__ __launch_bounds__(256, 2) void attn_dkv_kernel(AttnArgs p) {
     typedef typename Elem<E>::S S;
     typedef typename Elem<E>::Frag Frag;
     using Lds = BackwardLds<E, DP>;
@@ -251,10 +251,20 @@ __global__ __launch_bounds__(256, DP > 96 && sizeof(E) == 2 ? 1 : 2) void attn_d
     int64_t id = blockIdx.x;
     const int64_t kvh = id % p.G;
     id /= p.G;
-    const int64_t b = id % p.B, kb = id / p.B * KB;     // the keys most queries see come first
+    const int64_t b = id % p.B;
+    id /= p.B;
+    // this workgroup's part of the queries: some of the heads that share these keys, some of the rows
+    const int64_t part = id % p.splits, kb = id / p.splits * KB;     // the keys most queries see come first
+    const int64_t rep0 = part / p.row_splits * R / (p.splits / p.row_splits);
+    const int64_t rep1 = (part / p.row_splits + 1) * R / (p.splits / p.row_splits);
 
     const int64_t prefix = p.prefix ? clamp_to(p.prefix[b], p.N) : 0;
-    const int64_t q_begin = p.causal && kb >= prefix ? kb : 0;
+    int64_t q_begin = p.causal && kb >= prefix ? kb : 0, q_end = p.N;
+    if (p.row_splits > 1) {
+        const int64_t k = part % p.row_splits, tiles = (p.N - q_begin + QR - 1) / QR, from = q_begin;
+        q_begin = from + tiles * k / p.row_splits * QR;
+        q_end = min(p.N, from + tiles * (k + 1) / p.row_splits * QR);
+    }
     IdRange mine{0, 0, true};
     if (p.ids) mine = id_block(p, b, kb, KB);
     const int64_t w0 = kb + wave * 16 * KQ;             // this wave's first key
@@ -329,19 +339,19 @@ __global__ __launch_bounds__(256, DP > 96 && sizeof(E) == 2 ? 1 : 2) void attn_d
         }
     };
     int buf = 0;
-    for (int64_t rep = 0; rep < R; ++rep) {
+    for (int64_t rep = rep0; rep < rep1; ++rep) {
         const int64_t h = kvh * R + rep;
         const float slope2 = p.slopes ? p.slopes[h] * kLog2e : 0.0f;
-        TileWalk<QR> walk(p, b, p.N, mine);
+        TileWalk<QR> walk(p, b, q_end, mine);
         int64_t q0 = walk.next(q_begin);
-        if (q0 < p.N) {
+        if (q0 < q_end) {
             fetch(h, q0);
             place(q0, buf);
         }
         __syncthreads();
-        while (q0 < p.N) {
+        while (q0 < q_end) {
             const int64_t q1 = walk.next(q0 + QR);
-            if (q1 < p.N) fetch(h, q1);
+            if (q1 < q_end) fetch(h, q1);
             const bool hidden = w0 >= p.N || (p.causal && w0 > q0 + QR - 1 && w0 >= prefix);
             if (!hidden) {
                 const S* qt = ql + buf * QR * P;
@@ -422,7 +432,7 @@ __global__ __launch_bounds__(256, DP > 96 && sizeof(E) == 2 ? 1 : 2) void attn_d
                     }
                 }
             }
-            if (q1 < p.N) place(q1, buf ^ 1);
+            if (q1 < q_end) place(q1, buf ^ 1);
             __syncthreads();
             buf ^= 1;
             q0 = q1;
@@ -432,16 +442,36 @@ __global__ __launch_bounds__(256, DP > 96 && sizeof(E) == 2 ? 1 : 2) void attn_d
     for (int t = 0; t < KQ; ++t) {
         const int64_t j = w0 + 16 * t + c;
         if (j >= p.N) continue;
-        const int64_t row = ((b * p.N + j) * p.G + kvh) * p.D;
+        const int64_t row = ((b * p.N + j) * p.G + kvh) * p.D, all = p.B * p.N * p.G * p.D;
 #pragma unroll
         for (int d = 0; d < DT; ++d) {
             if (16 * d < p.D) {
                 typedef S S4 __attribute__((ext_vector_type(4)));
-                *reinterpret_cast<S4*>((S*)p.dk + row + 16 * d + 4 * g) = __builtin_convertvector(dk[t][d] * p.scale, S4);
-                *reinterpret_cast<S4*>((S*)p.dv + row + 16 * d + 4 * g) = __builtin_convertvector(dv[t][d] * kUnshift, S4);
+                const f32x4 k4 = dk[t][d] * p.scale, v4 = dv[t][d] * kUnshift;
+                const int64_t at = row + 16 * d + 4 * g;
+                if (p.splits > 1) {
+                    *reinterpret_cast<f32x4*>(p.parts + part * 2 * all + at) = k4;
+                    *reinterpret_cast<f32x4*>(p.parts + (part * 2 + 1) * all + at) = v4;
+                } else {
+                    *reinterpret_cast<S4*>((S*)p.dk + at) = __builtin_convertvector(k4, S4);
+                    *reinterpret_cast<S4*>((S*)p.dv + at) = __builtin_convertvector(v4, S4);
+                }
             }
         }
     }
+}
+
+// The parts' sums, in order.
+template <typename E>
+__global__ __launch_bounds__(256) void attn_parts_kernel(AttnArgs p) {
+    typedef typename Elem<E>::S S;
+    typedef S S4 __attribute__((ext_vector_type(4)));
+    const int64_t all = p.B * p.N * p.G * p.D, at = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
+    if (at >= 2 * all) return;
+    f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int64_t s = 0; s < p.splits; ++s) sum += *reinterpret_cast<const f32x4*>(p.parts + s * 2 * all + at);
+    S* to = at < all ? (S*)p.dk + at : (S*)p.dv + at - all;
+    *reinterpret_cast<S4*>(to) = __builtin_convertvector(sum, S4);
 }
 
 template <typename K>
@@ -459,15 +489,18 @@ static int backward_cap(const AttnArgs& p, hipStream_t stream) {
     constexpr int QT = sizeof(E) == 2 ? 2 : 1;
     constexpr size_t bytes = BackwardLds<E, DP>::bytes;
     auto dq = attn_dq_kernel<E, DP, QT, CAP>;
-    auto dkv = attn_dkv_kernel<E, DP, QT, CAP>;
+    constexpr int KQ = kv_tiles(sizeof(E), DP);
+    auto dkv = attn_dkv_kernel<E, DP, KQ, CAP>;
     int rc = allow_lds(dq, bytes, "attn_dq");
     if (rc == FLARE_OK) rc = allow_lds(dkv, bytes, "attn_dkv");
     if (rc != FLARE_OK) return rc;
     const int64_t blocks = ceil_div(p.N, 64 * QT) * p.B;
     dq<<<dim3((unsigned)(blocks * p.H)), 256, bytes, stream>>>(p);
     if ((rc = check_launch("attn_dq")) != FLARE_OK) return rc;
-    dkv<<<dim3((unsigned)(blocks * p.G)), 256, bytes, stream>>>(p);
-    return check_launch("attn_dkv");
+    dkv<<<dim3((unsigned)(ceil_div(p.N, 64 * KQ) * p.B * p.G * p.splits)), 256, bytes, stream>>>(p);
+    if ((rc = check_launch("attn_dkv")) != FLARE_OK || p.splits == 1) return rc;
+    attn_parts_kernel<E><<<dim3((unsigned)ceil_div(p.B * p.N * p.G * p.D / 2, 256)), 256, 0, stream>>>(p);
+    return check_launch("attn_parts");
 }
 template <typename E, int DP>
 static int backward_dp(const AttnArgs& p, hipStream_t stream) {

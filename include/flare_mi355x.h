@@ -406,7 +406,7 @@ int flare_attn_forward(const void* q, const void* k, const void* v, const int64_
                        float* lse, void* workspace, size_t workspace_bytes, void* stream);
 
 /* Its gradients without a cache, from y, lse and dy [B, N, H, D]: dq [B, N, H, D], dk, dv [B, N, G, D]. */
-size_t flare_attn_backward_workspace_size(int64_t B, int64_t N, int64_t H);
+size_t flare_attn_backward_workspace_size(int64_t B, int64_t N, int64_t H, int64_t G, int64_t D, int dtype);
 int flare_attn_backward(const void* q, const void* k, const void* v, const int64_t* strides, int dtype, int64_t B,
                         int64_t N, int64_t H, int64_t G, int64_t D, float scale, float softcap, const float* slopes,
                         int causal, const int32_t* document_ids, const int32_t* prefix_lengths, const void* y,
