@@ -69,10 +69,12 @@ def _rows(t, dtype):
 
 
 def _aligned_rows(t, dtype):
-    """`_rows`, and every row on a 16-byte boundary."""
+    """`_rows` of a [B, n, heads, D] tensor with every row on a 16-byte boundary, and tokens less than
+    2^22 elements apart."""
     t = _rows(t, dtype)
     size = t.element_size()
-    if t.data_ptr() % 16 or any(s * size % 16 for s in t.stride()[:-1]) or t.stride(-1) != 1:
+    if (t.data_ptr() % 16 or any(s * size % 16 for s in t.stride()[:-1]) or t.stride(-1) != 1
+            or t.stride(1) >= 1 << 22):
         t = t.clone(memory_format=torch.contiguous_format)
     return t
 

@@ -39,6 +39,7 @@ typedef u32 u32x4 __attribute__((ext_vector_type(4)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 
+constexpr int64_t kMostStride = 1 << 22;      // between rows, so that a tile's offsets fit 31 bits
 constexpr int kIdTile = 64;          // tokens of one entry of the id statistics
 
 struct Rows {                        // a [B, n, heads, D] tensor: element strides
@@ -164,28 +165,40 @@ __device__ __forceinline__ float tanh_log2(float x2) {
 }
 
 // ROWS rows of DP elements from memory to LDS through registers, 16 bytes a thread at a time:
-// rows that are none and columns behind D become 0.
+// rows that are none and columns behind D become 0.  The loads go through a buffer descriptor of
+// the tile's rows, so a lane's part of the address is one number for all tiles.
 template <typename E, int ROWS, int DP, int PITCH, int NT>
 struct Stage {
     typedef typename Elem<E>::S S;
     static constexpr int PER = 16 / sizeof(E), CPR = DP / PER, N = (ROWS * CPR + NT - 1) / NT;
-    static constexpr bool WHOLE = ROWS * CPR % NT == 0;
+    static constexpr bool EVEN = NT % CPR == 0;         // a round of the threads is whole rows
+    static constexpr int M = EVEN ? 1 : N;
     u32x4 r[N];
-    // `base`: row 0 of this head; rows first .. first+ROWS-1, those at or behind `end` are none
-    __device__ __forceinline__ void load(const S* base, int64_t stride, int64_t first, int64_t end, int D, int tid) {
+    u32 at[M], step, to[M];
+    __device__ __forceinline__ void begin(int64_t stride, int64_t D, int tid) {
+        step = EVEN ? (u32)(NT / CPR) * (u32)stride * sizeof(E) : 0;
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
+        for (int i = 0; i < M; ++i) {
             const int e = i * NT + tid, row = e / CPR, col = e % CPR * PER;
-            r[i] = u32x4{0, 0, 0, 0};
-            if ((WHOLE || e < ROWS * CPR) && first + row < end && col < D)
-                r[i] = *reinterpret_cast<const u32x4*>(base + (first + row) * stride + col);
+            at[i] = e < ROWS * CPR && col < D ? (u32)(row * (u32)stride + col) * (u32)sizeof(E) : 0x80000000u;
+            to[i] = row * PITCH + col;
         }
+    }
+    // `first`: row 0 of the tile; the `rows` of it that are there
+    __device__ __forceinline__ void load(const S* first, int64_t rows, int64_t stride, int64_t D) {
+        const int n = (int)min(rows, (int64_t)ROWS);
+        const int bytes = n > 0 ? ((n - 1) * (int)stride + (int)D) * (int)sizeof(E) : 0;
+        const auto rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<S*>(first), 0, bytes, 0x00020000);
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            r[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(
+                                                 rsrc, EVEN ? at[0] + i * step : at[i % M], 0, 0));
     }
     __device__ __forceinline__ void store(S* lds, int tid) const {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            const int e = i * NT + tid;
-            if (WHOLE || e < ROWS * CPR) *reinterpret_cast<u32x4*>(lds + e / CPR * PITCH + e % CPR * PER) = r[i];
+            if (ROWS * CPR % NT == 0 || i * NT + tid < ROWS * CPR)
+                *reinterpret_cast<u32x4*>(lds + (EVEN ? to[0] + i * (NT / CPR) * PITCH : to[i % M])) = r[i];
         }
     }
     // whether one of these elements is infinite or NaN

@@ -71,7 +71,8 @@ static size_t parts_bytes(const AttnArgs& p) {
 
 static bool aligned(const Rows& r, int dtype) {
     const int64_t per = dtype == FLARE_F32 ? 4 : 8;
-    return ((uintptr_t)r.p & 15) == 0 && r.sb % per == 0 && r.sn % per == 0 && r.sh % per == 0;
+    return ((uintptr_t)r.p & 15) == 0 && r.sb % per == 0 && r.sn % per == 0 && r.sh % per == 0 && r.sn >= 0 &&
+           r.sn < kMostStride;
 }
 
 // Workgroups of the step kernel for each sequence's keys: enough for four on each CU (1024 on
@@ -94,7 +95,7 @@ using namespace flare::attn;
     FLARE_REQUIRE(D >= 16 && D <= 128 && D % 16 == 0, name ": head dimension %lld is not a multiple of 16 up to " \
                   "128", (long long)D);                                                                           \
     FLARE_REQUIRE(N <= (1 << 30) && M <= (1 << 30) && B <= 65535 && H <= 65535 && B * H <= (1 << 24) &&           \
-                  (N + 63) / 64 * B * H <= INT32_MAX, name ": too large");                                        \
+                  (N + 63) / 64 * B * H <= INT32_MAX && H * D < kMostStride, name ": too large");                                        \
     FLARE_REQUIRE(softcap >= 0.0f && softcap < __builtin_huge_valf(), name ": the cap must be finite and not negative")
 
 static AttnArgs attn_args(const void* q, const void* k, const void* v, const int64_t* st, int64_t B, int64_t N,
@@ -120,7 +121,7 @@ extern "C" int flare_attn_forward(const void* q, const void* k, const void* v, c
     FLARE_REQUIRE(lengths || !new_lengths, "flare_attn_forward: new_lengths without lengths");
     AttnArgs p = attn_args(q, k, v, strides, B, N, M, H, G, D, scale, softcap, slopes);
     FLARE_REQUIRE(aligned(p.q, dtype) && aligned(p.k, dtype) && aligned(p.v, dtype) && ((uintptr_t)y & 15) == 0,
-                  "flare_attn_forward: rows must be 16-byte aligned");
+                  "flare_attn_forward: rows must be 16-byte aligned and less than 2^22 elements apart");
     p.causal = causal, p.ids = document_ids, p.prefix = prefix_lengths, p.lengths = lengths, p.fresh = new_lengths;
     p.y = y, p.lse = lse;
     if (document_ids && (!workspace || workspace_bytes < stats_bytes(B, N))) {
@@ -156,7 +157,7 @@ extern "C" int flare_attn_backward(const void* q, const void* k, const void* v, 
     AttnArgs p = attn_args(q, k, v, strides, B, N, M, H, G, D, scale, softcap, slopes);
     const uintptr_t out = (uintptr_t)y | (uintptr_t)dy | (uintptr_t)dq | (uintptr_t)dk | (uintptr_t)dv;
     FLARE_REQUIRE(aligned(p.q, dtype) && aligned(p.k, dtype) && aligned(p.v, dtype) && (out & 15) == 0 &&
-                  ((uintptr_t)workspace & 15) == 0, "flare_attn_backward: rows must be 16-byte aligned");
+                  ((uintptr_t)workspace & 15) == 0, "flare_attn_backward: rows must be 16-byte aligned and less than 2^22 elements apart");
     if (workspace_bytes < flare_attn_backward_workspace_size(B, N, H, G, D, dtype)) {
         set_error("flare_attn_backward: workspace of %zu bytes is too small", workspace_bytes);
         return FLARE_ERR_WORKSPACE;
@@ -181,7 +182,7 @@ extern "C" int flare_attn_append(const void* k, const void* v, const int64_t* st
     ATTN_REQUIRE_SIZES("flare_attn_append");
     const Rows kr = {k, strides[0], strides[1], strides[2]}, vr = {v, strides[3], strides[4], strides[5]};
     FLARE_REQUIRE(aligned(kr, dtype) && aligned(vr, dtype) && (((uintptr_t)k_cache | (uintptr_t)v_cache) & 15) == 0,
-                  "flare_attn_append: rows must be 16-byte aligned");
+                  "flare_attn_append: rows must be 16-byte aligned and less than 2^22 elements apart");
     const int64_t size = dtype == FLARE_F32 ? 4 : 2, work = B * N * G * (D * size / 16);
     FLARE_REQUIRE(work <= (int64_t)INT32_MAX * 256, "flare_attn_append: too large");
     attn_append_kernel<<<dim3((unsigned)ceil_div(work, 256)), 256, 0, (hipStream_t)stream>>>(
@@ -209,7 +210,7 @@ extern "C" int flare_attn_step(const void* q, const void* k, const void* v, cons
     p.v_new = v, p.vn_sb = strides[4], p.vn_sg = strides[5];
     const Rows kr = {k, strides[2], 0, strides[3]}, vr = {v, strides[4], 0, strides[5]};
     FLARE_REQUIRE(aligned(p.q, dtype) && aligned(kr, dtype) && aligned(vr, dtype) && aligned(p.k, dtype) &&
-                  aligned(p.v, dtype), "flare_attn_step: rows must be 16-byte aligned");
+                  aligned(p.v, dtype), "flare_attn_step: rows must be 16-byte aligned and less than 2^22 elements apart");
     FLARE_REQUIRE(B * G * ceil_div(H / G, 16) <= 65535, "flare_attn_step: too large");
     p.splits = step_splits(B, M, H, G);
     if (workspace_bytes < flare_attn_step_workspace_size(B, M, H, G, D) || (p.splits > 1 && !workspace)) {

@@ -104,11 +104,15 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnArgs p) {
     const float scale2 = p.scale * kLog2e, slope2 = p.slopes ? p.slopes[h] * kLog2e : 0.0f;
     const float cap2 = p.cap * kLog2e, into_cap = CAP ? 2.0f * kLog2e * p.scale / p.cap : 0.0f;
 
+    const float out_scale = CAP ? 4.0f * p.scale : p.scale;
     f32x4 acc[QT][DT];
+    float cap_lse[QT];
 #pragma unroll
-    for (int t = 0; t < QT; ++t)
+    for (int t = 0; t < QT; ++t) {
+        cap_lse[t] = cap2 - lse[t];
 #pragma unroll
         for (int d = 0; d < DT; ++d) acc[t][d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
 
     auto covers = [&](int64_t k0, int64_t first, int64_t last) {
         if (k0 + KT > p.N || last >= p.N) return false;
@@ -116,10 +120,12 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnArgs p) {
         return !p.ids || mine.same(id_range(p, b, k0 / kIdTile));
     };
     Stage<E, KT, DP, P, 256> ks, vs;
+    ks.begin(p.k.sn, p.D, tid);
+    vs.begin(p.v.sn, p.D, tid);
     int next_id = -1;
     auto fetch = [&](int64_t k0) {
-        ks.load(kbase, p.k.sn, k0, p.N, p.D, tid);
-        vs.load(vbase, p.v.sn, k0, p.N, p.D, tid);
+        ks.load(kbase + k0 * p.k.sn, p.N - k0, p.k.sn, p.D);
+        vs.load(vbase + k0 * p.v.sn, p.N - k0, p.v.sn, p.D);
         if (p.ids && tid < KT) next_id = k0 + tid < p.N ? p.ids[b * p.N + k0 + tid] : -1;
     };
     auto place = [&](int64_t k0, int buf) {
@@ -170,18 +176,18 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnArgs p) {
                 for (int n = 0; n < 2; ++n) {
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        float x = s[t][n][i], slant = 1.0f;
+                        float x = s[t][n][i], r = 0.0f;
                         if (CAP) {
-                            const float th = tanh_log2(x * into_cap);
-                            x = cap2 * th;
-                            slant = 1.0f - th * th;
+                            // cap tanh(x / cap) = cap (1 - 2 r), 1 - tanh^2 = 4 r (1 - r)
+                            r = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(x * into_cap));
+                            x = cap_lse[t] - 2.0f * cap2 * r;
                         } else {
-                            x *= scale2;
+                            x = x * scale2 - lse[t];
                         }
                         if (p.slopes) x -= slope2 * fabsf(base - (float)(16 * n + i));
-                        const float w = __builtin_amdgcn_exp2f(x - lse[t]);
+                        const float w = __builtin_amdgcn_exp2f(x);
                         float ds = w * (dp[t][n][i] - delta[t]);
-                        if (CAP) ds *= slant;
+                        if (CAP) ds *= r - r * r;              // and 4 in the end
                         s[t][n][i] = ds;
                     }
                 }
@@ -225,7 +231,7 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnArgs p) {
         for (int d = 0; d < DT; ++d) {
             if (16 * d < p.D) {
                 typedef S S4 __attribute__((ext_vector_type(4)));
-                *reinterpret_cast<S4*>(row + 16 * d + 4 * g) = __builtin_convertvector(acc[t][d] * p.scale, S4);
+                *reinterpret_cast<S4*>(row + 16 * d + 4 * g) = __builtin_convertvector(acc[t][d] * out_scale, S4);
             }
         }
     }
@@ -301,15 +307,17 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(AttnArgs p) {
         return !p.ids || mine.same(id_range(p, b, q0 / kIdTile));
     };
     Stage<E, QR, DP, P, 256> qs, gs;
+    qs.begin(p.q.sn, p.D, tid);
+    gs.begin(p.H * p.D, p.D, tid);
     float next_lse = 0.0f, next_delta = 0.0f;
     int next_id = -1;
     auto fetch = [&](int64_t h, int64_t q0) {
-        qs.load((const S*)p.q.p + b * p.q.sb + h * p.q.sh, p.q.sn, q0, p.N, p.D, tid);
-        gs.load((const S*)p.dy + (b * p.N * p.H + h) * p.D, p.H * p.D, q0, p.N, p.D, tid);
+        qs.load((const S*)p.q.p + b * p.q.sb + h * p.q.sh + q0 * p.q.sn, p.N - q0, p.q.sn, p.D);
+        gs.load((const S*)p.dy + ((b * p.N + q0) * p.H + h) * p.D, p.N - q0, p.H * p.D, p.D);
         if (tid < QR) {
             const bool live = q0 + tid < p.N;
             const int64_t at = (b * p.H + h) * p.N + q0 + tid;
-            next_lse = live ? p.lse[at] - kShift : -kNegInf;
+            next_lse = live ? p.lse[at] - kShift - cap2 : -kNegInf;
             next_delta = live ? p.delta[at] * kUnshift : 0.0f;
             if (p.ids) next_id = live ? p.ids[b * p.N + q0 + tid] : -1;
         }
@@ -385,18 +393,17 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(AttnArgs p) {
                         const float base = (float)(int)(q0 + 4 * g - (w0 + 16 * t + c));
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
-                            float x = s[t][n][i], slant = 1.0f;
+                            float x = s[t][n][i], r = 0.0f;
                             if (CAP) {
-                                const float th = tanh_log2(x * into_cap);
-                                x = cap2 * th;
-                                slant = 1.0f - th * th;
+                                r = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(x * into_cap));
+                                x = -2.0f * cap2 * r - lse[i];          // the log-sum-exp less the cap
                             } else {
-                                x *= scale2;
+                                x = x * scale2 - lse[i];
                             }
                             if (p.slopes) x -= slope2 * fabsf(base + (float)(16 * n + i));
-                            const float w = __builtin_amdgcn_exp2f(x - lse[i]);
+                            const float w = __builtin_amdgcn_exp2f(x);
                             float ds = w * (dp[t][n][i] * kUnshift - delta[i]);
-                            if (CAP) ds *= slant;
+                            if (CAP) ds *= r - r * r;
                             s[t][n][i] = w;
                             dp[t][n][i] = ds;
                         }
@@ -447,7 +454,7 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(AttnArgs p) {
         for (int d = 0; d < DT; ++d) {
             if (16 * d < p.D) {
                 typedef S S4 __attribute__((ext_vector_type(4)));
-                const f32x4 k4 = dk[t][d] * p.scale, v4 = dv[t][d] * kUnshift;
+                const f32x4 k4 = dk[t][d] * (CAP ? 4.0f * p.scale : p.scale), v4 = dv[t][d] * kUnshift;
                 const int64_t at = row + 16 * d + 4 * g;
                 if (p.splits > 1) {
                     *reinterpret_cast<f32x4*>(p.parts + part * 2 * all + at) = k4;

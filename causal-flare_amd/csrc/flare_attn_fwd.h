@@ -12,6 +12,12 @@
 namespace flare {
 namespace attn {
 
+// How scores are kept from overflowing: against a running maximum, or against the cap itself,
+// which bounds them.
+enum { kNoCap = 0, kCapRunning = 1, kCapFixed = 2 };
+// With weights of 2^(s - cap) a row's largest is at least 2^(-2 cap): fp32 and bf16 hold that, with
+// all that counts beside it, up to here (log2 units), and fp16 does not.
+constexpr float kCapFixedMost = 60.0f;
 constexpr float kSlack = 8.0f;       // log2 of the largest weight before the reference moves
 
 template <typename E, int DP, int KT>
@@ -21,7 +27,7 @@ struct ForwardLds {
     static constexpr size_t bytes = 2 * (k_bytes + v_bytes + KT * sizeof(int)) + sizeof(int);
 };
 
-template <typename E, int DP, int QT, int KT, bool CAP>
+template <typename E, int DP, int QT, int KT, int CAP>
 __global__ __launch_bounds__(256, 2) void attn_forward_kernel(AttnArgs p) {
     typedef typename Elem<E>::S S;
     typedef typename Elem<E>::Frag Frag;
@@ -80,20 +86,21 @@ __global__ __launch_bounds__(256, 2) void attn_forward_kernel(AttnArgs p) {
 #pragma unroll
         for (int kk = 0; kk < DK; ++kk) {
             const int d = 32 * kk + 8 * g;
+            qf[t][kk] = Frag{};
             if (live && d < p.D) qf[t][kk] = frag_rows<E>(row + d);
-            else qf[t][kk] = Frag{};
+            if (p.scale < 0.0f) qf[t][kk] = -qf[t][kk];          // scores then scale by |scale|
         }
     }
     const S* kbase = (const S*)p.k.p + b * p.k.sb + kvh * p.k.sh;
     const S* vbase = (const S*)p.v.p + b * p.v.sb + kvh * p.v.sh;
-    const float scale2 = p.scale * kLog2e, slope2 = p.slopes ? p.slopes[h] * kLog2e : 0.0f;
-    const float cap2 = p.cap * kLog2e, into_cap = CAP ? 2.0f * kLog2e * p.scale / p.cap : 0.0f;
+    const float scale2 = fabsf(p.scale) * kLog2e, slope2 = p.slopes ? p.slopes[h] * kLog2e : 0.0f;
+    const float cap2 = p.cap * kLog2e, into_cap = CAP ? 2.0f * kLog2e * fabsf(p.scale) / p.cap : 0.0f;
 
     f32x4 acc[QT][DT];
     float top[QT], sum[QT];
 #pragma unroll
     for (int t = 0; t < QT; ++t) {
-        top[t] = kNegInf;
+        top[t] = CAP == kCapFixed ? cap2 : kNegInf;
         sum[t] = 0.0f;
 #pragma unroll
         for (int d = 0; d < DT; ++d) acc[t][d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
@@ -106,10 +113,12 @@ __global__ __launch_bounds__(256, 2) void attn_forward_kernel(AttnArgs p) {
     };
     Stage<E, KT, DP, KP, 256> ks;
     Stage<E, KT, DP, VP, 256> vs;
+    ks.begin(p.k.sn, p.D, tid);
+    vs.begin(p.v.sn, p.D, tid);
     int next_id = -1;
     auto fetch = [&](int64_t k0) {
-        ks.load(kbase, p.k.sn, k0, kvlen, p.D, tid);
-        vs.load(vbase, p.v.sn, k0, kvlen, p.D, tid);
+        ks.load(kbase + k0 * p.k.sn, kvlen - k0, p.k.sn, p.D);
+        vs.load(vbase + k0 * p.v.sn, kvlen - k0, p.v.sn, p.D);
         if (p.ids && tid < KT) next_id = k0 + tid < p.N ? p.ids[b * p.N + k0 + tid] : -1;
     };
     auto place = [&](int64_t k0, int buf) {
@@ -158,15 +167,29 @@ __global__ __launch_bounds__(256, 2) void attn_forward_kernel(AttnArgs p) {
             const bool whole = covers(k0, w0, w0 + 16 * QT - 1);
 #pragma unroll
             for (int t = 0; t < QT; ++t) {
-                const float base = (float)(int)(pos[t] - k0 - 4 * g);
+                // Scores become log2 weights: those that the cap bounds relative to it (kCapFixed),
+                // others absolute, and plain ones stay as they are until their exponential.
+                const bool plain = CAP == kNoCap && whole && !p.slopes;
+                if (CAP != kNoCap) {
 #pragma unroll
-                for (int n = 0; n < NK; ++n) {
+                    for (int n = 0; n < NK; ++n) {
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        float x = s[t][n][i];
-                        x = CAP ? cap2 * tanh_log2(x * into_cap) : x * scale2;
-                        if (p.slopes) x -= slope2 * fabsf(base - (float)(16 * n + i));
-                        s[t][n][i] = x;
+                        for (int i = 0; i < 4; ++i) {
+                            // cap tanh(x / cap) = cap - 2 cap / (e^(2 x / cap) + 1)
+                            const float r = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(s[t][n][i] * into_cap));
+                            s[t][n][i] = CAP == kCapFixed ? -2.0f * cap2 * r : cap2 - 2.0f * cap2 * r;
+                        }
+                    }
+                } else if (!plain) {
+#pragma unroll
+                    for (int n = 0; n < NK; ++n) s[t][n] *= scale2;
+                }
+                if (p.slopes) {
+                    const float base = (float)(int)(pos[t] - k0 - 4 * g);
+#pragma unroll
+                    for (int n = 0; n < NK; ++n) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) s[t][n][i] -= slope2 * fabsf(base - (float)(16 * n + i));
                     }
                 }
                 if (!whole) {
@@ -182,29 +205,41 @@ __global__ __launch_bounds__(256, 2) void attn_forward_kernel(AttnArgs p) {
                         }
                     }
                 }
-                float m = s[t][0][0];
+                float ref = 0.0f;
+                if (CAP != kCapFixed) {
+                    float m = mfma::max3_raw(s[t][0][0], s[t][0][1], s[t][0][2]);
+                    m = mfma::max_raw(m, s[t][0][3]);
 #pragma unroll
-                for (int n = 0; n < NK; ++n)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) m = fmaxf(m, s[t][n][i]);
-                m = column_max(m);
-                if (__any(m > top[t] + kSlack)) {
-                    const float to = fmaxf(m, top[t]);
-                    const float f = top[t] == to ? 1.0f : __builtin_amdgcn_exp2f(top[t] - to);
-                    top[t] = to;
-                    sum[t] *= f;
-#pragma unroll
-                    for (int d = 0; d < DT; ++d) acc[t][d] *= f;
-                }
-                const float ref = top[t] == kNegInf ? 0.0f : top[t];
-#pragma unroll
-                for (int n = 0; n < NK; ++n) {
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        s[t][n][i] = __builtin_amdgcn_exp2f(s[t][n][i] - ref);
-                        sum[t] += s[t][n][i];
+                    for (int n = 1; n < NK; ++n) {
+                        m = mfma::max3_raw(m, s[t][n][0], s[t][n][1]);
+                        m = mfma::max3_raw(m, s[t][n][2], s[t][n][3]);
                     }
+                    m = column_max(m);
+                    if (plain) m *= scale2;
+                    if (__any(m > top[t] + kSlack)) {
+                        const float to = fmaxf(m, top[t]);
+                        const float f = top[t] == to ? 1.0f : __builtin_amdgcn_exp2f(top[t] - to);
+                        top[t] = to;
+                        sum[t] *= f;
+#pragma unroll
+                        for (int d = 0; d < DT; ++d) acc[t][d] *= f;
+                    }
+                    ref = top[t] == kNegInf ? 0.0f : top[t];
                 }
+                if (plain) {
+#pragma unroll
+                    for (int n = 0; n < NK; ++n)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) s[t][n][i] = __builtin_amdgcn_exp2f(s[t][n][i] * scale2 - ref);
+                } else {
+#pragma unroll
+                    for (int n = 0; n < NK; ++n)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            s[t][n][i] = __builtin_amdgcn_exp2f(CAP == kCapFixed ? s[t][n][i] : s[t][n][i] - ref);
+                }
+#pragma unroll
+                for (int n = 0; n < NK; ++n) sum[t] += (s[t][n][0] + s[t][n][1]) + (s[t][n][2] + s[t][n][3]);
             }
             Frag w[QT][NK / 2];
 #pragma unroll
@@ -274,7 +309,7 @@ __global__ __launch_bounds__(256, 2) void attn_forward_kernel(AttnArgs p) {
     }
 }
 
-template <typename E, int DP, bool CAP>
+template <typename E, int DP, int CAP>
 static int forward_cap(const AttnArgs& p, hipStream_t stream) {
     constexpr int QT = sizeof(E) == 2 ? 2 : 1, KT = sizeof(E) == 2 ? 64 : 32;
     constexpr size_t bytes = ForwardLds<E, DP, KT>::bytes;
@@ -293,7 +328,10 @@ static int forward_cap(const AttnArgs& p, hipStream_t stream) {
 }
 template <typename E, int DP>
 static int forward_dp(const AttnArgs& p, hipStream_t stream) {
-    return p.cap > 0.0f ? forward_cap<E, DP, true>(p, stream) : forward_cap<E, DP, false>(p, stream);
+    if (p.cap == 0.0f) return forward_cap<E, DP, kNoCap>(p, stream);
+    if constexpr (!__is_same(E, __half))
+        if (p.cap * kLog2e <= kCapFixedMost) return forward_cap<E, DP, kCapFixed>(p, stream);
+    return forward_cap<E, DP, kCapRunning>(p, stream);
 }
 template <typename E>
 int forward_e(const AttnArgs& p, hipStream_t stream) {

@@ -257,14 +257,17 @@ ATTENTION = [
     (1, 1, 1, 1, 16, ""), (2, 2, 2, 1, 32, "cap"), (1, 15, 4, 2, 48, "slopes"), (2, 63, 2, 2, 64, "docs"),
     (1, 64, 4, 1, 64, "cap slopes"), (2, 65, 2, 2, 80, "full"), (2, 130, 4, 2, 96, "prefix"),
     (3, 200, 3, 1, 128, "docs slopes"), (2, 257, 2, 1, 128, "cap docs prefix"), (1, 191, 2, 2, 112, "full docs slopes"),
-    (2, 300, 1, 1, 64, "prefix slopes"), (1, 513, 2, 2, 64, "docs"),
+    (2, 300, 1, 1, 64, "prefix slopes"), (1, 513, 2, 2, 64, "docs"), (1, 100, 2, 1, 64, "negative"),
+    (1, 140, 2, 2, 128, "wide-cap slopes negative"),
 ]
 
 
 def attention_options(g, what, B, N, H):
     o = {}
     if "cap" in what:
-        o["softcap"] = 3.0
+        o["softcap"] = 50.0 if "wide-cap" in what else 3.0
+    if "negative" in what:
+        o["scale"] = -0.2
     if "slopes" in what:
         o["slopes"] = torch.tensor([2.0 ** -(h + 1) for h in range(H)]).to(DEV)
     if "docs" in what:
@@ -278,7 +281,7 @@ def attention_options(g, what, B, N, H):
 
 def plain(o):
     o = dict(o)
-    return dict(softcap=o.get("softcap"), slopes=o.get("slopes"), ids=o.get("document_ids"),
+    return dict(scale=o.get("scale"), softcap=o.get("softcap"), slopes=o.get("slopes"), ids=o.get("document_ids"),
                 prefix=o.get("prefix_lengths"), causal=o.get("causal", True))
 
 
