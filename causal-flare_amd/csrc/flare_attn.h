@@ -73,6 +73,9 @@ struct AttnArgs {
 // Tiles of 16 keys a wave of the key gradients' kernel owns.
 constexpr int kv_tiles(int size, int DP) { return size == 2 && DP <= 64 ? 2 : 1; }
 
+// Ids as the kernels compare them: padding's negative ones are those of no key and of no query.
+constexpr int kNoKey = -1, kNoQuery = -2;
+
 __device__ __forceinline__ int64_t clamp_to(int64_t n, int64_t most) { return n < 0 ? 0 : (n > most ? most : n); }
 
 template <typename E> struct Elem;
@@ -185,8 +188,8 @@ struct Stage {
         }
     }
     // `first`: row 0 of the tile; the `rows` of it that are there
-    __device__ __forceinline__ void load(const S* first, int64_t rows, int64_t stride, int64_t D) {
-        const int n = (int)min(rows, (int64_t)ROWS);
+    __device__ __forceinline__ void load(const S* first, int rows, int64_t stride, int64_t D) {
+        const int n = min(rows, ROWS);
         const int bytes = n > 0 ? ((n - 1) * (int)stride + (int)D) * (int)sizeof(E) : 0;
         const auto rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<S*>(first), 0, bytes, 0x00020000);
 #pragma unroll
@@ -247,15 +250,15 @@ struct IdRange {
     __device__ __forceinline__ bool meets(const IdRange& o) const { return lo <= o.hi && o.lo <= hi; }
     __device__ __forceinline__ bool same(const IdRange& o) const { return pure && o.pure && lo == o.lo; }
 };
-__device__ __forceinline__ int64_t id_tiles(int64_t N) { return (N + kIdTile - 1) / kIdTile; }
-__device__ __forceinline__ IdRange id_range(const AttnArgs& p, int64_t b, int64_t tile) {
+__device__ __forceinline__ int id_tiles(int64_t N) { return ((int)N + kIdTile - 1) / kIdTile; }
+__device__ __forceinline__ IdRange id_range(const AttnArgs& p, int64_t b, int tile) {
     const int32_t* s = p.id_stats + (b * id_tiles(p.N) + tile) * 3;
     return IdRange{s[0], s[1], s[2] != 0};
 }
 // Tokens first .. first+n-1 (first a multiple of 64, or all within one tile).
-__device__ __forceinline__ IdRange id_block(const AttnArgs& p, int64_t b, int64_t first, int64_t n) {
+__device__ __forceinline__ IdRange id_block(const AttnArgs& p, int64_t b, int first, int n) {
     IdRange r = id_range(p, b, first / kIdTile);
-    for (int64_t t = first / kIdTile + 1; t * kIdTile < min(first + n, p.N); ++t) {
+    for (int t = first / kIdTile + 1; t * kIdTile < min(first + n, (int)p.N); ++t) {
         const IdRange o = id_range(p, b, t);
         r.pure = r.same(o);
         r.lo = min(r.lo, o.lo);
@@ -269,19 +272,20 @@ __device__ __forceinline__ IdRange id_block(const AttnArgs& p, int64_t b, int64_
 template <int STEP>
 struct TileWalk {
     const AttnArgs& p;
-    int64_t b, end;
+    int64_t b;
+    int end;
     IdRange mine;
-    int64_t window;                  // the 64 tiles of ids that `mask` tells of begin here
+    int window;                      // the 64 tiles of ids that `mask` tells of begin here
     uint64_t mask;
-    __device__ __forceinline__ TileWalk(const AttnArgs& p, int64_t b, int64_t end, IdRange mine)
+    __device__ __forceinline__ TileWalk(const AttnArgs& p, int64_t b, int end, IdRange mine)
         : p(p), b(b), end(end), mine(mine), window(-64), mask(0) {}
-    __device__ __forceinline__ int64_t next(int64_t k) {       // k: a multiple of STEP
+    __device__ __forceinline__ int next(int k) {       // k: a multiple of STEP
         if (!p.ids) return k;
         while (k < end) {
-            const int64_t t = k / kIdTile;
+            const int t = k / kIdTile;
             if (t >= window + 64) {
                 window = t;
-                const int64_t at = t + (threadIdx.x & 63);
+                const int at = t + (threadIdx.x & 63);
                 mask = __ballot(at < id_tiles(p.N) && id_range(p, b, at).meets(mine));
             }
             const uint64_t left = mask >> (t - window);

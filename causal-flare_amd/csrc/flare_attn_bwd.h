@@ -62,29 +62,33 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnArgs p) {
     int* oddl = idl + 2 * KT;                           // [2][4]
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int g = lane >> 4, c = lane & 15;
-    const int64_t R = p.H / p.G, nq = (p.N + QB - 1) / QB;
-    int64_t id = blockIdx.x;
-    const int64_t kvh = id % p.G;
-    id /= p.G;
-    const int64_t b = id % p.B;
-    id /= p.B;
-    const int64_t h = kvh * R + id % R, q0 = (nq - 1 - id / R) * QB;
+    const int N = (int)p.N, R = (int)(p.H / p.G), nq = (N + QB - 1) / QB;
+    int id = blockIdx.x;
+    const int kvh = id % (int)p.G;
+    id /= (int)p.G;
+    const int64_t b = id % (int)p.B;
+    id /= (int)p.B;
+    const int h = kvh * R + id % R, q0 = (nq - 1 - id / R) * QB;
 
-    const int64_t prefix = p.prefix ? clamp_to(p.prefix[b], p.N) : 0;
-    const int64_t kv_end = p.causal ? max(min(q0 + QB, p.N), prefix) : p.N;
+    const int prefix = p.prefix ? (int)clamp_to(p.prefix[b], p.N) : 0;
+    const int kv_end = p.causal ? max(min(q0 + QB, N), prefix) : N;
     IdRange mine{0, 0, true};
     if (p.ids) mine = id_block(p, b, q0, QB);
-    const int64_t w0 = q0 + wave * 16 * QT;
+    const int w0 = q0 + wave * 16 * QT;
     Frag qf[QT][DK], gf[QT][DK];
-    int64_t pos[QT];
-    int qid[QT];
+    int pos[QT], lim[QT], qid[QT];                     // as in attn_forward
     float lse[QT], delta[QT];
 #pragma unroll
     for (int t = 0; t < QT; ++t) {
-        const int64_t i = w0 + 16 * t + c;
-        const bool live = i < p.N;
-        pos[t] = live ? i : -1;
-        qid[t] = p.ids && live ? p.ids[b * p.N + i] : -1;
+        const int i = w0 + 16 * t + c;
+        const bool live = i < N;
+        pos[t] = i;
+        lim[t] = !live ? 0 : p.causal ? max(i + 1, prefix) : N;
+        qid[t] = kNoQuery;
+        if (p.ids && live) {
+            const int d = p.ids[b * p.N + i];
+            qid[t] = d < 0 ? kNoQuery : d;
+        }
         lse[t] = live ? p.lse[(b * p.H + h) * p.N + i] : -kNegInf;
         delta[t] = live ? p.delta[(b * p.H + h) * p.N + i] : 0.0f;
         const S* q = (const S*)p.q.p + b * p.q.sb + (live ? i : 0) * p.q.sn + h * p.q.sh;
@@ -114,8 +118,8 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnArgs p) {
         for (int d = 0; d < DT; ++d) acc[t][d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     }
 
-    auto covers = [&](int64_t k0, int64_t first, int64_t last) {
-        if (k0 + KT > p.N || last >= p.N) return false;
+    auto covers = [&](int k0, int first, int last) {
+        if (k0 + KT > N || last >= N) return false;
         if (p.causal && k0 + KT - 1 > first && k0 + KT > prefix) return false;
         return !p.ids || mine.same(id_range(p, b, k0 / kIdTile));
     };
@@ -123,12 +127,12 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnArgs p) {
     ks.begin(p.k.sn, p.D, tid);
     vs.begin(p.v.sn, p.D, tid);
     int next_id = -1;
-    auto fetch = [&](int64_t k0) {
-        ks.load(kbase + k0 * p.k.sn, p.N - k0, p.k.sn, p.D);
-        vs.load(vbase + k0 * p.v.sn, p.N - k0, p.v.sn, p.D);
-        if (p.ids && tid < KT) next_id = k0 + tid < p.N ? p.ids[b * p.N + k0 + tid] : -1;
+    auto fetch = [&](int k0) {
+        ks.load(kbase + k0 * p.k.sn, N - k0, p.k.sn, p.D);
+        vs.load(vbase + k0 * p.v.sn, N - k0, p.v.sn, p.D);
+        if (p.ids && tid < KT) next_id = max(k0 + tid < N ? p.ids[b * p.N + k0 + tid] : kNoKey, kNoKey);
     };
-    auto place = [&](int64_t k0, int buf) {
+    auto place = [&](int k0, int buf) {
         ks.store(kl + buf * KT * P, tid);
         vs.store(vl + buf * KT * P, tid);
         if (p.ids && tid < KT) idl[buf * KT + tid] = next_id;
@@ -136,7 +140,7 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnArgs p) {
         if (lane == 0) oddl[buf * 4 + wave] = odd;
     };
     TileWalk<KT> walk(p, b, kv_end, mine);
-    int64_t k0 = walk.next(0);
+    int k0 = walk.next(0);
     int buf = 0;
     if (k0 < kv_end) {
         fetch(k0);
@@ -144,9 +148,9 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnArgs p) {
     }
     __syncthreads();
     while (k0 < kv_end) {
-        const int64_t k1 = walk.next(k0 + KT);
+        const int k1 = walk.next(k0 + KT);
         if (k1 < kv_end) fetch(k1);
-        const bool hidden = w0 >= p.N || (p.causal && k0 > w0 + 16 * QT - 1 && k0 >= prefix);
+        const bool hidden = w0 >= N || (p.causal && k0 > w0 + 16 * QT - 1 && k0 >= prefix);
         if (!hidden) {
             const S* kt = kl + buf * KT * P;
             const S* vt = vl + buf * KT * P;
@@ -171,7 +175,7 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnArgs p) {
             const bool whole = covers(k0, w0, w0 + 16 * QT - 1);
 #pragma unroll
             for (int t = 0; t < QT; ++t) {
-                const float base = (float)(int)(pos[t] - k0 - 4 * g);
+                const float base = (float)(pos[t] - k0 - 4 * g);
 #pragma unroll
                 for (int n = 0; n < 2; ++n) {
 #pragma unroll
@@ -192,15 +196,17 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnArgs p) {
                     }
                 }
                 if (!whole) {
+                    const int left = lim[t] - k0 - 4 * g;
 #pragma unroll
                     for (int n = 0; n < 2; ++n) {
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const int64_t j = k0 + 16 * n + 4 * g + i;
-                            bool see = j < p.N && pos[t] >= 0;
-                            if (p.causal) see = see && (j <= pos[t] || j < prefix);
-                            if (p.ids) see = see && qid[t] >= 0 && idl[buf * KT + 16 * n + 4 * g + i] == qid[t];
-                            if (!see) s[t][n][i] = 0.0f;
+                        for (int i = 0; i < 4; ++i) s[t][n][i] = 16 * n + i < left ? s[t][n][i] : 0.0f;
+                        if (p.ids) {
+                            const int4 d = *reinterpret_cast<const int4*>(idl + buf * KT + 16 * n + 4 * g);
+                            s[t][n][0] = d.x == qid[t] ? s[t][n][0] : 0.0f;
+                            s[t][n][1] = d.y == qid[t] ? s[t][n][1] : 0.0f;
+                            s[t][n][2] = d.z == qid[t] ? s[t][n][2] : 0.0f;
+                            s[t][n][3] = d.w == qid[t] ? s[t][n][3] : 0.0f;
                         }
                     }
                 }
@@ -224,8 +230,8 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnArgs p) {
     }
 #pragma unroll
     for (int t = 0; t < QT; ++t) {
-        const int64_t i = w0 + 16 * t + c;
-        if (i >= p.N) continue;
+        const int i = w0 + 16 * t + c;
+        if (i >= N) continue;
         S* row = (S*)p.dq + ((b * p.N + i) * p.H + h) * p.D;
 #pragma unroll
         for (int d = 0; d < DT; ++d) {
@@ -253,34 +259,35 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(AttnArgs p) {
     int* oddl = idl + 2 * QR;                           // [2][4]
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int g = lane >> 4, c = lane & 15;
-    const int64_t R = p.H / p.G;
-    int64_t id = blockIdx.x;
-    const int64_t kvh = id % p.G;
-    id /= p.G;
-    const int64_t b = id % p.B;
-    id /= p.B;
+    const int N = (int)p.N, R = (int)(p.H / p.G), parts = (int)p.splits, row_parts = (int)p.row_splits;
+    int id = blockIdx.x;
+    const int kvh = id % (int)p.G;
+    id /= (int)p.G;
+    const int64_t b = id % (int)p.B;
+    id /= (int)p.B;
     // this workgroup's part of the queries: some of the heads that share these keys, some of the rows
-    const int64_t part = id % p.splits, kb = id / p.splits * KB;     // the keys most queries see come first
-    const int64_t rep0 = part / p.row_splits * R / (p.splits / p.row_splits);
-    const int64_t rep1 = (part / p.row_splits + 1) * R / (p.splits / p.row_splits);
+    const int part = id % parts, kb = id / parts * KB;               // the keys most queries see come first
+    const int rep0 = part / row_parts * R / (parts / row_parts);
+    const int rep1 = (part / row_parts + 1) * R / (parts / row_parts);
 
-    const int64_t prefix = p.prefix ? clamp_to(p.prefix[b], p.N) : 0;
-    int64_t q_begin = p.causal && kb >= prefix ? kb : 0, q_end = p.N;
-    if (p.row_splits > 1) {
-        const int64_t k = part % p.row_splits, tiles = (p.N - q_begin + QR - 1) / QR, from = q_begin;
-        q_begin = from + tiles * k / p.row_splits * QR;
-        q_end = min(p.N, from + tiles * (k + 1) / p.row_splits * QR);
+    const int prefix = p.prefix ? (int)clamp_to(p.prefix[b], p.N) : 0;
+    int q_begin = p.causal && kb >= prefix ? kb : 0, q_end = N;
+    if (row_parts > 1) {
+        const int k = part % row_parts, tiles = (N - q_begin + QR - 1) / QR, from = q_begin;
+        q_begin = from + (int)((int64_t)tiles * k / row_parts) * QR;
+        q_end = min(N, from + (int)((int64_t)tiles * (k + 1) / row_parts) * QR);
     }
     IdRange mine{0, 0, true};
     if (p.ids) mine = id_block(p, b, kb, KB);
-    const int64_t w0 = kb + wave * 16 * KQ;             // this wave's first key
+    const int w0 = kb + wave * 16 * KQ;                 // this wave's first key
     Frag kf[KQ][DK], vf[KQ][DK];
-    int kid[KQ];
+    int kid[KQ], from[KQ];                              // of this lane's keys: document, and the first row to see it
 #pragma unroll
     for (int t = 0; t < KQ; ++t) {
-        const int64_t j = w0 + 16 * t + c;
-        const bool live = j < p.N;
-        kid[t] = p.ids && live ? p.ids[b * p.N + j] : -1;
+        const int j = w0 + 16 * t + c;
+        const bool live = j < N;
+        from[t] = !live ? INT32_MAX : p.causal && j >= prefix ? j : 0;
+        kid[t] = !live ? kNoKey : p.ids ? max(p.ids[b * p.N + j], kNoKey) : 0;
         const S* k = (const S*)p.k.p + b * p.k.sb + (live ? j : 0) * p.k.sn + kvh * p.k.sh;
         const S* v = (const S*)p.v.p + b * p.v.sb + (live ? j : 0) * p.v.sn + kvh * p.v.sh;
 #pragma unroll
@@ -301,8 +308,8 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(AttnArgs p) {
 #pragma unroll
         for (int d = 0; d < DT; ++d) dk[t][d] = dv[t][d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 
-    auto covers = [&](int64_t q0, int64_t first, int64_t last) {
-        if (q0 + QR > p.N || last >= p.N) return false;
+    auto covers = [&](int q0, int first, int last) {
+        if (q0 + QR > N || last >= N) return false;
         if (p.causal && last > q0 && last >= prefix) return false;
         return !p.ids || mine.same(id_range(p, b, q0 / kIdTile));
     };
@@ -311,20 +318,21 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(AttnArgs p) {
     gs.begin(p.H * p.D, p.D, tid);
     float next_lse = 0.0f, next_delta = 0.0f;
     int next_id = -1;
-    auto fetch = [&](int64_t h, int64_t q0) {
-        qs.load((const S*)p.q.p + b * p.q.sb + h * p.q.sh + q0 * p.q.sn, p.N - q0, p.q.sn, p.D);
-        gs.load((const S*)p.dy + ((b * p.N + q0) * p.H + h) * p.D, p.N - q0, p.H * p.D, p.D);
+    auto fetch = [&](int h, int q0) {
+        qs.load((const S*)p.q.p + b * p.q.sb + h * p.q.sh + q0 * p.q.sn, N - q0, p.q.sn, p.D);
+        gs.load((const S*)p.dy + ((b * p.N + q0) * p.H + h) * p.D, N - q0, p.H * p.D, p.D);
         if (tid < QR) {
-            const bool live = q0 + tid < p.N;
+            const bool live = q0 + tid < N;
             const int64_t at = (b * p.H + h) * p.N + q0 + tid;
             next_lse = live ? p.lse[at] - kShift - cap2 : -kNegInf;
             next_delta = live ? p.delta[at] * kUnshift : 0.0f;
-            if (p.ids) next_id = live ? p.ids[b * p.N + q0 + tid] : -1;
+            next_id = !live ? kNoQuery : p.ids ? p.ids[b * p.N + q0 + tid] : 0;
+            next_id = next_id < 0 ? kNoQuery : next_id;
         }
     };
     // Tiles seen in part keep infinite values and NaNs out of LDS (0 times them is NaN); the rows
     // they are in have a log-sum-exp or a delta that is none, and their weights are NaN then.
-    auto place = [&](int64_t q0, int buf) {
+    auto place = [&](int q0, int buf) {
         bool odd = false;
         if (!covers(q0, kb, kb + KB - 1)) {
             if (qs.odd()) {
@@ -347,20 +355,20 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(AttnArgs p) {
         }
     };
     int buf = 0;
-    for (int64_t rep = rep0; rep < rep1; ++rep) {
-        const int64_t h = kvh * R + rep;
+    for (int rep = rep0; rep < rep1; ++rep) {
+        const int h = kvh * R + rep;
         const float slope2 = p.slopes ? p.slopes[h] * kLog2e : 0.0f;
         TileWalk<QR> walk(p, b, q_end, mine);
-        int64_t q0 = walk.next(q_begin);
+        int q0 = walk.next(q_begin);
         if (q0 < q_end) {
             fetch(h, q0);
             place(q0, buf);
         }
         __syncthreads();
         while (q0 < q_end) {
-            const int64_t q1 = walk.next(q0 + QR);
+            const int q1 = walk.next(q0 + QR);
             if (q1 < q_end) fetch(h, q1);
-            const bool hidden = w0 >= p.N || (p.causal && w0 > q0 + QR - 1 && w0 >= prefix);
+            const bool hidden = w0 >= N || (p.causal && w0 > q0 + QR - 1 && w0 >= prefix);
             if (!hidden) {
                 const S* qt = ql + buf * QR * P;
                 const S* gt = gl + buf * QR * P;
@@ -390,7 +398,7 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(AttnArgs p) {
                     const f32x4 delta = *reinterpret_cast<const f32x4*>(dell + buf * QR + 16 * n + 4 * g);
 #pragma unroll
                     for (int t = 0; t < KQ; ++t) {
-                        const float base = (float)(int)(q0 + 4 * g - (w0 + 16 * t + c));
+                        const float base = (float)(q0 + 4 * g - (w0 + 16 * t + c));
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
                             float x = s[t][n][i], r = 0.0f;
@@ -408,16 +416,16 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(AttnArgs p) {
                             dp[t][n][i] = ds;
                         }
                         if (!whole) {
-                            const int64_t j = w0 + 16 * t + c;
+                            const int late = from[t] - q0 - 4 * g - 16 * n;
+                            const int4 d = *reinterpret_cast<const int4*>(idl + buf * QR + 16 * n + 4 * g);
+                            const int row_id[4] = {d.x, d.y, d.z, d.w};
 #pragma unroll
                             for (int i = 0; i < 4; ++i) {
-                                const int64_t at = q0 + 16 * n + 4 * g + i;
-                                bool see = j < p.N && at < p.N;
-                                if (p.causal) see = see && (j <= at || j < prefix);
-                                if (p.ids) see = see && kid[t] >= 0 && idl[buf * QR + 16 * n + 4 * g + i] == kid[t];
+                                const bool see = i >= late && row_id[i] == kid[t];
                                 if (odd && !(fabsf(lse[i]) < -kNegInf && fabsf(delta[i]) < -kNegInf))
                                     s[t][n][i] = dp[t][n][i] = __builtin_nanf("");
-                                if (!see) s[t][n][i] = dp[t][n][i] = 0.0f;
+                                s[t][n][i] = see ? s[t][n][i] : 0.0f;
+                                dp[t][n][i] = see ? dp[t][n][i] : 0.0f;
                             }
                         }
                     }
@@ -447,8 +455,8 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(AttnArgs p) {
     }
 #pragma unroll
     for (int t = 0; t < KQ; ++t) {
-        const int64_t j = w0 + 16 * t + c;
-        if (j >= p.N) continue;
+        const int j = w0 + 16 * t + c;
+        if (j >= N) continue;
         const int64_t row = ((b * p.N + j) * p.G + kvh) * p.D, all = p.B * p.N * p.G * p.D;
 #pragma unroll
         for (int d = 0; d < DT; ++d) {

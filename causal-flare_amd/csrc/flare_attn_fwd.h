@@ -43,28 +43,26 @@ __global__ __launch_bounds__(256, 2) void attn_forward_kernel(AttnArgs p) {
 
     // heads that share keys, and then the tiles of one head, are 8 workgroups or a multiple of
     // that apart where there are 8 key heads: one XCD and its L2.  The longest rows come first.
-    const int64_t R = p.H / p.G, nq = (p.N + QB - 1) / QB;
-    int64_t id = blockIdx.x;
-    const int64_t kvh = id % p.G;
-    id /= p.G;
-    const int64_t b = id % p.B;
-    id /= p.B;
-    const int64_t h = kvh * R + id % R, q0 = (nq - 1 - id / R) * QB;
+    const int R = (int)(p.H / p.G), nq = ((int)p.N + QB - 1) / QB;
+    int id = blockIdx.x;
+    const int kvh = id % (int)p.G;
+    id /= (int)p.G;
+    const int64_t b = id % (int)p.B;
+    id /= (int)p.B;
+    const int h = kvh * R + id % R, q0 = (nq - 1 - id / R) * QB;
 
-    int64_t off = 0, qlen = p.N, kvlen = p.M;
+    int off = 0, qlen = (int)p.N, kvlen = (int)p.M;
     bool refused = false;
     if (p.lengths) {
         off = p.lengths[b];
-        qlen = p.fresh ? clamp_to(p.fresh[b], p.N) : p.N;
+        qlen = (int)(p.fresh ? clamp_to(p.fresh[b], p.N) : p.N);
         if (off < 0) off = qlen = 0;
+        refused = (int64_t)off + qlen > p.M;
+        if (refused) off = qlen = 0;
         kvlen = off + qlen;
-        if (kvlen > p.M) {
-            refused = true;
-            qlen = kvlen = 0;
-        }
     }
-    const int64_t prefix = p.prefix ? clamp_to(p.prefix[b], p.M) : 0;
-    int64_t kv_end = 0;
+    const int prefix = p.prefix ? (int)clamp_to(p.prefix[b], p.M) : 0;
+    int kv_end = 0;
     if (q0 < qlen) {
         kv_end = kvlen;
         if (p.causal) kv_end = min(kvlen, max(off + min(q0 + QB, qlen), prefix));
@@ -72,16 +70,21 @@ __global__ __launch_bounds__(256, 2) void attn_forward_kernel(AttnArgs p) {
     IdRange mine{0, 0, true};
     if (p.ids) mine = id_block(p, b, q0, QB);
 
-    const int64_t w0 = q0 + wave * 16 * QT;            // this wave's first query
+    const int w0 = q0 + wave * 16 * QT;                // this wave's first query
     Frag qf[QT][DK];
-    int64_t pos[QT];                                   // of this lane's queries
-    int qid[QT];
+    int pos[QT], lim[QT];                              // of this lane's queries: position, and the keys below
+    int qid[QT];                                       // which it sees those of its document
 #pragma unroll
     for (int t = 0; t < QT; ++t) {
-        const int64_t i = w0 + 16 * t + c;
+        const int i = w0 + 16 * t + c;
         const bool live = i < qlen;
-        pos[t] = live ? i + off : -1;                  // sees nothing but what a prefix shows
-        qid[t] = p.ids && live ? p.ids[b * p.N + i] : -1;
+        pos[t] = i + off;
+        lim[t] = !live ? 0 : p.causal ? min(kvlen, max(pos[t] + 1, prefix)) : kvlen;
+        qid[t] = kNoQuery;
+        if (p.ids && live) {
+            const int d = p.ids[b * p.N + i];
+            qid[t] = d < 0 ? kNoQuery : d;
+        }
         const S* row = (const S*)p.q.p + b * p.q.sb + (live ? i : 0) * p.q.sn + h * p.q.sh;
 #pragma unroll
         for (int kk = 0; kk < DK; ++kk) {
@@ -106,7 +109,7 @@ __global__ __launch_bounds__(256, 2) void attn_forward_kernel(AttnArgs p) {
         for (int d = 0; d < DT; ++d) acc[t][d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     }
 
-    auto covers = [&](int64_t k0, int64_t first, int64_t last) {       // every query sees every key
+    auto covers = [&](int k0, int first, int last) {       // every query sees every key
         if (k0 + KT > kvlen || last >= qlen) return false;
         if (p.causal && k0 + KT - 1 > first + off && k0 + KT > prefix) return false;
         return !p.ids || mine.same(id_range(p, b, k0 / kIdTile));
@@ -116,12 +119,12 @@ __global__ __launch_bounds__(256, 2) void attn_forward_kernel(AttnArgs p) {
     ks.begin(p.k.sn, p.D, tid);
     vs.begin(p.v.sn, p.D, tid);
     int next_id = -1;
-    auto fetch = [&](int64_t k0) {
+    auto fetch = [&](int k0) {
         ks.load(kbase + k0 * p.k.sn, kvlen - k0, p.k.sn, p.D);
         vs.load(vbase + k0 * p.v.sn, kvlen - k0, p.v.sn, p.D);
-        if (p.ids && tid < KT) next_id = k0 + tid < p.N ? p.ids[b * p.N + k0 + tid] : -1;
+        if (p.ids && tid < KT) next_id = max(k0 + tid < (int)p.N ? p.ids[b * p.N + k0 + tid] : kNoKey, kNoKey);
     };
-    auto place = [&](int64_t k0, int buf) {
+    auto place = [&](int k0, int buf) {
         // A weight of 0 times an infinite value is NaN: tiles that some query does not see whole
         // leave such values to the end.
         if (!covers(k0, q0, q0 + QB - 1) && vs.odd()) {
@@ -134,7 +137,7 @@ __global__ __launch_bounds__(256, 2) void attn_forward_kernel(AttnArgs p) {
     };
 
     TileWalk<KT> walk(p, b, kv_end, mine);
-    int64_t k0 = walk.next(0);
+    int k0 = walk.next(0);
     int buf = 0;
     if (tid == 0) *oddl = 0;
     __syncthreads();
@@ -144,7 +147,7 @@ __global__ __launch_bounds__(256, 2) void attn_forward_kernel(AttnArgs p) {
     }
     __syncthreads();
     while (k0 < kv_end) {
-        const int64_t k1 = walk.next(k0 + KT);
+        const int k1 = walk.next(k0 + KT);
         if (k1 < kv_end) fetch(k1);
         const bool hidden = w0 >= qlen || (p.causal && k0 > w0 + 16 * QT - 1 + off && k0 >= prefix);
         if (!hidden) {
@@ -185,7 +188,7 @@ __global__ __launch_bounds__(256, 2) void attn_forward_kernel(AttnArgs p) {
                     for (int n = 0; n < NK; ++n) s[t][n] *= scale2;
                 }
                 if (p.slopes) {
-                    const float base = (float)(int)(pos[t] - k0 - 4 * g);
+                    const float base = (float)(pos[t] - k0 - 4 * g);
 #pragma unroll
                     for (int n = 0; n < NK; ++n) {
 #pragma unroll
@@ -193,15 +196,17 @@ __global__ __launch_bounds__(256, 2) void attn_forward_kernel(AttnArgs p) {
                     }
                 }
                 if (!whole) {
+                    const int left = lim[t] - k0 - 4 * g;
 #pragma unroll
                     for (int n = 0; n < NK; ++n) {
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const int64_t j = k0 + 16 * n + 4 * g + i;
-                            bool see = j < kvlen && pos[t] >= 0;
-                            if (p.causal) see = see && (j <= pos[t] || j < prefix);
-                            if (p.ids) see = see && qid[t] >= 0 && idl[buf * KT + 16 * n + 4 * g + i] == qid[t];
-                            if (!see) s[t][n][i] = kNegInf;
+                        for (int i = 0; i < 4; ++i) s[t][n][i] = 16 * n + i < left ? s[t][n][i] : kNegInf;
+                        if (p.ids) {
+                            const int4 d = *reinterpret_cast<const int4*>(idl + buf * KT + 16 * n + 4 * g);
+                            s[t][n][0] = d.x == qid[t] ? s[t][n][0] : kNegInf;
+                            s[t][n][1] = d.y == qid[t] ? s[t][n][1] : kNegInf;
+                            s[t][n][2] = d.z == qid[t] ? s[t][n][2] : kNegInf;
+                            s[t][n][3] = d.w == qid[t] ? s[t][n][3] : kNegInf;
                         }
                     }
                 }
@@ -267,13 +272,10 @@ __global__ __launch_bounds__(256, 2) void attn_forward_kernel(AttnArgs p) {
         TileWalk<KT> again(p, b, kv_end, mine);
         for (k0 = again.next(0); k0 < kv_end; k0 = again.next(k0 + KT)) {
             if (covers(k0, q0, q0 + QB - 1)) continue;
-            for (int64_t j = k0; j < min(k0 + KT, kvlen); ++j) {
+            for (int j = k0; j < min(k0 + KT, kvlen); ++j) {
 #pragma unroll
                 for (int t = 0; t < QT; ++t) {
-                    bool see = pos[t] >= 0;
-                    if (p.causal) see = see && (j <= pos[t] || j < prefix);
-                    if (p.ids) see = see && qid[t] >= 0 && p.ids[b * p.N + j] == qid[t];
-                    if (!see) continue;
+                    if (j >= lim[t] || (p.ids && max(p.ids[b * p.N + j], kNoKey) != qid[t])) continue;
 #pragma unroll
                     for (int d = 0; d < DT; ++d) {
 #pragma unroll
@@ -290,7 +292,7 @@ __global__ __launch_bounds__(256, 2) void attn_forward_kernel(AttnArgs p) {
 
 #pragma unroll
     for (int t = 0; t < QT; ++t) {
-        const int64_t i = w0 + 16 * t + c;
+        const int i = w0 + 16 * t + c;
         const float total = column_sum(sum[t]);
         const float inv = total == 0.0f ? 0.0f : 1.0f / total;
         if (i >= p.N) continue;
