@@ -6,6 +6,8 @@ import ctypes
 
 import torch
 
+from .. import _lib
+
 
 def _check_device(name, **tensors):
     """Every tensor on one GPU, that of the first."""
@@ -42,11 +44,15 @@ def _check_integers(name, what, t, shape):
 
 
 def _int32(t):
-    return None if t is None else t.to(torch.int32).contiguous()
+    if t is None or (t.dtype is torch.int32 and t.is_contiguous()):
+        return t
+    return t.to(torch.int32).contiguous()
 
 
 def _f32(t):
-    return None if t is None else t.detach().to(torch.float32).contiguous()
+    if t is None or (t.dtype is torch.float32 and t.is_contiguous()):
+        return t
+    return t.detach().to(torch.float32).contiguous()
 
 
 def _row_mask(name, mask, B, device):
@@ -64,8 +70,9 @@ def _rows(t, dtype):
     """`t` in `dtype` with its last dimension adjacent in memory; other strides stay."""
     if t is None:
         return None
-    t = t.detach().to(dtype)
-    return t if t.shape[-1] <= 1 or t.stride(-1) == 1 else t.contiguous()
+    if t.dtype is not dtype:
+        t = t.detach().to(dtype)
+    return t if t.shape[-1] <= 1 or t.stride(-1) == 1 else t.detach().contiguous()
 
 
 def _aligned_rows(t, dtype):
@@ -75,7 +82,7 @@ def _aligned_rows(t, dtype):
     size = t.element_size()
     if (t.data_ptr() % 16 or any(s * size % 16 for s in t.stride()[:-1]) or t.stride(-1) != 1
             or t.stride(1) >= 1 << 22):
-        t = t.clone(memory_format=torch.contiguous_format)
+        t = t.detach().clone(memory_format=torch.contiguous_format)
     return t
 
 
@@ -92,3 +99,20 @@ def _on(device):
 
 def _training(*tensors):
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
+# Single tokens: the call's host work counts, and these look at what the common call needs to
+# hold, with no messages; where it does not, the caller takes the general path with its checks.
+_CODES = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}
+
+
+def _plain_f32(t, device, *shape):
+    return t is None or (t.dtype is torch.float32 and t.shape == shape and t.device == device and t.is_contiguous())
+
+
+def _raw_stream(index):
+    return torch._C._cuda_getCurrentRawStream(index)
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()

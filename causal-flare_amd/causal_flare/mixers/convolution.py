@@ -18,6 +18,7 @@ from torch.autograd.function import once_differentiable
 from .. import _lib
 from .._common import _compute_dtype
 from ._inputs import (
+    _CODES,
     _check_device,
     _check_float,
     _check_integers,
@@ -25,6 +26,9 @@ from ._inputs import (
     _f32,
     _int32,
     _on,
+    _plain_f32,
+    _ptr,
+    _raw_stream,
     _row_mask,
     _rows,
 )
@@ -151,6 +155,31 @@ def short_convolution_prefill(
     return y.to(x.dtype), {"window": new.to(x.dtype)}
 
 
+def _step_fast(x, weight, bias, activation, state):
+    """The common call, or None: x [B, C] or [B, 1, C] of the window's type, fp32 weights."""
+    if x.dim() == 3 and x.shape[1] == 1:
+        B, _, C = x.shape
+    elif x.dim() == 2:
+        B, C = x.shape
+    else:
+        return None
+    device, code = x.device, _CODES.get(x.dtype)
+    if code is None or not B * C or device.type != "cuda" or device.index != torch.cuda.current_device():
+        return None
+    W = weight.shape[-1]
+    window = state.get("window") if isinstance(state, dict) else None
+    if (activation not in (None, "silu") or W not in (2, 3, 4) or (C > 1 and x.stride(-1) != 1)
+            or not _plain_f32(weight, device, C, W) or not _plain_f32(bias, device, C) or window is None
+            or window.dtype is not x.dtype or window.shape != (B, W - 1, C) or window.device != device
+            or not window.is_contiguous()):
+        return None
+    y = torch.empty((B, 1, C), device=device, dtype=x.dtype)
+    _lib.check(_lib.lib().flare_conv_step(
+        x.data_ptr(), x.stride(0), weight.data_ptr(), _ptr(bias), 1 if activation else 0, code, B, C, W, None,
+        window.data_ptr(), y.data_ptr(), _raw_stream(device.index)), "flare_conv_step")
+    return y, {"window": window}
+
+
 def short_convolution_decode(
     x: torch.Tensor,
     weight: torch.Tensor,
@@ -165,6 +194,10 @@ def short_convolution_decode(
     [B, 1]: a row of 0 keeps its window and gets y = 0.
     """
     name = "short_convolution_decode"
+    if attention_mask is None and state is not None:
+        out = _step_fast(x, weight, bias, activation, state)
+        if out is not None:
+            return out
     if x.dim() == 2:
         x = x[:, None]
     _check(name, x, weight, bias, activation)

@@ -21,6 +21,7 @@ from torch.autograd.function import once_differentiable
 from .. import _lib
 from .._common import _compute_dtype
 from ._inputs import (
+    _CODES,
     _check_device,
     _check_float,
     _check_integers,
@@ -28,6 +29,9 @@ from ._inputs import (
     _f32,
     _int32,
     _on,
+    _plain_f32,
+    _ptr,
+    _raw_stream,
     _row_mask,
     _rows,
     _strides,
@@ -217,6 +221,41 @@ def state_space_scan_prefill(
     return y.to(x.dtype), {"h": h}
 
 
+def _step_fast(x, dt, A, B, C, D, z, dt_bias, softplus, state):
+    """The common call, or None: one type for x, dt, z, B and C, fp32 parameters and state."""
+    token = x.dim() == 3
+    if x.dim() not in (2, 3) or (token and x.shape[1] != 1) or A.dim() != 2:
+        return None
+    nb, c, s = x.shape[0], x.shape[-1], A.shape[1]
+    dtype, device = x.dtype, x.device
+    code = _CODES.get(dtype)
+    if (code is None or not nb * c or not 1 <= s <= _MAX_STATES or device.type != "cuda"
+            or device.index != torch.cuda.current_device()):
+        return None
+    grouped = B.dim() == x.dim() + 1
+    g = B.shape[-2] if grouped else 1
+    want = (nb, 1) if token else (nb,)
+    want = want + (g, s) if grouped else want + (s,)
+    if B.dim() != len(want) or B.shape != want or C.shape != want or g < 1 or c % g:
+        return None
+    for t, n in ((x, c), (dt, c), (z, c), (B, s), (C, s)):
+        if t is not None and (t.dtype is not dtype or t.device != device or (n > 1 and t.stride(-1) != 1)):
+            return None
+    h = state.get("h") if isinstance(state, dict) else None
+    if (dt.shape != x.shape or (z is not None and z.shape != x.shape) or not _plain_f32(A, device, c, s)
+            or not _plain_f32(D, device, c) or not _plain_f32(dt_bias, device, c) or h is None
+            or not _plain_f32(h, device, nb, c, s)):
+        return None
+    strides = _strides(x.stride(0), 0, dt.stride(0), 0, 0 if z is None else z.stride(0), 0, B.stride(0), 0,
+                       B.stride(-2) if grouped else 0, C.stride(0), 0, C.stride(-2) if grouped else 0)
+    y = torch.empty((nb, 1, c), device=device, dtype=dtype)
+    _lib.check(_lib.lib().flare_scan_step(
+        x.data_ptr(), dt.data_ptr(), A.data_ptr(), B.data_ptr(), C.data_ptr(), _ptr(D), _ptr(z), _ptr(dt_bias),
+        1 if softplus else 0, code, nb, c, s, g, strides, None, h.data_ptr(), y.data_ptr(),
+        _raw_stream(device.index)), "flare_scan_step")
+    return y, {"h": h}
+
+
 def state_space_scan_decode(
     x: torch.Tensor,
     dt: torch.Tensor,
@@ -237,6 +276,10 @@ def state_space_scan_decode(
     place and returned.  attention_mask [B] or [B, 1]: a row of 0 keeps its state and gets y = 0.
     """
     name = "state_space_scan_decode"
+    if attention_mask is None and state is not None:
+        out = _step_fast(x, dt, A, B, C, D, z, dt_bias, dt_softplus, state)
+        if out is not None:
+            return out
     if x.dim() == 2:
         x, dt, B, C = x[:, None], dt[:, None], B[:, None], C[:, None]
         z = None if z is None else z[:, None]

@@ -14,19 +14,25 @@
 namespace flare {
 namespace attn {
 
-// delta: a wave for each row of a head.
+// delta: `lanes` (a power of 2) for each row of a head, 16 bytes of it a lane.
 template <typename E>
-__global__ __launch_bounds__(256) void attn_delta_kernel(AttnArgs p, float* delta) {
+__global__ __launch_bounds__(256) void attn_delta_kernel(AttnArgs p, int lanes, float* delta) {
     typedef typename Elem<E>::S S;
-    const int lane = threadIdx.x & 63;
-    const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);         // (b, i, h)
-    if (row >= p.B * p.N * p.H) return;
-    const S *y = (const S*)p.y + row * p.D, *dy = (const S*)p.dy + row * p.D;
+    constexpr int PER = 16 / sizeof(E);
+    const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x, row = id / lanes;         // (b, i, h)
+    if (row >= p.B * p.N * p.H) return;                    // whole rows
+    const int col = (int)(id % lanes) * PER;
     float s = 0.0f;
-    for (int d = 2 * lane; d < p.D; d += 128) s += (float)y[d] * (float)dy[d] + (float)y[d + 1] * (float)dy[d + 1];
-    s = wave_sum(s);
+    if (col < p.D) {
+        typedef S V __attribute__((ext_vector_type(PER)));
+        const V y = *reinterpret_cast<const V*>((const S*)p.y + row * p.D + col);
+        const V dy = *reinterpret_cast<const V*>((const S*)p.dy + row * p.D + col);
+#pragma unroll
+        for (int i = 0; i < PER; ++i) s += (float)y[i] * (float)dy[i];
+    }
+    for (int o = lanes / 2; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
     const int64_t h = row % p.H, i = row / p.H % p.N, b = row / p.H / p.N;
-    if (lane == 0) delta[(b * p.H + h) * p.N + i] = s;
+    if (col == 0) delta[(b * p.H + h) * p.N + i] = s;
 }
 
 // An operand's infinite values and NaNs set to 0.
@@ -523,7 +529,9 @@ static int backward_dp(const AttnArgs& p, hipStream_t stream) {
 }
 template <typename E>
 int backward_e(const AttnArgs& p, float* delta, hipStream_t stream) {
-    attn_delta_kernel<E><<<dim3((unsigned)ceil_div(p.B * p.N * p.H, 4)), 256, 0, stream>>>(p, delta);
+    int lanes = 2;
+    while (lanes * (int)(16 / sizeof(E)) < p.D) lanes *= 2;
+    attn_delta_kernel<E><<<dim3((unsigned)ceil_div(p.B * p.N * p.H * lanes, 256)), 256, 0, stream>>>(p, lanes, delta);
     const int rc = check_launch("attn_delta");
     if (rc != FLARE_OK) return rc;
     return p.D <= 32   ? backward_dp<E, 32>(p, stream)

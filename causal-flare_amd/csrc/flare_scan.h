@@ -67,18 +67,19 @@ __device__ __forceinline__ scalar_f* scalar_ptr(const float* p) { return (scalar
 
 inline int64_t padded_states(int64_t S) { return S <= 8 ? 8 : S <= 16 ? 16 : S <= 32 ? 32 : 64; }
 
-// Chunk length: some four waves a SIMD (4096 on the card), in multiples of 32 tokens, and at most
-// `most` (0: any).
-inline int64_t chunk_length(int64_t B, int64_t N, int64_t C, int64_t G, int64_t most) {
-    const int64_t waves = B * G * ceil_div(C / G, 64);
-    const int64_t nc = ceil_div(4096, waves);
-    const int64_t L = ceil_div(ceil_div(N, nc), 32) * 32;
-    return most && L > most ? most : L;
-}
 // The backward holds B and C of a chunk in LDS, and recomputes its states from those the forward
 // kept: so far apart that what it keeps of a stretch itself stays small.
 constexpr int64_t kBackwardChunkMost = 128;
 constexpr int64_t kept_tokens(int64_t SP) { return SP <= 16 ? 32 : SP == 32 ? 16 : 8; }
+
+// Chunk length: some four waves a SIMD (4096 on the card).  Where the channels are too few for
+// that a token's latency counts, and chunks go down to 8 tokens (32 for the backward, whose chunks
+// hold whole stretches between kept states).
+inline int64_t chunk_length(int64_t B, int64_t N, int64_t C, int64_t S, int64_t G, bool backward) {
+    const int64_t waves = B * G * ceil_div(C / G, 64), nc = ceil_div(4096, waves), least = backward ? 32 : 8;
+    const int64_t L = ceil_div(ceil_div(N, nc), least) * least;
+    return backward && L > kBackwardChunkMost ? kBackwardChunkMost : L;
+}
 
 // strides: batch and token strides of x, dt, z; batch, token and group strides of B, C (elements).
 inline ScanArgs scan_args(const void* x, const void* dt, const float* A, const void* Bm, const void* Cm,
