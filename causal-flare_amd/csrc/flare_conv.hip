@@ -27,7 +27,18 @@ struct ConvArgs {
     void* dx;
     float* partial;
     int64_t B, N, C, tiles;
-    int silu;
+    int silu, run;
+};
+
+// VEC elements of a row as loaded.
+template <typename E, int VEC>
+struct alignas(VEC * sizeof(E)) Raw {
+    E v[VEC];
+    __device__ __forceinline__ void load(const E* p) { *this = *reinterpret_cast<const Raw*>(p); }
+    __device__ __forceinline__ void get(float (&out)[VEC]) const {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) out[i] = to_f32(v[i]);
+    }
 };
 
 __device__ __forceinline__ int64_t row_length(const int32_t* lengths, int64_t b, int64_t N) {
@@ -43,90 +54,136 @@ __device__ __forceinline__ int tokens_back(const int32_t* ids, int64_t t, int mo
     return n;
 }
 
-// T tokens a thread; threads of neighbouring channels are neighbours.
-template <typename E, int W, int VEC, int T>
+// `run` tokens a thread; threads of neighbouring channels are neighbours.  U rows are loaded
+// while the U before them are computed: what bounds the kernel is how many bytes are under way,
+// and eight rows of four channels leave registers for seven waves a SIMD.
+template <typename E, int W, int VEC, bool DOCS>
 __global__ __launch_bounds__(256) void conv_forward_kernel(ConvArgs p) {
+    constexpr int U = 8;
+    typedef Raw<E, VEC> R;
     const int64_t groups = p.C / VEC;
     const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
     if (id >= groups * p.tiles * p.B) return;
     const int64_t c = (id % groups) * VEC, tile = id / groups % p.tiles, b = id / groups / p.tiles;
-    const int64_t t0 = tile * T, len = row_length(p.lengths, b, p.N);
+    const int t0 = (int)tile * p.run, N = (int)p.N, end = min(t0 + p.run, N);
+    const int len = (int)row_length(p.lengths, b, p.N);
     const E* x = (const E*)p.x + b * p.x_sb + c;
     const E* win = p.window ? (const E*)p.window + b * (W - 1) * p.C + c : nullptr;
-    const int32_t* ids = p.ids ? p.ids + b * p.N : nullptr;
+    const int32_t* ids = DOCS ? p.ids + b * p.N : nullptr;
     E* y = (E*)p.y + b * p.N * p.C + c;
-
-    float w[W][VEC], bias[VEC];
+    // row t of the input: those before the first token come from the window, those that are none are 0
+    auto row = [&](int t) {
+        R r = {};
+        if (t >= 0 && t < len) r.load(x + t * p.x_sn);
+        else if (t < 0 && win) r.load(win + (t + W - 1) * p.C);
+        return r;
+    };
+    R raw[U];
+    int next_id[U] = {};
+    auto fetch = [&](int u, int t) {
+        if (t >= end) return;
+        raw[u] = row(t);
+        if (DOCS) next_id[u] = ids[t];
+    };
+#pragma unroll
+    for (int u = 0; u < U; ++u) fetch(u, t0 + u);
+    float w[W][VEC], bias[VEC], in[W][VEC];                    // in[k]: the input k tokens back
+#pragma unroll
+    for (int k = 1; k < W; ++k) row(t0 - k).get(in[k - 1]);
 #pragma unroll
     for (int i = 0; i < VEC; ++i) {
         bias[i] = p.bias ? p.bias[c + i] : 0.0f;
 #pragma unroll
         for (int k = 0; k < W; ++k) w[k][i] = p.weight[(c + i) * W + W - 1 - k];
     }
-    // rows t0-W+1 .. t0+T-1 of the input; those before the first token come from the window
-    float in[T + W - 1][VEC];
+    int back = DOCS ? tokens_back(ids, t0, W - 1) - 1 : W - 1, last_id = next_id[0];
+    for (int t4 = t0; t4 < end; t4 += U) {
+        R now[U];
+        int id[U];
 #pragma unroll
-    for (int r = 0; r < T + W - 1; ++r) {
-        const int64_t t = t0 + r - (W - 1);
-        if (t >= 0 && t < len) load_row<E, VEC>(x + t * p.x_sn, in[r]);
-        else if (t < 0 && win) load_row<E, VEC>(win + (t + W - 1) * p.C, in[r]);
-        else {
-#pragma unroll
-            for (int i = 0; i < VEC; ++i) in[r][i] = 0.0f;
+        for (int u = 0; u < U; ++u) {
+            now[u] = raw[u];
+            id[u] = next_id[u];
+            fetch(u, t4 + U + u);
         }
-    }
-    int back = ids ? tokens_back(ids, t0 < p.N ? t0 : 0, W - 1) : W - 1;
 #pragma unroll
-    for (int r = 0; r < T; ++r) {
-        const int64_t t = t0 + r;
-        if (t >= p.N) break;
-        bool live = t < len;
-        if (ids) {
-            if (r) back = ids[t] == ids[t - 1] ? min(back + 1, W - 1) : 0;
-            live = ids[t] >= 0;
+        for (int u = 0; u < U; ++u) {
+            const int t = t4 + u;
+            if (t >= end) break;
+            bool live = t < len;
+            if (DOCS) {
+                back = id[u] == last_id ? min(back + 1, W - 1) : 0;
+                last_id = id[u];
+                live = last_id >= 0;
+            }
+            float out[VEC];
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) {
+#pragma unroll
+                for (int k = W - 1; k > 0; --k) in[k][i] = in[k - 1][i];
+            }
+            now[u].get(in[0]);
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) {
+                float s = bias[i];
+#pragma unroll
+                for (int k = 0; k < W; ++k) s += !DOCS || k <= back ? w[k][i] * in[k][i] : 0.0f;
+                if (p.silu) s *= sigmoid(s);
+                out[i] = live ? s : 0.0f;
+            }
+            store_row<E, VEC>(y + (int64_t)t * p.C, out);
         }
-        float out[VEC];
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-            float s = bias[i];
-#pragma unroll
-            for (int k = 0; k < W; ++k) s += k <= back ? w[k][i] * in[r + W - 1 - k][i] : 0.0f;
-            if (p.silu) s *= sigmoid(s);
-            out[i] = live ? s : 0.0f;
-        }
-        store_row<E, VEC>(y + t * p.C, out);
     }
     // the window after the last token: inputs len-W+1 .. len-1
     if (p.window_out && tile == 0) {
         E* wo = (E*)p.window_out + b * (W - 1) * p.C + c;
 #pragma unroll
         for (int r = 0; r < W - 1; ++r) {
-            const int64_t t = len - (W - 1) + r;
             float v[VEC];
-#pragma unroll
-            for (int i = 0; i < VEC; ++i) v[i] = 0.0f;
-            if (t >= 0) load_row<E, VEC>(x + t * p.x_sn, v);
-            else if (win) load_row<E, VEC>(win + (t + W - 1) * p.C, v);
+            row(len - (W - 1) + r).get(v);
             store_row<E, VEC>(wo + r * p.C, v);
         }
     }
 }
 
-// A thread walks over tokens t0 .. t0+T+W-2: the last W - 1 of them only for the dx of the ones
+// A thread walks over tokens t0 .. t0+run+W-2: the last W - 1 of them only for the dx of the ones
 // before.  It leaves its sums for dw and db in partial [B * tiles][W + 1][C].
-template <typename E, int W, int VEC, int T>
+template <typename E, int W, int VEC, bool DOCS>
 __global__ __launch_bounds__(256) void conv_backward_kernel(ConvArgs p) {
+    constexpr int U = 4;
+    typedef Raw<E, VEC> R;
     const int64_t groups = p.C / VEC;
     const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
     if (id >= groups * p.tiles * p.B) return;
     const int64_t c = (id % groups) * VEC, tile = id / groups % p.tiles, b = id / groups / p.tiles;
-    const int64_t t0 = tile * T;
+    const int t0 = (int)tile * p.run, N = (int)p.N, end = min(t0 + p.run, N), stop = min(end + W - 1, N);
     const E* x = (const E*)p.x + b * p.x_sb + c;
     const E* dy = (const E*)p.dy + b * p.N * p.C + c;
     E* dx = (E*)p.dx + b * p.N * p.C + c;
-    const int32_t* ids = p.ids ? p.ids + b * p.N : nullptr;
-
+    const int32_t* ids = DOCS ? p.ids + b * p.N : nullptr;
+    struct Rows {
+        R x, dy;
+    };
+    Rows raw[U];
+    int next_id[U] = {};
+    auto fetch = [&](int u, int t) {
+        raw[u] = {};
+        if (t >= stop) return;
+        raw[u].x.load(x + t * p.x_sn);
+        raw[u].dy.load(dy + (int64_t)t * p.C);
+        if (DOCS) next_id[u] = ids[t];
+    };
+#pragma unroll
+    for (int u = 0; u < U; ++u) fetch(u, t0 + u);
     float w[W][VEC], bias[VEC], dw[W][VEC], db[VEC];
+    // in[k]: the input k tokens back; acc[k]: the dx so far of the token k back
+    float in[W][VEC], acc[W][VEC];
+#pragma unroll
+    for (int k = 1; k < W; ++k) {
+        R r = {};
+        if (t0 - k >= 0 && (!DOCS || ids[t0 - k] >= 0)) r.load(x + (t0 - k) * p.x_sn);
+        r.get(in[k - 1]);
+    }
 #pragma unroll
     for (int i = 0; i < VEC; ++i) {
         bias[i] = p.bias ? p.bias[c + i] : 0.0f;
@@ -134,37 +191,27 @@ __global__ __launch_bounds__(256) void conv_backward_kernel(ConvArgs p) {
 #pragma unroll
         for (int k = 0; k < W; ++k) {
             w[k][i] = p.weight[(c + i) * W + W - 1 - k];
-            dw[k][i] = 0.0f;
+            dw[k][i] = acc[k][i] = 0.0f;
         }
     }
-    // in[k]: the input k tokens back; acc[k]: the dx so far of the token k back
-    float in[W][VEC], acc[W][VEC];
-#pragma unroll
-    for (int k = 0; k < W; ++k) {
-        const int64_t t = t0 - 1 - k;
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) in[k][i] = acc[k][i] = 0.0f;
-        if (k < W - 1 && t >= 0 && (!ids || ids[t] >= 0)) load_row<E, VEC>(x + t * p.x_sn, in[k]);
-    }
-    int back = ids ? tokens_back(ids, t0, W - 1) : W - 1;
-    const int64_t end = min(t0 + T, p.N), stop = min(end + W - 1, p.N);
-    // A block of U tokens at once keeps 2 U loads in flight.
-    constexpr int U = 4;
-    for (int64_t t4 = t0; t4 < end + W - 1; t4 += U) {
-        float xs[U][VEC], ds[U][VEC];
+    int back = DOCS ? tokens_back(ids, t0, W - 1) - 1 : W - 1, last_id = next_id[0];
+    for (int t4 = t0; t4 < end + W - 1; t4 += U) {
+        Rows now[U];
+        int id[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
+            now[u] = raw[u];
+            id[u] = next_id[u];
+            fetch(u, t4 + U + u);
+        }
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) xs[u][i] = ds[u][i] = 0.0f;
-            if (t4 + u < stop && (!ids || ids[t4 + u] >= 0)) {
-                load_row<E, VEC>(x + (t4 + u) * p.x_sn, xs[u]);
-                load_row<E, VEC>(dy + (t4 + u) * p.C, ds[u]);
+        for (int u = 0; u < U; ++u) {
+            const int t = t4 + u;
+            if (DOCS && t < stop) {
+                back = id[u] == last_id ? min(back + 1, W - 1) : 0;
+                last_id = id[u];
             }
-        }
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int64_t t = t4 + u;
-            if (ids && t > t0 && t < stop) back = ids[t] == ids[t - 1] ? min(back + 1, W - 1) : 0;
+            const bool live = !DOCS || last_id >= 0;       // padding's rows are 0, whatever they hold
 #pragma unroll
             for (int i = 0; i < VEC; ++i) {
 #pragma unroll
@@ -172,26 +219,32 @@ __global__ __launch_bounds__(256) void conv_backward_kernel(ConvArgs p) {
                     in[k][i] = in[k - 1][i];
                     acc[k][i] = acc[k - 1][i];
                 }
-                in[0][i] = xs[u][i];
                 acc[0][i] = 0.0f;
-                float d = ds[u][i];
+            }
+            float ds[VEC];
+            now[u].x.get(in[0]);
+            now[u].dy.get(ds);
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) {
+                if (DOCS && !live) in[0][i] = ds[i] = 0.0f;
+                float d = ds[i];
                 if (p.silu) {
                     float s = bias[i];
 #pragma unroll
-                    for (int k = 0; k < W; ++k) s += k <= back ? w[k][i] * in[k][i] : 0.0f;
+                    for (int k = 0; k < W; ++k) s += !DOCS || k <= back ? w[k][i] * in[k][i] : 0.0f;
                     const float g = sigmoid(s);
                     d *= g * (1.0f + s * (1.0f - g));
                 }
 #pragma unroll
                 for (int k = 0; k < W; ++k) {
-                    acc[k][i] += k <= back ? w[k][i] * d : 0.0f;
-                    if (t < end) dw[k][i] += k <= back ? d * in[k][i] : 0.0f;
+                    acc[k][i] += !DOCS || k <= back ? w[k][i] * d : 0.0f;
+                    if (t < end) dw[k][i] += !DOCS || k <= back ? d * in[k][i] : 0.0f;
                 }
                 if (t < end) db[i] += d;
             }
             // token t - (W-1) has all its terms
-            const int64_t done = t - (W - 1);
-            if (done >= t0 && done < end) store_row<E, VEC>(dx + done * p.C, acc[W - 1]);
+            const int done = t - (W - 1);
+            if (done >= t0 && done < end) store_row<E, VEC>(dx + (int64_t)done * p.C, acc[W - 1]);
         }
     }
     float* out = p.partial + (b * p.tiles + tile) * (W + 1) * p.C + c;
@@ -275,56 +328,54 @@ int launch_column_sums(const float* partial, int64_t R, int64_t cols, float* out
 
 constexpr int kConvBackTokens = 32;
 
+// Adjacent channels a thread takes: four where that leaves `waves` waves or more and the rows are
+// aligned to it, two where it does not, and one where rows have no such alignment.
 template <typename E>
-static bool conv_vector(const ConvArgs& p, int64_t W) {
-    constexpr int V = 16 / sizeof(E);
-    auto bad = [](const void* q) { return ((uintptr_t)q & 15) != 0; };
-    return p.C % V == 0 && p.x_sb % V == 0 && p.x_sn % V == 0 && !bad(p.x) && !bad(p.y) && !bad(p.window) &&
-           !bad(p.window_out) && !bad(p.dy) && !bad(p.dx) && !bad(p.partial);
-}
-
-template <typename E, int W, int VEC>
-static void conv_forward_go(ConvArgs p, hipStream_t stream) {
-    // Long runs read the rows before a run less often, short ones spread a small call over the
-    // GPU.
-    const int64_t lanes = p.B * (p.C / VEC);
-    auto grid = [&](int T) {
-        p.tiles = ceil_div(p.N, T);
-        return dim3((unsigned)ceil_div(lanes * p.tiles, 256));
-    };
-    if (lanes * p.N >= (int64_t)8 * 65536) {
-        const dim3 g = grid(8);
-        conv_forward_kernel<E, W, VEC, 8><<<g, 256, 0, stream>>>(p);
-    } else {
-        const dim3 g = grid(2);
-        conv_forward_kernel<E, W, VEC, 2><<<g, 256, 0, stream>>>(p);
-    }
+static int conv_vector(const ConvArgs& p, int64_t runs, int64_t waves) {
+    const uintptr_t bits = (uintptr_t)p.x | (uintptr_t)p.y | (uintptr_t)p.window | (uintptr_t)p.window_out |
+                           (uintptr_t)p.dy | (uintptr_t)p.dx |
+                           ((uintptr_t)p.C | (uintptr_t)p.x_sb | (uintptr_t)p.x_sn) * sizeof(E);
+    auto fits = [&](unsigned v) { return bits % (v * sizeof(E)) == 0 && (uintptr_t)p.partial % (v * sizeof(float)) == 0; };
+    if (fits(4) && p.B * runs * (p.C / 4) >= waves * 64) return 4;
+    return fits(2) ? 2 : 1;
 }
 
 template <typename E, int VEC>
 static int conv_forward_w(const ConvArgs& p, int64_t W, hipStream_t stream) {
-    if (W == 2) conv_forward_go<E, 2, VEC>(p, stream);
-    else if (W == 3) conv_forward_go<E, 3, VEC>(p, stream);
-    else conv_forward_go<E, 4, VEC>(p, stream);
+    const dim3 g((unsigned)ceil_div(p.B * (p.C / VEC) * p.tiles, 256));
+    auto kernel = W == 2   ? (p.ids ? conv_forward_kernel<E, 2, VEC, true> : conv_forward_kernel<E, 2, VEC, false>)
+                  : W == 3 ? (p.ids ? conv_forward_kernel<E, 3, VEC, true> : conv_forward_kernel<E, 3, VEC, false>)
+                           : (p.ids ? conv_forward_kernel<E, 4, VEC, true> : conv_forward_kernel<E, 4, VEC, false>);
+    kernel<<<g, 256, 0, stream>>>(p);
     return check_launch("conv_forward");
 }
 template <typename E>
-static int conv_forward_e(const ConvArgs& p, int64_t W, hipStream_t stream) {
-    return conv_vector<E>(p, W) ? conv_forward_w<E, 16 / sizeof(E)>(p, W, stream) : conv_forward_w<E, 1>(p, W, stream);
+static int conv_forward_e(ConvArgs p, int64_t W, hipStream_t stream) {
+    // Long runs read the W - 1 rows before a run less often, short ones spread a small call over
+    // the GPU.
+    p.run = p.B * p.N * p.C >= (int64_t)1 << 22 ? 16 : 4;
+    p.tiles = ceil_div(p.N, p.run);
+    const int v = conv_vector<E>(p, p.tiles, 2048);
+    return v == 1 ? conv_forward_w<E, 1>(p, W, stream) : v == 2 ? conv_forward_w<E, 2>(p, W, stream)
+                                                                : conv_forward_w<E, 4>(p, W, stream);
 }
 
 template <typename E, int VEC>
-static int conv_backward_w(ConvArgs p, int64_t W, hipStream_t stream) {
-    p.tiles = ceil_div(p.N, kConvBackTokens);
+static int conv_backward_w(const ConvArgs& p, int64_t W, hipStream_t stream) {
     const dim3 g((unsigned)ceil_div(p.B * (p.C / VEC) * p.tiles, 256));
-    if (W == 2) conv_backward_kernel<E, 2, VEC, kConvBackTokens><<<g, 256, 0, stream>>>(p);
-    else if (W == 3) conv_backward_kernel<E, 3, VEC, kConvBackTokens><<<g, 256, 0, stream>>>(p);
-    else conv_backward_kernel<E, 4, VEC, kConvBackTokens><<<g, 256, 0, stream>>>(p);
+    auto kernel = W == 2   ? (p.ids ? conv_backward_kernel<E, 2, VEC, true> : conv_backward_kernel<E, 2, VEC, false>)
+                  : W == 3 ? (p.ids ? conv_backward_kernel<E, 3, VEC, true> : conv_backward_kernel<E, 3, VEC, false>)
+                           : (p.ids ? conv_backward_kernel<E, 4, VEC, true> : conv_backward_kernel<E, 4, VEC, false>);
+    kernel<<<g, 256, 0, stream>>>(p);
     return check_launch("conv_backward");
 }
 template <typename E>
-static int conv_backward_e(const ConvArgs& p, int64_t W, hipStream_t stream) {
-    return conv_vector<E>(p, W) ? conv_backward_w<E, 16 / sizeof(E)>(p, W, stream) : conv_backward_w<E, 1>(p, W, stream);
+static int conv_backward_e(ConvArgs p, int64_t W, hipStream_t stream) {
+    p.run = kConvBackTokens;
+    p.tiles = ceil_div(p.N, p.run);
+    const int v = conv_vector<E>(p, p.tiles, 4096);
+    return v == 1 ? conv_backward_w<E, 1>(p, W, stream) : v == 2 ? conv_backward_w<E, 2>(p, W, stream)
+                                                                 : conv_backward_w<E, 4>(p, W, stream);
 }
 
 template <typename E, int VEC>
@@ -337,8 +388,7 @@ static int conv_step_w(const ConvArgs& p, int64_t W, const int32_t* mask, hipStr
 }
 template <typename E>
 static int conv_step_e(const ConvArgs& p, int64_t W, const int32_t* mask, hipStream_t stream) {
-    return conv_vector<E>(p, W) ? conv_step_w<E, 16 / sizeof(E)>(p, W, mask, stream)
-                                : conv_step_w<E, 1>(p, W, mask, stream);
+    return conv_vector<E>(p, 1, 512) == 1 ? conv_step_w<E, 1>(p, W, mask, stream) : conv_step_w<E, 2>(p, W, mask, stream);
 }
 
 static size_t conv_backward_bytes(int64_t B, int64_t N, int64_t C, int64_t W) {
@@ -355,7 +405,7 @@ using namespace flare::mix;
     FLARE_REQUIRE(known_dtype(dtype), name ": unknown dtype %d", dtype);                                     \
     FLARE_REQUIRE(B >= 1 && N >= 1 && C >= 1, name ": B, N and C must be positive");                         \
     FLARE_REQUIRE(W >= 2 && W <= 4, name ": W must be 2, 3 or 4, got %lld", (long long)W);                   \
-    FLARE_REQUIRE(B <= INT32_MAX && N <= INT32_MAX && C <= (1 << 20) && B * N <= ((int64_t)1 << 38) / C,      \
+    FLARE_REQUIRE(B <= INT32_MAX && N <= (1 << 30) && C <= (1 << 20) && B * N <= ((int64_t)1 << 38) / C,      \
                   name ": too large")
 
 extern "C" int flare_conv_forward(const void* x, int64_t x_stride_b, int64_t x_stride_n, const float* weight,
