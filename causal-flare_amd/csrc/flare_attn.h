@@ -54,6 +54,7 @@ struct AttnArgs {
     const float* slopes;             // [H]
     const int32_t *ids, *prefix;     // [B, N], [B]
     const int32_t* id_stats;         // [B, tiles, 3]: smallest and largest id of 64 tokens, whether they have just one
+    const int32_t *order, *key_order;    // blocks of queries and of keys, the costliest first (or NULL)
     const int32_t *lengths, *fresh;  // [B]: tokens in the cache before these, and how many of these are real
     int64_t B, N, M, H, G, D;        // M: rows of k and v
     float scale, cap;
@@ -70,6 +71,8 @@ struct AttnArgs {
     int64_t splits;
 };
 
+// Tiles of 16 queries a wave of the forward's and the query gradients' kernels owns.
+constexpr int q_tiles(int size) { return size == 2 ? 2 : 1; }
 // Tiles of 16 keys a wave of the key gradients' kernel owns.
 constexpr int kv_tiles(int size, int DP) { return size == 2 && DP <= 64 ? 2 : 1; }
 
@@ -266,6 +269,22 @@ __device__ __forceinline__ IdRange id_block(const AttnArgs& p, int64_t b, int fi
     }
     return r;
 }
+
+// Which queries a workgroup takes: `id` without its key head.  In the order given, or, by length
+// alone, the last rows first.
+struct QueryBlock {
+    int64_t b;
+    int rep, tile;
+    __device__ __forceinline__ QueryBlock(const AttnArgs& p, int id, int R, int tiles) {
+        if (p.order) {
+            const int o = p.order[id / R];
+            rep = id % R, b = o / tiles, tile = o % tiles;
+        } else {
+            const int B = (int)p.B;
+            b = id % B, rep = id / B % R, tile = tiles - 1 - id / B / R;
+        }
+    }
+};
 
 // The tiles of STEP tokens in [begin, end) whose ids meet `mine`, in order; all of them without
 // ids.  64 tiles are looked at in one go, so every lane of the wave has to take part.

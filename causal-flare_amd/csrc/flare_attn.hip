@@ -27,6 +27,41 @@ __global__ __launch_bounds__(64) void attn_ids_kernel(const int32_t* ids, int64_
     }
 }
 
+// What each block of `rows` queries (blockIdx.y 0) or `key_rows` keys (1) costs: the tiles of ids it
+// meets.  A wave a block.
+__global__ __launch_bounds__(64) void attn_costs_kernel(AttnArgs p, int rows, int key_rows, int32_t* costs, int32_t* key_costs) {
+    const bool keys = blockIdx.y != 0;
+    const int n = keys ? key_rows : rows, tiles = ((int)p.N + n - 1) / n;
+    if ((int64_t)blockIdx.x >= p.B * tiles) return;
+    const int b = blockIdx.x / tiles, first = blockIdx.x % tiles * n, all = id_tiles(p.N);
+    const IdRange mine = id_block(p, b, first, n);
+    const int from = p.causal && keys ? first / kIdTile : 0;
+    const int to = p.causal && !keys ? min(all, (first + n + kIdTile - 1) / kIdTile) : all;
+    int cost = 0;
+    for (int t = from; t < to; t += 64) {
+        const int at = t + threadIdx.x;
+        cost += __popcll(__ballot(at < to && id_range(p, b, at).meets(mine)));
+    }
+    if (threadIdx.x == 0) (keys ? key_costs : costs)[blockIdx.x] = cost;
+}
+
+constexpr int kMostOrdered = 2048;
+
+// Blocks in falling order of cost, those of one cost as they stand.
+__global__ __launch_bounds__(1024) void attn_order_kernel(const int32_t* costs, int n, int32_t* order, const int32_t* key_costs,
+                                                          int key_n, int32_t* key_order) {
+    __shared__ int c[kMostOrdered];
+    if (blockIdx.x) costs = key_costs, n = key_n, order = key_order;
+    for (int i = threadIdx.x; i < n; i += 1024) c[i] = costs[i];
+    __syncthreads();
+    for (int i = threadIdx.x; i < n; i += 1024) {
+        const int mine = c[i];
+        int rank = 0;
+        for (int j = 0; j < n; ++j) rank += c[j] > mine || (c[j] == mine && j < i);
+        order[rank] = i;
+    }
+}
+
 // New keys and values to their place behind what each sequence's cache holds.  Nothing of a
 // sequence that does not fit.
 __global__ __launch_bounds__(256) void attn_append_kernel(Rows k, Rows v, const int32_t* lengths, const int32_t* fresh,
@@ -44,20 +79,44 @@ __global__ __launch_bounds__(256) void attn_append_kernel(Rows k, Rows v, const 
         *reinterpret_cast<const u32x4*>((const char*)v.p + (b * v.sb + t * v.sn + g * v.sh) * size + at);
 }
 
-static size_t stats_bytes(int64_t B, int64_t N) { return (size_t)(B * ceil_div(N, kIdTile) * 3) * sizeof(int32_t); }
+static int rows_of_queries(int dtype) { return 64 * q_tiles(dtype == FLARE_F32 ? 4 : 2); }
+static int rows_of_keys(int dtype, int64_t D) {
+    return 64 * kv_tiles(dtype == FLARE_F32 ? 4 : 2, (int)ceil_div(D, 32) * 32);
+}
+// Of the id statistics, and of two costs and orders.
+static size_t stats_bytes(int64_t B, int64_t N) {
+    return (size_t)(B * ceil_div(N, kIdTile) * 3 + 4 * kMostOrdered) * sizeof(int32_t);
+}
 
-static int launch_ids(AttnArgs& p, int32_t* stats, hipStream_t stream) {
+// Documents make blocks cost very different amounts of work, so that the costly ones have to start
+// first; that takes two small launches (some 10 us), and pays where there are more workgroups
+// than run at once (512).  Of 16384 tokens in six documents, 16 heads of 128 over 4, the forward
+// ran 580 us in the rows' order.
+static int launch_ids(AttnArgs& p, int dtype, bool keys, int32_t* stats, hipStream_t stream) {
     if (!p.ids) return FLARE_OK;
-    attn_ids_kernel<<<dim3((unsigned)ceil_div(p.N, kIdTile), (unsigned)p.B), 64, 0, stream>>>(p.ids, p.N, stats);
+    const int tiles = (int)ceil_div(p.N, kIdTile);
+    attn_ids_kernel<<<dim3((unsigned)tiles, (unsigned)p.B), 64, 0, stream>>>(p.ids, p.N, stats);
     p.id_stats = stats;
-    return check_launch("attn_ids");
+    int rc = check_launch("attn_ids");
+    const int rows = rows_of_queries(dtype), key_rows = rows_of_keys(dtype, p.D);
+    const int64_t n = p.B * ceil_div(p.N, rows), key_n = keys ? p.B * ceil_div(p.N, key_rows) : 0;
+    if (rc != FLARE_OK || n * p.H <= 512 || n > kMostOrdered || key_n > kMostOrdered) return rc;
+    int32_t* at = stats + p.B * tiles * 3;
+    attn_costs_kernel<<<dim3((unsigned)(n > key_n ? n : key_n), keys ? 2 : 1), 64, 0, stream>>>(p, rows, key_rows, at,
+                                                                                             at + kMostOrdered);
+    if ((rc = check_launch("attn_costs")) != FLARE_OK) return rc;
+    attn_order_kernel<<<dim3(keys ? 2 : 1), 1024, 0, stream>>>(at, (int)n, at + 2 * kMostOrdered, at + kMostOrdered, (int)key_n,
+                                                               at + 3 * kMostOrdered);
+    p.order = at + 2 * kMostOrdered;
+    p.key_order = keys ? at + 3 * kMostOrdered : nullptr;
+    return check_launch("attn_order");
 }
 
 // Parts that the queries of each block of keys are split into: so many that there are 2048
 // workgroups (eight a CU: blocks of keys cost very different amounts of work under a causal or
 // document mask), the heads first and then the rows, in parts of 256 or more.
 static void split_backward(AttnArgs& p, int dtype) {
-    const int64_t DP = ceil_div(p.D, 32) * 32, blocks = ceil_div(p.N, 64 * kv_tiles(dtype == FLARE_F32 ? 4 : 2, (int)DP));
+    const int64_t blocks = ceil_div(p.N, rows_of_keys(dtype, p.D));
     const int64_t R = p.H / p.G;
     int64_t want = ceil_div(2048, blocks * p.B * p.G);
     want = want > 8 ? 8 : want;
@@ -128,7 +187,7 @@ extern "C" int flare_attn_forward(const void* q, const void* k, const void* v, c
         set_error("flare_attn_forward: workspace of %zu bytes is too small", workspace_bytes);
         return FLARE_ERR_WORKSPACE;
     }
-    const int rc = launch_ids(p, (int32_t*)workspace, (hipStream_t)stream);
+    const int rc = launch_ids(p, dtype, false, (int32_t*)workspace, (hipStream_t)stream);
     if (rc != FLARE_OK) return rc;
     return FLARE_BY_DTYPE(dtype, forward_e, (p, (hipStream_t)stream));
 }
@@ -168,7 +227,7 @@ extern "C" int flare_attn_backward(const void* q, const void* k, const void* v, 
     p.dq = dq, p.dk = dk, p.dv = dv;
     split_backward(p, dtype);
     p.parts = (float*)((char*)workspace + backward_head_bytes(B, N, H));
-    const int rc = launch_ids(p, (int32_t*)(delta + B * H * N), (hipStream_t)stream);
+    const int rc = launch_ids(p, dtype, true, (int32_t*)(delta + B * H * N), (hipStream_t)stream);
     if (rc != FLARE_OK) return rc;
     return FLARE_BY_DTYPE(dtype, backward_e, (p, delta, (hipStream_t)stream));
 }

@@ -72,9 +72,9 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnArgs p) {
     int id = blockIdx.x;
     const int kvh = id % (int)p.G;
     id /= (int)p.G;
-    const int64_t b = id % (int)p.B;
-    id /= (int)p.B;
-    const int h = kvh * R + id % R, q0 = (nq - 1 - id / R) * QB;
+    const QueryBlock at(p, id, R, nq);
+    const int64_t b = at.b;
+    const int h = kvh * R + at.rep, q0 = at.tile * QB;
 
     const int prefix = p.prefix ? (int)clamp_to(p.prefix[b], p.N) : 0;
     const int kv_end = p.causal ? max(min(q0 + QB, N), prefix) : N;
@@ -269,10 +269,16 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(AttnArgs p) {
     int id = blockIdx.x;
     const int kvh = id % (int)p.G;
     id /= (int)p.G;
-    const int64_t b = id % (int)p.B;
-    id /= (int)p.B;
-    // this workgroup's part of the queries: some of the heads that share these keys, some of the rows
-    const int part = id % parts, kb = id / parts * KB;               // the keys most queries see come first
+    // this workgroup's part of the queries: some of the heads that share these keys, some of the
+    // rows; by length alone the keys most queries see come first
+    int64_t b;
+    int part, kb;
+    if (p.key_order) {
+        const int tiles = (N + KB - 1) / KB, o = p.key_order[id / parts];
+        part = id % parts, b = o / tiles, kb = o % tiles * KB;
+    } else {
+        b = id % (int)p.B, part = id / (int)p.B % parts, kb = id / (int)p.B / parts * KB;
+    }
     const int rep0 = part / row_parts * R / (parts / row_parts);
     const int rep1 = (part / row_parts + 1) * R / (parts / row_parts);
 
@@ -507,7 +513,7 @@ static int allow_lds(K kernel, size_t bytes, const char* what) {
 
 template <typename E, int DP, bool CAP>
 static int backward_cap(const AttnArgs& p, hipStream_t stream) {
-    constexpr int QT = sizeof(E) == 2 ? 2 : 1;
+    constexpr int QT = q_tiles(sizeof(E));
     constexpr size_t bytes = BackwardLds<E, DP>::bytes;
     auto dq = attn_dq_kernel<E, DP, QT, CAP>;
     constexpr int KQ = kv_tiles(sizeof(E), DP);

@@ -47,9 +47,9 @@ __global__ __launch_bounds__(256, 2) void attn_forward_kernel(AttnArgs p) {
     int id = blockIdx.x;
     const int kvh = id % (int)p.G;
     id /= (int)p.G;
-    const int64_t b = id % (int)p.B;
-    id /= (int)p.B;
-    const int h = kvh * R + id % R, q0 = (nq - 1 - id / R) * QB;
+    const QueryBlock at(p, id, R, nq);
+    const int64_t b = at.b;
+    const int h = kvh * R + at.rep, q0 = at.tile * QB;
 
     int off = 0, qlen = (int)p.N, kvlen = (int)p.M;
     bool refused = false;
@@ -313,7 +313,7 @@ __global__ __launch_bounds__(256, 2) void attn_forward_kernel(AttnArgs p) {
 
 template <typename E, int DP, int CAP>
 static int forward_cap(const AttnArgs& p, hipStream_t stream) {
-    constexpr int QT = sizeof(E) == 2 ? 2 : 1, KT = sizeof(E) == 2 ? 64 : 32;
+    constexpr int QT = q_tiles(sizeof(E)), KT = sizeof(E) == 2 ? 64 : 32;
     constexpr size_t bytes = ForwardLds<E, DP, KT>::bytes;
     auto kernel = attn_forward_kernel<E, DP, QT, KT, CAP>;
     if (bytes > 65536) {

@@ -308,6 +308,23 @@ def test_attention(dtype, B, N, H, G, D, what):
         close_attention(got, ref[n], n, dtype)
 
 
+@pytest.mark.parametrize("dtype, B, N, H, G", [(BF16, 34, 150, 16, 4), (F32, 20, 130, 16, 16), (F16, 36, 129, 16, 1)])
+def test_attention_of_many_documents_in_order_of_cost(dtype, B, N, H, G):
+    """More workgroups than run at once: blocks start in the order of what they cost."""
+    g = gen(N)
+    D = 32
+    q, k, v, dy = (normal(g, B, N, n, D, dtype=dtype) for n in (H, G, G, H))
+    ids = documents(g, B, N)
+    leaves = [t.clone().requires_grad_() for t in (q, k, v)]
+    y = cf.softmax_attention(*leaves, document_ids=ids)
+    grads = torch.autograd.grad(y, leaves, dy)
+    unit, tiny = (0.0 if dtype is F32 else U[dtype]), (2.0 ** -25 if dtype is F16 else 0.0)
+    ref = attention(q, k, v, ids=ids, dy=dy, unit=unit, tiny=tiny)
+    close_attention(y, ref["y"], "y", dtype)
+    for n, got in zip(("dq", "dk", "dv"), grads):
+        close_attention(got, ref[n], n, dtype)
+
+
 @pytest.mark.parametrize("dtype", [F32, BF16, F16])
 @pytest.mark.parametrize("B, T, H, G, D, S, what", [
     (4, 1, 2, 1, 64, 70, ""), (5, 7, 4, 2, 128, 200, "cap"), (5, 130, 2, 2, 48, 400, "slopes"),
