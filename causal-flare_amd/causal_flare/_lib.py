@@ -166,7 +166,7 @@ def _declare(lib):
     lib.flare_scan_step.restype = _i
     lib.flare_scan_step.argtypes = [_vp] * 8 + [_i, _i] + [_i64] * 4 + [_vp] * 5
     lib.flare_attn_forward_workspace_size.restype = _sz
-    lib.flare_attn_forward_workspace_size.argtypes = [_i64] * 2
+    lib.flare_attn_forward_workspace_size.argtypes = [_i64] * 5 + [_i]
     lib.flare_attn_forward.restype = _i
     lib.flare_attn_forward.argtypes = ([_vp] * 4 + [_i] + [_i64] * 6 + [_f, _f, _vp, _i] + [_vp] * 6
                                        + [_vp, _sz, _vp])

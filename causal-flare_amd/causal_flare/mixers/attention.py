@@ -106,10 +106,8 @@ class SoftmaxAttention(autograd.Function):
         y = torch.empty((B, N, H, D), device=Q.device, dtype=dtype)
         lse = torch.empty((B, H, N), device=Q.device, dtype=torch.float32) if training else None
         lib = _lib.lib()
-        ws, nbytes = None, 0
-        if ids is not None:
-            nbytes = lib.flare_attn_forward_workspace_size(B, N)
-            ws = torch.empty(nbytes, device=Q.device, dtype=torch.uint8)
+        nbytes = lib.flare_attn_forward_workspace_size(B, N, N, H, D, _lib.dtype_code(dtype))
+        ws = torch.empty(nbytes, device=Q.device, dtype=torch.uint8)
         P = _lib.ptr
         with _on(Q.device):
             rc = lib.flare_attn_forward(
@@ -214,6 +212,8 @@ def softmax_attention_prefill(
     q, k, v = (_aligned_rows(t, kc.dtype) for t in (Q, K, V))
     sl, pre, lens, new = _f32(slopes), _int32(prefix_lengths), _int32(lengths), _int32(new_lengths)
     lib, P = _lib.lib(), _lib.ptr
+    nbytes = lib.flare_attn_forward_workspace_size(B, T, S, H, D, code)
+    ws = torch.empty(nbytes, device=device, dtype=torch.uint8)
     with _on(device):
         stream = _lib.stream_of(device)
         rc = lib.flare_attn_append(P(k), P(v), _strides(*k.stride()[:3], *v.stride()[:3]), code, B, T, S, G, D, P(lens),
@@ -221,7 +221,8 @@ def softmax_attention_prefill(
         _lib.check(rc, "flare_attn_append")
         rc = lib.flare_attn_forward(
             P(q), P(kc), P(vc), _strides(*q.stride()[:3], *kc.stride()[:3], *vc.stride()[:3]), code, B, T, S, H, G, D,
-            _resolve_attn_scale(scale, D), cap, P(sl), 1, None, P(pre), P(lens), P(new), P(y), None, None, 0, stream)
+            _resolve_attn_scale(scale, D), cap, P(sl), 1, None, P(pre), P(lens), P(new), P(y), None, P(ws), nbytes,
+            stream)
     _lib.check(rc, "flare_attn_forward")
     return y, cache
 

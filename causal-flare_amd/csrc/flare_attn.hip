@@ -128,6 +128,18 @@ static size_t parts_bytes(const AttnArgs& p) {
     return p.splits == 1 ? 0 : (size_t)(p.splits * 2 * p.B * p.N * p.G * p.D) * sizeof(float);
 }
 
+// Parts that a row's keys are split into in the forward: two workgroups a CU (512) where the rows
+// leave less than that, in parts of 512 keys or more.
+static void split_forward(AttnArgs& p, int dtype) {
+    const int64_t blocks = ceil_div(p.N, rows_of_queries(dtype)) * p.B * p.H, want = ceil_div(512, blocks);
+    const int64_t most = ceil_div(p.M, 512);
+    p.splits = want < most ? want : most;
+}
+static size_t forward_head_bytes(int64_t B, int64_t N) { return (stats_bytes(B, N) + 255) / 256 * 256; }
+static size_t rows_bytes(const AttnArgs& p) {
+    return p.splits == 1 ? 0 : (size_t)(p.B * p.H * p.N * p.splits * (p.D + 4)) * sizeof(float);
+}
+
 static bool aligned(const Rows& r, int dtype) {
     const int64_t per = dtype == FLARE_F32 ? 4 : 8;
     return ((uintptr_t)r.p & 15) == 0 && r.sb % per == 0 && r.sn % per == 0 && r.sh % per == 0 && r.sn >= 0 &&
@@ -154,7 +166,7 @@ using namespace flare::attn;
     FLARE_REQUIRE(D >= 16 && D <= 128 && D % 16 == 0, name ": head dimension %lld is not a multiple of 16 up to " \
                   "128", (long long)D);                                                                           \
     FLARE_REQUIRE(N <= (1 << 30) && M <= (1 << 30) && B <= 65535 && H <= 65535 && B * H <= (1 << 24) &&           \
-                  (N + 63) / 64 * B * H <= INT32_MAX && H * D < kMostStride, name ": too large");                                        \
+                  (N + 63) / 64 * B * H <= (1 << 26) && H * D < kMostStride, name ": too large");                                        \
     FLARE_REQUIRE(softcap >= 0.0f && softcap < __builtin_huge_valf(), name ": the cap must be finite and not negative")
 
 static AttnArgs attn_args(const void* q, const void* k, const void* v, const int64_t* st, int64_t B, int64_t N,
@@ -166,7 +178,13 @@ static AttnArgs attn_args(const void* q, const void* k, const void* v, const int
     return p;
 }
 
-extern "C" size_t flare_attn_forward_workspace_size(int64_t B, int64_t N) { return stats_bytes(B, N); }
+extern "C" size_t flare_attn_forward_workspace_size(int64_t B, int64_t N, int64_t M, int64_t H, int64_t D, int dtype) {
+    if (B < 1 || N < 1 || M < 1 || H < 1) return 0;
+    AttnArgs p = {};
+    p.B = B, p.N = N, p.M = M, p.H = H, p.D = D;
+    split_forward(p, dtype);
+    return forward_head_bytes(B, N) + rows_bytes(p);
+}
 
 extern "C" int flare_attn_forward(const void* q, const void* k, const void* v, const int64_t* strides, int dtype,
                                   int64_t B, int64_t N, int64_t M, int64_t H, int64_t G, int64_t D, float scale,
@@ -183,8 +201,10 @@ extern "C" int flare_attn_forward(const void* q, const void* k, const void* v, c
                   "flare_attn_forward: rows must be 16-byte aligned and less than 2^22 elements apart");
     p.causal = causal, p.ids = document_ids, p.prefix = prefix_lengths, p.lengths = lengths, p.fresh = new_lengths;
     p.y = y, p.lse = lse;
-    if (document_ids && (!workspace || workspace_bytes < stats_bytes(B, N))) {
-        set_error("flare_attn_forward: workspace of %zu bytes is too small", workspace_bytes);
+    split_forward(p, dtype);
+    p.parts = (float*)((char*)workspace + forward_head_bytes(B, N));
+    if (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < forward_head_bytes(B, N) + rows_bytes(p)) {
+        set_error("flare_attn_forward: workspace of %zu bytes is too small or not 16-byte aligned", workspace_bytes);
         return FLARE_ERR_WORKSPACE;
     }
     const int rc = launch_ids(p, dtype, false, (int32_t*)workspace, (hipStream_t)stream);

@@ -4,7 +4,8 @@
 // operand in registers; K and V come through LDS in tiles of KT keys, two of each, the next
 // one's loads in flight while one is computed.  The running maximum moves only when a score
 // passes it by 2^8, so that most tiles rescale nothing.  Weights are rounded to the inputs' type
-// for the product with V (their sum is taken before that, in fp32).
+// for the product with V (their sum is taken before that, in fp32).  Where there are few rows the
+// keys are split over `splits` workgroups, whose shares attn_rows joins.
 #pragma once
 
 #include "flare_attn.h"
@@ -47,6 +48,8 @@ __global__ __launch_bounds__(256, 2) void attn_forward_kernel(AttnArgs p) {
     int id = blockIdx.x;
     const int kvh = id % (int)p.G;
     id /= (int)p.G;
+    const int parts = (int)p.splits, part = id % parts;            // of the keys
+    id /= parts;
     const QueryBlock at(p, id, R, nq);
     const int64_t b = at.b;
     const int h = kvh * R + at.rep, q0 = at.tile * QB;
@@ -66,6 +69,12 @@ __global__ __launch_bounds__(256, 2) void attn_forward_kernel(AttnArgs p) {
     if (q0 < qlen) {
         kv_end = kvlen;
         if (p.causal) kv_end = min(kvlen, max(off + min(q0 + QB, qlen), prefix));
+    }
+    int k_begin = 0;
+    if (parts > 1) {
+        const int tiles = (kv_end + KT - 1) / KT;
+        k_begin = tiles * part / parts * KT;
+        kv_end = min(kv_end, tiles * (part + 1) / parts * KT);
     }
     IdRange mine{0, 0, true};
     if (p.ids) mine = id_block(p, b, q0, QB);
@@ -137,7 +146,7 @@ __global__ __launch_bounds__(256, 2) void attn_forward_kernel(AttnArgs p) {
     };
 
     TileWalk<KT> walk(p, b, kv_end, mine);
-    int k0 = walk.next(0);
+    int k0 = walk.next(k_begin);
     int buf = 0;
     if (tid == 0) *oddl = 0;
     __syncthreads();
@@ -270,7 +279,7 @@ __global__ __launch_bounds__(256, 2) void attn_forward_kernel(AttnArgs p) {
     if (*oddl) {
         // the infinite values and NaNs that a query does see, from memory
         TileWalk<KT> again(p, b, kv_end, mine);
-        for (k0 = again.next(0); k0 < kv_end; k0 = again.next(k0 + KT)) {
+        for (k0 = again.next(k_begin); k0 < kv_end; k0 = again.next(k0 + KT)) {
             if (covers(k0, q0, q0 + QB - 1)) continue;
             for (int j = k0; j < min(k0 + KT, kvlen); ++j) {
 #pragma unroll
@@ -296,6 +305,17 @@ __global__ __launch_bounds__(256, 2) void attn_forward_kernel(AttnArgs p) {
         const float total = column_sum(sum[t]);
         const float inv = total == 0.0f ? 0.0f : 1.0f / total;
         if (i >= p.N) continue;
+        if (parts > 1) {
+            float* to = p.parts + (((b * p.H + h) * p.N + i) * parts + part) * (p.D + 4);
+#pragma unroll
+            for (int d = 0; d < DT; ++d)
+                if (16 * d < p.D) *reinterpret_cast<f32x4*>(to + 16 * d + 4 * g) = acc[t][d];
+            if (g == 0) {
+                to[p.D] = top[t];
+                to[p.D + 1] = total;
+            }
+            continue;
+        }
         if (p.lse && g == 0)
             p.lse[(b * p.H + h) * p.N + i] = total == 0.0f ? -kNegInf : top[t] + __builtin_amdgcn_logf(total);
         S* row = (S*)p.y + ((b * p.N + i) * p.H + h) * p.D;
@@ -311,6 +331,34 @@ __global__ __launch_bounds__(256, 2) void attn_forward_kernel(AttnArgs p) {
     }
 }
 
+// What the parts of each row leave, joined: 32 lanes a row, four dimensions a lane.
+template <typename E>
+__global__ __launch_bounds__(256) void attn_rows_kernel(AttnArgs p) {
+    typedef typename Elem<E>::S S;
+    typedef S S4 __attribute__((ext_vector_type(4)));
+    const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);             // (b, h, i)
+    const int d = (threadIdx.x & 31) * 4;
+    if (row >= p.B * p.H * p.N || d >= p.D) return;
+    const int64_t i = row % p.N, h = row / p.N % p.H, b = row / p.N / p.H;
+    const float* part = p.parts + row * p.splits * (p.D + 4);
+    float top = kNegInf, total = 0.0f;
+    f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int64_t s = 0; s < p.splits; ++s) top = fmaxf(top, part[s * (p.D + 4) + p.D]);
+    for (int64_t s = 0; s < p.splits; ++s) {
+        const float* q = part + s * (p.D + 4);
+        const float f = q[p.D] == top ? 1.0f : __builtin_amdgcn_exp2f(q[p.D] - top);
+        total += q[p.D + 1] * f;
+        v += *reinterpret_cast<const f32x4*>(q + d) * f;
+    }
+    v *= total == 0.0f ? 0.0f : 1.0f / total;
+    if (p.lengths) {
+        const int64_t off = p.lengths[b], n = p.fresh ? clamp_to(p.fresh[b], p.N) : p.N;
+        if (off >= 0 && off + n > p.M) v = f32x4{__builtin_nanf(""), __builtin_nanf(""), __builtin_nanf(""), __builtin_nanf("")};
+    }
+    *reinterpret_cast<S4*>((S*)p.y + ((b * p.N + i) * p.H + h) * p.D + d) = __builtin_convertvector(v, S4);
+    if (p.lse && d == 0) p.lse[row] = total == 0.0f ? -kNegInf : top + __builtin_amdgcn_logf(total);
+}
+
 template <typename E, int DP, int CAP>
 static int forward_cap(const AttnArgs& p, hipStream_t stream) {
     constexpr int QT = q_tiles(sizeof(E)), KT = sizeof(E) == 2 ? 64 : 32;
@@ -324,9 +372,12 @@ static int forward_cap(const AttnArgs& p, hipStream_t stream) {
             return FLARE_ERR_LAUNCH;
         }
     }
-    const int64_t blocks = ceil_div(p.N, 64 * QT) * p.H * p.B;
+    const int64_t blocks = ceil_div(p.N, 64 * QT) * p.H * p.B * p.splits;
     kernel<<<dim3((unsigned)blocks), 256, bytes, stream>>>(p);
-    return check_launch("attn_forward");
+    const int rc = check_launch("attn_forward");
+    if (rc != FLARE_OK || p.splits == 1) return rc;
+    attn_rows_kernel<E><<<dim3((unsigned)ceil_div(p.B * p.H * p.N, 8)), 256, 0, stream>>>(p);
+    return check_launch("attn_rows");
 }
 template <typename E, int DP>
 static int forward_dp(const AttnArgs& p, hipStream_t stream) {

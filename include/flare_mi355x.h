@@ -394,11 +394,11 @@ int flare_scan_step(const void* x, const void* dt, const float* A, const void* B
  * those below prefix_lengths[b] (or NULL).  Without `lengths` M == N.  With them k and v are
  * caches of M rows, the queries are at positions lengths[b] + i, and new_lengths[b] of them (all
  * if NULL) are real, whose keys are in the caches already (flare_attn_append); lengths[b] < 0: y =
- * 0; lengths[b] + new_lengths[b] > M: y is NaN.  document_ids exclude lengths and need the
- * workspace.  A query that sees nothing has y = 0.  lse [B, H, N] or NULL receives log2 of the sum
+ * 0; lengths[b] + new_lengths[b] > M: y is NaN.  document_ids exclude lengths.
+ * A query that sees nothing has y = 0.  lse [B, H, N] or NULL receives log2 of the sum
  * of exp(s_ij).
  */
-size_t flare_attn_forward_workspace_size(int64_t B, int64_t N);
+size_t flare_attn_forward_workspace_size(int64_t B, int64_t N, int64_t M, int64_t H, int64_t D, int dtype);
 int flare_attn_forward(const void* q, const void* k, const void* v, const int64_t* strides, int dtype, int64_t B,
                        int64_t N, int64_t M, int64_t H, int64_t G, int64_t D, float scale, float softcap,
                        const float* slopes, int causal, const int32_t* document_ids,

@@ -258,7 +258,7 @@ ATTENTION = [
     (1, 64, 4, 1, 64, "cap slopes"), (2, 65, 2, 2, 80, "full"), (2, 130, 4, 2, 96, "prefix"),
     (3, 200, 3, 1, 128, "docs slopes"), (2, 257, 2, 1, 128, "cap docs prefix"), (1, 191, 2, 2, 112, "full docs slopes"),
     (2, 300, 1, 1, 64, "prefix slopes"), (1, 513, 2, 2, 64, "docs"), (1, 100, 2, 1, 64, "negative"),
-    (1, 140, 2, 2, 128, "wide-cap slopes negative"),
+    (1, 140, 2, 2, 128, "wide-cap slopes negative"), (1, 1100, 1, 1, 32, "docs slopes"), (1, 1537, 2, 1, 48, "cap"),
 ]
 
 
@@ -328,7 +328,8 @@ def test_attention_of_many_documents_in_order_of_cost(dtype, B, N, H, G):
 @pytest.mark.parametrize("dtype", [F32, BF16, F16])
 @pytest.mark.parametrize("B, T, H, G, D, S, what", [
     (4, 1, 2, 1, 64, 70, ""), (5, 7, 4, 2, 128, 200, "cap"), (5, 130, 2, 2, 48, 400, "slopes"),
-    (5, 150, 4, 1, 96, 300, "prefix slopes"), (5, 64, 2, 2, 32, 129, "prefix")])
+    (5, 150, 4, 1, 96, 300, "prefix slopes"), (5, 64, 2, 2, 32, 129, "prefix"),
+    (5, 3, 4, 2, 64, 2500, "slopes"), (3, 140, 2, 1, 128, 1300, "cap prefix"), (5, 1, 1, 1, 16, 1100, "wide-cap")])
 def test_attention_prefill(dtype, B, T, H, G, D, S, what):
     g = gen(T + D)
     q, k, v = (normal(g, B, T, n, D, dtype=dtype) for n in (H, G, G))

@@ -133,6 +133,8 @@ def test_c_entry_points_check_before_they_launch():
                                            None, None, None, P, None, None, 0, None), b"16-byte")
     assert lib.flare_attn_forward(*attn, 1, 4, 4, 4, 4, 64, 1.0, 0.0, None, 1, P, None, None, None, P, None, None, 0,
                                   None) == -3
+    assert lib.flare_attn_forward(*attn, 1, 4000, 4000, 1, 1, 64, 1.0, 0.0, None, 1, None, None, None, None, P, None, P, 4096,
+                                  None) == -3
     assert lib.flare_attn_backward(*attn, 1, 4, 4, 4, 64, 1.0, 0.0, None, 1, None, None, P, P, P, P, P, P, P, 0, None) == -3
     assert _refused(lib.flare_attn_append(P, P, six, 1, 1, 4, 8, 4, 64, None, None, P, P, None), b"null pointer")
     assert lib.flare_attn_step(P, P, P, six, 1, 1, 4096, 4, 4, 64, 1.0, 0.0, None, P, P, P, P, None, 0, None) == -3
