@@ -67,21 +67,22 @@ def _row_mask(name, mask, B, device):
 
 
 def _rows(t, dtype):
-    """`t` in `dtype` with its last dimension adjacent in memory; other strides stay."""
+    """`t` [B, n, ..] in `dtype` with its last dimension adjacent in memory, and tokens less than 2^22
+    elements apart; other strides stay."""
     if t is None:
         return None
     if t.dtype is not dtype:
         t = t.detach().to(dtype)
-    return t if t.shape[-1] <= 1 or t.stride(-1) == 1 else t.detach().contiguous()
+    if (t.shape[-1] <= 1 or t.stride(-1) == 1) and t.stride(1) < 1 << 22:
+        return t
+    return t.detach().clone(memory_format=torch.contiguous_format)
 
 
 def _aligned_rows(t, dtype):
-    """`_rows` of a [B, n, heads, D] tensor with every row on a 16-byte boundary, and tokens less than
-    2^22 elements apart."""
+    """`_rows` with every row on a 16-byte boundary."""
     t = _rows(t, dtype)
     size = t.element_size()
-    if (t.data_ptr() % 16 or any(s * size % 16 for s in t.stride()[:-1]) or t.stride(-1) != 1
-            or t.stride(1) >= 1 << 22):
+    if t.data_ptr() % 16 or any(s * size % 16 for s in t.stride()[:-1]) or t.stride(-1) != 1:
         t = t.detach().clone(memory_format=torch.contiguous_format)
     return t
 

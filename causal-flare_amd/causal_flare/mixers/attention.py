@@ -35,6 +35,8 @@ from ._inputs import (
     _f32,
     _int32,
     _on,
+    _ptr,
+    _raw_stream,
     _strides,
     _training,
 )
@@ -108,12 +110,12 @@ class SoftmaxAttention(autograd.Function):
         lib = _lib.lib()
         nbytes = lib.flare_attn_forward_workspace_size(B, N, N, H, D, _lib.dtype_code(dtype))
         ws = torch.empty(nbytes, device=Q.device, dtype=torch.uint8)
-        P = _lib.ptr
+        P = _ptr
         with _on(Q.device):
             rc = lib.flare_attn_forward(
                 P(q), P(k), P(v), _strides(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3]), _lib.dtype_code(dtype),
                 B, N, N, H, G, D, scale, softcap, P(sl), int(causal), P(ids), P(pre), None, None, P(y), P(lse), P(ws),
-                nbytes, _lib.stream_of(Q.device))
+                nbytes, _raw_stream(Q.device.index))
         _lib.check(rc, "flare_attn_forward")
         if training:
             ctx.save_for_backward(Q, K, V, sl, ids, pre, y, lse)
@@ -135,12 +137,12 @@ class SoftmaxAttention(autograd.Function):
         lib = _lib.lib()
         nbytes = lib.flare_attn_backward_workspace_size(B, N, H, G, D, _lib.dtype_code(dtype))
         ws = torch.empty(nbytes, device=Q.device, dtype=torch.uint8)
-        P = _lib.ptr
+        P = _ptr
         with _on(Q.device):
             rc = lib.flare_attn_backward(
                 P(q), P(k), P(v), _strides(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3]), _lib.dtype_code(dtype),
                 B, N, H, G, D, scale, softcap, P(sl), int(causal), P(ids), P(pre), P(y), P(lse), P(g), P(dq), P(dk),
-                P(dv), P(ws), nbytes, _lib.stream_of(Q.device))
+                P(dv), P(ws), nbytes, _raw_stream(Q.device.index))
         _lib.check(rc, "flare_attn_backward")
         return (dq.to(Q.dtype), dk.to(K.dtype), dv.to(V.dtype)) + (None,) * 7
 
@@ -211,11 +213,11 @@ def softmax_attention_prefill(
     S, code = kc.shape[1], _lib.dtype_code(kc.dtype)
     q, k, v = (_aligned_rows(t, kc.dtype) for t in (Q, K, V))
     sl, pre, lens, new = _f32(slopes), _int32(prefix_lengths), _int32(lengths), _int32(new_lengths)
-    lib, P = _lib.lib(), _lib.ptr
+    lib, P = _lib.lib(), _ptr
     nbytes = lib.flare_attn_forward_workspace_size(B, T, S, H, D, code)
     ws = torch.empty(nbytes, device=device, dtype=torch.uint8)
     with _on(device):
-        stream = _lib.stream_of(device)
+        stream = _raw_stream(device.index)
         rc = lib.flare_attn_append(P(k), P(v), _strides(*k.stride()[:3], *v.stride()[:3]), code, B, T, S, G, D, P(lens),
                                    P(new), P(kc), P(vc), stream)
         _lib.check(rc, "flare_attn_append")
@@ -258,13 +260,13 @@ def softmax_attention_decode(
     S = kc.shape[1]
     q, k, v = (_aligned_rows(t, kc.dtype) for t in (Q, K, V))
     sl, lens = _f32(slopes), _int32(lengths)
-    lib, P = _lib.lib(), _lib.ptr
+    lib, P = _lib.lib(), _ptr
     nbytes = lib.flare_attn_step_workspace_size(B, S, H, G, D)
     ws = torch.empty(nbytes, device=device, dtype=torch.uint8) if nbytes else None
     strides = _strides(q.stride(0), q.stride(2), k.stride(0), k.stride(2), v.stride(0), v.stride(2))
     with _on(device):
         rc = lib.flare_attn_step(P(q), P(k), P(v), strides, _lib.dtype_code(kc.dtype), B, S, H, G, D,
                                  _resolve_attn_scale(scale, D), cap, P(sl), P(lens), P(kc), P(vc), P(y), P(ws), nbytes,
-                                 _lib.stream_of(device))
+                                 _raw_stream(device.index))
     _lib.check(rc, "flare_attn_step")
     return y, cache

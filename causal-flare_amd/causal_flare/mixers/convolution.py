@@ -61,11 +61,11 @@ def _run(x, weight, bias, activation, document_ids=None, lengths=None, window=No
     xr, w, b = _rows(x, dtype), _f32(weight), _f32(bias)
     ids, lens = _int32(document_ids), _int32(lengths)
     y = torch.empty((B, N, C), device=x.device, dtype=dtype)
-    P = _lib.ptr
+    P = _ptr
     with _on(x.device):
         rc = _lib.lib().flare_conv_forward(
             P(xr), xr.stride(0), xr.stride(1), P(w), P(b), int(activation == "silu"), _lib.dtype_code(dtype), B, N, C,
-            weight.shape[1], P(ids), P(lens), P(window), P(y), P(window_out), _lib.stream_of(x.device))
+            weight.shape[1], P(ids), P(lens), P(window), P(y), P(window_out), _raw_stream(x.device.index))
     _lib.check(rc, "flare_conv_forward")
     return y
 
@@ -98,11 +98,11 @@ class ShortConvolution(autograd.Function):
         lib = _lib.lib()
         nbytes = lib.flare_conv_backward_workspace_size(B, N, C, W)
         ws = torch.empty(nbytes, device=x.device, dtype=torch.uint8)
-        P = _lib.ptr
+        P = _ptr
         with _on(x.device):
             rc = lib.flare_conv_backward(
                 P(xr), xr.stride(0), xr.stride(1), P(w), P(b), int(ctx.activation == "silu"), _lib.dtype_code(dtype),
-                B, N, C, W, P(ids), P(g), P(dx), P(dw), P(db), P(ws), nbytes, _lib.stream_of(x.device))
+                B, N, C, W, P(ids), P(g), P(dx), P(dw), P(db), P(ws), nbytes, _raw_stream(x.device.index))
         _lib.check(rc, "flare_conv_backward")
         return dx.to(x.dtype), dw.to(weight.dtype), None if bias is None else db.to(bias.dtype), None, None
 
@@ -215,10 +215,10 @@ def short_convolution_decode(
     y = torch.empty((B, 1, C), device=device, dtype=dtype)
     if y.numel() == 0:
         return y.to(x.dtype), {"window": window}
-    P = _lib.ptr
+    P = _ptr
     with _on(device):
         rc = _lib.lib().flare_conv_step(P(xr), xr.stride(0), P(w), P(b), int(activation == "silu"),
                                         _lib.dtype_code(dtype), B, C, W, P(mask), P(window), P(y),
-                                        _lib.stream_of(device))
+                                        _raw_stream(device.index))
     _lib.check(rc, "flare_conv_step")
     return y.to(x.dtype), {"window": window}

@@ -78,7 +78,7 @@ class _Inputs:
                                 *self.B.stride()[:3], *self.C.stride()[:3])
 
     def pointers(self):
-        P = _lib.ptr
+        P = _ptr
         return P(self.x), P(self.dt), P(self.A), P(self.B), P(self.C), P(self.D), P(self.z), P(self.dt_bias)
 
 
@@ -101,11 +101,11 @@ def _run(x, dt, A, B, C, D, z, dt_bias, dt_softplus, sizes, training, document_i
     ws = torch.empty(nbytes, device=x.device, dtype=torch.uint8)
     y = torch.empty((nb, n, c), device=x.device, dtype=t.dtype)
     ids, lens = _int32(document_ids), _int32(lengths)
-    P = _lib.ptr
+    P = _ptr
     with _on(x.device):
         rc = lib.flare_scan_forward(*t.pointers(), int(bool(dt_softplus)), _lib.dtype_code(t.dtype), nb, n, c, s, g,
                                     t.strides, P(ids), P(lens), P(h0), P(y), P(h_fin), chunk, P(kept), P(ws),
-                                    nbytes, _lib.stream_of(x.device))
+                                    nbytes, _raw_stream(x.device.index))
     _lib.check(rc, "flare_scan_forward")
     return y, kept, chunk
 
@@ -147,11 +147,11 @@ class StateSpaceScan(autograd.Function):
         lib = _lib.lib()
         nbytes = lib.flare_scan_backward_workspace_size(nb, n, c, s, g, ctx.chunk)
         ws = torch.empty(nbytes, device=device, dtype=torch.uint8)
-        P = _lib.ptr
+        P = _ptr
         with _on(device):
             rc = lib.flare_scan_backward(*t.pointers(), int(bool(ctx.softplus)), _lib.dtype_code(t.dtype), nb, n, c, s,
                                          g, t.strides, P(ids), P(gy), ctx.chunk, P(kept), P(dx), P(ddt), P(dA),
-                                         P(dB), P(dC), P(dD), P(dz), P(dbias), P(ws), nbytes, _lib.stream_of(device))
+                                         P(dB), P(dC), P(dD), P(dz), P(dbias), P(ws), nbytes, _raw_stream(device.index))
         _lib.check(rc, "flare_scan_backward")
         grads = (dx, ddt, dA, dB.view(B.shape), dC.view(C.shape), dD, dz, dbias)
         return tuple(None if d is None else d.to(ref.dtype) for d, ref in zip(grads, leaves)) + (None,) * 4
@@ -296,9 +296,9 @@ def state_space_scan_decode(
     y = torch.empty((nb, 1, c), device=device, dtype=t.dtype)
     if y.numel() == 0:
         return y.to(x.dtype), {"h": h}
-    P = _lib.ptr
+    P = _ptr
     with _on(device):
         rc = _lib.lib().flare_scan_step(*t.pointers(), int(bool(dt_softplus)), _lib.dtype_code(t.dtype), nb, c, s, g,
-                                        t.strides, P(mask), P(h), P(y), _lib.stream_of(device))
+                                        t.strides, P(mask), P(h), P(y), _raw_stream(device.index))
     _lib.check(rc, "flare_scan_step")
     return y.to(x.dtype), {"h": h}

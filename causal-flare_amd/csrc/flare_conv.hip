@@ -283,48 +283,17 @@ __global__ __launch_bounds__(256) void conv_step_kernel(ConvArgs p, const int32_
     store_row<E, VEC>((E*)p.y + b * p.C + c, out);
 }
 
-// dw [C, W] and db [C] from the sums of the column sums' layout [W + 1][C].
-__global__ __launch_bounds__(256) void conv_weight_grad_kernel(const float* sums, int64_t C, int W, float* dw,
-                                                               float* db) {
-    const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (id >= C * (W + 1)) return;
-    const int64_t k = id / C, c = id % C;
-    if (k < W) dw[c * W + k] = sums[id];
-    else if (db) db[c] = sums[id];
-}
-
-// 64 columns a workgroup, 16 threads to a column, each over its share of the rows in order.
-__global__ __launch_bounds__(1024) void column_sums_kernel(const float* partial, int64_t R, int64_t cols, float* out) {
-    __shared__ float red[16][65];
-    const int lane = threadIdx.x & 63, part = threadIdx.x >> 6;
-    const int64_t col = (int64_t)blockIdx.x * 64 + lane;
-    float s = 0.0f;
-    if (col < cols) {
-        const int64_t per = (R + 15) / 16, r0 = part * per, r1 = min(r0 + per, R);
-        int64_t r = r0;
-        for (; r + 8 <= r1; r += 8) {
-            float v[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = partial[(r + i) * cols + col];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) s += v[i];
-        }
-        for (; r < r1; ++r) s += partial[r * cols + col];
+// Where the column sums of [W + 1][C] go: dw [C, W] and db [C].
+struct PutWeights {
+    int64_t C;
+    int W;
+    float *dw, *db;
+    __device__ __forceinline__ void operator()(int64_t col, float v) const {
+        const int64_t k = col / C, c = col % C;
+        if (k < W) dw[c * W + k] = v;
+        else if (db) db[c] = v;
     }
-    red[part][lane] = s;
-    __syncthreads();
-    if (part == 0 && col < cols) {
-        float t = 0.0f;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) t += red[i][lane];
-        out[col] = t;
-    }
-}
-
-int launch_column_sums(const float* partial, int64_t R, int64_t cols, float* out, hipStream_t stream) {
-    column_sums_kernel<<<dim3((unsigned)ceil_div(cols, 64)), 1024, 0, stream>>>(partial, R, cols, out);
-    return check_launch("column_sums");
-}
+};
 
 constexpr int kConvBackTokens = 32;
 
@@ -392,7 +361,7 @@ static int conv_step_e(const ConvArgs& p, int64_t W, const int32_t* mask, hipStr
 }
 
 static size_t conv_backward_bytes(int64_t B, int64_t N, int64_t C, int64_t W) {
-    return (size_t)(B * ceil_div(N, kConvBackTokens) + 1) * (W + 1) * C * sizeof(float);
+    return (size_t)(B * ceil_div(N, kConvBackTokens)) * (W + 1) * C * sizeof(float);
 }
 
 }  // namespace mix
@@ -441,15 +410,10 @@ extern "C" int flare_conv_backward(const void* x, int64_t x_stride_b, int64_t x_
     ConvArgs p = {};
     p.x = x, p.x_sb = x_stride_b, p.x_sn = x_stride_n, p.weight = weight, p.bias = bias, p.ids = document_ids;
     p.dy = dy, p.dx = dx, p.partial = (float*)workspace, p.B = B, p.N = N, p.C = C, p.silu = silu;
-    int rc = FLARE_BY_DTYPE(dtype, conv_backward_e, (p, W, (hipStream_t)stream));
+    const int rc = FLARE_BY_DTYPE(dtype, conv_backward_e, (p, W, (hipStream_t)stream));
     if (rc != FLARE_OK) return rc;
     const int64_t rows = B * ceil_div(N, kConvBackTokens), cols = (W + 1) * C;
-    float* sums = p.partial + rows * cols;
-    rc = launch_column_sums(p.partial, rows, cols, sums, (hipStream_t)stream);
-    if (rc != FLARE_OK) return rc;
-    conv_weight_grad_kernel<<<dim3((unsigned)ceil_div(cols, 256)), 256, 0, (hipStream_t)stream>>>(sums, C, (int)W,
-                                                                                                 dweight, dbias);
-    return check_launch("conv_weight_grad");
+    return launch_column_sums(p.partial, rows, cols, PutWeights{C, (int)W, dweight, dbias}, (hipStream_t)stream);
 }
 
 extern "C" int flare_conv_step(const void* x, int64_t x_stride_b, const float* weight, const float* bias, int silu,

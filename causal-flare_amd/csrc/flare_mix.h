@@ -78,8 +78,40 @@ __device__ __forceinline__ void store_row(T* p, const float (&in)[VEC]) {
     *reinterpret_cast<A*>(p) = a;
 }
 
-// Sums the R rows of partial [R, cols] in a fixed order into out [cols] (flare_conv.hip).
-int launch_column_sums(const float* partial, int64_t R, int64_t cols, float* out, hipStream_t stream);
+// The sums of each column of partial [R, cols], handed to put(column, sum): 64 columns a workgroup,
+// 16 threads to a column, each over its share of the rows in order.
+template <typename Put>
+__global__ __launch_bounds__(1024) void column_sums_kernel(const float* partial, int64_t R, int64_t cols, Put put) {
+    __shared__ float red[16][65];
+    const int lane = threadIdx.x & 63, part = threadIdx.x >> 6;
+    const int64_t col = (int64_t)blockIdx.x * 64 + lane;
+    float s = 0.0f;
+    if (col < cols) {
+        const int64_t per = (R + 15) / 16, r0 = part * per, r1 = min(r0 + per, R);
+        int64_t r = r0;
+        for (; r + 8 <= r1; r += 8) {
+            float v[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = partial[(r + i) * cols + col];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) s += v[i];
+        }
+        for (; r < r1; ++r) s += partial[r * cols + col];
+    }
+    red[part][lane] = s;
+    __syncthreads();
+    if (part == 0 && col < cols) {
+        float t = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) t += red[i][lane];
+        put(col, t);
+    }
+}
+template <typename Put>
+int launch_column_sums(const float* partial, int64_t R, int64_t cols, Put put, hipStream_t stream) {
+    column_sums_kernel<<<dim3((unsigned)ceil_div(cols, 64)), 1024, 0, stream>>>(partial, R, cols, put);
+    return check_launch("column_sums");
+}
 
 }  // namespace mix
 }  // namespace flare

@@ -70,6 +70,7 @@ inline int64_t padded_states(int64_t S) { return S <= 8 ? 8 : S <= 16 ? 16 : S <
 // The backward holds B and C of a chunk in LDS, and recomputes its states from those the forward
 // kept: so far apart that what it keeps of a stretch itself stays small.
 constexpr int64_t kBackwardChunkMost = 128;
+constexpr int64_t kMostStride = 1 << 22;        // between tokens, so that a chunk's offsets fit 31 bits
 constexpr int64_t kept_tokens(int64_t SP) { return SP <= 16 ? 32 : SP == 32 ? 16 : 8; }
 
 // Chunk length: some four waves a SIMD (4096 on the card).  Where the channels are too few for

@@ -10,26 +10,26 @@
 namespace flare {
 namespace scan {
 
-// B and C of every token in fp32 with zeros behind S: rows that scalar loads can take whole.
-// Padding's rows are 0, whatever they hold.
+// What the kernels read again and again, laid out once: B and C of every token in fp32 with zeros
+// behind S, rows that scalar loads can take whole (padding's rows are 0, whatever they hold); A in
+// log2 units and the state before the first chunk, [SP, C] each, so that lanes of neighbouring
+// channels read neighbouring words.
 template <typename E>
 __global__ __launch_bounds__(256) void scan_pack_kernel(ScanArgs p, int SP) {
-    const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (id >= p.B * p.N * p.G * 2 * SP) return;
-    const int s = (int)(id % SP), which = (int)(id / SP % 2);
-    const int64_t g = id / (2 * SP) % p.G, t = id / (2 * SP) / p.G % p.N, b = id / (2 * SP) / p.G / p.N;
-    float v = 0.0f;
-    if (s < p.S && !(p.ids && p.ids[b * p.N + t] < 0)) {
-        v = which ? to_f32(((const E*)p.Cm)[b * p.C_sb + t * p.C_sn + g * p.C_sg + s])
-                  : to_f32(((const E*)p.Bm)[b * p.B_sb + t * p.B_sn + g * p.B_sg + s]);
+    int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const int64_t rows = p.B * p.N * p.G * 2 * SP, n = (int64_t)SP * p.C;
+    if (id < rows) {
+        const int s = (int)(id % SP), which = (int)(id / SP % 2);
+        const int64_t g = id / (2 * SP) % p.G, t = id / (2 * SP) / p.G % p.N, b = id / (2 * SP) / p.G / p.N;
+        float v = 0.0f;
+        if (s < p.S && !(p.ids && p.ids[b * p.N + t] < 0)) {
+            v = which ? to_f32(((const E*)p.Cm)[b * p.C_sb + t * p.C_sn + g * p.C_sg + s])
+                      : to_f32(((const E*)p.Bm)[b * p.B_sb + t * p.B_sn + g * p.B_sg + s]);
+        }
+        p.bc[id] = v;
+        return;
     }
-    p.bc[id] = v;
-}
-
-// A in log2 units and the state before the first chunk, [SP, C] each, so that lanes of
-// neighbouring channels read neighbouring words.
-__global__ __launch_bounds__(256) void scan_lay_kernel(ScanArgs p, int SP) {
-    const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x, n = (int64_t)SP * p.C;
+    id -= rows;
     if (id >= n * (1 + p.B)) return;
     const int64_t c = id % p.C, s = id / p.C % SP, b = id / n - 1;
     if (b < 0) p.A2[id] = s < p.S ? p.A[c * p.S + s] * kLog2e : 0.0f;
@@ -38,11 +38,9 @@ __global__ __launch_bounds__(256) void scan_lay_kernel(ScanArgs p, int SP) {
 
 template <typename E>
 static int pack_go(const ScanArgs& p, int64_t SP, hipStream_t stream) {
-    scan_pack_kernel<E><<<dim3((unsigned)ceil_div(p.B * p.N * p.G * 2 * SP, 256)), 256, 0, stream>>>(p, (int)SP);
-    const int rc = check_launch("scan_pack");
-    if (rc != FLARE_OK) return rc;
-    scan_lay_kernel<<<dim3((unsigned)ceil_div(SP * p.C * (1 + p.B), 256)), 256, 0, stream>>>(p, (int)SP);
-    return check_launch("scan_lay");
+    const int64_t work = p.B * p.N * p.G * 2 * SP + SP * p.C * (1 + p.B);
+    scan_pack_kernel<E><<<dim3((unsigned)ceil_div(work, 256)), 256, 0, stream>>>(p, (int)SP);
+    return check_launch("scan_pack");
 }
 int launch_pack(const ScanArgs& p, int dtype, int64_t SP, hipStream_t stream) {
     return FLARE_BY_DTYPE(dtype, pack_go, (p, SP, stream));

@@ -9,13 +9,17 @@
 // kept, the last one first: forward over a stretch, leaving a state every T tokens in LDS, and
 // backward over these pieces of T tokens, each recomputed with a_t and a_t h_{t-1} in registers.
 //
-// There four lanes share a channel (SL = S / 4 states each) and a wave has 16 channels: a piece
-// of T = 16 tokens then fits 128 registers at S = 16, where a lane with all the states of a
-// channel could hold only 4 tokens.  What one lane would do alone for a token (the exponentials
-// of the gates, the loads and stores) lane q of a channel does for the tokens 4i + q, and the
-// others read it through DPP.  dB and dC are summed over the wave's channels by halving: each
-// step adds two values and leaves one, half the lanes' worth of work at a time; the waves' sums
-// meet in LDS and the workgroups' in scan_dbc, always in the same order.
+// There four lanes share a channel (SL = S / 4 states each) and a wave has 16 channels: the
+// decays of a piece then take 2 T SL registers, where a lane with all the states of a channel
+// would need four times that.  What one lane would do alone for a token (the exponentials of the
+// gates, the loads and stores) lane q of a channel does for the tokens 4i + q, and the others read
+// it through DPP.  dB and dC are summed over the wave's channels by halving: each step adds two
+// values and leaves one, half the lanes' worth of work at a time; the waves' sums meet in LDS and
+// the workgroups' in scan_dbc, always in the same order.
+//
+// Vector instructions bound it, some 34 for an element of the state.  4 x 4096 tokens, 2048
+// channels of 16 states, bf16: 654 us with T = 4 and three workgroups of four waves a CU (167
+// registers); T = 8 (216 registers, two waves a SIMD) 691, eight waves a workgroup 773 to 881.
 #include <type_traits>
 #include <utility>
 
@@ -237,18 +241,46 @@ __device__ __forceinline__ void each_token(F&& fn, std::integer_sequence<int, J.
     (fn(std::integral_constant<int, J>{}), ...);
 }
 
-constexpr int kWaves = 8;              // 128 channels a workgroup
+constexpr int kWaves = 4;              // 64 channels a workgroup
 
 template <int SP>
 struct GradLayout {
     static constexpr int SL = SP / 4;
-    static constexpr int T = SL <= 4 ? 8 : 4;
+    static constexpr int T = 4;
     static constexpr int keep = (int)kept_tokens(SP), pieces = keep / T;
     static constexpr int bc_floats = (int)kBackwardChunkMost * 2 * SP;
     static constexpr int keep_floats = kWaves * pieces * 64 * SL;
     static constexpr int red_floats = kWaves * T * 2 * SP;
     static constexpr size_t bytes = sizeof(float) * (bc_floats + keep_floats + red_floats);
     static_assert(bytes <= 160 * 1024, "LDS of a CU");
+};
+
+// One value of each token of a chunk through a buffer descriptor: tokens behind the chunk's last
+// one and lanes without a channel load 0 and store nothing, and an address costs one addition.
+template <typename E>
+struct TokenValues {
+    __amdgpu_buffer_rsrc_t r;
+    unsigned at, step;               // bytes: this lane's channel, or past everything; a token
+    // `base`: the chunk's first token; n tokens `stride` elements apart
+    __device__ __forceinline__ TokenValues(const void* base, int n, int64_t stride, int64_t C, int64_t c, bool active)
+        : r(__builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0,
+                                              base ? (int)((n - 1) * stride + C) * (int)sizeof(E) : 0, 0x00020000)),
+          at(active ? (unsigned)c * (unsigned)sizeof(E) : 0x80000000u), step((unsigned)stride * (unsigned)sizeof(E)) {}
+    __device__ __forceinline__ E load(int lane_token, int k) const {
+        const unsigned o = at + lane_token * step + k * step;
+        if constexpr (sizeof(E) == 2) {
+            const unsigned short v = __builtin_amdgcn_raw_buffer_load_b16(r, o, 0, 0);
+            return __builtin_bit_cast(E, v);
+        } else {
+            const unsigned v = __builtin_amdgcn_raw_buffer_load_b32(r, o, 0, 0);
+            return __builtin_bit_cast(E, v);
+        }
+    }
+    __device__ __forceinline__ void store(int lane_token, int k, float x) const {
+        const unsigned o = at + lane_token * step + k * step;
+        if constexpr (sizeof(E) == 2) __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(unsigned short, from_f32<E>(x)), r, o, 0, 0);
+        else __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(unsigned, x), r, o, 0, 0);
+    }
 };
 
 // SL adjacent floats of LDS, aligned to all of them (or 16 bytes).
@@ -281,11 +313,14 @@ __global__ __launch_bounds__(64 * kWaves) void scan_gradient_kernel(ScanArgs p) 
     const int64_t t0 = chunk * p.L;
     const int n = (int)(min(t0 + p.L, p.N) - t0);          // tokens of this chunk
     const int32_t* ids = p.ids ? p.ids + b * p.N + t0 : nullptr;
-    const E* x = (const E*)p.x + b * p.x_sb + t0 * p.x_sn + c;
-    const E* dt = (const E*)p.dt + b * p.dt_sb + t0 * p.dt_sn + c;
-    const E* z = p.z ? (const E*)p.z + b * p.z_sb + t0 * p.z_sn + c : nullptr;
-    const int64_t row0 = (b * p.N + t0) * p.C + c;
-    const E* dy = (const E*)p.dy + row0;
+    const bool z = p.z != nullptr;
+    const int64_t row0 = (b * p.N + t0) * p.C;
+    auto values = [&](const void* base, int64_t first, int64_t stride) {
+        return TokenValues<E>(base ? (const E*)base + first : nullptr, n, stride, p.C, c, active);
+    };
+    const auto xs = values(p.x, b * p.x_sb + t0 * p.x_sn, p.x_sn), dts = values(p.dt, b * p.dt_sb + t0 * p.dt_sn, p.dt_sn);
+    const auto zs = values(p.z, b * p.z_sb + t0 * p.z_sn, p.z_sn), dys = values(p.dy, row0, p.C);
+    const auto dxs = values(p.dx, row0, p.C), ddts = values(p.ddt, row0, p.C), dzs = values(p.dz, row0, p.C);
 
     const int rows = (n + T - 1) / T * T;                  // tokens behind the last one have B = C = 0
     for (int i = tid; i < rows * 2 * SP; i += 64 * kWaves)
@@ -305,7 +340,7 @@ __global__ __launch_bounds__(64 * kWaves) void scan_gradient_kernel(ScanArgs p) 
     const float bias = p.dt_bias ? p.dt_bias[c] : 0.0f, skip = p.D ? p.D[c] : 0.0f;
     float dD = 0.0f, dbias = 0.0f;
 
-    // The tokens 4 i + q of the piece at k0, as loaded: rows that are none load the last one's.
+    // The tokens 4 i + q of the piece at k0, as loaded.
     struct Raw {
         E dt[TQ], x[TQ], dy[TQ], z[TQ];
         int id[TQ];
@@ -313,12 +348,12 @@ __global__ __launch_bounds__(64 * kWaves) void scan_gradient_kernel(ScanArgs p) 
     auto fetch = [&](Raw& r, int k0, bool all) {
 #pragma unroll
         for (int i = 0; i < TQ; ++i) {
-            const int k = min(max(k0, 0) + 4 * i + q, n - 1);
-            r.dt[i] = dt[k * p.dt_sn];
-            r.x[i] = x[k * p.x_sn];
-            if (all) r.dy[i] = dy[k * p.C];
-            if (all && z) r.z[i] = z[k * p.z_sn];
-            r.id[i] = ids ? ids[k] : 0;
+            const int k = max(k0, 0) + 4 * i;
+            r.dt[i] = dts.load(q, k);
+            r.x[i] = xs.load(q, k);
+            if (all) r.dy[i] = dys.load(q, k);
+            if (all && z) r.z[i] = zs.load(q, k);
+            r.id[i] = ids ? ids[min(k + q, n - 1)] : 0;
         }
     };
     // a token that is none has delta = x = 0
@@ -392,7 +427,7 @@ __global__ __launch_bounds__(64 * kWaves) void scan_gradient_kernel(ScanArgs p) 
             const int k0 = first + piece * T;
             const Raw now = next;
             fetch(next, k0 - T, true);
-            float raw[TQ], delta[TQ], xv[TQ], du[TQ], gy[TQ], dyv[TQ], zv[TQ];
+            float raw[TQ], delta[TQ], xv[TQ], du[TQ], gy[TQ], dyv[TQ], zv[TQ], gate[TQ];
             bool live[TQ];
 #pragma unroll
             for (int i = 0; i < TQ; ++i) {
@@ -400,7 +435,8 @@ __global__ __launch_bounds__(64 * kWaves) void scan_gradient_kernel(ScanArgs p) 
                 du[i] = delta[i] * xv[i];
                 dyv[i] = live[i] ? to_f32(now.dy[i]) : 0.0f;
                 zv[i] = live[i] && z ? to_f32(now.z[i]) : 0.0f;
-                gy[i] = z ? dyv[i] * zv[i] * mix::sigmoid(zv[i]) : dyv[i];
+                gate[i] = z ? mix::sigmoid(zv[i]) : 1.0f;
+                gy[i] = z ? dyv[i] * zv[i] * gate[i] : dyv[i];
             }
             float a[T][SL], ah[T][SL];
 #pragma unroll
@@ -451,20 +487,16 @@ __global__ __launch_bounds__(64 * kWaves) void scan_gradient_kernel(ScanArgs p) 
                 if constexpr (jq == 0) {
                     constexpr int i = j / 4;
                     const float pq = quad_gather(pA, q) * kLn2, sq = quad_gather(sB, q), lq = quad_gather(lin, q);
-                    const int k = k0 + 4 * i + q;
                     float ddt = pq + xv[i] * sq;
                     if (p.softplus) ddt *= mix::sigmoid(raw[i]);
                     if (!live[i]) ddt = 0.0f;
                     dbias += ddt;
                     dD += gy[i] * xv[i];
-                    if (active && k < n) {
-                        ((E*)p.dx)[row0 + k * p.C] = from_f32<E>(live[i] ? delta[i] * sq + gy[i] * skip : 0.0f);
-                        ((E*)p.ddt)[row0 + k * p.C] = from_f32<E>(ddt);
-                        if (z) {
-                            const float sg = mix::sigmoid(zv[i]);
-                            const float dz = dyv[i] * (lq + skip * xv[i]) * sg * (1.0f + zv[i] * (1.0f - sg));
-                            ((E*)p.dz)[row0 + k * p.C] = from_f32<E>(live[i] ? dz : 0.0f);
-                        }
+                    dxs.store(q, k0 + 4 * i, live[i] ? delta[i] * sq + gy[i] * skip : 0.0f);
+                    ddts.store(q, k0 + 4 * i, ddt);
+                    if (z) {
+                        const float dz = dyv[i] * (lq + skip * xv[i]) * gate[i] * (1.0f + zv[i] * (1.0f - gate[i]));
+                        dzs.store(q, k0 + 4 * i, live[i] ? dz : 0.0f);
                     }
                 }
             };
@@ -505,16 +537,17 @@ __global__ __launch_bounds__(256) void scan_dbc_kernel(ScanArgs p, int SP, int64
     out[(bn * p.G + g) * p.S + col] = from_f32<E>(v);
 }
 
-// dA [C, S], dD [C] and ddt_bias [C] from the column sums [C, SP + 2].
-__global__ __launch_bounds__(256) void scan_param_kernel(const float* sums, int64_t C, int S, int SP, float* dA,
-                                                         float* dD, float* dbias) {
-    const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (id >= C * (SP + 2)) return;
-    const int64_t c = id / (SP + 2), s = id % (SP + 2);
-    if (s < S) dA[c * S + s] = sums[id];
-    else if (s == SP && dD) dD[c] = sums[id];
-    else if (s == SP + 1 && dbias) dbias[c] = sums[id];
-}
+// Where the column sums of [C, SP + 2] go: dA [C, S], dD [C] and ddt_bias [C].
+struct PutParams {
+    int S, SP;
+    float *dA, *dD, *dbias;
+    __device__ __forceinline__ void operator()(int64_t col, float v) const {
+        const int64_t c = col / (SP + 2), s = col % (SP + 2);
+        if (s < S) dA[c * S + s] = v;
+        else if (s == SP && dD) dD[c] = v;
+        else if (s == SP + 1 && dbias) dbias[c] = v;
+    }
+};
 
 template <typename E, int SP>
 static int backward_go(const ScanArgs& p, hipStream_t stream) {
@@ -552,7 +585,7 @@ static int backward_e(const ScanArgs& p, int64_t SP, hipStream_t stream) {
 }
 
 struct BackwardLayout {
-    size_t bc, A2, carry, dsum, cuts, dbc, dpar, sums, total;      // in floats
+    size_t bc, A2, carry, dsum, cuts, dbc, dpar, total;      // in floats
     BackwardLayout(int64_t B, int64_t N, int64_t C, int64_t S, int64_t G, int64_t NC) {
         const int64_t SP = padded_states(S), blocks = G * ceil_div(C / G, 16 * kWaves);
         bc = 0;
@@ -562,8 +595,7 @@ struct BackwardLayout {
         cuts = dsum + B * NC * C;
         dbc = cuts + B * NC;
         dpar = dbc + blocks * B * N * 2 * SP;
-        sums = dpar + B * NC * C * (SP + 2);
-        total = sums + C * (SP + 2);
+        total = dpar + B * NC * C * (SP + 2);
     }
 };
 
@@ -595,6 +627,8 @@ extern "C" int flare_scan_backward(const void* x, const void* dt, const float* A
                   (long long)kBackwardChunkMost);
     ScanArgs p = scan_args(x, dt, A, Bm, Cm, D, z, dt_bias, softplus, B, N, C, S, G, strides);
     p.L = chunk, p.NC = ceil_div(N, chunk);
+    for (int i = 1; i < 6; i += 2)
+        FLARE_REQUIRE(strides[i] >= 0 && strides[i] < kMostStride, "flare_scan_backward: tokens must be less than 2^22 elements apart");
     const BackwardLayout lay(B, N, C, S, G, p.NC);
     if (workspace_bytes < lay.total * sizeof(float)) {
         set_error("flare_scan_backward: workspace of %zu bytes is too small", workspace_bytes);
@@ -608,9 +642,6 @@ extern "C" int flare_scan_backward(const void* x, const void* dt, const float* A
     hipStream_t st = (hipStream_t)stream;
     int rc = launch_pack(p, dtype, SP, st);
     if (rc == FLARE_OK) rc = FLARE_BY_DTYPE(dtype, backward_e, (p, SP, st));
-    if (rc == FLARE_OK) rc = mix::launch_column_sums(p.dpar, B * p.NC, C * (SP + 2), ws + lay.sums, st);
     if (rc != FLARE_OK) return rc;
-    scan_param_kernel<<<dim3((unsigned)ceil_div(C * (SP + 2), 256)), 256, 0, st>>>(ws + lay.sums, C, (int)S, (int)SP, dA,
-                                                                                dD, ddt_bias);
-    return check_launch("scan_param");
+    return mix::launch_column_sums(p.dpar, B * p.NC, C * (SP + 2), PutParams{(int)S, (int)SP, dA, dD, ddt_bias}, st);
 }
