@@ -14,7 +14,7 @@ namespace flare {
 namespace attn {
 
 // How scores are kept from overflowing: against a running maximum, or against the cap itself,
-// which bounds them.
+// which bounds them where nothing is added.
 enum { kNoCap = 0, kCapRunning = 1, kCapFixed = 2 };
 // With weights of 2^(s - cap) a row's largest is at least 2^(-2 cap): fp32 and bf16 hold that, with
 // all that counts beside it, up to here (log2 units), and fp16 does not.
@@ -73,8 +73,8 @@ __global__ __launch_bounds__(256, 2) void attn_forward_kernel(AttnArgs p) {
     int k_begin = 0;
     if (parts > 1) {
         const int tiles = (kv_end + KT - 1) / KT;
-        k_begin = tiles * part / parts * KT;
-        kv_end = min(kv_end, tiles * (part + 1) / parts * KT);
+        k_begin = (int)((int64_t)tiles * part / parts) * KT;
+        kv_end = min(kv_end, (int)((int64_t)tiles * (part + 1) / parts) * KT);
     }
     IdRange mine{0, 0, true};
     if (p.ids) mine = id_block(p, b, q0, QB);
@@ -383,7 +383,7 @@ template <typename E, int DP>
 static int forward_dp(const AttnArgs& p, hipStream_t stream) {
     if (p.cap == 0.0f) return forward_cap<E, DP, kNoCap>(p, stream);
     if constexpr (!__is_same(E, __half))
-        if (p.cap * kLog2e <= kCapFixedMost) return forward_cap<E, DP, kCapFixed>(p, stream);
+        if (!p.slopes && p.cap * kLog2e <= kCapFixedMost) return forward_cap<E, DP, kCapFixed>(p, stream);
     return forward_cap<E, DP, kCapRunning>(p, stream);
 }
 template <typename E>

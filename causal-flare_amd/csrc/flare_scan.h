@@ -58,6 +58,12 @@ __device__ __forceinline__ int64_t row_length(const ScanArgs& p, int64_t b) {
     const int64_t n = p.lengths[b];
     return n < 0 ? 0 : (n > p.N ? p.N : n);
 }
+// The state `h` behind a chunk whose tokens sum up to A2 dsum (log2 units).  In two halves: a decay
+// that grows past fp32 over a chunk is none of a state that is 0 or small enough.
+__device__ __forceinline__ float decayed(float h, float A2dsum) {
+    const float e = __builtin_amdgcn_exp2f(0.5f * A2dsum);
+    return h * e * e;
+}
 // Whether token t begins a document.
 __device__ __forceinline__ bool begins(const int32_t* ids, int64_t t) { return t > 0 && ids[t] != ids[t - 1]; }
 
@@ -100,7 +106,8 @@ inline ScanArgs scan_args(const void* x, const void* dt, const float* A, const v
     FLARE_REQUIRE(S >= 1 && S <= 64, name ": 1 to 64 states a channel, got %lld", (long long)S);              \
     FLARE_REQUIRE(G >= 1 && C % G == 0, name ": the channels must divide into the groups of B and C");        \
     FLARE_REQUIRE(B <= 65535 && C <= (1 << 20) && N <= (1 << 30) && B * N <= ((int64_t)1 << 36) / (128 * G),  \
-                  name ": too large")
+                  name ": too large");                                                                        \
+    FLARE_REQUIRE(G * ceil_div(C / G, 64) <= 65535, name ": too many groups")
 
 // Waves a SIMD of the kernels whose lanes hold all SP states of a channel.
 constexpr int lane_waves(int SP) { return SP <= 16 ? 4 : SP == 32 ? 2 : 1; }

@@ -224,14 +224,14 @@ __global__ __launch_bounds__(256) void scan_states_kernel(ScanArgs p, int SP) {
         for (int u = 0; u < U; ++u) {
             const int64_t k = min(k0 + u, p.NC - 2);
             own[u] = slot[(k + 1) * step];
-            dec[u] = __builtin_amdgcn_exp2f(A2 * dsum[k * p.C]);
+            dec[u] = A2 * dsum[k * p.C];
         }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int64_t k = k0 + u;
             if (k + 1 >= p.NC) break;
             // a document's beginning cuts off what came before it
-            h = p.ids && p.cuts[b * p.NC + k] ? own[u] : dec[u] * h + own[u];
+            h = p.ids && p.cuts[b * p.NC + k] ? own[u] : decayed(h, dec[u]) + own[u];
             slot[(k + 1) * step] = h;
         }
     }

@@ -164,13 +164,13 @@ __global__ __launch_bounds__(256) void scan_carries_kernel(ScanArgs p, int SP) {
         for (int u = 0; u < U; ++u) {
             const int64_t k = max(k0 - u, (int64_t)1);
             own[u] = slot[(k - 1) * step];
-            dec[u] = __builtin_amdgcn_exp2f(A2 * dsum[k * p.C]);
+            dec[u] = A2 * dsum[k * p.C];
         }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int64_t k = k0 - u;
             if (k < 1) break;
-            r = p.ids && p.cuts[b * p.NC + k] ? own[u] : dec[u] * r + own[u];
+            r = p.ids && p.cuts[b * p.NC + k] ? own[u] : decayed(r, dec[u]) + own[u];
             slot[(k - 1) * step] = r;
         }
     }

@@ -184,7 +184,7 @@ def attention(q, k, v, scale=None, causal=True, softcap=None, slopes=None, ids=N
 
     unit: half a step of the type that weights and score gradients are rounded to (0: none), tiny:
     half its smallest step, 2^-25 for fp16, by which a weight or score gradient below 2^-14 is
-    off.  (Weights are at most that much off after the division by their sum, which is at least 1.)
+    off; 2^-126 for the others, below which an exponential is 0.  (Weights are at most that much off after the division by their sum, which is at least 1.)
     offset [B]: position of query 0 (k and v then hold positions 0 ..).  The tolerances hold the
     inner roundings; the caller adds that of the result.
     """
@@ -241,7 +241,7 @@ def attention(q, k, v, scale=None, causal=True, softcap=None, slopes=None, ids=N
             edp = e32 * (16 + D) * (do.abs() @ vv.abs().t()) + (do.abs() * ((unit * 2 + 2 * es + e32 * 64) * pv
                                                                           + unit * o.abs())).sum(1, keepdim=True)
             eds = p * cut * edp + (2 * es + e32 * 64) * p * (dp - delta).abs() * (cut + (4 if softcap else 0))
-            eds = eds + unit * ds.abs() + tiny * see
+            eds = eds + unit * ds.abs() + tiny * see * (1 + (dp - delta).abs())
             dq[b, :, h] = ds @ kk * scale
             tq[b, :, h] = (eds @ kk.abs() + e32 * 64 * (ds.abs() @ kk.abs())) * abs(scale)
             dk[b, :, m] += ds.t() @ qq * scale

@@ -228,6 +228,18 @@ def test_scan_prefill_and_decode(dtype, B, N, C, S, G):
     close(st["h"][1::2], ref["h"], "h of the others", F32, ref["k"])
 
 
+def test_scan_of_growing_states_that_are_zero():
+    """A decay past fp32 over a chunk (2^180) leaves a state of 0, and one of 2^-100, what it is."""
+    B, N, C, S = 1, 400, 64, 16
+    z = lambda *s: torch.zeros(s, device=DEV)
+    x, dt, A = z(B, N, C), z(B, N, C) + 1, z(C, S) + math.log(2.0) * 180 / 300
+    h0 = z(B, C, S)
+    h0[:, 0] = 2.0 ** -150 * 2.0 ** 50
+    y, st = cf.state_space_scan_prefill(x, dt, A, z(B, N, S), z(B, N, S) + 1, state={"h": h0}, lengths=torch.tensor([300], device=DEV))
+    assert not st["h"][:, 1:].any() and not y[:, :, 1:].any()
+    assert torch.allclose(st["h"][:, 0], torch.full((B, S), 2.0 ** 80, device=DEV), rtol=1e-3)
+
+
 def test_scan_reads_slices_and_promotes():
     g = gen(5)
     t = scan_inputs(g, 2, 50, 64, 16, 1, BF16)
@@ -259,6 +271,7 @@ ATTENTION = [
     (3, 200, 3, 1, 128, "docs slopes"), (2, 257, 2, 1, 128, "cap docs prefix"), (1, 191, 2, 2, 112, "full docs slopes"),
     (2, 300, 1, 1, 64, "prefix slopes"), (1, 513, 2, 2, 64, "docs"), (1, 100, 2, 1, 64, "negative"),
     (1, 140, 2, 2, 128, "wide-cap slopes negative"), (1, 1100, 1, 1, 32, "docs slopes"), (1, 1537, 2, 1, 48, "cap"),
+    (1, 200, 2, 2, 64, "cap rising slopes"),
 ]
 
 
@@ -269,7 +282,7 @@ def attention_options(g, what, B, N, H):
     if "negative" in what:
         o["scale"] = -0.2
     if "slopes" in what:
-        o["slopes"] = torch.tensor([2.0 ** -(h + 1) for h in range(H)]).to(DEV)
+        o["slopes"] = torch.tensor([2.0 ** -(h + 1) for h in range(H)]).to(DEV) * (-1 if "rising" in what else 1)
     if "docs" in what:
         o["document_ids"] = documents(g, B, N)
     if "prefix" in what:
@@ -299,7 +312,7 @@ def test_attention(dtype, B, N, H, G, D, what):
     leaves = [t.clone().requires_grad_() for t in (q, k, v)]
     y = cf.softmax_attention(*leaves, **o)
     grads = torch.autograd.grad(y, leaves, dy)
-    unit, tiny = (0.0 if dtype is F32 else U[dtype]), (2.0 ** -25 if dtype is F16 else 0.0)
+    unit, tiny = (0.0 if dtype is F32 else U[dtype]), (2.0 ** -25 if dtype is F16 else 2.0 ** -126)
     ref = attention(q, k, v, **plain(o), dy=dy, unit=unit, tiny=tiny)
     close_attention(y, ref["y"], "y", dtype)
     with torch.no_grad():
@@ -318,7 +331,7 @@ def test_attention_of_many_documents_in_order_of_cost(dtype, B, N, H, G):
     leaves = [t.clone().requires_grad_() for t in (q, k, v)]
     y = cf.softmax_attention(*leaves, document_ids=ids)
     grads = torch.autograd.grad(y, leaves, dy)
-    unit, tiny = (0.0 if dtype is F32 else U[dtype]), (2.0 ** -25 if dtype is F16 else 0.0)
+    unit, tiny = (0.0 if dtype is F32 else U[dtype]), (2.0 ** -25 if dtype is F16 else 2.0 ** -126)
     ref = attention(q, k, v, ids=ids, dy=dy, unit=unit, tiny=tiny)
     close_attention(y, ref["y"], "y", dtype)
     for n, got in zip(("dq", "dk", "dv"), grads):
@@ -344,7 +357,7 @@ def test_attention_prefill(dtype, B, T, H, G, D, S, what):
     cache = {"k": ck.clone(), "v": cv.clone()}
     y, same = cf.softmax_attention_prefill(q, k, v, cache, held, **o, new_lengths=new)
     assert same is cache
-    unit, tiny = (0.0 if dtype is F32 else U[dtype]), (2.0 ** -25 if dtype is F16 else 0.0)
+    unit, tiny = (0.0 if dtype is F32 else U[dtype]), (2.0 ** -25 if dtype is F16 else 2.0 ** -126)
     for b in range(B):
         n, at = int(new[b]), int(held[b])
         want_k, want_v = ck[b].clone(), cv[b].clone()
@@ -379,7 +392,7 @@ def test_attention_decode(dtype, B, H, G, D, S, what):
     cache = {"k": ck.clone(), "v": cv.clone()}
     y, same = cf.softmax_attention_decode(q, k, v, cache, held, **o)
     assert same is cache and y.shape == (B, 1, H, D)
-    unit, tiny = (0.0 if dtype is F32 else U[dtype]), (2.0 ** -25 if dtype is F16 else 0.0)
+    unit, tiny = (0.0 if dtype is F32 else U[dtype]), (2.0 ** -25 if dtype is F16 else 2.0 ** -126)
     for b in range(B):
         at = int(held[b])
         want_k, want_v = ck[b].clone(), cv[b].clone()
