@@ -168,12 +168,12 @@ def _declare(lib):
     lib.flare_attn_forward_workspace_size.restype = _sz
     lib.flare_attn_forward_workspace_size.argtypes = [_i64] * 5 + [_i]
     lib.flare_attn_forward.restype = _i
-    lib.flare_attn_forward.argtypes = ([_vp] * 4 + [_i] + [_i64] * 6 + [_f, _f, _vp, _i] + [_vp] * 6
+    lib.flare_attn_forward.argtypes = ([_vp] * 4 + [_i] + [_i64] * 6 + [_f, _f, _vp, _i] + [_vp] * 7
                                        + [_vp, _sz, _vp])
     lib.flare_attn_backward_workspace_size.restype = _sz
     lib.flare_attn_backward_workspace_size.argtypes = [_i64] * 5 + [_i]
     lib.flare_attn_backward.restype = _i
-    lib.flare_attn_backward.argtypes = ([_vp] * 4 + [_i] + [_i64] * 5 + [_f, _f, _vp, _i] + [_vp] * 8
+    lib.flare_attn_backward.argtypes = ([_vp] * 4 + [_i] + [_i64] * 5 + [_f, _f, _vp, _i] + [_vp] * 9
                                         + [_vp, _sz, _vp])
     lib.flare_attn_append.restype = _i
     lib.flare_attn_append.argtypes = [_vp] * 3 + [_i] + [_i64] * 5 + [_vp] * 5

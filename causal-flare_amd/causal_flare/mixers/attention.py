@@ -100,13 +100,14 @@ class SoftmaxAttention(autograd.Function):
         G = K.shape[2]
         ctx.options = (scale, causal, softcap)
         if Q.numel() == 0:
-            ctx.save_for_backward(Q, K, V, None, None, None, None, None)
+            ctx.save_for_backward(Q, K, V, None, None, None, None, None, None)
             return torch.empty_like(Q)
         dtype = _compute_dtype(Q, K, V)
         q, k, v = (_aligned_rows(t, dtype) for t in (Q, K, V))
         sl, ids, pre = _f32(slopes), _int32(document_ids), _int32(prefix_lengths)
         y = torch.empty((B, N, H, D), device=Q.device, dtype=dtype)
         lse = torch.empty((B, H, N), device=Q.device, dtype=torch.float32) if training else None
+        rest = torch.empty_like(y) if training and dtype is not torch.float32 else None
         lib = _lib.lib()
         nbytes = lib.flare_attn_forward_workspace_size(B, N, N, H, D, _lib.dtype_code(dtype))
         ws = torch.empty(nbytes, device=Q.device, dtype=torch.uint8)
@@ -114,17 +115,17 @@ class SoftmaxAttention(autograd.Function):
         with _on(Q.device):
             rc = lib.flare_attn_forward(
                 P(q), P(k), P(v), _strides(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3]), _lib.dtype_code(dtype),
-                B, N, N, H, G, D, scale, softcap, P(sl), int(causal), P(ids), P(pre), None, None, P(y), P(lse), P(ws),
-                nbytes, _raw_stream(Q.device.index))
+                B, N, N, H, G, D, scale, softcap, P(sl), int(causal), P(ids), P(pre), None, None, P(y), P(rest),
+                P(lse), P(ws), nbytes, _raw_stream(Q.device.index))
         _lib.check(rc, "flare_attn_forward")
         if training:
-            ctx.save_for_backward(Q, K, V, sl, ids, pre, y, lse)
+            ctx.save_for_backward(Q, K, V, sl, ids, pre, y, rest, lse)
         return y.to(Q.dtype)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        Q, K, V, sl, ids, pre, y, lse = ctx.saved_tensors
+        Q, K, V, sl, ids, pre, y, rest, lse = ctx.saved_tensors
         if Q.numel() == 0:
             return tuple(torch.zeros_like(t) for t in (Q, K, V)) + (None,) * 7
         B, N, H, D = Q.shape
@@ -141,8 +142,8 @@ class SoftmaxAttention(autograd.Function):
         with _on(Q.device):
             rc = lib.flare_attn_backward(
                 P(q), P(k), P(v), _strides(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3]), _lib.dtype_code(dtype),
-                B, N, H, G, D, scale, softcap, P(sl), int(causal), P(ids), P(pre), P(y), P(lse), P(g), P(dq), P(dk),
-                P(dv), P(ws), nbytes, _raw_stream(Q.device.index))
+                B, N, H, G, D, scale, softcap, P(sl), int(causal), P(ids), P(pre), P(y), P(rest), P(lse), P(g), P(dq),
+                P(dk), P(dv), P(ws), nbytes, _raw_stream(Q.device.index))
         _lib.check(rc, "flare_attn_backward")
         return (dq.to(Q.dtype), dk.to(K.dtype), dv.to(V.dtype)) + (None,) * 7
 
@@ -223,7 +224,7 @@ def softmax_attention_prefill(
         _lib.check(rc, "flare_attn_append")
         rc = lib.flare_attn_forward(
             P(q), P(kc), P(vc), _strides(*q.stride()[:3], *kc.stride()[:3], *vc.stride()[:3]), code, B, T, S, H, G, D,
-            _resolve_attn_scale(scale, D), cap, P(sl), 1, None, P(pre), P(lens), P(new), P(y), None, P(ws), nbytes,
+            _resolve_attn_scale(scale, D), cap, P(sl), 1, None, P(pre), P(lens), P(new), P(y), None, None, P(ws), nbytes,
             stream)
     _lib.check(rc, "flare_attn_forward")
     return y, cache

@@ -50,6 +50,7 @@ struct Rows {                        // a [B, n, heads, D] tensor: element strid
 struct AttnArgs {
     Rows q, k, v;
     void* y;                         // [B, N, H, D]
+    void* y_rest;                    // [B, N, H, D] or NULL: what y was rounded by, for the backward's dy . y
     float* lse;                      // [B, H, N], log2 units; +inf for a row that sees nothing
     const float* slopes;             // [H]
     const int32_t *ids, *prefix;     // [B, N], [B]
@@ -75,6 +76,15 @@ struct AttnArgs {
 constexpr int q_tiles(int size) { return size == 2 ? 2 : 1; }
 // Tiles of 16 keys a wave of the key gradients' kernel owns.
 constexpr int kv_tiles(int size, int DP) { return size == 2 && DP <= 64 ? 2 : 1; }
+
+// Four dimensions of a row of y at element `at`, and what they are rounded by.
+template <typename S>
+__device__ __forceinline__ void put_y(const AttnArgs& p, int64_t at, f32x4 o) {
+    typedef S S4 __attribute__((ext_vector_type(4)));
+    const S4 y = __builtin_convertvector(o, S4);
+    *reinterpret_cast<S4*>((S*)p.y + at) = y;
+    if (p.y_rest) *reinterpret_cast<S4*>((S*)p.y_rest + at) = __builtin_convertvector(o - __builtin_convertvector(y, f32x4), S4);
+}
 
 // Ids as the kernels compare them: padding's negative ones are those of no key and of no query.
 constexpr int kNoKey = -1, kNoQuery = -2;

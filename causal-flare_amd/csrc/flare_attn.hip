@@ -190,17 +190,17 @@ extern "C" int flare_attn_forward(const void* q, const void* k, const void* v, c
                                   int64_t B, int64_t N, int64_t M, int64_t H, int64_t G, int64_t D, float scale,
                                   float softcap, const float* slopes, int causal, const int32_t* document_ids,
                                   const int32_t* prefix_lengths, const int32_t* lengths, const int32_t* new_lengths,
-                                  void* y, float* lse, void* workspace, size_t workspace_bytes, void* stream) {
+                                  void* y, void* y_rest, float* lse, void* workspace, size_t workspace_bytes, void* stream) {
     FLARE_REQUIRE(q && k && v && strides && y, "flare_attn_forward: null pointer");
     ATTN_REQUIRE_SIZES("flare_attn_forward");
     FLARE_REQUIRE(lengths || M == N, "flare_attn_forward: as many keys as queries without a cache");
     FLARE_REQUIRE(!(document_ids && lengths), "flare_attn_forward: document_ids exclude a cache");
     FLARE_REQUIRE(lengths || !new_lengths, "flare_attn_forward: new_lengths without lengths");
     AttnArgs p = attn_args(q, k, v, strides, B, N, M, H, G, D, scale, softcap, slopes);
-    FLARE_REQUIRE(aligned(p.q, dtype) && aligned(p.k, dtype) && aligned(p.v, dtype) && ((uintptr_t)y & 15) == 0,
+    FLARE_REQUIRE(aligned(p.q, dtype) && aligned(p.k, dtype) && aligned(p.v, dtype) && (((uintptr_t)y | (uintptr_t)y_rest) & 15) == 0,
                   "flare_attn_forward: rows must be 16-byte aligned and less than 2^22 elements apart");
     p.causal = causal, p.ids = document_ids, p.prefix = prefix_lengths, p.lengths = lengths, p.fresh = new_lengths;
-    p.y = y, p.lse = lse;
+    p.y = y, p.y_rest = y_rest, p.lse = lse;
     split_forward(p, dtype);
     p.parts = (float*)((char*)workspace + forward_head_bytes(B, N));
     if (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < forward_head_bytes(B, N) + rows_bytes(p)) {
@@ -226,7 +226,8 @@ extern "C" size_t flare_attn_backward_workspace_size(int64_t B, int64_t N, int64
 extern "C" int flare_attn_backward(const void* q, const void* k, const void* v, const int64_t* strides, int dtype,
                                    int64_t B, int64_t N, int64_t H, int64_t G, int64_t D, float scale, float softcap,
                                    const float* slopes, int causal, const int32_t* document_ids,
-                                   const int32_t* prefix_lengths, const void* y, const float* lse, const void* dy,
+                                   const int32_t* prefix_lengths, const void* y, const void* y_rest,
+                                   const float* lse, const void* dy,
                                    void* dq, void* dk, void* dv, void* workspace, size_t workspace_bytes,
                                    void* stream) {
     const int64_t M = N;
@@ -234,7 +235,7 @@ extern "C" int flare_attn_backward(const void* q, const void* k, const void* v, 
                   "flare_attn_backward: null pointer");
     ATTN_REQUIRE_SIZES("flare_attn_backward");
     AttnArgs p = attn_args(q, k, v, strides, B, N, M, H, G, D, scale, softcap, slopes);
-    const uintptr_t out = (uintptr_t)y | (uintptr_t)dy | (uintptr_t)dq | (uintptr_t)dk | (uintptr_t)dv;
+    const uintptr_t out = (uintptr_t)y | (uintptr_t)y_rest | (uintptr_t)dy | (uintptr_t)dq | (uintptr_t)dk | (uintptr_t)dv;
     FLARE_REQUIRE(aligned(p.q, dtype) && aligned(p.k, dtype) && aligned(p.v, dtype) && (out & 15) == 0 &&
                   ((uintptr_t)workspace & 15) == 0, "flare_attn_backward: rows must be 16-byte aligned and less than 2^22 elements apart");
     if (workspace_bytes < flare_attn_backward_workspace_size(B, N, H, G, D, dtype)) {
@@ -243,7 +244,7 @@ extern "C" int flare_attn_backward(const void* q, const void* k, const void* v, 
     }
     float* delta = (float*)workspace;
     p.causal = causal, p.ids = document_ids, p.prefix = prefix_lengths;
-    p.y = const_cast<void*>(y), p.lse = const_cast<float*>(lse), p.dy = dy, p.delta = delta;
+    p.y = const_cast<void*>(y), p.y_rest = const_cast<void*>(y_rest), p.lse = const_cast<float*>(lse), p.dy = dy, p.delta = delta;
     p.dq = dq, p.dk = dk, p.dv = dv;
     split_backward(p, dtype);
     p.parts = (float*)((char*)workspace + backward_head_bytes(B, N, H));

@@ -318,14 +318,13 @@ __global__ __launch_bounds__(256, 2) void attn_forward_kernel(AttnArgs p) {
         }
         if (p.lse && g == 0)
             p.lse[(b * p.H + h) * p.N + i] = total == 0.0f ? -kNegInf : top[t] + __builtin_amdgcn_logf(total);
-        S* row = (S*)p.y + ((b * p.N + i) * p.H + h) * p.D;
+        const int64_t row = ((b * p.N + i) * p.H + h) * p.D;
 #pragma unroll
         for (int d = 0; d < DT; ++d) {
             if (16 * d < p.D) {
                 f32x4 o = acc[t][d] * inv;
                 if (refused) o = f32x4{__builtin_nanf(""), __builtin_nanf(""), __builtin_nanf(""), __builtin_nanf("")};
-                typedef S S4 __attribute__((ext_vector_type(4)));
-                *reinterpret_cast<S4*>(row + 16 * d + 4 * g) = __builtin_convertvector(o, S4);
+                put_y<S>(p, row + 16 * d + 4 * g, o);
             }
         }
     }
@@ -335,7 +334,6 @@ __global__ __launch_bounds__(256, 2) void attn_forward_kernel(AttnArgs p) {
 template <typename E>
 __global__ __launch_bounds__(256) void attn_rows_kernel(AttnArgs p) {
     typedef typename Elem<E>::S S;
-    typedef S S4 __attribute__((ext_vector_type(4)));
     const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);             // (b, h, i)
     const int d = (threadIdx.x & 31) * 4;
     if (row >= p.B * p.H * p.N || d >= p.D) return;
@@ -355,7 +353,7 @@ __global__ __launch_bounds__(256) void attn_rows_kernel(AttnArgs p) {
         const int64_t off = p.lengths[b], n = p.fresh ? clamp_to(p.fresh[b], p.N) : p.N;
         if (off >= 0 && off + n > p.M) v = f32x4{__builtin_nanf(""), __builtin_nanf(""), __builtin_nanf(""), __builtin_nanf("")};
     }
-    *reinterpret_cast<S4*>((S*)p.y + ((b * p.N + i) * p.H + h) * p.D + d) = __builtin_convertvector(v, S4);
+    put_y<S>(p, ((b * p.N + i) * p.H + h) * p.D + d, v);
     if (p.lse && d == 0) p.lse[row] = total == 0.0f ? -kNegInf : top + __builtin_amdgcn_logf(total);
 }
 

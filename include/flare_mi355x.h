@@ -395,7 +395,8 @@ int flare_scan_step(const void* x, const void* dt, const float* A, const void* B
  * caches of M rows, the queries are at positions lengths[b] + i, and new_lengths[b] of them (all
  * if NULL) are real, whose keys are in the caches already (flare_attn_append); lengths[b] < 0: y =
  * 0; lengths[b] + new_lengths[b] > M: y is NaN.  document_ids exclude lengths.
- * A query that sees nothing has y = 0.  lse [B, H, N] or NULL receives log2 of the sum
+ * A query that sees nothing has y = 0.  y_rest [B,
+ * N, H, D] or NULL receives what y was rounded by (16-bit types; for the backward).  lse [B, H, N] or NULL receives log2 of the sum
  * of exp(s_ij).
  */
 size_t flare_attn_forward_workspace_size(int64_t B, int64_t N, int64_t M, int64_t H, int64_t D, int dtype);
@@ -403,14 +404,14 @@ int flare_attn_forward(const void* q, const void* k, const void* v, const int64_
                        int64_t N, int64_t M, int64_t H, int64_t G, int64_t D, float scale, float softcap,
                        const float* slopes, int causal, const int32_t* document_ids,
                        const int32_t* prefix_lengths, const int32_t* lengths, const int32_t* new_lengths, void* y,
-                       float* lse, void* workspace, size_t workspace_bytes, void* stream);
+                       void* y_rest, float* lse, void* workspace, size_t workspace_bytes, void* stream);
 
-/* Its gradients without a cache, from y, lse and dy [B, N, H, D]: dq [B, N, H, D], dk, dv [B, N, G, D]. */
+/* Its gradients without a cache, from y, y_rest (or NULL), lse and dy [B, N, H, D]: dq [B, N, H, D], dk, dv [B, N, G, D]. */
 size_t flare_attn_backward_workspace_size(int64_t B, int64_t N, int64_t H, int64_t G, int64_t D, int dtype);
 int flare_attn_backward(const void* q, const void* k, const void* v, const int64_t* strides, int dtype, int64_t B,
                         int64_t N, int64_t H, int64_t G, int64_t D, float scale, float softcap, const float* slopes,
                         int causal, const int32_t* document_ids, const int32_t* prefix_lengths, const void* y,
-                        const float* lse, const void* dy, void* dq, void* dk, void* dv, void* workspace,
+                        const void* y_rest, const float* lse, const void* dy, void* dq, void* dk, void* dv, void* workspace,
                         size_t workspace_bytes, void* stream);
 
 /* Rows k, v [B, N, G, D] (strides: batch, token and head of k, v; 6 numbers, host) to positions

@@ -121,21 +121,22 @@ def test_c_entry_points_check_before_they_launch():
         chunk = lib.flare_scan_chunk(1, 10 ** 7, 64, states, 1, 1)
         assert 1 <= chunk <= 128 and chunk % lib.flare_scan_kept_tokens(states) == 0
     attn = [P, P, P, nine, 1]
-    assert _refused(lib.flare_attn_forward(*attn, 1, 4, 4, 4, 3, 64, 1.0, 0.0, None, 1, None, None, None, None, P, None, None,
+    assert _refused(lib.flare_attn_forward(*attn, 1, 4, 4, 4, 3, 64, 1.0, 0.0, None, 1, None, None, None, None, P, None, None, None,
                                            0, None), b"divide")
-    assert _refused(lib.flare_attn_forward(*attn, 1, 4, 4, 4, 4, 24, 1.0, 0.0, None, 1, None, None, None, None, P, None, None,
+    assert _refused(lib.flare_attn_forward(*attn, 1, 4, 4, 4, 4, 24, 1.0, 0.0, None, 1, None, None, None, None, P, None, None, None,
                                            0, None), b"multiple of 16")
-    assert _refused(lib.flare_attn_forward(*attn, 1, 4, 5, 4, 4, 64, 1.0, 0.0, None, 1, None, None, None, None, P, None, None,
+    assert _refused(lib.flare_attn_forward(*attn, 1, 4, 5, 4, 4, 64, 1.0, 0.0, None, 1, None, None, None, None, P, None, None, None,
                                            0, None), b"without a cache")
     assert _refused(lib.flare_attn_forward(*attn, 1, 4, 4, 4, 4, 64, 1.0, -1.0, None, 1, None, None, None, None, P, None,
-                                           None, 0, None), b"cap")
+                                           None, None, 0, None), b"cap")
     assert _refused(lib.flare_attn_forward(P, P, ctypes.c_void_p(4098), nine, 1, 1, 4, 4, 4, 4, 64, 1.0, 0.0, None, 1, None,
-                                           None, None, None, P, None, None, 0, None), b"16-byte")
-    assert lib.flare_attn_forward(*attn, 1, 4, 4, 4, 4, 64, 1.0, 0.0, None, 1, P, None, None, None, P, None, None, 0,
-                                  None) == -3
-    assert lib.flare_attn_forward(*attn, 1, 4000, 4000, 1, 1, 64, 1.0, 0.0, None, 1, None, None, None, None, P, None, P, 4096,
-                                  None) == -3
-    assert lib.flare_attn_backward(*attn, 1, 4, 4, 4, 64, 1.0, 0.0, None, 1, None, None, P, P, P, P, P, P, P, 0, None) == -3
+                                           None, None, None, P, None, None, None, 0, None), b"16-byte")
+    assert lib.flare_attn_forward(*attn, 1, 4, 4, 4, 4, 64, 1.0, 0.0, None, 1, P, None, None, None, P, None, None, None,
+                                  0, None) == -3
+    assert lib.flare_attn_forward(*attn, 1, 4000, 4000, 1, 1, 64, 1.0, 0.0, None, 1, None, None, None, None, P, None, None, P,
+                                  4096, None) == -3
+    assert lib.flare_attn_backward(*attn, 1, 4, 4, 4, 64, 1.0, 0.0, None, 1, None, None, P, None, P, P, P, P, P, P, 0,
+                                   None) == -3
     assert _refused(lib.flare_attn_append(P, P, six, 1, 1, 4, 8, 4, 64, None, None, P, P, None), b"null pointer")
     assert lib.flare_attn_step(P, P, P, six, 1, 1, 4096, 4, 4, 64, 1.0, 0.0, None, P, P, P, P, None, 0, None) == -3
 
