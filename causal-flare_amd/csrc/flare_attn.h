@@ -140,6 +140,28 @@ __device__ __forceinline__ f16x8 frag_tiles(f32x4 a, f32x4 b, f16) {
 __device__ __forceinline__ f32x8 frag_tiles(f32x4 a, f32x4 b, float) {
     return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
 }
+// The same, and what that rounds the values by as an operand of its own.
+__device__ __forceinline__ bf16x8 split_tiles(f32x4 a, f32x4 b, bf16x8& rest, bf16 type) {
+    // the upper half of each value; the rest is exact in fp32
+    auto pack = [](f32x4 v) {
+        typedef bf16 v4 __attribute__((ext_vector_type(4)));
+        const u32x4 u = __builtin_bit_cast(u32x4, v);
+        const u32x2 hi = {__builtin_amdgcn_perm(u[1], u[0], 0x07060302u), __builtin_amdgcn_perm(u[3], u[2], 0x07060302u)};
+        return __builtin_bit_cast(v4, hi);
+    };
+    auto left = [](f32x4 v) {
+        return v - __builtin_bit_cast(f32x4, __builtin_bit_cast(u32x4, v) & 0xffff0000u);
+    };
+    rest = frag_tiles(left(a), left(b), type);
+    return __builtin_shufflevector(pack(a), pack(b), 0, 1, 2, 3, 4, 5, 6, 7);
+}
+__device__ __forceinline__ f16x8 split_tiles(f32x4 a, f32x4 b, f16x8& rest, f16 type) {
+    typedef f16 v4 __attribute__((ext_vector_type(4)));
+    const v4 ha = __builtin_convertvector(a, v4), hb = __builtin_convertvector(b, v4);
+    rest = frag_tiles(a - __builtin_convertvector(ha, f32x4), b - __builtin_convertvector(hb, f32x4), type);
+    return __builtin_shufflevector(ha, hb, 0, 1, 2, 3, 4, 5, 6, 7);
+}
+__device__ __forceinline__ f32x8 split_tiles(f32x4 a, f32x4 b, f32x8&, float type) { return frag_tiles(a, b, type); }
 // Rows 4g+i and 16+4g+i of column c of a tile in LDS (rows `pitch` apart): the operand that
 // goes with frag_tiles.
 template <typename E>

@@ -225,15 +225,18 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnArgs p) {
                 }
             }
             const bool odd = (oddl[buf * 4] | oddl[buf * 4 + 1] | oddl[buf * 4 + 2] | oddl[buf * 4 + 3]) != 0;
-            Frag w[QT];
+            Frag w[QT], rest[QT];
 #pragma unroll
-            for (int t = 0; t < QT; ++t) w[t] = frag_tiles(s[t][0], s[t][1], S{});
+            for (int t = 0; t < QT; ++t) w[t] = split_tiles(s[t][0], s[t][1], rest[t], S{});
 #pragma unroll
             for (int d = 0; d < DT; ++d) {
                 Frag a = frag_columns<E>(kt + 16 * d, P, g, c);
                 if (odd) a = finite(a);                 // 0 times an infinite value is NaN
 #pragma unroll
-                for (int t = 0; t < QT; ++t) acc[t][d] = mma(a, w[t], acc[t][d]);
+                for (int t = 0; t < QT; ++t) {
+                    acc[t][d] = mma(a, w[t], acc[t][d]);
+                    if (sizeof(E) == 2) acc[t][d] = mma(a, rest[t], acc[t][d]);
+                }
             }
         }
         if (k1 < kv_end) place(k1, buf ^ 1);
@@ -449,11 +452,11 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(AttnArgs p) {
                         }
                     }
                 }
-                Frag w[KQ], ds[KQ];
+                Frag w[KQ], ds[KQ], rest[KQ];
 #pragma unroll
                 for (int t = 0; t < KQ; ++t) {
                     w[t] = frag_tiles(s[t][0], s[t][1], S{});
-                    ds[t] = frag_tiles(dp[t][0], dp[t][1], S{});
+                    ds[t] = split_tiles(dp[t][0], dp[t][1], rest[t], S{});
                 }
 #pragma unroll
                 for (int d = 0; d < DT; ++d) {
@@ -462,6 +465,7 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(AttnArgs p) {
 #pragma unroll
                     for (int t = 0; t < KQ; ++t) {
                         dk[t][d] = mma(a, ds[t], dk[t][d]);
+                        if (sizeof(E) == 2) dk[t][d] = mma(a, rest[t], dk[t][d]);
                         dv[t][d] = mma(o, w[t], dv[t][d]);
                     }
                 }
