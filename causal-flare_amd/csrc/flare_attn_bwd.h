@@ -57,7 +57,8 @@ template <typename E> constexpr float weight_shift() { return __is_same(E, __hal
 
 template <typename E, int DP>
 struct BackwardLds {
-    static constexpr int T = 32, P = column_pitch<E, DP>();            // rows of a tile; read both ways
+    static constexpr int T = sizeof(E) == 2 ? 64 : 32;                 // rows of a tile, taken 32 at a time
+    static constexpr int P = column_pitch<E, DP>();                    // read both ways
     static constexpr size_t tile = sizeof(E) * T * P;
     static constexpr size_t bytes = 4 * tile + 2 * (3 * T + 4) * sizeof(float);
 };
@@ -131,9 +132,9 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnArgs p) {
         for (int d = 0; d < DT; ++d) acc[t][d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     }
 
-    auto covers = [&](int k0, int first, int last) {
-        if (k0 + KT > N || last >= N) return false;
-        if (p.causal && k0 + KT - 1 > first && k0 + KT > prefix) return false;
+    auto covers = [&](int k0, int rows, int first, int last) {
+        if (k0 + rows > N || last >= N) return false;
+        if (p.causal && k0 + rows - 1 > first && k0 + rows > prefix) return false;
         return !p.ids || mine.same(id_range(p, b, k0 / kIdTile));
     };
     Stage<E, KT, DP, P, 256> ks, vs;
@@ -149,24 +150,28 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnArgs p) {
         ks.store(kl + buf * KT * P, tid);
         vs.store(vl + buf * KT * P, tid);
         if (p.ids && tid < KT) idl[buf * KT + tid] = next_id;
-        const bool odd = !covers(k0, q0, q0 + QB - 1) && __any(ks.odd());
+        const bool odd = !covers(k0, KT, q0, q0 + QB - 1) && __any(ks.odd());
         if (lane == 0) oddl[buf * 4 + wave] = odd;
     };
     TileWalk<KT> walk(p, b, kv_end, mine);
-    int k0 = walk.next(0);
+    int tile = walk.next(0);
     int buf = 0;
-    if (k0 < kv_end) {
-        fetch(k0);
-        place(k0, 0);
+    if (tile < kv_end) {
+        fetch(tile);
+        place(tile, 0);
     }
     __syncthreads();
-    while (k0 < kv_end) {
-        const int k1 = walk.next(k0 + KT);
+    while (tile < kv_end) {
+        const int k1 = walk.next(tile + KT);
         if (k1 < kv_end) fetch(k1);
-        const bool hidden = w0 >= N || (p.causal && k0 > w0 + 16 * QT - 1 && k0 >= prefix);
-        if (!hidden) {
-            const S* kt = kl + buf * KT * P;
-            const S* vt = vl + buf * KT * P;
+        const bool odd = (oddl[buf * 4] | oddl[buf * 4 + 1] | oddl[buf * 4 + 2] | oddl[buf * 4 + 3]) != 0;
+#pragma unroll 1
+        for (int part = 0; part < KT; part += 32) {
+            const int k0 = tile + part;
+            const bool hidden = w0 >= N || k0 >= N || (p.causal && k0 > w0 + 16 * QT - 1 && k0 >= prefix);
+            if (hidden) continue;
+            const S* kt = kl + (buf * KT + part) * P;
+            const S* vt = vl + (buf * KT + part) * P;
             f32x4 s[QT][2], dp[QT][2];
 #pragma unroll
             for (int t = 0; t < QT; ++t)
@@ -185,7 +190,7 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnArgs p) {
                     }
                 }
             }
-            const bool whole = covers(k0, w0, w0 + 16 * QT - 1);
+            const bool whole = covers(k0, 32, w0, w0 + 16 * QT - 1);
 #pragma unroll
             for (int t = 0; t < QT; ++t) {
                 const float base = (float)(pos[t] - k0 - 4 * g);
@@ -215,7 +220,7 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnArgs p) {
 #pragma unroll
                         for (int i = 0; i < 4; ++i) s[t][n][i] = 16 * n + i < left ? s[t][n][i] : 0.0f;
                         if (p.ids) {
-                            const int4 d = *reinterpret_cast<const int4*>(idl + buf * KT + 16 * n + 4 * g);
+                            const int4 d = *reinterpret_cast<const int4*>(idl + buf * KT + part + 16 * n + 4 * g);
                             s[t][n][0] = d.x == qid[t] ? s[t][n][0] : 0.0f;
                             s[t][n][1] = d.y == qid[t] ? s[t][n][1] : 0.0f;
                             s[t][n][2] = d.z == qid[t] ? s[t][n][2] : 0.0f;
@@ -224,7 +229,6 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnArgs p) {
                     }
                 }
             }
-            const bool odd = (oddl[buf * 4] | oddl[buf * 4 + 1] | oddl[buf * 4 + 2] | oddl[buf * 4 + 3]) != 0;
             Frag w[QT], rest[QT];
 #pragma unroll
             for (int t = 0; t < QT; ++t) w[t] = split_tiles(s[t][0], s[t][1], rest[t], S{});
@@ -242,7 +246,7 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnArgs p) {
         if (k1 < kv_end) place(k1, buf ^ 1);
         __syncthreads();
         buf ^= 1;
-        k0 = k1;
+        tile = k1;
     }
 #pragma unroll
     for (int t = 0; t < QT; ++t) {
@@ -330,8 +334,8 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(AttnArgs p) {
 #pragma unroll
         for (int d = 0; d < DT; ++d) dk[t][d] = dv[t][d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 
-    auto covers = [&](int q0, int first, int last) {
-        if (q0 + QR > N || last >= N) return false;
+    auto covers = [&](int q0, int rows, int first, int last) {
+        if (q0 + rows > N || last >= N) return false;
         if (p.causal && last > q0 && last >= prefix) return false;
         return !p.ids || mine.same(id_range(p, b, q0 / kIdTile));
     };
@@ -356,7 +360,7 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(AttnArgs p) {
     // they are in have a log-sum-exp or a delta that is none, and their weights are NaN then.
     auto place = [&](int q0, int buf) {
         bool odd = false;
-        if (!covers(q0, kb, kb + KB - 1)) {
+        if (!covers(q0, QR, kb, kb + KB - 1)) {
             if (qs.odd()) {
                 odd = true;
                 qs.clean();
@@ -381,19 +385,23 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(AttnArgs p) {
         const int h = kvh * R + rep;
         const float slope2 = p.slopes ? p.slopes[h] * kLog2e : 0.0f;
         TileWalk<QR> walk(p, b, q_end, mine);
-        int q0 = walk.next(q_begin);
-        if (q0 < q_end) {
-            fetch(h, q0);
-            place(q0, buf);
+        int tile = walk.next(q_begin);
+        if (tile < q_end) {
+            fetch(h, tile);
+            place(tile, buf);
         }
         __syncthreads();
-        while (q0 < q_end) {
-            const int q1 = walk.next(q0 + QR);
+        while (tile < q_end) {
+            const int q1 = walk.next(tile + QR);
             if (q1 < q_end) fetch(h, q1);
-            const bool hidden = w0 >= N || (p.causal && w0 > q0 + QR - 1 && w0 >= prefix);
-            if (!hidden) {
-                const S* qt = ql + buf * QR * P;
-                const S* gt = gl + buf * QR * P;
+            const bool odd = (oddl[buf * 4] | oddl[buf * 4 + 1] | oddl[buf * 4 + 2] | oddl[buf * 4 + 3]) != 0;
+#pragma unroll 1
+            for (int from_row = 0; from_row < QR; from_row += 32) {
+                const int q0 = tile + from_row;
+                const bool hidden = w0 >= N || q0 >= N || (p.causal && w0 > q0 + 31 && w0 >= prefix);
+                if (hidden) continue;
+                const S* qt = ql + (buf * QR + from_row) * P;
+                const S* gt = gl + (buf * QR + from_row) * P;
                 f32x4 s[KQ][2], dp[KQ][2];
 #pragma unroll
                 for (int t = 0; t < KQ; ++t)
@@ -412,12 +420,11 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(AttnArgs p) {
                         }
                     }
                 }
-                const bool whole = covers(q0, w0, w0 + 16 * KQ - 1);
-                const bool odd = (oddl[buf * 4] | oddl[buf * 4 + 1] | oddl[buf * 4 + 2] | oddl[buf * 4 + 3]) != 0;
+                const bool whole = !odd && covers(q0, 32, w0, w0 + 16 * KQ - 1);
 #pragma unroll
                 for (int n = 0; n < 2; ++n) {
-                    const f32x4 lse = *reinterpret_cast<const f32x4*>(lsel + buf * QR + 16 * n + 4 * g);
-                    const f32x4 delta = *reinterpret_cast<const f32x4*>(dell + buf * QR + 16 * n + 4 * g);
+                    const f32x4 lse = *reinterpret_cast<const f32x4*>(lsel + buf * QR + from_row + 16 * n + 4 * g);
+                    const f32x4 delta = *reinterpret_cast<const f32x4*>(dell + buf * QR + from_row + 16 * n + 4 * g);
 #pragma unroll
                     for (int t = 0; t < KQ; ++t) {
                         const float base = (float)(q0 + 4 * g - (w0 + 16 * t + c));
@@ -439,7 +446,7 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(AttnArgs p) {
                         }
                         if (!whole) {
                             const int late = from[t] - q0 - 4 * g - 16 * n;
-                            const int4 d = *reinterpret_cast<const int4*>(idl + buf * QR + 16 * n + 4 * g);
+                            const int4 d = *reinterpret_cast<const int4*>(idl + buf * QR + from_row + 16 * n + 4 * g);
                             const int row_id[4] = {d.x, d.y, d.z, d.w};
 #pragma unroll
                             for (int i = 0; i < 4; ++i) {
@@ -473,7 +480,7 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(AttnArgs p) {
             if (q1 < q_end) place(q1, buf ^ 1);
             __syncthreads();
             buf ^= 1;
-            q0 = q1;
+            tile = q1;
         }
     }
 #pragma unroll

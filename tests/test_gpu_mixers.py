@@ -506,16 +506,27 @@ def test_attention_keeps_infinite_values_to_who_sees_them(dtype, where):
             assert sees.isnan().all() if math.isnan(poison) else (sees == poison).all()
         else:
             assert not y1[0, at, 0].isfinite().all()
-    # a gradient that is infinite in one row stays with the keys that row sees
+    # a gradient that is infinite in one row stays with the keys that row sees, and reaches them all
     leaves = [t[n].clone().requires_grad_() for n in ("q", "k", "v")]
     dirty = dy.clone()
     dirty[0, at, 0, 5] = float("inf")
-    y = cf.softmax_attention(*leaves, document_ids=ids)
-    clean, got = torch.autograd.grad(y, leaves, dy, retain_graph=True), torch.autograd.grad(y, leaves, dirty)
-    assert torch.equal(clean[0][:, apart], got[0][:, apart])
-    for i in (1, 2):
-        assert torch.equal(clean[i][:, at + 1:], got[i][:, at + 1:])
-        assert not got[i][0, :at + 1, 0].isfinite().all(-1).any()
+    for o in ({"document_ids": ids}, {}):
+        y = cf.softmax_attention(*leaves, **o)
+        clean, got = torch.autograd.grad(y, leaves, dy, retain_graph=True), torch.autograd.grad(y, leaves, dirty)
+        rows = [i for i in range(N) if i != at]
+        assert torch.equal(clean[0][:, rows], got[0][:, rows])
+        for i in (1, 2):
+            assert torch.equal(clean[i][:, at + 1:], got[i][:, at + 1:])
+            assert not got[i][0, :at + 1, 0].isfinite().all(-1).any()
+    # without documents a key that is infinite is seen by every later query
+    if where != "v":
+        dirty = {n: v.clone() for n, v in t.items()}
+        dirty[where][0, at, 0, 5] = float("inf")
+        leaves = [dirty[n].requires_grad_() for n in ("q", "k", "v")]
+        grads = torch.autograd.grad(cf.softmax_attention(*leaves), leaves, dy)
+        seen = range(at + 1) if where == "q" else range(N)
+        assert not grads[1][0, [*seen][:at + 1], 0].isfinite().all(-1).any()
+        assert all(x[:, :, 1].isfinite().all() for x in grads)
 
 
 def test_a_query_that_sees_nothing():
