@@ -43,7 +43,7 @@ from ._inputs import (
 
 
 def _check_scores(name, H, scale, softcap, slopes):
-    """(scale or None, cap or 0) of checked arguments."""
+    """The cap, 0 for none, of checked arguments."""
     _check_shape(name, "slopes", slopes, (H,))
     _check_float(name, slopes=slopes)
     if slopes is not None and slopes.requires_grad and torch.is_grad_enabled():

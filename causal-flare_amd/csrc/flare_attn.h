@@ -65,6 +65,8 @@ struct AttnArgs {
     const float* delta;              // [B, H, N]: dy . y
     void *dq, *dk, *dv;
     int64_t row_splits;              // of `splits`: parts of the rows, times parts of the heads
+    float* dq_parts;                 // what `dq_splits` workgroups leave of each row of dq
+    int64_t dq_splits;
     // single tokens
     const void *k_new, *v_new;       // [B, G, D]
     int64_t kn_sb, kn_sg, vn_sb, vn_sg;
@@ -346,6 +348,40 @@ struct TileWalk {
         return k;
     }
 };
+
+// What `splits` workgroups left of a row, joined: D floats each, and behind them the reference and the
+// sum, `stride` apart.  Parts `from`, from + STEP, .. of the dimensions d .. d+3; U of them are under way at
+// a time, as one after the other their latency is all that a row costs.
+struct Joined {
+    float top, total;
+    f32x4 v;
+    __device__ __forceinline__ void add(float t, float sum, f32x4 o) {
+        const float to = fmaxf(top, t);
+        const float mine = top == to ? 1.0f : __builtin_amdgcn_exp2f(top - to);
+        const float its = t == to ? 1.0f : __builtin_amdgcn_exp2f(t - to);
+        top = to;
+        total = total * mine + sum * its;
+        v = v * mine + o * its;
+    }
+};
+template <int STEP, int U>
+__device__ __forceinline__ Joined join_parts(const float* part, int from, int splits, int64_t D, int d) {
+    const int64_t stride = D + 4;
+    Joined j{kNegInf, 0.0f, f32x4{0.0f, 0.0f, 0.0f, 0.0f}};
+    for (int s0 = from; s0 < splits; s0 += U * STEP) {
+        f32x4 o[U], end[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const float* q = part + min(s0 + u * STEP, splits - 1) * stride;
+            o[u] = *reinterpret_cast<const f32x4*>(q + d);
+            end[u] = *reinterpret_cast<const f32x4*>(q + D);
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (s0 + u * STEP < splits) j.add(end[u][0], end[u][1], o[u]);
+    }
+    return j;
+}
 
 }  // namespace attn
 }  // namespace flare

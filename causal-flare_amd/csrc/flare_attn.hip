@@ -112,24 +112,36 @@ static int launch_ids(AttnArgs& p, int dtype, bool keys, int32_t* stats, hipStre
     return check_launch("attn_order");
 }
 
-// Parts that the queries of each block of keys are split into: so many that there are 2048
-// workgroups (eight a CU: blocks of keys cost very different amounts of work under a causal or
-// document mask), the heads first and then the rows, in parts of 256 or more.
+// Parts that the queries of each block of keys are split into (blocks of keys cost very different
+// amounts of work under a causal or document mask): the heads that share them until there are 2048
+// workgroups, and then the rows until there are 1024, in parts of 256 or more.  us, the parts' sums
+// included: 16384 rows, 16 heads of 128 over 4, two parts 3245, one 3334; 2 x 2048 rows, 16 heads of 64,
+// four parts of the rows 113, two 94, one 99.  The keys of each block of rows likewise, for dq: 1024
+// workgroups for that call 54 us, 512 (one part) 80.
+constexpr int64_t kDqBlocks = 1024;
 static void split_backward(AttnArgs& p, int dtype) {
     const int64_t blocks = ceil_div(p.N, rows_of_keys(dtype, p.D));
     const int64_t R = p.H / p.G;
     int64_t want = ceil_div(2048, blocks * p.B * p.G);
     want = want > 8 ? 8 : want;
-    const int64_t heads = want < R ? want : R, rows = ceil_div(want, heads), most = ceil_div(p.N, 256);
+    const int64_t heads = want < R ? want : R, most = ceil_div(p.N, 256);
+    int64_t rows = ceil_div(1024, blocks * p.B * p.G * heads);
+    rows = rows * heads > 8 ? ceil_div(8, heads) : rows;
     p.row_splits = rows < most ? rows : most;
     p.splits = heads * p.row_splits;
+    const int64_t dq_want = ceil_div(kDqBlocks, ceil_div(p.N, rows_of_queries(dtype)) * p.B * p.H);
+    p.dq_splits = dq_want < most ? dq_want : most;
 }
 static size_t parts_bytes(const AttnArgs& p) {
     return p.splits == 1 ? 0 : (size_t)(p.splits * 2 * p.B * p.N * p.G * p.D) * sizeof(float);
 }
+static size_t dq_bytes(const AttnArgs& p) {
+    return p.dq_splits == 1 ? 0 : (size_t)(p.dq_splits * p.B * p.N * p.H * p.D) * sizeof(float);
+}
 
 // Parts that a row's keys are split into in the forward: two workgroups a CU (512) where the rows
-// leave less than that, in parts of 512 keys or more.
+// leave less than that, in parts of 512 keys or more.  us, the joining included, with parts and
+// without: 64 new tokens behind 8000, 16 heads of 128 over 4, 34 and 274; 2 x 512 behind 3000 55 and 118.
 static void split_forward(AttnArgs& p, int dtype) {
     const int64_t blocks = ceil_div(p.N, rows_of_queries(dtype)) * p.B * p.H, want = ceil_div(512, blocks);
     const int64_t most = ceil_div(p.M, 512);
@@ -146,10 +158,12 @@ static bool aligned(const Rows& r, int dtype) {
            r.sn < kMostStride;
 }
 
-// Workgroups of the step kernel for each sequence's keys: enough for four on each CU (1024 on
-// the card), and no more than the cache has shares of 128 keys.
+// Workgroups of the step kernel for each sequence's keys: enough for one on each CU (256 on the
+// card), whose four waves have the loads under way that its memory takes, and no more than the cache
+// has shares of 128 keys.  us, the joining included, for 256, 512 and 1024: 64 sequences of 8000
+// tokens, 4 key heads of 128, bf16, 182, 194, 198; 16 of them 47, 48, 50; one 13 with any.
 static int64_t step_splits(int64_t B, int64_t M, int64_t H, int64_t G) {
-    const int64_t rows = B * G * ceil_div(H / G, 16), s = ceil_div(1024, rows), most = ceil_div(M, 128);
+    const int64_t rows = B * G * ceil_div(H / G, 16), s = ceil_div(256, rows), most = ceil_div(M, 128);
     return s < 1 ? 1 : (s > most ? most : s);
 }
 
@@ -220,7 +234,7 @@ extern "C" size_t flare_attn_backward_workspace_size(int64_t B, int64_t N, int64
     AttnArgs p = {};
     p.B = B, p.N = N, p.H = H, p.G = G, p.D = D;
     split_backward(p, dtype);
-    return backward_head_bytes(B, N, H) + parts_bytes(p);
+    return backward_head_bytes(B, N, H) + parts_bytes(p) + dq_bytes(p);
 }
 
 extern "C" int flare_attn_backward(const void* q, const void* k, const void* v, const int64_t* strides, int dtype,
@@ -248,6 +262,7 @@ extern "C" int flare_attn_backward(const void* q, const void* k, const void* v, 
     p.dq = dq, p.dk = dk, p.dv = dv;
     split_backward(p, dtype);
     p.parts = (float*)((char*)workspace + backward_head_bytes(B, N, H));
+    p.dq_parts = (float*)((char*)p.parts + parts_bytes(p));
     const int rc = launch_ids(p, dtype, true, (int32_t*)(delta + B * H * N), (hipStream_t)stream);
     if (rc != FLARE_OK) return rc;
     return FLARE_BY_DTYPE(dtype, backward_e, (p, delta, (hipStream_t)stream));
@@ -273,7 +288,7 @@ extern "C" int flare_attn_append(const void* k, const void* v, const int64_t* st
 extern "C" size_t flare_attn_step_workspace_size(int64_t B, int64_t M, int64_t H, int64_t G, int64_t D) {
     if (B < 1 || M < 1 || G < 1 || H % G) return 0;
     const int64_t s = step_splits(B, M, H, G);
-    return s == 1 ? 0 : (size_t)(B * H * s * (D + 2)) * sizeof(float);
+    return s == 1 ? 0 : (size_t)(B * H * s * (D + 4)) * sizeof(float);
 }
 
 extern "C" int flare_attn_step(const void* q, const void* k, const void* v, const int64_t* strides, int dtype,
@@ -290,11 +305,11 @@ extern "C" int flare_attn_step(const void* q, const void* k, const void* v, cons
     p.v_new = v, p.vn_sb = strides[4], p.vn_sg = strides[5];
     const Rows kr = {k, strides[2], 0, strides[3]}, vr = {v, strides[4], 0, strides[5]};
     FLARE_REQUIRE(aligned(p.q, dtype) && aligned(kr, dtype) && aligned(vr, dtype) && aligned(p.k, dtype) &&
-                  aligned(p.v, dtype), "flare_attn_step: rows must be 16-byte aligned and less than 2^22 elements apart");
+                  aligned(p.v, dtype) && ((uintptr_t)y & 15) == 0, "flare_attn_step: rows must be 16-byte aligned and less than 2^22 elements apart");
     FLARE_REQUIRE(B * G * ceil_div(H / G, 16) <= 65535, "flare_attn_step: too large");
     p.splits = step_splits(B, M, H, G);
-    if (workspace_bytes < flare_attn_step_workspace_size(B, M, H, G, D) || (p.splits > 1 && !workspace)) {
-        set_error("flare_attn_step: workspace of %zu bytes is too small", workspace_bytes);
+    if (workspace_bytes < flare_attn_step_workspace_size(B, M, H, G, D) || (p.splits > 1 && (!workspace || ((uintptr_t)workspace & 15)))) {
+        set_error("flare_attn_step: workspace of %zu bytes is too small or not 16-byte aligned", workspace_bytes);
         return FLARE_ERR_WORKSPACE;
     }
     p.lengths = lengths, p.y = y, p.parts = (float*)workspace;

@@ -80,12 +80,19 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnArgs p) {
     int id = blockIdx.x;
     const int kvh = id % (int)p.G;
     id /= (int)p.G;
+    const int parts = (int)p.dq_splits, part_id = id % parts;      // of the keys
+    id /= parts;
     const QueryBlock at(p, id, R, nq);
     const int64_t b = at.b;
     const int h = kvh * R + at.rep, q0 = at.tile * QB;
 
     const int prefix = p.prefix ? (int)clamp_to(p.prefix[b], p.N) : 0;
-    const int kv_end = p.causal ? max(min(q0 + QB, N), prefix) : N;
+    int k_begin = 0, kv_end = p.causal ? max(min(q0 + QB, N), prefix) : N;
+    if (parts > 1) {
+        const int tiles = (kv_end + KT - 1) / KT;
+        k_begin = (int)((int64_t)tiles * part_id / parts) * KT;
+        kv_end = min(kv_end, (int)((int64_t)tiles * (part_id + 1) / parts) * KT);
+    }
     IdRange mine{0, 0, true};
     if (p.ids) mine = id_block(p, b, q0, QB);
     const int w0 = q0 + wave * 16 * QT;
@@ -154,7 +161,7 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnArgs p) {
         if (lane == 0) oddl[buf * 4 + wave] = odd;
     };
     TileWalk<KT> walk(p, b, kv_end, mine);
-    int tile = walk.next(0);
+    int tile = walk.next(k_begin);
     int buf = 0;
     if (tile < kv_end) {
         fetch(tile);
@@ -252,12 +259,15 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnArgs p) {
     for (int t = 0; t < QT; ++t) {
         const int i = w0 + 16 * t + c;
         if (i >= N) continue;
-        S* row = (S*)p.dq + ((b * p.N + i) * p.H + h) * p.D;
+        const int64_t row = ((b * p.N + i) * p.H + h) * p.D;
 #pragma unroll
         for (int d = 0; d < DT; ++d) {
             if (16 * d < p.D) {
                 typedef S S4 __attribute__((ext_vector_type(4)));
-                *reinterpret_cast<S4*>(row + 16 * d + 4 * g) = __builtin_convertvector(acc[t][d] * out_scale, S4);
+                const int64_t at = row + 16 * d + 4 * g;
+                const f32x4 v = acc[t][d] * out_scale;
+                if (parts > 1) *reinterpret_cast<f32x4*>(p.dq_parts + part_id * (p.B * p.N * p.H * p.D) + at) = v;
+                else *reinterpret_cast<S4*>((S*)p.dq + at) = __builtin_convertvector(v, S4);
             }
         }
     }
@@ -506,16 +516,28 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(AttnArgs p) {
     }
 }
 
-// The parts' sums, in order.
+// The parts' sums, in order: of dq (blockIdx.y 0), dk and dv, those that were split.
 template <typename E>
 __global__ __launch_bounds__(256) void attn_parts_kernel(AttnArgs p) {
     typedef typename Elem<E>::S S;
     typedef S S4 __attribute__((ext_vector_type(4)));
-    const int64_t all = p.B * p.N * p.G * p.D, at = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
-    if (at >= 2 * all) return;
+    constexpr int U = 4;
+    const int what = blockIdx.y;
+    const int64_t rows = p.B * p.N * p.D, all = rows * (what ? p.G : p.H), at = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
+    const int splits = (int)(what ? p.splits : p.dq_splits);
+    if (at >= all || splits == 1) return;
+    const int64_t stride = what ? 2 * all : all;
+    const float* from = (what ? p.parts + (what - 1) * all : p.dq_parts) + at;
     f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int64_t s = 0; s < p.splits; ++s) sum += *reinterpret_cast<const f32x4*>(p.parts + s * 2 * all + at);
-    S* to = at < all ? (S*)p.dk + at : (S*)p.dv + at - all;
+    for (int s0 = 0; s0 < splits; s0 += U) {
+        f32x4 v[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) v[u] = *reinterpret_cast<const f32x4*>(from + min(s0 + u, splits - 1) * stride);
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (s0 + u < splits) sum += v[u];
+    }
+    S* to = (S*)(what == 0 ? p.dq : what == 1 ? p.dk : p.dv) + at;
     *reinterpret_cast<S4*>(to) = __builtin_convertvector(sum, S4);
 }
 
@@ -540,11 +562,12 @@ static int backward_cap(const AttnArgs& p, hipStream_t stream) {
     if (rc == FLARE_OK) rc = allow_lds(dkv, bytes, "attn_dkv");
     if (rc != FLARE_OK) return rc;
     const int64_t blocks = ceil_div(p.N, 64 * QT) * p.B;
-    dq<<<dim3((unsigned)(blocks * p.H)), 256, bytes, stream>>>(p);
+    dq<<<dim3((unsigned)(blocks * p.H * p.dq_splits)), 256, bytes, stream>>>(p);
     if ((rc = check_launch("attn_dq")) != FLARE_OK) return rc;
     dkv<<<dim3((unsigned)(ceil_div(p.N, 64 * KQ) * p.B * p.G * p.splits)), 256, bytes, stream>>>(p);
-    if ((rc = check_launch("attn_dkv")) != FLARE_OK || p.splits == 1) return rc;
-    attn_parts_kernel<E><<<dim3((unsigned)ceil_div(p.B * p.N * p.G * p.D / 2, 256)), 256, 0, stream>>>(p);
+    if ((rc = check_launch("attn_dkv")) != FLARE_OK || (p.splits == 1 && p.dq_splits == 1)) return rc;
+    const int64_t most = p.B * p.N * p.D * (p.dq_splits > 1 ? p.H : p.G);
+    attn_parts_kernel<E><<<dim3((unsigned)ceil_div(most, 1024), p.splits > 1 ? 3 : 1), 256, 0, stream>>>(p);
     return check_launch("attn_parts");
 }
 template <typename E, int DP>

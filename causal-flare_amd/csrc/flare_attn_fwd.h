@@ -338,23 +338,14 @@ __global__ __launch_bounds__(256) void attn_rows_kernel(AttnArgs p) {
     const int d = (threadIdx.x & 31) * 4;
     if (row >= p.B * p.H * p.N || d >= p.D) return;
     const int64_t i = row % p.N, h = row / p.N % p.H, b = row / p.N / p.H;
-    const float* part = p.parts + row * p.splits * (p.D + 4);
-    float top = kNegInf, total = 0.0f;
-    f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int64_t s = 0; s < p.splits; ++s) top = fmaxf(top, part[s * (p.D + 4) + p.D]);
-    for (int64_t s = 0; s < p.splits; ++s) {
-        const float* q = part + s * (p.D + 4);
-        const float f = q[p.D] == top ? 1.0f : __builtin_amdgcn_exp2f(q[p.D] - top);
-        total += q[p.D + 1] * f;
-        v += *reinterpret_cast<const f32x4*>(q + d) * f;
-    }
-    v *= total == 0.0f ? 0.0f : 1.0f / total;
+    const Joined j = join_parts<1, 4>(p.parts + row * p.splits * (p.D + 4), 0, (int)p.splits, p.D, d);
+    f32x4 v = j.v * (j.total == 0.0f ? 0.0f : 1.0f / j.total);
     if (p.lengths) {
         const int64_t off = p.lengths[b], n = p.fresh ? clamp_to(p.fresh[b], p.N) : p.N;
         if (off >= 0 && off + n > p.M) v = f32x4{__builtin_nanf(""), __builtin_nanf(""), __builtin_nanf(""), __builtin_nanf("")};
     }
     put_y<S>(p, ((b * p.N + i) * p.H + h) * p.D + d, v);
-    if (p.lse && d == 0) p.lse[row] = total == 0.0f ? -kNegInf : top + __builtin_amdgcn_logf(total);
+    if (p.lse && d == 0) p.lse[row] = j.total == 0.0f ? -kNegInf : j.top + __builtin_amdgcn_logf(j.total);
 }
 
 template <typename E, int DP, int CAP>

@@ -186,7 +186,7 @@ __global__ __launch_bounds__(256) void attn_step_kernel(AttnArgs p) {
         if (p.splits == 1) {
             ((S*)p.y)[row * p.D + d] = (S)(v / total);
         } else {
-            float* part = p.parts + (row * p.splits + split) * (p.D + 2);
+            float* part = p.parts + (row * p.splits + split) * (p.D + 4);
             part[d] = v;
             if (d == 0) {
                 part[p.D] = first < last ? t : kNegInf;
@@ -196,27 +196,37 @@ __global__ __launch_bounds__(256) void attn_step_kernel(AttnArgs p) {
     }
 }
 
+// A workgroup a row: 32 lanes, four dimensions a lane, take every eighth part, and the first of them
+// what the eight leave, in order.
 template <typename E>
-__global__ __launch_bounds__(128) void attn_join_kernel(AttnArgs p) {
+__global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs p) {
     typedef typename Elem<E>::S S;
+    typedef S S4 __attribute__((ext_vector_type(4)));
+    __shared__ __align__(16) float left[8][128 + 4];
     const int64_t row = blockIdx.x, b = row / p.H, len = p.lengths[b];
-    const int d = threadIdx.x;
-    if (d >= p.D) return;
-    S* y = (S*)p.y + row * p.D + d;
-    if (len < 0 || len >= p.M) {
-        *y = (S)(len < 0 ? 0.0f : __builtin_nanf(""));
-        return;
+    const int d = (threadIdx.x & 31) * 4, set = threadIdx.x >> 5;
+    const bool idle = len < 0 || len >= p.M;
+    if (!idle && d < p.D) {
+        const Joined j = join_parts<8, 8>(p.parts + row * p.splits * (p.D + 4), set, (int)p.splits, p.D, d);
+        *reinterpret_cast<f32x4*>(&left[set][d]) = j.v;
+        if (d == 0) {
+            left[set][p.D] = j.top;
+            left[set][p.D + 1] = j.total;
+        }
     }
-    const float* part = p.parts + row * p.splits * (p.D + 2);
-    float top = kNegInf, total = 0.0f, v = 0.0f;
-    for (int64_t s = 0; s < p.splits; ++s) top = fmaxf(top, part[s * (p.D + 2) + p.D]);
-    for (int64_t s = 0; s < p.splits; ++s) {
-        const float* q = part + s * (p.D + 2);
-        const float f = q[p.D] == top ? 1.0f : __builtin_amdgcn_exp2f(q[p.D] - top);
-        total += q[p.D + 1] * f;
-        v += q[d] * f;
+    __syncthreads();
+    if (set || d >= p.D) return;
+    f32x4 v;
+    if (idle) {
+        const float none = len < 0 ? 0.0f : __builtin_nanf("");
+        v = f32x4{none, none, none, none};
+    } else {
+        Joined j{kNegInf, 0.0f, f32x4{0.0f, 0.0f, 0.0f, 0.0f}};
+#pragma unroll
+        for (int s = 0; s < 8; ++s) j.add(left[s][p.D], left[s][p.D + 1], *reinterpret_cast<const f32x4*>(&left[s][d]));
+        v = j.v / j.total;
     }
-    *y = (S)(v / total);
+    *reinterpret_cast<S4*>((S*)p.y + row * p.D + d) = __builtin_convertvector(v, S4);
 }
 
 template <typename E, int DP, bool CAP>
@@ -235,7 +245,7 @@ static int step_cap(const AttnArgs& p, hipStream_t stream) {
     kernel<<<dim3((unsigned)p.splits, (unsigned)(p.B * p.G * HG)), 256, bytes, stream>>>(p);
     int rc = check_launch("attn_step");
     if (rc != FLARE_OK || p.splits == 1) return rc;
-    attn_join_kernel<E><<<dim3((unsigned)(p.B * p.H)), 128, 0, stream>>>(p);
+    attn_join_kernel<E><<<dim3((unsigned)(p.B * p.H)), 256, 0, stream>>>(p);
     return check_launch("attn_join");
 }
 template <typename E, int DP>

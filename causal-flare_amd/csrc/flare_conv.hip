@@ -295,10 +295,13 @@ struct PutWeights {
     }
 };
 
-constexpr int kConvBackTokens = 32;
+// Tokens a thread of the backward walks over.  bf16, us with 8, 16, 32 of them, the sums of the weights'
+// gradients included: 2^19 elements 10, 11, 16; 2^22 17, 16, 20; 2^23 28, 22, 25; 2^25 94, 71, 69.
+static int conv_back_tokens(int64_t B, int64_t N, int64_t C) { return B * N * C >= (int64_t)1 << 24 ? 32 : 16; }
 
 // Adjacent channels a thread takes: four where that leaves `waves` waves or more and the rows are
-// aligned to it, two where it does not, and one where rows have no such alignment.
+// aligned to it, two where it does not, and one where rows have no such alignment.  With four and with
+// two, us: forward of 2^25 elements 36.4, 40.8, of 2^19 4.6, 4.3; backward of 2^22 22.2, 17.3.
 template <typename E>
 static int conv_vector(const ConvArgs& p, int64_t runs, int64_t waves) {
     const uintptr_t bits = (uintptr_t)p.x | (uintptr_t)p.y | (uintptr_t)p.window | (uintptr_t)p.window_out |
@@ -320,9 +323,11 @@ static int conv_forward_w(const ConvArgs& p, int64_t W, hipStream_t stream) {
 }
 template <typename E>
 static int conv_forward_e(ConvArgs p, int64_t W, hipStream_t stream) {
-    // Long runs read the W - 1 rows before a run less often, short ones spread a small call over
-    // the GPU.
-    p.run = p.B * p.N * p.C >= (int64_t)1 << 22 ? 16 : 4;
+    // Long runs read the W - 1 rows before a run less often, short ones spread a small call over the
+    // GPU.  bf16, us with runs of 4, 8, 16 tokens: 2^19 elements 4.3, 4.7, 7.0; 2^22 8.2, 8.1, 9.7; 2^23 13.2,
+    // 12.7, 14.4; 2^25 43.9, 40.4, 36.4.
+    const int64_t work = p.B * p.N * p.C;
+    p.run = work >= (int64_t)1 << 24 ? 16 : work >= (int64_t)1 << 22 ? 8 : 4;
     p.tiles = ceil_div(p.N, p.run);
     const int v = conv_vector<E>(p, p.tiles, 2048);
     return v == 1 ? conv_forward_w<E, 1>(p, W, stream) : v == 2 ? conv_forward_w<E, 2>(p, W, stream)
@@ -340,7 +345,7 @@ static int conv_backward_w(const ConvArgs& p, int64_t W, hipStream_t stream) {
 }
 template <typename E>
 static int conv_backward_e(ConvArgs p, int64_t W, hipStream_t stream) {
-    p.run = kConvBackTokens;
+    p.run = conv_back_tokens(p.B, p.N, p.C);
     p.tiles = ceil_div(p.N, p.run);
     const int v = conv_vector<E>(p, p.tiles, 4096);
     return v == 1 ? conv_backward_w<E, 1>(p, W, stream) : v == 2 ? conv_backward_w<E, 2>(p, W, stream)
@@ -361,7 +366,7 @@ static int conv_step_e(const ConvArgs& p, int64_t W, const int32_t* mask, hipStr
 }
 
 static size_t conv_backward_bytes(int64_t B, int64_t N, int64_t C, int64_t W) {
-    return (size_t)(B * ceil_div(N, kConvBackTokens)) * (W + 1) * C * sizeof(float);
+    return (size_t)(B * ceil_div(N, conv_back_tokens(B, N, C))) * (W + 1) * C * sizeof(float);
 }
 
 }  // namespace mix
@@ -412,7 +417,7 @@ extern "C" int flare_conv_backward(const void* x, int64_t x_stride_b, int64_t x_
     p.dy = dy, p.dx = dx, p.partial = (float*)workspace, p.B = B, p.N = N, p.C = C, p.silu = silu;
     const int rc = FLARE_BY_DTYPE(dtype, conv_backward_e, (p, W, (hipStream_t)stream));
     if (rc != FLARE_OK) return rc;
-    const int64_t rows = B * ceil_div(N, kConvBackTokens), cols = (W + 1) * C;
+    const int64_t rows = B * ceil_div(N, conv_back_tokens(B, N, C)), cols = (W + 1) * C;
     return launch_column_sums(p.partial, rows, cols, PutWeights{C, (int)W, dweight, dbias}, (hipStream_t)stream);
 }
 

@@ -361,7 +361,7 @@ using namespace flare::scan;
 
 extern "C" int64_t flare_scan_chunk(int64_t B, int64_t N, int64_t C, int64_t S, int64_t G, int for_backward) {
     if (B < 1 || N < 1 || C < 1 || S < 1 || S > 64 || G < 1 || C % G) return 0;
-    return chunk_length(B, N, C, S, G, for_backward != 0);
+    return chunk_length(B, N, C, G, for_backward != 0);
 }
 extern "C" int64_t flare_scan_kept_tokens(int64_t S) { return S < 1 || S > 64 ? 0 : kept_tokens(padded_states(S)); }
 
