@@ -5,6 +5,9 @@ Every compute call runs hand-written HIP kernels for gfx950 from
 ``_lib/libflare_mi355x.so``; there is no CPU fallback.  Out of scope here and
 raising ``NotImplementedError``: the semi-autoregressive prefill/decode stubs
 (stubs in the reference too).
+
+``mixers`` holds token mixers for hybrid stacks, without a counterpart in the reference: a short
+convolution, a state space scan and softmax attention.
 """
 from . import autoregressive, mixers, semi_autoregressive
 from .autoregressive.training import flare_autoregressive_triton

@@ -74,9 +74,10 @@ struct AttnArgs {
     int64_t splits;
 };
 
-// Tiles of 16 queries a wave of the forward's and the query gradients' kernels owns.
+// Tiles of 16 queries a wave of the forward's and the query gradients' kernels owns (fp32 operands take
+// twice the registers).
 constexpr int q_tiles(int size) { return size == 2 ? 2 : 1; }
-// Tiles of 16 keys a wave of the key gradients' kernel owns.
+// Tiles of 16 keys a wave of the key gradients' kernel owns: as many as leave two waves a SIMD.
 constexpr int kv_tiles(int size, int DP) { return size == 2 && DP <= 64 ? 2 : 1; }
 
 // Four dimensions of a row of y at element `at`, and what they are rounded by.

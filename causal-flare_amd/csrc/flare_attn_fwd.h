@@ -6,6 +6,12 @@
 // passes it by 2^8, so that most tiles rescale nothing.  Weights are rounded to the inputs' type
 // for the product with V (their sum is taken before that, in fp32).  Where there are few rows the
 // keys are split over `splits` workgroups, whose shares attn_rows joins.
+//
+// Bound: at two waves a SIMD (the registers hold Q, 32 x 64 scores and 32 x D sums a wave) the
+// products and the exponentials of a wave alternate and overlap only with the other wave's.  bf16,
+// causal, products at a large matrix product's rate for comparison: 16384 rows, 16 heads of 128 over
+// 4, 1243 us, 0.88 PFLOP/s of 1.34; 4 x 4096 rows, 16 heads of 64, capped scores (three
+// transcendental instructions a pair) 260 us, 0.53.  32 queries a wave against 16: 275 and 285 us.
 #pragma once
 
 #include "flare_attn.h"

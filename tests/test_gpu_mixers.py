@@ -86,6 +86,11 @@ def test_conv(dtype, B, N, C, W, docs):
             close(grads[2], ref["dbias"], "dbias", F32, CONV_K + 32 + B * N / 8)
 
 
+@pytest.mark.parametrize("B, N, C, W, docs", [(1, 2101, 2050, 4, 3), (2, 4099, 2052, 3, 0)])
+def test_conv_of_longer_runs(B, N, C, W, docs):
+    test_conv(BF16, B, N, C, W, docs)
+
+
 @pytest.mark.parametrize("dtype", [F32, BF16, F16])
 @pytest.mark.parametrize("B, N, C, W", [(4, 1, 16, 4), (5, 2, 24, 4), (6, 9, 10, 3), (8, 70, 64, 2)])
 def test_conv_prefill_and_decode(dtype, B, N, C, W):
@@ -405,6 +410,19 @@ def test_attention_decode(dtype, B, H, G, D, S, what):
             assert y[b].isnan().all() if at >= S else not y[b].any()
         assert torch.equal(cache["k"][b].nan_to_num(9.0), want_k.nan_to_num(9.0))
         assert torch.equal(cache["v"][b].nan_to_num(9.0, posinf=9.0), want_v.nan_to_num(9.0, posinf=9.0))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+def test_attention_decode_of_many_parts(dtype):
+    # 128 keys a workgroup: one sequence with nothing, one with all and one with half of 86 parts
+    test_attention_decode(dtype, 3, 4, 2, 48, 20011, "cap slopes")
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("B, N, H, G, D, what", [
+    (1, 2900, 6, 2, 80, "docs slopes"), (2, 1300, 4, 4, 128, "prefix"), (1, 2100, 1, 1, 64, "full cap"), (1, 1800, 5, 1, 32, "")])
+def test_attention_of_few_rows_in_parts(dtype, B, N, H, G, D, what):
+    test_attention(dtype, B, N, H, G, D, what)
 
 
 def test_attention_reads_slices_and_promotes():
