@@ -142,9 +142,13 @@ static size_t dq_bytes(const AttnArgs& p) {
 // Parts that a row's keys are split into in the forward: two workgroups a CU (512) where the rows
 // leave less than that, in parts of 512 keys or more.  us, the joining included, with parts and
 // without: 64 new tokens behind 8000, 16 heads of 128 over 4, 34 and 274; 2 x 512 behind 3000 55 and 118.
+// One round of workgroups under a causal mask alone is as long as its last rows, and two parts even
+// that out: 4096 rows, 16 heads of 128 over 4, 127 and 151; with 6400 rows, or 2048 behind 2048, they
+// are slower (269 and 250, 172 and 163).
 static void split_forward(AttnArgs& p, int dtype) {
-    const int64_t blocks = ceil_div(p.N, rows_of_queries(dtype)) * p.B * p.H, want = ceil_div(512, blocks);
-    const int64_t most = ceil_div(p.M, 512);
+    const int64_t blocks = ceil_div(p.N, rows_of_queries(dtype)) * p.B * p.H, most = ceil_div(p.M, 512);
+    int64_t want = ceil_div(512, blocks);
+    if (want < 2 && blocks <= 512 && p.causal && p.M == p.N) want = 2;
     p.splits = want < most ? want : most;
 }
 static size_t forward_head_bytes(int64_t B, int64_t N) { return (stats_bytes(B, N) + 255) / 256 * 256; }
@@ -195,7 +199,7 @@ static AttnArgs attn_args(const void* q, const void* k, const void* v, const int
 extern "C" size_t flare_attn_forward_workspace_size(int64_t B, int64_t N, int64_t M, int64_t H, int64_t D, int dtype) {
     if (B < 1 || N < 1 || M < 1 || H < 1) return 0;
     AttnArgs p = {};
-    p.B = B, p.N = N, p.M = M, p.H = H, p.D = D;
+    p.B = B, p.N = N, p.M = M, p.H = H, p.D = D, p.causal = 1;       // which needs the most
     split_forward(p, dtype);
     return forward_head_bytes(B, N) + rows_bytes(p);
 }
