@@ -649,6 +649,36 @@ def test_repeats_streams_and_graphs(name):
             assert same(out, want), i
 
 
+def test_graphs_of_the_largest_head_dimension():
+    """128 dimensions take more LDS than a workgroup has by default, rows in parts a workspace."""
+    g = gen(77)
+    q, k, v, dy = (normal(g, 1, 700, n, 128, dtype=BF16) for n in (4, 2, 2, 4))
+    ids = documents(g, 1, 700)
+    cache = {n: normal(g, 1, 1500, 2, 128, dtype=BF16) for n in "kv"}
+    lens = torch.tensor([650], device=DEV)
+
+    def call():
+        leaves = [t.clone().requires_grad_() for t in (q, k, v)]
+        y = cf.softmax_attention(*leaves, document_ids=ids)
+        out = [y.detach(), *torch.autograd.grad(y, leaves, dy)]
+        for f, n in ((cf.softmax_attention_prefill, 700), (cf.softmax_attention_decode, 1)):
+            y, c = f(q[:, :n], k[:, :n], v[:, :n], {n: t.clone() for n, t in cache.items()}, lens)
+            out += [y, c["k"], c["v"]]
+        return out
+
+    want = call()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = call()
+    for i in range(3):
+        for x in out:
+            x.fill_(1.0)
+        graph.replay()
+        assert same(call(), want)
+        torch.cuda.synchronize()
+        assert same(out, want), i
+
+
 def test_differences():
     """Directional derivatives of the fp32 calls.  f is of order 1 per output and changes by e d1 +
     e^3 d3 / 6; with e = 2^-7 the rounding of f (2^-22 of the sum of its terms) over e and the
