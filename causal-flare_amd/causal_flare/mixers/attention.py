@@ -27,6 +27,7 @@ from torch.autograd.function import once_differentiable
 from .. import _lib
 from .._common import _compute_dtype, _resolve_attn_scale
 from ._inputs import (
+    _CODES,
     _aligned_rows,
     _check_device,
     _check_float,
@@ -35,6 +36,7 @@ from ._inputs import (
     _f32,
     _int32,
     _on,
+    _plain_f32,
     _ptr,
     _raw_stream,
     _strides,
@@ -230,6 +232,52 @@ def softmax_attention_prefill(
     return y, cache
 
 
+def _step_fast(Q, K, V, cache, lengths, scale, softcap, slopes):
+    """The common call, or None: one type, rows and a cache that the kernel reads in place, int32 lengths."""
+    token = Q.dim() == 4
+    if Q.dim() not in (3, 4) or (token and Q.shape[1] != 1) or not isinstance(cache, dict):
+        return None
+    kc, vc = cache.get("k"), cache.get("v")
+    B, H, D = Q.shape[0], Q.shape[-2], Q.shape[-1]
+    dtype, device = Q.dtype, Q.device
+    code = _CODES.get(dtype)
+    if (kc is None or vc is None or kc.dim() != 4 or K.dim() != Q.dim() or code is None or device.type != "cuda"
+            or device.index != torch.cuda.current_device()):
+        return None
+    S, G = kc.shape[1], K.shape[-2]
+    want = (B, 1, G, D) if token else (B, G, D)
+    if (K.shape != want or V.shape != want or kc.shape != (B, S, G, D) or vc.shape != kc.shape or not B * S * G
+            or H < 1 or H % G or D % 16 or not 16 <= D <= 128 or lengths.dtype is not torch.int32
+            or lengths.shape != (B,) or lengths.device != device or not lengths.is_contiguous()
+            or not _plain_f32(slopes, device, H) or (slopes is not None and slopes.requires_grad)
+            or (softcap is not None and not 0.0 < softcap < math.inf)):
+        return None
+    pointers = [t.data_ptr() for t in (Q, K, V, kc, vc)]
+    strides, spread = [], 0
+    for t in (Q, K, V):
+        strides += (t.stride(0), t.stride(-2))
+        if t.stride(-1) != 1:
+            return None
+    for x in strides:
+        spread |= x * Q.element_size()
+    for x in pointers:
+        spread |= x
+    if spread % 16 or not (kc.is_contiguous() and vc.is_contiguous()):
+        return None
+    for t in (K, V, kc, vc):
+        if t.dtype is not dtype or t.device != device:
+            return None
+    y = torch.empty((B, 1, H, D), device=device, dtype=dtype)
+    lib = _lib.lib()
+    nbytes = lib.flare_attn_step_workspace_size(B, S, H, G, D)
+    ws = torch.empty(nbytes, device=device, dtype=torch.uint8) if nbytes else None
+    _lib.check(lib.flare_attn_step(
+        *pointers[:3], _strides(*strides), code, B, S, H, G, D, _resolve_attn_scale(scale, D), softcap or 0.0,
+        _ptr(slopes), lengths.data_ptr(), *pointers[3:], y.data_ptr(), _ptr(ws), nbytes, _raw_stream(device.index)),
+        "flare_attn_step")
+    return y, cache
+
+
 def softmax_attention_decode(
     Q: torch.Tensor,
     K: torch.Tensor,
@@ -248,6 +296,9 @@ def softmax_attention_decode(
     is full is not written, and its y is NaN.
     """
     name = "softmax_attention_decode"
+    out = _step_fast(Q, K, V, cache, lengths, scale, softcap, slopes)
+    if out is not None:
+        return out
     Q, K, V = (t[:, None] if t.dim() == 3 else t for t in (Q, K, V))
     B, T, H, G, D = _check_heads(name, Q, K, V)
     if T != 1:

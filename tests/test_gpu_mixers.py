@@ -425,6 +425,25 @@ def test_attention_of_few_rows_in_parts(dtype, B, N, H, G, D, what):
     test_attention(dtype, B, N, H, G, D, what)
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("H, G, D, sloped", [(4, 2, 64, False), (16, 4, 128, True), (3, 3, 16, True)])
+def test_attention_decode_of_any_integer_lengths(dtype, H, G, D, sloped):
+    """Slices of one projection, rows that sit out and a full cache: the same for int32 lengths and others."""
+    g = gen(D)
+    qkv = normal(g, 5, 1, H + 2 * G, D, dtype=dtype)
+    cache = {n: normal(g, 5, 300, G, D, dtype=dtype) for n in "kv"}
+    held = torch.tensor([0, 299, 300, -1, 7], device=DEV, dtype=torch.int32)
+    o = dict(softcap=20, slopes=normal(g, H).abs() if sloped else None)
+    runs = []
+    for rows in (qkv, qkv[:, 0], qkv.clone()[:, 0]):
+        for lens in (held, held.long(), held.to(torch.int16)):
+            c = {n: t.clone() for n, t in cache.items()}
+            y, _ = cf.softmax_attention_decode(*rows.split((H, G, G), -2), c, lens, **o)
+            runs.append([y.nan_to_num(7.0), c["k"], c["v"]])
+    assert all(same(r, runs[0]) for r in runs)
+    assert runs[0][0][2].eq(7.0).all() and not runs[0][0][3].any() and runs[0][0][4].ne(7.0).any()
+
+
 def test_attention_reads_slices_and_promotes():
     g = gen(8)
     qkv = normal(g, 2, 70, 8, 64, dtype=BF16)
