@@ -227,12 +227,13 @@ __global__ __launch_bounds__(256, 2) void attn_forward_kernel(AttnArgs p) {
                 }
                 float ref = 0.0f;
                 if (CAP != kCapFixed) {
-                    float m = mfma::max3_raw(s[t][0][0], s[t][0][1], s[t][0][2]);
-                    m = mfma::max_raw(m, s[t][0][3]);
+                    // not the inline assembly of max3_raw: the compiler leaves no wait states between a
+                    // product and assembly that reads it
+                    float m = kNegInf;
 #pragma unroll
-                    for (int n = 1; n < NK; ++n) {
-                        m = mfma::max3_raw(m, s[t][n][0], s[t][n][1]);
-                        m = mfma::max3_raw(m, s[t][n][2], s[t][n][3]);
+                    for (int n = 0; n < NK; ++n) {
+                        m = fmaxf(fmaxf(s[t][n][0], s[t][n][1]), m);
+                        m = fmaxf(fmaxf(s[t][n][2], s[t][n][3]), m);
                     }
                     m = column_max(m);
                     if (plain) m *= scale2;

@@ -2,11 +2,11 @@
 //
 // scan_chunk: a lane is a channel and holds its S states and rates in registers, so B_t and
 // C_t are the same for the whole wave: they are scalar loads, and scalar operands of the
-// vector instructions.  An element of the state costs an exponential (16 cycles of a SIMD a
-// wave), two products and two fused products (4 each): vector instructions bound it, and both
-// passes over a chunk pay them.  16384 tokens, 2048 channels of 16 states, bf16: the chunks' ends
-// 122 us, the output 162 us, where the exponentials alone take some 60 us a pass; scan_states 22 us
-// (34 MB read and written).
+// vector instructions.  An element of the state costs an exponential (8 cycles of a SIMD a wave,
+// measured), two products and one or two fused products (4 each), a token a softplus and its gate:
+// vector instructions bound it, and both passes over a chunk pay them.  16384 tokens, 2048 channels
+// of 16 states, bf16: the chunks' ends 122 us, the output 162 us, where the elements' instructions
+// alone are 70 and 84; scan_states 22 us (34 MB read and written).
 #include "flare_scan.h"
 
 namespace flare {
