@@ -141,7 +141,7 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnArgs p) {
     const S* kbase = (const S*)p.k.p + b * p.k.sb + kvh * p.k.sh;
     const S* vbase = (const S*)p.v.p + b * p.v.sb + kvh * p.v.sh;
     const float scale2 = p.scale * kLog2e, slope2 = p.slopes ? p.slopes[h] * kLog2e : 0.0f;
-    const float cap2 = p.cap * kLog2e, into_cap = CAP ? 2.0f * kLog2e * p.scale / p.cap : 0.0f;
+    const float cap2 = p.cap * kLog2e, to_tanh = CAP ? p.scale / p.cap : 0.0f, into_cap = 2.0f * kLog2e * to_tanh;
 
     const float out_scale = CAP ? 4.0f * p.scale : p.scale;
     f32x4 acc[QT][DT];
@@ -219,18 +219,23 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnArgs p) {
                 for (int n = 0; n < 2; ++n) {
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        float x = s[t][n][i], r = 0.0f;
-                        if (CAP) {
+                        float x = s[t][n][i], slope = 1.0f;        // a quarter of 1 - tanh^2
+                        if (CAP && sizeof(E) == 4) {
+                            const Tanh u = fine_tanh(x * to_tanh);
+                            x = cap2 * u.t - lse[t];
+                            slope = u.slope;
+                        } else if (CAP) {
                             // cap tanh(x / cap) = cap (1 - 2 r), 1 - tanh^2 = 4 r (1 - r)
-                            r = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(x * into_cap));
+                            const float r = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(x * into_cap));
                             x = cap_lse[t] - 2.0f * cap2 * r;
+                            slope = r - r * r;
                         } else {
                             x = x * scale2 - lse[t];
                         }
                         if (p.slopes) x -= slope2 * fabsf(base - (float)(16 * n + i));
                         const float w = __builtin_amdgcn_exp2f(x);
                         float ds = w * (dp[t][n][i] - delta[t]);
-                        if (CAP) ds *= r - r * r;              // and 4 in the end
+                        if (CAP) ds *= slope;                  // and 4 in the end
                         s[t][n][i] = ds;
                     }
                 }
@@ -351,7 +356,7 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(AttnArgs p) {
         }
     }
     const float scale2 = p.scale * kLog2e;
-    const float cap2 = p.cap * kLog2e, into_cap = CAP ? 2.0f * kLog2e * p.scale / p.cap : 0.0f;
+    const float cap2 = p.cap * kLog2e, to_tanh = CAP ? p.scale / p.cap : 0.0f, into_cap = 2.0f * kLog2e * to_tanh;
     f32x4 dk[KQ][DT], dv[KQ][DT];
 #pragma unroll
     for (int t = 0; t < KQ; ++t)
@@ -374,7 +379,7 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(AttnArgs p) {
         if (tid < QR) {
             const bool live = q0 + tid < N;
             const int64_t at = (b * p.H + h) * p.N + q0 + tid;
-            next_lse = live ? p.lse[at] - kShift - cap2 : -kNegInf;
+            next_lse = live ? p.lse[at] - kShift - (sizeof(E) == 4 ? 0.0f : cap2) : -kNegInf;
             next_delta = live ? p.delta[at] * kUnshift : 0.0f;
             next_id = !live ? kNoQuery : p.ids ? p.ids[b * p.N + q0 + tid] : 0;
             next_id = next_id < 0 ? kNoQuery : next_id;
@@ -454,17 +459,22 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(AttnArgs p) {
                         const float base = (float)(q0 + 4 * g - (w0 + 16 * t + c));
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
-                            float x = s[t][n][i], r = 0.0f;
-                            if (CAP) {
-                                r = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(x * into_cap));
+                            float x = s[t][n][i], slope = 1.0f;
+                            if (CAP && sizeof(E) == 4) {
+                                const Tanh u = fine_tanh(x * to_tanh);
+                                x = cap2 * u.t - lse[i];
+                                slope = u.slope;
+                            } else if (CAP) {
+                                const float r = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(x * into_cap));
                                 x = -2.0f * cap2 * r - lse[i];          // the log-sum-exp less the cap
+                                slope = r - r * r;
                             } else {
                                 x = x * scale2 - lse[i];
                             }
                             if (p.slopes) x -= slope2 * fabsf(base + (float)(16 * n + i));
                             const float w = __builtin_amdgcn_exp2f(x);
                             float ds = w * (dp[t][n][i] * kUnshift - delta[i]);
-                            if (CAP) ds *= r - r * r;
+                            if (CAP) ds *= slope;
                             s[t][n][i] = w;
                             dp[t][n][i] = ds;
                         }

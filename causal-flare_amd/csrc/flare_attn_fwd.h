@@ -22,8 +22,9 @@ namespace attn {
 // How scores are kept from overflowing: against a running maximum, or against the cap itself,
 // which bounds them where nothing is added.
 enum { kNoCap = 0, kCapRunning = 1, kCapFixed = 2 };
-// With weights of 2^(s - cap) a row's largest is at least 2^(-2 cap): fp32 and bf16 hold that, with
-// all that counts beside it, up to here (log2 units), and fp16 does not.
+// With weights of 2^(s - cap) a row's largest is at least 2^(-2 cap): bf16 holds that, with all that
+// counts beside it, up to here (log2 units), and fp16 does not.  fp32 would, but s - cap rounds to fewer
+// digits than s has.
 constexpr float kCapFixedMost = 60.0f;
 constexpr float kSlack = 8.0f;       // log2 of the largest weight before the reference moves
 
@@ -112,7 +113,7 @@ __global__ __launch_bounds__(256, 2) void attn_forward_kernel(AttnArgs p) {
     const S* kbase = (const S*)p.k.p + b * p.k.sb + kvh * p.k.sh;
     const S* vbase = (const S*)p.v.p + b * p.v.sb + kvh * p.v.sh;
     const float scale2 = fabsf(p.scale) * kLog2e, slope2 = p.slopes ? p.slopes[h] * kLog2e : 0.0f;
-    const float cap2 = p.cap * kLog2e, into_cap = CAP ? 2.0f * kLog2e * fabsf(p.scale) / p.cap : 0.0f;
+    const float cap2 = p.cap * kLog2e, to_tanh = CAP ? fabsf(p.scale) / p.cap : 0.0f, into_cap = 2.0f * kLog2e * to_tanh;
 
     f32x4 acc[QT][DT];
     float top[QT], sum[QT];
@@ -193,6 +194,10 @@ __global__ __launch_bounds__(256, 2) void attn_forward_kernel(AttnArgs p) {
                     for (int n = 0; n < NK; ++n) {
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
+                            if constexpr (sizeof(E) == 4) {
+                                s[t][n][i] = cap2 * fine_tanh(s[t][n][i] * to_tanh).t;
+                                continue;
+                            }
                             // cap tanh(x / cap) = cap - 2 cap / (e^(2 x / cap) + 1)
                             const float r = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(s[t][n][i] * into_cap));
                             s[t][n][i] = CAP == kCapFixed ? -2.0f * cap2 * r : cap2 - 2.0f * cap2 * r;
@@ -378,7 +383,7 @@ static int forward_cap(const AttnArgs& p, hipStream_t stream) {
 template <typename E, int DP>
 static int forward_dp(const AttnArgs& p, hipStream_t stream) {
     if (p.cap == 0.0f) return forward_cap<E, DP, kNoCap>(p, stream);
-    if constexpr (!__is_same(E, __half))
+    if constexpr (__is_same(E, __hip_bfloat16))
         if (!p.slopes && p.cap * kLog2e <= kCapFixedMost) return forward_cap<E, DP, kCapFixed>(p, stream);
     return forward_cap<E, DP, kCapRunning>(p, stream);
 }

@@ -70,7 +70,7 @@ __global__ __launch_bounds__(256) void attn_step_kernel(AttnArgs p) {
         if (head && d < p.D) qf[kk] = frag_rows<E>((const S*)p.q.p + b * p.q.sb + h * p.q.sh + d);
     }
     const float scale2 = p.scale * kLog2e, slope2 = p.slopes ? p.slopes[h] * kLog2e : 0.0f;
-    const float cap2 = p.cap * kLog2e, into_cap = CAP ? 2.0f * kLog2e * p.scale / p.cap : 0.0f;
+    const float cap2 = p.cap * kLog2e, to_tanh = CAP ? p.scale / p.cap : 0.0f, into_cap = 2.0f * kLog2e * to_tanh;
     f32x4 acc[DT];
 #pragma unroll
     for (int d = 0; d < DT; ++d) acc[d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
@@ -120,7 +120,8 @@ __global__ __launch_bounds__(256) void attn_step_kernel(AttnArgs p) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 float x = s[m][i];
-                x = CAP ? cap2 * tanh_log2(x * into_cap) : x * scale2;
+                if (CAP && sizeof(E) == 4) x = cap2 * fine_tanh(x * to_tanh).t;
+                else x = CAP ? cap2 * tanh_log2(x * into_cap) : x * scale2;
                 x -= slope2 * (base - (float)(16 * m + i));
                 s[m][i] = k0 + 16 * m + 4 * g + i < last ? x : kNegInf;
             }

@@ -412,6 +412,34 @@ def test_attention_decode(dtype, B, H, G, D, S, what):
         assert torch.equal(cache["v"][b].nan_to_num(9.0, posinf=9.0), want_v.nan_to_num(9.0, posinf=9.0))
 
 
+@pytest.mark.parametrize("cap", [3.0, 30.0, 200.0])
+def test_capped_scores_of_fp32_keep_their_digits(cap):
+    """As near to 64 bits as elementary fp32 operations, whose scores are off by the same few roundings
+    (2.5 times their error leaves room for the order of the sums and exponentials of one unit)."""
+    g = gen(int(cap))
+    q, k, v, dy = (normal(g, 2, 300, 2, 64, std=s) for s in (2.0, 1.0, 1.0, 1.0))
+
+    def whole(dtype):
+        a, b, c = (t.to(dtype).transpose(1, 2).contiguous().requires_grad_() for t in (q, k, v))
+        x = cap * torch.tanh((a @ b.transpose(-1, -2).contiguous()) * 0.125 / cap)
+        x = x.masked_fill(torch.ones(300, 300, device=DEV, dtype=torch.bool).triu(1), float("-inf"))
+        y = torch.softmax(x, -1) @ c
+        grads = torch.autograd.grad(y, (a, b, c), dy.to(dtype).transpose(1, 2))
+        return [t.detach().double().transpose(1, 2) for t in (y, *grads)]
+
+    leaves = [t.clone().requires_grad_() for t in (q, k, v)]
+    y = cf.softmax_attention(*leaves, softcap=cap)
+    got = [y.detach().double(), *(t.double() for t in torch.autograd.grad(y, leaves, dy))]
+    cache = {n: torch.cat([t[:, :299], torch.zeros_like(t[:, :1])], 1) for n, t in (("k", k), ("v", v))}
+    held = torch.full((2,), 299, device=DEV, dtype=torch.int32)
+    last = cf.softmax_attention_decode(q[:, 299], k[:, 299], v[:, 299], cache, held, softcap=cap)[0].double()
+    want, plain32 = whole(torch.float64), whole(torch.float32)
+    for name, a, b, c in zip(("y", "dq", "dk", "dv"), got, plain32, want):
+        assert (a - c).norm() <= 2.5 * (b - c).norm(), (name, float((a - c).norm() / c.norm()), float((b - c).norm() / c.norm()))
+    a, b, c = last, plain32[0][:, 299:], want[0][:, 299:]
+    assert (a - c).norm() <= 2.5 * (b - c).norm(), ("token", float((a - c).norm() / c.norm()), float((b - c).norm() / c.norm()))
+
+
 @pytest.mark.parametrize("dtype", [F32, BF16, F16])
 def test_attention_decode_of_many_parts(dtype):
     # 128 keys a workgroup: one sequence with nothing, one with all and one with half of 86 parts
