@@ -56,12 +56,19 @@ __global__ __launch_bounds__(256) void attn_delta_kernel(AttnArgs p, int lanes, 
     if (col == 0) delta[(b * p.H + h) * p.N + i] = s;
 }
 
+// An infinite value or NaN in a row of K, Q or dY counts for the pairs that see that row, and a weight
+// of 0 times it is NaN for the others.  So tiles that not every pair sees and that hold one take
+// their products from operands without such values; what they add to the pairs that do see them
+// comes by element from memory in the end: in dq and dk NaN, as the score gradient beside an
+// infinite score is 0 or NaN (under a cap with finite weights), and in dv the value itself.
+__device__ __forceinline__ bool is_odd(float x) { return !(fabsf(x) < -kNegInf); }
+
 // An operand's infinite values and NaNs set to 0.
 template <typename F>
 __device__ __forceinline__ F finite(F f) {
 #pragma unroll
     for (int i = 0; i < 8; ++i)
-        if (!(fabsf((float)f[i]) < -kNegInf)) f[i] = 0.0f;
+        if (is_odd((float)f[i])) f[i] = 0.0f;
     return f;
 }
 
@@ -176,7 +183,7 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnArgs p) {
     };
     TileWalk<KT> walk(p, b, kv_end, mine);
     int tile = walk.next(k_begin);
-    int buf = 0;
+    int buf = 0, any_odd = 0;
     if (tile < kv_end) {
         fetch(tile);
         place(tile, 0);
@@ -185,7 +192,8 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnArgs p) {
     while (tile < kv_end) {
         const int k1 = walk.next(tile + KT);
         if (k1 < kv_end) fetch(k1);
-        const bool odd = (oddl[buf * 4] | oddl[buf * 4 + 1] | oddl[buf * 4 + 2] | oddl[buf * 4 + 3]) != 0;
+        const int odd = __builtin_amdgcn_readfirstlane(oddl[buf * 4] | oddl[buf * 4 + 1] | oddl[buf * 4 + 2] | oddl[buf * 4 + 3]);
+        any_odd |= odd;
 #pragma unroll 1
         for (int part = 0; part < KT; part += 32) {
             const int k0 = tile + part;
@@ -261,7 +269,7 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnArgs p) {
 #pragma unroll
             for (int d = 0; d < DT; ++d) {
                 Frag a = frag_columns<E>(kt + 16 * d, P, g, c);
-                if (odd) a = finite(a);                 // 0 times an infinite value is NaN
+                if (odd) a = finite(a);
 #pragma unroll
                 for (int t = 0; t < QT; ++t) {
                     acc[t][d] = mma(a, w[t], acc[t][d]);
@@ -273,6 +281,24 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnArgs p) {
         __syncthreads();
         buf ^= 1;
         tile = k1;
+    }
+    if (any_odd) {
+        TileWalk<KT> again(p, b, kv_end, mine);
+        for (tile = again.next(k_begin); tile < kv_end; tile = again.next(tile + KT)) {
+            if (covers(tile, KT, q0, q0 + QB - 1)) continue;
+            for (int j = tile; j < min(tile + KT, N); ++j) {
+#pragma unroll
+                for (int t = 0; t < QT; ++t) {
+                    if (j >= lim[t] || (p.ids && max(p.ids[b * p.N + j], kNoKey) != qid[t])) continue;
+#pragma unroll
+                    for (int d = 0; d < DT; ++d) {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            if (16 * d < p.D && is_odd((float)kbase[j * p.k.sn + 16 * d + 4 * g + e])) acc[t][d][e] = __builtin_nanf("");
+                    }
+                }
+            }
+        }
     }
 #pragma unroll
     for (int t = 0; t < QT; ++t) {
@@ -385,21 +411,8 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(AttnArgs p) {
             next_id = next_id < 0 ? kNoQuery : next_id;
         }
     };
-    // Tiles seen in part keep infinite values and NaNs out of LDS (0 times them is NaN); the rows
-    // they are in have a log-sum-exp or a delta that is none, and their weights are NaN then.
     auto place = [&](int q0, int buf) {
-        bool odd = false;
-        if (!covers(q0, QR, kb, kb + KB - 1)) {
-            if (qs.odd()) {
-                odd = true;
-                qs.clean();
-            }
-            if (gs.odd()) {
-                odd = true;
-                gs.clean();
-            }
-        }
-        odd = __any(odd);
+        const bool odd = !covers(q0, QR, kb, kb + KB - 1) && __any(qs.odd() || gs.odd());
         if (lane == 0) oddl[buf * 4 + wave] = odd;
         qs.store(ql + buf * QR * P, tid);
         gs.store(gl + buf * QR * P, tid);
@@ -409,7 +422,7 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(AttnArgs p) {
             idl[buf * QR + tid] = next_id;
         }
     };
-    int buf = 0;
+    int buf = 0, any_odd = 0;
     for (int rep = rep0; rep < rep1; ++rep) {
         const int h = kvh * R + rep;
         const float slope2 = p.slopes ? p.slopes[h] * kLog2e : 0.0f;
@@ -423,7 +436,8 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(AttnArgs p) {
         while (tile < q_end) {
             const int q1 = walk.next(tile + QR);
             if (q1 < q_end) fetch(h, q1);
-            const bool odd = (oddl[buf * 4] | oddl[buf * 4 + 1] | oddl[buf * 4 + 2] | oddl[buf * 4 + 3]) != 0;
+            const int odd = __builtin_amdgcn_readfirstlane(oddl[buf * 4] | oddl[buf * 4 + 1] | oddl[buf * 4 + 2] | oddl[buf * 4 + 3]);
+            any_odd |= odd;
 #pragma unroll 1
             for (int from_row = 0; from_row < QR; from_row += 32) {
                 const int q0 = tile + from_row;
@@ -449,7 +463,7 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(AttnArgs p) {
                         }
                     }
                 }
-                const bool whole = !odd && covers(q0, 32, w0, w0 + 16 * KQ - 1);
+                const bool whole = covers(q0, 32, w0, w0 + 16 * KQ - 1);
 #pragma unroll
                 for (int n = 0; n < 2; ++n) {
                     const f32x4 lse = *reinterpret_cast<const f32x4*>(lsel + buf * QR + from_row + 16 * n + 4 * g);
@@ -484,9 +498,8 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(AttnArgs p) {
                             const int row_id[4] = {d.x, d.y, d.z, d.w};
 #pragma unroll
                             for (int i = 0; i < 4; ++i) {
-                                const bool see = i >= late && row_id[i] == kid[t];
-                                if (odd && !(fabsf(lse[i]) < -kNegInf && fabsf(delta[i]) < -kNegInf))
-                                    s[t][n][i] = dp[t][n][i] = __builtin_nanf("");
+                                // no branch (&&): in one the compiler left some unseen pairs their weights
+                                const bool see = (i >= late) & (row_id[i] == kid[t]);
                                 s[t][n][i] = see ? s[t][n][i] : 0.0f;
                                 dp[t][n][i] = see ? dp[t][n][i] : 0.0f;
                             }
@@ -501,8 +514,12 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(AttnArgs p) {
                 }
 #pragma unroll
                 for (int d = 0; d < DT; ++d) {
-                    const Frag a = frag_columns<E>(qt + 16 * d, P, g, c);
-                    const Frag o = frag_columns<E>(gt + 16 * d, P, g, c);
+                    Frag a = frag_columns<E>(qt + 16 * d, P, g, c);
+                    Frag o = frag_columns<E>(gt + 16 * d, P, g, c);
+                    if (odd) {
+                        a = finite(a);
+                        o = finite(o);
+                    }
 #pragma unroll
                     for (int t = 0; t < KQ; ++t) {
                         dk[t][d] = mma(a, ds[t], dk[t][d]);
@@ -515,6 +532,31 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(AttnArgs p) {
             __syncthreads();
             buf ^= 1;
             tile = q1;
+        }
+    }
+    for (int rep = rep0; rep < (any_odd ? rep1 : rep0); ++rep) {
+        TileWalk<QR> again(p, b, q_end, mine);
+        for (int tile = again.next(q_begin); tile < q_end; tile = again.next(tile + QR)) {
+            if (covers(tile, QR, kb, kb + KB - 1)) continue;
+            for (int i = tile; i < min(tile + QR, N); ++i) {
+                const int row_id = p.ids ? p.ids[b * p.N + i] : 0;
+                const S* q = (const S*)p.q.p + b * p.q.sb + (kvh * R + rep) * p.q.sh + i * p.q.sn + 4 * g;
+                const S* dy = (const S*)p.dy + ((b * p.N + i) * p.H + kvh * R + rep) * p.D + 4 * g;
+#pragma unroll
+                for (int t = 0; t < KQ; ++t) {
+                    if (i < from[t] || row_id < 0 || row_id != kid[t]) continue;
+#pragma unroll
+                    for (int d = 0; d < DT; ++d) {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            if (16 * d >= p.D) continue;
+                            const float o = (float)dy[16 * d + e];
+                            if (is_odd((float)q[16 * d + e])) dk[t][d][e] = __builtin_nanf("");
+                            if (is_odd(o)) dv[t][d][e] += o;
+                        }
+                    }
+                }
+            }
         }
     }
 #pragma unroll

@@ -1,0 +1,96 @@
+"""The token mixers on the GPU where a formula meets its edges: infinite values that a cap or a mask
+bounds, growth past fp32, gradients below a type's range, chunks of other lengths."""
+import math
+
+import pytest
+import torch
+
+import causal_flare as cf
+from _mixers import U, attention, check, scan
+from test_gpu_mixers import BF16, DEV, E32, F16, F32, gen, normal, test_attention
+
+pytestmark = pytest.mark.gpu
+INF, NAN = math.inf, math.nan
+
+
+# ---------------------------------------------------------------------------------------
+# Softmax attention
+# ---------------------------------------------------------------------------------------
+def seen_sums(see, w, x):
+    """sum_j w_ij x_jd over the pairs of `see` alone: what is not seen may be infinite."""
+    return torch.where(see[..., None], w[..., None] * x[None], 0.0).sum(1)
+
+
+def one_head(q, k, v, dy, see, cap, unit, slope=0.0):
+    """{name: (value, tolerance)} of one head [N, D] with every sum over the seen pairs alone; the
+    tolerances are those of `attention` in _mixers.py, a saturated score's own error being 0."""
+    N, D = q.shape
+    scale = D ** -0.5
+    far = slope * (torch.arange(N)[:, None] - torch.arange(N)[None]).abs()
+    x = q @ k.t() * scale
+    th = torch.tanh(x / cap)
+    s = torch.where(see, cap * th - far, -INF)
+    p = torch.softmax(s, 1)
+    sums = lambda w, t: seen_sums(see, w, t)
+    y, pv = sums(p, v), sums(p, v.abs())
+    dp = dy @ v.t()
+    delta = (dy * y).sum(1, keepdim=True)
+    cut = 1 - th * th
+    ds = p * (dp - delta) * cut * scale
+    out = {"y": y, "dq": sums(ds, k), "dk": seen_sums(see.t(), ds.t(), q), "dv": seen_sums(see.t(), p.t(), dy)}
+    size = (q.abs() @ k.abs().t() * scale).nan_to_num(0.0, 0.0, 0.0) + far
+    es = E32 * (torch.where(see, size, 0.0).amax(1, keepdim=True) * (8 + D / 4) + 16 + 8 * cap)
+    edp = E32 * (16 + D) * (dy.abs() @ v.abs().t()) + (dy.abs() * ((2 * unit + 2 * es + 64 * E32) * pv + unit * y.abs())).sum(1, keepdim=True)
+    eds = (p * cut * edp + (2 * es + 64 * E32) * p * (dp - delta).abs() * (cut + 4) + unit * ds.abs() / scale
+           + 2.0 ** -25 * (1 + (dp - delta).abs())) * scale
+    tol = {"y": (unit + 2 * es + 64 * E32) * pv + 2.0 ** -25 * seen_sums(see, torch.ones_like(p), v.abs()),
+           "dq": sums(eds + 64 * E32 * ds.abs(), k.abs()),
+           "dk": seen_sums(see.t(), (eds + 64 * E32 * ds.abs()).t(), q.abs()),
+           "dv": seen_sums(see.t(), ((unit + 2 * es + 64 * E32) * p + 2.0 ** -25).t(), dy.abs())}
+    return {n: (out[n], tol[n]) for n in out}
+
+
+def check_finite_part(got, ref, what, dtype):
+    """The same entries are finite, and those are near."""
+    value, tol = ref
+    have, want = got.isfinite().cpu(), value.isfinite()
+    assert torch.equal(have, want), (what, (have != want).nonzero()[:5].tolist())
+    tol = tol.nan_to_num(0.0, 0.0, 0.0)
+    check(torch.where(have.to(got.device), got.float(), 0.0).to(got.dtype), torch.where(want, value, 0.0),
+          U[dtype] * (value.nan_to_num(0.0, 0.0, 0.0).abs() + tol) + tol, what, dtype)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("where", ["q", "k", "q and dy"])
+@pytest.mark.parametrize("cap, D, docs, sloped", [(3.0, 64, True, False), (3.0, 128, False, True), (50.0, 48, True, False),
+                                                  (2.0, 32, False, False)])
+def test_a_cap_bounds_infinite_scores(dtype, where, cap, D, docs, sloped):
+    """An infinite element of a query or key makes scores of +-cap: weights, y and dv are finite, and only
+    the gradients that multiply a score gradient of 0 by that element are none."""
+    g = gen(D)
+    N, at = 150, 70
+    q, k, v, dy = (normal(g, 1, N, 2, D, dtype=dtype) for _ in range(4))
+    (q if "q" in where else k)[0, at, 0, 5] = INF
+    if "dy" in where:
+        dy[0, at + 3, 0, 7] = -INF
+    ids = torch.zeros((1, N), dtype=torch.int32, device=DEV)
+    ids[:, 100:] = 1
+    slopes = torch.tensor([0.25, 0.5], device=DEV) if sloped else None
+    leaves = [t.clone().requires_grad_() for t in (q, k, v)]
+    y = cf.softmax_attention(*leaves, softcap=cap, document_ids=ids if docs else None, slopes=slopes)
+    grads = torch.autograd.grad(y, leaves, dy)
+    see = torch.ones((N, N), dtype=torch.bool).tril()
+    if docs:
+        see &= ids[0].cpu()[:, None] == ids[0].cpu()[None]
+    for h in range(2):
+        ref = one_head(*(t[0, :, h].double().cpu() for t in (q, k, v, dy)), see, cap, 0.0 if dtype is F32 else U[dtype],
+                       float(slopes[h]) if sloped else 0.0)
+        for n, got in zip(("y", "dq", "dk", "dv"), (y, *grads)):
+            check_finite_part(got[0, :, h].detach(), ref[n], f"{n} of head {h}", dtype)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("D", [16, 32, 48, 80, 128])
+@pytest.mark.parametrize("what", ["docs", "cap docs", "cap docs prefix slopes", "full docs slopes"])
+def test_attention_of_every_width_with_documents(dtype, D, what):
+    test_attention(dtype, 2, 150, 4, 2, D, what)
