@@ -333,7 +333,7 @@ __global__ __launch_bounds__(64 * kWaves) void scan_gradient_kernel(ScanArgs p) 
     for (int i = 0; i < SL; ++i) {
         const int s = q * SL + i;
         A2[i] = p.A2[s * p.C + c];
-        r[i] = p.NC > 1 ? p.carry[((b * p.NC + chunk) * SP + s) * p.C + c] : 0.0f;
+        r[i] = active && p.NC > 1 ? p.carry[((b * p.NC + chunk) * SP + s) * p.C + c] : 0.0f;
         dA[i] = 0.0f;
     }
     const float* kept = p.kept + ((b * ((p.N + KEEP - 1) / KEEP) + t0 / KEEP) * SP + q * SL) * p.C + c;
@@ -393,7 +393,7 @@ __global__ __launch_bounds__(64 * kWaves) void scan_gradient_kernel(ScanArgs p) 
     for (int first = (n - 1) / KEEP * KEEP; first >= 0; first -= KEEP) {
         const int here = min(KEEP, n - first), pieces = (here + T - 1) / T;
 #pragma unroll
-        for (int i = 0; i < SL; ++i) h[i] = kept[(int64_t)(first / KEEP) * SP * p.C + i * p.C];
+        for (int i = 0; i < SL; ++i) h[i] = active ? kept[(int64_t)(first / KEEP) * SP * p.C + i * p.C] : 0.0f;
         // forward, keeping the state before each piece
         Raw raws[Lay::pieces - 1];
 #pragma unroll
@@ -471,6 +471,10 @@ __global__ __launch_bounds__(64 * kWaves) void scan_gradient_kernel(ScanArgs p) 
                     v[i] = r[i] * uj;
                     v[SL + i] = gj * hv;
                     r[i] *= a[j][i];
+                }
+                if (__builtin_expect(starts >> j & 1, 0)) {      // a decay of 0 times an infinite r is NaN
+#pragma unroll
+                    for (int i = 0; i < SL; ++i) r[i] = 0.0f;
                 }
                 int at;
                 bool own;

@@ -6,11 +6,13 @@ import pytest
 import torch
 
 import causal_flare as cf
+from causal_flare import _lib
 from _mixers import U, attention, check, scan
-from test_gpu_mixers import BF16, DEV, E32, F16, F32, gen, normal, test_attention
+from test_gpu_mixers import BF16, DEV, E32, F16, F32, documents, gen, normal, scan_inputs, test_attention
 
 pytestmark = pytest.mark.gpu
 INF, NAN = math.inf, math.nan
+ORDER = ("x", "dt", "A", "B", "C", "D", "z", "dt_bias")
 
 
 # ---------------------------------------------------------------------------------------
@@ -94,3 +96,54 @@ def test_a_cap_bounds_infinite_scores(dtype, where, cap, D, docs, sloped):
 @pytest.mark.parametrize("what", ["docs", "cap docs", "cap docs prefix slopes", "full docs slopes"])
 def test_attention_of_every_width_with_documents(dtype, D, what):
     test_attention(dtype, 2, 150, 4, 2, D, what)
+
+
+# ---------------------------------------------------------------------------------------
+# State space scan
+# ---------------------------------------------------------------------------------------
+class WithChunk:
+    """The library with chunks of a given length for the scan."""
+
+    def __init__(self, lib, chunk):
+        self._lib, self.flare_scan_chunk = lib, lambda *sizes: chunk
+
+    def __getattr__(self, name):
+        return getattr(self._lib, name)
+
+
+@pytest.fixture
+def chunks(monkeypatch):
+    lib = _lib.lib()
+    return lambda n: monkeypatch.setattr(_lib, "lib", lambda: WithChunk(lib, n))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("chunk", [32, 128])
+@pytest.mark.parametrize("where", ["dy", "x", "z"])
+@pytest.mark.parametrize("C, S", [(48, 16), (70, 8), (20, 40)])
+@pytest.mark.parametrize("poison", [INF, NAN])
+def test_scan_keeps_documents_apart_whatever_one_holds(dtype, chunk, where, C, S, poison, chunks):
+    """A document's infinite values and gradients stay its own: in it, before it and behind it, at
+    borders within a piece of four tokens, within a stretch and where a chunk ends."""
+    chunks(chunk)
+    g = gen(C)
+    N = 200
+    t = scan_inputs(g, 1, N, C, S, 1, dtype)
+    dy = normal(g, 1, N, C, dtype=dtype)
+    ids = torch.zeros((1, N), dtype=torch.int32, device=DEV)
+    for i, cut in enumerate((29, 46, 64, 131, 160)):
+        ids[:, cut:] = i + 1
+    outs = []
+    for bad in (False, True):
+        s, d = {n: x.clone() for n, x in t.items()}, dy.clone()
+        if bad:
+            for row in (40, 130):                                 # documents 1 and 3
+                (d if where == "dy" else s[where])[0, row, C - 1] = poison
+        leaves = [s[n].requires_grad_() for n in ORDER]
+        y = cf.state_space_scan(*leaves, dt_softplus=True, document_ids=ids)
+        grads = torch.autograd.grad(y, leaves, d)
+        outs.append([y.detach()] + [grads[ORDER.index(n)] for n in ("x", "dt", "B", "C", "z")])
+    apart = ((ids[0] != 1) & (ids[0] != 3)).cpu()
+    for name, a, b in zip(("y", "dx", "ddt", "dB", "dC", "dz"), *outs):
+        assert torch.equal(a[:, apart], b[:, apart]), name
+    assert not outs[1][1 if where == "dy" else 0].isfinite().all()
