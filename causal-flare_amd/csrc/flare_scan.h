@@ -58,11 +58,12 @@ __device__ __forceinline__ int64_t row_length(const ScanArgs& p, int64_t b) {
     const int64_t n = p.lengths[b];
     return n < 0 ? 0 : (n > p.N ? p.N : n);
 }
-// The state `h` behind a chunk whose tokens sum up to A2 dsum (log2 units).  In two halves: a decay
-// that grows past fp32 over a chunk is none of a state that is 0 or small enough.
+// The state `h` behind a chunk whose tokens sum up to A2 dsum (log2 units).  In two halves, so that
+// growth past fp32 leaves a small state what it is token by token; past 2^256 any but 0 is infinite,
+// and 0 stays 0.
 __device__ __forceinline__ float decayed(float h, float A2dsum) {
     const float e = __builtin_amdgcn_exp2f(0.5f * A2dsum);
-    return h * e * e;
+    return h == 0.0f ? 0.0f : h * e * e;
 }
 // Whether token t begins a document.
 __device__ __forceinline__ bool begins(const int32_t* ids, int64_t t) { return t > 0 && ids[t] != ids[t - 1]; }

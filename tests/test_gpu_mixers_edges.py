@@ -8,7 +8,7 @@ import torch
 import causal_flare as cf
 from causal_flare import _lib
 from _mixers import U, attention, check, scan
-from test_gpu_mixers import BF16, DEV, E32, F16, F32, documents, gen, normal, scan_inputs, test_attention
+from test_gpu_mixers import BF16, DEV, E32, F16, F32, close, documents, gen, normal, scan_inputs, test_attention
 
 pytestmark = pytest.mark.gpu
 INF, NAN = math.inf, math.nan
@@ -147,3 +147,28 @@ def test_scan_keeps_documents_apart_whatever_one_holds(dtype, chunk, where, C, S
     for name, a, b in zip(("y", "dx", "ddt", "dB", "dC", "dz"), *outs):
         assert torch.equal(a[:, apart], b[:, apart]), name
     assert not outs[1][1 if where == "dy" else 0].isfinite().all()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("chunk", [32, 128])
+def test_scan_of_zero_states_and_gradients_under_any_growth(dtype, chunk, chunks):
+    """States grow by 2^9 a token, 2^288 and more over a chunk: one of 0 stays 0 as it does token by
+    token, and so does the gradient that enters from behind."""
+    chunks(chunk)
+    g = gen(3)
+    N, C, S = 400, 20, 16
+    z = torch.zeros((1, N, C), dtype=dtype, device=DEV)
+    t = {"x": z.clone(), "dt": z + 1, "A": torch.full((C, S), 9 * math.log(2.0), device=DEV),
+         "B": normal(g, 1, N, 1, S, dtype=dtype), "C": normal(g, 1, N, 1, S, dtype=dtype), "D": normal(g, C),
+         "z": normal(g, 1, N, C, dtype=dtype), "dt_bias": None}
+    dy = z.clone()
+    t["x"][:, -6:], dy[:, :6] = normal(g, 1, 6, C, dtype=dtype), normal(g, 1, 6, C, dtype=dtype)
+    names = [n for n in ORDER if t[n] is not None]
+    leaves = {n: t[n].clone().requires_grad_() for n in names}
+    y = cf.state_space_scan(*[leaves.get(n) for n in ORDER])
+    grads = torch.autograd.grad(y, [leaves[n] for n in names], dy)
+    ref = scan(**t, dy=dy)
+    assert y.isfinite().all() and all(x.isfinite().all() for x in grads)
+    close(y, ref["y"], "y", dtype, ref["k"])
+    for n, got in zip(names, grads):
+        close(got, ref["d" + n], "d" + n, F32 if n in "AD" else dtype, 2 * ref["k"] + C)
