@@ -315,7 +315,10 @@ __global__ __launch_bounds__(256, 2) void attn_forward_kernel(AttnArgs p) {
     for (int t = 0; t < QT; ++t) {
         const int i = w0 + 16 * t + c;
         const float total = column_sum(sum[t]);
-        const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+        // Every query but padding and those behind the length sees itself.  (A sum of 0 does not tell: the
+        // scores of one that sees keys may all be -inf, and its y is NaN.)
+        const bool sees = lim[t] > 0 && (!p.ids || qid[t] != kNoQuery);
+        const float inv = sees ? 1.0f / total : 0.0f;
         if (i >= p.N) continue;
         if (parts > 1) {
             float* to = p.parts + (((b * p.H + h) * p.N + i) * parts + part) * (p.D + 4);
@@ -329,7 +332,7 @@ __global__ __launch_bounds__(256, 2) void attn_forward_kernel(AttnArgs p) {
             continue;
         }
         if (p.lse && g == 0)
-            p.lse[(b * p.H + h) * p.N + i] = total == 0.0f ? -kNegInf : top[t] + __builtin_amdgcn_logf(total);
+            p.lse[(b * p.H + h) * p.N + i] = sees ? top[t] + __builtin_amdgcn_logf(total) : -kNegInf;
         const int64_t row = ((b * p.N + i) * p.H + h) * p.D;
 #pragma unroll
         for (int d = 0; d < DT; ++d) {
@@ -351,13 +354,16 @@ __global__ __launch_bounds__(256) void attn_rows_kernel(AttnArgs p) {
     if (row >= p.B * p.H * p.N || d >= p.D) return;
     const int64_t i = row % p.N, h = row / p.N % p.H, b = row / p.N / p.H;
     const Joined j = join_parts<1, 4>(p.parts + row * p.splits * (p.D + 4), 0, (int)p.splits, p.D, d);
-    f32x4 v = j.v * (j.total == 0.0f ? 0.0f : 1.0f / j.total);
+    bool sees = !p.ids || p.ids[b * p.N + i] >= 0, refused = false;       // as in attn_forward
     if (p.lengths) {
         const int64_t off = p.lengths[b], n = p.fresh ? clamp_to(p.fresh[b], p.N) : p.N;
-        if (off >= 0 && off + n > p.M) v = f32x4{__builtin_nanf(""), __builtin_nanf(""), __builtin_nanf(""), __builtin_nanf("")};
+        sees = off >= 0 && i < n;
+        refused = off >= 0 && off + n > p.M;
     }
+    f32x4 v = sees ? j.v * (1.0f / j.total) : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    if (refused) v = f32x4{__builtin_nanf(""), __builtin_nanf(""), __builtin_nanf(""), __builtin_nanf("")};
     put_y<S>(p, ((b * p.N + i) * p.H + h) * p.D + d, v);
-    if (p.lse && d == 0) p.lse[row] = j.total == 0.0f ? -kNegInf : j.top + __builtin_amdgcn_logf(j.total);
+    if (p.lse && d == 0) p.lse[row] = sees ? j.top + __builtin_amdgcn_logf(j.total) : -kNegInf;
 }
 
 template <typename E, int DP, int CAP>

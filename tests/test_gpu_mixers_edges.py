@@ -98,6 +98,39 @@ def test_attention_of_every_width_with_documents(dtype, D, what):
     test_attention(dtype, 2, 150, 4, 2, D, what)
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("N", [130, 1700])
+def test_a_row_of_scores_that_are_all_minus_infinity_is_nan(dtype, N):
+    """It sees keys, so it is no row of 0; rows and keys apart from it stay as they are.  1700 rows run in
+    parts of the keys."""
+    g = gen(N)
+    H, D, at = 2, 64, 67
+    q, k, v, dy = (normal(g, 1, N, H, D, dtype=dtype) for _ in range(4))
+    k[0, :, 0, 0] = -1.0
+    bad = q.clone()
+    bad[0, at, 0, 0] = INF
+    outs = []
+    for x in (q, bad):
+        leaves = [x.clone().requires_grad_(), k.clone().requires_grad_(), v.clone().requires_grad_()]
+        y = cf.softmax_attention(*leaves)
+        outs.append([y.detach(), *torch.autograd.grad(y, leaves, dy)])
+    rest = [i for i in range(N) if i != at]
+    assert outs[1][0][0, at, 0].isnan().all() and outs[1][1][0, at, 0].isnan().all()
+    for i in (0, 1):
+        assert torch.equal(outs[0][i][:, rest], outs[1][i][:, rest])
+    for i in (2, 3):
+        assert torch.equal(outs[0][i][:, at + 1:], outs[1][i][:, at + 1:])
+        assert torch.equal(outs[0][i][:, :, 1], outs[1][i][:, :, 1])
+        assert outs[1][i][0, :at + 1, 0].isnan().all()
+    cache = {"k": k.clone(), "v": v.clone()}
+    held = torch.tensor([at], device=DEV)
+    new = [t[:, at:at + 4] for t in (bad, k, v)]
+    y, _ = cf.softmax_attention_prefill(*new, cache, held, new_lengths=torch.tensor([2], device=DEV))
+    assert y[0, 0, 0].isnan().all() and y[0, 1].isfinite().all() and not y[0, 2:].any()
+    y, _ = cf.softmax_attention_decode(*(t[:, 0] for t in new), cache, held)
+    assert y[0, 0, 0].isnan().all() and y[0, 0, 1].isfinite().all()
+
+
 # ---------------------------------------------------------------------------------------
 # State space scan
 # ---------------------------------------------------------------------------------------
