@@ -18,8 +18,6 @@ holds is the caller's to keep, in `lengths`.
 """
 from __future__ import annotations
 
-import math
-
 import torch
 import torch.autograd as autograd
 from torch.autograd.function import once_differentiable
@@ -44,6 +42,10 @@ from ._inputs import (
 )
 
 
+# Caps that the kernels take: what scale / cap and the cap itself can be with in float32.
+_LEAST_CAP, _MOST_CAP = 2.0 ** -100, 2.0 ** 100
+
+
 def _check_scores(name, H, scale, softcap, slopes):
     """The cap, 0 for none, of checked arguments."""
     _check_shape(name, "slopes", slopes, (H,))
@@ -52,8 +54,8 @@ def _check_scores(name, H, scale, softcap, slopes):
         raise NotImplementedError(f"{name} has no gradient for slopes; pass slopes.detach()")
     if softcap is None:
         return 0.0
-    if not (math.isfinite(softcap) and softcap > 0):
-        raise ValueError(f"{name} expects softcap None or positive. Got {softcap!r}")
+    if not _LEAST_CAP <= softcap <= _MOST_CAP:
+        raise ValueError(f"{name} expects softcap None or positive, between 2^-100 and 2^100. Got {softcap!r}")
     return float(softcap)
 
 
@@ -163,7 +165,7 @@ def softmax_attention(
 ):
     """Softmax attention of whole sequences, differentiable in Q, K and V.
 
-    scale: D**-0.5 by default.  slopes: [H], the bias on distance (constants, no gradient).
+    scale: D**-0.5 by default.  softcap: between 2^-100 and 2^100.  slopes: [H], the bias on distance (constants, no gradient).
     document_ids: integers [B, N]; queries see keys of their own id only, and a negative id is
     padding, with y = 0 and no gradient.  prefix_lengths: integers [B]; the first so many keys of
     a sequence are seen by all its queries (of the same document).
@@ -250,7 +252,7 @@ def _step_fast(Q, K, V, cache, lengths, scale, softcap, slopes):
             or H < 1 or H % G or D % 16 or not 16 <= D <= 128 or lengths.dtype is not torch.int32
             or lengths.shape != (B,) or lengths.device != device or not lengths.is_contiguous()
             or not _plain_f32(slopes, device, H) or (slopes is not None and slopes.requires_grad)
-            or (softcap is not None and not 0.0 < softcap < math.inf)):
+            or (softcap is not None and not _LEAST_CAP <= softcap <= _MOST_CAP)):
         return None
     pointers = [t.data_ptr() for t in (Q, K, V, kc, vc)]
     strides, spread = [], 0

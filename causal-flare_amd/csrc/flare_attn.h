@@ -74,6 +74,19 @@ struct AttnArgs {
     int64_t splits;
 };
 
+// How a kernel takes scores: as they are; capped, with tanh to an absolute error (kCap), and against the
+// cap itself in place of a running maximum where nothing is added (kCapFixed, forward); or with a tanh that
+// keeps the digits of small scores too (kCapFine).
+enum { kNoCap = 0, kCap = 1, kCapFixed = 2, kCapFine = 3 };
+// tanh as 1 - 2 / (e^2x + 1) leaves a score some 1.3e-7 of the cap off, however small it is: up to this cap
+// 2^-15, a sixteenth of what fp16's rounding of a weight is off by.  Beyond it, and for fp32 inputs,
+// kCapFine.  us of 4 x 4096 rows, 16 heads of 64, fp16, with caps of 200 and of 300: forward 286, 401; dq
+// 442, 535; dk and dv 554, 738.  (Single tokens always: 185 us with either.)
+constexpr float kCoarseCapMost = 256.0f;
+// Caps that keep scale / cap and cap log2(e) far from fp32's ends.
+constexpr float kLeastCap = 0x1p-100f, kMostCap = 0x1p100f;
+inline bool coarse_cap(float cap, int size) { return size == 2 && cap <= kCoarseCapMost; }
+
 // Tiles of 16 queries a wave of the forward's and the query gradients' kernels owns (fp32 operands take
 // twice the registers).
 constexpr int q_tiles(int size) { return size == 2 ? 2 : 1; }
@@ -199,12 +212,7 @@ __device__ __forceinline__ float column_sum(float x) {
     return b.first + b.second;
 }
 
-// tanh(x) = 1 - 2 / (e^2x + 1): absolute error some 1e-7, which times the cap is far less than the
-// scores of 16-bit inputs are off by.  `x2`: 2 x log2(e).
-__device__ __forceinline__ float tanh_log2(float x2) {
-    return 1.0f - 2.0f * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(x2));
-}
-// For fp32 inputs: tanh(x) with a relative error of some 2^-23 for small x too, and (1 - tanh^2) / 4.  Below
+// tanh(x) with a relative error of some 2^-23 for small x too, and (1 - tanh^2) / 4.  Below
 // 0.7 the continued fraction x / (1 + x^2 / (3 + x^2 / (5 + x^2 / (7 + x^2 / 9)))), 2e-9 off there.
 struct Tanh {
     float t, slope;

@@ -185,7 +185,8 @@ using namespace flare::attn;
                   "128", (long long)D);                                                                           \
     FLARE_REQUIRE(N <= (1 << 30) && M <= (1 << 30) && B <= 65535 && H <= 65535 && B * H <= (1 << 24) &&           \
                   (N + 63) / 64 * B * H <= (1 << 26) && H * D < kMostStride, name ": too large");                                        \
-    FLARE_REQUIRE(softcap >= 0.0f && softcap < __builtin_huge_valf(), name ": the cap must be finite and not negative")
+    FLARE_REQUIRE(softcap == 0.0f || (softcap >= kLeastCap && softcap <= kMostCap),                                \
+                  name ": the cap must be 0 (none) or between 2^-100 and 2^100")
 
 static AttnArgs attn_args(const void* q, const void* k, const void* v, const int64_t* st, int64_t B, int64_t N,
                           int64_t M, int64_t H, int64_t G, int64_t D, float scale, float softcap,

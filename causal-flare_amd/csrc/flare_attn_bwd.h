@@ -84,7 +84,7 @@ struct BackwardLds {
     static constexpr size_t bytes = 4 * tile + 2 * (3 * T + 4) * sizeof(float);
 };
 
-template <typename E, int DP, int QT, bool CAP>
+template <typename E, int DP, int QT, int CAP>
 __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnArgs p) {
     typedef typename Elem<E>::S S;
     typedef typename Elem<E>::Frag Frag;
@@ -228,7 +228,7 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnArgs p) {
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         float x = s[t][n][i], slope = 1.0f;        // a quarter of 1 - tanh^2
-                        if (CAP && sizeof(E) == 4) {
+                        if (CAP == kCapFine) {
                             const Tanh u = fine_tanh(x * to_tanh);
                             x = cap2 * u.t - lse[t];
                             slope = u.slope;
@@ -318,7 +318,7 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnArgs p) {
     }
 }
 
-template <typename E, int DP, int KQ, bool CAP>
+template <typename E, int DP, int KQ, int CAP>
 __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(AttnArgs p) {
     typedef typename Elem<E>::S S;
     typedef typename Elem<E>::Frag Frag;
@@ -405,7 +405,7 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(AttnArgs p) {
         if (tid < QR) {
             const bool live = q0 + tid < N;
             const int64_t at = (b * p.H + h) * p.N + q0 + tid;
-            next_lse = live ? p.lse[at] - kShift - (sizeof(E) == 4 ? 0.0f : cap2) : -kNegInf;
+            next_lse = live ? p.lse[at] - kShift - (CAP == kCap ? cap2 : 0.0f) : -kNegInf;
             next_delta = live ? p.delta[at] * kUnshift : 0.0f;
             next_id = !live ? kNoQuery : p.ids ? p.ids[b * p.N + q0 + tid] : 0;
             next_id = next_id < 0 ? kNoQuery : next_id;
@@ -474,7 +474,7 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(AttnArgs p) {
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
                             float x = s[t][n][i], slope = 1.0f;
-                            if (CAP && sizeof(E) == 4) {
+                            if (CAP == kCapFine) {
                                 const Tanh u = fine_tanh(x * to_tanh);
                                 x = cap2 * u.t - lse[i];
                                 slope = u.slope;
@@ -617,7 +617,7 @@ static int allow_lds(K kernel, size_t bytes, const char* what) {
     return FLARE_ERR_LAUNCH;
 }
 
-template <typename E, int DP, bool CAP>
+template <typename E, int DP, int CAP>
 static int backward_cap(const AttnArgs& p, hipStream_t stream) {
     constexpr int QT = q_tiles(sizeof(E));
     constexpr size_t bytes = BackwardLds<E, DP>::bytes;
@@ -638,7 +638,10 @@ static int backward_cap(const AttnArgs& p, hipStream_t stream) {
 }
 template <typename E, int DP>
 static int backward_dp(const AttnArgs& p, hipStream_t stream) {
-    return p.cap > 0.0f ? backward_cap<E, DP, true>(p, stream) : backward_cap<E, DP, false>(p, stream);
+    if (p.cap == 0.0f) return backward_cap<E, DP, kNoCap>(p, stream);
+    if constexpr (sizeof(E) == 2)
+        if (coarse_cap(p.cap, sizeof(E))) return backward_cap<E, DP, kCap>(p, stream);
+    return backward_cap<E, DP, kCapFine>(p, stream);
 }
 template <typename E>
 int backward_e(const AttnArgs& p, float* delta, hipStream_t stream) {

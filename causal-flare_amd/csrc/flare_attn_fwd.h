@@ -19,9 +19,6 @@
 namespace flare {
 namespace attn {
 
-// How scores are kept from overflowing: against a running maximum, or against the cap itself,
-// which bounds them where nothing is added.
-enum { kNoCap = 0, kCapRunning = 1, kCapFixed = 2 };
 // With weights of 2^(s - cap) a row's largest is at least 2^(-2 cap): bf16 holds that, with all that
 // counts beside it, up to here (log2 units), and fp16 does not.  fp32 would, but s - cap rounds to fewer
 // digits than s has.
@@ -194,7 +191,7 @@ __global__ __launch_bounds__(256, 2) void attn_forward_kernel(AttnArgs p) {
                     for (int n = 0; n < NK; ++n) {
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
-                            if constexpr (sizeof(E) == 4) {
+                            if constexpr (CAP == kCapFine) {
                                 s[t][n][i] = cap2 * fine_tanh(s[t][n][i] * to_tanh).t;
                                 continue;
                             }
@@ -391,7 +388,9 @@ static int forward_dp(const AttnArgs& p, hipStream_t stream) {
     if (p.cap == 0.0f) return forward_cap<E, DP, kNoCap>(p, stream);
     if constexpr (__is_same(E, __hip_bfloat16))
         if (!p.slopes && p.cap * kLog2e <= kCapFixedMost) return forward_cap<E, DP, kCapFixed>(p, stream);
-    return forward_cap<E, DP, kCapRunning>(p, stream);
+    if constexpr (sizeof(E) == 2)
+        if (coarse_cap(p.cap, sizeof(E))) return forward_cap<E, DP, kCap>(p, stream);
+    return forward_cap<E, DP, kCapFine>(p, stream);
 }
 template <typename E>
 int forward_e(const AttnArgs& p, hipStream_t stream) {

@@ -388,7 +388,7 @@ int flare_scan_step(const void* x, const void* dt, const float* A, const void* B
 
 /*
  * y_i = sum_j softmax_j(s_ij) v_j, s_ij = x_ij - slopes[h] |i - j|, x_ij = scale q_i . k_j or (softcap
- * > 0) softcap tanh(scale q_i . k_j / softcap).  q [B, N, H, D], k and v [B, M, G, D], head h reads
+ * > 0, from 2^-100 to 2^100) softcap tanh(scale q_i . k_j / softcap).  q [B, N, H, D], k and v [B, M, G, D], head h reads
  * key head h / (H / G); D a multiple of 16 up to 128; every row on a 16-byte boundary.  strides:
  * batch, token and head of q, k, v (9 numbers, host).  causal: query i sees keys j <= i, and
  * those below prefix_lengths[b] (or NULL).  Without `lengths` M == N.  With them k and v are

@@ -8,7 +8,8 @@ import torch
 import causal_flare as cf
 from causal_flare import _lib
 from _mixers import U, attention, check, scan
-from test_gpu_mixers import BF16, DEV, E32, F16, F32, close, documents, gen, normal, scan_inputs, test_attention
+from test_gpu_mixers import (BF16, DEV, E32, F16, F32, close, close_attention, documents, gen, normal, scan_inputs,
+                             test_attention)
 
 pytestmark = pytest.mark.gpu
 INF, NAN = math.inf, math.nan
@@ -129,6 +130,34 @@ def test_a_row_of_scores_that_are_all_minus_infinity_is_nan(dtype, N):
     assert y[0, 0, 0].isnan().all() and y[0, 1].isfinite().all() and not y[0, 2:].any()
     y, _ = cf.softmax_attention_decode(*(t[:, 0] for t in new), cache, held)
     assert y[0, 0, 0].isnan().all() and y[0, 0, 1].isfinite().all()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("cap", [300.0, 1e4, 1e6, 1e8, 1e20])
+@pytest.mark.parametrize("sloped", [False, True])
+def test_large_caps_leave_small_scores_their_digits(dtype, cap, sloped):
+    """A score far below the cap is nearly itself, so its error is that of a score without a cap
+    (the tolerance of the call without one), however large the cap."""
+    g = gen(41)
+    N, H, D = 150, 2, 64
+    q, k, v, dy = (normal(g, 1, N, H, D, dtype=dtype, std=s) for s in (2.0, 1.0, 1.0, 1.0))
+    o = {"slopes": torch.tensor([0.125, 0.5], device=DEV)} if sloped else {}
+    leaves = [t.clone().requires_grad_() for t in (q, k, v)]
+    y = cf.softmax_attention(*leaves, softcap=cap, **o)
+    grads = torch.autograd.grad(y, leaves, dy)
+    unit = 0.0 if dtype is F32 else U[dtype]
+    tiny = 2.0 ** -25 if dtype is F16 else 2.0 ** -126
+    ref, loose = (attention(q, k, v, softcap=c, dy=dy, unit=unit, tiny=tiny, **o) for c in (cap, None))
+    for n, got in zip(("y", "dq", "dk", "dv"), (y, *grads)):
+        close_attention(got, (ref[n][0], loose[n][1]), n, dtype)
+    at = N - 1
+    cache = {n: torch.cat((t[:, :at], torch.zeros_like(t)), 1) for n, t in (("k", k), ("v", v))}
+    held = torch.tensor([at], device=DEV, dtype=torch.int32)
+    step, _ = cf.softmax_attention_decode(q[:, at], k[:, at], v[:, at], cache, held, softcap=cap, **o)
+    close_attention(step, (ref["y"][0][:, at:], loose["y"][1][:, at:]), "token", dtype)
+    held -= 40
+    y, _ = cf.softmax_attention_prefill(q[:, at - 40:], k[:, at - 40:], v[:, at - 40:], cache, held, softcap=cap, **o)
+    close_attention(y, (ref["y"][0][:, at - 40:], loose["y"][1][:, at - 40:]), "prompt", dtype)
 
 
 # ---------------------------------------------------------------------------------------

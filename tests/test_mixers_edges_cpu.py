@@ -1,0 +1,32 @@
+"""Refusals of the token mixers where an argument leaves its range, without a GPU."""
+import ctypes
+
+import pytest
+import torch
+
+import causal_flare as cf
+from causal_flare import _lib
+
+
+def t(*shape, dtype=torch.float32):
+    return torch.zeros(shape, dtype=dtype)
+
+
+def ints(*shape):
+    return torch.zeros(shape, dtype=torch.int32)
+
+
+@pytest.mark.parametrize("cap", [1e-50, 1e-31, 1e31, 1e39, float("nan"), -1.0])
+def test_caps_out_of_range_are_refused(cap):
+    """Below float32's range a cap would be 0, which stands for none."""
+    qkv, cache = [t(2, 5, 4, 32)] * 3, {x: t(2, 9, 4, 32) for x in "kv"}
+    for call in (lambda: cf.softmax_attention(*qkv, softcap=cap),
+                 lambda: cf.softmax_attention_prefill(*qkv, cache, ints(2), softcap=cap),
+                 lambda: cf.softmax_attention_decode(*(x[:, 0] for x in qkv), cache, ints(2), softcap=cap)):
+        with pytest.raises(ValueError, match="softcap None or positive"):
+            call()
+    if cap in (1e-31, 1e31, -1.0):
+        lib, P, nine = _lib.lib(), ctypes.c_void_p(4096), (ctypes.c_int64 * 9)(*[8] * 9)
+        rc = lib.flare_attn_forward(P, P, P, nine, 1, 1, 4, 4, 4, 4, 64, 1.0, cap, None, 1, None, None, None, None, P, None,
+                                    None, None, 0, None)
+        assert rc == -1 and b"cap" in lib.flare_last_error()
