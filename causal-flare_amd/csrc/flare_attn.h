@@ -63,6 +63,8 @@ struct AttnArgs {
     // backward
     const void* dy;                  // [B, N, H, D]
     const float* delta;              // [B, H, N]: dy . y
+    const float* norms;              // [B, H, N]: sum of |dy| (fp16)
+    const float* ranges;             // [B, tiles, 2]: of 64 tokens the largest norm and |v| (fp16)
     void *dq, *dk, *dv;
     int64_t row_splits;              // of `splits`: parts of the rows, times parts of the heads
     float* dq_parts;                 // what `dq_splits` workgroups leave of each row of dq

@@ -6,7 +6,7 @@ namespace flare {
 namespace attn {
 
 template <typename E> int forward_e(const AttnArgs& p, hipStream_t stream);
-template <typename E> int backward_e(const AttnArgs& p, float* delta, hipStream_t stream);
+template <typename E> int backward_e(const AttnArgs& p, float* delta, float* norms, float* ranges, hipStream_t stream);
 int attn_step(const AttnArgs& p, int dtype, hipStream_t stream);
 
 // A wave for each 64 tokens.
@@ -231,15 +231,19 @@ extern "C" int flare_attn_forward(const void* q, const void* k, const void* v, c
     return FLARE_BY_DTYPE(dtype, forward_e, (p, (hipStream_t)stream));
 }
 
-static size_t backward_head_bytes(int64_t B, int64_t N, int64_t H) {
-    return ((size_t)(B * H * N) * sizeof(float) + stats_bytes(B, N) + 255) / 256 * 256;
+// delta, fp16's norms and ranges, and the id statistics.
+static int64_t norms_floats(int64_t B, int64_t N, int64_t H, int dtype) { return dtype == FLARE_F16 ? B * H * N : 0; }
+static int64_t ranges_floats(int64_t B, int64_t N, int dtype) { return dtype == FLARE_F16 ? B * ceil_div(N, kIdTile) * 2 : 0; }
+static size_t backward_head_bytes(int64_t B, int64_t N, int64_t H, int dtype) {
+    const int64_t floats = B * H * N + norms_floats(B, N, H, dtype) + ranges_floats(B, N, dtype);
+    return ((size_t)floats * sizeof(float) + stats_bytes(B, N) + 255) / 256 * 256;
 }
 extern "C" size_t flare_attn_backward_workspace_size(int64_t B, int64_t N, int64_t H, int64_t G, int64_t D, int dtype) {
     if (B < 1 || N < 1 || H < 1 || G < 1 || H % G) return 0;
     AttnArgs p = {};
     p.B = B, p.N = N, p.H = H, p.G = G, p.D = D;
     split_backward(p, dtype);
-    return backward_head_bytes(B, N, H) + parts_bytes(p) + dq_bytes(p);
+    return backward_head_bytes(B, N, H, dtype) + parts_bytes(p) + dq_bytes(p);
 }
 
 extern "C" int flare_attn_backward(const void* q, const void* k, const void* v, const int64_t* strides, int dtype,
@@ -262,15 +266,18 @@ extern "C" int flare_attn_backward(const void* q, const void* k, const void* v, 
         return FLARE_ERR_WORKSPACE;
     }
     float* delta = (float*)workspace;
+    float* norms = delta + B * H * N;
+    float* ranges = norms + norms_floats(B, N, H, dtype);
+    int32_t* stats = (int32_t*)(ranges + ranges_floats(B, N, dtype));
     p.causal = causal, p.ids = document_ids, p.prefix = prefix_lengths;
-    p.y = const_cast<void*>(y), p.y_rest = const_cast<void*>(y_rest), p.lse = const_cast<float*>(lse), p.dy = dy, p.delta = delta;
+    p.y = const_cast<void*>(y), p.y_rest = const_cast<void*>(y_rest), p.lse = const_cast<float*>(lse), p.dy = dy, p.delta = delta, p.norms = norms, p.ranges = ranges;
     p.dq = dq, p.dk = dk, p.dv = dv;
     split_backward(p, dtype);
-    p.parts = (float*)((char*)workspace + backward_head_bytes(B, N, H));
+    p.parts = (float*)((char*)workspace + backward_head_bytes(B, N, H, dtype));
     p.dq_parts = (float*)((char*)p.parts + parts_bytes(p));
-    const int rc = launch_ids(p, dtype, true, (int32_t*)(delta + B * H * N), (hipStream_t)stream);
+    const int rc = launch_ids(p, dtype, true, stats, (hipStream_t)stream);
     if (rc != FLARE_OK) return rc;
-    return FLARE_BY_DTYPE(dtype, backward_e, (p, delta, (hipStream_t)stream));
+    return FLARE_BY_DTYPE(dtype, backward_e, (p, delta, norms, ranges, (hipStream_t)stream));
 }
 
 extern "C" int flare_attn_append(const void* k, const void* v, const int64_t* strides, int dtype, int64_t B, int64_t N,

@@ -5,6 +5,6 @@
 namespace flare {
 namespace attn {
 template int forward_e<__hip_bfloat16>(const AttnArgs&, hipStream_t);
-template int backward_e<__hip_bfloat16>(const AttnArgs&, float*, hipStream_t);
+template int backward_e<__hip_bfloat16>(const AttnArgs&, float*, float*, float*, hipStream_t);
 }  // namespace attn
 }  // namespace flare

@@ -28,32 +28,105 @@
 namespace flare {
 namespace attn {
 
+// Score gradients of fp16 inputs go into their products times a power of 2: with a small dy or long rows
+// they lie below fp16's smallest numbers otherwise, the second part too (4096 keys, dy of 1e-4: dq 8%
+// off).  |dS_ij| <= |dy_i . v_j| + |dy_i . y_i| <= 2 |dy_i|_1 max|v| comes to between 2^14 and 2^15 so: row by
+// row in dq, in dk for all rows that see a workgroup's keys.  attn_ranges, which that takes, is 5 us for
+// 512 rows of 8 heads of 64, 7 for 16384 of 16 heads of 128 over 4.
+template <typename E> constexpr bool kScaled = __is_same(E, __half);
+
 // delta, from y before its rounding (y and what it was rounded by): an error of delta adds to all of
 // a row's dS with one sign.  bf16 dq and dk were 2.7e-3 to 3.0e-3 off the 64-bit ones (norms) with
 // delta from the rounded y.  `lanes` (a power of 2) for each row of a head, 16 bytes of it a lane.
 template <typename E>
-__global__ __launch_bounds__(256) void attn_delta_kernel(AttnArgs p, int lanes, float* delta) {
+__global__ __launch_bounds__(256) void attn_delta_kernel(AttnArgs p, int lanes, float* delta, float* norms) {
     typedef typename Elem<E>::S S;
     constexpr int PER = 16 / sizeof(E);
     const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x, row = id / lanes;         // (b, i, h)
     if (row >= p.B * p.N * p.H) return;                    // whole rows
     const int col = (int)(id % lanes) * PER;
-    float s = 0.0f;
+    float s = 0.0f, norm = 0.0f;
     if (col < p.D) {
         typedef S V __attribute__((ext_vector_type(PER)));
         const V y = *reinterpret_cast<const V*>((const S*)p.y + row * p.D + col);
         const V dy = *reinterpret_cast<const V*>((const S*)p.dy + row * p.D + col);
 #pragma unroll
-        for (int i = 0; i < PER; ++i) s += (float)y[i] * (float)dy[i];
+        for (int i = 0; i < PER; ++i) {
+            s += (float)y[i] * (float)dy[i];
+            if (kScaled<E>) norm += fabsf((float)dy[i]);
+        }
         if (p.y_rest) {
             const V rest = *reinterpret_cast<const V*>((const S*)p.y_rest + row * p.D + col);
 #pragma unroll
             for (int i = 0; i < PER; ++i) s += (float)rest[i] * (float)dy[i];
         }
     }
-    for (int o = lanes / 2; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
+    for (int o = lanes / 2; o > 0; o >>= 1) {
+        s += __shfl_xor(s, o, 64);
+        if (kScaled<E>) norm += __shfl_xor(norm, o, 64);
+    }
     const int64_t h = row % p.H, i = row / p.H % p.N, b = row / p.H / p.N;
-    if (col == 0) delta[(b * p.H + h) * p.N + i] = s;
+    if (col) return;
+    delta[(b * p.H + h) * p.N + i] = s;
+    if (kScaled<E>) norms[(b * p.H + h) * p.N + i] = norm;
+}
+
+// The largest of each 64 tokens' |dy|_1 and |v|: padding and what is infinite or NaN do not count.
+__device__ __forceinline__ float wave_max(float x) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) x = fmaxf(x, __shfl_xor(x, o, 64));
+    return x;
+}
+template <typename E>
+__global__ __launch_bounds__(1024) void attn_ranges_kernel(AttnArgs p, float* ranges) {
+    typedef typename Elem<E>::S S;
+    __shared__ float left[16][2];
+    const int64_t b = blockIdx.y, first = (int64_t)blockIdx.x * kIdTile;
+    const int n = (int)min((int64_t)kIdTile, p.N - first), D8 = (int)p.D / 8, GD8 = (int)p.G * D8;
+    const int32_t* ids = p.ids ? p.ids + b * p.N + first : nullptr;
+    float norm = 0.0f, most = 0.0f;
+    for (int e = threadIdx.x; e < (int)p.H * kIdTile; e += 1024) {
+        const int i = e % kIdTile;
+        if (i >= n || (ids && ids[i] < 0)) continue;
+        const float x = p.norms[(b * p.H + e / kIdTile) * p.N + first + i];
+        if (x < -kNegInf) norm = fmaxf(norm, x);
+    }
+#pragma unroll 4
+    for (int e = threadIdx.x; e < n * GD8; e += 1024) {
+        const int i = e / GD8, g = e % GD8 / D8;
+        if (ids && ids[i] < 0) continue;
+        const auto v = frag_rows<E>((const S*)p.v.p + b * p.v.sb + (first + i) * p.v.sn + g * p.v.sh + e % D8 * 8);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const float x = fabsf((float)v[j]);
+            if (x < -kNegInf) most = fmaxf(most, x);
+        }
+    }
+    norm = wave_max(norm), most = wave_max(most);
+    if ((threadIdx.x & 63) == 0) {
+        left[threadIdx.x >> 6][0] = norm;
+        left[threadIdx.x >> 6][1] = most;
+    }
+    __syncthreads();
+    if (threadIdx.x < 2) {
+        float x = 0.0f;
+#pragma unroll
+        for (int w = 0; w < 16; ++w) x = fmaxf(x, left[w][threadIdx.x]);
+        ranges[(b * gridDim.x + blockIdx.x) * 2 + threadIdx.x] = x;
+    }
+}
+// Over the tiles of tokens first .. last-1 that `mine` meets; the same in all lanes of the wave.
+__device__ __forceinline__ float largest(const AttnArgs& p, int64_t b, int which, int first, int last, IdRange mine) {
+    const int tiles = id_tiles(p.N);
+    float most = 0.0f;
+    for (int t = first / kIdTile + (threadIdx.x & 63); t * kIdTile < last; t += 64)
+        if (!p.ids || id_range(p, b, t).meets(mine)) most = fmaxf(most, p.ranges[(b * tiles + t) * 2 + which]);
+    return wave_max(most);
+}
+// The power of 2 that brings `bound` to between 2^14 and 2^15.
+__device__ __forceinline__ float scale_to(float bound) {
+    if (!(bound > 0.0f && bound < -kNegInf)) return 1.0f;
+    return __builtin_ldexpf(1.0f, 15 - __builtin_amdgcn_frexp_expf(bound));
 }
 
 // An infinite value or NaN in a row of K, Q or dY counts for the pairs that see that row, and a weight
@@ -119,7 +192,8 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnArgs p) {
     const int w0 = q0 + wave * 16 * QT;
     Frag qf[QT][DK], gf[QT][DK];
     int pos[QT], lim[QT], qid[QT];                     // as in attn_forward
-    float lse[QT], delta[QT];
+    float lse[QT], delta[QT], factor[QT];
+    const float most_v = kScaled<E> ? largest(p, b, 1, k_begin, kv_end, mine) : 0.0f;
 #pragma unroll
     for (int t = 0; t < QT; ++t) {
         const int i = w0 + 16 * t + c;
@@ -133,6 +207,11 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnArgs p) {
         }
         lse[t] = live ? p.lse[(b * p.H + h) * p.N + i] : -kNegInf;
         delta[t] = live ? p.delta[(b * p.H + h) * p.N + i] : 0.0f;
+        factor[t] = 1.0f;
+        if (kScaled<E>) {
+            factor[t] = scale_to(live ? 2.0f * most_v * p.norms[(b * p.H + h) * p.N + i] : 0.0f);
+            delta[t] *= factor[t];
+        }
         const S* q = (const S*)p.q.p + b * p.q.sb + (live ? i : 0) * p.q.sn + h * p.q.sh;
         const S* dy = (const S*)p.dy + ((b * p.N + (live ? i : 0)) * p.H + h) * p.D;
 #pragma unroll
@@ -242,7 +321,7 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnArgs p) {
                         }
                         if (p.slopes) x -= slope2 * fabsf(base - (float)(16 * n + i));
                         const float w = __builtin_amdgcn_exp2f(x);
-                        float ds = w * (dp[t][n][i] - delta[t]);
+                        float ds = w * (kScaled<E> ? dp[t][n][i] * factor[t] - delta[t] : dp[t][n][i] - delta[t]);
                         if (CAP) ds *= slope;                  // and 4 in the end
                         s[t][n][i] = ds;
                     }
@@ -310,7 +389,7 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnArgs p) {
             if (16 * d < p.D) {
                 typedef S S4 __attribute__((ext_vector_type(4)));
                 const int64_t at = row + 16 * d + 4 * g;
-                const f32x4 v = acc[t][d] * out_scale;
+                const f32x4 v = acc[t][d] * (out_scale / factor[t]);
                 if (parts > 1) *reinterpret_cast<f32x4*>(p.dq_parts + part_id * (p.B * p.N * p.H * p.D) + at) = v;
                 else *reinterpret_cast<S4*>((S*)p.dq + at) = __builtin_convertvector(v, S4);
             }
@@ -383,6 +462,12 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(AttnArgs p) {
     }
     const float scale2 = p.scale * kLog2e;
     const float cap2 = p.cap * kLog2e, to_tanh = CAP ? p.scale / p.cap : 0.0f, into_cap = 2.0f * kLog2e * to_tanh;
+    float factor = 1.0f;
+    if (kScaled<E>) {
+        factor = scale_to(2.0f * largest(p, b, 0, q_begin, q_end, mine) * largest(p, b, 1, 0, N, mine));
+        factor = __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, factor)));
+    }
+    const float to_ds = kUnshift * factor;              // of dP and delta beside a shifted weight
     f32x4 dk[KQ][DT], dv[KQ][DT];
 #pragma unroll
     for (int t = 0; t < KQ; ++t)
@@ -406,7 +491,7 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(AttnArgs p) {
             const bool live = q0 + tid < N;
             const int64_t at = (b * p.H + h) * p.N + q0 + tid;
             next_lse = live ? p.lse[at] - kShift - (CAP == kCap ? cap2 : 0.0f) : -kNegInf;
-            next_delta = live ? p.delta[at] * kUnshift : 0.0f;
+            next_delta = live ? p.delta[at] * to_ds : 0.0f;
             next_id = !live ? kNoQuery : p.ids ? p.ids[b * p.N + q0 + tid] : 0;
             next_id = next_id < 0 ? kNoQuery : next_id;
         }
@@ -487,7 +572,7 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(AttnArgs p) {
                             }
                             if (p.slopes) x -= slope2 * fabsf(base + (float)(16 * n + i));
                             const float w = __builtin_amdgcn_exp2f(x);
-                            float ds = w * (dp[t][n][i] * kUnshift - delta[i]);
+                            float ds = w * (dp[t][n][i] * to_ds - delta[i]);
                             if (CAP) ds *= slope;
                             s[t][n][i] = w;
                             dp[t][n][i] = ds;
@@ -568,7 +653,7 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(AttnArgs p) {
         for (int d = 0; d < DT; ++d) {
             if (16 * d < p.D) {
                 typedef S S4 __attribute__((ext_vector_type(4)));
-                const f32x4 k4 = dk[t][d] * (CAP ? 4.0f * p.scale : p.scale), v4 = dv[t][d] * kUnshift;
+                const f32x4 k4 = dk[t][d] * ((CAP ? 4.0f * p.scale : p.scale) / factor), v4 = dv[t][d] * kUnshift;
                 const int64_t at = row + 16 * d + 4 * g;
                 if (p.splits > 1) {
                     *reinterpret_cast<f32x4*>(p.parts + part * 2 * all + at) = k4;
@@ -644,12 +729,16 @@ static int backward_dp(const AttnArgs& p, hipStream_t stream) {
     return backward_cap<E, DP, kCapFine>(p, stream);
 }
 template <typename E>
-int backward_e(const AttnArgs& p, float* delta, hipStream_t stream) {
+int backward_e(const AttnArgs& p, float* delta, float* norms, float* ranges, hipStream_t stream) {
     int lanes = 2;
     while (lanes * (int)(16 / sizeof(E)) < p.D) lanes *= 2;
-    attn_delta_kernel<E><<<dim3((unsigned)ceil_div(p.B * p.N * p.H * lanes, 256)), 256, 0, stream>>>(p, lanes, delta);
-    const int rc = check_launch("attn_delta");
+    attn_delta_kernel<E><<<dim3((unsigned)ceil_div(p.B * p.N * p.H * lanes, 256)), 256, 0, stream>>>(p, lanes, delta, norms);
+    int rc = check_launch("attn_delta");
     if (rc != FLARE_OK) return rc;
+    if constexpr (kScaled<E>) {
+        attn_ranges_kernel<E><<<dim3((unsigned)ceil_div(p.N, kIdTile), (unsigned)p.B), 1024, 0, stream>>>(p, ranges);
+        if ((rc = check_launch("attn_ranges")) != FLARE_OK) return rc;
+    }
     return p.D <= 32   ? backward_dp<E, 32>(p, stream)
            : p.D <= 64 ? backward_dp<E, 64>(p, stream)
            : p.D <= 96 ? backward_dp<E, 96>(p, stream)

@@ -5,6 +5,6 @@
 namespace flare {
 namespace attn {
 template int forward_e<float>(const AttnArgs&, hipStream_t);
-template int backward_e<float>(const AttnArgs&, float*, hipStream_t);
+template int backward_e<float>(const AttnArgs&, float*, float*, float*, hipStream_t);
 }  // namespace attn
 }  // namespace flare

@@ -160,6 +160,38 @@ def test_large_caps_leave_small_scores_their_digits(dtype, cap, sloped):
     close_attention(y, (ref["y"][0][:, at - 40:], loose["y"][1][:, at - 40:]), "prompt", dtype)
 
 
+@pytest.mark.parametrize("std", [1e3, 1e-2, 1e-4, 1e-5])
+@pytest.mark.parametrize("N, H, G, D, what", [(1025, 4, 2, 64, ""), (300, 2, 1, 128, "cap"), (700, 2, 2, 48, "docs"),
+                                              (2100, 1, 1, 32, "")])
+def test_small_and_large_gradients_of_fp16(std, N, H, G, D, what):
+    """Score gradients of fp16 inputs keep their digits far below fp16's smallest numbers.  What rounding
+    one may cost absolutely is half a step of 2^-24 where the largest that dy and v allow (2 |dy|_1 max|v|,
+    a bound of |dP| + |delta|) lies at 2^14 or above: 2^-39 of that bound."""
+    g = gen(N)
+    q, k, v = (normal(g, 1, N, n, D, dtype=F16) for n in (H, G, G))
+    dy = normal(g, 1, N, H, D, std=std).to(F16)
+    o = {"softcap": 5.0} if what == "cap" else {}
+    groups = [slice(0, N)]
+    if what == "docs":
+        # documents of very different gradients, and padding that holds large numbers
+        ids = torch.zeros((1, N), dtype=torch.int32, device=DEV)
+        ids[:, 200:], ids[:, 500:] = 1, -1
+        groups, o["document_ids"] = [slice(0, 200), slice(200, 500)], ids
+        dy[:, 200:500] *= 2.0 ** -6
+        dy[:, 500:], v[:, 500:] = 6e4, 6e4
+    leaves = [t.clone().requires_grad_() for t in (q, k, v)]
+    grads = torch.autograd.grad(cf.softmax_attention(*leaves, **o), leaves, dy)
+    real = slice(0, groups[-1].stop)
+    bound = 2 * float(dy[:, real].double().abs().sum(-1).max()) * float(v[:, real].double().abs().max())
+    for s in groups:
+        part = [t[:, s] for t in (q, k, v)]
+        ref = attention(*part, softcap=o.get("softcap"), dy=dy[:, s], unit=U[F16], tiny=2.0 ** -39 * bound)
+        for n, got in zip(("dq", "dk"), grads):
+            close_attention(got[:, s], ref[n], n, F16)
+    if what == "docs":
+        assert all(not t[:, 500:].any() for t in grads)
+
+
 # ---------------------------------------------------------------------------------------
 # State space scan
 # ---------------------------------------------------------------------------------------
