@@ -142,13 +142,15 @@ static size_t dq_bytes(const AttnArgs& p) {
 // Parts that a row's keys are split into in the forward: two workgroups a CU (512) where the rows
 // leave less than that, in parts of 512 keys or more.  us, the joining included, with parts and
 // without: 64 new tokens behind 8000, 16 heads of 128 over 4, 34 and 274; 2 x 512 behind 3000 55 and 118.
-// One round of workgroups under a causal mask alone is as long as its last rows, and two parts even
-// that out: 4096 rows, 16 heads of 128 over 4, 127 and 151; with 6400 rows, or 2048 behind 2048, they
-// are slower (269 and 250, 172 and 163).
+// A round of workgroups under a causal mask alone is as long as its last rows, and two parts even that
+// out, up to five quarters of a round.  us without parts and with two, 16 heads of 128 over 4: 4096 rows
+// (512 workgroups) 151, 127; 4608 172, 154; 5120 (640) 193, 186; 5632 215, 219; 6400 251, 270.  16 heads of 64:
+// 4096 106, 78; 5120 136, 114; 6400 174, 169.  (4096 in documents of 700 tokens 57, 98; with a prefix of 2000
+// 155, 153; 2048 behind 2048 in a cache 163, 172.)
 static void split_forward(AttnArgs& p, int dtype) {
     const int64_t blocks = ceil_div(p.N, rows_of_queries(dtype)) * p.B * p.H, most = ceil_div(p.M, 512);
     int64_t want = ceil_div(512, blocks);
-    if (want < 2 && blocks <= 512 && p.causal && p.M == p.N) want = 2;
+    if (want < 2 && blocks <= 640 && p.causal && p.M == p.N && !p.ids && !p.prefix) want = 2;
     p.splits = want < most ? want : most;
 }
 static size_t forward_head_bytes(int64_t B, int64_t N) { return (stats_bytes(B, N) + 255) / 256 * 256; }

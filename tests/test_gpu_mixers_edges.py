@@ -192,6 +192,24 @@ def test_small_and_large_gradients_of_fp16(std, N, H, G, D, what):
         assert all(not t[:, 500:].any() for t in grads)
 
 
+@pytest.mark.parametrize("N", [2048, 2081, 2600])
+def test_attention_of_a_round_of_workgroups(N):
+    """Sizes at which rows of 16 heads take two parts, and above them: against 64 bits on the GPU.  A
+    score is a product over D (8 + D / 4 roundings of its terms' sizes), an exponential and the sums some
+    64 more, as in `attention` of _mixers.py."""
+    g = gen(N)
+    H, D = 16, 32
+    q, k, v = (normal(g, 1, N, H, D) for _ in range(3))
+    y = cf.softmax_attention(q, k, v)
+    see = torch.ones((N, N), dtype=torch.bool, device=DEV).tril()
+    for h in (0, 7, 15):
+        a, b, c = (t[0, :, h].double() for t in (q, k, v))
+        p = torch.softmax(torch.where(see, (a @ b.t()) * D ** -0.5, -INF), 1)
+        size = torch.where(see, (a.abs() @ b.abs().t()) * D ** -0.5, 0.0).amax(1, keepdim=True)
+        tol = E32 * (2 * (size * (8 + D / 4) + 16) + 64) * (p @ c.abs())
+        check(y[0, :, h], (p @ c).cpu(), (tol + E32 * (p @ c).abs()).cpu(), f"y of head {h}")
+
+
 # ---------------------------------------------------------------------------------------
 # State space scan
 # ---------------------------------------------------------------------------------------

@@ -30,3 +30,12 @@ def test_caps_out_of_range_are_refused(cap):
         rc = lib.flare_attn_forward(P, P, P, nine, 1, 1, 4, 4, 4, 4, 64, 1.0, cap, None, 1, None, None, None, None, P, None,
                                     None, None, 0, None)
         assert rc == -1 and b"cap" in lib.flare_last_error()
+
+
+def test_parts_of_a_causal_forward_come_for_a_range_of_sizes():
+    """Rows of 16 heads that are a round of 512 workgroups, and up to five quarters of one, run in two
+    parts: the workspace holds each part's sums."""
+    lib, H, D = _lib.lib(), 16, 128
+    parts = lambda N: lib.flare_attn_forward_workspace_size(1, N, N, H, D, 1) // (N * H * (D + 4) * 4)
+    assert [parts(N) for N in (4096, 4097, 4500, 5120)] == [2] * 4
+    assert parts(5121) == 0 and parts(20000) == 0
