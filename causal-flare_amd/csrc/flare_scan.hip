@@ -370,8 +370,8 @@ extern "C" int64_t flare_scan_kept_tokens(int64_t S) { return S < 1 || S > 64 ? 
 
 extern "C" size_t flare_scan_forward_workspace_size(int64_t B, int64_t N, int64_t C, int64_t S, int64_t G,
                                                     int64_t chunk) {
-    if (chunk < 1) return 0;
-    const int64_t SP = padded_states(S), NC = ceil_div(N, chunk);
+    if (chunk < 1 || N < 1) return 0;
+    const int64_t SP = padded_states(S), NC = ceil_div(N, chunk < N ? chunk : N);
     return (size_t)(B * N * G * 2 * SP + SP * C + B * NC * (C * (SP + 1) + 1)) * sizeof(float);
 }
 
@@ -390,7 +390,7 @@ extern "C" int flare_scan_forward(const void* x, const void* dt, const float* A,
                   "flare_scan_forward: chunks must be positive, and multiples of the kept states' distance");
     ScanArgs p = scan_args(x, dt, A, Bm, Cm, D, z, dt_bias, softplus, B, N, C, S, G, strides);
     const int64_t SP = padded_states(S);
-    p.L = chunk, p.NC = ceil_div(N, chunk);
+    p.L = chunk < N ? chunk : N, p.NC = ceil_div(N, p.L);
     if (workspace_bytes < flare_scan_forward_workspace_size(B, N, C, S, G, chunk)) {
         set_error("flare_scan_forward: workspace of %zu bytes is too small", workspace_bytes);
         return FLARE_ERR_WORKSPACE;

@@ -9,7 +9,7 @@ import causal_flare as cf
 from causal_flare import _lib
 from _mixers import U, attention, check, scan
 from test_gpu_mixers import (BF16, DEV, E32, F16, F32, close, close_attention, documents, gen, normal, scan_inputs,
-                             test_attention)
+                             test_attention, test_scan_prefill_and_decode as prefill_and_decode)
 
 pytestmark = pytest.mark.gpu
 INF, NAN = math.inf, math.nan
@@ -284,3 +284,11 @@ def test_scan_of_zero_states_and_gradients_under_any_growth(dtype, chunk, chunks
     close(y, ref["y"], "y", dtype, ref["k"])
     for n, got in zip(names, grads):
         close(got, ref["d" + n], "d" + n, F32 if n in "AD" else dtype, 2 * ref["k"] + C)
+
+
+@pytest.mark.parametrize("chunk, dtype, B, N, C, S, G", [
+    (13, F32, 3, 260, 40, 8, 1), (128, BF16, 3, 260, 40, 8, 1), (128, F16, 4, 300, 64, 20, 1), (64, F32, 3, 65, 16, 64, 1),
+    (1 << 32, BF16, 3, 65, 16, 16, 1), ((1 << 63) - 1, F16, 3, 65, 16, 16, 1)])
+def test_scan_prefill_in_other_chunks(chunk, dtype, B, N, C, S, G, chunks):
+    chunks(chunk)
+    prefill_and_decode(dtype, B, N, C, S, G)
