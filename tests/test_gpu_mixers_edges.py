@@ -9,7 +9,7 @@ import causal_flare as cf
 from causal_flare import _lib
 from _mixers import U, attention, check, scan
 from test_gpu_mixers import (BF16, DEV, E32, F16, F32, close, close_attention, documents, gen, normal, scan_inputs,
-                             test_attention, test_scan_prefill_and_decode as prefill_and_decode)
+                             test_attention, test_scan, test_scan_prefill_and_decode as prefill_and_decode)
 
 pytestmark = pytest.mark.gpu
 INF, NAN = math.inf, math.nan
@@ -284,6 +284,23 @@ def test_scan_of_zero_states_and_gradients_under_any_growth(dtype, chunk, chunks
     close(y, ref["y"], "y", dtype, ref["k"])
     for n, got in zip(names, grads):
         close(got, ref["d" + n], "d" + n, F32 if n in "AD" else dtype, 2 * ref["k"] + C)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("chunk, B, N, C, S, G, docs, more", [
+    (128, 2, 300, 70, 16, 1, True, True), (128, 1, 257, 48, 4, 1, False, False), (96, 1, 200, 130, 16, 2, False, True),
+    (64, 2, 131, 20, 33, 1, True, True), (128, 1, 260, 24, 64, 1, False, True), (128, 1, 250, 32, 24, 2, True, True),
+    (120, 1, 250, 32, 40, 1, True, True)])
+def test_scan_in_longer_chunks(chunk, dtype, B, N, C, S, G, docs, more, chunks):
+    """The chunks of large calls on small ones: several kept stretches a chunk, forward chunks of more than
+    8 tokens."""
+    chunks(chunk)
+    test_scan(dtype, B, N, C, S, G, docs, more)
+
+
+@pytest.mark.parametrize("dtype, B, N, C, S, G", [(F16, 4, 1, 16, 16, 1), (F16, 5, 33, 70, 16, 2), (F16, 4, 90, 64, 20, 1)])
+def test_scan_prefill_and_decode_of_fp16(dtype, B, N, C, S, G):
+    prefill_and_decode(dtype, B, N, C, S, G)
 
 
 @pytest.mark.parametrize("chunk, dtype, B, N, C, S, G", [
