@@ -81,6 +81,9 @@ def _check_cache(name, cache, lengths, Q, K, V, B, G, D):
     if not isinstance(cache, dict) or "k" not in cache or "v" not in cache:
         raise ValueError(f"{name} expects a cache {{'k', 'v'}} of [B, S, G, D]. Got {cache!r:.80}")
     k, v = cache["k"], cache["v"]
+    for what, t in (("cache['k']", k), ("cache['v']", v), ("lengths", lengths)):
+        if not isinstance(t, torch.Tensor):
+            raise ValueError(f"{name} expects a tensor in {what}. Got {t!r:.80}")
     if k.dim() != 4 or k.shape[1] < 1 or (k.shape[0], k.shape[2], k.shape[3]) != (B, G, D) or k.shape != v.shape:
         raise ValueError(f"{name} expects cache['k'] and cache['v'] [B, S, G, D] with B={B}, G={G}, D={D}. "
                          f"Got {tuple(k.shape)}, {tuple(v.shape)}")
@@ -243,7 +246,8 @@ def _step_fast(Q, K, V, cache, lengths, scale, softcap, slopes):
     B, H, D = Q.shape[0], Q.shape[-2], Q.shape[-1]
     dtype, device = Q.dtype, Q.device
     code = _CODES.get(dtype)
-    if (kc is None or vc is None or kc.dim() != 4 or K.dim() != Q.dim() or code is None or device.type != "cuda"
+    if (not isinstance(kc, torch.Tensor) or not isinstance(vc, torch.Tensor) or not isinstance(lengths, torch.Tensor)
+            or kc.dim() != 4 or K.dim() != Q.dim() or code is None or device.type != "cuda"
             or device.index != torch.cuda.current_device()):
         return None
     S, G = kc.shape[1], K.shape[-2]

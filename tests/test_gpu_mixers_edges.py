@@ -192,6 +192,13 @@ def test_small_and_large_gradients_of_fp16(std, N, H, G, D, what):
         assert all(not t[:, 500:].any() for t in grads)
 
 
+def test_lengths_that_are_no_tensor_are_refused():
+    qkv, cache = [normal(gen(0), 2, 1, 4, 32) for _ in range(3)], {n: normal(gen(1), 2, 9, 4, 32) for n in "kv"}
+    for call in (cf.softmax_attention_prefill, cf.softmax_attention_decode):
+        with pytest.raises(ValueError, match="expects a tensor in lengths"):
+            call(*qkv, cache, None)
+
+
 @pytest.mark.parametrize("N", [2048, 2081, 2600])
 def test_attention_of_a_round_of_workgroups(N):
     """Sizes at which rows of 16 heads take two parts, and above them: against 64 bits on the GPU.  A

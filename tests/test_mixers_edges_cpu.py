@@ -32,6 +32,16 @@ def test_caps_out_of_range_are_refused(cap):
         assert rc == -1 and b"cap" in lib.flare_last_error()
 
 
+@pytest.mark.parametrize("lengths", [None, [3, 4], 3])
+def test_lengths_that_are_no_tensor_are_refused(lengths):
+    qkv, cache = [t(2, 1, 4, 32)] * 3, {x: t(2, 9, 4, 32) for x in "kv"}
+    for call in (cf.softmax_attention_prefill, cf.softmax_attention_decode):
+        with pytest.raises(ValueError, match="expects a tensor in lengths"):
+            call(*qkv, cache, lengths)
+        with pytest.raises(ValueError, match=r"expects a tensor in cache\['v'\]"):
+            call(*qkv, {"k": cache["k"], "v": None}, ints(2))
+
+
 def test_parts_of_a_causal_forward_come_for_a_range_of_sizes():
     """Rows of 16 heads that are a round of 512 workgroups, and up to five quarters of one, run in two
     parts: the workspace holds each part's sums."""
