@@ -20,9 +20,10 @@ namespace flare {
 namespace attn {
 
 // With weights of 2^(s - cap) a row's largest is at least 2^(-2 cap): bf16 holds that, with all that
-// counts beside it, up to here (log2 units), and fp16 does not.  fp32 would, but s - cap rounds to fewer
-// digits than s has.
-constexpr float kCapFixedMost = 60.0f;
+// counts beside it, and fp16 does not.  Up to here (log2 units; caps of 30.5) it is 2^-88 or more, and its
+// products with values of 2^-49 keep 12 digits above fp32's smallest number.  (fp32 inputs would lose
+// digits: s - cap rounds to fewer than s has.)
+constexpr float kCapFixedMost = 44.0f;
 constexpr float kSlack = 8.0f;       // log2 of the largest weight before the reference moves
 
 template <typename E, int DP, int KT>

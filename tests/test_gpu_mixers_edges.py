@@ -132,6 +132,22 @@ def test_a_row_of_scores_that_are_all_minus_infinity_is_nan(dtype, N):
     assert y[0, 0, 0].isnan().all() and y[0, 0, 1].isfinite().all()
 
 
+@pytest.mark.parametrize("cap, std", [(30.0, 1e-12), (30.4, 1e-14), (41.0, 1e-9), (50.0, 1e-12)])
+def test_small_values_beside_scores_at_the_lower_end_of_a_cap(cap, std):
+    """Rows whose scores are all -cap: their weights are of any size until the sum divides them.  y is off
+    by the rounding of a weight and its own (bf16)."""
+    g = gen(1)
+    N, D = 200, 64
+    q = torch.full((1, N, 1, D), 4.0, dtype=BF16, device=DEV)
+    k = (torch.rand((1, N, 1, D), generator=g) * -100 - 100).to(BF16).to(DEV)
+    v = normal(g, 1, N, 1, D, dtype=BF16, std=std)
+    y = cf.softmax_attention(q, k, v, softcap=cap)
+    p = torch.ones((N, N), dtype=torch.float64).tril()
+    p /= p.sum(1, keepdim=True)
+    v = v[0, :, 0].double().cpu()
+    check(y[0, :, 0], p @ v, U[BF16] * (p @ v).abs() + 1.01 * U[BF16] * (p @ v.abs()), "y", BF16)
+
+
 @pytest.mark.parametrize("dtype", [F32, BF16, F16])
 @pytest.mark.parametrize("cap", [300.0, 1e4, 1e6, 1e8, 1e20])
 @pytest.mark.parametrize("sloped", [False, True])
