@@ -12,7 +12,7 @@
 // There four lanes share a channel (SL = S / 4 states each) and a wave has 16 channels: the
 // decays of a piece then take 2 T SL registers, where a lane with all the states of a channel
 // would need four times that.  What one lane would do alone for a token (the exponentials of the
-// gates, the loads and stores) lane q of a channel does for the tokens 4i + q, and the others read
+// gates, the loads and stores) lane q of a channel does for token q of a piece, and the others read
 // it through DPP.  dB and dC are summed over the wave's channels by halving: each step adds two
 // values and leaves one, half the lanes' worth of work at a time; the waves' sums meet in LDS and
 // the workgroups' in scan_dbc, always in the same order.
@@ -246,7 +246,7 @@ constexpr int kWaves = 4;              // 64 channels a workgroup
 template <int SP>
 struct GradLayout {
     static constexpr int SL = SP / 4;
-    static constexpr int T = 4;
+    static constexpr int T = 4;                          // a token for each lane of a channel
     static constexpr int keep = (int)kept_tokens(SP), pieces = keep / T;
     static constexpr int bc_floats = (int)kBackwardChunkMost * 2 * SP;
     static constexpr int keep_floats = kWaves * pieces * 64 * SL;
@@ -299,7 +299,11 @@ __device__ __forceinline__ void lds_row(const float* p, float (&out)[SL]) {
 template <typename E, int SP>
 __global__ __launch_bounds__(64 * kWaves) void scan_gradient_kernel(ScanArgs p) {
     using Lay = GradLayout<SP>;
-    constexpr int SL = Lay::SL, T = Lay::T, TQ = T / 4, KEEP = Lay::keep;
+    constexpr int SL = Lay::SL, T = Lay::T, KEEP = Lay::keep;
+    // Where a document begins r becomes 0, and a decay of 0 times an infinite r is NaN.  By a branch, or
+    // element by element where registers are short: us with either, 16 states (4 x 4096 x 2048) 532,
+    // 546; 32 (2 x 2048 x 2048) 258, 261; 64 (2 x 2048 x 1024) 370, 342.
+    constexpr bool SELECT = SP == 64;
     extern __shared__ __align__(16) float lds[];
     float* bcs = lds;                                      // [L][2][SP]
     float* keeps = bcs + Lay::bc_floats;                   // [waves][pieces][SL][64]
@@ -340,28 +344,25 @@ __global__ __launch_bounds__(64 * kWaves) void scan_gradient_kernel(ScanArgs p) 
     const float bias = p.dt_bias ? p.dt_bias[c] : 0.0f, skip = p.D ? p.D[c] : 0.0f;
     float dD = 0.0f, dbias = 0.0f;
 
-    // The tokens 4 i + q of the piece at k0, as loaded.
+    // Token q of the piece at k0, as loaded.
     struct Raw {
-        E dt[TQ], x[TQ], dy[TQ], z[TQ];
-        int id[TQ];
+        E dt, x, dy, z;
+        int id;
     };
     auto fetch = [&](Raw& r, int k0, bool all) {
-#pragma unroll
-        for (int i = 0; i < TQ; ++i) {
-            const int k = max(k0, 0) + 4 * i;
-            r.dt[i] = dts.load(q, k);
-            r.x[i] = xs.load(q, k);
-            if (all) r.dy[i] = dys.load(q, k);
-            if (all && z) r.z[i] = zs.load(q, k);
-            r.id[i] = ids ? ids[min(k + q, n - 1)] : 0;
-        }
+        const int k = max(k0, 0);
+        r.dt = dts.load(q, k);
+        r.x = xs.load(q, k);
+        if (all) r.dy = dys.load(q, k);
+        if (all && z) r.z = zs.load(q, k);
+        r.id = ids ? ids[min(k + q, n - 1)] : 0;
     };
     // a token that is none has delta = x = 0
-    auto step_of = [&](const Raw& r, int i, int k, float& raw, float& delta, float& xv) {
-        const bool live = active && k < n && r.id[i] >= 0;
-        raw = live ? to_f32(r.dt[i]) + bias : 0.0f;
+    auto step_of = [&](const Raw& r, int k, float& raw, float& delta, float& xv) {
+        const bool live = active && k < n && r.id >= 0;
+        raw = live ? to_f32(r.dt) + bias : 0.0f;
         delta = live ? (p.softplus ? mix::softplus(raw) : raw) : 0.0f;
-        xv = live ? to_f32(r.x[i]) : 0.0f;
+        xv = live ? to_f32(r.x) : 0.0f;
         return live;
     };
     auto piece_begins = [&](int k0) {      // bit j: a document begins at token k0 + j
@@ -371,13 +372,13 @@ __global__ __launch_bounds__(64 * kWaves) void scan_gradient_kernel(ScanArgs p) 
     };
     // h over the piece at k0; `take`(j, i, a, a h) sees each decay and what it leaves.  CUT: a
     // document begins in it.
-    auto forward = [&](auto cutc, int k0, unsigned starts, const float (&delta)[TQ], const float (&du)[TQ], auto&& take) {
+    auto forward = [&](auto cutc, int k0, unsigned starts, float delta, float du, auto&& take) {
         constexpr bool CUT = decltype(cutc)::value;
         auto token = [&](auto jc) {
             constexpr int j = decltype(jc)::value;
             float B[SL];
             lds_row<SL>(bcs + (k0 + j) * 2 * SP + q * SL, B);
-            const float dj = quad_bcast<(j & 3)>(delta[j / 4]), uj = quad_bcast<(j & 3)>(du[j / 4]);
+            const float dj = quad_bcast<j>(delta), uj = quad_bcast<j>(du);
             const bool cut = CUT && (starts >> j & 1);
 #pragma unroll
             for (int i = 0; i < SL; ++i) {
@@ -407,17 +408,12 @@ __global__ __launch_bounds__(64 * kWaves) void scan_gradient_kernel(ScanArgs p) 
         for (int piece = 0; piece + 1 < Lay::pieces; ++piece) {
             if (piece + 1 >= pieces) break;
             const int k0 = first + piece * T;
-            float delta[TQ], du[TQ];
-#pragma unroll
-            for (int i = 0; i < TQ; ++i) {
-                float raw, xv;
-                step_of(raws[piece], i, k0 + 4 * i + q, raw, delta[i], xv);
-                du[i] = delta[i] * xv;
-            }
+            float raw, delta, xv;
+            step_of(raws[piece], k0 + q, raw, delta, xv);
             const unsigned starts = piece_begins(k0);
             auto nothing = [](auto, int, float, float) {};
-            if (starts) forward(std::true_type{}, k0, starts, delta, du, nothing);
-            else forward(std::false_type{}, k0, 0u, delta, du, nothing);
+            if (starts) forward(std::true_type{}, k0, starts, delta, delta * xv, nothing);
+            else forward(std::false_type{}, k0, 0u, delta, delta * xv, nothing);
 #pragma unroll
             for (int i = 0; i < SL; ++i) keep[((piece + 1) * SL + i) * 64] = h[i];
         }
@@ -427,17 +423,10 @@ __global__ __launch_bounds__(64 * kWaves) void scan_gradient_kernel(ScanArgs p) 
             const int k0 = first + piece * T;
             const Raw now = next;
             fetch(next, k0 - T, true);
-            float raw[TQ], delta[TQ], xv[TQ], du[TQ], gy[TQ], dyv[TQ], zv[TQ], gate[TQ];
-            bool live[TQ];
-#pragma unroll
-            for (int i = 0; i < TQ; ++i) {
-                live[i] = step_of(now, i, k0 + 4 * i + q, raw[i], delta[i], xv[i]);
-                du[i] = delta[i] * xv[i];
-                dyv[i] = live[i] ? to_f32(now.dy[i]) : 0.0f;
-                zv[i] = live[i] && z ? to_f32(now.z[i]) : 0.0f;
-                gate[i] = z ? mix::sigmoid(zv[i]) : 1.0f;
-                gy[i] = z ? dyv[i] * zv[i] * gate[i] : dyv[i];
-            }
+            float raw, delta, xv;
+            const bool live = step_of(now, k0 + q, raw, delta, xv);
+            const float du = delta * xv, dyv = live ? to_f32(now.dy) : 0.0f, zv = live && z ? to_f32(now.z) : 0.0f;
+            const float gate = z ? mix::sigmoid(zv) : 1.0f, gy = z ? dyv * zv * gate : dyv;
             float a[T][SL], ah[T][SL];
 #pragma unroll
             for (int i = 0; i < SL; ++i) h[i] = keep[(piece * SL + i) * 64];
@@ -448,31 +437,30 @@ __global__ __launch_bounds__(64 * kWaves) void scan_gradient_kernel(ScanArgs p) 
             };
             if (starts) forward(std::true_type{}, k0, starts, delta, du, hold);
             else forward(std::false_type{}, k0, 0u, delta, du, hold);
-            // the tokens in reverse, and after each four of them what their lanes do with the sums
-            float pA[4], sB[4], lin[4];
+            // the tokens in reverse, and then what their lanes do with the sums
+            float pA[T], sB[T], lin[T];
             auto back = [&](auto jc) {
-                constexpr int j = T - 1 - decltype(jc)::value, jq = j & 3;
+                constexpr int j = T - 1 - decltype(jc)::value;
                 const float* row = bcs + (k0 + j) * 2 * SP + q * SL;
-                const float dj = quad_bcast<jq>(delta[j / 4]), uj = quad_bcast<jq>(du[j / 4]);
-                const float gj = quad_bcast<jq>(gy[j / 4]);
+                const float dj = quad_bcast<j>(delta), uj = quad_bcast<j>(du), gj = quad_bcast<j>(gy);
                 float v[2 * SL], B[SL], Cv[SL];
                 lds_row<SL>(row, B);
                 lds_row<SL>(row + SP, Cv);
-                pA[jq] = sB[jq] = lin[jq] = 0.0f;
+                pA[j] = sB[j] = lin[j] = 0.0f;
 #pragma unroll
                 for (int i = 0; i < SL; ++i) {
                     const float hv = ah[j][i] + uj * B[i];
                     r[i] += Cv[i] * gj;
                     const float w = r[i] * ah[j][i];
-                    pA[jq] += w * A2[i];
+                    pA[j] += w * A2[i];
                     dA[i] += w * dj;
-                    sB[jq] += r[i] * B[i];
-                    lin[jq] += Cv[i] * hv;
+                    sB[j] += r[i] * B[i];
+                    lin[j] += Cv[i] * hv;
                     v[i] = r[i] * uj;
                     v[SL + i] = gj * hv;
-                    r[i] *= a[j][i];
+                    r[i] = SELECT && (starts >> j & 1) ? 0.0f : r[i] * a[j][i];
                 }
-                if (__builtin_expect(starts >> j & 1, 0)) {      // a decay of 0 times an infinite r is NaN
+                if (!SELECT && __builtin_expect(starts >> j & 1, 0)) {
 #pragma unroll
                     for (int i = 0; i < SL; ++i) r[i] = 0.0f;
                 }
@@ -488,19 +476,18 @@ __global__ __launch_bounds__(64 * kWaves) void scan_gradient_kernel(ScanArgs p) 
                         out[idx < SL ? idx : SP + idx - SL] = v[m];
                     }
                 }
-                if constexpr (jq == 0) {
-                    constexpr int i = j / 4;
+                if constexpr (j == 0) {
                     const float pq = quad_gather(pA, q) * kLn2, sq = quad_gather(sB, q), lq = quad_gather(lin, q);
-                    float ddt = pq + xv[i] * sq;
-                    if (p.softplus) ddt *= mix::sigmoid(raw[i]);
-                    if (!live[i]) ddt = 0.0f;
+                    float ddt = pq + xv * sq;
+                    if (p.softplus) ddt *= mix::sigmoid(raw);
+                    if (!live) ddt = 0.0f;
                     dbias += ddt;
-                    dD += gy[i] * xv[i];
-                    dxs.store(q, k0 + 4 * i, live[i] ? delta[i] * sq + gy[i] * skip : 0.0f);
-                    ddts.store(q, k0 + 4 * i, ddt);
+                    dD += gy * xv;
+                    dxs.store(q, k0, live ? delta * sq + gy * skip : 0.0f);
+                    ddts.store(q, k0, ddt);
                     if (z) {
-                        const float dz = dyv[i] * (lq + skip * xv[i]) * gate[i] * (1.0f + zv[i] * (1.0f - gate[i]));
-                        dzs.store(q, k0 + 4 * i, live[i] ? dz : 0.0f);
+                        const float dz = dyv * (lq + skip * xv) * gate * (1.0f + zv * (1.0f - gate));
+                        dzs.store(q, k0, live ? dz : 0.0f);
                     }
                 }
             };
