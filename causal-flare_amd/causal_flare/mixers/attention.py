@@ -9,9 +9,11 @@ same document id, not negative.  A query that sees nothing gives y = 0.
 Layouts: Q [B, N, H, D], K and V [B, N, G, D] with H a multiple of G (head h reads key head
 h // (H / G)), D a multiple of 16 up to 128.  Q, K and V may be slices of wider tensors: rows of
 D adjacent elements on 16-byte boundaries are read in place, anything else is copied.  They may
-be float32, bfloat16 or float16 (one type: their promotion).  Scores, maxima, sums and outputs
-are kept in float32; 16-bit inputs have their weights (and in the backward the scores'
-gradients) rounded to their type for the products with V, K and Q.
+be float32, bfloat16 or float16 (one type: their promotion; float64 is computed in float32).  Scores,
+maxima and sums are kept in float32; 16-bit inputs have their weights rounded to their type for the
+products with V and dY, and the scores' gradients in two parts for those with K and Q.  A call that is
+to be differentiated keeps Q, K, V, y, a float32 a row of a head and, of 16-bit inputs, what y was
+rounded by (as large as y) until its backward.
 
 A cache is ``{"k": [B, S, G, D], "v": [B, S, G, D]}``, room for S tokens a sequence; how many each
 holds is the caller's to keep, in `lengths`.
@@ -168,10 +170,10 @@ def softmax_attention(
 ):
     """Softmax attention of whole sequences, differentiable in Q, K and V.
 
-    scale: D**-0.5 by default.  softcap: between 2^-100 and 2^100.  slopes: [H], the bias on distance (constants, no gradient).
-    document_ids: integers [B, N]; queries see keys of their own id only, and a negative id is
-    padding, with y = 0 and no gradient.  prefix_lengths: integers [B]; the first so many keys of
-    a sequence are seen by all its queries (of the same document).
+    scale: D**-0.5 by default.  softcap: between 2^-100 and 2^100.  slopes: [H], the bias on distance
+    (constants, no gradient).  document_ids: integers [B, N]; queries see keys of their own id only,
+    and a negative id is padding, with y = 0 and no gradient.  prefix_lengths: integers [B]; the
+    first so many keys of a sequence are seen by all its queries (of the same document).
     """
     name = "softmax_attention"
     B, N, H, G, D = _check_heads(name, Q, K, V)

@@ -4,8 +4,8 @@
 
 Layouts: x [B, N, C], weight [C, W] (W of 2, 3 or 4; the last column meets the token itself),
 bias [C], y [B, N, C].  x may be a slice of a wider tensor: its last dimension has to be
-adjacent in memory, and anything else is copied.  x may be float32, bfloat16 or float16; weight
-and bias are used in float32 and sums are kept in float32.
+adjacent in memory, and anything else is copied.  x may be float32, bfloat16 or float16 (float64 is
+computed in float32); weight and bias are used in float32 and sums are kept in float32.
 
 A cache is ``{"window": [B, W - 1, C]}``, the last inputs in x's type, oldest first.
 """

@@ -7,7 +7,8 @@
 Layouts: x, dt, z [B, N, C]; A [C, S] (1 to 64 states a channel); B, C [B, N, S], or [B, N, G, S]
 where channel c reads group c // (C / G); D, dt_bias [C].  x, dt, z, B and C may be slices of
 wider tensors: the last dimension has to be adjacent in memory, and anything else is copied.
-They may be float32, bfloat16 or float16 (one type: their promotion); A, D and dt_bias are used
+They may be float32, bfloat16 or float16 (one type: their promotion; float64 is computed in
+float32); A, D and dt_bias are used
 in float32, and so are states, decays and sums.
 
 A cache is ``{"h": [B, C, S]}`` in float32.

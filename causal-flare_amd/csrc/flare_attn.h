@@ -101,7 +101,10 @@ __device__ __forceinline__ void put_y(const AttnArgs& p, int64_t at, f32x4 o) {
     typedef S S4 __attribute__((ext_vector_type(4)));
     const S4 y = __builtin_convertvector(o, S4);
     *reinterpret_cast<S4*>((S*)p.y + at) = y;
-    if (p.y_rest) *reinterpret_cast<S4*>((S*)p.y_rest + at) = __builtin_convertvector(o - __builtin_convertvector(y, f32x4), S4);
+    if (p.y_rest) {
+        const f32x4 rest = o - __builtin_convertvector(y, f32x4);
+        *reinterpret_cast<S4*>((S*)p.y_rest + at) = __builtin_convertvector(rest, S4);
+    }
 }
 
 // Ids as the kernels compare them: padding's negative ones are those of no key and of no query.

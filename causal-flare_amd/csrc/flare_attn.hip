@@ -29,7 +29,8 @@ __global__ __launch_bounds__(64) void attn_ids_kernel(const int32_t* ids, int64_
 
 // What each block of `rows` queries (blockIdx.y 0) or `key_rows` keys (1) costs: the tiles of ids it
 // meets.  A wave a block.
-__global__ __launch_bounds__(64) void attn_costs_kernel(AttnArgs p, int rows, int key_rows, int32_t* costs, int32_t* key_costs) {
+__global__ __launch_bounds__(64) void attn_costs_kernel(AttnArgs p, int rows, int key_rows, int32_t* costs,
+                                                        int32_t* key_costs) {
     const bool keys = blockIdx.y != 0;
     const int n = keys ? key_rows : rows, tiles = ((int)p.N + n - 1) / n;
     if ((int64_t)blockIdx.x >= p.B * tiles) return;
@@ -48,8 +49,8 @@ __global__ __launch_bounds__(64) void attn_costs_kernel(AttnArgs p, int rows, in
 constexpr int kMostOrdered = 2048;
 
 // Blocks in falling order of cost, those of one cost as they stand.
-__global__ __launch_bounds__(1024) void attn_order_kernel(const int32_t* costs, int n, int32_t* order, const int32_t* key_costs,
-                                                          int key_n, int32_t* key_order) {
+__global__ __launch_bounds__(1024) void attn_order_kernel(const int32_t* costs, int n, int32_t* order,
+                                                          const int32_t* key_costs, int key_n, int32_t* key_order) {
     __shared__ int c[kMostOrdered];
     if (blockIdx.x) costs = key_costs, n = key_n, order = key_order;
     for (int i = threadIdx.x; i < n; i += 1024) c[i] = costs[i];
@@ -91,7 +92,7 @@ static size_t stats_bytes(int64_t B, int64_t N) {
 // Documents make blocks cost very different amounts of work, so that the costly ones have to start
 // first; that takes two small launches (some 10 us), and pays where there are more workgroups
 // than run at once (512).  16384 tokens in six documents, 16 heads of 128 over 4, us in the rows'
-// order and in this: forward 580, 523; dq 704, 639; dk and dv 1356, 1164.
+// order and in this: forward 598, 555; dq 749, 693; dk and dv 1121, 1049.
 static int launch_ids(AttnArgs& p, int dtype, bool keys, int32_t* stats, hipStream_t stream) {
     if (!p.ids) return FLARE_OK;
     const int tiles = (int)ceil_div(p.N, kIdTile);
@@ -105,8 +106,8 @@ static int launch_ids(AttnArgs& p, int dtype, bool keys, int32_t* stats, hipStre
     attn_costs_kernel<<<dim3((unsigned)(n > key_n ? n : key_n), keys ? 2 : 1), 64, 0, stream>>>(p, rows, key_rows, at,
                                                                                              at + kMostOrdered);
     if ((rc = check_launch("attn_costs")) != FLARE_OK) return rc;
-    attn_order_kernel<<<dim3(keys ? 2 : 1), 1024, 0, stream>>>(at, (int)n, at + 2 * kMostOrdered, at + kMostOrdered, (int)key_n,
-                                                               at + 3 * kMostOrdered);
+    attn_order_kernel<<<dim3(keys ? 2 : 1), 1024, 0, stream>>>(at, (int)n, at + 2 * kMostOrdered, at + kMostOrdered,
+                                                               (int)key_n, at + 3 * kMostOrdered);
     p.order = at + 2 * kMostOrdered;
     p.key_order = keys ? at + 3 * kMostOrdered : nullptr;
     return check_launch("attn_order");
@@ -186,7 +187,7 @@ using namespace flare::attn;
     FLARE_REQUIRE(D >= 16 && D <= 128 && D % 16 == 0, name ": head dimension %lld is not a multiple of 16 up to " \
                   "128", (long long)D);                                                                           \
     FLARE_REQUIRE(N <= (1 << 30) && M <= (1 << 30) && B <= 65535 && H <= 65535 && B * H <= (1 << 24) &&           \
-                  (N + 63) / 64 * B * H <= (1 << 26) && H * D < kMostStride, name ": too large");                                        \
+                  (N + 63) / 64 * B * H <= (1 << 26) && H * D < kMostStride, name ": too large");            \
     FLARE_REQUIRE(softcap == 0.0f || (softcap >= kLeastCap && softcap <= kMostCap),                                \
                   name ": the cap must be 0 (none) or between 2^-100 and 2^100")
 
@@ -211,14 +212,16 @@ extern "C" int flare_attn_forward(const void* q, const void* k, const void* v, c
                                   int64_t B, int64_t N, int64_t M, int64_t H, int64_t G, int64_t D, float scale,
                                   float softcap, const float* slopes, int causal, const int32_t* document_ids,
                                   const int32_t* prefix_lengths, const int32_t* lengths, const int32_t* new_lengths,
-                                  void* y, void* y_rest, float* lse, void* workspace, size_t workspace_bytes, void* stream) {
+                                  void* y, void* y_rest, float* lse, void* workspace, size_t workspace_bytes,
+                                  void* stream) {
     FLARE_REQUIRE(q && k && v && strides && y, "flare_attn_forward: null pointer");
     ATTN_REQUIRE_SIZES("flare_attn_forward");
     FLARE_REQUIRE(lengths || M == N, "flare_attn_forward: as many keys as queries without a cache");
     FLARE_REQUIRE(!(document_ids && lengths), "flare_attn_forward: document_ids exclude a cache");
     FLARE_REQUIRE(lengths || !new_lengths, "flare_attn_forward: new_lengths without lengths");
     AttnArgs p = attn_args(q, k, v, strides, B, N, M, H, G, D, scale, softcap, slopes);
-    FLARE_REQUIRE(aligned(p.q, dtype) && aligned(p.k, dtype) && aligned(p.v, dtype) && (((uintptr_t)y | (uintptr_t)y_rest) & 15) == 0,
+    const uintptr_t out = (uintptr_t)y | (uintptr_t)y_rest;
+    FLARE_REQUIRE(aligned(p.q, dtype) && aligned(p.k, dtype) && aligned(p.v, dtype) && (out & 15) == 0,
                   "flare_attn_forward: rows must be 16-byte aligned and less than 2^22 elements apart");
     p.causal = causal, p.ids = document_ids, p.prefix = prefix_lengths, p.lengths = lengths, p.fresh = new_lengths;
     p.y = y, p.y_rest = y_rest, p.lse = lse;
@@ -235,7 +238,9 @@ extern "C" int flare_attn_forward(const void* q, const void* k, const void* v, c
 
 // delta, fp16's norms and ranges, and the id statistics.
 static int64_t norms_floats(int64_t B, int64_t N, int64_t H, int dtype) { return dtype == FLARE_F16 ? B * H * N : 0; }
-static int64_t ranges_floats(int64_t B, int64_t N, int dtype) { return dtype == FLARE_F16 ? B * ceil_div(N, kIdTile) * 2 : 0; }
+static int64_t ranges_floats(int64_t B, int64_t N, int dtype) {
+    return dtype == FLARE_F16 ? B * ceil_div(N, kIdTile) * 2 : 0;
+}
 static size_t backward_head_bytes(int64_t B, int64_t N, int64_t H, int dtype) {
     const int64_t floats = B * H * N + norms_floats(B, N, H, dtype) + ranges_floats(B, N, dtype);
     return ((size_t)floats * sizeof(float) + stats_bytes(B, N) + 255) / 256 * 256;
@@ -262,7 +267,8 @@ extern "C" int flare_attn_backward(const void* q, const void* k, const void* v, 
     AttnArgs p = attn_args(q, k, v, strides, B, N, M, H, G, D, scale, softcap, slopes);
     const uintptr_t out = (uintptr_t)y | (uintptr_t)y_rest | (uintptr_t)dy | (uintptr_t)dq | (uintptr_t)dk | (uintptr_t)dv;
     FLARE_REQUIRE(aligned(p.q, dtype) && aligned(p.k, dtype) && aligned(p.v, dtype) && (out & 15) == 0 &&
-                  ((uintptr_t)workspace & 15) == 0, "flare_attn_backward: rows must be 16-byte aligned and less than 2^22 elements apart");
+                  ((uintptr_t)workspace & 15) == 0,
+                  "flare_attn_backward: rows must be 16-byte aligned and less than 2^22 elements apart");
     if (workspace_bytes < flare_attn_backward_workspace_size(B, N, H, G, D, dtype)) {
         set_error("flare_attn_backward: workspace of %zu bytes is too small", workspace_bytes);
         return FLARE_ERR_WORKSPACE;
@@ -272,7 +278,8 @@ extern "C" int flare_attn_backward(const void* q, const void* k, const void* v, 
     float* ranges = norms + norms_floats(B, N, H, dtype);
     int32_t* stats = (int32_t*)(ranges + ranges_floats(B, N, dtype));
     p.causal = causal, p.ids = document_ids, p.prefix = prefix_lengths;
-    p.y = const_cast<void*>(y), p.y_rest = const_cast<void*>(y_rest), p.lse = const_cast<float*>(lse), p.dy = dy, p.delta = delta, p.norms = norms, p.ranges = ranges;
+    p.y = const_cast<void*>(y), p.y_rest = const_cast<void*>(y_rest), p.lse = const_cast<float*>(lse), p.dy = dy;
+    p.delta = delta, p.norms = norms, p.ranges = ranges;
     p.dq = dq, p.dk = dk, p.dv = dv;
     split_backward(p, dtype);
     p.parts = (float*)((char*)workspace + backward_head_bytes(B, N, H, dtype));
@@ -319,10 +326,12 @@ extern "C" int flare_attn_step(const void* q, const void* k, const void* v, cons
     p.v_new = v, p.vn_sb = strides[4], p.vn_sg = strides[5];
     const Rows kr = {k, strides[2], 0, strides[3]}, vr = {v, strides[4], 0, strides[5]};
     FLARE_REQUIRE(aligned(p.q, dtype) && aligned(kr, dtype) && aligned(vr, dtype) && aligned(p.k, dtype) &&
-                  aligned(p.v, dtype) && ((uintptr_t)y & 15) == 0, "flare_attn_step: rows must be 16-byte aligned and less than 2^22 elements apart");
+                  aligned(p.v, dtype) && ((uintptr_t)y & 15) == 0,
+                  "flare_attn_step: rows must be 16-byte aligned and less than 2^22 elements apart");
     FLARE_REQUIRE(B * G * ceil_div(H / G, 16) <= 65535, "flare_attn_step: too large");
     p.splits = step_splits(B, M, H, G);
-    if (workspace_bytes < flare_attn_step_workspace_size(B, M, H, G, D) || (p.splits > 1 && (!workspace || ((uintptr_t)workspace & 15)))) {
+    if (workspace_bytes < flare_attn_step_workspace_size(B, M, H, G, D) ||
+        (p.splits > 1 && (!workspace || ((uintptr_t)workspace & 15)))) {
         set_error("flare_attn_step: workspace of %zu bytes is too small or not 16-byte aligned", workspace_bytes);
         return FLARE_ERR_WORKSPACE;
     }

@@ -14,10 +14,10 @@
 // 1.9e-3 with both, for 8% of the step.
 //
 // Tiles of 64 rows (32 in fp32), taken 32 at a time: a tile of 32 rows in LDS, with a barrier for
-// each, took 1270 us for dk and dv of 16384 rows in six documents (16 heads of 128 over 4, bf16) and
-// 723 for dq, where these take 1055 and 624.  Of 16384 causal rows of one document dq takes 1909 us:
-// 3 + 1 products at 1.15 PFLOP/s; dk and dv 3194 us, 4 + 1 products at 0.86 (a large matrix product:
-// 1.34); with capped scores (4 x 4096 rows, 16 heads of 64) 444 and 574 us, vector instructions.
+// each, took 20% longer for dk and dv and 16% for dq (16384 rows in six documents, 16 heads of 128 over
+// 4, bf16).  Of 16384 causal rows of one document dq takes 1990 us: 3 + 1 products at 1.1 PFLOP/s; dk and
+// dv 3120 us, 4 + 1 products at 0.88 (a large matrix product: 1.34); with capped scores (4 x 4096 rows, 16
+// heads of 64) 444 and 577 us, vector instructions.
 //
 // What a wave owns, us: 32 queries against 16 (D = 64, dq) 476, 526; 32 keys against 16 at D = 64
 // (dk and dv) 604, 633; at D = 128 32 keys leave room for one wave a SIMD: 3405, 2439.
@@ -271,7 +271,8 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnArgs p) {
     while (tile < kv_end) {
         const int k1 = walk.next(tile + KT);
         if (k1 < kv_end) fetch(k1);
-        const int odd = __builtin_amdgcn_readfirstlane(oddl[buf * 4] | oddl[buf * 4 + 1] | oddl[buf * 4 + 2] | oddl[buf * 4 + 3]);
+        const int4 odds = *reinterpret_cast<const int4*>(oddl + buf * 4);
+        const int odd = __builtin_amdgcn_readfirstlane(odds.x | odds.y | odds.z | odds.w);
         any_odd |= odd;
 #pragma unroll 1
         for (int part = 0; part < KT; part += 32) {
@@ -371,9 +372,10 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnArgs p) {
                     if (j >= lim[t] || (p.ids && max(p.ids[b * p.N + j], kNoKey) != qid[t])) continue;
 #pragma unroll
                     for (int d = 0; d < DT; ++d) {
+                        const S* k = kbase + j * p.k.sn + 16 * d + 4 * g;
 #pragma unroll
                         for (int e = 0; e < 4; ++e)
-                            if (16 * d < p.D && is_odd((float)kbase[j * p.k.sn + 16 * d + 4 * g + e])) acc[t][d][e] = __builtin_nanf("");
+                            if (16 * d < p.D && is_odd((float)k[e])) acc[t][d][e] = __builtin_nanf("");
                     }
                 }
             }
@@ -521,7 +523,8 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(AttnArgs p) {
         while (tile < q_end) {
             const int q1 = walk.next(tile + QR);
             if (q1 < q_end) fetch(h, q1);
-            const int odd = __builtin_amdgcn_readfirstlane(oddl[buf * 4] | oddl[buf * 4 + 1] | oddl[buf * 4 + 2] | oddl[buf * 4 + 3]);
+            const int4 odds = *reinterpret_cast<const int4*>(oddl + buf * 4);
+            const int odd = __builtin_amdgcn_readfirstlane(odds.x | odds.y | odds.z | odds.w);
             any_odd |= odd;
 #pragma unroll 1
             for (int from_row = 0; from_row < QR; from_row += 32) {
@@ -674,7 +677,7 @@ __global__ __launch_bounds__(256) void attn_parts_kernel(AttnArgs p) {
     typedef S S4 __attribute__((ext_vector_type(4)));
     constexpr int U = 4;
     const int what = blockIdx.y;
-    const int64_t rows = p.B * p.N * p.D, all = rows * (what ? p.G : p.H), at = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
+    const int64_t all = p.B * p.N * p.D * (what ? p.G : p.H), at = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
     const int splits = (int)(what ? p.splits : p.dq_splits);
     if (at >= all || splits == 1) return;
     const int64_t stride = what ? 2 * all : all;
@@ -732,7 +735,8 @@ template <typename E>
 int backward_e(const AttnArgs& p, float* delta, float* norms, float* ranges, hipStream_t stream) {
     int lanes = 2;
     while (lanes * (int)(16 / sizeof(E)) < p.D) lanes *= 2;
-    attn_delta_kernel<E><<<dim3((unsigned)ceil_div(p.B * p.N * p.H * lanes, 256)), 256, 0, stream>>>(p, lanes, delta, norms);
+    const int64_t threads = p.B * p.N * p.H * lanes;
+    attn_delta_kernel<E><<<dim3((unsigned)ceil_div(threads, 256)), 256, 0, stream>>>(p, lanes, delta, norms);
     int rc = check_launch("attn_delta");
     if (rc != FLARE_OK) return rc;
     if constexpr (kScaled<E>) {

@@ -278,7 +278,8 @@ struct TokenValues {
     }
     __device__ __forceinline__ void store(int lane_token, int k, float x) const {
         const unsigned o = at + lane_token * step + k * step;
-        if constexpr (sizeof(E) == 2) __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(unsigned short, from_f32<E>(x)), r, o, 0, 0);
+        if constexpr (sizeof(E) == 2)
+            __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(unsigned short, from_f32<E>(x)), r, o, 0, 0);
         else __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(unsigned, x), r, o, 0, 0);
     }
 };
@@ -619,7 +620,8 @@ extern "C" int flare_scan_backward(const void* x, const void* dt, const float* A
     ScanArgs p = scan_args(x, dt, A, Bm, Cm, D, z, dt_bias, softplus, B, N, C, S, G, strides);
     p.L = chunk, p.NC = ceil_div(N, chunk);
     for (int i = 1; i < 6; i += 2)
-        FLARE_REQUIRE(strides[i] >= 0 && strides[i] < kMostStride, "flare_scan_backward: tokens must be less than 2^22 elements apart");
+        FLARE_REQUIRE(strides[i] >= 0 && strides[i] < kMostStride,
+                      "flare_scan_backward: tokens must be less than 2^22 elements apart");
     const BackwardLayout lay(B, N, C, S, G, p.NC);
     if (workspace_bytes < lay.total * sizeof(float)) {
         set_error("flare_scan_backward: workspace of %zu bytes is too small", workspace_bytes);
@@ -628,8 +630,8 @@ extern "C" int flare_scan_backward(const void* x, const void* dt, const float* A
     float* ws = (float*)workspace;
     p.ids = document_ids, p.dy = dy, p.kept = const_cast<float*>(kept), p.keep = kept_tokens(SP);
     p.dx = dx, p.ddt = ddt, p.dB = dB, p.dC = dC, p.dz = dz;
-    p.bc = ws + lay.bc, p.A2 = ws + lay.A2, p.carry = ws + lay.carry, p.dsum = ws + lay.dsum, p.cuts = (int32_t*)(ws + lay.cuts);
-    p.dbc = ws + lay.dbc, p.dpar = ws + lay.dpar;
+    p.bc = ws + lay.bc, p.A2 = ws + lay.A2, p.carry = ws + lay.carry, p.dsum = ws + lay.dsum;
+    p.cuts = (int32_t*)(ws + lay.cuts), p.dbc = ws + lay.dbc, p.dpar = ws + lay.dpar;
     hipStream_t st = (hipStream_t)stream;
     int rc = launch_pack(p, dtype, SP, st);
     if (rc == FLARE_OK) rc = FLARE_BY_DTYPE(dtype, backward_e, (p, SP, st));

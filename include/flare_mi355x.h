@@ -388,16 +388,16 @@ int flare_scan_step(const void* x, const void* dt, const float* A, const void* B
 
 /*
  * y_i = sum_j softmax_j(s_ij) v_j, s_ij = x_ij - slopes[h] |i - j|, x_ij = scale q_i . k_j or (softcap
- * > 0, from 2^-100 to 2^100) softcap tanh(scale q_i . k_j / softcap).  q [B, N, H, D], k and v [B, M, G, D], head h reads
- * key head h / (H / G); D a multiple of 16 up to 128; every row on a 16-byte boundary.  strides:
+ * not 0, from 2^-100 to 2^100) softcap tanh(scale q_i . k_j / softcap).  q [B, N, H, D], k and v
+ * [B, M, G, D], head h reads key head h / (H / G); D a multiple of 16 up to 128; every row on a
+ * 16-byte boundary.  strides:
  * batch, token and head of q, k, v (9 numbers, host).  causal: query i sees keys j <= i, and
  * those below prefix_lengths[b] (or NULL).  Without `lengths` M == N.  With them k and v are
  * caches of M rows, the queries are at positions lengths[b] + i, and new_lengths[b] of them (all
  * if NULL) are real, whose keys are in the caches already (flare_attn_append); lengths[b] < 0: y =
  * 0; lengths[b] + new_lengths[b] > M: y is NaN.  document_ids exclude lengths.
- * A query that sees nothing has y = 0.  y_rest [B,
- * N, H, D] or NULL receives what y was rounded by (16-bit types; for the backward).  lse [B, H, N] or NULL receives log2 of the sum
- * of exp(s_ij).
+ * A query that sees nothing has y = 0.  y_rest [B, N, H, D] or NULL receives what y was rounded by
+ * (16-bit types; for the backward).  lse [B, H, N] or NULL receives log2 of the sum of exp(s_ij).
  */
 size_t flare_attn_forward_workspace_size(int64_t B, int64_t N, int64_t M, int64_t H, int64_t D, int dtype);
 int flare_attn_forward(const void* q, const void* k, const void* v, const int64_t* strides, int dtype, int64_t B,
@@ -406,7 +406,8 @@ int flare_attn_forward(const void* q, const void* k, const void* v, const int64_
                        const int32_t* prefix_lengths, const int32_t* lengths, const int32_t* new_lengths, void* y,
                        void* y_rest, float* lse, void* workspace, size_t workspace_bytes, void* stream);
 
-/* Its gradients without a cache, from y, y_rest (or NULL), lse and dy [B, N, H, D]: dq [B, N, H, D], dk, dv [B, N, G, D]. */
+/* Its gradients without a cache, from y, y_rest (or NULL), lse and dy [B, N, H, D]: dq [B, N, H, D], dk
+ * and dv [B, N, G, D]. */
 size_t flare_attn_backward_workspace_size(int64_t B, int64_t N, int64_t H, int64_t G, int64_t D, int dtype);
 int flare_attn_backward(const void* q, const void* k, const void* v, const int64_t* strides, int dtype, int64_t B,
                         int64_t N, int64_t H, int64_t G, int64_t D, float scale, float softcap, const float* slopes,
