@@ -328,7 +328,6 @@ extern "C" int flare_attn_step(const void* q, const void* k, const void* v, cons
     FLARE_REQUIRE(aligned(p.q, dtype) && aligned(kr, dtype) && aligned(vr, dtype) && aligned(p.k, dtype) &&
                   aligned(p.v, dtype) && ((uintptr_t)y & 15) == 0,
                   "flare_attn_step: rows must be 16-byte aligned and less than 2^22 elements apart");
-    FLARE_REQUIRE(B * G * ceil_div(H / G, 16) <= 65535, "flare_attn_step: too large");
     p.splits = step_splits(B, M, H, G);
     if (workspace_bytes < flare_attn_step_workspace_size(B, M, H, G, D) ||
         (p.splits > 1 && (!workspace || ((uintptr_t)workspace & 15)))) {

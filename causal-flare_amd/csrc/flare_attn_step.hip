@@ -33,7 +33,8 @@ __global__ __launch_bounds__(256) void attn_step_kernel(AttnArgs p) {
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int g = lane >> 4, c = lane & 15;
     const int64_t R = p.H / p.G, HG = (R + 15) / 16;
-    const int64_t split = blockIdx.x, hg = blockIdx.y % HG, kvh = blockIdx.y / HG % p.G, b = blockIdx.y / HG / p.G;
+    const int64_t split = blockIdx.x % (unsigned)p.splits, row = blockIdx.x / (unsigned)p.splits;
+    const int64_t hg = row % HG, kvh = row / HG % p.G, b = row / HG / p.G;
     const int64_t len = p.lengths[b];
     if (len < 0 || len >= p.M) {
         // an idle row, or a full cache
@@ -243,7 +244,7 @@ static int step_cap(const AttnArgs& p, hipStream_t stream) {
         }
     }
     const int64_t HG = ceil_div(p.H / p.G, 16);
-    kernel<<<dim3((unsigned)p.splits, (unsigned)(p.B * p.G * HG)), 256, bytes, stream>>>(p);
+    kernel<<<dim3((unsigned)(p.splits * p.B * p.G * HG)), 256, bytes, stream>>>(p);
     int rc = check_launch("attn_step");
     if (rc != FLARE_OK || p.splits == 1) return rc;
     attn_join_kernel<E><<<dim3((unsigned)(p.B * p.H)), 256, 0, stream>>>(p);

@@ -30,19 +30,20 @@ def one_head(q, k, v, dy, see, cap, unit, slope=0.0):
     N, D = q.shape
     scale = D ** -0.5
     far = slope * (torch.arange(N)[:, None] - torch.arange(N)[None]).abs()
+    some = see.any(1, keepdim=True)
     x = q @ k.t() * scale
-    th = torch.tanh(x / cap)
-    s = torch.where(see, cap * th - far, -INF)
-    p = torch.softmax(s, 1)
+    th = torch.tanh(x / cap) if cap else torch.zeros_like(x)
+    s = torch.where(see, (cap * th if cap else x) - far, -INF)
+    p = torch.where(some, torch.softmax(s, 1), 0.0)
     sums = lambda w, t: seen_sums(see, w, t)
     y, pv = sums(p, v), sums(p, v.abs())
     dp = dy @ v.t()
-    delta = (dy * y).sum(1, keepdim=True)
+    delta = torch.where(some, (dy * y).sum(1, keepdim=True), 0.0)
     cut = 1 - th * th
     ds = p * (dp - delta) * cut * scale
     out = {"y": y, "dq": sums(ds, k), "dk": seen_sums(see.t(), ds.t(), q), "dv": seen_sums(see.t(), p.t(), dy)}
     size = (q.abs() @ k.abs().t() * scale).nan_to_num(0.0, 0.0, 0.0) + far
-    es = E32 * (torch.where(see, size, 0.0).amax(1, keepdim=True) * (8 + D / 4) + 16 + 8 * cap)
+    es = E32 * (torch.where(see, size, 0.0).amax(1, keepdim=True) * (8 + D / 4) + 16 + 8 * (cap or 0.0))
     edp = E32 * (16 + D) * (dy.abs() @ v.abs().t()) + (dy.abs() * ((2 * unit + 2 * es + 64 * E32) * pv + unit * y.abs())).sum(1, keepdim=True)
     eds = (p * cut * edp + (2 * es + 64 * E32) * p * (dp - delta).abs() * (cut + 4) + unit * ds.abs() / scale
            + 2.0 ** -25 * (1 + (dp - delta).abs())) * scale
@@ -206,6 +207,23 @@ def test_small_and_large_gradients_of_fp16(std, N, H, G, D, what):
             close_attention(got[:, s], ref[n], n, F16)
     if what == "docs":
         assert all(not t[:, 500:].any() for t in grads)
+
+
+def test_decode_of_many_sequences_and_heads():
+    """More rows of keys than a grid's second dimension takes: each as in a call of its own."""
+    g = gen(9)
+    B, H, G, D, S = 9000, 16, 8, 16, 3
+    q, k, v = (normal(g, B, n, D, dtype=BF16) for n in (H, G, G))
+    cache = {n: normal(g, B, S, G, D, dtype=BF16) for n in "kv"}
+    held = torch.arange(B, device=DEV, dtype=torch.int32) % 5 - 1          # idle, 0, 1, 2 and full
+    parts = []
+    for s in (slice(0, 4500), slice(4500, B)):
+        part = {n: t[s].clone() for n, t in cache.items()}
+        parts.append([cf.softmax_attention_decode(q[s], k[s], v[s], part, held[s])[0], part["k"], part["v"]])
+    y, _ = cf.softmax_attention_decode(q, k, v, cache, held)
+    for got, want in zip((y, cache["k"], cache["v"]), zip(*parts)):
+        assert torch.equal(got.nan_to_num(9.0), torch.cat(want).nan_to_num(9.0))
+    assert y[4::5].isnan().all() and not y[0::5].any()
 
 
 def test_lengths_that_are_no_tensor_are_refused():
