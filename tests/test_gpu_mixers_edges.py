@@ -1,6 +1,7 @@
 """The token mixers on the GPU where a formula meets its edges: infinite values that a cap or a mask
 bounds, growth past fp32, gradients below a type's range, chunks of other lengths."""
 import math
+import random
 
 import pytest
 import torch
@@ -224,6 +225,45 @@ def test_decode_of_many_sequences_and_heads():
     for got, want in zip((y, cache["k"], cache["v"]), zip(*parts)):
         assert torch.equal(got.nan_to_num(9.0), torch.cat(want).nan_to_num(9.0))
     assert y[4::5].isnan().all() and not y[0::5].any()
+
+
+@pytest.mark.parametrize("seed", range(12))
+def test_infinite_values_reach_what_the_formula_gives_them_to(seed):
+    """Which entries of y and of the gradients are finite, with infinite values and NaNs anywhere."""
+    for case in range(20):
+        rng, g = random.Random(100 * seed + case), gen(100 * seed + case)
+        dtype, D = rng.choice([F32, BF16, F16]), rng.choice([16, 32, 48, 64, 80, 96, 112, 128])
+        N = rng.choice([3, 17, 40, 64, 65, 100, 129, 150, 200, 260, 700])
+        t = {n: normal(g, 1, N, 1, D, dtype=dtype) for n in "qkvd"}
+        o, see = {}, torch.ones((N, N), dtype=torch.bool)
+        if rng.random() < 0.8:
+            see = see.tril()
+            if rng.random() < 0.3:
+                o["prefix_lengths"] = torch.tensor([rng.randrange(N + 1)], device=DEV)
+                see |= torch.arange(N)[None] < int(o["prefix_lengths"])
+        else:
+            o["causal"] = False
+        if rng.random() < 0.5:
+            o["document_ids"] = documents(g, 1, N)
+            ids = o["document_ids"][0].cpu()
+            see &= (ids[:, None] == ids[None]) & (ids[:, None] >= 0)
+        cap = rng.choice([None, None, 3.0, 20.0, 40.0, 400.0])
+        if cap:
+            o["softcap"] = cap
+        slope = rng.choice([0.0, 0.25, -0.01])
+        if slope:
+            o["slopes"] = torch.tensor([slope], device=DEV)
+        holes = [(rng.choice("qkvd"), rng.randrange(N), rng.randrange(D), rng.choice([INF, -INF, NAN]))
+                 for _ in range(rng.randrange(4))]
+        for n, i, d, x in holes:
+            t[n][0, i, 0, d] = x
+        leaves = [t[n].clone().requires_grad_() for n in "qkv"]
+        y = cf.softmax_attention(*leaves, **o)
+        grads = torch.autograd.grad(y, leaves, t["d"])
+        ref = one_head(*(t[n][0, :, 0].double().cpu() for n in "qkvd"), see, cap, 0.0, slope)
+        for n, got in zip(("y", "dq", "dk", "dv"), (y, *grads)):
+            have, want = got[0, :, 0].isfinite().cpu(), ref[n][0].isfinite()
+            assert torch.equal(have, want), (n, dtype, N, D, list(o), cap, slope, holes, (have != want).nonzero()[:3].tolist())
 
 
 def test_lengths_that_are_no_tensor_are_refused():
