@@ -87,7 +87,6 @@ enum { kNoCap = 0, kCap = 1, kCapFixed = 2, kCapFine = 3 };
 constexpr float kCoarseCapMost = 256.0f;
 // Caps that keep scale / cap and cap log2(e) far from fp32's ends.
 constexpr float kLeastCap = 0x1p-100f, kMostCap = 0x1p100f;
-inline bool coarse_cap(float cap, int size) { return size == 2 && cap <= kCoarseCapMost; }
 
 // Tiles of 16 queries a wave of the forward's and the query gradients' kernels owns (fp32 operands take
 // twice the registers).

@@ -728,7 +728,7 @@ template <typename E, int DP>
 static int backward_dp(const AttnArgs& p, hipStream_t stream) {
     if (p.cap == 0.0f) return backward_cap<E, DP, kNoCap>(p, stream);
     if constexpr (sizeof(E) == 2)
-        if (coarse_cap(p.cap, sizeof(E))) return backward_cap<E, DP, kCap>(p, stream);
+        if (p.cap <= kCoarseCapMost) return backward_cap<E, DP, kCap>(p, stream);
     return backward_cap<E, DP, kCapFine>(p, stream);
 }
 template <typename E>

@@ -390,7 +390,7 @@ static int forward_dp(const AttnArgs& p, hipStream_t stream) {
     if constexpr (__is_same(E, __hip_bfloat16))
         if (!p.slopes && p.cap * kLog2e <= kCapFixedMost) return forward_cap<E, DP, kCapFixed>(p, stream);
     if constexpr (sizeof(E) == 2)
-        if (coarse_cap(p.cap, sizeof(E))) return forward_cap<E, DP, kCap>(p, stream);
+        if (p.cap <= kCoarseCapMost) return forward_cap<E, DP, kCap>(p, stream);
     return forward_cap<E, DP, kCapFine>(p, stream);
 }
 template <typename E>

@@ -9,8 +9,8 @@ import torch
 import causal_flare as cf
 from causal_flare import _lib
 from _mixers import U, attention, check, scan
-from test_gpu_mixers import (BF16, DEV, E32, F16, F32, close, close_attention, documents, gen, normal, scan_inputs,
-                             test_attention, test_scan, test_scan_prefill_and_decode as prefill_and_decode)
+from test_gpu_mixers import (BF16, DEV, E32, F16, F32, close, close_attention, documents, gen, normal, same,
+                             scan_inputs, test_attention, test_scan, test_scan_prefill_and_decode as prefill_and_decode)
 
 pytestmark = pytest.mark.gpu
 INF, NAN = math.inf, math.nan
@@ -208,6 +208,32 @@ def test_small_and_large_gradients_of_fp16(std, N, H, G, D, what):
             close_attention(got[:, s], ref[n], n, F16)
     if what == "docs":
         assert all(not t[:, 500:].any() for t in grads)
+
+
+def test_fp16_training_steps_in_graphs():
+    """The scales of fp16 score gradients are taken anew at every replay."""
+    g = gen(51)
+    q, k, v, dy = (normal(g, 2, 300, n, 64, dtype=F16) for n in (4, 2, 2, 4))
+    ids = documents(g, 2, 300)
+
+    def call():
+        leaves = [t.clone().requires_grad_() for t in (q, k, v)]
+        y = cf.softmax_attention(*leaves, softcap=20.0, document_ids=ids)
+        return [y.detach(), *torch.autograd.grad(y, leaves, dy)]
+
+    call()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = call()
+    for i in range(4):
+        dy.copy_(normal(g, 2, 300, 4, 64, std=10.0 ** -i).to(F16))
+        v.mul_(0.5)
+        for x in out:
+            x.fill_(1.0)
+        graph.replay()
+        want = call()
+        torch.cuda.synchronize()
+        assert same(out, want), i
 
 
 def test_decode_of_many_sequences_and_heads():
