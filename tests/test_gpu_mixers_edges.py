@@ -9,8 +9,9 @@ import torch
 import causal_flare as cf
 from causal_flare import _lib
 from _mixers import U, attention, check, scan
+import test_gpu_mixers as mixers
 from test_gpu_mixers import (BF16, DEV, E32, F16, F32, close, close_attention, documents, gen, normal, same,
-                             scan_inputs, test_attention, test_scan, test_scan_prefill_and_decode as prefill_and_decode)
+                             scan_inputs)
 
 pytestmark = pytest.mark.gpu
 INF, NAN = math.inf, math.nan
@@ -45,7 +46,8 @@ def one_head(q, k, v, dy, see, cap, unit, slope=0.0):
     out = {"y": y, "dq": sums(ds, k), "dk": seen_sums(see.t(), ds.t(), q), "dv": seen_sums(see.t(), p.t(), dy)}
     size = (q.abs() @ k.abs().t() * scale).nan_to_num(0.0, 0.0, 0.0) + far
     es = E32 * (torch.where(see, size, 0.0).amax(1, keepdim=True) * (8 + D / 4) + 16 + 8 * (cap or 0.0))
-    edp = E32 * (16 + D) * (dy.abs() @ v.abs().t()) + (dy.abs() * ((2 * unit + 2 * es + 64 * E32) * pv + unit * y.abs())).sum(1, keepdim=True)
+    ey = (2 * unit + 2 * es + 64 * E32) * pv + unit * y.abs()
+    edp = E32 * (16 + D) * (dy.abs() @ v.abs().t()) + (dy.abs() * ey).sum(1, keepdim=True)
     eds = (p * cut * edp + (2 * es + 64 * E32) * p * (dp - delta).abs() * (cut + 4) + unit * ds.abs() / scale
            + 2.0 ** -25 * (1 + (dp - delta).abs())) * scale
     tol = {"y": (unit + 2 * es + 64 * E32) * pv + 2.0 ** -25 * seen_sums(see, torch.ones_like(p), v.abs()),
@@ -67,8 +69,8 @@ def check_finite_part(got, ref, what, dtype):
 
 @pytest.mark.parametrize("dtype", [F32, BF16, F16])
 @pytest.mark.parametrize("where", ["q", "k", "q and dy"])
-@pytest.mark.parametrize("cap, D, docs, sloped", [(3.0, 64, True, False), (3.0, 128, False, True), (50.0, 48, True, False),
-                                                  (2.0, 32, False, False)])
+@pytest.mark.parametrize("cap, D, docs, sloped", [
+    (3.0, 64, True, False), (3.0, 128, False, True), (50.0, 48, True, False), (2.0, 32, False, False)])
 def test_a_cap_bounds_infinite_scores(dtype, where, cap, D, docs, sloped):
     """An infinite element of a query or key makes scores of +-cap: weights, y and dv are finite, and only
     the gradients that multiply a score gradient of 0 by that element are none."""
@@ -98,7 +100,7 @@ def test_a_cap_bounds_infinite_scores(dtype, where, cap, D, docs, sloped):
 @pytest.mark.parametrize("D", [16, 32, 48, 80, 128])
 @pytest.mark.parametrize("what", ["docs", "cap docs", "cap docs prefix slopes", "full docs slopes"])
 def test_attention_of_every_width_with_documents(dtype, D, what):
-    test_attention(dtype, 2, 150, 4, 2, D, what)
+    mixers.test_attention(dtype, 2, 150, 4, 2, D, what)
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16, F16])
@@ -289,7 +291,8 @@ def test_infinite_values_reach_what_the_formula_gives_them_to(seed):
         ref = one_head(*(t[n][0, :, 0].double().cpu() for n in "qkvd"), see, cap, 0.0, slope)
         for n, got in zip(("y", "dq", "dk", "dv"), (y, *grads)):
             have, want = got[0, :, 0].isfinite().cpu(), ref[n][0].isfinite()
-            assert torch.equal(have, want), (n, dtype, N, D, list(o), cap, slope, holes, (have != want).nonzero()[:3].tolist())
+            off = (have != want).nonzero()[:3].tolist()
+            assert not off, (n, dtype, N, D, list(o), cap, slope, holes, off)
 
 
 def test_lengths_that_are_no_tensor_are_refused():
@@ -402,17 +405,19 @@ def test_scan_in_longer_chunks(chunk, dtype, B, N, C, S, G, docs, more, chunks):
     """The chunks of large calls on small ones: several kept stretches a chunk, forward chunks of more than
     8 tokens."""
     chunks(chunk)
-    test_scan(dtype, B, N, C, S, G, docs, more)
+    mixers.test_scan(dtype, B, N, C, S, G, docs, more)
 
 
-@pytest.mark.parametrize("dtype, B, N, C, S, G", [(F16, 4, 1, 16, 16, 1), (F16, 5, 33, 70, 16, 2), (F16, 4, 90, 64, 20, 1)])
+@pytest.mark.parametrize("dtype, B, N, C, S, G", [
+    (F16, 4, 1, 16, 16, 1), (F16, 5, 33, 70, 16, 2), (F16, 4, 90, 64, 20, 1)])
 def test_scan_prefill_and_decode_of_fp16(dtype, B, N, C, S, G):
-    prefill_and_decode(dtype, B, N, C, S, G)
+    mixers.test_scan_prefill_and_decode(dtype, B, N, C, S, G)
 
 
 @pytest.mark.parametrize("chunk, dtype, B, N, C, S, G", [
-    (13, F32, 3, 260, 40, 8, 1), (128, BF16, 3, 260, 40, 8, 1), (128, F16, 4, 300, 64, 20, 1), (64, F32, 3, 65, 16, 64, 1),
+    (13, F32, 3, 260, 40, 8, 1), (128, BF16, 3, 260, 40, 8, 1), (128, F16, 4, 300, 64, 20, 1),
+    (64, F32, 3, 65, 16, 64, 1),
     (1 << 32, BF16, 3, 65, 16, 16, 1), ((1 << 63) - 1, F16, 3, 65, 16, 16, 1)])
 def test_scan_prefill_in_other_chunks(chunk, dtype, B, N, C, S, G, chunks):
     chunks(chunk)
-    prefill_and_decode(dtype, B, N, C, S, G)
+    mixers.test_scan_prefill_and_decode(dtype, B, N, C, S, G)
