@@ -182,6 +182,7 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnArgs p) {
 
     const int prefix = p.prefix ? (int)clamp_to(p.prefix[b], p.N) : 0;
     int k_begin = 0, kv_end = p.causal ? max(min(q0 + QB, N), prefix) : N;
+    const int seen_end = kv_end;                        // of all parts: y is of all that a row sees
     if (parts > 1) {
         const int tiles = (kv_end + KT - 1) / KT;
         k_begin = (int)((int64_t)tiles * part_id / parts) * KT;
@@ -193,7 +194,7 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnArgs p) {
     Frag qf[QT][DK], gf[QT][DK];
     int pos[QT], lim[QT], qid[QT];                     // as in attn_forward
     float lse[QT], delta[QT], factor[QT];
-    const float most_v = kScaled<E> ? largest(p, b, 1, k_begin, kv_end, mine) : 0.0f;
+    const float most_v = kScaled<E> ? largest(p, b, 1, 0, seen_end, mine) : 0.0f;
 #pragma unroll
     for (int t = 0; t < QT; ++t) {
         const int i = w0 + 16 * t + c;

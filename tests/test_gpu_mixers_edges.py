@@ -320,6 +320,26 @@ def test_attention_of_a_round_of_workgroups(N):
         check(y[0, :, h], (p @ c).cpu(), (tol + E32 * (p @ c).abs()).cpu(), f"y of head {h}")
 
 
+@pytest.mark.parametrize("N", [300, 1500])
+def test_fp16_gradients_where_few_keys_hold_large_values(N):
+    """Rows that divide their weight between a key of large values and one of small ones far behind it,
+    which of 1500 rows other workgroups take: dy . y is as large as the former."""
+    g = gen(N)
+    D, far = 64, N - 100
+    q, k, v, dy = (torch.zeros((1, N, 1, D), dtype=F16, device=DEV) for _ in range(4))
+    q[..., :8], k[0, 10, 0, :8], k[0, far, 0, :8] = 4.0, 8.0, 8.0          # scores of 32 and of 0
+    v[:] = normal(g, 1, N, 1, D, dtype=F16)
+    v[0, 10] = 1000.0
+    dy[:] = normal(g, 1, N, 1, D).abs().to(F16)
+    leaves = [t.clone().requires_grad_() for t in (q, k, v)]
+    grads = torch.autograd.grad(cf.softmax_attention(*leaves), leaves, dy)
+    bound = 2 * float(dy.double().abs().sum(-1).max()) * float(v.double().abs().max())
+    ref = attention(q, k, v, dy=dy, unit=U[F16], tiny=2.0 ** -39 * bound)
+    # (dk of key 10 is past fp16's largest number: 100 rows of dS = 1/4 1000 |dy|_1 scale, times q = 4)
+    for n, got in zip(("dq", "dk"), grads):
+        close_attention(got, ref[n], n, F16)
+
+
 # ---------------------------------------------------------------------------------------
 # State space scan
 # ---------------------------------------------------------------------------------------
