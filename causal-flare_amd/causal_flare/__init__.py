@@ -7,7 +7,7 @@ raising ``NotImplementedError``: the semi-autoregressive prefill/decode stubs
 (stubs in the reference too).
 
 ``mixers`` holds token mixers for hybrid stacks, without a counterpart in the reference: a short
-convolution, a state space scan and softmax attention.
+convolution, a state space scan and softmax attention, with rotary positions and caches of 8 or 4 bits.
 """
 from . import autoregressive, mixers, semi_autoregressive
 from .autoregressive.training import flare_autoregressive_triton
@@ -22,6 +22,11 @@ from .semi_autoregressive.inference import (
     flare_semi_autoregressive_prefill_trition,
 )
 from .mixers import (
+    quantized_cache,
+    quantized_cache_read,
+    quantized_cache_write,
+    rotary_frequencies,
+    rotary_positions,
     short_convolution,
     short_convolution_decode,
     short_convolution_prefill,
@@ -47,6 +52,11 @@ __all__ = [
     "flare_semi_autoregressive_decode_trition",
     "flare_semi_autoregressive_prefill_trition",
     "flare_semi_autoregressive_trition",
+    "quantized_cache",
+    "quantized_cache_read",
+    "quantized_cache_write",
+    "rotary_frequencies",
+    "rotary_positions",
     "short_convolution",
     "short_convolution_decode",
     "short_convolution_prefill",

@@ -63,6 +63,11 @@ HEADER_FUNCTIONS = (
     "flare_attn_append",
     "flare_attn_step_workspace_size",
     "flare_attn_step",
+    "flare_rotary",
+    "flare_qcache_write",
+    "flare_qcache_read",
+    "flare_qattn_workspace_size",
+    "flare_qattn",
 )
 
 F32, BF16, F16 = 0, 1, 2
@@ -181,6 +186,16 @@ def _declare(lib):
     lib.flare_attn_step_workspace_size.argtypes = [_i64] * 5
     lib.flare_attn_step.restype = _i
     lib.flare_attn_step.argtypes = ([_vp] * 4 + [_i] + [_i64] * 5 + [_f, _f] + [_vp] * 5 + [_vp, _sz, _vp])
+    lib.flare_rotary.restype = _i
+    lib.flare_rotary.argtypes = [_vp] * 3 + [_i] + [_i64] * 6 + [_vp] * 3 + [_i, _i] + [_vp] * 3
+    lib.flare_qcache_write.restype = _i
+    lib.flare_qcache_write.argtypes = [_vp] * 3 + [_i, _i] + [_i64] * 5 + [_vp] * 7
+    lib.flare_qcache_read.restype = _i
+    lib.flare_qcache_read.argtypes = [_vp] * 4 + [_i, _i] + [_i64] * 5 + [_vp] * 4
+    lib.flare_qattn_workspace_size.restype = _sz
+    lib.flare_qattn_workspace_size.argtypes = [_i64] * 6 + [_i]
+    lib.flare_qattn.restype = _i
+    lib.flare_qattn.argtypes = ([_vp] * 4 + [_i, _i] + [_i64] * 6 + [_f, _f] + [_vp] * 9 + [_vp, _sz, _vp])
 
 
 def _check_single_hip_runtime():

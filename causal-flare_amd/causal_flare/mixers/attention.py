@@ -15,8 +15,8 @@ products with V and dY, and the scores' gradients in two parts for those with K 
 to be differentiated keeps Q, K, V, y, a float32 a row of a head and, of 16-bit inputs, what y was
 rounded by (as large as y) until its backward.
 
-A cache is ``{"k": [B, S, G, D], "v": [B, S, G, D]}``, room for S tokens a sequence; how many each
-holds is the caller's to keep, in `lengths`.
+A cache is ``{"k": [B, S, G, D], "v": [B, S, G, D]}``, room for S tokens a sequence, or one of
+`quantized_cache`, in 8 or 4 bits; how many tokens each holds is the caller's to keep, in `lengths`.
 """
 from __future__ import annotations
 
@@ -42,6 +42,7 @@ from ._inputs import (
     _strides,
     _training,
 )
+from .quantized import attend_quantized, is_quantized
 
 
 # Caps that the kernels take: what scale / cap and the cap itself can be with in float32.
@@ -212,6 +213,11 @@ def softmax_attention_prefill(
     name = "softmax_attention_prefill"
     B, T, H, G, D = _check_heads(name, Q, K, V)
     cap = _check_scores(name, H, scale, softcap, slopes)
+    if is_quantized(cache):
+        _check_integers(name, "prefix_lengths", prefix_lengths, (B,))
+        _check_integers(name, "new_lengths", new_lengths, (B,))
+        return attend_quantized(name, Q, K, V, cache, lengths, _resolve_attn_scale(scale, D), cap, slopes, prefix_lengths,
+                                new_lengths), cache
     kc, vc = _check_cache(name, cache, lengths, Q, K, V, B, G, D)
     _check_integers(name, "prefix_lengths", prefix_lengths, (B,))
     _check_integers(name, "new_lengths", new_lengths, (B,))
@@ -304,7 +310,8 @@ def softmax_attention_decode(
     is full is not written, and its y is NaN.
     """
     name = "softmax_attention_decode"
-    out = _step_fast(Q, K, V, cache, lengths, scale, softcap, slopes)
+    quantized = is_quantized(cache)
+    out = None if quantized else _step_fast(Q, K, V, cache, lengths, scale, softcap, slopes)
     if out is not None:
         return out
     Q, K, V = (t[:, None] if t.dim() == 3 else t for t in (Q, K, V))
@@ -312,6 +319,8 @@ def softmax_attention_decode(
     if T != 1:
         raise ValueError(f"{name} expects one token a sequence. Got Q={tuple(Q.shape)}")
     cap = _check_scores(name, H, scale, softcap, slopes)
+    if quantized:
+        return attend_quantized(name, Q, K, V, cache, lengths, _resolve_attn_scale(scale, D), cap, slopes, None, None), cache
     kc, vc = _check_cache(name, cache, lengths, Q, K, V, B, G, D)
     device = _check_device(name, Q=Q, K=K, V=V, cache_k=kc, cache_v=vc, lengths=lengths, slopes=slopes)
     y = torch.empty((B, 1, H, D), device=device, dtype=kc.dtype)

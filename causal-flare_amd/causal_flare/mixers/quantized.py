@@ -1,0 +1,188 @@
+"""A cache of keys and values in 8 or 4 bits, for softmax attention.
+
+``{"k", "v", "k_scale", "v_scale"}``: a token's key or value of one head is cut into blocks of 32
+dimensions (the last may have 16), each with a power of 2 of its own,
+
+    value = code 2^(scale - 127)
+
+k, v: 8 bits, float8_e4m3fn [B, S, G, D], or 4, uint8 [B, S, G, D / 2] of two e2m1 codes (0, 1/2, 1, 3/2, 2,
+3, 4, 6 and a sign; the lower index in the lower half).  k_scale, v_scale: uint8 [B, S, G, ceil(D / 32)].  The
+scale is the least for which the block's largest value rounds to no more than the largest code (up to the
+range of the type that is written from); values are rounded to the nearest code, ties to the even one.  A block
+that holds an infinite value or a NaN is NaN, with a scale of 255.  The root of the mean square of what
+normally distributed values are rounded by is 2.7% of theirs with 8 bits and 11% with 4.
+
+`softmax_attention_prefill` and `softmax_attention_decode` take such a cache in place of one of the queries'
+type.  They write new keys and values to it first and see them as it holds them, so that a prompt in pieces gives
+what it gives whole.  Its codes have to be such as the calls write.
+"""
+from __future__ import annotations
+
+import torch
+
+from .. import _lib
+from ._inputs import (
+    _aligned_rows,
+    _check_device,
+    _check_float,
+    _check_integers,
+    _f32,
+    _int32,
+    _on,
+    _ptr,
+    _raw_stream,
+    _strides,
+)
+
+_BLOCK = 32
+_PARTS = ("k", "k_scale", "v", "v_scale")
+
+
+def is_quantized(cache) -> bool:
+    return isinstance(cache, dict) and "k_scale" in cache
+
+
+def quantized_cache(B: int, S: int, G: int, D: int, bits: int = 8, device="cuda") -> dict[str, torch.Tensor]:
+    """An empty cache of S tokens for each of B sequences, G key heads of D dimensions, in 8 or 4 bits."""
+    name = "quantized_cache"
+    if bits not in (4, 8):
+        raise ValueError(f"{name} expects 8 or 4 bits. Got {bits!r}")
+    if B < 0 or S < 1 or G < 1 or D % 16 or not 16 <= D <= 128:
+        raise ValueError(f"{name} expects positive sizes, and head dimensions that are multiples of 16 up to 128. "
+                         f"Got B={B}, S={S}, G={G}, D={D}")
+    cache = {}
+    for n in ("k", "v"):
+        codes = torch.zeros((B, S, G, D * bits // 8), device=device, dtype=torch.uint8)
+        cache[n] = codes.view(torch.float8_e4m3fn) if bits == 8 else codes
+        cache[n + "_scale"] = torch.zeros((B, S, G, -(-D // _BLOCK)), device=device, dtype=torch.uint8)
+    return cache
+
+
+def check_quantized(name, cache):
+    """(bits, B, S, G, D) of a cache whose tensors are what the kernels read and write in place."""
+    if not isinstance(cache, dict) or any(not isinstance(cache.get(n), torch.Tensor) for n in _PARTS):
+        raise ValueError(f"{name} expects a cache {{'k', 'v', 'k_scale', 'v_scale'}} of quantized_cache. Got {cache!r:.80}")
+    k = cache["k"]
+    if k.dtype not in (torch.uint8, torch.float8_e4m3fn):
+        raise ValueError(f"{name} expects codes of float8_e4m3fn, or uint8 for 4 bits. Got {k.dtype}")
+    bits = 4 if k.dtype is torch.uint8 else 8
+    if k.dim() != 4:
+        raise ValueError(f"{name} expects cache['k'] [B, S, G, D or D / 2]. Got {tuple(k.shape)}")
+    B, S, G, D = k.shape[0], k.shape[1], k.shape[2], k.shape[3] * 8 // bits
+    if D % 16 or not 16 <= D <= 128 or S < 1 or G < 1:
+        raise ValueError(f"{name} supports head dimensions that are multiples of 16 up to 128. Got cache['k'] "
+                         f"{tuple(k.shape)} of {bits} bits")
+    scales = (B, S, G, -(-D // _BLOCK))
+    for n, shape, dtype in (("v", k.shape, k.dtype), ("k_scale", scales, torch.uint8), ("v_scale", scales, torch.uint8)):
+        if tuple(cache[n].shape) != tuple(shape) or cache[n].dtype is not dtype:
+            raise ValueError(f"{name} expects cache[{n!r}] {list(shape)} of {dtype}. Got {tuple(cache[n].shape)} of "
+                             f"{cache[n].dtype}")
+    for n in _PARTS:
+        if not cache[n].is_contiguous() or (n in ("k", "v") and cache[n].data_ptr() % 16):
+            raise ValueError(f"{name} writes the cache in place and expects it contiguous, on 16-byte boundaries")
+    return bits, B, S, G, D
+
+
+def check_lengths(name, lengths, B):
+    if not isinstance(lengths, torch.Tensor):
+        raise ValueError(f"{name} expects a tensor in lengths. Got {lengths!r:.80}")
+    _check_integers(name, "lengths", lengths, (B,))
+
+
+def quantized_cache_write(
+    cache: dict[str, torch.Tensor],
+    K: torch.Tensor,
+    V: torch.Tensor,
+    lengths: torch.Tensor,
+    new_lengths: torch.Tensor | None = None,
+):
+    """K and V [B, T, G, D] behind what the cache holds, in place; returns the cache.
+
+    lengths: integers [B], the tokens each sequence's cache holds already, not changed.  new_lengths: integers
+    [B], how many of the T rows are real (all by default); those behind them are not written.  A sequence of
+    negative length sits out, and one whose new tokens do not fit the cache is not written at all.
+    """
+    name = "quantized_cache_write"
+    bits, B, S, G, D = check_quantized(name, cache)
+    if K.dim() != 4 or V.shape != K.shape or (K.shape[0], K.shape[2], K.shape[3]) != (B, G, D):
+        raise ValueError(f"{name} expects K and V [B, T, G, D] with B={B}, G={G}, D={D}. Got {tuple(K.shape)}, "
+                         f"{tuple(V.shape)}")
+    _check_float(name, K=K, V=V)
+    if V.dtype != K.dtype:
+        raise ValueError(f"{name} expects one type for K and V. Got {K.dtype}, {V.dtype}")
+    code = _lib.dtype_code(K.dtype)
+    check_lengths(name, lengths, B)
+    _check_integers(name, "new_lengths", new_lengths, (B,))
+    device = _check_device(name, K=K, V=V, lengths=lengths, new_lengths=new_lengths, **{"cache_" + n: cache[n] for n in _PARTS})
+    if K.numel() == 0:
+        return cache
+    k, v = _aligned_rows(K, K.dtype), _aligned_rows(V, K.dtype)
+    lens, new = _int32(lengths), _int32(new_lengths)
+    P = _ptr
+    with _on(device):
+        rc = _lib.lib().flare_qcache_write(
+            P(k), P(v), _strides(*k.stride()[:3], *v.stride()[:3]), code, bits, B, K.shape[1], S, G, D, P(lens), P(new),
+            *(cache[n].data_ptr() for n in _PARTS), _raw_stream(device.index))
+    _lib.check(rc, "flare_qcache_write")
+    return cache
+
+
+def quantized_cache_read(
+    cache: dict[str, torch.Tensor],
+    first: torch.Tensor | None = None,
+    count: int | None = None,
+    dtype: torch.dtype = torch.bfloat16,
+):
+    """What the cache holds as tensors K, V [B, count, G, D] of `dtype`: rows first[b] .. first[b] + count - 1 of
+    each sequence (all by default), 0 where these lie outside of the cache.
+
+    first: integers [B].  dtype: bfloat16 or float32, in which every value is exact, or float16, in which it is
+    if it was written from that type (and rounded to it otherwise, infinite beyond its range).
+    """
+    name = "quantized_cache_read"
+    bits, B, S, G, D = check_quantized(name, cache)
+    code = _lib.dtype_code(dtype)
+    _check_integers(name, "first", first, (B,))
+    count = S if count is None else int(count)
+    if count < 0:
+        raise ValueError(f"{name} expects a count of rows, not negative. Got {count}")
+    device = _check_device(name, first=first, **{"cache_" + n: cache[n] for n in _PARTS})
+    k, v = (torch.empty((B, count, G, D), device=device, dtype=dtype) for _ in range(2))
+    if k.numel() == 0:
+        return k, v
+    at = _int32(first)
+    P = _ptr
+    with _on(device):
+        rc = _lib.lib().flare_qcache_read(*(cache[n].data_ptr() for n in _PARTS), code, bits, B, count, S, G, D, P(at), P(k),
+                                          P(v), _raw_stream(device.index))
+    _lib.check(rc, "flare_qcache_read")
+    return k, v
+
+
+def attend_quantized(name, Q, K, V, cache, lengths, scale, cap, slopes, prefix_lengths, new_lengths):
+    """Attention of new tokens, K and V of checked shapes, over a quantised cache that receives them: y."""
+    B, T, H, D = Q.shape
+    bits, cB, S, G, cD = check_quantized(name, cache)
+    if (cB, G, cD) != (B, K.shape[2], D):
+        raise ValueError(f"{name} expects a cache of B={B} sequences, G={K.shape[2]} heads of D={D}. Got B={cB}, G={G}, D={cD}")
+    if K.dtype != Q.dtype or V.dtype != Q.dtype:
+        raise ValueError(f"{name} expects one type for Q, K and V. Got {Q.dtype}, {K.dtype}, {V.dtype}")
+    code = _lib.dtype_code(Q.dtype)
+    check_lengths(name, lengths, B)
+    device = _check_device(name, Q=Q, K=K, V=V, **{"cache_" + n: cache[n] for n in _PARTS}, lengths=lengths, slopes=slopes,
+                           prefix_lengths=prefix_lengths, new_lengths=new_lengths)
+    y = torch.empty((B, T, H, D), device=device, dtype=Q.dtype)
+    if y.numel() == 0:
+        return y
+    q, k, v = (_aligned_rows(t, Q.dtype) for t in (Q, K, V))
+    sl, pre, lens, new = _f32(slopes), _int32(prefix_lengths), _int32(lengths), _int32(new_lengths)
+    lib, P = _lib.lib(), _ptr
+    nbytes = lib.flare_qattn_workspace_size(B, T, S, H, G, D, code)
+    ws = torch.empty(nbytes, device=device, dtype=torch.uint8) if nbytes else None
+    with _on(device):
+        rc = lib.flare_qattn(
+            P(q), P(k), P(v), _strides(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3]), code, bits, B, T, S, H, G, D,
+            scale, cap, P(sl), P(pre), P(lens), P(new), *(cache[n].data_ptr() for n in _PARTS), P(y), P(ws), nbytes,
+            _raw_stream(device.index))
+    _lib.check(rc, "flare_qattn")
+    return y

@@ -1,0 +1,152 @@
+"""Rotary positions of queries and keys, for softmax attention beside or in place of its bias on distance.
+
+Pair i of a head's first R dimensions, (a, b), is turned by the angle position * frequencies[i]:
+
+    (a, b) -> (a cos - b sin, a sin + b cos)
+
+The pairs are dimensions i and i + R / 2, or 2i and 2i + 1 (`interleaved`); dimensions from R on stay
+as they are.  Angles are exact to some 1e-9 of a radian and more, however far the position; products are
+taken in float32 and rounded once.
+"""
+from __future__ import annotations
+
+import math
+
+import torch
+import torch.autograd as autograd
+from torch.autograd.function import once_differentiable
+
+from .. import _lib
+from .._common import _compute_dtype
+from ._inputs import (
+    _check_device,
+    _check_float,
+    _check_integers,
+    _int32,
+    _on,
+    _ptr,
+    _raw_stream,
+    _rows,
+    _strides,
+)
+
+
+def rotary_frequencies(
+    dim: int,
+    base: float = 10000.0,
+    factor: float = 1.0,
+    original_length: float | None = None,
+    low_turns: float = 1.0,
+    high_turns: float = 32.0,
+) -> torch.Tensor:
+    """Radians a token of each pair, float64 [dim / 2] on the host: base^(-2 i / dim), for contexts `factor`
+    times as long.
+
+    Without original_length all frequencies are divided by factor.  With it, those that make at least
+    high_turns turns over so many tokens stay as they are, those of low_turns and fewer are divided by factor,
+    and those between are mixed, linearly in the turns.
+    """
+    if dim < 2 or dim % 2:
+        raise ValueError(f"rotary_frequencies expects an even number of dimensions. Got {dim}")
+    if not (0 < base < math.inf and 0 < factor < math.inf):
+        raise ValueError(f"rotary_frequencies expects positive base and factor. Got {base!r}, {factor!r}")
+    f = float(base) ** (-torch.arange(0, dim, 2, dtype=torch.float64) / dim)
+    if original_length is None:
+        return f / factor
+    if not (0 < original_length < math.inf and low_turns < high_turns):
+        raise ValueError("rotary_frequencies expects a positive original_length and low_turns below high_turns. "
+                         f"Got {original_length!r}, {low_turns!r}, {high_turns!r}")
+    keep = ((original_length * f / (2 * math.pi) - low_turns) / (high_turns - low_turns)).clamp(0, 1)
+    return f * (keep + (1 - keep) / factor)
+
+
+def _turn(q, k, frequencies, positions, lengths, interleaved, inverse):
+    """The pairs of q [B, N, H, D] and k [B, N, G, D] (or None), of one type, turned."""
+    dtype = _compute_dtype(q, k)
+    qr, kr = _rows(q, dtype), _rows(k, dtype)
+    B, N, H, D = q.shape
+    q_out = torch.empty((B, N, H, D), device=q.device, dtype=dtype)
+    k_out = None if k is None else torch.empty(k.shape, device=q.device, dtype=dtype)
+    strides = _strides(*qr.stride()[:3], *((0, 0, 0) if k is None else kr.stride()[:3]))
+    P = _ptr
+    with _on(q.device):
+        rc = _lib.lib().flare_rotary(
+            P(qr), P(kr), strides, _lib.dtype_code(dtype), B, N, H, 0 if k is None else k.shape[2], D,
+            2 * frequencies.shape[0], P(frequencies), P(positions), P(lengths), int(interleaved), int(inverse), P(q_out),
+            P(k_out), _raw_stream(q.device.index))
+    _lib.check(rc, "flare_rotary")
+    return q_out.to(q.dtype), None if k is None else k_out.to(k.dtype)
+
+
+class RotaryPositions(autograd.Function):
+    """Turned queries and keys; their gradients are turned back."""
+
+    @staticmethod
+    def forward(ctx, Q, K, frequencies, positions, lengths, interleaved):
+        ctx.save_for_backward(positions, lengths)
+        ctx.options = (frequencies, interleaved)
+        ctx.keys = K is not None
+        q, k = _turn(Q, K, frequencies, positions, lengths, interleaved, False)
+        return (q, k) if ctx.keys else q
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, *grads):
+        positions, lengths = ctx.saved_tensors
+        frequencies, interleaved = ctx.options
+        need_q, need_k = ctx.needs_input_grad[0], ctx.keys and ctx.needs_input_grad[1]
+        dq, dk = None, None
+        if need_q:
+            dq, dk = _turn(grads[0], grads[1] if need_k else None, frequencies, positions, lengths, interleaved, True)
+        elif need_k:
+            dk, _ = _turn(grads[1], None, frequencies, positions, lengths, interleaved, True)
+        return dq, dk, None, None, None, None
+
+
+def rotary_positions(
+    Q: torch.Tensor,
+    K: torch.Tensor | None,
+    frequencies: torch.Tensor,
+    positions: torch.Tensor | None = None,
+    lengths: torch.Tensor | None = None,
+    interleaved: bool = False,
+):
+    """Q [B, N, H, D] and K [B, N, G, D] (or None) turned by their positions: (Q, K), or Q alone.
+
+    Differentiable in Q and K.  Single tokens may be given as [B, H, D] and [B, G, D].  frequencies: float64
+    [R / 2] on the host (`rotary_frequencies`), R up to D; the rest of a head stays as it is.  positions: integers
+    [B, N] (of packed documents, say), any sign; or lengths: integers [B], the tokens that each sequence's cache
+    holds already: token t is at position lengths[b] + t.  Without either it is at t.  D up to 256.
+    """
+    name = "rotary_positions"
+    token = Q.dim() == 3
+    if Q.dim() not in (3, 4) or (K is not None and K.dim() != Q.dim()):
+        raise ValueError(f"{name} expects Q [B, N, H, D] and K [B, N, G, D], or without N. Got Q={tuple(Q.shape)}"
+                         + ("" if K is None else f", K={tuple(K.shape)}"))
+    if token:
+        Q, K = Q[:, None], None if K is None else K[:, None]
+    B, N, H, D = Q.shape
+    if K is not None and (K.shape[:2] != Q.shape[:2] or K.shape[3] != D):
+        raise ValueError(f"{name} expects K [B, N, G, D] with B={B}, N={N}, D={D}. Got {tuple(K.shape)}")
+    if H < 1 or (K is not None and K.shape[2] < 1):
+        raise ValueError(f"{name} expects heads. Got Q={tuple(Q.shape)}" + ("" if K is None else f", K={tuple(K.shape)}"))
+    _check_float(name, Q=Q, K=K)
+    if (not isinstance(frequencies, torch.Tensor) or frequencies.device.type != "cpu"
+            or frequencies.dtype is not torch.float64 or frequencies.dim() != 1):
+        raise ValueError(f"{name} expects frequencies as a float64 tensor [R / 2] on the host. Got {frequencies!r:.80}")
+    R = 2 * frequencies.shape[0]
+    if not 2 <= R <= D or D > 256:
+        raise ValueError(f"{name} turns 2 to D dimensions of heads of up to 256. Got {R} of D={D}")
+    _check_integers(name, "positions", positions, (B, N))
+    _check_integers(name, "lengths", lengths, (B,))
+    if positions is not None and lengths is not None:
+        raise ValueError(f"{name} expects positions or lengths, not both")
+    _check_device(name, Q=Q, K=K, positions=positions, lengths=lengths)
+    if B * N == 0:
+        out = Q.clone() if K is None else (Q.clone(), K.clone())
+    else:
+        out = RotaryPositions.apply(Q, K, frequencies.detach().contiguous(), _int32(positions), _int32(lengths),
+                                    bool(interleaved))
+    if K is None:
+        return out[:, 0] if token else out
+    return (out[0][:, 0], out[1][:, 0]) if token else out

@@ -47,6 +47,13 @@ struct Rows {                        // a [B, n, heads, D] tensor: element strid
     int64_t sb, sn, sh;
 };
 
+// Rows on 16-byte boundaries.
+inline bool aligned(const Rows& r, int dtype) {
+    const int64_t per = dtype == FLARE_F32 ? 4 : 8;
+    return ((uintptr_t)r.p & 15) == 0 && r.sb % per == 0 && r.sn % per == 0 && r.sh % per == 0 && r.sn >= 0 &&
+           r.sn < kMostStride;
+}
+
 struct AttnArgs {
     Rows q, k, v;
     void* y;                         // [B, N, H, D]
@@ -74,6 +81,8 @@ struct AttnArgs {
     int64_t kn_sb, kn_sg, vn_sb, vn_sg;
     float* parts;                    // what `splits` workgroups leave of each sum
     int64_t splits;
+    // a cache of 8 or 4 bits: the codes are k.p and v.p
+    uint8_t *k_scale, *v_scale;      // [B, M, G, blocks of 32 dimensions]
 };
 
 // How a kernel takes scores: as they are; capped, with tanh to an absolute error (kCap), and against the

@@ -7,6 +7,8 @@ namespace attn {
 
 template <typename E> int forward_e(const AttnArgs& p, hipStream_t stream);
 template <typename E> int backward_e(const AttnArgs& p, float* delta, float* norms, float* ranges, hipStream_t stream);
+template <typename E, int BITS> int forward_bits(const AttnArgs& p, hipStream_t stream);
+template <typename E, int BITS> int rows_e(const AttnArgs& p, int tiles, hipStream_t stream);
 int attn_step(const AttnArgs& p, int dtype, hipStream_t stream);
 
 // A wave for each 64 tokens.
@@ -159,12 +161,6 @@ static size_t rows_bytes(const AttnArgs& p) {
     return p.splits == 1 ? 0 : (size_t)(p.B * p.H * p.N * p.splits * (p.D + 4)) * sizeof(float);
 }
 
-static bool aligned(const Rows& r, int dtype) {
-    const int64_t per = dtype == FLARE_F32 ? 4 : 8;
-    return ((uintptr_t)r.p & 15) == 0 && r.sb % per == 0 && r.sn % per == 0 && r.sh % per == 0 && r.sn >= 0 &&
-           r.sn < kMostStride;
-}
-
 // Workgroups of the step kernel for each sequence's keys: enough for one on each CU (256 on the
 // card), whose four waves have the loads under way that its memory takes, and no more than the cache
 // has shares of 128 keys.  us, the joining included, for 256, 512 and 1024: 64 sequences of 8000
@@ -172,6 +168,25 @@ static bool aligned(const Rows& r, int dtype) {
 static int64_t step_splits(int64_t B, int64_t M, int64_t H, int64_t G) {
     const int64_t rows = B * G * ceil_div(H / G, 16), s = ceil_div(256, rows), most = ceil_div(M, 128);
     return s < 1 ? 1 : (s > most ? most : s);
+}
+
+// A few new tokens over a cache of 8 or 4 bits: rows (token, head) of the heads that share keys.
+constexpr int64_t kFewRows = 64;
+static int row_tiles(int64_t N, int64_t H, int64_t G) { return H / G * N > 16 ? 2 : 1; }
+static bool few_rows(int64_t N, int64_t H, int64_t G) { return H / G * N <= kFewRows; }
+// Workgroups for each sequence's keys, as step_splits: 
+static int64_t rows_splits(int64_t B, int64_t N, int64_t M, int64_t H, int64_t G) {
+    const int64_t rows = B * G * ceil_div(H / G * N, 16 * row_tiles(N, H, G));
+    const int64_t s = ceil_div(512, rows), most = ceil_div(M, 256);
+    return s < 1 ? 1 : (s > most ? most : s);
+}
+template <typename E>
+static int qattn_rows(const AttnArgs& p, int bits, int tiles, hipStream_t stream) {
+    return bits == 8 ? rows_e<E, 8>(p, tiles, stream) : rows_e<E, 4>(p, tiles, stream);
+}
+template <typename E>
+static int qattn_forward(const AttnArgs& p, int bits, hipStream_t stream) {
+    return bits == 8 ? forward_bits<E, 8>(p, stream) : forward_bits<E, 4>(p, stream);
 }
 
 }  // namespace attn
@@ -336,4 +351,56 @@ extern "C" int flare_attn_step(const void* q, const void* k, const void* v, cons
     }
     p.lengths = lengths, p.y = y, p.parts = (float*)workspace;
     return attn_step(p, dtype, (hipStream_t)stream);
+}
+
+extern "C" size_t flare_qattn_workspace_size(int64_t B, int64_t N, int64_t M, int64_t H, int64_t G, int64_t D, int dtype) {
+    if (B < 1 || N < 1 || M < 1 || H < 1 || G < 1 || H % G) return 0;
+    if (few_rows(N, H, G)) {
+        const int64_t s = rows_splits(B, N, M, H, G);
+        return s == 1 ? 0 : (size_t)(B * N * H * s * (D + 4)) * sizeof(float);
+    }
+    AttnArgs p = {};
+    p.B = B, p.N = N, p.M = M, p.H = H, p.D = D, p.causal = 1;
+    split_forward(p, dtype);
+    return rows_bytes(p);
+}
+
+extern "C" int flare_qattn(const void* q, const void* k, const void* v, const int64_t* strides, int dtype, int bits, int64_t B,
+                           int64_t N, int64_t M, int64_t H, int64_t G, int64_t D, float scale, float softcap,
+                           const float* slopes, const int32_t* prefix_lengths, const int32_t* lengths,
+                           const int32_t* new_lengths, void* k_cache, void* k_scale, void* v_cache, void* v_scale, void* y,
+                           void* workspace, size_t workspace_bytes, void* stream) {
+    FLARE_REQUIRE(q && k && v && strides && lengths && k_cache && k_scale && v_cache && v_scale && y,
+                  "flare_qattn: null pointer");
+    ATTN_REQUIRE_SIZES("flare_qattn");
+    FLARE_REQUIRE(bits == 4 || bits == 8, "flare_qattn: %d bits; 4 or 8", bits);
+    AttnArgs p = attn_args(q, k_cache, v_cache, strides, B, N, M, H, G, D, scale, softcap, slopes);
+    const Rows kr = {k, strides[3], strides[4], strides[5]}, vr = {v, strides[6], strides[7], strides[8]};
+    const uintptr_t held = (uintptr_t)k_cache | (uintptr_t)v_cache | (uintptr_t)y;
+    FLARE_REQUIRE(aligned(p.q, dtype) && aligned(kr, dtype) && aligned(vr, dtype) && (held & 15) == 0,
+                  "flare_qattn: rows must be 16-byte aligned and less than 2^22 elements apart");
+    if (workspace_bytes < flare_qattn_workspace_size(B, N, M, H, G, D, dtype) ||
+        (workspace_bytes && (!workspace || ((uintptr_t)workspace & 15)))) {
+        set_error("flare_qattn: workspace of %zu bytes is too small or not 16-byte aligned", workspace_bytes);
+        return FLARE_ERR_WORKSPACE;
+    }
+    p.k_scale = (uint8_t*)k_scale, p.v_scale = (uint8_t*)v_scale;
+    p.lengths = lengths, p.fresh = new_lengths, p.prefix = prefix_lengths, p.causal = 1;
+    p.y = y, p.parts = (float*)workspace;
+    const bool few = few_rows(N, H, G);
+    // one token's key and value are quantised on the way
+    if (N == 1 && few && !new_lengths) {
+        p.k_new = k, p.kn_sb = strides[3], p.kn_sg = strides[5];
+        p.v_new = v, p.vn_sb = strides[6], p.vn_sg = strides[8];
+    } else {
+        const int rc = flare_qcache_write(k, v, strides + 3, dtype, bits, B, N, M, G, D, lengths, new_lengths, k_cache,
+                                          k_scale, v_cache, v_scale, stream);
+        if (rc != FLARE_OK) return rc;
+    }
+    if (few) {
+        p.splits = rows_splits(B, N, M, H, G);
+        return FLARE_BY_DTYPE(dtype, qattn_rows, (p, bits, row_tiles(N, H, G), (hipStream_t)stream));
+    }
+    split_forward(p, dtype);
+    return FLARE_BY_DTYPE(dtype, qattn_forward, (p, bits, (hipStream_t)stream));
 }

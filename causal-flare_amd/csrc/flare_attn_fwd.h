@@ -14,10 +14,86 @@
 // transcendental instructions a pair) 260 us, 0.53.  32 queries a wave against 16: 275 and 285 us.
 #pragma once
 
-#include "flare_attn.h"
+#include "flare_qcache.h"
 
 namespace flare {
 namespace attn {
+
+// What Stage does, from a cache of 8 or 4 bits: codes to LDS as the values they stand for, a unit of 16 of
+// them a thread at a time.  Rows that are none, columns behind D, and blocks that are NaN where `clean` is
+// called, become 0.
+template <typename E, int BITS, int ROWS, int DP, int PITCH, int NT>
+struct CodeStage {
+    typedef typename Elem<E>::S S;
+    typedef typename Elem<E>::Frag Frag;
+    static constexpr int CPR = DP / 16, N = (ROWS * CPR + NT - 1) / NT, W8 = BITS / 4;    // W8: words of eight codes
+    u32 w[N][2 * W8], scale[N];
+    u32 at[N], scale_at[N], to[N];
+    // Adjacent threads' 32-byte results would meet in the same banks: every second four of them store their
+    // second half first.
+    u32 second;
+    __device__ __forceinline__ void begin(int64_t G, int64_t D, int tid) {
+        const u32 codes = (u32)(G * qcache::row_codes(D, BITS)), scales = (u32)(G * qcache::row_scales(D));
+        second = sizeof(E) == 2 ? tid >> 2 & 1 : 0;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int e = i * NT + tid, row = e / CPR, col = e % CPR * 16;
+            const bool there = e < ROWS * CPR && col < D;
+            at[i] = there ? row * codes + (u32)(col * BITS / 8) : 0x80000000u;
+            scale_at[i] = there ? row * scales + (u32)(col / qcache::kBlock) : 0x80000000u;
+            to[i] = row * PITCH + col;
+        }
+    }
+    // `first`, `first_scale`: row 0 of the tile; the `rows` of it that are there
+    __device__ __forceinline__ void load(const uint8_t* first, const uint8_t* first_scale, int rows, int64_t G, int64_t D) {
+        const int n = min(rows, ROWS);
+        const int codes = (int)qcache::row_codes(D, BITS), scales = (int)qcache::row_scales(D);
+        const int bytes = n > 0 ? (n - 1) * (int)G * codes + codes : 0, sbytes = n > 0 ? (n - 1) * (int)G * scales + scales : 0;
+        const auto rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(first), 0, bytes, 0x00020000);
+        const auto ssrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(first_scale), 0, sbytes, 0x00020000);
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            if constexpr (BITS == 4) {
+                const u32x2 r = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(rsrc, at[i], 0, 0));
+                w[i][0] = r[0], w[i][1] = r[1];
+            } else {
+                const u32x4 r = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rsrc, at[i], 0, 0));
+#pragma unroll
+                for (int j = 0; j < 4; ++j) w[i][j] = r[j];
+            }
+            scale[i] = (u32)(uint8_t)__builtin_amdgcn_raw_buffer_load_b8(ssrc, scale_at[i], 0, 0);
+        }
+    }
+    __device__ __forceinline__ void store(S* lds, int tid) const {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            if (ROWS * CPR % NT != 0 && i * NT + tid >= ROWS * CPR) continue;
+            const float f = qcache::scale_value(scale[i]);
+            u32 a[W8], b[W8];
+#pragma unroll
+            for (int j = 0; j < W8; ++j) a[j] = second ? w[i][W8 + j] : w[i][j], b[j] = second ? w[i][j] : w[i][W8 + j];
+            *reinterpret_cast<Frag*>(lds + to[i] + 8 * second) = qcache::decode<BITS>(a, f, S{});
+            *reinterpret_cast<Frag*>(lds + to[i] + 8 * (second ^ 1)) = qcache::decode<BITS>(b, f, S{});
+        }
+    }
+    __device__ __forceinline__ bool odd() const {
+        bool any = false;
+#pragma unroll
+        for (int i = 0; i < N; ++i) any |= scale[i] == qcache::kNoValue;
+        return any;
+    }
+    __device__ __forceinline__ void clean() {
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            if (scale[i] == qcache::kNoValue) scale[i] = 0;
+    }
+};
+template <bool Q, typename A, typename B> struct Either {
+    typedef A Type;
+};
+template <typename A, typename B> struct Either<false, A, B> {
+    typedef B Type;
+};
 
 // With weights of 2^(s - cap) a row's largest is at least 2^(-2 cap): bf16 holds that, with all that
 // counts beside it, and fp16 does not.  Up to here (log2 units; caps of 30.5) it is 2^-88 or more, and its
@@ -33,7 +109,8 @@ struct ForwardLds {
     static constexpr size_t bytes = 2 * (k_bytes + v_bytes + KT * sizeof(int)) + sizeof(int);
 };
 
-template <typename E, int DP, int QT, int KT, int CAP>
+// BITS: of a cache of 8 or 4 bits (and no `ids`), 0 for keys and values of the queries' type.
+template <typename E, int DP, int QT, int KT, int CAP, int BITS>
 __global__ __launch_bounds__(256, 2) void attn_forward_kernel(AttnArgs p) {
     typedef typename Elem<E>::S S;
     typedef typename Elem<E>::Frag Frag;
@@ -110,6 +187,9 @@ __global__ __launch_bounds__(256, 2) void attn_forward_kernel(AttnArgs p) {
     }
     const S* kbase = (const S*)p.k.p + b * p.k.sb + kvh * p.k.sh;
     const S* vbase = (const S*)p.v.p + b * p.v.sb + kvh * p.v.sh;
+    // of a cache of codes: its row of position 0
+    const int64_t code_row = b * p.M * p.G + kvh, codes = qcache::row_codes(p.D, BITS), scales = qcache::row_scales(p.D);
+    const uint8_t* vscale = p.v_scale + code_row * scales;
     const float scale2 = fabsf(p.scale) * kLog2e, slope2 = p.slopes ? p.slopes[h] * kLog2e : 0.0f;
     const float cap2 = p.cap * kLog2e, to_tanh = CAP ? fabsf(p.scale) / p.cap : 0.0f, into_cap = 2.0f * kLog2e * to_tanh;
 
@@ -128,14 +208,21 @@ __global__ __launch_bounds__(256, 2) void attn_forward_kernel(AttnArgs p) {
         if (p.causal && k0 + KT - 1 > first + off && k0 + KT > prefix) return false;
         return !p.ids || mine.same(id_range(p, b, k0 / kIdTile));
     };
-    Stage<E, KT, DP, KP, 256> ks;
-    Stage<E, KT, DP, VP, 256> vs;
-    ks.begin(p.k.sn, p.D, tid);
-    vs.begin(p.v.sn, p.D, tid);
+    constexpr int CODED = BITS ? BITS : 8;
+    typename Either<BITS != 0, CodeStage<E, CODED, KT, DP, KP, 256>, Stage<E, KT, DP, KP, 256>>::Type ks;
+    typename Either<BITS != 0, CodeStage<E, CODED, KT, DP, VP, 256>, Stage<E, KT, DP, VP, 256>>::Type vs;
+    ks.begin(BITS ? p.G : p.k.sn, p.D, tid);
+    vs.begin(BITS ? p.G : p.v.sn, p.D, tid);
     int next_id = -1;
     auto fetch = [&](int k0) {
-        ks.load(kbase + k0 * p.k.sn, kvlen - k0, p.k.sn, p.D);
-        vs.load(vbase + k0 * p.v.sn, kvlen - k0, p.v.sn, p.D);
+        if constexpr (BITS != 0) {
+            const int64_t row = code_row + k0 * p.G;
+            ks.load((const uint8_t*)p.k.p + row * codes, p.k_scale + row * scales, kvlen - k0, p.G, p.D);
+            vs.load((const uint8_t*)p.v.p + row * codes, p.v_scale + row * scales, kvlen - k0, p.G, p.D);
+        } else {
+            ks.load(kbase + k0 * p.k.sn, kvlen - k0, p.k.sn, p.D);
+            vs.load(vbase + k0 * p.v.sn, kvlen - k0, p.v.sn, p.D);
+        }
         if (p.ids && tid < KT) next_id = max(k0 + tid < (int)p.N ? p.ids[b * p.N + k0 + tid] : kNoKey, kNoKey);
     };
     auto place = [&](int k0, int buf) {
@@ -300,7 +387,10 @@ __global__ __launch_bounds__(256, 2) void attn_forward_kernel(AttnArgs p) {
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
                             if (16 * d >= p.D) continue;
-                            const float v = (float)vbase[j * p.v.sn + 16 * d + 4 * g + e];
+                            float v;
+                            if constexpr (BITS != 0)
+                                v = vscale[j * p.G * scales + d / 2] == qcache::kNoValue ? __builtin_nanf("") : 0.0f;
+                            else v = (float)vbase[j * p.v.sn + 16 * d + 4 * g + e];
                             if (!(fabsf(v) < -kNegInf)) acc[t][d][e] += v;
                         }
                     }
@@ -364,11 +454,11 @@ __global__ __launch_bounds__(256) void attn_rows_kernel(AttnArgs p) {
     if (p.lse && d == 0) p.lse[row] = sees ? j.top + __builtin_amdgcn_logf(j.total) : -kNegInf;
 }
 
-template <typename E, int DP, int CAP>
+template <typename E, int DP, int CAP, int BITS>
 static int forward_cap(const AttnArgs& p, hipStream_t stream) {
     constexpr int QT = q_tiles(sizeof(E)), KT = sizeof(E) == 2 ? 64 : 32;
     constexpr size_t bytes = ForwardLds<E, DP, KT>::bytes;
-    auto kernel = attn_forward_kernel<E, DP, QT, KT, CAP>;
+    auto kernel = attn_forward_kernel<E, DP, QT, KT, CAP, BITS>;
     if (bytes > 65536) {
         const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
                                                  hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
@@ -384,22 +474,24 @@ static int forward_cap(const AttnArgs& p, hipStream_t stream) {
     attn_rows_kernel<E><<<dim3((unsigned)ceil_div(p.B * p.H * p.N, 8)), 256, 0, stream>>>(p);
     return check_launch("attn_rows");
 }
-template <typename E, int DP>
+template <typename E, int DP, int BITS>
 static int forward_dp(const AttnArgs& p, hipStream_t stream) {
-    if (p.cap == 0.0f) return forward_cap<E, DP, kNoCap>(p, stream);
+    if (p.cap == 0.0f) return forward_cap<E, DP, kNoCap, BITS>(p, stream);
     if constexpr (__is_same(E, __hip_bfloat16))
-        if (!p.slopes && p.cap * kLog2e <= kCapFixedMost) return forward_cap<E, DP, kCapFixed>(p, stream);
+        if (!p.slopes && p.cap * kLog2e <= kCapFixedMost) return forward_cap<E, DP, kCapFixed, BITS>(p, stream);
     if constexpr (sizeof(E) == 2)
-        if (p.cap <= kCoarseCapMost) return forward_cap<E, DP, kCap>(p, stream);
-    return forward_cap<E, DP, kCapFine>(p, stream);
+        if (p.cap <= kCoarseCapMost) return forward_cap<E, DP, kCap, BITS>(p, stream);
+    return forward_cap<E, DP, kCapFine, BITS>(p, stream);
+}
+template <typename E, int BITS>
+int forward_bits(const AttnArgs& p, hipStream_t stream) {
+    return p.D <= 32   ? forward_dp<E, 32, BITS>(p, stream)
+           : p.D <= 64 ? forward_dp<E, 64, BITS>(p, stream)
+           : p.D <= 96 ? forward_dp<E, 96, BITS>(p, stream)
+                       : forward_dp<E, 128, BITS>(p, stream);
 }
 template <typename E>
-int forward_e(const AttnArgs& p, hipStream_t stream) {
-    return p.D <= 32   ? forward_dp<E, 32>(p, stream)
-           : p.D <= 64 ? forward_dp<E, 64>(p, stream)
-           : p.D <= 96 ? forward_dp<E, 96>(p, stream)
-                       : forward_dp<E, 128>(p, stream);
-}
+int forward_e(const AttnArgs& p, hipStream_t stream) { return forward_bits<E, 0>(p, stream); }
 
 }  // namespace attn
 }  // namespace flare

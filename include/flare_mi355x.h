@@ -431,6 +431,42 @@ int flare_attn_step(const void* q, const void* k, const void* v, const int64_t* 
                     const int32_t* lengths, void* k_cache, void* v_cache, void* y, void* workspace,
                     size_t workspace_bytes, void* stream);
 
+/*
+ * Rotary positions.  q [B, N, H, D] and k [B, N, G, D] or NULL (strides: batch, token and head of q, k; 6
+ * numbers, host) to contiguous q_out, k_out: pair i of the first R dimensions (i and i + R/2; interleaved: 2i
+ * and 2i + 1) is turned by position * frequencies[i] (radians; R/2 numbers, host), the other way if inverse (the
+ * gradient).  The position of token t is positions[b, t], or lengths[b] + t, or t where both are NULL.
+ * D up to 256.
+ */
+int flare_rotary(const void* q, const void* k, const int64_t* strides, int dtype, int64_t B, int64_t N, int64_t H,
+                 int64_t G, int64_t D, int64_t R, const double* frequencies, const int32_t* positions,
+                 const int32_t* lengths, int interleaved, int inverse, void* q_out, void* k_out, void* stream);
+
+/*
+ * A cache of keys and values in 8 or 4 bits: codes [B, M, G, D bits / 8] (16-byte aligned) and a byte e + 127
+ * for each 32 dimensions of a row, [B, M, G, ceil(D / 32)].  A value is its code (e4m3, or e2m1 with the
+ * lower index in the lower half of a byte) times 2^e, e the least (within the type's range) for which the
+ * block's largest value rounds to no more than the largest code; 255: the block held an infinite value or a
+ * NaN and is NaN.  flare_qcache_write is flare_attn_append for it; flare_qcache_read gives the values of rows
+ * first[b] (0 if NULL) .. + N - 1 of each sequence as k, v [B, N, G, D], 0 for rows outside of 0 .. M - 1.
+ */
+int flare_qcache_write(const void* k, const void* v, const int64_t* strides, int dtype, int bits, int64_t B, int64_t N,
+                       int64_t M, int64_t G, int64_t D, const int32_t* lengths, const int32_t* new_lengths, void* k_cache,
+                       void* k_scale, void* v_cache, void* v_scale, void* stream);
+int flare_qcache_read(const void* k_cache, const void* k_scale, const void* v_cache, const void* v_scale, int dtype,
+                      int bits, int64_t B, int64_t N, int64_t M, int64_t G, int64_t D, const int32_t* first, void* k,
+                      void* v, void* stream);
+
+/* Softmax attention of N new tokens a sequence over such a cache, which receives their k and v [B, N, G, D] first
+ * (strides: batch, token and head of q, k, v; 9 numbers, host): the rows are seen as the cache holds them.
+ * lengths, new_lengths, prefix_lengths and y as for flare_attn_append and flare_attn_forward. */
+size_t flare_qattn_workspace_size(int64_t B, int64_t N, int64_t M, int64_t H, int64_t G, int64_t D, int dtype);
+int flare_qattn(const void* q, const void* k, const void* v, const int64_t* strides, int dtype, int bits, int64_t B,
+                int64_t N, int64_t M, int64_t H, int64_t G, int64_t D, float scale, float softcap, const float* slopes,
+                const int32_t* prefix_lengths, const int32_t* lengths, const int32_t* new_lengths, void* k_cache,
+                void* k_scale, void* v_cache, void* v_scale, void* y, void* workspace, size_t workspace_bytes,
+                void* stream);
+
 #ifdef __cplusplus
 }
 #endif
