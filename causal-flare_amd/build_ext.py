@@ -44,6 +44,7 @@ FILE_FLAGS = {
     "flare_ar_pc.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
     **{f"flare_wave_{k}.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form", "-Werror=pass-failed"]
        for k in ("f32", "bf16", "f16", "bwd_f32", "bwd_bf16", "bwd_f16")},
+    **{f"flare_qattn_{k}_{bits}.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"] for k in ("f32", "bf16", "f16") for bits in (4, 8)},
 }
 
 

@@ -73,7 +73,8 @@ struct AttnArgs {
     const float* norms;              // [B, H, N]: sum of |dy| (fp16)
     const float* ranges;             // [B, tiles, 2]: of 64 tokens the largest norm and |v| (fp16)
     void *dq, *dk, *dv;
-    int64_t row_splits;              // of `splits`: parts of the rows, times parts of the heads
+    int64_t row_splits;              // of `splits`: parts of the rows, times parts of the heads; over a cache of 8 or 4
+                                     // bits: key heads of the same tokens that a workgroup's waves take side by side
     float* dq_parts;                 // what `dq_splits` workgroups leave of each row of dq
     int64_t dq_splits;
     // single tokens

@@ -172,12 +172,19 @@ static int64_t step_splits(int64_t B, int64_t M, int64_t H, int64_t G) {
 
 // A few new tokens over a cache of 8 or 4 bits: rows (token, head) of the heads that share keys.
 constexpr int64_t kFewRows = 64;
-static int row_tiles(int64_t N, int64_t H, int64_t G) { return H / G * N > 16 ? 2 : 1; }
+static int row_tiles(int64_t N, int64_t H, int64_t G, int dtype) { return H / G * N > 16 && dtype != FLARE_F32 ? 2 : 1; }
 static bool few_rows(int64_t N, int64_t H, int64_t G) { return H / G * N <= kFewRows; }
-// Workgroups for each sequence's keys, as step_splits: 
-static int64_t rows_splits(int64_t B, int64_t N, int64_t M, int64_t H, int64_t G) {
-    const int64_t rows = B * G * ceil_div(H / G * N, 16 * row_tiles(N, H, G));
-    const int64_t s = ceil_div(512, rows), most = ceil_div(M, 256);
+// Key heads of the same tokens that the waves of a workgroup take side by side.
+static int64_t rows_heads(int64_t B, int64_t N, int64_t H, int64_t G, int tiles) {
+    if (tiles > 1 || B * G < 128) return 1;
+    return G % 4 == 0 ? 4 : G % 2 == 0 ? 2 : 1;
+}
+// Workgroups for each sequence's keys, as step_splits.
+static int64_t rows_splits(int64_t B, int64_t N, int64_t M, int64_t H, int64_t G, int dtype, int bits) {
+    const int tiles = row_tiles(N, H, G, dtype);
+    const int64_t heads = rows_heads(B, N, H, G, tiles);
+    const int64_t rows = B * (G / heads) * ceil_div(H / G * N, 16 * tiles);
+    const int64_t s = ceil_div(tiles == 1 ? 768 : 512, rows), most = ceil_div(M, 256 / heads);
     return s < 1 ? 1 : (s > most ? most : s);
 }
 template <typename E>
@@ -353,10 +360,11 @@ extern "C" int flare_attn_step(const void* q, const void* k, const void* v, cons
     return attn_step(p, dtype, (hipStream_t)stream);
 }
 
-extern "C" size_t flare_qattn_workspace_size(int64_t B, int64_t N, int64_t M, int64_t H, int64_t G, int64_t D, int dtype) {
+extern "C" size_t flare_qattn_workspace_size(int64_t B, int64_t N, int64_t M, int64_t H, int64_t G, int64_t D, int dtype,
+                                             int bits) {
     if (B < 1 || N < 1 || M < 1 || H < 1 || G < 1 || H % G) return 0;
     if (few_rows(N, H, G)) {
-        const int64_t s = rows_splits(B, N, M, H, G);
+        const int64_t s = rows_splits(B, N, M, H, G, dtype, bits);
         return s == 1 ? 0 : (size_t)(B * N * H * s * (D + 4)) * sizeof(float);
     }
     AttnArgs p = {};
@@ -379,7 +387,7 @@ extern "C" int flare_qattn(const void* q, const void* k, const void* v, const in
     const uintptr_t held = (uintptr_t)k_cache | (uintptr_t)v_cache | (uintptr_t)y;
     FLARE_REQUIRE(aligned(p.q, dtype) && aligned(kr, dtype) && aligned(vr, dtype) && (held & 15) == 0,
                   "flare_qattn: rows must be 16-byte aligned and less than 2^22 elements apart");
-    if (workspace_bytes < flare_qattn_workspace_size(B, N, M, H, G, D, dtype) ||
+    if (workspace_bytes < flare_qattn_workspace_size(B, N, M, H, G, D, dtype, bits) ||
         (workspace_bytes && (!workspace || ((uintptr_t)workspace & 15)))) {
         set_error("flare_qattn: workspace of %zu bytes is too small or not 16-byte aligned", workspace_bytes);
         return FLARE_ERR_WORKSPACE;
@@ -398,8 +406,8 @@ extern "C" int flare_qattn(const void* q, const void* k, const void* v, const in
         if (rc != FLARE_OK) return rc;
     }
     if (few) {
-        p.splits = rows_splits(B, N, M, H, G);
-        return FLARE_BY_DTYPE(dtype, qattn_rows, (p, bits, row_tiles(N, H, G), (hipStream_t)stream));
+        p.splits = rows_splits(B, N, M, H, G, dtype, bits), p.row_splits = rows_heads(B, N, H, G, row_tiles(N, H, G, dtype));
+        return FLARE_BY_DTYPE(dtype, qattn_rows, (p, bits, row_tiles(N, H, G, dtype), (hipStream_t)stream));
     }
     split_forward(p, dtype);
     return FLARE_BY_DTYPE(dtype, qattn_forward, (p, bits, (hipStream_t)stream));

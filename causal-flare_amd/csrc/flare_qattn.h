@@ -57,8 +57,36 @@ __device__ __forceinline__ void three_parts(float x, bf16& a, bf16& b, bf16& c) 
     c = odd ? (bf16)0.0f : (bf16)(rest - mid);
 }
 
+// W dwords from `offset` bytes of a buffer, 0 where that lies behind its end.
+typedef __amdgpu_buffer_rsrc_t Buffer;
+__device__ __forceinline__ Buffer buffer_of(const uint8_t* p, int bytes) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(p), 0, bytes, 0x00020000);
+}
+template <int W>
+__device__ __forceinline__ void load_words(Buffer from, u32 offset, u32* to) {
+    if constexpr (W >= 4) {
+        const u32x4 r = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(from, offset, 0, 0));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) to[i] = r[i];
+        if constexpr (W > 4) load_words<W - 4>(from, offset + 16, to + 4);
+    } else if constexpr (W == 3) {
+        typedef u32 u32x3 __attribute__((ext_vector_type(3)));
+        const u32x3 r = __builtin_bit_cast(u32x3, __builtin_amdgcn_raw_buffer_load_b96(from, offset, 0, 0));
+        to[0] = r[0], to[1] = r[1], to[2] = r[2];
+    } else if constexpr (W == 2) {
+        const u32x2 r = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(from, offset, 0, 0));
+        to[0] = r[0], to[1] = r[1];
+    } else {
+        to[0] = __builtin_bit_cast(u32, __builtin_amdgcn_raw_buffer_load_b32(from, offset, 0, 0));
+    }
+}
+constexpr u32 kNowhere = 0x80000000u;        // an offset behind every buffer's end
+
+// Waves a SIMD: as many as the registers of a tile of scores, its codes and the sums leave.
+constexpr int rows_waves(int size, int bits, int tiles) { return tiles == 2 || size == 4 ? 2 : bits == 4 ? 4 : 3; }
+
 template <typename E, int BITS, int DP, int CAP, int RT>
-__global__ __launch_bounds__(256) void qattn_rows_kernel(AttnArgs p) {
+__global__ __launch_bounds__(256, rows_waves(sizeof(E), BITS, RT)) void qattn_rows_kernel(AttnArgs p) {
     typedef typename Elem<E>::S S;
     typedef typename Held<E>::Type HE;                 // what the products take
     typedef typename Elem<HE>::S HS;
@@ -66,78 +94,171 @@ __global__ __launch_bounds__(256) void qattn_rows_kernel(AttnArgs p) {
     using Lds = RowsLds<DP>;
     constexpr int PARTS = Held<E>::parts;
     constexpr int DK = DP / 32, DT = DP / 16, NB = DP / kBlock, P = Lds::P;
-    constexpr int TK = BITS == 4 && RT == 1 ? 64 : 32, NM = TK / 16, W8 = BITS / 4;      // W8: words of eight codes
+    constexpr int TK = 32, NM = TK / 16, W8 = BITS / 4;                                  // W8: words of eight codes
     constexpr int NSC = DK == 3 ? 3 : 1;               // blocks that a lane's dimensions of K may lie in
-    constexpr int NVH = (32 * NB + 63) / 64;           // blocks of V a lane takes, of 32 keys
+    constexpr int NV = (TK * NB + 63) / 64;            // blocks of V a lane takes
     extern __shared__ __align__(16) char smem[];
-    __shared__ u32 new_codes[2][4 * BITS];
-    __shared__ u32 new_scales[2][4];
+    __shared__ u32 new_codes[4][2][4 * BITS];
+    __shared__ u32 new_scales[4][2][4];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int g = lane >> 4, c = lane & 15;
-    const int D = (int)p.D;
-    const int64_t R = p.H / p.G, rows = R * p.N, groups = (rows + 16 * RT - 1) / (16 * RT);
-    const int64_t split = blockIdx.x % (unsigned)p.splits, id = blockIdx.x / (unsigned)p.splits;
-    const int64_t group = id % groups, kvh = id / groups % p.G, b = id / groups / p.G;
+    const unsigned D = (unsigned)p.D, G = (unsigned)p.G, H = (unsigned)p.H, N = (unsigned)p.N, splits = (unsigned)p.splits;
+    const unsigned R = H / G, rows = R * N, groups = (rows + 16 * RT - 1) / (16 * RT);
+    // of the workgroup's waves, and of this one
+    const unsigned heads = (unsigned)p.row_splits, shares = 4 / heads, head = wave % heads, part = wave / heads, sets = G / heads;
+    // workgroups of the same tokens are 8 apart: one XCD, as their rows share lines of its L2
+    const unsigned kvh0 = blockIdx.x / 8 % sets * heads, kvh = kvh0 + head, unit = blockIdx.x / (8 * sets) * 8 + blockIdx.x % 8;
+    const unsigned split = unit % splits, group = unit / splits % groups, b = unit / (splits * groups);
+    if (b >= (unsigned)p.B) return;
     const bool single = p.k_new != nullptr;            // its key and value are not in the cache yet
-    int64_t off = p.lengths[b];
-    const int64_t fresh = p.fresh ? clamp_to(p.fresh[b], p.N) : p.N;
-    if (off < 0 || off + fresh > p.M) {
+    const int off = p.lengths[b], fresh = p.fresh ? min(max(p.fresh[b], 0), (int)N) : (int)N;
+    S* y = (S*)p.y + (int64_t)b * N * H * D;
+    if (off < 0 || (int64_t)off + fresh > p.M) {
         // an idle sequence, or a full cache
-        if (p.splits == 1) {
-            for (int i = tid; i < 16 * RT * D; i += 256) {
-                const int64_t r = group * 16 * RT + i / D;
-                if (r < rows)
-                    ((S*)p.y)[((b * p.N + r / R) * p.H + kvh * R + r % R) * D + i % D] =
-                        (S)(off < 0 ? 0.0f : __builtin_nanf(""));
+        if (splits == 1) {
+            for (unsigned i = lane + 64 * part; i < 16 * RT * D; i += 64 * shares) {
+                const unsigned r = group * 16 * RT + i / D;
+                if (r < rows) y[((int64_t)(r / R) * H + kvh * R + r % R) * D + i % D] = (S)(off < 0 ? 0.0f : __builtin_nanf(""));
             }
         }
         return;
     }
-    const int64_t n = off + fresh, prefix = p.prefix ? clamp_to(p.prefix[b], n) : 0;
-    const int64_t per = ((n + p.splits - 1) / p.splits + 4 * TK - 1) / (4 * TK) * (4 * TK);
-    const int64_t first = split * per, last = min(first + per, n);
-    const int64_t held = single ? min(last, off) : last;       // what of it memory holds
-    const int64_t codes = qcache::row_codes(D, BITS), scales = qcache::row_scales(D);
-    uint8_t* kc = (uint8_t*)p.k.p + (b * p.M * p.G + kvh) * codes;
-    uint8_t* vc = (uint8_t*)p.v.p + (b * p.M * p.G + kvh) * codes;
-    uint8_t* ksc = p.k_scale + (b * p.M * p.G + kvh) * scales;
-    uint8_t* vsc = p.v_scale + (b * p.M * p.G + kvh) * scales;
-    const int64_t stride = p.G * codes, scale_stride = p.G * scales;
+    const int n = off + fresh, prefix = p.prefix ? min(max(p.prefix[b], 0), n) : 0;
+    const int step = (int)shares * TK;
+    const unsigned share = ((unsigned)n + splits - 1) / splits;
+    const int per = (int)((share + step - 1) / step * step);
+    const int first = (int)min((int64_t)split * per, (int64_t)n), last = (int)min((int64_t)first + per, (int64_t)n);
+    const int held = single ? min(last, off) : last;           // what of it memory holds
+    const unsigned codes = D * BITS / 8, scales = (D + kBlock - 1) / kBlock;
+    const unsigned stride = G * codes, scale_stride = G * scales;
+    const int64_t row0 = (int64_t)b * p.M * G + kvh;
+    const uint8_t* kc = (const uint8_t*)p.k.p + row0 * codes;
+    const uint8_t* vc = (const uint8_t*)p.v.p + row0 * codes;
+    const uint8_t* ksc = p.k_scale + row0 * scales;
+    const uint8_t* vsc = p.v_scale + row0 * scales;
 
-    // the single token's key and value: a quad of lanes a block
+    // the single token's keys and values: a quad of lanes a block
     if (single && first <= off && off < last) {
-        if (tid < 8 * NB) {
-            const int which = tid / (4 * NB), block = tid / 4 % NB, d = block * kBlock + (tid & 3) * 8;
-            const S* from = which ? (const S*)p.v_new + b * p.vn_sb + kvh * p.vn_sg
-                                  : (const S*)p.k_new + b * p.kn_sb + kvh * p.kn_sg;
+        if (tid < (int)heads * 8 * NB) {
+            const unsigned at = tid / (8 * NB), value = tid / (4 * NB) % 2, block = tid / 4 % NB, d = block * kBlock + (tid & 3) * 8;
+            const S* from = value ? (const S*)p.v_new + b * p.vn_sb + (kvh0 + at) * p.vn_sg
+                                  : (const S*)p.k_new + b * p.kn_sb + (kvh0 + at) * p.kn_sg;
             float x[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
             if (d < D) qcache::load8(reinterpret_cast<const E*>(from) + d, x);
             const u32 byte = qcache::scale_of<BITS>(qcache::quad_max(qcache::top_of(x)), __is_same(E, __half));
             const Codes<BITS> w = qcache::encode<BITS>(x, byte);
 #pragma unroll
-            for (int i = 0; i < W8; ++i) new_codes[which][d / 8 * W8 + i] = w.w[i];
-            if ((tid & 3) == 0) new_scales[which][block] = byte;
+            for (int i = 0; i < W8; ++i) new_codes[at][value][d / 8 * W8 + i] = w.w[i];
+            if ((tid & 3) == 0) new_scales[at][value][block] = byte;
             if (group == 0 && d < D) {
-                *reinterpret_cast<Codes<BITS>*>((which ? vc : kc) + off * stride + d * BITS / 8) = w;
-                if ((tid & 3) == 0) (which ? vsc : ksc)[off * scale_stride + block] = (uint8_t)byte;
+                const int64_t row = ((int64_t)b * p.M + off) * G + kvh0 + at;
+                *reinterpret_cast<Codes<BITS>*>((uint8_t*)(value ? p.v.p : p.k.p) + row * codes + d * BITS / 8) = w;
+                if ((tid & 3) == 0) (value ? p.v_scale : p.k_scale)[row * scales + block] = (uint8_t)byte;
             }
         }
         __syncthreads();
     }
+
+    HS* vt = (HS*)(smem + wave * Lds::v_bytes);
+    const bool full = D == DP;
+    u32 kw[NM][DK * W8], kb[NM][NSC];                  // codes and scales of the tile that is next
+    u32 vw[NV][BITS], vb[NV];
+    // key and block of V of this lane's unit i: keys 0, 2, 1, 3 follow each other, as rows two apart
+    // lie half the banks apart
+    auto unit_key = [&](int i) {
+        const int t = (i * 64 + lane) / NB;
+        return (t & ~3) | (t & 1) << 1 | (t >> 1 & 1);
+    };
+    auto unit_block = [&](int i) { return (i * 64 + lane) % NB; };
+    auto unit_there = [&](int i) { return TK * NB % 64 == 0 || i * 64 + lane < TK * NB; };
+    // a lane's offsets within a tile
+    u32 k_at[DK], ks_at[NSC], v_at[NV], vs_at[NV];
+#pragma unroll
+    for (int kk = 0; kk < DK; ++kk) {
+        const unsigned d = 8 * (DK * g + kk);
+        k_at[kk] = d < D ? c * stride + d * BITS / 8 : kNowhere;
+    }
+#pragma unroll
+    for (int i = 0; i < NSC; ++i) {
+        const unsigned block = 8 * (DK * g + i) / kBlock;
+        ks_at[i] = block < scales ? c * scale_stride + block : kNowhere;
+    }
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const unsigned block = unit_block(i);
+        const bool there = unit_there(i) && block < scales;
+        v_at[i] = there ? unit_key(i) * stride + block * (4 * BITS) : kNowhere;
+        vs_at[i] = there ? unit_key(i) * scale_stride + block : kNowhere;
+    }
+    // a last block of V may have half the values
+    bool half[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) half[i] = (unsigned)(unit_block(i) + 1) * kBlock > D;
+    auto fetch = [&](int k0) {
+        // (as scalars: a buffer whose size the compiler holds in a vector register costs a loop a load)
+        const int there = __builtin_amdgcn_readfirstlane(min(max(held - k0, 0), TK));
+        const int64_t at = k0;
+        const int bytes = there ? (there - 1) * (int)stride + (int)codes : 0;
+        const int sbytes = there ? (there - 1) * (int)scale_stride + (int)scales : 0;
+        const Buffer kr = buffer_of(kc + at * stride, bytes), vr = buffer_of(vc + at * stride, bytes);
+        const Buffer kr_s = buffer_of(ksc + at * scale_stride, sbytes), vr_s = buffer_of(vsc + at * scale_stride, sbytes);
+#pragma unroll
+        for (int m = 0; m < NM; ++m) {
+            if (full) {
+                load_words<DK * W8>(kr, k_at[0] + 16 * m * stride, kw[m]);
+            } else {
+#pragma unroll
+                for (int kk = 0; kk < DK; ++kk) load_words<W8>(kr, k_at[kk] + 16 * m * stride, &kw[m][kk * W8]);
+            }
+#pragma unroll
+            for (int i = 0; i < NSC; ++i)
+                kb[m][i] = (u32)(uint8_t)__builtin_amdgcn_raw_buffer_load_b8(kr_s, ks_at[i] + 16 * m * scale_stride, 0, 0);
+        }
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            if (full) {
+                load_words<BITS>(vr, v_at[i], vw[i]);
+            } else {
+                load_words<BITS / 2>(vr, v_at[i], vw[i]);
+                load_words<BITS / 2>(vr, half[i] ? kNowhere : v_at[i] + 2 * BITS, vw[i] + BITS / 2);
+            }
+            vb[i] = (u32)(uint8_t)__builtin_amdgcn_raw_buffer_load_b8(vr_s, vs_at[i], 0, 0);
+        }
+    };
+    // the single token's codes, for the lanes that take its place
+    auto insert = [&](int k0) {
+#pragma unroll
+        for (int m = 0; m < NM; ++m) {
+            if (k0 + 16 * m + c != off) continue;
+#pragma unroll
+            for (int i = 0; i < DK * W8; ++i) kw[m][i] = new_codes[head][0][DK * W8 * g + i];
+#pragma unroll
+            for (int i = 0; i < NSC; ++i) kb[m][i] = new_scales[head][0][8 * (DK * g + i) / kBlock];
+        }
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            if (!unit_there(i) || k0 + unit_key(i) != off) continue;
+#pragma unroll
+            for (int w = 0; w < BITS; ++w) vw[i][w] = new_codes[head][1][unit_block(i) * BITS + w];
+            vb[i] = new_scales[head][1][unit_block(i)];
+        }
+    };
+    const int begin = first + (int)part * TK;
+    if (begin < last) fetch(begin);
 
     Frag qf[RT][PARTS][DK];
     float slope2[RT];
     int lim[RT], pos[RT];                              // of this lane's rows: the keys it sees are below, and its place
 #pragma unroll
     for (int t = 0; t < RT; ++t) {
-        const int64_t r = group * 16 * RT + 16 * t + c, token = r / R, h = kvh * R + r % R;
-        const bool live = r < rows && token < fresh;
-        pos[t] = (int)(off + token);
-        lim[t] = live ? (int)min(n, max(off + token + 1, prefix)) : 0;
+        const unsigned r = group * 16 * RT + 16 * t + c, token = r / R, h = kvh * R + r % R;
+        const bool live = r < rows && (int)token < fresh;
+        pos[t] = off + (int)token;
+        lim[t] = live ? min(n, max(pos[t] + 1, prefix)) : 0;
         slope2[t] = p.slopes && live ? p.slopes[h] * kLog2e : 0.0f;
 #pragma unroll
         for (int kk = 0; kk < DK; ++kk) {
-            const int d = 8 * (DK * g + kk);
+            const unsigned d = 8 * (DK * g + kk);
 #pragma unroll
             for (int i = 0; i < PARTS; ++i) qf[t][i][kk] = Frag{};
             if (!live || d >= D) continue;
@@ -167,83 +288,7 @@ __global__ __launch_bounds__(256) void qattn_rows_kernel(AttnArgs p) {
         for (int d = 0; d < DT; ++d) acc[t][d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     }
 
-    HS* vt = (HS*)(smem + wave * Lds::v_bytes);
-    const bool full = D == DP;
-    u32 kw[NM][DK * W8], kb[NM][NSC];
-    u32 vw[NM / 2][NVH][BITS], vb[NM / 2][NVH];
-    // key (of 32) and block of V of this lane's unit i: keys 0, 2, 1, 3 follow each other, as rows two apart
-    // lie half the banks apart
-    auto unit_key = [&](int i) {
-        const int t = (i * 64 + lane) / NB;
-        return (t & ~3) | (t & 1) << 1 | (t >> 1 & 1);
-    };
-    auto unit_block = [&](int i) { return (i * 64 + lane) % NB; };
-    auto fetch = [&](int64_t k0) {
-#pragma unroll
-        for (int m = 0; m < NM; ++m) {
-            const int64_t j = k0 + 16 * m + c;
-            const bool there = j < held;
-            const uint8_t* row = kc + j * stride + DK * W8 * 4 * g;
-#pragma unroll
-            for (int i = 0; i < DK * W8; ++i) kw[m][i] = 0;
-            if (full) {
-                if (there) __builtin_memcpy(kw[m], __builtin_assume_aligned(row, 4), sizeof(kw[m]));
-            } else {
-#pragma unroll
-                for (int kk = 0; kk < DK; ++kk)
-                    if (there && 8 * (DK * g + kk) < D)
-                        __builtin_memcpy(&kw[m][kk * W8], __builtin_assume_aligned(row + kk * W8 * 4, 4), W8 * 4);
-            }
-#pragma unroll
-            for (int i = 0; i < NSC; ++i) {
-                const int block = 8 * (DK * g + i) / kBlock;
-                kb[m][i] = there && block < scales ? ksc[j * scale_stride + block] : 0;
-            }
-        }
-#pragma unroll
-        for (int h = 0; h < NM / 2; ++h) {
-#pragma unroll
-            for (int i = 0; i < NVH; ++i) {
-                const int64_t j = k0 + 32 * h + unit_key(i);
-                const int block = unit_block(i), d = block * kBlock;
-                const bool there = i * 64 + lane < 32 * NB && j < held && d < D;
-                const uint8_t* row = vc + j * stride + block * (4 * BITS);
-#pragma unroll
-                for (int w = 0; w < BITS; ++w) vw[h][i][w] = 0;
-                if (there) {
-                    // a last block may have half the values
-                    if (full || d + kBlock <= D) __builtin_memcpy(vw[h][i], __builtin_assume_aligned(row, 8), 4 * BITS);
-                    else __builtin_memcpy(vw[h][i], __builtin_assume_aligned(row, 8), 2 * BITS);
-                }
-                vb[h][i] = there ? vsc[j * scale_stride + block] : 0;
-            }
-        }
-    };
-    // the single token's codes, for the lanes that take its place
-    auto insert = [&](int64_t k0) {
-#pragma unroll
-        for (int m = 0; m < NM; ++m) {
-            if (k0 + 16 * m + c != off) continue;
-#pragma unroll
-            for (int i = 0; i < DK * W8; ++i) kw[m][i] = new_codes[0][DK * W8 * g + i];
-#pragma unroll
-            for (int i = 0; i < NSC; ++i) kb[m][i] = new_scales[0][8 * (DK * g + i) / kBlock];
-        }
-#pragma unroll
-        for (int h = 0; h < NM / 2; ++h) {
-#pragma unroll
-            for (int i = 0; i < NVH; ++i) {
-                if (i * 64 + lane >= 32 * NB || k0 + 32 * h + unit_key(i) != off) continue;
-#pragma unroll
-                for (int w = 0; w < BITS; ++w) vw[h][i][w] = new_codes[1][unit_block(i) * BITS + w];
-                vb[h][i] = new_scales[1][unit_block(i)];
-            }
-        }
-    };
-
-    int64_t k0 = first + wave * TK;
-    if (k0 < last) fetch(k0);
-    for (; k0 < last; k0 += 4 * TK) {
+    for (int k0 = begin; k0 < last; k0 += step) {
         if (single && k0 <= off && off < k0 + TK) insert(k0);
         f32x4 s[RT][NM];
 #pragma unroll
@@ -259,53 +304,36 @@ __global__ __launch_bounds__(256) void qattn_rows_kernel(AttnArgs p) {
                     for (int t = 0; t < RT; ++t) s[t][m] = mma(a, qf[t][i][kk], s[t][m]);
             }
         }
-        // V's first 32 keys to LDS; the rest follow when these have been read
-        const int64_t now = k0;
-        const bool whole = single || (now + TK <= off + 1);        // every row sees all of these keys
-        auto place = [&](int h) {
-#pragma unroll
-            for (int i = 0; i < NVH; ++i) {
-                if (i * 64 + lane >= 32 * NB) continue;
-                float scale = qcache::scale_value(vb[h][i]);
-                if (!whole && vb[h][i] == kNoValue) scale = 0.0f;
-                HS* to = vt + unit_key(i) * P + 8 * unit_block(i);
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    *reinterpret_cast<Frag*>(to + e * 8 * NB) = qcache::decode<BITS>(&vw[h][i][e * W8], scale, HS{});
-            }
-        };
+        const bool whole = single || k0 + TK <= off + 1;           // every row sees all of these keys
         if (!whole) {
             bool odd = false;
 #pragma unroll
-            for (int h = 0; h < NM / 2; ++h)
-#pragma unroll
-                for (int i = 0; i < NVH; ++i) odd |= vb[h][i] == kNoValue;
+            for (int i = 0; i < NV; ++i) odd |= vb[i] == kNoValue;
             if (__any(odd)) {
                 // which rows see blocks that are NaN, as 0 times NaN is NaN to the others too
-                for (int64_t j = now; j < min(now + TK, last); ++j) {
+                for (int j = k0; j < min(k0 + TK, last); ++j) {
                     for (int i = 0; i < (int)scales; ++i) {
-                        if (vsc[j * scale_stride + i] != kNoValue) continue;
+                        if (vsc[(int64_t)j * scale_stride + i] != kNoValue) continue;
 #pragma unroll
                         for (int t = 0; t < RT; ++t)
                             if (j < lim[t]) lost[t] |= 1u << i;
                     }
                 }
+#pragma unroll
+                for (int i = 0; i < NV; ++i) vb[i] = vb[i] == kNoValue ? 0 : vb[i];
             }
         }
-        place(0);
-        u32 vw_rest[NM / 2][NVH][BITS], vb_rest[NM / 2][NVH];
-        if constexpr (NM > 2) {
 #pragma unroll
-            for (int h = 1; h < NM / 2; ++h) {
+        for (int i = 0; i < NV; ++i) {
+            if (!unit_there(i)) continue;
+            const float scale = qcache::scale_value(vb[i]);
+            HS* to = vt + unit_key(i) * P + 8 * unit_block(i);
 #pragma unroll
-                for (int i = 0; i < NVH; ++i) {
-                    vb_rest[h][i] = vb[h][i];
-#pragma unroll
-                    for (int w = 0; w < BITS; ++w) vw_rest[h][i][w] = vw[h][i][w];
-                }
-            }
+            for (int e = 0; e < 4; ++e)
+                *reinterpret_cast<Frag*>(to + e * 8 * NB) = qcache::decode<BITS>(&vw[i][e * W8], scale, HS{});
         }
-        if (k0 + 4 * TK < last) fetch(k0 + 4 * TK);
+        if (k0 + step < last) fetch(k0 + step);
+        Frag w[RT][PARTS];
 #pragma unroll
         for (int t = 0; t < RT; ++t) {
 #pragma unroll
@@ -320,14 +348,14 @@ __global__ __launch_bounds__(256) void qattn_rows_kernel(AttnArgs p) {
                 }
             }
             if (p.slopes) {
-                const float base = (float)(pos[t] - (int)now - 4 * g);
+                const float base = (float)(pos[t] - k0 - 4 * g);
 #pragma unroll
                 for (int m = 0; m < NM; ++m)
 #pragma unroll
                     for (int i = 0; i < 4; ++i) s[t][m][i] -= slope2[t] * fabsf(base - (float)(16 * m + i));
             }
-            if (!whole || now + TK > last) {
-                const int left = min(lim[t], (int)last) - (int)now - 4 * g;
+            if (!whole || k0 + TK > last) {
+                const int left = min(lim[t], last) - k0 - 4 * g;
 #pragma unroll
                 for (int m = 0; m < NM; ++m)
 #pragma unroll
@@ -354,55 +382,33 @@ __global__ __launch_bounds__(256) void qattn_rows_kernel(AttnArgs p) {
                 for (int i = 0; i < 4; ++i) s[t][m][i] = __builtin_amdgcn_exp2f(s[t][m][i] - ref);
                 sum[t] += (s[t][m][0] + s[t][m][1]) + (s[t][m][2] + s[t][m][3]);
             }
-        }
+            if constexpr (PARTS == 1) {
+                w[t][0] = frag_tiles(s[t][0], s[t][1], HS{});
+            } else {
 #pragma unroll
-        for (int h = 0; h < NM / 2; ++h) {
-            Frag w[RT][PARTS];
-#pragma unroll
-            for (int t = 0; t < RT; ++t) {
-                if constexpr (PARTS == 1) {
-                    w[t][0] = frag_tiles(s[t][2 * h], s[t][2 * h + 1], HS{});
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        bf16 u, v, x;
-                        three_parts(s[t][2 * h + e / 4][e % 4], u, v, x);
-                        w[t][0][e] = u, w[t][PARTS / 2][e] = v, w[t][PARTS - 1][e] = x;
-                    }
-                }
-            }
-            // the LDS of a wave is its own, and its operations stay in order
-            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-            __builtin_amdgcn_wave_barrier();
-#pragma unroll
-            for (int d = 0; d < DT; ++d) {
-                const Frag a = frag_columns<HE>(vt + 16 * d, P, g, c);
-#pragma unroll
-                for (int i = PARTS - 1; i >= 0; --i)
-#pragma unroll
-                    for (int t = 0; t < RT; ++t) acc[t][d] = mma(a, w[t][i], acc[t][d]);
-            }
-            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-            __builtin_amdgcn_wave_barrier();
-            if constexpr (NM > 2) {
-                if (h + 1 < NM / 2) {
-#pragma unroll
-                    for (int i = 0; i < NVH; ++i) {
-                        if (i * 64 + lane >= 32 * NB) continue;
-                        float scale = qcache::scale_value(vb_rest[h + 1][i]);
-                        if (!whole && vb_rest[h + 1][i] == kNoValue) scale = 0.0f;
-                        HS* to = vt + unit_key(i) * P + 8 * unit_block(i);
-#pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            *reinterpret_cast<Frag*>(to + e * 8 * NB) =
-                                qcache::decode<BITS>(&vw_rest[h + 1][i][e * W8], scale, HS{});
-                    }
+                for (int e = 0; e < 8; ++e) {
+                    bf16 u, v, x;
+                    three_parts(s[t][e / 4][e % 4], u, v, x);
+                    w[t][0][e] = u, w[t][PARTS / 2][e] = v, w[t][PARTS - 1][e] = x;
                 }
             }
         }
+        // the LDS of a wave is its own, and its operations stay in order
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int d = 0; d < DT; ++d) {
+            const Frag a = frag_columns<HE>(vt + 16 * d, P, g, c);
+#pragma unroll
+            for (int i = PARTS - 1; i >= 0; --i)
+#pragma unroll
+                for (int t = 0; t < RT; ++t) acc[t][d] = mma(a, w[t][i], acc[t][d]);
+        }
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
     }
 
-    // the four waves' shares of one tile of rows at a time: out [wave][row][DP + 2]
+    // the waves' shares of one tile of rows at a time: out [wave][row][DP + 2]
     float* out = (float*)smem;
 #pragma unroll
     for (int t = 0; t < RT; ++t) {
@@ -423,31 +429,38 @@ __global__ __launch_bounds__(256) void qattn_rows_kernel(AttnArgs p) {
             mine[DP + 1] = total;
         }
         __syncthreads();
-        for (int i = tid; i < 16 * DP; i += 256) {
-            const int r = i / DP, d = i % DP;
-            const int64_t row = group * 16 * RT + 16 * t + r;
-            if (row >= rows || d >= D) continue;
-            const float* o = out + r * (DP + 2);
-            constexpr int step = 16 * (DP + 2);
-            const float best = fmaxf(fmaxf(o[DP], o[step + DP]), fmaxf(o[2 * step + DP], o[3 * step + DP]));
-            float all = 0.0f, v = 0.0f;
+        const unsigned row_begin = group * 16 * RT + 16 * t, live = rows > row_begin ? min(rows - row_begin, 16u) : 0;
+        for (unsigned at = 0; at < heads; ++at) {
+            for (unsigned i = tid; i < live * DP; i += 256) {
+                const unsigned r = i / DP, d = i % DP;
+                if (d >= D) continue;
+                // this head's waves are `heads` apart
+                float tops[4], sums[4], o[4], best = kNegInf, all = 0.0f, v = 0.0f;
 #pragma unroll
-            for (int w = 0; w < 4; ++w) {
-                // a wave without a key that is seen has a sum of 0 and no reference
-                const float top_w = o[w * step + DP];
-                const float f = top_w == best ? 1.0f : __builtin_amdgcn_exp2f(top_w - best);
-                all += o[w * step + DP + 1] * f;
-                v += o[w * step + d] * f;
-            }
-            const int64_t token = row / R, h = kvh * R + row % R;
-            if (p.splits == 1) {
-                ((S*)p.y)[((b * p.N + token) * p.H + h) * D + d] = (S)(token < fresh ? v / all : 0.0f);
-            } else {
-                float* part = p.parts + (((b * p.N + token) * p.H + h) * p.splits + split) * (D + 4);
-                part[d] = v;
-                if (d == 0) {
-                    part[D] = best;
-                    part[D + 1] = all;
+                for (unsigned w = 0; w < 4; ++w) {
+                    const float* from = out + ((min(w, shares - 1) * heads + at) * 16 + r) * (DP + 2);
+                    tops[w] = from[DP], sums[w] = from[DP + 1], o[w] = from[d];
+                    best = fmaxf(best, tops[w]);
+                }
+#pragma unroll
+                for (unsigned w = 0; w < 4; ++w) {
+                    if (w >= shares) continue;
+                    // a wave without a key that is seen has a sum of 0 and no reference
+                    const float f = tops[w] == best ? 1.0f : __builtin_amdgcn_exp2f(tops[w] - best);
+                    all += sums[w] * f;
+                    v += o[w] * f;
+                }
+                const unsigned row = row_begin + r, token = row / R, h = (kvh0 + at) * R + row % R;
+                const int64_t to = (int64_t)token * H + h;
+                if (splits == 1) {
+                    y[to * D + d] = (S)((int)token < fresh ? v / all : 0.0f);
+                } else {
+                    float* left = p.parts + (((int64_t)b * N * H + to) * splits + split) * (D + 4);
+                    left[d] = v;
+                    if (d == 0) {
+                        left[D] = best;
+                        left[D + 1] = all;
+                    }
                 }
             }
         }
@@ -461,10 +474,11 @@ __global__ __launch_bounds__(256) void qattn_join_kernel(AttnArgs p) {
     typedef typename Elem<E>::S S;
     typedef S S4 __attribute__((ext_vector_type(4)));
     __shared__ __align__(16) float left[8][128 + 4];
-    const int64_t row = blockIdx.x, token = row / p.H % p.N, b = row / p.H / p.N, len = p.lengths[b];
-    const int64_t fresh = p.fresh ? clamp_to(p.fresh[b], p.N) : p.N;
+    const unsigned b = blockIdx.y, token = blockIdx.x / (unsigned)p.H;
+    const int64_t row = (int64_t)b * p.N * p.H + blockIdx.x;
+    const int len = p.lengths[b], fresh = p.fresh ? min(max(p.fresh[b], 0), (int)p.N) : (int)p.N;
     const int d = (threadIdx.x & 31) * 4, set = threadIdx.x >> 5;
-    const bool idle = len < 0 || len + fresh > p.M;
+    const bool idle = len < 0 || (int64_t)len + fresh > p.M;
     if (!idle && d < p.D) {
         const Joined j = join_parts<8, 8>(p.parts + row * p.splits * (p.D + 4), set, (int)p.splits, p.D, d);
         *reinterpret_cast<f32x4*>(&left[set][d]) = j.v;
@@ -476,7 +490,7 @@ __global__ __launch_bounds__(256) void qattn_join_kernel(AttnArgs p) {
     __syncthreads();
     if (set || d >= p.D) return;
     f32x4 v;
-    if (idle || token >= fresh) {
+    if (idle || (int)token >= fresh) {
         const float none = !idle || len < 0 ? 0.0f : __builtin_nanf("");
         v = f32x4{none, none, none, none};
     } else {
@@ -490,17 +504,19 @@ __global__ __launch_bounds__(256) void qattn_join_kernel(AttnArgs p) {
 
 template <typename E, int BITS, int DP, int CAP, int RT>
 static int rows_launch(const AttnArgs& p, hipStream_t stream) {
-    const int64_t groups = ceil_div(p.H / p.G * p.N, 16 * RT);
+    const int64_t units = p.splits * p.B * ceil_div(p.H / p.G * p.N, 16 * RT), sets = p.G / p.row_splits;
     qattn_rows_kernel<E, BITS, DP, CAP, RT>
-        <<<dim3((unsigned)(p.splits * p.B * p.G * groups)), 256, RowsLds<DP>::bytes, stream>>>(p);
+        <<<dim3((unsigned)(ceil_div(units, 8) * 8 * sets)), 256, RowsLds<DP>::bytes, stream>>>(p);
     const int rc = check_launch("qattn_rows");
     if (rc != FLARE_OK || p.splits == 1) return rc;
-    qattn_join_kernel<E><<<dim3((unsigned)(p.B * p.N * p.H)), 256, 0, stream>>>(p);
+    qattn_join_kernel<E><<<dim3((unsigned)(p.N * p.H), (unsigned)p.B), 256, 0, stream>>>(p);
     return check_launch("qattn_join");
 }
 template <typename E, int BITS, int DP, int CAP>
 static int rows_rt(const AttnArgs& p, int tiles, hipStream_t stream) {
-    return tiles == 1 ? rows_launch<E, BITS, DP, CAP, 1>(p, stream) : rows_launch<E, BITS, DP, CAP, 2>(p, stream);
+    if constexpr (sizeof(E) == 2)
+        if (tiles == 2) return rows_launch<E, BITS, DP, CAP, 2>(p, stream);
+    return rows_launch<E, BITS, DP, CAP, 1>(p, stream);
 }
 template <typename E, int BITS, int DP>
 static int rows_dp(const AttnArgs& p, int tiles, hipStream_t stream) {
@@ -509,7 +525,7 @@ static int rows_dp(const AttnArgs& p, int tiles, hipStream_t stream) {
         if (p.cap <= kCoarseCapMost) return rows_rt<E, BITS, DP, kCap>(p, tiles, stream);
     return rows_rt<E, BITS, DP, kCapFine>(p, tiles, stream);
 }
-// tiles: of 16 rows a wave owns, 1 or 2.
+// tiles: of 16 rows a wave owns, 1, or 2 of 16-bit queries (the parts of fp32 ones take three times the registers).
 template <typename E, int BITS>
 int rows_e(const AttnArgs& p, int tiles, hipStream_t stream) {
     return p.D <= 32   ? rows_dp<E, BITS, 32>(p, tiles, stream)
