@@ -42,7 +42,7 @@ from ._inputs import (
     _strides,
     _training,
 )
-from .quantized import attend_quantized, is_quantized
+from .quantized import attend_quantized, is_quantized, step_fast
 
 
 # Caps that the kernels take: what scale / cap and the cap itself can be with in float32.
@@ -311,9 +311,14 @@ def softmax_attention_decode(
     """
     name = "softmax_attention_decode"
     quantized = is_quantized(cache)
-    out = None if quantized else _step_fast(Q, K, V, cache, lengths, scale, softcap, slopes)
-    if out is not None:
-        return out
+    if not quantized:
+        out = _step_fast(Q, K, V, cache, lengths, scale, softcap, slopes)
+        if out is not None:
+            return out
+    elif softcap is None or _LEAST_CAP <= softcap <= _MOST_CAP:
+        y = step_fast(Q, K, V, cache, lengths, _resolve_attn_scale(scale, Q.shape[-1]), softcap, slopes)
+        if y is not None:
+            return y, cache
     Q, K, V = (t[:, None] if t.dim() == 3 else t for t in (Q, K, V))
     B, T, H, G, D = _check_heads(name, Q, K, V)
     if T != 1:

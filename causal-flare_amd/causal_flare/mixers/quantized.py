@@ -22,6 +22,7 @@ import torch
 
 from .. import _lib
 from ._inputs import (
+    _CODES,
     _aligned_rows,
     _check_device,
     _check_float,
@@ -29,6 +30,7 @@ from ._inputs import (
     _f32,
     _int32,
     _on,
+    _plain_f32,
     _ptr,
     _raw_stream,
     _strides,
@@ -36,6 +38,7 @@ from ._inputs import (
 
 _BLOCK = 32
 _PARTS = ("k", "k_scale", "v", "v_scale")
+_FORMS = {torch.uint8: 4, torch.float8_e4m3fn: 8}
 
 
 def is_quantized(cache) -> bool:
@@ -83,6 +86,71 @@ def check_quantized(name, cache):
     return bits, B, S, G, D
 
 
+def _plain_parts(cache, device):
+    """(bits, shape of k, pointers of the four) of a cache that the kernels take on `device`, or None."""
+    try:
+        k, ks, v, vs = (cache[n] for n in _PARTS)
+        shape, dtype = k.shape, k.dtype
+        B, S, G, W = shape
+        bits = _FORMS[dtype]
+        D = W * 8 // bits
+        scales = (B, S, G, (D + _BLOCK - 1) // _BLOCK)
+        if (v.shape != shape or v.dtype is not dtype or ks.shape != scales or vs.shape != scales or D % 16 or not 16 <= D <= 128
+                or ks.dtype is not torch.uint8 or vs.dtype is not torch.uint8 or not B * S * G):
+            return None
+        for t in (k, ks, v, vs):
+            if t.device != device or not t.is_contiguous():
+                return None
+        pointers = (k.data_ptr(), ks.data_ptr(), v.data_ptr(), vs.data_ptr())
+    except (KeyError, TypeError, ValueError, AttributeError):
+        return None
+    return None if (pointers[0] | pointers[2]) % 16 else (bits, B, S, G, D, pointers)
+
+
+def step_fast(Q, K, V, cache, lengths, scale, softcap, slopes):
+    """y of the common single token, or None: one type, rows and a cache that the kernel reads in place, int32 lengths.
+    softcap: None or within the kernels' range."""
+    dtype, device, shape = Q.dtype, Q.device, Q.shape
+    code = _CODES.get(dtype)
+    if code is None or device.type != "cuda" or device.index != torch.cuda.current_device():
+        return None
+    parts = _plain_parts(cache, device)
+    if parts is None or not isinstance(lengths, torch.Tensor):
+        return None
+    bits, B, S, G, D, held = parts
+    token = len(shape) == 4
+    if len(shape) not in (3, 4) or (token and shape[1] != 1):
+        return None
+    H = shape[-2]
+    want = (B, 1, G, D) if token else (B, G, D)
+    if (shape[0] != B or shape[-1] != D or H < 1 or H % G or K.shape != want or V.shape != want
+            or lengths.dtype is not torch.int32 or lengths.shape != (B,) or lengths.device != device
+            or not lengths.is_contiguous()):
+        return None
+    if slopes is not None and (not _plain_f32(slopes, device, H) or slopes.requires_grad):
+        return None
+    strides, spread = [], 0
+    for t in (Q, K, V):
+        if t.stride(-1) != 1 or t.dtype is not dtype or t.device != device:
+            return None
+        a, b = t.stride(0), t.stride(-2)
+        strides += (a, 0, b)
+        spread |= a | b
+    pointers = (Q.data_ptr(), K.data_ptr(), V.data_ptr())
+    if (spread * Q.element_size() | pointers[0] | pointers[1] | pointers[2]) % 16:
+        return None
+    y = torch.empty((B, 1, H, D), device=device, dtype=dtype)
+    lib = _lib.lib()
+    nbytes = lib.flare_qattn_workspace_size(B, 1, S, H, G, D, code)
+    ws = torch.empty(nbytes, device=device, dtype=torch.uint8) if nbytes else None
+    rc = lib.flare_qattn(
+        *pointers, _strides(*strides), code, bits, B, 1, S, H, G, D, scale, softcap or 0.0, _ptr(slopes), None,
+        lengths.data_ptr(), None, *held, y.data_ptr(), _ptr(ws), nbytes, _raw_stream(device.index))
+    if rc:
+        _lib.check(rc, "flare_qattn")
+    return y
+
+
 def check_lengths(name, lengths, B):
     if not isinstance(lengths, torch.Tensor):
         raise ValueError(f"{name} expects a tensor in lengths. Got {lengths!r:.80}")
@@ -127,6 +195,34 @@ def quantized_cache_write(
     return cache
 
 
+def _read_fast(cache, first, count, dtype):
+    """The common call, or None: a cache on the current device, int32 `first`."""
+    code = _CODES.get(dtype)
+    device = cache["k"].device if isinstance(cache, dict) and isinstance(cache.get("k"), torch.Tensor) else None
+    if code is None or device is None or device.type != "cuda" or device.index != torch.cuda.current_device():
+        return None
+    parts = _plain_parts(cache, device)
+    if parts is None:
+        return None
+    bits, B, S, G, D, held = parts
+    count = S if count is None else count
+    if type(count) is not int or count < 1:
+        return None
+    at = None
+    if first is not None:
+        if (not isinstance(first, torch.Tensor) or first.dtype is not torch.int32 or first.shape != (B,)
+                or first.device != device or not first.is_contiguous()):
+            return None
+        at = first.data_ptr()
+    k = torch.empty((B, count, G, D), device=device, dtype=dtype)
+    v = torch.empty_like(k)
+    rc = _lib.lib().flare_qcache_read(*held, code, bits, B, count, S, G, D, at, k.data_ptr(), v.data_ptr(),
+                                      _raw_stream(device.index))
+    if rc:
+        _lib.check(rc, "flare_qcache_read")
+    return k, v
+
+
 def quantized_cache_read(
     cache: dict[str, torch.Tensor],
     first: torch.Tensor | None = None,
@@ -140,6 +236,9 @@ def quantized_cache_read(
     if it was written from that type (and rounded to it otherwise, infinite beyond its range).
     """
     name = "quantized_cache_read"
+    out = _read_fast(cache, first, count, dtype)
+    if out is not None:
+        return out
     bits, B, S, G, D = check_quantized(name, cache)
     code = _lib.dtype_code(dtype)
     _check_integers(name, "first", first, (B,))
@@ -177,7 +276,7 @@ def attend_quantized(name, Q, K, V, cache, lengths, scale, cap, slopes, prefix_l
     q, k, v = (_aligned_rows(t, Q.dtype) for t in (Q, K, V))
     sl, pre, lens, new = _f32(slopes), _int32(prefix_lengths), _int32(lengths), _int32(new_lengths)
     lib, P = _lib.lib(), _ptr
-    nbytes = lib.flare_qattn_workspace_size(B, T, S, H, G, D, code, bits)
+    nbytes = lib.flare_qattn_workspace_size(B, T, S, H, G, D, code)
     ws = torch.empty(nbytes, device=device, dtype=torch.uint8) if nbytes else None
     with _on(device):
         rc = lib.flare_qattn(

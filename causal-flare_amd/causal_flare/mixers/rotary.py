@@ -19,6 +19,7 @@ from torch.autograd.function import once_differentiable
 from .. import _lib
 from .._common import _compute_dtype
 from ._inputs import (
+    _CODES,
     _check_device,
     _check_float,
     _check_integers,
@@ -78,6 +79,40 @@ def _turn(q, k, frequencies, positions, lengths, interleaved, inverse):
     return q_out.to(q.dtype), None if k is None else k_out.to(k.dtype)
 
 
+def _turn_fast(Q, K, frequencies, positions, lengths, interleaved):
+    """The common call that is not differentiated, or None: Q and K of one type on the current device, rows that the
+    kernel reads in place, int32 positions or lengths."""
+    if K is None or (torch.is_grad_enabled() and (Q.requires_grad or K.requires_grad)):
+        return None
+    dtype, device, shape, keys = Q.dtype, Q.device, Q.shape, K.shape
+    code = _CODES.get(dtype)
+    if (code is None or device.type != "cuda" or device.index != torch.cuda.current_device() or len(shape) not in (3, 4)
+            or len(keys) != len(shape) or K.dtype is not dtype or K.device != device or Q.stride(-1) != 1
+            or K.stride(-1) != 1 or not isinstance(frequencies, torch.Tensor)):
+        return None
+    B, H, D, G = shape[0], shape[-2], shape[-1], keys[-2]
+    N = shape[1] if len(shape) == 4 else 1
+    if keys != (shape[:-2] + (G, D)) or not B * N * H * G or frequencies.dtype is not torch.float64 or (
+            frequencies.dim() != 1 or frequencies.device.type != "cpu" or not frequencies.is_contiguous()):
+        return None
+    R = 2 * frequencies.shape[0]
+    if not 2 <= R <= D or D > 256 or (positions is not None and lengths is not None):
+        return None
+    for t, want in ((positions, (B, N)), (lengths, (B,))):
+        if t is not None and (t.dtype is not torch.int32 or t.shape != want or t.device != device or not t.is_contiguous()):
+            return None
+    step = (Q.stride(1), K.stride(1)) if len(shape) == 4 else (0, 0)
+    q = torch.empty_like(Q, memory_format=torch.contiguous_format)
+    k = torch.empty_like(K, memory_format=torch.contiguous_format)
+    rc = _lib.lib().flare_rotary(
+        Q.data_ptr(), K.data_ptr(), _strides(Q.stride(0), step[0], Q.stride(-2), K.stride(0), step[1], K.stride(-2)), code, B,
+        N, H, G, D, R, frequencies.data_ptr(), _ptr(positions), _ptr(lengths), 1 if interleaved else 0, 0, q.data_ptr(),
+        k.data_ptr(), _raw_stream(device.index))
+    if rc:
+        _lib.check(rc, "flare_rotary")
+    return q, k
+
+
 class RotaryPositions(autograd.Function):
     """Turned queries and keys; their gradients are turned back."""
 
@@ -119,6 +154,9 @@ def rotary_positions(
     holds already: token t is at position lengths[b] + t.  Without either it is at t.  D up to 256.
     """
     name = "rotary_positions"
+    out = _turn_fast(Q, K, frequencies, positions, lengths, interleaved)
+    if out is not None:
+        return out
     token = Q.dim() == 3
     if Q.dim() not in (3, 4) or (K is not None and K.dim() != Q.dim()):
         raise ValueError(f"{name} expects Q [B, N, H, D] and K [B, N, G, D], or without N. Got Q={tuple(Q.shape)}"

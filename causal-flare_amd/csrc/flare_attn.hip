@@ -1,6 +1,6 @@
 // flare_attn.hip -- softmax attention: C entry points, id statistics, and writing prompts to caches.
-#include "flare_attn.h"
 #include "flare_internal.h"
+#include "flare_qcache.h"
 
 namespace flare {
 namespace attn {
@@ -170,17 +170,34 @@ static int64_t step_splits(int64_t B, int64_t M, int64_t H, int64_t G) {
     return s < 1 ? 1 : (s > most ? most : s);
 }
 
-// A few new tokens over a cache of 8 or 4 bits: rows (token, head) of the heads that share keys.
-constexpr int64_t kFewRows = 64;
 static int row_tiles(int64_t N, int64_t H, int64_t G, int dtype) { return H / G * N > 16 && dtype != FLARE_F32 ? 2 : 1; }
-static bool few_rows(int64_t N, int64_t H, int64_t G) { return H / G * N <= kFewRows; }
+// Which kernel takes N new tokens over a cache of 8 or 4 bits.  kRows: rows (token, head) of the heads that share keys
+// in groups of 16 or 32, whose codes go straight into operands.  kFused: attn_forward with the codes turned into values
+// as they go to LDS, once for each 128 tokens of each head.  kExpanded: attn_forward over 16-bit values that the
+// codes are turned into first.
+//   A group of 32 rows takes a third of what 128 rows of a head take.  us, fused and by rows, 16 heads of 128 over 4, 4
+// bits: 16 x 8192 cached tokens, 32 new 177, 86; 64 new 185, 124; 128 new 195, 232; one sequence of 1000, 64 new
+// 31, 21.  fp32 queries: 16 x 4096 cached, 8 heads of 64, 32 new 106, 55; 512 new 595, 304, so these always go by rows.
+enum { kRows, kFused, kExpanded };
+constexpr int64_t kExpandRows = 16;
+static int qattn_path(int64_t N, int64_t H, int64_t G, int dtype) {
+    const int64_t R = H / G, blocks = R * ceil_div(N, 128);
+    if (dtype == FLARE_F32 || ceil_div(R * N, 32) <= 3 * blocks) return kRows;
+    return blocks < kExpandRows ? kFused : kExpanded;
+}
+// Sequences that are expanded at a time: 1 GiB of values, or one.
+static int64_t expand_slice(int64_t B, int64_t M, int64_t G, int64_t D) {
+    const int64_t s = (int64_t)(1 << 30) / (M * G * D * 4);
+    return s < 1 ? 1 : (s > B ? B : s);
+}
+static size_t expanded_bytes(int64_t B, int64_t M, int64_t G, int64_t D) { return (size_t)(B * M * G * D * 4 + 255) / 256 * 256; }
 // Key heads of the same tokens that the waves of a workgroup take side by side.
 static int64_t rows_heads(int64_t B, int64_t N, int64_t H, int64_t G, int tiles) {
     if (tiles > 1 || B * G < 128) return 1;
     return G % 4 == 0 ? 4 : G % 2 == 0 ? 2 : 1;
 }
 // Workgroups for each sequence's keys, as step_splits.
-static int64_t rows_splits(int64_t B, int64_t N, int64_t M, int64_t H, int64_t G, int dtype, int bits) {
+static int64_t rows_splits(int64_t B, int64_t N, int64_t M, int64_t H, int64_t G, int dtype) {
     const int tiles = row_tiles(N, H, G, dtype);
     const int64_t heads = rows_heads(B, N, H, G, tiles);
     const int64_t rows = B * (G / heads) * ceil_div(H / G * N, 16 * tiles);
@@ -194,6 +211,31 @@ static int qattn_rows(const AttnArgs& p, int bits, int tiles, hipStream_t stream
 template <typename E>
 static int qattn_forward(const AttnArgs& p, int bits, hipStream_t stream) {
     return bits == 8 ? forward_bits<E, 8>(p, stream) : forward_bits<E, 4>(p, stream);
+}
+
+static int qattn_expanded(const AttnArgs& all, int dtype, int bits, void* workspace, hipStream_t stream) {
+    const int64_t slice = expand_slice(all.B, all.M, all.G, all.D), row = all.G * all.D, codes = row * bits / 8;
+    const int64_t scales = all.G * qcache::row_scales(all.D);
+    for (int64_t b = 0; b < all.B; b += slice) {
+        AttnArgs p = all;
+        p.B = slice < all.B - b ? slice : all.B - b;
+        const int64_t held = b * p.M;
+        p.q.p = (const char*)all.q.p + b * p.q.sb * 2, p.y = (char*)all.y + b * p.N * p.H * p.D * 2;
+        p.lengths = all.lengths + b, p.fresh = all.fresh ? all.fresh + b : nullptr;
+        p.prefix = all.prefix ? all.prefix + b : nullptr;
+        p.k.p = (const char*)all.k.p + held * codes, p.v.p = (const char*)all.v.p + held * codes;
+        p.k_scale = all.k_scale + held * scales, p.v_scale = all.v_scale + held * scales;
+        char* k = (char*)workspace;
+        char* v = k + slice * p.M * row * 2;
+        int rc = qcache::qcache_expand(p, dtype, bits, k, v, stream);
+        if (rc != FLARE_OK) return rc;
+        p.k = {k, p.M * row, row, p.D}, p.v = {v, p.M * row, row, p.D};
+        split_forward(p, dtype);
+        p.parts = (float*)(k + expanded_bytes(slice, p.M, p.G, p.D));
+        rc = dtype == FLARE_BF16 ? forward_e<__hip_bfloat16>(p, stream) : forward_e<__half>(p, stream);
+        if (rc != FLARE_OK) return rc;
+    }
+    return FLARE_OK;
 }
 
 }  // namespace attn
@@ -360,17 +402,23 @@ extern "C" int flare_attn_step(const void* q, const void* k, const void* v, cons
     return attn_step(p, dtype, (hipStream_t)stream);
 }
 
-extern "C" size_t flare_qattn_workspace_size(int64_t B, int64_t N, int64_t M, int64_t H, int64_t G, int64_t D, int dtype,
-                                             int bits) {
+extern "C" size_t flare_qattn_workspace_size(int64_t B, int64_t N, int64_t M, int64_t H, int64_t G, int64_t D, int dtype) {
     if (B < 1 || N < 1 || M < 1 || H < 1 || G < 1 || H % G) return 0;
-    if (few_rows(N, H, G)) {
-        const int64_t s = rows_splits(B, N, M, H, G, dtype, bits);
+    const int path = qattn_path(N, H, G, dtype);
+    if (path == kRows) {
+        const int64_t s = rows_splits(B, N, M, H, G, dtype);
         return s == 1 ? 0 : (size_t)(B * N * H * s * (D + 4)) * sizeof(float);
     }
     AttnArgs p = {};
-    p.B = B, p.N = N, p.M = M, p.H = H, p.D = D, p.causal = 1;
-    split_forward(p, dtype);
-    return rows_bytes(p);
+    p.B = path == kFused ? B : expand_slice(B, M, G, D), p.N = N, p.M = M, p.H = H, p.D = D, p.causal = 1;
+    size_t most = 0;
+    // (the last slice may be smaller and split its keys more often)
+    for (const int64_t left = path == kFused ? B : B % p.B ? B % p.B : p.B;; p.B = left) {
+        split_forward(p, dtype);
+        most = rows_bytes(p) > most ? rows_bytes(p) : most;
+        if (p.B == left) break;
+    }
+    return most + (path == kFused ? 0 : expanded_bytes(expand_slice(B, M, G, D), M, G, D));
 }
 
 extern "C" int flare_qattn(const void* q, const void* k, const void* v, const int64_t* strides, int dtype, int bits, int64_t B,
@@ -382,12 +430,13 @@ extern "C" int flare_qattn(const void* q, const void* k, const void* v, const in
                   "flare_qattn: null pointer");
     ATTN_REQUIRE_SIZES("flare_qattn");
     FLARE_REQUIRE(bits == 4 || bits == 8, "flare_qattn: %d bits; 4 or 8", bits);
+    FLARE_REQUIRE(N * H <= (1 << 30) && N * G <= (1 << 27), "flare_qattn: too large");
     AttnArgs p = attn_args(q, k_cache, v_cache, strides, B, N, M, H, G, D, scale, softcap, slopes);
     const Rows kr = {k, strides[3], strides[4], strides[5]}, vr = {v, strides[6], strides[7], strides[8]};
     const uintptr_t held = (uintptr_t)k_cache | (uintptr_t)v_cache | (uintptr_t)y;
     FLARE_REQUIRE(aligned(p.q, dtype) && aligned(kr, dtype) && aligned(vr, dtype) && (held & 15) == 0,
                   "flare_qattn: rows must be 16-byte aligned and less than 2^22 elements apart");
-    if (workspace_bytes < flare_qattn_workspace_size(B, N, M, H, G, D, dtype, bits) ||
+    if (workspace_bytes < flare_qattn_workspace_size(B, N, M, H, G, D, dtype) ||
         (workspace_bytes && (!workspace || ((uintptr_t)workspace & 15)))) {
         set_error("flare_qattn: workspace of %zu bytes is too small or not 16-byte aligned", workspace_bytes);
         return FLARE_ERR_WORKSPACE;
@@ -395,9 +444,9 @@ extern "C" int flare_qattn(const void* q, const void* k, const void* v, const in
     p.k_scale = (uint8_t*)k_scale, p.v_scale = (uint8_t*)v_scale;
     p.lengths = lengths, p.fresh = new_lengths, p.prefix = prefix_lengths, p.causal = 1;
     p.y = y, p.parts = (float*)workspace;
-    const bool few = few_rows(N, H, G);
+    const int path = qattn_path(N, H, G, dtype);
     // one token's key and value are quantised on the way
-    if (N == 1 && few && !new_lengths) {
+    if (N == 1 && path == kRows && !new_lengths) {
         p.k_new = k, p.kn_sb = strides[3], p.kn_sg = strides[5];
         p.v_new = v, p.vn_sb = strides[6], p.vn_sg = strides[8];
     } else {
@@ -405,10 +454,12 @@ extern "C" int flare_qattn(const void* q, const void* k, const void* v, const in
                                           k_scale, v_cache, v_scale, stream);
         if (rc != FLARE_OK) return rc;
     }
-    if (few) {
-        p.splits = rows_splits(B, N, M, H, G, dtype, bits), p.row_splits = rows_heads(B, N, H, G, row_tiles(N, H, G, dtype));
+    if (path == kRows) {
+        p.splits = rows_splits(B, N, M, H, G, dtype), p.row_splits = rows_heads(B, N, H, G, row_tiles(N, H, G, dtype));
         return FLARE_BY_DTYPE(dtype, qattn_rows, (p, bits, row_tiles(N, H, G, dtype), (hipStream_t)stream));
     }
+    if (path == kExpanded) return qattn_expanded(p, dtype, bits, workspace, (hipStream_t)stream);
     split_forward(p, dtype);
-    return FLARE_BY_DTYPE(dtype, qattn_forward, (p, bits, (hipStream_t)stream));
+    return dtype == FLARE_BF16 ? qattn_forward<__hip_bfloat16>(p, bits, (hipStream_t)stream)
+                               : qattn_forward<__half>(p, bits, (hipStream_t)stream);
 }

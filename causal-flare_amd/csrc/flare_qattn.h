@@ -124,10 +124,13 @@ __global__ __launch_bounds__(256, rows_waves(sizeof(E), BITS, RT)) void qattn_ro
         return;
     }
     const int n = off + fresh, prefix = p.prefix ? min(max(p.prefix[b], 0), n) : 0;
+    // the tokens whose rows these are, and the keys that the last of them sees
+    const int token0 = (int)(group * 16 * RT / R), token1 = min((int)min((group * 16 * RT + 16 * RT - 1) / R, N), fresh - 1);
+    const int seen = token0 < fresh ? min(n, max(off + token1 + 1, prefix)) : 0;
     const int step = (int)shares * TK;
-    const unsigned share = ((unsigned)n + splits - 1) / splits;
+    const unsigned share = ((unsigned)seen + splits - 1) / splits;
     const int per = (int)((share + step - 1) / step * step);
-    const int first = (int)min((int64_t)split * per, (int64_t)n), last = (int)min((int64_t)first + per, (int64_t)n);
+    const int first = (int)min((int64_t)split * per, (int64_t)seen), last = (int)min((int64_t)first + per, (int64_t)seen);
     const int held = single ? min(last, off) : last;           // what of it memory holds
     const unsigned codes = D * BITS / 8, scales = (D + kBlock - 1) / kBlock;
     const unsigned stride = G * codes, scale_stride = G * scales;
@@ -304,7 +307,7 @@ __global__ __launch_bounds__(256, rows_waves(sizeof(E), BITS, RT)) void qattn_ro
                     for (int t = 0; t < RT; ++t) s[t][m] = mma(a, qf[t][i][kk], s[t][m]);
             }
         }
-        const bool whole = single || k0 + TK <= off + 1;           // every row sees all of these keys
+        const bool whole = single || k0 + TK <= off + token0 + 1;  // every row sees all of these keys
         if (!whole) {
             bool odd = false;
 #pragma unroll

@@ -1,10 +1,8 @@
 // flare_qattn_f32_4.hip -- softmax attention of f32 queries over a cache of 4 bits.
-#include "flare_attn_fwd.h"
 #include "flare_qattn.h"
 
 namespace flare {
 namespace attn {
-template int forward_bits<float, 4>(const AttnArgs&, hipStream_t);
 template int rows_e<float, 4>(const AttnArgs&, int, hipStream_t);
 }  // namespace attn
 }  // namespace flare

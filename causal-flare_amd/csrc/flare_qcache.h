@@ -170,6 +170,10 @@ __device__ __forceinline__ void load8(const T* p, float (&v)[8]) {
     if constexpr (sizeof(T) == 4) mix::load_row<T, 4>(p + 4, reinterpret_cast<float (&)[4]>(v[4]));
 }
 
+// What the cache of `p` holds of each sequence, its new tokens included, as k and v [B, M, G, D] of `dtype`; rows
+// behind that are left as they are.
+int qcache_expand(const attn::AttnArgs& p, int dtype, int bits, void* k, void* v, hipStream_t stream);
+
 __host__ __device__ __forceinline__ int64_t row_codes(int64_t D, int bits) { return D * bits / 8; }
 __host__ __device__ __forceinline__ int64_t row_scales(int64_t D) { return (D + kBlock - 1) / kBlock; }
 

@@ -37,13 +37,19 @@ __global__ __launch_bounds__(256) void qcache_write_kernel(Rows k, Rows v, const
     if ((id & 3) == 0) (blockIdx.y ? to.v_scale : to.k_scale)[row * NB + block] = (uint8_t)byte;
 }
 
-// Rows first[b] .. first[b] + N - 1 of each sequence; 0 outside of it.  Eight values a thread.
+// Rows first[b] .. first[b] + N - 1 of each sequence; 0 outside of it.  Eight values a thread.  With `lengths`
+// those that a sequence of so many tokens and `fresh` (or all N_new) new ones holds, and no others.
 template <typename T, int BITS>
 __global__ __launch_bounds__(256) void qcache_read_kernel(Cache from, const int32_t* first, unsigned N, int64_t M, unsigned G,
-                                                          unsigned D, T* k, T* v) {
+                                                          unsigned D, const int32_t* lengths, const int32_t* fresh,
+                                                          int64_t N_new, T* k, T* v) {
     const unsigned per = D / 8, NB = (D + kBlock - 1) / kBlock, b = blockIdx.z;
     const unsigned id = blockIdx.x * 256 + threadIdx.x, d = id % per * 8, g = id / per % G, t = id / per / G;
     if (t >= N) return;
+    if (lengths) {
+        const int64_t off = lengths[b], n = fresh ? clamp_to(fresh[b], N_new) : N_new;
+        if (off < 0 || t >= off + n) return;
+    }
     const int64_t at = (first ? (int64_t)first[b] : 0) + t;
     f32x8 x = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
     if (at >= 0 && at < M) {
@@ -73,11 +79,17 @@ static int write_type(const Rows& k, const Rows& v, int bits, const int32_t* len
 }
 template <typename T>
 static int read_type(const Cache& from, int bits, const int32_t* first, int64_t B, int64_t N, int64_t M, int64_t G, int64_t D,
-                     void* k, void* v, hipStream_t stream) {
+                     const int32_t* lengths, const int32_t* fresh, int64_t N_new, void* k, void* v, hipStream_t stream) {
     const dim3 grid((unsigned)ceil_div(N * G * D / 8, 256), 2, (unsigned)B);
     const auto kernel = bits == 8 ? qcache_read_kernel<T, 8> : qcache_read_kernel<T, 4>;
-    kernel<<<grid, 256, 0, stream>>>(from, first, (unsigned)N, M, (unsigned)G, (unsigned)D, (T*)k, (T*)v);
+    kernel<<<grid, 256, 0, stream>>>(from, first, (unsigned)N, M, (unsigned)G, (unsigned)D, lengths, fresh, N_new,
+                                      (T*)k, (T*)v);
     return check_launch("qcache_read");
+}
+
+int qcache_expand(const attn::AttnArgs& p, int dtype, int bits, void* k, void* v, hipStream_t stream) {
+    const Cache from = {(uint8_t*)p.k.p, (uint8_t*)p.v.p, p.k_scale, p.v_scale};
+    return FLARE_BY_DTYPE(dtype, read_type, (from, bits, nullptr, p.B, p.M, p.M, p.G, p.D, p.lengths, p.fresh, p.N, k, v, stream));
 }
 
 }  // namespace qcache
@@ -116,5 +128,5 @@ extern "C" int flare_qcache_read(const void* k_cache, const void* k_scale, const
     FLARE_REQUIRE((((uintptr_t)k_cache | (uintptr_t)v_cache | (uintptr_t)k | (uintptr_t)v) & 15) == 0,
                   "flare_qcache_read: tensors must be 16-byte aligned");
     const Cache from = {(uint8_t*)k_cache, (uint8_t*)v_cache, (uint8_t*)k_scale, (uint8_t*)v_scale};
-    return FLARE_BY_DTYPE(dtype, read_type, (from, bits, first, B, N, M, G, D, k, v, (hipStream_t)stream));
+    return FLARE_BY_DTYPE(dtype, read_type, (from, bits, first, B, N, M, G, D, nullptr, nullptr, 0, k, v, (hipStream_t)stream));
 }

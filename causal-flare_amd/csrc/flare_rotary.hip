@@ -19,6 +19,7 @@ namespace rotary {
 using mix::ceil_div;
 
 constexpr int kMostPairs = 128;
+constexpr long double kTurns = 0x1p64L / 6.283185307179586476925286766559L;       // of a radian, in 2^-64 turns
 
 struct Head {                        // a [B, N, heads, D] tensor: element strides
     const void* p;
@@ -197,9 +198,13 @@ extern "C" int flare_rotary(const void* q, const void* k, const int64_t* strides
     p.B = B, p.N = N, p.H = (int)H, p.G = k ? (int)G : 0, p.D = (int)D, p.R = (int)R;
     p.positions = positions, p.lengths = lengths, p.interleaved = interleaved, p.inverse = inverse;
     for (int i = 0; i < R / 2; ++i) {
+        const long double f = frequencies[i];
+        if (f >= 0.0L && f < 6.0L) {
+            p.turns[i] = (uint64_t)(f * kTurns);            // below 0.96 2^64
+            continue;
+        }
         FLARE_REQUIRE(isfinite(frequencies[i]), "flare_rotary: frequency %d is not finite", i);
-        const long double turns = (long double)frequencies[i] / 6.283185307179586476925286766559L;
-        const long double part = turns - floorl(turns);            // in [0, 1]: 1 only by rounding
+        const long double turns = f * (kTurns * 0x1p-64L), part = turns - floorl(turns);     // in [0, 1]: 1 only by rounding
         p.turns[i] = part < 1.0L ? (uint64_t)ldexpl(part, 64) : 0;
     }
     return FLARE_BY_DTYPE(dtype, launch_type, (p, (hipStream_t)stream));

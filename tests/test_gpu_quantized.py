@@ -215,6 +215,24 @@ def test_prompts(dtype, bits, H, G, D, T):
     check_attention(dtype, bits, H, G, D, S, T, [33], cap=300.0, slopes=[0.25 / (1 + h) for h in range(H)], seed=T)
 
 
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("H, G, D, T", [(4, 4, 64, 128), (2, 2, 128, 250), (3, 1, 80, 256), (4, 4, 16, 131), (2, 1, 96, 384), (2, 2, 32, 200),
+                                        (8, 1, 48, 256), (16, 2, 128, 270), (8, 1, 96, 300), (16, 1, 64, 129), (8, 1, 32, 257)])
+def test_longer_prompts(dtype, bits, H, G, D, T):
+    S = T + 70
+    check_attention(dtype, bits, H, G, D, S, T, [0, 70, 71, -1, 33], seed=T)
+    check_attention(dtype, bits, H, G, D, S, T, [64, 3], new=[T - 7, 0], prefix=[100, 3], seed=T, cap=20.0)
+    check_attention(dtype, bits, H, G, D, S, T, [70], cap=300.0, slopes=[0.25 / (1 + h) for h in range(H)], seed=T)
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+def test_prompts_of_a_large_cache(bits):
+    # long rooms of many sequences: more values than are turned into 16 bits at a time
+    check_attention("bf16", bits, 4, 1, 64, 1 << 20, 512, [0, 200, (1 << 20) - 512, 5, (1 << 20) - 511, 31],
+                    new=[512, 7, 0, 512, 512, 500], seed=3)
+
+
 @pytest.mark.parametrize("dtype", list(TYPES))
 def test_parts_of_long_caches(dtype):
     # keys split over workgroups, of a token, of drafts and of a prompt
@@ -251,6 +269,8 @@ def test_nan_reaches_the_rows_that_see_it(dtype, bits):
     _visible_nan(dtype, bits, 6, 4, 2, 128, 200, 100, [(3, 40, math.nan), (5, 0, math.inf)])
     _visible_nan(dtype, bits, 16, 2, 2, 80, 200, 60, [(9, 79, -math.inf)])
     _visible_nan(dtype, bits, 150, 2, 1, 64, 400, 130, [(70, 5, math.nan), (149, 63, math.inf)])
+    _visible_nan(dtype, bits, 200, 2, 2, 96, 400, 130, [(70, 5, math.nan), (199, 63, math.inf)])
+    _visible_nan(dtype, bits, 256, 8, 1, 64, 400, 130, [(70, 5, math.nan), (255, 63, math.inf)])
 
 
 @pytest.mark.parametrize("T, pieces", [(150, (70, 1, 9, 66, 4)), (20, (1,) * 20)])
