@@ -29,6 +29,7 @@ from ._inputs import (
     _raw_stream,
     _rows,
     _strides,
+    _training,
 )
 
 
@@ -61,56 +62,57 @@ def rotary_frequencies(
     return f * (keep + (1 - keep) / factor)
 
 
-def _turn(q, k, frequencies, positions, lengths, interleaved, inverse):
-    """The pairs of q [B, N, H, D] and k [B, N, G, D] (or None), of one type, turned."""
-    dtype = _compute_dtype(q, k)
-    qr, kr = _rows(q, dtype), _rows(k, dtype)
-    B, N, H, D = q.shape
-    q_out = torch.empty((B, N, H, D), device=q.device, dtype=dtype)
-    k_out = None if k is None else torch.empty(k.shape, device=q.device, dtype=dtype)
-    strides = _strides(*qr.stride()[:3], *((0, 0, 0) if k is None else kr.stride()[:3]))
-    P = _ptr
-    with _on(q.device):
-        rc = _lib.lib().flare_rotary(
-            P(qr), P(kr), strides, _lib.dtype_code(dtype), B, N, H, 0 if k is None else k.shape[2], D,
-            2 * frequencies.shape[0], P(frequencies), P(positions), P(lengths), int(interleaved), int(inverse), P(q_out),
-            P(k_out), _raw_stream(q.device.index))
-    _lib.check(rc, "flare_rotary")
-    return q_out.to(q.dtype), None if k is None else k_out.to(k.dtype)
-
-
-def _turn_fast(Q, K, frequencies, positions, lengths, interleaved):
-    """The common call that is not differentiated, or None: Q and K of one type on the current device, rows that the
-    kernel reads in place, int32 positions or lengths."""
-    if K is None or (torch.is_grad_enabled() and (Q.requires_grad or K.requires_grad)):
-        return None
-    dtype, device, shape, keys = Q.dtype, Q.device, Q.shape, K.shape
-    code = _CODES.get(dtype)
-    if (code is None or device.type != "cuda" or device.index != torch.cuda.current_device() or len(shape) not in (3, 4)
-            or len(keys) != len(shape) or K.dtype is not dtype or K.device != device or Q.stride(-1) != 1
-            or K.stride(-1) != 1 or not isinstance(frequencies, torch.Tensor)):
-        return None
-    B, H, D, G = shape[0], shape[-2], shape[-1], keys[-2]
-    N = shape[1] if len(shape) == 4 else 1
-    if keys != (shape[:-2] + (G, D)) or not B * N * H * G or frequencies.dtype is not torch.float64 or (
-            frequencies.dim() != 1 or frequencies.device.type != "cpu" or not frequencies.is_contiguous()):
-        return None
-    R = 2 * frequencies.shape[0]
-    if not 2 <= R <= D or D > 256 or (positions is not None and lengths is not None):
-        return None
-    for t, want in ((positions, (B, N)), (lengths, (B,))):
-        if t is not None and (t.dtype is not torch.int32 or t.shape != want or t.device != device or not t.is_contiguous()):
-            return None
-    step = (Q.stride(1), K.stride(1)) if len(shape) == 4 else (0, 0)
-    q = torch.empty_like(Q, memory_format=torch.contiguous_format)
-    k = torch.empty_like(K, memory_format=torch.contiguous_format)
+def _launch(q, k, dtype, frequencies, positions, lengths, interleaved, inverse):
+    """Rows that the kernel reads in place, [B, N, heads, D] or one token's [B, heads, D], of `dtype`, turned."""
+    shape, step, G, to = q.shape, (0, 0), 0, None
+    if len(shape) == 4:
+        step = (q.stride(1), 0 if k is None else k.stride(1))
+    out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    strides = (q.stride(0), step[0], q.stride(-2))
+    if k is None:
+        strides += (0, 0, 0)
+    else:
+        G, to = k.shape[-2], torch.empty_like(k, memory_format=torch.contiguous_format)
+        strides += (k.stride(0), step[1], k.stride(-2))
     rc = _lib.lib().flare_rotary(
-        Q.data_ptr(), K.data_ptr(), _strides(Q.stride(0), step[0], Q.stride(-2), K.stride(0), step[1], K.stride(-2)), code, B,
-        N, H, G, D, R, frequencies.data_ptr(), _ptr(positions), _ptr(lengths), 1 if interleaved else 0, 0, q.data_ptr(),
-        k.data_ptr(), _raw_stream(device.index))
+        q.data_ptr(), _ptr(k), _strides(*strides), _CODES[dtype], shape[0], shape[1] if len(shape) == 4 else 1, shape[-2], G,
+        shape[-1], 2 * frequencies.shape[0], frequencies.data_ptr(), _ptr(positions), _ptr(lengths), int(interleaved),
+        int(inverse), out.data_ptr(), _ptr(to), _raw_stream(q.device.index))
     if rc:
         _lib.check(rc, "flare_rotary")
-    return q, k
+    return out, to
+
+
+def _turn(q, k, frequencies, positions, lengths, interleaved, inverse):
+    """The pairs of q [B, N, H, D] and k [B, N, G, D] (or None) turned; each keeps its type."""
+    dtype = _compute_dtype(q, k)
+    with _on(q.device):
+        y, z = _launch(_rows(q, dtype), _rows(k, dtype), dtype, frequencies, positions, lengths, interleaved, inverse)
+    return y if q.dtype is dtype else y.to(q.dtype), z if k is None or k.dtype is dtype else z.to(k.dtype)
+
+
+def _plain(Q, K, frequencies, positions, lengths):
+    """Whether this is the common call: Q and K of one type on the current device, rows that the kernel reads in place,
+    int32 positions or lengths."""
+    if K is None:
+        return False
+    dtype, device, shape, keys = Q.dtype, Q.device, Q.shape, K.shape
+    if (dtype not in _CODES or device.type != "cuda" or device.index != torch.cuda.current_device() or len(shape) not in (3, 4)
+            or len(keys) != len(shape) or K.dtype is not dtype or K.device != device or Q.stride(-1) != 1
+            or K.stride(-1) != 1 or not isinstance(frequencies, torch.Tensor)):
+        return False
+    D, G = shape[-1], keys[-2]
+    if (keys != (shape[:-2] + (G, D)) or not Q.numel() or not G or frequencies.dtype is not torch.float64
+            or frequencies.dim() != 1 or frequencies.device.type != "cpu" or not frequencies.is_contiguous()):
+        return False
+    if not 2 <= 2 * frequencies.shape[0] <= D or D > 256 or (positions is not None and lengths is not None):
+        return False
+    if positions is not None:
+        t, want = positions, (shape[0], shape[1] if len(shape) == 4 else 1)
+    else:
+        t, want = lengths, shape[:1]
+    return t is None or (isinstance(t, torch.Tensor) and t.dtype is torch.int32 and t.shape == want and t.device == device
+                         and t.is_contiguous())
 
 
 class RotaryPositions(autograd.Function):
@@ -119,17 +121,16 @@ class RotaryPositions(autograd.Function):
     @staticmethod
     def forward(ctx, Q, K, frequencies, positions, lengths, interleaved):
         ctx.save_for_backward(positions, lengths)
-        ctx.options = (frequencies, interleaved)
-        ctx.keys = K is not None
+        ctx.options = (frequencies, interleaved, K is not None)
         q, k = _turn(Q, K, frequencies, positions, lengths, interleaved, False)
-        return (q, k) if ctx.keys else q
+        return q if k is None else (q, k)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, *grads):
         positions, lengths = ctx.saved_tensors
-        frequencies, interleaved = ctx.options
-        need_q, need_k = ctx.needs_input_grad[0], ctx.keys and ctx.needs_input_grad[1]
+        frequencies, interleaved, keys = ctx.options
+        need_q, need_k = ctx.needs_input_grad[0], keys and ctx.needs_input_grad[1]
         dq, dk = None, None
         if need_q:
             dq, dk = _turn(grads[0], grads[1] if need_k else None, frequencies, positions, lengths, interleaved, True)
@@ -154,9 +155,11 @@ def rotary_positions(
     holds already: token t is at position lengths[b] + t.  Without either it is at t.  D up to 256.
     """
     name = "rotary_positions"
-    out = _turn_fast(Q, K, frequencies, positions, lengths, interleaved)
-    if out is not None:
-        return out
+    if _plain(Q, K, frequencies, positions, lengths):
+        if not _training(Q, K):
+            return _launch(Q, K, Q.dtype, frequencies, positions, lengths, interleaved, False)
+        if Q.dim() == 4:
+            return RotaryPositions.apply(Q, K, frequencies, positions, lengths, interleaved)
     token = Q.dim() == 3
     if Q.dim() not in (3, 4) or (K is not None and K.dim() != Q.dim()):
         raise ValueError(f"{name} expects Q [B, N, H, D] and K [B, N, G, D], or without N. Got Q={tuple(Q.shape)}"

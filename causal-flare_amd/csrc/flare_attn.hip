@@ -213,6 +213,16 @@ static int qattn_forward(const AttnArgs& p, int bits, hipStream_t stream) {
     return bits == 8 ? forward_bits<E, 8>(p, stream) : forward_bits<E, 4>(p, stream);
 }
 
+// attn_forward's splits over values turned into 16 bits.  Where its blocks are more than a round of workgroups (512) but
+// less than one and a half, or may be many without a row that is real, two parts even the last round out.  us, one part
+// and two, 16 heads of 128 over 4: 4608 rows (576 blocks) behind 8000 625, 545; 5120 707, 574; 6144 (768) 777, 661; 8192
+// (1024) 929, 937; 2700 to 4096 real rows of 4096 (512) behind 11000 610, 494; all of 4 x 1024 behind 7000 (512) 314, 334.
+static void split_expanded(AttnArgs& p, int dtype, bool ragged) {
+    split_forward(p, dtype);
+    const int64_t blocks = ceil_div(p.N, rows_of_queries(dtype)) * p.B * p.H;
+    if (p.splits == 1 && p.M > 512 && blocks <= 768 && (blocks > 512 || ragged)) p.splits = 2;
+}
+
 static int qattn_expanded(const AttnArgs& all, int dtype, int bits, void* workspace, hipStream_t stream) {
     const int64_t slice = expand_slice(all.B, all.M, all.G, all.D), row = all.G * all.D, codes = row * bits / 8;
     const int64_t scales = all.G * qcache::row_scales(all.D);
@@ -230,7 +240,7 @@ static int qattn_expanded(const AttnArgs& all, int dtype, int bits, void* worksp
         int rc = qcache::qcache_expand(p, dtype, bits, k, v, stream);
         if (rc != FLARE_OK) return rc;
         p.k = {k, p.M * row, row, p.D}, p.v = {v, p.M * row, row, p.D};
-        split_forward(p, dtype);
+        split_expanded(p, dtype, p.fresh != nullptr);
         p.parts = (float*)(k + expanded_bytes(slice, p.M, p.G, p.D));
         rc = dtype == FLARE_BF16 ? forward_e<__hip_bfloat16>(p, stream) : forward_e<__half>(p, stream);
         if (rc != FLARE_OK) return rc;
@@ -414,7 +424,8 @@ extern "C" size_t flare_qattn_workspace_size(int64_t B, int64_t N, int64_t M, in
     size_t most = 0;
     // (the last slice may be smaller and split its keys more often)
     for (const int64_t left = path == kFused ? B : B % p.B ? B % p.B : p.B;; p.B = left) {
-        split_forward(p, dtype);
+        if (path == kFused) split_forward(p, dtype);
+        else split_expanded(p, dtype, true);
         most = rows_bytes(p) > most ? rows_bytes(p) : most;
         if (p.B == left) break;
     }

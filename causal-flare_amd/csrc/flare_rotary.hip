@@ -68,12 +68,17 @@ struct alignas(V * sizeof(T)) Vec {
     T v[V];
 };
 
+// Heads a thread turns, where there is work for more threads than the card takes at once: four vectors of loads
+// under way.  us of 4 x 4096 tokens, 16 and 4 heads of 128, bf16: pairs of halves with 2, 4 and 8 heads 36, 41, 45;
+// adjacent pairs with 2, 4 and 8 39, 31, 32 (a copy of these 168 MB takes 34).  Stores that pass by the last-level
+// cache take 33, and what reads the result then takes that much longer.
+constexpr int heads_of(bool interleaved) { return interleaved ? 4 : 2; }
+
 // V: elements of a vector; 1: element by element, whatever the strides.
-// A thread turns the same pairs of heads part, part + parts, ..: the angles are computed once for them,
-// and kBatch heads' loads are under way at a time.
+// A thread turns the same pairs of heads part, part + parts, ..: the angles are computed once for them.
 template <typename T, int V, bool INTERLEAVED>
 __global__ __launch_bounds__(256) void rotary_kernel(Args p) {
-    constexpr int kBatch = 4, PAIRS = INTERLEAVED && V > 1 ? V / 2 : V, VECS = INTERLEAVED && V > 1 ? 1 : 2;
+    constexpr int kBatch = heads_of(INTERLEAVED), PAIRS = INTERLEAVED && V > 1 ? V / 2 : V, VECS = INTERLEAVED && V > 1 ? 1 : 2;
     typedef Vec<T, V> W;
     const int per = p.units * p.parts, tokens = 256 / per;
     const int within = threadIdx.x % per, unit = within % p.units, part = within / p.units;
@@ -140,9 +145,9 @@ static int launch(Args p, hipStream_t stream) {
     const int heads = p.H + p.G;
     const int pairs = p.interleaved && V > 1 ? V / 2 : V;
     p.units = p.R / 2 / pairs + (p.D - p.R) / V;
-    // a head a thread where that leaves no more than the card takes at once, four otherwise
+    // a head a thread where that leaves no more than the card takes at once
     const int64_t all = p.B * p.N * heads * p.units;
-    const int want = all <= 256 * 1024 ? heads : (heads + 3) / 4;
+    const int each = heads_of(p.interleaved), want = all <= 256 * 1024 ? heads : (heads + each - 1) / each;
     p.parts = 256 / p.units < want ? 256 / p.units : want;
     const int64_t blocks = ceil_div(p.B * p.N, 256 / (p.units * p.parts));
     if (blocks > INT32_MAX) {
