@@ -16,34 +16,36 @@ struct Cache {
     uint8_t *k, *v, *k_scale, *v_scale;
 };
 
-// blockIdx.z: a sequence; y: keys or values; x: quads of its rows.
+// blockIdx.y: a sequence; x: quads of its rows, each of a key and of its value.
 template <typename T, int BITS>
 __global__ __launch_bounds__(256) void qcache_write_kernel(Rows k, Rows v, const int32_t* lengths, const int32_t* fresh,
                                                            unsigned N, int64_t M, unsigned G, unsigned D, Cache to) {
-    const unsigned NB = (D + kBlock - 1) / kBlock, b = blockIdx.z;
+    const unsigned NB = (D + kBlock - 1) / kBlock, b = blockIdx.y;
     const unsigned id = blockIdx.x * 256 + threadIdx.x, quad = id >> 2, block = quad % NB, g = quad / NB % G;
     const unsigned t = quad / NB / G, d = block * kBlock + (id & 3) * 8;
     const int64_t off = lengths[b], n = fresh ? clamp_to(fresh[b], N) : N;
     if (off < 0 || off + n > M || t >= n) return;                       // a quad at a time
-    const Rows from = blockIdx.y ? v : k;
-    float x[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
-    if (d < D) load8((const T*)from.p + b * from.sb + t * from.sn + g * from.sh + d, x);
-    const u32 byte = scale_of<BITS>(quad_max(top_of(x)), __is_same(T, __half));
-    const int64_t row = ((int64_t)b * M + off + t) * G + g;
+    float x[2][8] = {};
     if (d < D) {
-        const Codes<BITS> c = encode<BITS>(x, byte);
-        *reinterpret_cast<Codes<BITS>*>((blockIdx.y ? to.v : to.k) + row * (D * BITS / 8) + d * BITS / 8) = c;
+        load8((const T*)k.p + b * k.sb + t * k.sn + g * k.sh + d, x[0]);
+        load8((const T*)v.p + b * v.sb + t * v.sn + g * v.sh + d, x[1]);
     }
-    if ((id & 3) == 0) (blockIdx.y ? to.v_scale : to.k_scale)[row * NB + block] = (uint8_t)byte;
+    const int64_t row = ((int64_t)b * M + off + t) * G + g;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const u32 byte = scale_of<BITS>(quad_max(top_of(x[i])), __is_same(T, __half));
+        if (d < D) *reinterpret_cast<Codes<BITS>*>((i ? to.v : to.k) + row * (D * BITS / 8) + d * BITS / 8) = encode<BITS>(x[i], byte);
+        if ((id & 3) == 0) (i ? to.v_scale : to.k_scale)[row * NB + block] = (uint8_t)byte;
+    }
 }
 
-// Rows first[b] .. first[b] + N - 1 of each sequence; 0 outside of it.  Eight values a thread.  With `lengths`
-// those that a sequence of so many tokens and `fresh` (or all N_new) new ones holds, and no others.
+// Rows first[b] .. first[b] + N - 1 of each sequence; 0 outside of it.  Eight values of a key and of its value a
+// thread.  With `lengths` those that a sequence of so many tokens and `fresh` (or all N_new) new ones holds, and no others.
 template <typename T, int BITS>
 __global__ __launch_bounds__(256) void qcache_read_kernel(Cache from, const int32_t* first, unsigned N, int64_t M, unsigned G,
                                                           unsigned D, const int32_t* lengths, const int32_t* fresh,
                                                           int64_t N_new, T* k, T* v) {
-    const unsigned per = D / 8, NB = (D + kBlock - 1) / kBlock, b = blockIdx.z;
+    const unsigned per = D / 8, NB = (D + kBlock - 1) / kBlock, b = blockIdx.y;
     const unsigned id = blockIdx.x * 256 + threadIdx.x, d = id % per * 8, g = id / per % G, t = id / per / G;
     if (t >= N) return;
     if (lengths) {
@@ -51,28 +53,32 @@ __global__ __launch_bounds__(256) void qcache_read_kernel(Cache from, const int3
         if (off < 0 || t >= off + n) return;
     }
     const int64_t at = (first ? (int64_t)first[b] : 0) + t;
-    f32x8 x = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+    f32x8 x[2] = {};
     if (at >= 0 && at < M) {
-        const int64_t row = ((int64_t)b * M + at) * G + g;
-        const Codes<BITS> c = *reinterpret_cast<const Codes<BITS>*>((blockIdx.y ? from.v : from.k) + row * (D * BITS / 8) +
-                                                                    d * BITS / 8);
-        x = decode<BITS>(c.w, scale_value((blockIdx.y ? from.v_scale : from.k_scale)[row * NB + d / kBlock]), float{});
+        const int64_t row = ((int64_t)b * M + at) * G + g, codes = row * (D * BITS / 8) + d * BITS / 8, scale = row * NB + d / kBlock;
+        const Codes<BITS> c = *reinterpret_cast<const Codes<BITS>*>(from.k + codes);
+        const Codes<BITS> w = *reinterpret_cast<const Codes<BITS>*>(from.v + codes);
+        x[0] = decode<BITS>(c.w, scale_value(from.k_scale[scale]), float{});
+        x[1] = decode<BITS>(w.w, scale_value(from.v_scale[scale]), float{});
     }
-    T* to = (blockIdx.y ? v : k) + (((int64_t)b * N + t) * G + g) * D + d;
+    const int64_t to = (((int64_t)b * N + t) * G + g) * D + d;
     constexpr int PER = 16 / sizeof(T);
 #pragma unroll
-    for (int i = 0; i < 8; i += PER) {
-        float o[PER];
+    for (int j = 0; j < 2; ++j) {
 #pragma unroll
-        for (int e = 0; e < PER; ++e) o[e] = x[i + e];
-        mix::store_row<T, PER>(to + i, o);
+        for (int i = 0; i < 8; i += PER) {
+            float o[PER];
+#pragma unroll
+            for (int e = 0; e < PER; ++e) o[e] = x[j][i + e];
+            mix::store_row<T, PER>((j ? v : k) + to + i, o);
+        }
     }
 }
 
 template <typename T>
 static int write_type(const Rows& k, const Rows& v, int bits, const int32_t* lengths, const int32_t* fresh, int64_t B,
                       int64_t N, int64_t M, int64_t G, int64_t D, const Cache& to, hipStream_t stream) {
-    const dim3 grid((unsigned)ceil_div(N * G * row_scales(D) * 4, 256), 2, (unsigned)B);
+    const dim3 grid((unsigned)ceil_div(N * G * row_scales(D) * 4, 256), (unsigned)B);
     const auto kernel = bits == 8 ? qcache_write_kernel<T, 8> : qcache_write_kernel<T, 4>;
     kernel<<<grid, 256, 0, stream>>>(k, v, lengths, fresh, (unsigned)N, M, (unsigned)G, (unsigned)D, to);
     return check_launch("qcache_write");
@@ -80,7 +86,7 @@ static int write_type(const Rows& k, const Rows& v, int bits, const int32_t* len
 template <typename T>
 static int read_type(const Cache& from, int bits, const int32_t* first, int64_t B, int64_t N, int64_t M, int64_t G, int64_t D,
                      const int32_t* lengths, const int32_t* fresh, int64_t N_new, void* k, void* v, hipStream_t stream) {
-    const dim3 grid((unsigned)ceil_div(N * G * D / 8, 256), 2, (unsigned)B);
+    const dim3 grid((unsigned)ceil_div(N * G * D / 8, 256), (unsigned)B);
     const auto kernel = bits == 8 ? qcache_read_kernel<T, 8> : qcache_read_kernel<T, 4>;
     kernel<<<grid, 256, 0, stream>>>(from, first, (unsigned)N, M, (unsigned)G, (unsigned)D, lengths, fresh, N_new,
                                       (T*)k, (T*)v);
