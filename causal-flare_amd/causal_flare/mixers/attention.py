@@ -42,7 +42,7 @@ from ._inputs import (
     _strides,
     _training,
 )
-from .quantized import attend_quantized, is_quantized, step_fast
+from .quantized import attend_fast, attend_quantized, is_quantized
 
 
 # Caps that the kernels take: what scale / cap and the cap itself can be with in float32.
@@ -211,9 +211,15 @@ def softmax_attention_prefill(
     written at all, and its y is NaN.
     """
     name = "softmax_attention_prefill"
+    quantized = is_quantized(cache)
+    if quantized and Q.dim() == 4 and (softcap is None or _LEAST_CAP <= softcap <= _MOST_CAP):
+        y = attend_fast(Q, K, V, cache, lengths, _resolve_attn_scale(scale, Q.shape[-1]), softcap, slopes, prefix_lengths,
+                        new_lengths)
+        if y is not None:
+            return y, cache
     B, T, H, G, D = _check_heads(name, Q, K, V)
     cap = _check_scores(name, H, scale, softcap, slopes)
-    if is_quantized(cache):
+    if quantized:
         _check_integers(name, "prefix_lengths", prefix_lengths, (B,))
         _check_integers(name, "new_lengths", new_lengths, (B,))
         return attend_quantized(name, Q, K, V, cache, lengths, _resolve_attn_scale(scale, D), cap, slopes, prefix_lengths,
@@ -315,8 +321,8 @@ def softmax_attention_decode(
         out = _step_fast(Q, K, V, cache, lengths, scale, softcap, slopes)
         if out is not None:
             return out
-    elif softcap is None or _LEAST_CAP <= softcap <= _MOST_CAP:
-        y = step_fast(Q, K, V, cache, lengths, _resolve_attn_scale(scale, Q.shape[-1]), softcap, slopes)
+    elif (Q.dim() == 3 or (Q.dim() == 4 and Q.shape[1] == 1)) and (softcap is None or _LEAST_CAP <= softcap <= _MOST_CAP):
+        y = attend_fast(Q, K, V, cache, lengths, _resolve_attn_scale(scale, Q.shape[-1]), softcap, slopes, None, None)
         if y is not None:
             return y, cache
     Q, K, V = (t[:, None] if t.dim() == 3 else t for t in (Q, K, V))

@@ -107,25 +107,30 @@ def _plain_parts(cache, device):
     return None if (pointers[0] | pointers[2]) % 16 else (bits, B, S, G, D, pointers)
 
 
-def step_fast(Q, K, V, cache, lengths, scale, softcap, slopes):
-    """y of the common single token, or None: one type, rows and a cache that the kernel reads in place, int32 lengths.
-    softcap: None or within the kernels' range."""
+def _plain_int32(t, device, B):
+    return t is None or (isinstance(t, torch.Tensor) and t.dtype is torch.int32 and t.shape == (B,) and t.device == device
+                         and t.is_contiguous())
+
+
+def attend_fast(Q, K, V, cache, lengths, scale, softcap, slopes, prefix_lengths, new_lengths):
+    """y [B, T, H, D] of the common call, or None: one type, rows and a cache that the kernels read in place, on the
+    current device, int32 lengths; Q, K, V of T tokens or, without that dimension, of one.  softcap: None or within the
+    kernels' range."""
     dtype, device, shape = Q.dtype, Q.device, Q.shape
     code = _CODES.get(dtype)
-    if code is None or device.type != "cuda" or device.index != torch.cuda.current_device():
+    if (code is None or device.type != "cuda" or device.index != torch.cuda.current_device() or lengths is None
+            or len(shape) not in (3, 4)):
         return None
     parts = _plain_parts(cache, device)
-    if parts is None or not isinstance(lengths, torch.Tensor):
+    if parts is None:
         return None
     bits, B, S, G, D, held = parts
-    token = len(shape) == 4
-    if len(shape) not in (3, 4) or (token and shape[1] != 1):
-        return None
-    H = shape[-2]
-    want = (B, 1, G, D) if token else (B, G, D)
-    if (shape[0] != B or shape[-1] != D or H < 1 or H % G or K.shape != want or V.shape != want
-            or lengths.dtype is not torch.int32 or lengths.shape != (B,) or lengths.device != device
-            or not lengths.is_contiguous()):
+    many = len(shape) == 4
+    T, H = shape[1] if many else 1, shape[-2]
+    want = (B, T, G, D) if many else (B, G, D)
+    if (shape[0] != B or shape[-1] != D or T < 1 or H < 1 or H % G or K.shape != want or V.shape != want
+            or not (_plain_int32(lengths, device, B) and _plain_int32(prefix_lengths, device, B)
+                    and _plain_int32(new_lengths, device, B))):
         return None
     if slopes is not None and (not _plain_f32(slopes, device, H) or slopes.requires_grad):
         return None
@@ -133,19 +138,21 @@ def step_fast(Q, K, V, cache, lengths, scale, softcap, slopes):
     for t in (Q, K, V):
         if t.stride(-1) != 1 or t.dtype is not dtype or t.device != device:
             return None
-        a, b = t.stride(0), t.stride(-2)
-        strides += (a, 0, b)
-        spread |= a | b
+        a, b, c = t.stride(0), t.stride(1) if many else 0, t.stride(-2)
+        if b >= 1 << 22:
+            return None
+        strides += (a, b, c)
+        spread |= a | b | c
     pointers = (Q.data_ptr(), K.data_ptr(), V.data_ptr())
     if (spread * Q.element_size() | pointers[0] | pointers[1] | pointers[2]) % 16:
         return None
-    y = torch.empty((B, 1, H, D), device=device, dtype=dtype)
+    y = torch.empty((B, T, H, D), device=device, dtype=dtype)
     lib = _lib.lib()
-    nbytes = lib.flare_qattn_workspace_size(B, 1, S, H, G, D, code)
+    nbytes = lib.flare_qattn_workspace_size(B, T, S, H, G, D, code)
     ws = torch.empty(nbytes, device=device, dtype=torch.uint8) if nbytes else None
     rc = lib.flare_qattn(
-        *pointers, _strides(*strides), code, bits, B, 1, S, H, G, D, scale, softcap or 0.0, _ptr(slopes), None,
-        lengths.data_ptr(), None, *held, y.data_ptr(), _ptr(ws), nbytes, _raw_stream(device.index))
+        *pointers, _strides(*strides), code, bits, B, T, S, H, G, D, scale, softcap or 0.0, _ptr(slopes), _ptr(prefix_lengths),
+        lengths.data_ptr(), _ptr(new_lengths), *held, y.data_ptr(), _ptr(ws), nbytes, _raw_stream(device.index))
     if rc:
         _lib.check(rc, "flare_qattn")
     return y

@@ -188,6 +188,19 @@ def test_decode_scores(dtype, bits, cap, slopes):
 
 
 @pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("H, G, D, B, S", [(16, 4, 64, 36, 500), (8, 8, 48, 17, 300), (12, 6, 96, 30, 300), (4, 4, 128, 33, 70),
+                                           (4, 4, 32, 800, 40), (2, 2, 16, 800, 37)])
+def test_decode_of_many_sequences(dtype, bits, H, G, D, B, S):
+    # key heads side by side in a workgroup, with their keys in one share and in several
+    at = torch.randint(-1, S + 1, (B,), generator=rng(B)).tolist()
+    check_attention(dtype, bits, H, G, D, S, 1, at, seed=D, decode=True, cap=30.0 if D == 64 else None,
+                    slopes=[2.0 ** -(1 + h % 8) for h in range(H)] if D == 96 else None)
+    if H // G > 1:
+        check_attention(dtype, bits, H, G, D, S, 2, at[:32] if B > 32 else at, seed=D)
+
+
+@pytest.mark.parametrize("bits", [4, 8])
 def test_decode_of_large_scores(bits):
     # weights that move the reference again and again, and rows whose first keys count for nothing
     check_attention("bf16", bits, 4, 1, 128, 900, 1, [899, 640], seed=5, decode=True, q_std=60.0)
@@ -271,6 +284,62 @@ def test_nan_reaches_the_rows_that_see_it(dtype, bits):
     _visible_nan(dtype, bits, 150, 2, 1, 64, 400, 130, [(70, 5, math.nan), (149, 63, math.inf)])
     _visible_nan(dtype, bits, 200, 2, 2, 96, 400, 130, [(70, 5, math.nan), (199, 63, math.inf)])
     _visible_nan(dtype, bits, 256, 8, 1, 64, 400, 130, [(70, 5, math.nan), (255, 63, math.inf)])
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("T, H, G, D", [(6, 4, 2, 128), (200, 2, 2, 96), (256, 8, 1, 64)])
+def test_nan_keys_reach_the_rows_that_see_them(dtype, bits, T, H, G, D):
+    dt, g = TYPES[dtype], rng(5)
+    off, S = 60, T + 70
+    k, v, q = normal(g, 1, T, G, D, dtype=dt), normal(g, 1, T, G, D, dtype=dt), normal(g, 1, T, H, D, dtype=dt)
+    at = T - 3
+    bad = k.clone()
+    bad[0, at, 0, 7] = math.inf
+    old = [normal(g, 1, off, G, D, dtype=dt).cuda() for _ in range(2)]
+    out = []
+    for keys in (k, bad):
+        cache = cf.quantized_cache(1, S, G, D, bits)
+        cf.quantized_cache_write(cache, *old, ints(0))
+        out.append(cf.softmax_attention_prefill(q.cuda(), keys.cuda(), v.cuda(), cache, ints(off))[0].cpu())
+    want = torch.zeros((1, T, H, D), dtype=torch.bool)
+    want[0, at:, :H // G] = True
+    assert torch.equal(torch.isnan(out[1]), want)
+    assert torch.equal(out[1][~want], out[0][~want])
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("T, H, G, D", [(1, 4, 2, 64), (6, 4, 2, 128), (200, 2, 2, 96), (256, 8, 1, 64)])
+def test_infinite_queries(dtype, T, H, G, D):
+    """A query with an infinite element: its scores are infinite, or of the cap; other rows know nothing of it."""
+    dt, g = TYPES[dtype], rng(15)
+    off, S = 60, T + 70
+    k, v, q = normal(g, 1, T, G, D, dtype=dt), normal(g, 1, T, G, D, dtype=dt), normal(g, 1, T, H, D, dtype=dt)
+    old = [normal(g, 1, off, G, D, dtype=dt) for _ in range(2)]
+    for x in (k, old[0]):
+        x[..., 5] = torch.where(x[..., 5].abs() < 0.25, 0.25, x[..., 5])       # no code of 0 there
+    t0, h0 = T // 2, H - 1
+    odd = q.clone()
+    odd[0, t0, h0, 5] = -math.inf
+    for cap in (None, 7.0):
+        out = []
+        for queries in (q, odd):
+            cache = cf.quantized_cache(1, S, G, D, 8)
+            cf.quantized_cache_write(cache, *(x.cuda() for x in old), ints(0))
+            out.append(cf.softmax_attention_prefill(queries.cuda(), k.cuda(), v.cuda(), cache, ints(off), softcap=cap)[0].cpu())
+        rest = torch.ones((1, T, H, D), dtype=torch.bool)
+        rest[0, t0, h0] = False
+        assert torch.equal(out[0][rest], out[1][rest])
+        n = off + t0 + 1
+        kk, vv = (Q.held(cache[x][0, :n, -1], cache[x + "_scale"][0, :n, -1]) for x in ("k", "v"))
+        assert (kk[:, 5] != 0).all() and (kk[:, 5] < 0).any()
+        if cap is None:
+            assert torch.isnan(out[1][0, t0, h0]).all()           # one of the scores is +inf
+        else:
+            w = torch.softmax(-cap * torch.sign(kk[:, 5]), 0)
+            ref, mag = w @ vv, w @ vv.abs()
+            u = M.U[dt] if dt is not torch.float32 else 0.0
+            M.check(out[1][0, t0, h0], ref, (u + 2.0 ** -18) * mag + M.U[dt] * ref.abs(), "y", dt)
 
 
 @pytest.mark.parametrize("T, pieces", [(150, (70, 1, 9, 66, 4)), (20, (1,) * 20)])

@@ -90,6 +90,9 @@ QKV = [t(2, 5, 4, 32)] * 3
     (lambda: cf.softmax_attention_prefill(*QKV, cache(), ints(2), new_lengths=t(2)), ValueError, "integers"),
     (lambda: cf.softmax_attention_prefill(*QKV, cache(), ints(2)), RuntimeError, CPU),
     (lambda: cf.softmax_attention_decode(*QKV, cache(), ints(2)), ValueError, "one token"),
+    (lambda: cf.softmax_attention_decode(*[t(32)] * 3, cache(), ints(2)), ValueError, "expects Q"),
+    (lambda: cf.softmax_attention_decode(t(), t(), t(), cache(), ints(2)), ValueError, "expects Q"),
+    (lambda: cf.softmax_attention_prefill(*[t(2, 4, 32)] * 3, cache(), ints(2)), ValueError, "expects Q"),
     (lambda: cf.softmax_attention_decode(*[t(2, 4, 32)] * 3, cache(8), ints(3)), ValueError, "lengths"),
     (lambda: cf.softmax_attention_decode(*[t(2, 4, 32)] * 3, cache(8), ints(2)), RuntimeError, CPU),
 ])
