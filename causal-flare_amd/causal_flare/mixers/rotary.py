@@ -85,6 +85,10 @@ def _launch(q, k, dtype, frequencies, positions, lengths, interleaved, inverse):
 
 def _turn(q, k, frequencies, positions, lengths, interleaved, inverse):
     """The pairs of q [B, N, H, D] and k [B, N, G, D] (or None) turned; each keeps its type."""
+    dtype = q.dtype
+    if (k is not None and dtype in _CODES and k.dtype is dtype and q.stride(-1) == 1 and k.stride(-1) == 1
+            and q.device.index == torch.cuda.current_device()):
+        return _launch(q, k, dtype, frequencies, positions, lengths, interleaved, inverse)
     dtype = _compute_dtype(q, k)
     with _on(q.device):
         y, z = _launch(_rows(q, dtype), _rows(k, dtype), dtype, frequencies, positions, lengths, interleaved, inverse)

@@ -170,38 +170,52 @@ static int64_t step_splits(int64_t B, int64_t M, int64_t H, int64_t G) {
     return s < 1 ? 1 : (s > most ? most : s);
 }
 
+// Tiles of 16 rows (token, head) a wave of qattn_rows owns.
 static int row_tiles(int64_t N, int64_t H, int64_t G, int dtype) { return H / G * N > 16 && dtype != FLARE_F32 ? 2 : 1; }
-// Which kernel takes N new tokens over a cache of 8 or 4 bits.  kRows: rows (token, head) of the heads that share keys
-// in groups of 16 or 32, whose codes go straight into operands.  kFused: attn_forward with the codes turned into values
-// as they go to LDS, once for each 128 tokens of each head.  kExpanded: attn_forward over 16-bit values that the
-// codes are turned into first.
-//   A group of 32 rows takes a third of what 128 rows of a head take.  us, fused and by rows, 16 heads of 128 over 4, 4
-// bits: 16 x 8192 cached tokens, 32 new 177, 86; 64 new 185, 124; 128 new 195, 232; one sequence of 1000, 64 new
-// 31, 21.  fp32 queries: 16 x 4096 cached, 8 heads of 64, 32 new 106, 55; 512 new 595, 304, so these always go by rows.
+
+// Which kernel takes N new tokens over a cache of 8 or 4 bits.  kRows: rows of the heads that share keys, in groups of 16
+// or 32, whose codes go straight into operands.  kFused: attn_forward with the codes turned into values as they go to
+// LDS, once for each 128 tokens of each head.  kExpanded: attn_forward over 16-bit values that the codes are turned
+// into first.
+//   A group of 32 rows takes a third of what 128 tokens of a head take.  us, fused and by rows, 16 heads of 128 over 4,
+// 4 bits, behind 8192 tokens of 16 sequences: 32 new tokens 177, 86; 64 185, 124; 128 195, 232; behind 1000 of one, 64 31,
+// 21.  fp32 queries, 8 heads of 64, behind 4096 of 16: 32 new tokens 106, 55; 512 595, 304: these always go by rows.
+//   Values turned into 16 bits once pay from 16 blocks that read them.  us, fused and expanded: 16 x 256 new tokens behind
+// 8192, 348, 396; 512 (16 blocks) 684, 689; 2048 2512, 2218; one sequence, 1024 behind 15,300 191, 180; 2048 351, 317.
 enum { kRows, kFused, kExpanded };
-constexpr int64_t kExpandRows = 16;
-static int qattn_path(int64_t N, int64_t H, int64_t G, int dtype) {
+constexpr int64_t kExpandBlocks = 16, kMostExpanded = (int64_t)8 << 30;      // bytes of one sequence's values
+static int64_t expanded_row(int64_t G, int64_t D) { return 2 * 2 * G * D; }  // of a token, k and v
+static int qattn_path(int64_t N, int64_t M, int64_t H, int64_t G, int64_t D, int dtype) {
     const int64_t R = H / G, blocks = R * ceil_div(N, 128);
     if (dtype == FLARE_F32 || ceil_div(R * N, 32) <= 3 * blocks) return kRows;
-    return blocks < kExpandRows ? kFused : kExpanded;
+    return blocks < kExpandBlocks || M * expanded_row(G, D) > kMostExpanded ? kFused : kExpanded;
 }
 // Sequences that are expanded at a time: 1 GiB of values, or one.
 static int64_t expand_slice(int64_t B, int64_t M, int64_t G, int64_t D) {
-    const int64_t s = (int64_t)(1 << 30) / (M * G * D * 4);
+    const int64_t s = (int64_t)(1 << 30) / (M * expanded_row(G, D));
     return s < 1 ? 1 : (s > B ? B : s);
 }
-static size_t expanded_bytes(int64_t B, int64_t M, int64_t G, int64_t D) { return (size_t)(B * M * G * D * 4 + 255) / 256 * 256; }
-// Key heads of the same tokens that the waves of a workgroup take side by side.
-static int64_t rows_heads(int64_t B, int64_t N, int64_t H, int64_t G, int tiles) {
+static size_t expanded_bytes(int64_t B, int64_t M, int64_t G, int64_t D) {
+    return (size_t)(B * M * expanded_row(G, D) + 255) / 256 * 256;
+}
+
+// Key heads of the same tokens that the waves of a workgroup take side by side: their rows share lines of memory, which
+// tells where bytes bound the call.  us, one head a workgroup and four, 16 heads of 64 of 16 x 4096 tokens, 8 bits: 48,
+// 40; 16 of 128 over 4 of 64 x 8192, 4 bits: 66, 66; one sequence of 1000: 10.6, 13.6, as its keys have fewer waves then.
+static int64_t rows_heads(int64_t B, int64_t G, int tiles) {
     if (tiles > 1 || B * G < 128) return 1;
     return G % 4 == 0 ? 4 : G % 2 == 0 ? 2 : 1;
 }
-// Workgroups for each sequence's keys, as step_splits.
+// Workgroups for each sequence's keys: three on a CU (two with two tiles a wave), with shares of 256 keys a head, or of
+// 128 until there are 32.  us, workgroups of 512, 768 and 1024: 64 x 8192 tokens, 4 key heads of 128, 4 bits 76, 66, 70;
+// 16 x 8192, five tokens, 8 bits (two tiles) 45, 55, 54.  Shares of 128 and of 256 for one sequence of 1000 10.0, 11.1; of
+// 4000 10.5, 11.7; of 16384 (128 and 64 of them) 14.4, 12.5.
 static int64_t rows_splits(int64_t B, int64_t N, int64_t M, int64_t H, int64_t G, int dtype) {
     const int tiles = row_tiles(N, H, G, dtype);
-    const int64_t heads = rows_heads(B, N, H, G, tiles);
-    const int64_t rows = B * (G / heads) * ceil_div(H / G * N, 16 * tiles);
-    const int64_t s = ceil_div(tiles == 1 ? 768 : 512, rows), most = ceil_div(M, 256 / heads);
+    const int64_t heads = rows_heads(B, G, tiles), rows = B * (G / heads) * ceil_div(H / G * N, 16 * tiles);
+    const int64_t s = ceil_div(tiles == 1 ? 768 : 512, rows), small = ceil_div(M, 128);
+    int64_t most = ceil_div(M, 256 / heads);
+    if (heads == 1 && most < 32) most = small < 32 ? small : 32;
     return s < 1 ? 1 : (s > most ? most : s);
 }
 template <typename E>
@@ -224,6 +238,7 @@ static void split_expanded(AttnArgs& p, int dtype, bool ragged) {
 }
 
 static int qattn_expanded(const AttnArgs& all, int dtype, int bits, void* workspace, hipStream_t stream) {
+    // one slice of sequences after another, in the same workspace
     const int64_t slice = expand_slice(all.B, all.M, all.G, all.D), row = all.G * all.D, codes = row * bits / 8;
     const int64_t scales = all.G * qcache::row_scales(all.D);
     for (int64_t b = 0; b < all.B; b += slice) {
@@ -414,7 +429,7 @@ extern "C" int flare_attn_step(const void* q, const void* k, const void* v, cons
 
 extern "C" size_t flare_qattn_workspace_size(int64_t B, int64_t N, int64_t M, int64_t H, int64_t G, int64_t D, int dtype) {
     if (B < 1 || N < 1 || M < 1 || H < 1 || G < 1 || H % G) return 0;
-    const int path = qattn_path(N, H, G, dtype);
+    const int path = qattn_path(N, M, H, G, D, dtype);
     if (path == kRows) {
         const int64_t s = rows_splits(B, N, M, H, G, dtype);
         return s == 1 ? 0 : (size_t)(B * N * H * s * (D + 4)) * sizeof(float);
@@ -455,7 +470,7 @@ extern "C" int flare_qattn(const void* q, const void* k, const void* v, const in
     p.k_scale = (uint8_t*)k_scale, p.v_scale = (uint8_t*)v_scale;
     p.lengths = lengths, p.fresh = new_lengths, p.prefix = prefix_lengths, p.causal = 1;
     p.y = y, p.parts = (float*)workspace;
-    const int path = qattn_path(N, H, G, dtype);
+    const int path = qattn_path(N, M, H, G, D, dtype);
     // one token's key and value are quantised on the way
     if (N == 1 && path == kRows && !new_lengths) {
         p.k_new = k, p.kn_sb = strides[3], p.kn_sg = strides[5];
@@ -466,7 +481,7 @@ extern "C" int flare_qattn(const void* q, const void* k, const void* v, const in
         if (rc != FLARE_OK) return rc;
     }
     if (path == kRows) {
-        p.splits = rows_splits(B, N, M, H, G, dtype), p.row_splits = rows_heads(B, N, H, G, row_tiles(N, H, G, dtype));
+        p.splits = rows_splits(B, N, M, H, G, dtype), p.row_splits = rows_heads(B, G, row_tiles(N, H, G, dtype));
         return FLARE_BY_DTYPE(dtype, qattn_rows, (p, bits, row_tiles(N, H, G, dtype), (hipStream_t)stream));
     }
     if (path == kExpanded) return qattn_expanded(p, dtype, bits, workspace, (hipStream_t)stream);

@@ -19,9 +19,10 @@
 namespace flare {
 namespace attn {
 
-// What Stage does, from a cache of 8 or 4 bits: codes to LDS as the values they stand for, a unit of 16 of
+// What Stage does, from a cache of 8 or 4 bits: codes to LDS as the 16-bit values they stand for, a unit of 16 of
 // them a thread at a time.  Rows that are none, columns behind D, and blocks that are NaN where `clean` is
-// called, become 0.
+// called, become 0.  Each block of queries of each head turns the codes anew: 16% of a long prompt's time (620
+// against 534 us over 16-bit keys and values, 4096 rows of 16 heads of 128 over 4 behind 11,000).
 template <typename E, int BITS, int ROWS, int DP, int PITCH, int NT>
 struct CodeStage {
     typedef typename Elem<E>::S S;
@@ -34,7 +35,7 @@ struct CodeStage {
     u32 second;
     __device__ __forceinline__ void begin(int64_t G, int64_t D, int tid) {
         const u32 codes = (u32)(G * qcache::row_codes(D, BITS)), scales = (u32)(G * qcache::row_scales(D));
-        second = sizeof(E) == 2 ? tid >> 2 & 1 : 0;
+        second = tid >> 2 & 1;
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             const int e = i * NT + tid, row = e / CPR, col = e % CPR * 16;
@@ -109,7 +110,7 @@ struct ForwardLds {
     static constexpr size_t bytes = 2 * (k_bytes + v_bytes + KT * sizeof(int)) + sizeof(int);
 };
 
-// BITS: of a cache of 8 or 4 bits (and no `ids`), 0 for keys and values of the queries' type.
+// BITS: of a cache of 8 or 4 bits (16-bit queries, no `ids`), 0 for keys and values of the queries' type.
 template <typename E, int DP, int QT, int KT, int CAP, int BITS>
 __global__ __launch_bounds__(256, 2) void attn_forward_kernel(AttnArgs p) {
     typedef typename Elem<E>::S S;
