@@ -193,7 +193,7 @@ def _declare(lib):
     lib.flare_qcache_read.restype = _i
     lib.flare_qcache_read.argtypes = [_vp] * 4 + [_i, _i] + [_i64] * 5 + [_vp] * 4
     lib.flare_qattn_workspace_size.restype = _sz
-    lib.flare_qattn_workspace_size.argtypes = [_i64] * 6 + [_i]
+    lib.flare_qattn_workspace_size.argtypes = [_i64] * 6 + [_i, _i]
     lib.flare_qattn.restype = _i
     lib.flare_qattn.argtypes = ([_vp] * 4 + [_i, _i] + [_i64] * 6 + [_f, _f] + [_vp] * 9 + [_vp, _sz, _vp])
 

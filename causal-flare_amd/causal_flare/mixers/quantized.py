@@ -148,7 +148,7 @@ def attend_fast(Q, K, V, cache, lengths, scale, softcap, slopes, prefix_lengths,
         return None
     y = torch.empty((B, T, H, D), device=device, dtype=dtype)
     lib = _lib.lib()
-    nbytes = lib.flare_qattn_workspace_size(B, T, S, H, G, D, code)
+    nbytes = lib.flare_qattn_workspace_size(B, T, S, H, G, D, code, bits)
     ws = torch.empty(nbytes, device=device, dtype=torch.uint8) if nbytes else None
     rc = lib.flare_qattn(
         *pointers, _strides(*strides), code, bits, B, T, S, H, G, D, scale, softcap or 0.0, _ptr(slopes), _ptr(prefix_lengths),
@@ -283,7 +283,7 @@ def attend_quantized(name, Q, K, V, cache, lengths, scale, cap, slopes, prefix_l
     q, k, v = (_aligned_rows(t, Q.dtype) for t in (Q, K, V))
     sl, pre, lens, new = _f32(slopes), _int32(prefix_lengths), _int32(lengths), _int32(new_lengths)
     lib, P = _lib.lib(), _ptr
-    nbytes = lib.flare_qattn_workspace_size(B, T, S, H, G, D, code)
+    nbytes = lib.flare_qattn_workspace_size(B, T, S, H, G, D, code, bits)
     ws = torch.empty(nbytes, device=device, dtype=torch.uint8) if nbytes else None
     with _on(device):
         rc = lib.flare_qattn(

@@ -200,20 +200,23 @@ static size_t expanded_bytes(int64_t B, int64_t M, int64_t G, int64_t D) {
 }
 
 // Key heads of the same tokens that the waves of a workgroup take side by side: their rows share lines of memory, which
-// tells where bytes bound the call.  us, one head a workgroup and four, 16 heads of 64 of 16 x 4096 tokens, 8 bits: 48,
-// 40; 16 of 128 over 4 of 64 x 8192, 4 bits: 66, 66; one sequence of 1000: 10.6, 13.6, as its keys have fewer waves then.
-static int64_t rows_heads(int64_t B, int64_t G, int tiles) {
-    if (tiles > 1 || B * G < 128) return 1;
+// tells where bytes bound the call.  us, one head a workgroup and four: 64 x 8192 tokens, 8 bits, 4 key heads of 128 110,
+// 100; 8 of 64 127, 112; in 4 bits 97, 80, and 4 of 128 67, 66; one sequence of 1000 10.6, 13.6, as its keys have fewer
+// waves then; 256 x 1024, 4 bits, 4 of 128 36, 44, as one head a workgroup needs no shares to be joined.
+static int64_t rows_heads(int64_t B, int64_t M, int64_t G, int tiles) {
+    if (tiles > 1 || B * G < 128 || (B * G >= 768 && M < 4096)) return 1;
     return G % 4 == 0 ? 4 : G % 2 == 0 ? 2 : 1;
 }
-// Workgroups for each sequence's keys: three on a CU (two with two tiles a wave), with shares of 256 keys a head, or of
-// 128 until there are 32.  us, workgroups of 512, 768 and 1024: 64 x 8192 tokens, 4 key heads of 128, 4 bits 76, 66, 70;
-// 16 x 8192, five tokens, 8 bits (two tiles) 45, 55, 54.  Shares of 128 and of 256 for one sequence of 1000 10.0, 11.1; of
+// Workgroups for each sequence's keys: three on a CU, two where a wave's tiles, parts or codes leave registers for no more,
+// with shares of 256 keys a head, or of 128 until there are 32.  us, workgroups of 512, 768 and 1024, 64 x 8192 tokens, 4 key
+// heads of 128: 4 bits 75, 66, 69; 8 bits 100, 106, 111; fp32 queries 80, 99, 86; five tokens, 8 bits, 16 x 8192 45,
+// 55, 54.  16 x 4096 in 8 bits, 16 heads of 64 43, 39, 41.  Shares of 128 and of 256 for one sequence of 1000 10.0, 11.1; of
 // 4000 10.5, 11.7; of 16384 (128 and 64 of them) 14.4, 12.5.
-static int64_t rows_splits(int64_t B, int64_t N, int64_t M, int64_t H, int64_t G, int dtype) {
+static int64_t rows_splits(int64_t B, int64_t N, int64_t M, int64_t H, int64_t G, int64_t D, int dtype, int bits) {
     const int tiles = row_tiles(N, H, G, dtype);
-    const int64_t heads = rows_heads(B, G, tiles), rows = B * (G / heads) * ceil_div(H / G * N, 16 * tiles);
-    const int64_t s = ceil_div(tiles == 1 ? 768 : 512, rows), small = ceil_div(M, 128);
+    const int64_t heads = rows_heads(B, M, G, tiles), rows = B * (G / heads) * ceil_div(H / G * N, 16 * tiles);
+    const bool three = tiles == 1 && dtype != FLARE_F32 && D * bits <= 512;
+    const int64_t s = ceil_div(three ? 768 : 512, rows), small = ceil_div(M, 128);
     int64_t most = ceil_div(M, 256 / heads);
     if (heads == 1 && most < 32) most = small < 32 ? small : 32;
     return s < 1 ? 1 : (s > most ? most : s);
@@ -427,11 +430,12 @@ extern "C" int flare_attn_step(const void* q, const void* k, const void* v, cons
     return attn_step(p, dtype, (hipStream_t)stream);
 }
 
-extern "C" size_t flare_qattn_workspace_size(int64_t B, int64_t N, int64_t M, int64_t H, int64_t G, int64_t D, int dtype) {
+extern "C" size_t flare_qattn_workspace_size(int64_t B, int64_t N, int64_t M, int64_t H, int64_t G, int64_t D, int dtype,
+                                             int bits) {
     if (B < 1 || N < 1 || M < 1 || H < 1 || G < 1 || H % G) return 0;
     const int path = qattn_path(N, M, H, G, D, dtype);
     if (path == kRows) {
-        const int64_t s = rows_splits(B, N, M, H, G, dtype);
+        const int64_t s = rows_splits(B, N, M, H, G, D, dtype, bits);
         return s == 1 ? 0 : (size_t)(B * N * H * s * (D + 4)) * sizeof(float);
     }
     AttnArgs p = {};
@@ -462,7 +466,7 @@ extern "C" int flare_qattn(const void* q, const void* k, const void* v, const in
     const uintptr_t held = (uintptr_t)k_cache | (uintptr_t)v_cache | (uintptr_t)y;
     FLARE_REQUIRE(aligned(p.q, dtype) && aligned(kr, dtype) && aligned(vr, dtype) && (held & 15) == 0,
                   "flare_qattn: rows must be 16-byte aligned and less than 2^22 elements apart");
-    if (workspace_bytes < flare_qattn_workspace_size(B, N, M, H, G, D, dtype) ||
+    if (workspace_bytes < flare_qattn_workspace_size(B, N, M, H, G, D, dtype, bits) ||
         (workspace_bytes && (!workspace || ((uintptr_t)workspace & 15)))) {
         set_error("flare_qattn: workspace of %zu bytes is too small or not 16-byte aligned", workspace_bytes);
         return FLARE_ERR_WORKSPACE;
@@ -481,7 +485,7 @@ extern "C" int flare_qattn(const void* q, const void* k, const void* v, const in
         if (rc != FLARE_OK) return rc;
     }
     if (path == kRows) {
-        p.splits = rows_splits(B, N, M, H, G, dtype), p.row_splits = rows_heads(B, G, row_tiles(N, H, G, dtype));
+        p.splits = rows_splits(B, N, M, H, G, D, dtype, bits), p.row_splits = rows_heads(B, M, G, row_tiles(N, H, G, dtype));
         return FLARE_BY_DTYPE(dtype, qattn_rows, (p, bits, row_tiles(N, H, G, dtype), (hipStream_t)stream));
     }
     if (path == kExpanded) return qattn_expanded(p, dtype, bits, workspace, (hipStream_t)stream);

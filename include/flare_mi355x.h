@@ -460,7 +460,7 @@ int flare_qcache_read(const void* k_cache, const void* k_scale, const void* v_ca
 /* Softmax attention of N new tokens a sequence over such a cache, which receives their k and v [B, N, G, D] first
  * (strides: batch, token and head of q, k, v; 9 numbers, host): the rows are seen as the cache holds them.
  * lengths, new_lengths, prefix_lengths and y as for flare_attn_append and flare_attn_forward. */
-size_t flare_qattn_workspace_size(int64_t B, int64_t N, int64_t M, int64_t H, int64_t G, int64_t D, int dtype);
+size_t flare_qattn_workspace_size(int64_t B, int64_t N, int64_t M, int64_t H, int64_t G, int64_t D, int dtype, int bits);
 int flare_qattn(const void* q, const void* k, const void* v, const int64_t* strides, int dtype, int bits, int64_t B,
                 int64_t N, int64_t M, int64_t H, int64_t G, int64_t D, float scale, float softcap, const float* slopes,
                 const int32_t* prefix_lengths, const int32_t* lengths, const int32_t* new_lengths, void* k_cache,

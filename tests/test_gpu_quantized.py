@@ -200,6 +200,27 @@ def test_decode_of_many_sequences(dtype, bits, H, G, D, B, S):
         check_attention(dtype, bits, H, G, D, S, 2, at[:32] if B > 32 else at, seed=D)
 
 
+@pytest.mark.parametrize("bits, dtype", [(4, "bf16"), (8, "fp32")])
+def test_decode_of_many_long_caches(bits, dtype):
+    """As many sequences as fill the card alone: key heads side by side, each sequence's keys in one workgroup."""
+    dt, g = TYPES[dtype], rng(21)
+    B, G, D, S = 256, 16, 16, 4100
+    cache = cf.quantized_cache(B, S, G, D, bits)
+    k, v, q = (normal(g, B, 40, G, D, dtype=dt).cuda() for _ in range(3))
+    lens = torch.randint(0, S, (B,), generator=g).int()
+    lens[:6] = torch.tensor([0, 1, S - 1, S, -1, 4000])
+    cf.quantized_cache_write(cache, k[:, 1:], v[:, 1:], (lens - 39).clamp_min(0).cuda())       # the last ones it holds
+    y, _ = cf.softmax_attention_decode(q[:, 0], k[:, 0], v[:, 0], cache, lens.cuda(), softcap=20.0)
+    assert torch.isnan(y[3]).all() and (y[4] == 0).all()
+    for b in (0, 1, 2, 5, 6, 77, 255):
+        n = int(lens[b]) + 1
+        kk, vv = (Q.held(cache[x][b:b + 1, :n], cache[x + "_scale"][b:b + 1, :n]) for x in ("k", "v"))
+        assert torch.equal(kk[:, n - 1], Q.rounded(k[b:b + 1, 0].cpu(), bits)[0])
+        ref, tol = M.attention(q[b:b + 1, :1], kk, vv, softcap=20.0, offset=[n - 1], unit=0.0 if dtype == "fp32" else M.U[dt],
+                               tiny=2.0 ** -126)["y"]
+        M.check(y[b:b + 1], ref, tol + M.U[dt] * ref.abs(), f"y of sequence {b}", dt)
+
+
 @pytest.mark.parametrize("bits", [4, 8])
 def test_decode_of_large_scores(bits):
     # weights that move the reference again and again, and rows whose first keys count for nothing

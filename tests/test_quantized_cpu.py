@@ -138,10 +138,10 @@ def test_c_entry_points_check_before_they_launch():
     assert _refused(attend(q=None), b"null pointer") and _refused(attend(bits=2), b"2 bits") and _refused(attend(H=6), b"divide")
     assert _refused(attend(D=200), b"multiple of 16") and _refused(attend(cap=-1.0), b"cap") and _refused(attend(kc=odd), b"16-byte")
     for n in (1, 9, 200):
-        need = lib.flare_qattn_workspace_size(1, n, 4096, 4, 4, 64, 1)
+        need = lib.flare_qattn_workspace_size(1, n, 4096, 4, 4, 64, 1, 4)
         assert need > 0 and need % 16 == 0
         assert attend(N=n) == -3 and attend(N=n, ws=P, size=need - 1) == -3 and attend(N=n, ws=odd, size=need) == -3
-    assert lib.flare_qattn_workspace_size(0, 1, 8, 4, 4, 64, 1) == 0 and lib.flare_qattn_workspace_size(1, 1, 8, 4, 3, 64, 1) == 0
+    assert lib.flare_qattn_workspace_size(0, 1, 8, 4, 4, 64, 1, 4) == 0 and lib.flare_qattn_workspace_size(1, 1, 8, 4, 3, 64, 1, 8) == 0
 
 
 def test_names():
