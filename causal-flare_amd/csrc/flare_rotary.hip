@@ -9,6 +9,9 @@
 // the point: its product with a whole position, without the turns before the point, is exact however
 // far the position.  Sine and cosine of what is left after the nearest quarter turn are their series to
 // x^9 and x^10, below 2e-9 off at an eighth of a turn.
+//
+// Bytes bound all but small calls, 36 us for 168 MB (4.7 TB/s; a copy goes at 4.9); one token for 64 sequences takes 4,
+// a launch and a chain of loads.
 #include "flare_mix.h"
 
 #include <math.h>
