@@ -124,16 +124,16 @@ class RotaryPositions(autograd.Function):
 
     @staticmethod
     def forward(ctx, Q, K, frequencies, positions, lengths, interleaved):
-        ctx.save_for_backward(positions, lengths)
-        ctx.options = (frequencies, interleaved, K is not None)
+        ctx.save_for_backward(frequencies, positions, lengths)
+        ctx.options = (interleaved, K is not None)
         q, k = _turn(Q, K, frequencies, positions, lengths, interleaved, False)
         return q if k is None else (q, k)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, *grads):
-        positions, lengths = ctx.saved_tensors
-        frequencies, interleaved, keys = ctx.options
+        frequencies, positions, lengths = ctx.saved_tensors
+        interleaved, keys = ctx.options
         need_q, need_k = ctx.needs_input_grad[0], keys and ctx.needs_input_grad[1]
         dq, dk = None, None
         if need_q:

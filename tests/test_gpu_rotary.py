@@ -139,6 +139,33 @@ def test_strides_types_and_missing_parts():
     assert cf.rotary_positions(q[:0], None, f, lengths=ints()).shape == (0, 9, 8, 64)
 
 
+def test_gradients_of_two_types_and_changed_arguments():
+    g = rng(14)
+    f = cf.rotary_frequencies(32)
+    at = torch.arange(9).expand(2, 9)
+    q, k = normal(g, 2, 9, 4, 48, dtype=torch.bfloat16).cuda().requires_grad_(), normal(g, 2, 9, 2, 48).cuda().requires_grad_()
+    y = cf.rotary_positions(q, k, f)
+    dy = [normal(g, *t.shape, dtype=t.dtype).cuda() for t in y]
+    for dx, d, x in zip(torch.autograd.grad(y, (q, k), dy), dy, (q, k)):
+        assert dx.dtype is x.dtype
+        near(dx, d, f, at, False, "gradient", inverse=True)
+    # queries alone, gradients that lie apart
+    y = cf.rotary_positions(q, None, f)
+    dy = normal(g, 2, 9, 48, 4, dtype=torch.bfloat16).cuda().transpose(2, 3)
+    dx, = torch.autograd.grad(y, q, dy)
+    near(dx, dy, f, at, False, "gradient", inverse=True)
+    # what the gradients need may not change before they are taken
+    for change in ("frequencies", "positions"):
+        mine, where = f.clone(), torch.arange(9, dtype=torch.int32, device="cuda").expand(2, 9).contiguous()
+        y = cf.rotary_positions(k, k, mine, positions=where)
+        (mine if change == "frequencies" else where).add_(1)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            torch.autograd.grad(y[0].sum(), k)
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        dx, = torch.autograd.grad(cf.rotary_positions(k, k, f)[0].square().sum(), k, create_graph=True)
+        dx.sum().backward()
+
+
 def test_nan_stays_in_its_pair():
     f = cf.rotary_frequencies(16)
     for dt in TYPES.values():
