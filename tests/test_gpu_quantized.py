@@ -460,6 +460,38 @@ def test_captured_tokens_and_drafts(bits):
                 assert torch.equal(cache[n].view(torch.uint8), plain[n].view(torch.uint8)), (T, step, n)
 
 
+@pytest.mark.parametrize("T", [128, 512])
+def test_captured_prompts(T):
+    """A graph of a prompt, by codes and by values turned into 16 bits, replayed with other inputs and lengths."""
+    g = rng(16)
+    B, H, G, D, S = 3, 8, 2, 96, 1700
+    cache, plain = cf.quantized_cache(B, S, G, D, 4), cf.quantized_cache(B, S, G, D, 4)
+    q, k, v = (normal(g, B, T, h, D, dtype=torch.float16).cuda() for h in (H, G, G))
+    lens, new = torch.zeros(B, dtype=torch.int32, device="cuda"), torch.zeros(B, dtype=torch.int32, device="cuda")
+
+    def call(to):
+        return cf.softmax_attention_prefill(q, k, v, to, lens, softcap=30.0, new_lengths=new)[0]
+
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        call(cache)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = call(cache)
+    for step in range(4):
+        for t, h in ((q, H), (k, G), (v, G)):
+            t.copy_(normal(g, B, T, h, D, dtype=torch.float16))
+        new.copy_(torch.randint(0, T + 1, (B,), generator=g))
+        graph.replay()
+        want = call(plain)
+        torch.cuda.synchronize()
+        assert torch.equal(y, want), step
+        for n in PARTS:
+            assert torch.equal(cache[n].view(torch.uint8), plain[n].view(torch.uint8)), (step, n)
+        lens += new
+
+
 def test_calls_on_two_streams():
     g = rng(7)
     H, G, D, S = 8, 2, 64, 3000
