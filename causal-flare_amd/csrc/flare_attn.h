@@ -80,6 +80,7 @@ struct AttnArgs {
     // single tokens
     const void *k_new, *v_new;       // [B, G, D]
     int64_t kn_sb, kn_sg, vn_sb, vn_sg;
+    int64_t kn_sn, vn_sn;            // of their tokens, where there may be more than one
     float* parts;                    // what `splits` workgroups leave of each sum
     int64_t splits;
     // a cache of 8 or 4 bits: the codes are k.p and v.p

@@ -475,10 +475,10 @@ extern "C" int flare_qattn(const void* q, const void* k, const void* v, const in
     p.lengths = lengths, p.fresh = new_lengths, p.prefix = prefix_lengths, p.causal = 1;
     p.y = y, p.parts = (float*)workspace;
     const int path = qattn_path(N, M, H, G, D, dtype);
-    // one token's key and value are quantised on the way
-    if (N == 1 && path == kRows && !new_lengths) {
-        p.k_new = k, p.kn_sb = strides[3], p.kn_sg = strides[5];
-        p.v_new = v, p.vn_sb = strides[6], p.vn_sg = strides[8];
+    // a few tokens' keys and values are quantised on the way
+    if (N <= 16 && path == kRows) {
+        p.k_new = k, p.kn_sb = strides[3], p.kn_sn = strides[4], p.kn_sg = strides[5];
+        p.v_new = v, p.vn_sb = strides[6], p.vn_sn = strides[7], p.vn_sg = strides[8];
     } else {
         const int rc = flare_qcache_write(k, v, strides + 3, dtype, bits, B, N, M, G, D, lengths, new_lengths, k_cache,
                                           k_scale, v_cache, v_scale, stream);

@@ -13,9 +13,9 @@
 // weights enter as three bf16 parts, 24 bits.
 //
 // The keys of a sequence are split over `splits` workgroups of four waves by its true length; qattn_join adds
-// up what they leave.  A workgroup's waves are shares of one head's keys, or heads that lie side by side.  A single
-// token's key and value are quantised by the workgroups whose share they are in, one of which puts them into the
-// cache.
+// up what they leave.  A workgroup's waves are shares of one head's keys, or heads that lie side by side.  Up to 16 new
+// keys and values a sequence are quantised by the workgroups whose share they are in, each put into the cache by one of
+// them; qcache_write puts more there first.
 //
 // 64 sequences of up to 8192 tokens, 4 key heads of 128, 4 bits, 250 MB: 59 us and 6 for the joining, 66 a call (a copy
 // of these bytes takes 51).  The same loads without the rest take 63 a call, so that 46% of the vector issue slots and
@@ -51,6 +51,9 @@ struct RowsLds {
     static constexpr size_t v_bytes = 2 * 32 * P;                                  // of a wave
     static constexpr size_t o_bytes = sizeof(float) * 16 * (DP + 2);               // of a wave, after the loop
     static constexpr size_t bytes = 4 * (v_bytes > o_bytes ? v_bytes : o_bytes);
+    // and behind that codes and scales of `tokens` new keys and values of each of `heads` heads
+    static constexpr size_t row_words(int bits) { return 4 * bits + 4; }
+    static size_t all(int64_t heads, int64_t tokens, int bits) { return bytes + heads * 2 * tokens * row_words(bits) * 4; }
 };
 
 // x as three parts of 8 bits that add up to it; an infinite value or a NaN is the first alone.
@@ -105,8 +108,6 @@ __global__ __launch_bounds__(256, rows_waves(sizeof(E), BITS, RT)) void qattn_ro
     constexpr int NSC = DK == 3 ? 3 : 1;               // blocks that a lane's dimensions of K may lie in
     constexpr int NV = (TK * NB + 63) / 64;            // blocks of V a lane takes
     extern __shared__ __align__(16) char smem[];
-    __shared__ u32 new_codes[4][2][4 * BITS];
-    __shared__ u32 new_scales[4][2][4];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int g = lane >> 4, c = lane & 15;
     const unsigned D = (unsigned)p.D, G = (unsigned)p.G, H = (unsigned)p.H, N = (unsigned)p.N, splits = (unsigned)p.splits;
@@ -117,7 +118,7 @@ __global__ __launch_bounds__(256, rows_waves(sizeof(E), BITS, RT)) void qattn_ro
     const unsigned kvh0 = blockIdx.x / 8 % sets * heads, kvh = kvh0 + head, unit = blockIdx.x / (8 * sets) * 8 + blockIdx.x % 8;
     const unsigned split = unit % splits, group = unit / splits % groups, b = unit / (splits * groups);
     if (b >= (unsigned)p.B) return;
-    const bool single = p.k_new != nullptr;            // its key and value are not in the cache yet
+    const bool fused = p.k_new != nullptr;             // the new keys and values are not in the cache yet
     const int off = p.lengths[b], fresh = p.fresh ? min(max(p.fresh[b], 0), (int)N) : (int)N;
     S* y = (S*)p.y + (int64_t)b * N * H * D;
     if (off < 0 || (int64_t)off + fresh > p.M) {
@@ -138,7 +139,7 @@ __global__ __launch_bounds__(256, rows_waves(sizeof(E), BITS, RT)) void qattn_ro
     const unsigned share = ((unsigned)seen + splits - 1) / splits;
     const int per = (int)((share + step - 1) / step * step);
     const int first = (int)min((int64_t)split * per, (int64_t)seen), last = (int)min((int64_t)first + per, (int64_t)seen);
-    const int held = single ? min(last, off) : last;           // what of it memory holds
+    const int held = fused ? min(last, off) : last;            // what of it memory holds
     const unsigned codes = D * BITS / 8, scales = (D + kBlock - 1) / kBlock;
     const unsigned stride = G * codes, scale_stride = G * scales;
     const int64_t row0 = (int64_t)b * p.M * G + kvh;
@@ -147,23 +148,32 @@ __global__ __launch_bounds__(256, rows_waves(sizeof(E), BITS, RT)) void qattn_ro
     const uint8_t* ksc = p.k_scale + row0 * scales;
     const uint8_t* vsc = p.v_scale + row0 * scales;
 
-    // the single token's keys and values: a quad of lanes a block
-    if (single && first <= off && off < last) {
-        if (tid < (int)heads * 8 * NB) {
-            const unsigned at = tid / (8 * NB), value = tid / (4 * NB) % 2, block = tid / 4 % NB, d = block * kBlock + (tid & 3) * 8;
-            const S* from = value ? (const S*)p.v_new + b * p.vn_sb + (kvh0 + at) * p.vn_sg
-                                  : (const S*)p.k_new + b * p.kn_sb + (kvh0 + at) * p.kn_sg;
+    // the new keys and values of this share: a quad of lanes a block.  A token goes into the cache from the group that its
+    // last row is in, as that sees it.
+    constexpr unsigned RW = Lds::row_words(BITS);
+    u32* fresh_rows = (u32*)(smem + Lds::bytes);
+    auto fresh_row = [&](unsigned head, unsigned value, unsigned token) {
+        return fresh_rows + ((head * 2 + value) * N + token) * RW;       // codes, and the scales of four blocks
+    };
+    if (fused && last > max(first, off)) {
+        const unsigned begin = max(first, off) - off, count = last - max(first, off);
+        for (unsigned i = tid; i < heads * count * 8 * NB; i += 256) {
+            const unsigned block = i / 4 % NB, value = i / (4 * NB) % 2, t = begin + i / (8 * NB) % count;
+            const unsigned at = i / (8 * NB) / count, d = block * kBlock + (i & 3) * 8;
+            const S* from = value ? (const S*)p.v_new + b * p.vn_sb + t * p.vn_sn + (kvh0 + at) * p.vn_sg
+                                  : (const S*)p.k_new + b * p.kn_sb + t * p.kn_sn + (kvh0 + at) * p.kn_sg;
             float x[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
             if (d < D) qcache::load8(reinterpret_cast<const E*>(from) + d, x);
             const u32 byte = qcache::scale_of<BITS>(qcache::quad_max(qcache::top_of(x)), __is_same(E, __half));
             const Codes<BITS> w = qcache::encode<BITS>(x, byte);
+            u32* to = fresh_row(at, value, t);
 #pragma unroll
-            for (int i = 0; i < W8; ++i) new_codes[at][value][d / 8 * W8 + i] = w.w[i];
-            if ((tid & 3) == 0) new_scales[at][value][block] = byte;
-            if (group == 0 && d < D) {
-                const int64_t row = ((int64_t)b * p.M + off) * G + kvh0 + at;
+            for (int j = 0; j < W8; ++j) to[d / 8 * W8 + j] = w.w[j];
+            if ((i & 3) == 0) to[4 * BITS + block] = byte;
+            if ((t * R + R - 1) / (16 * RT) == group && d < D) {
+                const int64_t row = ((int64_t)b * p.M + off + t) * G + kvh0 + at;
                 *reinterpret_cast<Codes<BITS>*>((uint8_t*)(value ? p.v.p : p.k.p) + row * codes + d * BITS / 8) = w;
-                if ((tid & 3) == 0) (value ? p.v_scale : p.k_scale)[row * scales + block] = (uint8_t)byte;
+                if ((i & 3) == 0) (value ? p.v_scale : p.k_scale)[row * scales + block] = (uint8_t)byte;
             }
         }
         __syncthreads();
@@ -235,22 +245,26 @@ __global__ __launch_bounds__(256, rows_waves(sizeof(E), BITS, RT)) void qattn_ro
             vb[i] = (u32)(uint8_t)__builtin_amdgcn_raw_buffer_load_b8(vr_s, vs_at[i], 0, 0);
         }
     };
-    // the single token's codes, for the lanes that take its place
+    // the new tokens' codes, for the lanes that take their place
     auto insert = [&](int k0) {
 #pragma unroll
         for (int m = 0; m < NM; ++m) {
-            if (k0 + 16 * m + c != off) continue;
+            const int j = k0 + 16 * m + c;
+            if (j < off || j >= last) continue;
+            const u32* from = fresh_row(head, 0, j - off);
 #pragma unroll
-            for (int i = 0; i < DK * W8; ++i) kw[m][i] = new_codes[head][0][DK * W8 * g + i];
+            for (int i = 0; i < DK * W8; ++i) kw[m][i] = from[DK * W8 * g + i];
 #pragma unroll
-            for (int i = 0; i < NSC; ++i) kb[m][i] = new_scales[head][0][8 * (DK * g + i) / kBlock];
+            for (int i = 0; i < NSC; ++i) kb[m][i] = from[4 * BITS + 8 * (DK * g + i) / kBlock];
         }
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            if (!unit_there(i) || k0 + unit_key(i) != off) continue;
+            const int j = k0 + unit_key(i);
+            if (!unit_there(i) || j < off || j >= last) continue;
+            const u32* from = fresh_row(head, 1, j - off);
 #pragma unroll
-            for (int w = 0; w < BITS; ++w) vw[i][w] = new_codes[head][1][unit_block(i) * BITS + w];
-            vb[i] = new_scales[head][1][unit_block(i)];
+            for (int w = 0; w < BITS; ++w) vw[i][w] = from[unit_block(i) * BITS + w];
+            vb[i] = from[4 * BITS + unit_block(i)];
         }
     };
     const int begin = first + (int)part * TK;
@@ -299,7 +313,7 @@ __global__ __launch_bounds__(256, rows_waves(sizeof(E), BITS, RT)) void qattn_ro
     }
 
     for (int k0 = begin; k0 < last; k0 += step) {
-        if (single && k0 <= off && off < k0 + TK) insert(k0);
+        if (fused && off < k0 + TK) insert(k0);
         f32x4 s[RT][NM];
 #pragma unroll
         for (int m = 0; m < NM; ++m) {
@@ -314,7 +328,7 @@ __global__ __launch_bounds__(256, rows_waves(sizeof(E), BITS, RT)) void qattn_ro
                     for (int t = 0; t < RT; ++t) s[t][m] = mma(a, qf[t][i][kk], s[t][m]);
             }
         }
-        const bool whole = single || k0 + TK <= off + token0 + 1;  // every row sees all of these keys
+        const bool whole = N == 1 || k0 + TK <= off + token0 + 1;  // every row sees all of these keys
         if (!whole) {
             bool odd = false;
 #pragma unroll
@@ -323,7 +337,8 @@ __global__ __launch_bounds__(256, rows_waves(sizeof(E), BITS, RT)) void qattn_ro
                 // which rows see blocks that are NaN, as 0 times NaN is NaN to the others too
                 for (int j = k0; j < min(k0 + TK, last); ++j) {
                     for (int i = 0; i < (int)scales; ++i) {
-                        if (vsc[(int64_t)j * scale_stride + i] != kNoValue) continue;
+                        if ((j < held ? vsc[(int64_t)j * scale_stride + i] : fresh_row(head, 1, j - off)[4 * BITS + i]) != kNoValue)
+                            continue;
 #pragma unroll
                         for (int t = 0; t < RT; ++t)
                             if (j < lim[t]) lost[t] |= 1u << i;
@@ -516,7 +531,7 @@ template <typename E, int BITS, int DP, int CAP, int RT>
 static int rows_launch(const AttnArgs& p, hipStream_t stream) {
     const int64_t units = p.splits * p.B * ceil_div(p.H / p.G * p.N, 16 * RT), sets = p.G / p.row_splits;
     qattn_rows_kernel<E, BITS, DP, CAP, RT>
-        <<<dim3((unsigned)(ceil_div(units, 8) * 8 * sets)), 256, RowsLds<DP>::bytes, stream>>>(p);
+        <<<dim3((unsigned)(ceil_div(units, 8) * 8 * sets)), 256, RowsLds<DP>::all(p.row_splits, p.k_new ? p.N : 0, BITS), stream>>>(p);
     const int rc = check_launch("qattn_rows");
     if (rc != FLARE_OK || p.splits == 1) return rc;
     qattn_join_kernel<E><<<dim3((unsigned)(p.N * p.H), (unsigned)p.B), 256, 0, stream>>>(p);
