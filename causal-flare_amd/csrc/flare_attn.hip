@@ -432,7 +432,7 @@ extern "C" int flare_attn_step(const void* q, const void* k, const void* v, cons
 
 extern "C" size_t flare_qattn_workspace_size(int64_t B, int64_t N, int64_t M, int64_t H, int64_t G, int64_t D, int dtype,
                                              int bits) {
-    if (B < 1 || N < 1 || M < 1 || H < 1 || G < 1 || H % G) return 0;
+    if (B < 1 || N < 1 || M < 1 || H < 1 || G < 1 || D < 1 || H % G) return 0;
     const int path = qattn_path(N, M, H, G, D, dtype);
     if (path == kRows) {
         const int64_t s = rows_splits(B, N, M, H, G, D, dtype, bits);

@@ -141,6 +141,7 @@ def test_c_entry_points_check_before_they_launch():
         need = lib.flare_qattn_workspace_size(1, n, 4096, 4, 4, 64, 1, 4)
         assert need > 0 and need % 16 == 0
         assert attend(N=n) == -3 and attend(N=n, ws=P, size=need - 1) == -3 and attend(N=n, ws=odd, size=need) == -3
+    assert lib.flare_qattn_workspace_size(1, 4096, 8, 4, 4, 0, 1, 4) == 0
     assert lib.flare_qattn_workspace_size(0, 1, 8, 4, 4, 64, 1, 4) == 0 and lib.flare_qattn_workspace_size(1, 1, 8, 4, 3, 64, 1, 8) == 0
 
 
