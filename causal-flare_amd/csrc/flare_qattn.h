@@ -492,37 +492,45 @@ __global__ __launch_bounds__(256, rows_waves(sizeof(E), BITS, RT)) void qattn_ro
     }
 }
 
-// A workgroup a row: 32 lanes, four dimensions a lane, take every eighth part, and the first of them
-// what the eight leave, in order.
-template <typename E>
+// What the parts of each row leave, joined: 32 lanes, four dimensions a lane, take every SETS-th part.
+// With SETS = 8 a row is a workgroup's, and the first 32 lanes join what the eight leave, in order;
+// otherwise a workgroup has eight rows, each with all of its parts.
+template <typename E, int SETS>
 __global__ __launch_bounds__(256) void qattn_join_kernel(AttnArgs p) {
     typedef typename Elem<E>::S S;
     typedef S S4 __attribute__((ext_vector_type(4)));
-    __shared__ __align__(16) float left[8][128 + 4];
-    const unsigned b = blockIdx.y, token = blockIdx.x / (unsigned)p.H;
-    const int64_t row = (int64_t)b * p.N * p.H + blockIdx.x;
-    const int len = p.lengths[b], fresh = p.fresh ? min(max(p.fresh[b], 0), (int)p.N) : (int)p.N;
+    __shared__ __align__(16) float left[SETS == 8 ? 8 : 1][128 + 4];
     const int d = (threadIdx.x & 31) * 4, set = threadIdx.x >> 5;
-    const bool idle = len < 0 || (int64_t)len + fresh > p.M;
-    if (!idle && d < p.D) {
-        const Joined j = join_parts<8, 8>(p.parts + row * p.splits * (p.D + 4), set, (int)p.splits, p.D, d);
-        *reinterpret_cast<f32x4*>(&left[set][d]) = j.v;
-        if (d == 0) {
-            left[set][p.D] = j.top;
-            left[set][p.D + 1] = j.total;
+    const unsigned b = blockIdx.y, rows = (unsigned)(p.N * p.H);
+    const unsigned at = SETS == 8 ? blockIdx.x : blockIdx.x * 8 + set, token = at / (unsigned)p.H;
+    const int64_t row = (int64_t)b * rows + at;
+    const int len = p.lengths[b], fresh = p.fresh ? min(max(p.fresh[b], 0), (int)p.N) : (int)p.N;
+    const bool idle = len < 0 || (int64_t)len + fresh > p.M, there = at < rows && d < p.D;
+    Joined j{kNegInf, 0.0f, f32x4{0.0f, 0.0f, 0.0f, 0.0f}};
+    if (!idle && there)
+        j = join_parts<SETS, 8>(p.parts + row * p.splits * (p.D + 4), SETS == 8 ? set : 0, (int)p.splits, p.D, d);
+    if constexpr (SETS == 8) {
+        if (!idle && there) {
+            *reinterpret_cast<f32x4*>(&left[set][d]) = j.v;
+            if (d == 0) {
+                left[set][p.D] = j.top;
+                left[set][p.D + 1] = j.total;
+            }
+        }
+        __syncthreads();
+        if (set) return;
+        j = Joined{kNegInf, 0.0f, f32x4{0.0f, 0.0f, 0.0f, 0.0f}};
+        if (!idle && there) {
+#pragma unroll
+            for (int s = 0; s < 8; ++s)
+                j.add(left[s][p.D], left[s][p.D + 1], *reinterpret_cast<const f32x4*>(&left[s][d]));
         }
     }
-    __syncthreads();
-    if (set || d >= p.D) return;
-    f32x4 v;
+    if (!there) return;
+    f32x4 v = j.v / j.total;
     if (idle || (int)token >= fresh) {
         const float none = !idle || len < 0 ? 0.0f : __builtin_nanf("");
         v = f32x4{none, none, none, none};
-    } else {
-        Joined j{kNegInf, 0.0f, f32x4{0.0f, 0.0f, 0.0f, 0.0f}};
-#pragma unroll
-        for (int s = 0; s < 8; ++s) j.add(left[s][p.D], left[s][p.D + 1], *reinterpret_cast<const f32x4*>(&left[s][d]));
-        v = j.v / j.total;
     }
     *reinterpret_cast<S4*>((S*)p.y + row * p.D + d) = __builtin_convertvector(v, S4);
 }
@@ -534,7 +542,13 @@ static int rows_launch(const AttnArgs& p, hipStream_t stream) {
         <<<dim3((unsigned)(ceil_div(units, 8) * 8 * sets)), 256, RowsLds<DP>::all(p.row_splits, p.k_new ? p.N : 0, BITS), stream>>>(p);
     const int rc = check_launch("qattn_rows");
     if (rc != FLARE_OK || p.splits == 1) return rc;
-    qattn_join_kernel<E><<<dim3((unsigned)(p.N * p.H), (unsigned)p.B), 256, 0, stream>>>(p);
+    // Eight parts are one lane's loads under way at once and need no second pass: eight tokens (4 bits,
+    // 16 heads of 128 over 4) for 64 sequences of 4096 take 54 us for 62 with a workgroup a row, 257
+    // tokens (float, 8 heads of 64) behind 1021 23.4 for 27.6. With up to 16 parts that way one token for
+    // 16 of 4096 (8 bits, 16 heads of 64) takes 41.3 for 39.7.
+    const unsigned rows = (unsigned)(p.N * p.H), sequences = (unsigned)p.B;
+    if (p.splits <= 8) qattn_join_kernel<E, 1><<<dim3((rows + 7) / 8, sequences), 256, 0, stream>>>(p);
+    else qattn_join_kernel<E, 8><<<dim3(rows, sequences), 256, 0, stream>>>(p);
     return check_launch("qattn_join");
 }
 template <typename E, int BITS, int DP, int CAP>
