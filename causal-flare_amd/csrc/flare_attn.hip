@@ -210,8 +210,8 @@ static int64_t rows_heads(int64_t B, int64_t M, int64_t G, int tiles) {
 // Workgroups for each sequence's keys: three on a CU, two where a wave's tiles, parts or codes leave registers for no more,
 // with shares of 256 keys a head, or of 128 until there are 32.  us, workgroups of 512, 768 and 1024, 64 x 8192 tokens, 4 key
 // heads of 128: 4 bits 75, 66, 69; 8 bits 100, 106, 111; fp32 queries 80, 99, 86; five tokens, 8 bits, 16 x 8192
-// 45, 55, 54 (with a launch to write them).  16 x 4096 in 8 bits, 16 heads of 64 43, 39, 41.  Shares of 128 and of 256 for one sequence of 1000 10.0, 11.1; of
-// 4000 10.5, 11.7; of 16384 (128 and 64 of them) 14.4, 12.5.
+// 45, 55, 54 (with a launch to write them).  16 x 4096 in 8 bits, 16 heads of 64 43, 39, 41.  Shares of 128 and
+// of 256 for one sequence of 1000 10.0, 11.1; of 4000 10.5, 11.7; of 16384 (128 and 64 of them) 14.4, 12.5.
 static int64_t rows_splits(int64_t B, int64_t N, int64_t M, int64_t H, int64_t G, int64_t D, int dtype, int bits) {
     const int tiles = row_tiles(N, H, G, dtype);
     const int64_t heads = rows_heads(B, M, G, tiles), rows = B * (G / heads) * ceil_div(H / G * N, 16 * tiles);
