@@ -14,6 +14,7 @@ import math
 
 import torch
 import torch.autograd as autograd
+import torch.autograd.forward_ad as forward_ad
 from torch.autograd.function import once_differentiable
 
 from .. import _lib
@@ -97,8 +98,8 @@ def _turn(q, k, frequencies, positions, lengths, interleaved, inverse):
 
 def _plain(Q, K, frequencies, positions, lengths):
     """Whether this is the common call: Q and K of one type on the current device, rows that the kernel reads in place,
-    int32 positions or lengths."""
-    if K is None:
+    int32 positions or lengths, and no tangents, which `RotaryPositions` has none for and refuses."""
+    if K is None or forward_ad._current_level >= 0:
         return False
     dtype, device, shape, keys = Q.dtype, Q.device, Q.shape, K.shape
     if (dtype not in _CODES or device.type != "cuda" or device.index != torch.cuda.current_device() or len(shape) not in (3, 4)
@@ -153,10 +154,11 @@ def rotary_positions(
 ):
     """Q [B, N, H, D] and K [B, N, G, D] (or None) turned by their positions: (Q, K), or Q alone.
 
-    Differentiable in Q and K.  Single tokens may be given as [B, H, D] and [B, G, D].  frequencies: float64
-    [R / 2] on the host (`rotary_frequencies`), R up to D; the rest of a head stays as it is.  positions: integers
-    [B, N] (of packed documents, say), any sign; or lengths: integers [B], the tokens that each sequence's cache
-    holds already: token t is at position lengths[b] + t.  Without either it is at t.  D up to 256.
+    Differentiable in Q and K, backwards (tangents are refused).  Single tokens may be given as [B, H, D] and
+    [B, G, D].  frequencies: float64 [R / 2] on the host (`rotary_frequencies`), R up to D; the rest of a head
+    stays as it is.  positions: integers [B, N] (of packed documents, say), any sign; or lengths: integers [B],
+    the tokens that each sequence's cache holds already: token t is at position lengths[b] + t.  Without either
+    it is at t.  D up to 256.
     """
     name = "rotary_positions"
     if _plain(Q, K, frequencies, positions, lengths):
@@ -190,7 +192,7 @@ def rotary_positions(
     if B * N == 0:
         out = Q.clone() if K is None else (Q.clone(), K.clone())
     else:
-        out = RotaryPositions.apply(Q, K, frequencies.detach().contiguous(), _int32(positions), _int32(lengths),
+        out = RotaryPositions.apply(Q, K, frequencies.contiguous(), _int32(positions), _int32(lengths),
                                     bool(interleaved))
     if K is None:
         return out[:, 0] if token else out

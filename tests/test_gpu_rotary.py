@@ -1,6 +1,7 @@
 """Rotary positions against their plain 64-bit form."""
 import pytest
 import torch
+import torch.autograd.forward_ad as forward_ad
 
 import _mixers as M
 import _quantized as Q
@@ -238,3 +239,21 @@ def test_positions_cache_and_attention_together():
             assert torch.equal(vv[:, lengths[b]:], Q.rounded(v[b:b + 1].cpu(), bits)[0])
             ref, tol = M.attention(turned[0], kk, vv, offset=[lengths[b]], unit=M.U[torch.bfloat16], tiny=2.0 ** -126)["y"]
             M.check(y[b:b + 1], ref, tol + M.U[torch.bfloat16] * ref.abs(), "y", torch.bfloat16)
+
+
+@pytest.mark.parametrize("shape", [(2, 7), (2,)])
+def test_tangents_are_refused(shape):
+    g = rng(20)
+    f = cf.rotary_frequencies(32)
+    q, k = normal(g, *shape, 4, 32).cuda(), normal(g, *shape, 2, 32).cuda()
+    lens = ints(3, 50)
+    plain = cf.rotary_positions(q, k, f, lengths=lens)
+    with forward_ad.dual_level():
+        for turned in ((forward_ad.make_dual(q, torch.ones_like(q)), k), (q, forward_ad.make_dual(k, torch.ones_like(k))),
+                       (forward_ad.make_dual(q, torch.ones_like(q)), None)):
+            with pytest.raises(NotImplementedError, match="jvp"):
+                cf.rotary_positions(*turned, f, lengths=lens)
+        with pytest.raises(NotImplementedError, match="jvp"):
+            cf.rotary_positions(q, k, forward_ad.make_dual(f, torch.ones_like(f)), lengths=lens)
+        inside = cf.rotary_positions(q, k, f, lengths=lens)
+    assert all(torch.equal(a, b) for a, b in zip(plain, inside))
