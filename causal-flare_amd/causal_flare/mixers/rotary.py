@@ -108,7 +108,8 @@ def _plain(Q, K, frequencies, positions, lengths):
         return False
     D, G = shape[-1], keys[-2]
     if (keys != (shape[:-2] + (G, D)) or not Q.numel() or not G or frequencies.dtype is not torch.float64
-            or frequencies.dim() != 1 or frequencies.device.type != "cpu" or not frequencies.is_contiguous()):
+            or frequencies.dim() != 1 or frequencies.device.type != "cpu" or not frequencies.is_contiguous()
+            or frequencies.requires_grad):
         return False
     if not 2 <= 2 * frequencies.shape[0] <= D or D > 256 or (positions is not None and lengths is not None):
         return False
@@ -181,6 +182,8 @@ def rotary_positions(
     if (not isinstance(frequencies, torch.Tensor) or frequencies.device.type != "cpu"
             or frequencies.dtype is not torch.float64 or frequencies.dim() != 1):
         raise ValueError(f"{name} expects frequencies as a float64 tensor [R / 2] on the host. Got {frequencies!r:.80}")
+    if frequencies.requires_grad and torch.is_grad_enabled():
+        raise NotImplementedError(f"{name} has no gradient for frequencies; pass frequencies.detach()")
     R = 2 * frequencies.shape[0]
     if not 2 <= R <= D or D > 256:
         raise ValueError(f"{name} turns 2 to D dimensions of heads of up to 256. Got {R} of D={D}")

@@ -199,3 +199,13 @@ def test_rotary_gradients_against_differences():
         want = float(((hi - lo) * dy).sum() / 2e-5)
         have = float((Q.rotary(dy, f, at, interleaved, inverse=True)[0] * way).sum())
         assert abs(have - want) < 1e-7 * (1 + abs(want))
+
+
+@pytest.mark.parametrize("token", [False, True])
+def test_frequencies_have_no_gradient(token):
+    f, q = F.clone().requires_grad_(), t(2, 4, 32) if token else t(2, 5, 4, 32)
+    for k in (None, q):
+        with pytest.raises(NotImplementedError, match="no gradient for frequencies"):
+            cf.rotary_positions(q, k, f)
+        with torch.no_grad(), pytest.raises(RuntimeError, match=CPU):
+            cf.rotary_positions(q, k, f)
