@@ -42,7 +42,8 @@ _FORMS = {torch.uint8: 4, torch.float8_e4m3fn: 8}
 
 
 def is_quantized(cache) -> bool:
-    return isinstance(cache, dict) and "k_scale" in cache
+    """Whether a cache is one of `quantized_cache`: with scales, and no keys of a type that queries have."""
+    return isinstance(cache, dict) and "k_scale" in cache and getattr(cache.get("k"), "dtype", None) not in _CODES
 
 
 def quantized_cache(B: int, S: int, G: int, D: int, bits: int = 8, device="cuda") -> dict[str, torch.Tensor]:

@@ -209,3 +209,15 @@ def test_frequencies_have_no_gradient(token):
             cf.rotary_positions(q, k, f)
         with torch.no_grad(), pytest.raises(RuntimeError, match=CPU):
             cf.rotary_positions(q, k, f)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_other_entries_of_a_cache_are_the_callers(dtype):
+    """Keys and values of the queries' type stay such a cache, whatever else its dict holds."""
+    qkv = [t(2, 5, 4, 32, dtype=dtype)] * 3
+    plain = {n: t(2, 9, 4, 32, dtype=dtype) for n in ("k", "v")}
+    for more in ({}, {"k_scale": t(4)}, {"k_scale": None, "v_scale": 1.0}):
+        with pytest.raises(RuntimeError, match=CPU):
+            cf.softmax_attention_prefill(*qkv, dict(plain, **more), ints(2))
+        with pytest.raises(RuntimeError, match=CPU):
+            cf.softmax_attention_decode(*(x[:, 0] for x in qkv), dict(plain, **more), ints(2))
