@@ -221,6 +221,14 @@ static int64_t rows_splits(int64_t B, int64_t N, int64_t M, int64_t H, int64_t G
     if (heads == 1 && most < 32) most = small < 32 ? small : 32;
     return s < 1 ? 1 : (s > most ? most : s);
 }
+// Workgroups of the largest launch of a call.  (Where attn_forward splits its keys there are few.)
+static int64_t qattn_blocks(int64_t B, int64_t N, int64_t M, int64_t H, int64_t G, int64_t D, int dtype, int bits) {
+    const int path = qattn_path(N, M, H, G, D, dtype), tiles = row_tiles(N, H, G, dtype);
+    if (path != kRows)
+        return ceil_div(N, rows_of_queries(dtype)) * H * (path == kFused ? B : expand_slice(B, M, G, D));
+    const int64_t units = rows_splits(B, N, M, H, G, D, dtype, bits) * B * ceil_div(H / G * N, 16 * tiles);
+    return ceil_div(units, 8) * 8 * (G / rows_heads(B, M, G, tiles));
+}
 template <typename E>
 static int qattn_rows(const AttnArgs& p, int bits, int tiles, hipStream_t stream) {
     return bits == 8 ? rows_e<E, 8>(p, tiles, stream) : rows_e<E, 4>(p, tiles, stream);
@@ -460,7 +468,8 @@ extern "C" int flare_qattn(const void* q, const void* k, const void* v, const in
                   "flare_qattn: null pointer");
     ATTN_REQUIRE_SIZES("flare_qattn");
     FLARE_REQUIRE(bits == 4 || bits == 8, "flare_qattn: %d bits; 4 or 8", bits);
-    FLARE_REQUIRE(N * H <= (1 << 30) && N * G <= (1 << 27), "flare_qattn: too large");
+    FLARE_REQUIRE(N * H <= (1 << 30) && N * G <= (1 << 27) &&
+                  qattn_blocks(B, N, M, H, G, D, dtype, bits) <= mix::kMostBlocks, "flare_qattn: too large");
     AttnArgs p = attn_args(q, k_cache, v_cache, strides, B, N, M, H, G, D, scale, softcap, slopes);
     const Rows kr = {k, strides[3], strides[4], strides[5]}, vr = {v, strides[6], strides[7], strides[8]};
     const uintptr_t held = (uintptr_t)k_cache | (uintptr_t)v_cache | (uintptr_t)y;

@@ -18,6 +18,8 @@ using mfma::kLog2e;
 
 inline bool known_dtype(int dtype) { return dtype == FLARE_F32 || dtype == FLARE_BF16 || dtype == FLARE_F16; }
 inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+// Workgroups of 256 that a dimension of a grid takes: less than 2^32 threads.
+constexpr int64_t kMostBlocks = (1 << 24) - 1;
 
 __device__ __forceinline__ float sigmoid(float x) { return __builtin_amdgcn_rcpf(1.0f + __expf(-x)); }
 

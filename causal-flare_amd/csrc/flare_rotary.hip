@@ -153,7 +153,7 @@ static int launch(Args p, hipStream_t stream) {
     const int each = heads_of(p.interleaved), want = all <= 256 * 1024 ? heads : (heads + each - 1) / each;
     p.parts = 256 / p.units < want ? 256 / p.units : want;
     const int64_t blocks = ceil_div(p.B * p.N, 256 / (p.units * p.parts));
-    if (blocks > INT32_MAX) {
+    if (blocks > mix::kMostBlocks) {
         set_error("flare_rotary: too large");
         return FLARE_ERR_INVALID;
     }

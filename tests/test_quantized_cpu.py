@@ -221,3 +221,22 @@ def test_other_entries_of_a_cache_are_the_callers(dtype):
             cf.softmax_attention_prefill(*qkv, dict(plain, **more), ints(2))
         with pytest.raises(RuntimeError, match=CPU):
             cf.softmax_attention_decode(*(x[:, 0] for x in qkv), dict(plain, **more), ints(2))
+
+
+def test_grids_that_cannot_be_launched_are_refused_first():
+    """2^32 threads and more in a dimension of a grid, which a launch does not take: nothing may be written before."""
+    lib, P = _lib.lib(), ctypes.c_void_p(4096)
+    six, nine = ((ctypes.c_int64 * n)(*[16] * n) for n in (6, 9))
+    f = (ctypes.c_double * 128)(*[0.5] * 128)
+
+    def attend(dtype, B, N, M, H, G, D=16, bits=4):
+        size = lib.flare_qattn_workspace_size(B, N, M, H, G, D, dtype, bits)
+        return lib.flare_qattn(P, P, P, nine, dtype, bits, B, N, M, H, G, D, 1.0, 0.0, None, None, P, None, P, P, P, P, P, P, size, None)
+    assert _refused(attend(0, 32, 1 << 24, 1 << 25, 8, 1), b"too large")               # rows: 2^28 workgroups
+    assert _refused(attend(0, 1, 1 << 24, 1 << 25, 16, 1), b"too large")               # 2^24
+    assert _refused(attend(1, 1 << 14, 1024, 4096, 256, 256, bits=8), b"too large")    # prompts, by codes: 2^25
+    assert _refused(attend(2, 8192, 1 << 16, 16, 8, 1), b"too large")                  # over values of 16 bits: 2^25
+
+    def rotary(N, H=32, D=256, R=256):
+        return lib.flare_rotary(P, P, six, 1, 1, N, H, H, D, R, f, None, None, 0, 0, P, P, None)
+    assert _refused(rotary(1 << 24), b"too large") and _refused(rotary((1 << 25) - 1, R=32), b"too large")
