@@ -37,6 +37,7 @@ from ._inputs import (
 )
 
 _BLOCK = 32
+_FAR = 2 ** 31 - 1
 _PARTS = ("k", "k_scale", "v", "v_scale")
 _FORMS = {torch.uint8: 4, torch.float8_e4m3fn: 8}
 
@@ -257,6 +258,8 @@ def quantized_cache_read(
     k, v = (torch.empty((B, count, G, D), device=device, dtype=dtype) for _ in range(2))
     if k.numel() == 0:
         return k, v
+    if first is not None and first.dtype is torch.int64:
+        first = first.clamp(-_FAR, _FAR)             # rows beyond 32 bits are outside too
     at = _int32(first)
     P = _ptr
     with _on(device):

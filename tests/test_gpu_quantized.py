@@ -538,3 +538,14 @@ def test_offsets_past_32_bits():
             # weights and y rounded to bf16, sums over a million terms in 32 bits
             mag = (w[:, :, None] * vv[b, :n].cpu().transpose(0, 1).abs()).sum(1) / (w.sum(1, keepdim=True) + off)
             M.check(row, ref, (2 * M.U[torch.bfloat16] + 2.0 ** -10) * mag, "y", torch.bfloat16)
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+def test_rows_beyond_32_bits_are_outside(bits):
+    cache = filled(rng(23), 6, 9, 2, 32, bits)
+    at = torch.tensor([2 ** 32, -2 ** 32, 2 ** 32 + 3, 2 ** 31, -2 ** 40 + 1, 4], device="cuda")
+    got = cf.quantized_cache_read(cache, at, 3, torch.float32)
+    for n, x in zip(("k", "v"), got):
+        assert (x[:5] == 0).all()
+        want = Q.held(cache[n][5, 4:7], cache[n + "_scale"][5, 4:7]).float()
+        assert torch.equal(x[5].cpu().nan_to_num(nan=7e37), want.nan_to_num(nan=7e37))
