@@ -182,17 +182,19 @@ static int row_tiles(int64_t N, int64_t H, int64_t G, int dtype) { return H / G 
 // 21.  fp32 queries, 8 heads of 64, behind 4096 of 16: 32 new tokens 106, 55; 512 595, 304: these always go by rows.
 //   Values turned into 16 bits once pay from 16 blocks that read them.  us, fused and expanded: 16 x 256 new tokens behind
 // 8192, 348, 396; 512 (16 blocks) 684, 689; 2048 2512, 2218; one sequence, 1024 behind 15,300 191, 180; 2048 351, 317.
+// That is a tenth of the time for memory that a cache of 4 bits was chosen to save, and rooms count whole, whatever they
+// hold: 1 GiB of values at a time, and sequences whose values are more go by their codes.
 enum { kRows, kFused, kExpanded };
-constexpr int64_t kExpandBlocks = 16, kMostExpanded = (int64_t)8 << 30;      // bytes of one sequence's values
+constexpr int64_t kExpandBlocks = 16, kMostExpanded = (int64_t)1 << 30;      // bytes of values
 static int64_t expanded_row(int64_t G, int64_t D) { return 2 * 2 * G * D; }  // of a token, k and v
 static int qattn_path(int64_t N, int64_t M, int64_t H, int64_t G, int64_t D, int dtype) {
     const int64_t R = H / G, blocks = R * ceil_div(N, 128);
     if (dtype == FLARE_F32 || ceil_div(R * N, 32) <= 3 * blocks) return kRows;
     return blocks < kExpandBlocks || M * expanded_row(G, D) > kMostExpanded ? kFused : kExpanded;
 }
-// Sequences that are expanded at a time: 1 GiB of values, or one.
+// Sequences that are expanded at a time.
 static int64_t expand_slice(int64_t B, int64_t M, int64_t G, int64_t D) {
-    const int64_t s = (int64_t)(1 << 30) / (M * expanded_row(G, D));
+    const int64_t s = kMostExpanded / (M * expanded_row(G, D));
     return s < 1 ? 1 : (s > B ? B : s);
 }
 static size_t expanded_bytes(int64_t B, int64_t M, int64_t G, int64_t D) {

@@ -549,3 +549,24 @@ def test_rows_beyond_32_bits_are_outside(bits):
         assert (x[:5] == 0).all()
         want = Q.held(cache[n][5, 4:7], cache[n + "_scale"][5, 4:7]).float()
         assert torch.equal(x[5].cpu().nan_to_num(nan=7e37), want.nan_to_num(nan=7e37))
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+def test_prompts_by_codes_of_a_large_room(dtype, bits):
+    """As many blocks of queries as have values turned into 16 bits first, in rooms whose values would pass 1 GiB."""
+    dt, g = TYPES[dtype], rng(24)
+    B, T, H, G, D, S = 2, 200, 8, 1, 128, (1 << 21) + 64
+    cache = cf.quantized_cache(B, S, G, D, bits)
+    q, k, v = (normal(g, B, T, h, D, dtype=dt) for h in (H, G, G))
+    old = [normal(g, B, 70, G, D, dtype=dt).cuda() for _ in range(2)]
+    cf.quantized_cache_write(cache, *old, ints(0, 0))
+    y, _ = cf.softmax_attention_prefill(q.cuda(), k.cuda(), v.cuda(), cache, ints(33, S - T + 1), new_lengths=ints(T - 3, T),
+                                        prefix_lengths=ints(50, 0))
+    assert torch.isnan(y[1]).all() and (y[0, T - 3:] == 0).all()
+    n = 33 + T - 3
+    kk, vv = (Q.held(cache[x][:1, :n], cache[x + "_scale"][:1, :n]) for x in ("k", "v"))
+    assert torch.equal(kk[:, 33:], Q.rounded(k[:1, :T - 3], bits)[0])
+    ref, tol = M.attention(q[:1, :T - 3], kk, vv, offset=[33], prefix=[50], unit=M.U[dt],
+                           tiny=2.0 ** -25 if dtype == "fp16" else 2.0 ** -126)["y"]
+    M.check(y[:1, :T - 3], ref, tol + M.U[dt] * ref.abs(), "y", dt)

@@ -240,3 +240,18 @@ def test_grids_that_cannot_be_launched_are_refused_first():
     def rotary(N, H=32, D=256, R=256):
         return lib.flare_rotary(P, P, six, 1, 1, N, H, H, D, R, f, None, None, 0, 0, P, P, None)
     assert _refused(rotary(1 << 24), b"too large") and _refused(rotary((1 << 25) - 1, R=32), b"too large")
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+def test_workspace_of_large_rooms(bits):
+    """Values turned into 16 bits take 1 GiB at most, whatever a cache has room for; the rest is what parts of rows leave."""
+    size, B, N, H, G, D = _lib.lib().flare_qattn_workspace_size, 3, 4096, 16, 4, 128
+    parts = 2 * 4 * B * N * H * (D + 4)
+    some = 0
+    for room in (1 << 14, 1 << 17, (1 << 19) - 1, 1 << 19, (1 << 19) + 1, 1 << 20, 1 << 21, 1 << 22, 1 << 24, 1 << 30):
+        need = size(B, N, room, H, G, D, 1, bits)
+        assert need <= (1 << 30) + parts, room
+        some = max(some, need)
+        if room > 1 << 19:
+            assert need <= parts
+    assert some >= 1 << 30
