@@ -6,9 +6,10 @@
 // interleaved; dimensions from R on stay as they are.
 //
 // An angle matters to a whole turn only, so a frequency is taken as turns a token in 64 bits behind
-// the point: its product with a whole position, without the turns before the point, is exact however
-// far the position.  Sine and cosine of what is left after the nearest quarter turn are their series to
-// x^9 and x^10, below 2e-9 off at an eighth of a turn.
+// the point, the nearest: its product with a whole position, without the turns before the point, is exact
+// however far the position, and is rounded to the nearest 2^-32 of a turn (0.7e-9 off).  Sine and cosine of
+// what is left after the nearest quarter turn are their series to x^9 and x^10, below 2e-9 off at an
+// eighth of a turn.
 //
 // Bytes bound all but small calls, 36 us for 168 MB (4.7 TB/s; a copy goes at 4.9); one token for 64 sequences takes 4,
 // a launch and a chain of loads.
@@ -44,7 +45,7 @@ struct Turn {
     float c, s;
 };
 __device__ __forceinline__ Turn turn_of(int64_t position, uint64_t turns) {
-    const uint32_t at = (uint32_t)(((uint64_t)position * turns) >> 32);
+    const uint32_t at = (uint32_t)(((uint64_t)position * turns + 0x80000000u) >> 32);
     const uint32_t quarter = (at + 0x20000000u) >> 30;
     const float x = (float)(int32_t)(at - (quarter << 30)) * 1.46291807926715968105e-9f;      // 2 pi / 2^32
     const float q = x * x;
@@ -208,12 +209,12 @@ extern "C" int flare_rotary(const void* q, const void* k, const int64_t* strides
     for (int i = 0; i < R / 2; ++i) {
         const long double f = frequencies[i];
         if (f >= 0.0L && f < 6.0L) {
-            p.turns[i] = (uint64_t)(f * kTurns);            // below 0.96 2^64
+            p.turns[i] = (uint64_t)roundl(f * kTurns);      // below 0.96 2^64
             continue;
         }
         FLARE_REQUIRE(isfinite(frequencies[i]), "flare_rotary: frequency %d is not finite", i);
         const long double turns = f * (kTurns * 0x1p-64L), part = turns - floorl(turns);     // in [0, 1]: 1 only by rounding
-        p.turns[i] = part < 1.0L ? (uint64_t)ldexpl(part, 64) : 0;
+        p.turns[i] = part < 1.0L ? (uint64_t)roundl(ldexpl(part, 64)) : 0;      // at most 2^64 - 1, which 64 bits hold
     }
     return FLARE_BY_DTYPE(dtype, launch_type, (p, (hipStream_t)stream));
 }

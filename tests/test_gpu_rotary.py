@@ -1,4 +1,6 @@
 """Rotary positions against their plain 64-bit form."""
+import math
+
 import pytest
 import torch
 import torch.autograd.forward_ad as forward_ad
@@ -257,3 +259,31 @@ def test_tangents_are_refused(shape):
             cf.rotary_positions(q, k, forward_ad.make_dual(f, torch.ones_like(f)), lengths=lens)
         inside = cf.rotary_positions(q, k, f, lengths=lens)
     assert all(torch.equal(a, b) for a, b in zip(plain, inside))
+
+
+def test_angles_are_rounded_to_the_nearest():
+    """Angles near quarter turns, where a sine or cosine is as far off as its angle."""
+    from fractions import Fraction
+    two_pi = Fraction(884279719003555, 140737488355328) + Fraction(2.449293598294706e-16)        # 2 pi to 106 bits
+    g = rng(22)
+    at = torch.randint(1, 2 ** 17, (40,), generator=g)
+    worst = 0.0
+    for i in range(len(at)):
+        p = int(at[i])
+        # turns a token by which p tokens make a whole number of quarter turns, but for 2^-13 of a turn at most
+        quarters = torch.randint(0, p, (64,), generator=g).double() + torch.randn(64, generator=g).double().clamp(-3, 3) * 2.0 ** -13
+        f = quarters / 4 / p * (2 * math.pi)
+        x = torch.zeros(1, 1, 1, 128)
+        x[..., :64] = 1.0
+        y = cf.rotary_positions(x.cuda(), None, f, positions=torch.tensor([[p]], device="cuda"))[0, 0, 0].double().cpu()
+        for j in range(64):
+            turns = Fraction(float(f[j])) / two_pi * p
+            quarter = round(4 * turns)
+            rest = float((turns - Fraction(quarter, 4)) * two_pi)        # |rest| < 2^-8
+            # that of cosine and sine which is small
+            got, sign = (y[64 + j], 1 if quarter % 4 == 0 else -1) if quarter % 2 == 0 else (y[j], 1 if quarter % 4 == 3 else -1)
+            # half a step of 2^-32 turns, the frequency's of 2^-64 (and as much again in 64-bit turns of a radian) p times, and
+            # three roundings of a number of 2^-8
+            tol = 2 * math.pi * (2.0 ** -33 + 3 * 2.0 ** -64 * p) + 4 * 2.0 ** -24 * abs(rest)
+            worst = max(worst, abs(float(got) - sign * math.sin(rest)) / tol)
+    assert worst <= 1.0, worst
