@@ -16,7 +16,8 @@ to be differentiated keeps Q, K, V, y, a float32 a row of a head and, of 16-bit 
 rounded by (as large as y) until its backward.
 
 A cache is ``{"k": [B, S, G, D], "v": [B, S, G, D]}``, room for S tokens a sequence, or one of
-`quantized_cache`, in 8 or 4 bits; how many tokens each holds is the caller's to keep, in `lengths`.
+`quantized_cache`, in 8 or 4 bits (whatever type wrote it); how many tokens each holds is the caller's to
+keep, in `lengths`.
 """
 from __future__ import annotations
 

@@ -14,7 +14,8 @@ normally distributed values are rounded by is 2.7% of theirs with 8 bits and 11%
 
 `softmax_attention_prefill` and `softmax_attention_decode` take such a cache in place of one of the queries'
 type.  They write new keys and values to it first and see them as it holds them, so that a prompt in pieces gives
-what it gives whole.  Its codes have to be such as the calls write.
+what it gives whole.  Its codes have to be such as the calls write.  Queries of float16 see what it holds rounded to
+float16: of a cache written from a wider type, values beyond 65504 are infinite to them.
 """
 from __future__ import annotations
 

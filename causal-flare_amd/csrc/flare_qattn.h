@@ -9,8 +9,10 @@
 // the lanes' writes lie side by side.  The columns of S^T are rows (token, head) of the heads that share the
 // keys, the heads of one token next to each other; a wave owns RT tiles of 16.
 //
-// What the cache holds is exact in bf16, and in fp16 where that is the queries' type.  fp32 queries and
-// weights enter as three bf16 parts, 24 bits.
+// What the cache holds is exact in bf16, and in fp16 where it was written from that.  fp16 queries see values of
+// wider types rounded, infinite beyond fp16's range.  Such values stand before the call's own tokens, where every row
+// sees them: the weights of 0 of keys that a row may not see meet values that are finite, or of blocks that are NaN.
+// fp32 queries and weights enter as three bf16 parts, 24 bits.
 //
 // The keys of a sequence are split over `splits` workgroups of four waves by its true length; qattn_join adds
 // up what they leave.  A workgroup's waves are shares of one head's keys, or heads that lie side by side.  Up to 16 new

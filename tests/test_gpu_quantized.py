@@ -570,3 +570,42 @@ def test_prompts_by_codes_of_a_large_room(dtype, bits):
     ref, tol = M.attention(q[:1, :T - 3], kk, vv, offset=[33], prefix=[50], unit=M.U[dt],
                            tiny=2.0 ** -25 if dtype == "fp16" else 2.0 ** -126)["y"]
     M.check(y[:1, :T - 3], ref, tol + M.U[dt] * ref.abs(), "y", dt)
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("T, H, G, D", [(1, 4, 2, 64), (6, 4, 2, 128), (40, 4, 2, 80), (200, 2, 2, 96), (256, 8, 1, 64)])
+def test_fp16_attention_over_what_bf16_wrote(bits, T, H, G, D):
+    """Queries of fp16 see what a cache holds rounded to fp16, infinite beyond its range, whichever kernel takes them."""
+    g = rng(25)
+    off, S = 100, T + 110
+    old = [normal(g, 3, off, G, D) * 2.0 ** torch.randint(-30, 3, (3, off, G, 1), generator=g) for _ in range(2)]
+    old[1][1, 77, 0, 5], old[1][1, 77, 0, 6], old[1][1, 99, G - 1, D - 1] = 1e5, -1e5, 3e38
+    old[0][2, 88, 0, 3] = 1e5
+    cache = cf.quantized_cache(3, S, G, D, bits)
+    cf.quantized_cache_write(cache, *(t.bfloat16().cuda() for t in old), ints(0, 0, 0))
+    k, v, q = normal(g, 3, T, G, D).half(), normal(g, 3, T, G, D).half(), normal(g, 3, T, H, D).half()
+    y, _ = cf.softmax_attention_prefill(q.cuda(), k.cuda(), v.cuda(), cache, ints(off, off, off))
+    y = y.cpu()
+    kk, vv = (Q.held(cache[x][:, :off + T], cache[x + "_scale"][:, :off + T]).half().double() for x in ("k", "v"))
+
+    def near(b, heads, keys, values, odd, before):
+        ref, tol = M.attention(q[b:b + 1, :, heads], keys[None], values[None], offset=[before], unit=M.U[torch.float16], tiny=2.0 ** -25)["y"]
+        M.check(y[b:b + 1, :, heads].masked_fill(odd, 0.0), ref.masked_fill(odd, 0.0), tol + M.U[torch.float16] * ref.abs(),
+                f"y of sequence {b}", torch.float16)
+    every, no = slice(0, H), torch.zeros(1, dtype=torch.bool)
+    near(0, every, kk[0], vv[0], no, off)
+    # infinite values: whatever their weight, y is infinite in their dimension, with their sign, and nowhere else
+    infinite = torch.isinf(vv[1])
+    assert infinite[77, 0, 5] and infinite[77, 0, 6] and infinite[99, G - 1, D - 1]
+    odd = infinite.any(0).repeat_interleave(H // G, 0).expand(T, H, D)
+    sign = torch.where(infinite, vv[1].sign(), 0.0).sum(0).repeat_interleave(H // G, 0).expand(T, H, D)
+    assert (y[1][odd] == sign[odd] * math.inf).all()
+    near(1, every, kk[1], vv[1].masked_fill(infinite, 0.0), odd, off)
+    # a key's infinite element: a score of +inf (or, of 0 times it, NaN) makes a row NaN; one of -inf has a weight of 0
+    assert torch.isinf(kk[2]).nonzero().tolist() == [[88, 0, 3]]
+    none = (q[2, :, :H // G, 3] >= 0)[..., None].expand(T, H // G, D)
+    assert torch.isnan(y[2, :, :H // G][none]).all()
+    rest = torch.arange(off + T) != 88
+    near(2, slice(0, H // G), kk[2][rest][:, :1], vv[2][rest][:, :1], none, off - 1)
+    if G > 1:
+        near(2, slice(H // G, H), kk[2][:, 1:], vv[2][:, 1:], no, off)
