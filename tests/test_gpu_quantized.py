@@ -609,3 +609,46 @@ def test_fp16_attention_over_what_bf16_wrote(bits, T, H, G, D):
     near(2, slice(0, H // G), kk[2][rest][:, :1], vv[2][rest][:, :1], none, off - 1)
     if G > 1:
         near(2, slice(H // G, H), kk[2][:, 1:], vv[2][:, 1:], no, off)
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("dtype, B, H, G, D, T", [("bf16", 32, 4, 4, 128, 5), ("bf16", 66, 4, 2, 80, 6), ("fp16", 32, 8, 4, 64, 8),
+                                                  ("fp32", 32, 8, 4, 128, 16), ("fp32", 64, 2, 2, 48, 9)])
+def test_nan_with_key_heads_side_by_side(dtype, bits, B, H, G, D, T):
+    """Drafts of as many sequences as let a workgroup's waves take several key heads: NaN keys and values of one head reach the
+    rows of its own queries that see them."""
+    dt, g = TYPES[dtype], rng(26)
+    S = 90
+    lens = torch.randint(0, S - T + 1, (B,), generator=g).int()
+    old = [normal(g, B, S - T, G, D, dtype=dt).cuda() for _ in range(2)]
+    k, v, q = normal(g, B, T, G, D, dtype=dt), normal(g, B, T, G, D, dtype=dt), normal(g, B, T, H, D, dtype=dt)
+    bad_k, bad_v = k.clone(), v.clone()
+    want = torch.zeros((B, T, H, D), dtype=torch.bool)
+    R = H // G
+    for b in range(B):
+        at, h, d = b % T, b // 2 % G, 7 * b % D
+        if b % 3 == 0:
+            bad_v[b, at, h, d] = math.nan
+            want[b, at:, h * R:(h + 1) * R, d // 32 * 32:(d // 32 + 1) * 32] = True
+        if b % 3 == 1:
+            bad_k[b, at, h, d] = math.inf
+            want[b, at:, h * R:(h + 1) * R] = True
+    out = []
+    for keys, values in ((k, v), (bad_k, bad_v)):
+        cache = cf.quantized_cache(B, S, G, D, bits)
+        cf.quantized_cache_write(cache, *old, torch.zeros_like(lens).cuda())
+        out.append(cf.softmax_attention_prefill(q.cuda(), keys.cuda(), values.cuda(), cache, lens.cuda())[0].cpu())
+    assert torch.equal(torch.isnan(out[1]), want)
+    assert torch.equal(out[1][~want], out[0][~want])
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("dtype, B, H, G, D, T", [("fp32", 33, 8, 4, 128, 16), ("fp32", 64, 8, 2, 64, 15), ("fp32", 32, 4, 4, 80, 11),
+                                                  ("bf16", 64, 2, 2, 96, 16), ("fp16", 32, 8, 4, 112, 8)])
+def test_drafts_with_key_heads_side_by_side(dtype, bits, B, H, G, D, T):
+    S = 140
+    g = rng(27)
+    at = torch.randint(-1, S - T + 2, (B,), generator=g).tolist()
+    check_attention(dtype, bits, H, G, D, S, T, at, seed=D)
+    check_attention(dtype, bits, H, G, D, S, T, at, new=torch.randint(0, T + 1, (B,), generator=g).tolist(), seed=D, cap=25.0,
+                    prefix=torch.randint(0, S, (B,), generator=g).tolist(), slopes=[0.5 / (1 + h) for h in range(H)])
