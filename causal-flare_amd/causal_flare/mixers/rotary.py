@@ -5,7 +5,7 @@ Pair i of a head's first R dimensions, (a, b), is turned by the angle position *
     (a, b) -> (a cos - b sin, a sin + b cos)
 
 The pairs are dimensions i and i + R / 2, or 2i and 2i + 1 (`interleaved`); dimensions from R on stay
-as they are.  Angles are exact to some 1e-9 of a radian and more, however far the position; products are
+as they are.  Angles are exact to some 1e-9 of a radian, however far the position; sines, cosines and products are
 taken in float32 and rounded once.
 """
 from __future__ import annotations
@@ -157,9 +157,9 @@ def rotary_positions(
 
     Differentiable in Q and K, backwards (tangents are refused).  Single tokens may be given as [B, H, D] and
     [B, G, D].  frequencies: float64 [R / 2] on the host (`rotary_frequencies`), R up to D; the rest of a head
-    stays as it is.  positions: integers [B, N] (of packed documents, say), any sign; or lengths: integers [B],
-    the tokens that each sequence's cache holds already: token t is at position lengths[b] + t.  Without either
-    it is at t.  D up to 256.
+    stays as it is.  positions: integers [B, N] within 32 bits (of packed documents, say), any sign; or
+    lengths: integers [B], the tokens that each sequence's cache holds already: token t is at position lengths[b] + t.
+    Without either it is at t.  D up to 256.
     """
     name = "rotary_positions"
     if _plain(Q, K, frequencies, positions, lengths):

@@ -12,7 +12,11 @@
 // What the cache holds is exact in bf16, and in fp16 where it was written from that.  fp16 queries see values of
 // wider types rounded, infinite beyond fp16's range.  Such values stand before the call's own tokens, where every row
 // sees them: the weights of 0 of keys that a row may not see meet values that are finite, or of blocks that are NaN.
-// fp32 queries and weights enter as three bf16 parts, 24 bits.
+// Weights of 16-bit queries are rounded to their type for the product with V, as the matrix instructions take them (sums of
+// weights, maxima and what is joined are fp32): y is 1.9e-3 to 2.1e-3 off in bf16, where rounding y alone leaves 1.7e-3.
+// fp32 queries and weights enter as three bf16 parts, 24 bits: three products for each of the others', and registers
+// for two waves a SIMD, 90 us for 64 sequences of 8192 tokens where bf16 queries take 61 (4 key heads of 128, 4 bits, 16
+// heads, 285 MB).
 //
 // The keys of a sequence are split over `splits` workgroups of four waves by its true length; qattn_join adds
 // up what they leave.  A workgroup's waves are shares of one head's keys, or heads that lie side by side.  Up to 16 new

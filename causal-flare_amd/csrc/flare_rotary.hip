@@ -74,8 +74,9 @@ struct alignas(V * sizeof(T)) Vec {
 
 // Heads a thread turns, where there is work for more threads than the card takes at once: four vectors of loads
 // under way.  us of 4 x 4096 tokens, 16 and 4 heads of 128, bf16: pairs of halves with 2, 4 and 8 heads 36, 41, 45;
-// adjacent pairs with 2, 4 and 8 39, 31, 32 (a copy of these 168 MB takes 34).  Stores that pass by the last-level
-// cache take 33, and what reads the result then takes that much longer.
+// adjacent pairs with 2, 4 and 8 39, 31, 32 (a copy of these 168 MB takes 34, and repeated calls find part of their inputs
+// in the last-level cache).  Stores that pass by that cache take 33, and what reads the result then takes that much
+// longer.
 constexpr int heads_of(bool interleaved) { return interleaved ? 4 : 2; }
 
 // V: elements of a vector; 1: element by element, whatever the strides.
