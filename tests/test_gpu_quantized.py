@@ -652,3 +652,31 @@ def test_drafts_with_key_heads_side_by_side(dtype, bits, B, H, G, D, T):
     check_attention(dtype, bits, H, G, D, S, T, at, seed=D)
     check_attention(dtype, bits, H, G, D, S, T, at, new=torch.randint(0, T + 1, (B,), generator=g).tolist(), seed=D, cap=25.0,
                     prefix=torch.randint(0, S, (B,), generator=g).tolist(), slopes=[0.5 / (1 + h) for h in range(H)])
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("T, H, G, D", [(5, 8, 4, 128), (16, 2, 2, 80), (40, 4, 2, 64), (150, 2, 1, 96), (256, 8, 1, 64)])
+def test_padding_holds_anything(dtype, bits, T, H, G, D):
+    """Rows behind new_lengths, and all of a sequence that sits out, are NaN; lengths of new tokens and prefixes beyond their
+    ends count as these."""
+    dt, g = TYPES[dtype], rng(28)
+    B, S = 5, T + 60
+    lens, new = ints(0, 50, 60, -7, 33), (T - 2, 0, T + 9, T, 1)
+    q, k, v = normal(g, B, T, H, D, dtype=dt), normal(g, B, T, G, D, dtype=dt), normal(g, B, T, G, D, dtype=dt)
+    old = [normal(g, B, 60, G, D, dtype=dt).cuda() for _ in range(2)]
+    bad = [x.clone() for x in (q, k, v)]
+    for b in range(B):
+        for x in bad:
+            x[b, 0 if b == 3 else min(new[b], T):] = math.nan
+    out = []
+    for i, tensors in enumerate(((q, k, v), bad)):
+        cache = cf.quantized_cache(B, S, G, D, bits)
+        cf.quantized_cache_write(cache, *old, torch.zeros_like(lens))
+        fresh, prefix = (ints(*(min(n, T) for n in new)), ints(0, 50, S, 0, 20)) if i == 0 else \
+            (ints(T - 2, -1, T + 9, T, 1), ints(-4, 2 ** 31 - 1, 2 ** 30, 5, 20))
+        y, _ = cf.softmax_attention_prefill(*(x.cuda() for x in tensors), cache, lens, prefix_lengths=prefix, new_lengths=fresh)
+        out.append((y, raw(cache)))
+    assert torch.isfinite(out[0][0]).all() and torch.equal(out[0][0], out[1][0])
+    for n in PARTS:
+        assert torch.equal(out[0][1][n], out[1][1][n]), n
